@@ -39,7 +39,7 @@
 extern "C" {
 #endif
 
-#define MF_ABI_VERSION 11
+#define MF_ABI_VERSION 12
 
 typedef enum mf_status {
   MF_OK = 0,
@@ -641,6 +641,58 @@ typedef struct mf_pair_mlp_bwd_args {
 
 uint64_t mf_pair_mlp_bias_bwd_workspace_size(int32_t hidden);
 int mf_pair_mlp_bias_bwd(const mf_pair_mlp_bwd_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Rotary positions (ABI 12).  Every pair (x0, x1) of a head's first         */
+/* rotary_dim entries is turned by theta = position[axis(p)] frequencies[p]: */
+/*   y0 = gain (x0 cos - x1 sin),   y1 = gain (x0 sin + x1 cos)              */
+/* (inverse != 0: by -theta, the gradient's direction).  Pair p is entries   */
+/* (p, p + rotary_dim / 2), or (2 p, 2 p + 1) when interleaved; axis a owns  */
+/* the pairs [a, a + 1) * rotary_dim / (2 axes).  Entries past rotary_dim    */
+/* and parts with turn = 0 are copied.                                       */
+/* Up to three parts (q, k, v of a projection) between two strided layouts:  */
+/* element d of (b, h, n) of part k lies at stride[0] b + stride[1] h +      */
+/* stride[2] n + d.  With a slot map (batch * tokens entries), the rows of   */
+/* (b, n) on slot_side lie at slot * stride[2] + stride[1] h + d instead     */
+/* (packed rows); slot -1 writes zeros (MF_SLOT_SRC) or nothing              */
+/* (MF_SLOT_DST).  src and dst must not overlap.  The angle is formed in     */
+/* fp64 and reduced to one turn there; products and sums are fp32, rounded   */
+/* once to dst_dtype.  head_dim <= 256.                                      */
+/* ------------------------------------------------------------------------ */
+#define MF_POS_F32 0
+#define MF_POS_F64 1
+#define MF_POS_I32 2
+#define MF_POS_I64 3
+#define MF_SLOT_NONE 0
+#define MF_SLOT_SRC 1
+#define MF_SLOT_DST 2
+typedef struct mf_rotary_args {
+  const void* src[3];
+  void* dst[3];
+  int64_t src_stride[3][3];      /* per part {batch, head, token}, elements  */
+  int64_t dst_stride[3][3];
+  int32_t heads[3];
+  int32_t turn[3];               /* 0: the part is copied                    */
+  const void* positions;
+  int64_t position_stride[3];    /* {batch, token, axis}, elements           */
+  const double* frequencies;     /* [rotary_dim / 2] radians per position    */
+  const int32_t* slot;           /* [batch * tokens] or NULL                 */
+  float gain;
+  int32_t position_type;         /* MF_POS_*                                 */
+  int32_t slot_side;             /* MF_SLOT_*                                */
+  int32_t parts;
+  int32_t batch;
+  int32_t tokens;
+  int32_t head_dim;
+  int32_t rotary_dim;
+  int32_t axes;
+  int32_t interleaved;
+  int32_t inverse;
+  int32_t src_dtype;
+  int32_t dst_dtype;
+} mf_rotary_args;
+
+int mf_rotary(const mf_rotary_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -28,6 +28,14 @@ MF_DTYPE_F32 = 0
 MF_DTYPE_F16 = 1
 MF_DTYPE_BF16 = 2
 
+MF_POS_F32 = 0
+MF_POS_F64 = 1
+MF_POS_I32 = 2
+MF_POS_I64 = 3
+MF_SLOT_NONE = 0
+MF_SLOT_SRC = 1
+MF_SLOT_DST = 2
+
 MF_PREC = {"bf16_tc": 0, "tf32": 1, "ieee_fp32": 2}
 
 # Every symbol include/mf_capi.h declares (tests check the library exports them).
@@ -56,9 +64,10 @@ EXPORTED_SYMBOLS = (
     "mf_lattice_terms",
     "mf_pair_mlp_bias_bwd",
     "mf_pair_mlp_bias_bwd_workspace_size",
+    "mf_rotary",
 )
 
-EXPECTED_ABI_VERSION = 11
+EXPECTED_ABI_VERSION = 12
 
 _DTYPE_CODE = {
     torch.float32: MF_DTYPE_F32,
@@ -225,6 +234,15 @@ class MfPairMlpBwdArgs(ctypes.Structure):
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
 
 
+class MfRotaryArgs(ctypes.Structure):
+    _fields_ = [("src", ctypes.c_void_p * 3), ("dst", ctypes.c_void_p * 3), ("src_stride", ctypes.c_int64 * 3 * 3),
+                ("dst_stride", ctypes.c_int64 * 3 * 3), ("heads", ctypes.c_int32 * 3), ("turn", ctypes.c_int32 * 3),
+                ("positions", ctypes.c_void_p), ("position_stride", ctypes.c_int64 * 3),
+                ("frequencies", ctypes.c_void_p), ("slot", ctypes.c_void_p), ("gain", ctypes.c_float)] + [
+        (n, ctypes.c_int32) for n in ("position_type", "slot_side", "parts", "batch", "tokens", "head_dim",
+                                      "rotary_dim", "axes", "interleaved", "inverse", "src_dtype", "dst_dtype")]
+
+
 _LIB: ctypes.CDLL | None = None
 _LOAD_ERROR: str | None = None
 
@@ -260,6 +278,7 @@ def _load() -> ctypes.CDLL | None:
         ("mf_heads_to_rows", MfHeadsToRowsArgs),
         ("mf_pair_mlp_bias", MfPairMlpArgs),
         ("mf_pair_mlp_bias_bwd", MfPairMlpBwdArgs),
+        ("mf_rotary", MfRotaryArgs),
     ):
         fn = getattr(lib, name, None)
         if fn is not None:

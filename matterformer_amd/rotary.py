@@ -1,0 +1,343 @@
+"""Rotary positions: pairs of a head's entries turned by an angle that grows with the token's position, so that the
+product of a turned query and a turned key depends on their positions' difference.
+
+  theta_p = position[axis(p)] * f_p
+  (x0, x1) -> gain * (x0 cos theta - x1 sin theta, x0 sin theta + x1 cos theta)
+
+The reference turns heads by three coordinates in its rotary multi-head attention
+(src/matterformer/models/regular_attention.py:112-271); here a position is one index or up to three coordinates.
+
+  rotary_frequencies  the table f_p (fp64) of a head: base, part of the head, axes, scaling for long contexts
+  apply_rotary        q and k heads (strided views too) -> turned contiguous heads
+  rotary_heads        in_proj rows (B, N, (H + 2 KV) D) -> q, k turned and v, as heads, in one pass
+
+GPU tensors run mf_rotary (csrc/rotary.hip), one launch each way, with gradients of the heads or rows (positions and
+frequencies take none); a missing library raises.  CPU tensors take the torch formulation.
+"""
+
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from matterformer_amd import _native
+
+LAYOUTS = ("half", "interleaved")
+SCALINGS = ("none", "linear", "ntk", "yarn")
+
+_POSITION_TYPES = {torch.float32: _native.MF_POS_F32, torch.float64: _native.MF_POS_F64,
+                   torch.int32: _native.MF_POS_I32, torch.int64: _native.MF_POS_I64}
+_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+@dataclass(frozen=True)
+class RotaryFrequencies:
+    """``table`` (rotary_dim / 2,) fp64: radians per unit of position of each pair.  Axis a of ``axes`` owns the pairs
+    [a, a + 1) * rotary_dim / (2 axes).  ``gain`` multiplies the turned part."""
+
+    table: torch.Tensor
+    axes: int = 1
+    gain: float = 1.0
+
+    def __post_init__(self) -> None:
+        if self.table.ndim != 1 or self.table.dtype != torch.float64 or not self.table.is_contiguous():
+            raise ValueError("the frequency table must be a contiguous 1-D float64 tensor")
+        if not 1 <= int(self.axes) <= 3:
+            raise ValueError(f"axes must be 1, 2 or 3, got {self.axes}")
+        if self.table.numel() == 0 or self.table.numel() % int(self.axes) != 0:
+            raise ValueError("the pairs must be a positive multiple of axes")
+        if not math.isfinite(float(self.gain)):
+            raise ValueError("gain must be finite")
+
+    @property
+    def rotary_dim(self) -> int:
+        return 2 * self.table.numel()
+
+    def to(self, device) -> "RotaryFrequencies":
+        return RotaryFrequencies(self.table.to(device), self.axes, self.gain)
+
+
+def rotary_frequencies(rotary_dim: int, *, axes: int = 1, base: float = 10000.0, scaling: str = "none",
+                       factor: float = 1.0, original_length: float | None = None, beta_fast: float = 32.0,
+                       beta_slow: float = 1.0, device=None) -> RotaryFrequencies:
+    """f_i = base^(-i / P), i < P = rotary_dim / (2 axes), for every axis.  ``scaling`` stretches a table that was
+    trained on positions up to original_length to ``factor`` (s) times that:
+
+      linear  f_i / s (positions interpolated)
+      ntk     base s^(P / (P - 1)) for base: the fastest pair stays, the slowest is f_{P-1} / s
+      yarn    by parts: pairs of at least beta_fast turns over original_length stay, those of at most beta_slow are
+              interpolated, a linear ramp in between; gain = 0.1 ln s + 1
+    """
+    rotary_dim, axes = int(rotary_dim), int(axes)
+    if not 1 <= axes <= 3:
+        raise ValueError(f"axes must be 1, 2 or 3, got {axes}")
+    if rotary_dim <= 0 or rotary_dim % (2 * axes) != 0:
+        raise ValueError(f"rotary_dim must be a positive multiple of {2 * axes}, got {rotary_dim}")
+    if not (math.isfinite(base) and base > 0.0):
+        raise ValueError(f"base must be positive, got {base}")
+    if scaling not in SCALINGS:
+        raise ValueError(f"Unsupported scaling: {scaling}; expected one of {SCALINGS}")
+    if not (math.isfinite(factor) and factor >= 1.0):
+        raise ValueError(f"factor must be at least 1, got {factor}")
+    per = rotary_dim // (2 * axes)
+    i = torch.arange(per, dtype=torch.float64)
+    gain = 1.0
+    if scaling == "ntk" and per > 1:
+        base = base * factor ** (per / (per - 1))
+    f = torch.pow(torch.tensor(float(base), dtype=torch.float64), -i / per)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "yarn":
+        if original_length is None or not original_length > 0:
+            raise ValueError("yarn scaling needs original_length")
+        if not beta_fast > beta_slow:
+            raise ValueError("beta_fast must be greater than beta_slow")
+        turns = float(original_length) * f / (2.0 * math.pi)
+        keep = ((turns - beta_slow) / (beta_fast - beta_slow)).clamp(0.0, 1.0)
+        f = f * keep + f / factor * (1.0 - keep)
+        gain = 0.1 * math.log(factor) + 1.0
+    return RotaryFrequencies(f.repeat(axes).contiguous().to(device), axes, gain)
+
+
+def _check_positions(positions: torch.Tensor, batch: int, tokens: int, frequencies: RotaryFrequencies,
+                     device: torch.device) -> torch.Tensor:
+    """(B, N, axes) view of the positions; one row for the batch is expanded."""
+    axes = int(frequencies.axes)
+    if positions.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("rotary positions take no gradient: detach them")
+    if positions.dtype not in _POSITION_TYPES:
+        raise RuntimeError(f"rotary positions must be float32, float64, int32 or int64, got {positions.dtype}")
+    if frequencies.table.device != device or positions.device != device:
+        raise RuntimeError("positions and frequencies must be on the device of the heads")
+    if axes == 1 and positions.ndim == 2:
+        positions = positions[..., None]
+    if positions.ndim != 3 or positions.shape[0] not in (1, batch) or tuple(positions.shape[1:]) != (tokens, axes):
+        want = f"({batch}, {tokens})" if axes == 1 else f"({batch}, {tokens}, {axes})"
+        raise ValueError(f"positions must have shape {want} (or one row for the batch), got {tuple(positions.shape)}")
+    return positions.detach().expand(batch, tokens, axes)
+
+
+def _check_layout(layout: str, head_dim: int, frequencies: RotaryFrequencies) -> bool:
+    if layout not in LAYOUTS:
+        raise ValueError(f"Unsupported rotary layout: {layout}; expected one of {LAYOUTS}")
+    if frequencies.rotary_dim > head_dim:
+        raise ValueError(f"rotary_dim {frequencies.rotary_dim} is greater than head_dim {head_dim}")
+    return layout == "interleaved"
+
+
+def _rotate_torch(x: torch.Tensor, positions: torch.Tensor, frequencies: RotaryFrequencies,
+                  interleaved: bool) -> torch.Tensor:
+    """(B, H, N, D) heads turned by torch expressions: angles in fp64, products in fp32 (fp64 for fp64 heads)."""
+    per = frequencies.table.numel() // frequencies.axes
+    angle = positions.double().repeat_interleave(per, dim=-1) * frequencies.table
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    cos = (angle.cos() * frequencies.gain).to(wide)[:, None]
+    sin = (angle.sin() * frequencies.gain).to(wide)[:, None]
+    R = frequencies.rotary_dim
+    xr = x[..., :R].to(wide)
+    if interleaved:
+        a, b = xr[..., 0::2], xr[..., 1::2]
+        y = torch.stack([a * cos - b * sin, a * sin + b * cos], dim=-1).flatten(-2)
+    else:
+        a, b = xr[..., :R // 2], xr[..., R // 2:]
+        y = torch.cat([a * cos - b * sin, a * sin + b * cos], dim=-1)
+    return torch.cat([y.to(x.dtype), x[..., R:]], dim=-1)
+
+
+class _Plan:
+    """What a launch and its gradient share: positions (B, N, axes), frequencies and the pairs' layout; for packed
+    rows the slot map."""
+
+    def __init__(self, positions, frequencies, interleaved, slot=None):
+        self.positions = positions
+        self.frequencies = frequencies
+        self.interleaved = interleaved
+        self.slot = slot
+
+
+def _launch(plan: _Plan, parts, *, batch: int, tokens: int, head_dim: int, inverse: bool, slot_side: int) -> None:
+    """parts: (src, src strides {batch, head, token}, dst, dst strides, heads, turned), src and dst (tensor, element
+    offset); the dtypes are those of the first part."""
+    args = _native.MfRotaryArgs(
+        positions=plan.positions.data_ptr(), frequencies=plan.frequencies.table.data_ptr(),
+        slot=_native.ptr(plan.slot), gain=float(plan.frequencies.gain),
+        position_type=_POSITION_TYPES[plan.positions.dtype], slot_side=slot_side, parts=len(parts), batch=batch,
+        tokens=tokens, head_dim=head_dim, rotary_dim=plan.frequencies.rotary_dim, axes=int(plan.frequencies.axes),
+        interleaved=int(plan.interleaved), inverse=int(inverse), src_dtype=_native.dtype_code(parts[0][0][0].dtype),
+        dst_dtype=_native.dtype_code(parts[0][2][0].dtype))
+    for i, stride in enumerate(plan.positions.stride()):
+        args.position_stride[i] = stride
+    for k, ((src, s0), ss, (dst, d0), ds, heads, turn) in enumerate(parts):
+        args.src[k] = src.data_ptr() + s0 * src.element_size()
+        args.dst[k] = dst.data_ptr() + d0 * dst.element_size()
+        args.heads[k] = heads
+        args.turn[k] = int(turn)
+        for i in range(3):
+            args.src_stride[k][i] = ss[i]
+            args.dst_stride[k][i] = ds[i]
+    dev = parts[0][0][0].device
+    with torch.cuda.device(dev):
+        _native.check(_native.lib().mf_rotary(args, _native.current_stream(dev)), "mf_rotary")
+
+
+def _unit(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _strides(t: torch.Tensor) -> tuple:
+    """{batch, head, token} strides of (B, H, N, D) heads; 0 for an axis of one entry, whose stride means nothing."""
+    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3]))
+
+
+def _turn_heads(plan: _Plan, heads: list[torch.Tensor], inverse: bool) -> list[torch.Tensor]:
+    """(B, H, N, D) heads -> turned contiguous heads, in one launch."""
+    outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in heads]
+    B, _, N, D = heads[0].shape
+    parts = []
+    for t, o in zip((_unit(t) for t in heads), outs):
+        parts.append(((t, 0), _strides(t), (o, 0), _strides(o), t.shape[1], True))
+    if B * N > 0:
+        _launch(plan, parts, batch=B, tokens=N, head_dim=D, inverse=inverse, slot_side=_native.MF_SLOT_NONE)
+    return outs
+
+
+class _HeadsFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, plan, *heads):
+        ctx.plan = plan
+        return tuple(_turn_heads(plan, list(heads), False))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        return (None, *_turn_heads(ctx.plan, list(grads), True))
+
+
+def _head_parts(counts, head_dim: int, batch_stride: int, row_stride: int):
+    """Offset, {batch, head, token} strides of each part inside rows of (H + 2 KV) head_dim columns."""
+    out, offset = [], 0
+    for heads in counts:
+        out.append((offset, (batch_stride, head_dim, row_stride), heads))
+        offset += heads * head_dim
+    return out
+
+
+def _rows_to_heads(plan: _Plan, rows: torch.Tensor, counts, batch: int, tokens: int, head_dim: int, dtype):
+    """rows (B, N, columns), or packed (T, columns) through plan.slot -> one (B, heads, N, D) tensor a part."""
+    outs = [torch.empty(batch, h, tokens, head_dim, dtype=dtype, device=rows.device) for h in counts]
+    packed = plan.slot is not None
+    rows = _unit(rows)
+    layout = _head_parts(counts, head_dim, 0 if packed else rows.stride(0), rows.stride(-2))
+    parts = [((rows, offset), strides, (o, 0), _strides(o), h, k < 2)
+             for k, ((offset, strides, h), o) in enumerate(zip(layout, outs))]
+    if batch * tokens > 0:
+        _launch(plan, parts, batch=batch, tokens=tokens, head_dim=head_dim, inverse=False,
+                slot_side=_native.MF_SLOT_SRC if packed else _native.MF_SLOT_NONE)
+    return outs
+
+
+class _RowsFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, plan, rows, counts, batch, tokens, head_dim, dtype):
+        ctx.plan, ctx.counts, ctx.sizes = plan, counts, (batch, tokens, head_dim)
+        ctx.rows = (rows.shape, rows.dtype)
+        return tuple(_rows_to_heads(plan, rows, counts, batch, tokens, head_dim, dtype))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        plan, (batch, tokens, head_dim), (shape, dtype) = ctx.plan, ctx.sizes, ctx.rows
+        packed = plan.slot is not None
+        out = torch.empty(shape, dtype=dtype, device=grads[0].device)
+        layout = _head_parts(ctx.counts, head_dim, 0 if packed else out.stride(0), out.stride(-2))
+        parts = []
+        for k, ((offset, strides, h), g) in enumerate(zip(layout, (_unit(g) for g in grads))):
+            parts.append(((g, 0), _strides(g), (out, offset), strides, h, k < 2))
+        if out.numel() > 0:
+            _launch(plan, parts, batch=batch, tokens=tokens, head_dim=head_dim, inverse=True,
+                    slot_side=_native.MF_SLOT_DST if packed else _native.MF_SLOT_NONE)
+        return (None, out, None, None, None, None, None)
+
+
+def _check_kernel(head_dim: int, dtype: torch.dtype) -> None:
+    if dtype not in _DTYPES:
+        raise RuntimeError(f"rotary positions support bfloat16, float16 and float32 heads on the GPU, got {dtype}")
+    if head_dim > 256:
+        raise RuntimeError(f"rotary positions support head_dim up to 256, got {head_dim}")
+
+
+def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, frequencies: RotaryFrequencies, *,
+                 layout: str = "half"):
+    """q (B, H, N, D) and k (B, KV, N, D; or None) turned by their tokens' positions.
+
+    positions (B, N), or (B, N, axes) for more than one axis: float32, float64, int32 or int64; the batch may be 1
+    for all.  ``layout``: a pair is entries (p, p + rotary_dim / 2) ("half") or (2p, 2p + 1) ("interleaved"); entries
+    past rotary_dim stay.  q and k may be views into one projection (any strides).  Returns contiguous (q', k'),
+    differentiable in q and k."""
+    if q.ndim != 4 or (k is not None and (k.ndim != 4 or k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:])):
+        raise ValueError("q must have shape (B, H, N, D) and k (B, KV, N, D)")
+    heads = [q] if k is None else [q, k]
+    if any(t.dtype != q.dtype or t.device != q.device for t in heads):
+        raise RuntimeError("q and k must share a dtype and a device")
+    B, _, N, D = q.shape
+    interleaved = _check_layout(layout, D, frequencies)
+    pos = _check_positions(positions, B, N, frequencies, q.device)
+    if q.device.type != "cuda":
+        out = [_rotate_torch(t, pos, frequencies, interleaved).contiguous() for t in heads]
+    else:
+        _check_kernel(D, q.dtype)
+        out = _HeadsFunction.apply(_Plan(pos, frequencies, interleaved), *heads)
+    return (out[0], None) if k is None else (out[0], out[1])
+
+
+def _rows_torch(rows, pos, frequencies, interleaved, counts, head_dim, dtype):
+    """rows (B, N, columns) -> heads by torch expressions."""
+    B, N, _ = rows.shape
+    outs = []
+    for k, part in enumerate(rows.split([h * head_dim for h in counts], dim=-1)):
+        t = part.reshape(B, N, counts[k], head_dim).transpose(1, 2)
+        outs.append((_rotate_torch(t, pos, frequencies, interleaved) if k < 2 else t).to(dtype).contiguous())
+    return tuple(outs)
+
+
+def rotary_heads(rows: torch.Tensor, positions: torch.Tensor, frequencies: RotaryFrequencies, *, heads: int,
+                 kv_heads: int | None = None, layout: str = "half"):
+    """The heads of in_proj rows (B, N, (heads + 2 kv_heads) D), q and k turned as apply_rotary turns them: contiguous
+    q (B, heads, N, D), k and v (B, kv_heads, N, D), in one pass.  Differentiable in rows."""
+    heads = int(heads)
+    kv_heads = heads if kv_heads is None else int(kv_heads)
+    if heads < 1 or kv_heads < 1:
+        raise ValueError("heads and kv_heads must be positive")
+    if rows.ndim != 3 or rows.shape[-1] == 0 or rows.shape[-1] % (heads + 2 * kv_heads) != 0:
+        raise ValueError(f"rows must have shape (B, N, {heads + 2 * kv_heads} * head_dim), got {tuple(rows.shape)}")
+    B, N, columns = rows.shape
+    D = columns // (heads + 2 * kv_heads)
+    interleaved = _check_layout(layout, D, frequencies)
+    pos = _check_positions(positions, B, N, frequencies, rows.device)
+    counts = (heads, kv_heads, kv_heads)
+    if rows.device.type != "cuda":
+        return _rows_torch(rows, pos, frequencies, interleaved, counts, D, rows.dtype)
+    _check_kernel(D, rows.dtype)
+    return _RowsFunction.apply(_Plan(pos, frequencies, interleaved), rows, counts, B, N, D, rows.dtype)
+
+
+def _packed_rotary_heads(rows: torch.Tensor, slot: torch.Tensor, positions: torch.Tensor,
+                        frequencies: RotaryFrequencies, *, heads: int, head_dim: int, layout: str,
+                        dtype: torch.dtype):
+    """rotary_heads for packed rows (T, 3 heads head_dim): slot (B * W) int32 names the row of each slot, -1 an empty
+    one (zeros); every row has one slot.  positions (B, W[, axes]); the heads come in ``dtype``.  GPU tensors only
+    (TokenPacking.to_rotary_heads)."""
+    B, W = positions.shape[:2]
+    if rows.ndim != 2 or rows.shape[1] != 3 * heads * head_dim or slot.numel() != B * W or slot.dtype != torch.int32:
+        raise ValueError(f"rows must have shape (T, {3 * heads * head_dim}) and slot hold {B * W} int32 entries")
+    if rows.device.type != "cuda" or slot.device != rows.device:
+        raise RuntimeError("packed rotary heads need CUDA (ROCm) tensors on one device")
+    interleaved = _check_layout(layout, head_dim, frequencies)
+    pos = _check_positions(positions, B, W, frequencies, rows.device)
+    _check_kernel(head_dim, rows.dtype)
+    _check_kernel(head_dim, dtype)
+    plan = _Plan(pos, frequencies, interleaved, slot.contiguous())
+    return _RowsFunction.apply(plan, rows, (heads, heads, heads), B, W, head_dim, dtype)

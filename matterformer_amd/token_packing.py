@@ -127,6 +127,20 @@ class TokenPacking:
         out.permute(1, 3, 0, 2, 4)[self.mol, self.pos] = src.to(dtype)
         return out
 
+    def to_rotary_heads(self, xp: torch.Tensor, heads: int, head_dim: int, dtype: torch.dtype, positions: torch.Tensor,
+                        frequencies, layout: str = "half"):
+        """(T, 3 * heads * head_dim) q, k, v projections -> q and k turned by their atoms' positions (compact
+        (B, W, axes)) and v, each (B, heads, W, head_dim) in ``dtype``, empty slots zero: splitting, turning and
+        padding in one mf_rotary pass, as is the gradient."""
+        from matterformer_amd.rotary import _packed_rotary_heads
+
+        if xp.shape != (self.tokens, 3 * heads * head_dim):
+            raise ValueError(f"projections must have shape ({self.tokens}, {3 * heads * head_dim})")
+        if positions.shape[:2] != (self.batch, self.width):
+            raise ValueError(f"positions must have shape ({self.batch}, {self.width}, ...)")
+        return _packed_rotary_heads(xp, self.slot32, positions, frequencies, heads=heads, head_dim=head_dim,
+                                    layout=layout, dtype=dtype)
+
     def from_heads(self, out: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
         """(B, H, W, D) attention output -> (T, H * D) in ``dtype`` (default: out's)."""
         B, H, W, D = out.shape
