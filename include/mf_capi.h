@@ -694,6 +694,54 @@ typedef struct mf_rotary_args {
 
 int mf_rotary(const mf_rotary_args* args, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Gated linear layer (ABI 12).  Wg = weight[:hidden], Wu = weight[hidden:]: */
+/*   a = x Wg^T + bias[:hidden],  b = x Wu^T + bias[hidden:],                */
+/*   out = activation(a) * b                                                 */
+/* in one kernel: sums, activation and product in fp32, out rounded once.    */
+/* Backward, for grad_out = dL/dout (a and b are formed again):              */
+/*   dA = grad_out b act'(a),  dB = grad_out act(a)   (rounded to dtype)     */
+/*   dx = [dA dB] weight,  dweight = [dA dB]^T x,  dbias = column sums of    */
+/* the unrounded [dA dB]; any of the three may be NULL.  Every sum is in a   */
+/* fixed order (two calls give identical bits).  Workspaces need no fill:    */
+/* the forward's holds aligned copies of operands whose rows are no multiple */
+/* of 16 bytes (0 bytes otherwise).                                          */
+/* ------------------------------------------------------------------------ */
+#define MF_ACT_SILU 0
+#define MF_ACT_GELU 1        /* by the error function                        */
+#define MF_ACT_GELU_TANH 2
+#define MF_ACT_RELU 3
+#define MF_ACT_SIGMOID 4
+typedef struct mf_gated_linear_args {
+  const void* x;             /* [tokens, channels], rows x_stride apart      */
+  const void* weight;        /* [2 hidden, channels]                         */
+  const void* bias;          /* [2 hidden] or NULL                           */
+  void* out;                 /* [tokens, hidden]                             */
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t x_stride;          /* elements between rows of x                   */
+  int32_t tokens;
+  int32_t channels;
+  int32_t hidden;
+  int32_t activation;        /* MF_ACT_*                                     */
+  int32_t dtype;             /* of every tensor                              */
+} mf_gated_linear_args;
+
+typedef struct mf_gated_linear_bwd_args {
+  mf_gated_linear_args fwd;  /* its out and workspace are not used           */
+  const void* grad_out;      /* [tokens, hidden]                             */
+  void* dx;                  /* [tokens, channels] or NULL                   */
+  void* dweight;             /* [2 hidden, channels] or NULL                 */
+  void* dbias;               /* [2 hidden] or NULL                           */
+  void* workspace;
+  uint64_t workspace_bytes;
+} mf_gated_linear_bwd_args;
+
+uint64_t mf_gated_linear_workspace_size(const mf_gated_linear_args* args);
+int mf_gated_linear(const mf_gated_linear_args* args, void* stream);
+uint64_t mf_gated_linear_bwd_workspace_size(const mf_gated_linear_bwd_args* args);
+int mf_gated_linear_bwd(const mf_gated_linear_bwd_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -36,6 +36,8 @@ MF_SLOT_NONE = 0
 MF_SLOT_SRC = 1
 MF_SLOT_DST = 2
 
+MF_ACT = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3, "sigmoid": 4}
+
 MF_PREC = {"bf16_tc": 0, "tf32": 1, "ieee_fp32": 2}
 
 # Every symbol include/mf_capi.h declares (tests check the library exports them).
@@ -65,6 +67,10 @@ EXPORTED_SYMBOLS = (
     "mf_pair_mlp_bias_bwd",
     "mf_pair_mlp_bias_bwd_workspace_size",
     "mf_rotary",
+    "mf_gated_linear",
+    "mf_gated_linear_workspace_size",
+    "mf_gated_linear_bwd",
+    "mf_gated_linear_bwd_workspace_size",
 )
 
 EXPECTED_ABI_VERSION = 12
@@ -243,6 +249,18 @@ class MfRotaryArgs(ctypes.Structure):
                                       "rotary_dim", "axes", "interleaved", "inverse", "src_dtype", "dst_dtype")]
 
 
+class MfGatedLinearArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "weight", "bias", "out", "workspace")] + [
+        ("workspace_bytes", ctypes.c_uint64), ("x_stride", ctypes.c_int64)] + [
+        (n, ctypes.c_int32) for n in ("tokens", "channels", "hidden", "activation", "dtype")]
+
+
+class MfGatedLinearBwdArgs(ctypes.Structure):
+    _fields_ = [("fwd", MfGatedLinearArgs)] + [
+        (n, ctypes.c_void_p) for n in ("grad_out", "dx", "dweight", "dbias", "workspace")] + [
+        ("workspace_bytes", ctypes.c_uint64)]
+
+
 _LIB: ctypes.CDLL | None = None
 _LOAD_ERROR: str | None = None
 
@@ -279,6 +297,8 @@ def _load() -> ctypes.CDLL | None:
         ("mf_pair_mlp_bias", MfPairMlpArgs),
         ("mf_pair_mlp_bias_bwd", MfPairMlpBwdArgs),
         ("mf_rotary", MfRotaryArgs),
+        ("mf_gated_linear", MfGatedLinearArgs),
+        ("mf_gated_linear_bwd", MfGatedLinearBwdArgs),
     ):
         fn = getattr(lib, name, None)
         if fn is not None:
@@ -301,6 +321,12 @@ def _load() -> ctypes.CDLL | None:
         lib.mf_lattice_terms.argtypes = [ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
                                          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
         lib.mf_lattice_terms.restype = ctypes.c_int
+    for name, argtype in (("mf_gated_linear_workspace_size", MfGatedLinearArgs),
+                          ("mf_gated_linear_bwd_workspace_size", MfGatedLinearBwdArgs)):
+        fn = getattr(lib, name, None)
+        if fn is not None:
+            fn.argtypes = [ctypes.POINTER(argtype)]
+            fn.restype = ctypes.c_uint64
     version = lib.mf_abi_version()
     if version != EXPECTED_ABI_VERSION:
         _LOAD_ERROR = f"{path} has ABI version {version}, expected {EXPECTED_ABI_VERSION}"

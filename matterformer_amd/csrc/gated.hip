@@ -1,0 +1,821 @@
+// Gated linear layer (mf_gated_linear, mf_gated_linear_bwd) on gfx950:
+//   a = x Wg^T + bg,  b = x Wu^T + bu,  h = act(a) * b,
+// with Wg the first F and Wu the last F rows of one weight [2F, C].
+// Backward, go = dL/dh:
+//   dA = go b act'(a),  dB = go act(a),
+//   dx = [dA dB] W,  dW = [dA dB]^T x,  dbias = column sums of [dA dB].
+//
+// The forward is one kernel: a tile of a and the matching tile of b are held by
+// the same lanes, so activation and product happen on the fp32 accumulators and
+// only h is written.  The backward forms a and b again (4 T C F flops) in the
+// same kernel with another epilogue rather than keeping them: keeping them is
+// 4 T F values more to write and read, as long as the products take at the
+// widths of a few hundred to a thousand (512 columns, 16384 rows: 67 GFLOP,
+// 60 us, against 268 MB, 54 us), and would round them to the 16-bit type before
+// the derivative.  [dA dB] is rounded to the operands' type for the two
+// products that follow, as any 16-bit matrix product's input is.
+//
+// All three products run on one tile kernel.  Its matrix-core "row" operand is
+// the output's contiguous axis (h's columns, dx's and dW's channels), the
+// "column" operand the output's rows, so that a lane ends with 16 consecutive
+// output columns (see frag_row): stores of 32 bytes a lane, 128 a row and wave.
+// Tiles are 128 bytes of K deep, copied from global memory straight to LDS
+// (16 bytes a lane) while the previous tile is multiplied; two buffers, one
+// barrier a step.  Rows past the ends are fetched from an out-of-range buffer
+// offset, which reads zero, on both sides (a zero times what lies behind a
+// matrix could be NaN).  Operands whose contiguous axis is K are stored as
+// rows of 128 bytes and read as 16-byte pieces; operands whose K axis is the
+// outer one (W in dx, both in dW) are stored as they lie and read transposed.
+#include <algorithm>
+#include <cmath>
+
+#include "mf_common.h"
+
+namespace mf {
+namespace gated {
+
+enum Mode { kFwd, kBwd, kDx, kDw };
+
+// -- activations: value and derivative in fp32 ---------------------------------------------------------------
+// exp of -|..| only where the result must not overflow to inf / inf: 1 / (1 + exp(-a)) is 0 for a -> -inf.
+template <bool FAST>
+__device__ __forceinline__ float exp_(float x) {
+  return FAST ? fast_exp2(x * kLog2e) : expf(x);
+}
+template <bool FAST>
+__device__ __forceinline__ float rcp_(float x) {
+  return FAST ? __builtin_amdgcn_rcpf(x) : 1.0f / x;
+}
+template <bool FAST>
+__device__ __forceinline__ float sigmoid_(float x) {
+  return rcp_<FAST>(1.0f + exp_<FAST>(-x));
+}
+
+// FAST (16-bit outputs): hardware exp2 and reciprocal, one unit in the last place of fp32 each.
+template <bool FAST>
+__device__ __forceinline__ float act_value(int act, float a) {
+  switch (act) {
+    case MF_ACT_GELU: return 0.5f * a * erfcf(-0.70710678118654752f * a);
+    case MF_ACT_GELU_TANH: {
+      // 0.5 (1 + tanh u) = sigmoid(2 u): no cancellation for negative u
+      const float u2 = 1.5957691216057308f * (a + 0.044715f * a * a * a);
+      return a * sigmoid_<FAST>(u2);
+    }
+    case MF_ACT_RELU: return a > 0.0f ? a : (a == a ? 0.0f : a);
+    case MF_ACT_SIGMOID: return sigmoid_<FAST>(a);
+    default: return a * sigmoid_<FAST>(a);
+  }
+}
+template <bool FAST>
+__device__ __forceinline__ void act_both(int act, float a, float& y, float& dy) {
+  switch (act) {
+    case MF_ACT_GELU: {
+      const float cdf = 0.5f * erfcf(-0.70710678118654752f * a);
+      y = a * cdf;
+      dy = cdf + a * 0.3989422804014327f * exp_<FAST>(-0.5f * a * a);
+      return;
+    }
+    case MF_ACT_GELU_TANH: {
+      const float a2 = a * a;
+      const float u2 = 1.5957691216057308f * (a + 0.044715f * a * a2);
+      const float s = sigmoid_<FAST>(u2), ns = sigmoid_<FAST>(-u2);
+      y = a * s;
+      dy = s + a * s * ns * 1.5957691216057308f * (1.0f + 0.134145f * a2);
+      return;
+    }
+    case MF_ACT_RELU:
+      y = a > 0.0f ? a : (a == a ? 0.0f : a);
+      dy = a > 0.0f ? 1.0f : 0.0f;
+      return;
+    case MF_ACT_SIGMOID:
+      y = sigmoid_<FAST>(a);
+      dy = y * sigmoid_<FAST>(-a);
+      return;
+    default: {
+      const float s = sigmoid_<FAST>(a);
+      y = a * s;
+      dy = s * (1.0f + a * sigmoid_<FAST>(-a));
+      return;
+    }
+  }
+}
+
+// -- 16 bytes of K as one matrix-core operand ----------------------------------------------------------------
+template <typename T>
+struct Mma {
+  using Frag = typename Elem<T>::Operand;
+  __device__ static __forceinline__ void run(Frag a, Frag b, mf_f32x4& c) { c = Elem<T>::mma(a, b, c); }
+};
+template <>
+struct Mma<float> {
+  using Frag = mf_f32x4;
+  __device__ static __forceinline__ void run(Frag a, Frag b, mf_f32x4& c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+  }
+};
+
+constexpr int kRowBytes = 128;                        // K bytes of a tile
+template <typename T> constexpr int kBK = kRowBytes / int(sizeof(T));
+template <typename T> constexpr int kEpc = 16 / int(sizeof(T));  // elements per 16-byte chunk
+constexpr unsigned kOutside = 0x80000000u;            // a buffer offset that is out of range: reads 0
+
+// Row operand ("A", M axis): lane r of fragment j in a group of 64 holds group row 16 (r >> 2) + 4 j + (r & 3),
+// so accumulator register q of fragment j in lane group g is row 16 g + 4 j + q: over j and q, 16 rows in order.
+__device__ __forceinline__ int frag_row(int r, int j) { return ((r >> 2) << 4) + 4 * j + (r & 3); }
+
+// Chunk swizzles (16-byte chunks of a stored row) that spread a wave's reads over the LDS banks.
+// K-contiguous rows: the eight rows that eight consecutive lanes read get eight different chunk positions.
+template <bool ROW_OPERAND>
+__device__ __forceinline__ int swz_row(int row) {
+  return ROW_OPERAND ? (row & 3) | ((row >> 2) & 4) : row & 7;
+}
+// K-outer rows (one k each): see read_frag.
+template <typename T, bool ROW_OPERAND>
+__device__ __forceinline__ int swz_k(int k) {
+  if constexpr (sizeof(T) == 2) return ROW_OPERAND ? (k & 1) | ((k & 2) << 2) : 2 * (k & 3) | ((k >> 3) & 1) << 3;
+  else return ROW_OPERAND ? (k >> 2) & 3 : ((k >> 2) & 3) << 2;
+}
+
+typedef __attribute__((address_space(3))) void* LdsPtr;
+
+// One operand's tile: EXT rows (or columns) of the M or N axis by 128 bytes of K, loaded by NW waves.
+// KOUT: K is the outer axis in memory.
+template <typename T, bool KOUT, bool ROW_OPERAND, int EXT, int NW>
+struct Tile {
+  static constexpr int kBytes = EXT * kRowBytes;
+  static constexpr int kLoads = kBytes / (64 * 16 * NW);  // 16-byte loads per lane
+  static_assert(kLoads * 64 * 16 * NW == kBytes, "tile shape");
+  static constexpr int kPitch = KOUT ? EXT * int(sizeof(T)) : kRowBytes;
+  static_assert(!KOUT || EXT >= 128, "the swizzle of K-outer rows needs 16 chunks");
+  unsigned off[kLoads];  // buffer offset of the lane's chunk, or kOutside for a row or column past the end
+  int k[kLoads];         // its first k within the tile
+
+  // `valid`: rows (columns) of the tile that exist; K-contiguous rows r >= split continue at +jump bytes
+  __device__ __forceinline__ void init(int wave, int lane, int64_t ld_bytes, int valid, int split, int valid2,
+                                       int64_t jump) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int q = (wave * kLoads + i) * 64 + lane;
+      if constexpr (KOUT) {
+        const int row = q / (kPitch / 16), pos = q % (kPitch / 16);
+        const int c = pos ^ swz_k<T, ROW_OPERAND>(row);
+        k[i] = row;
+        off[i] = c * kEpc<T> < valid ? unsigned(row * ld_bytes + c * 16) : kOutside;
+      } else {
+        const int row = q >> 3, pos = q & 7;
+        const int c = pos ^ swz_row<ROW_OPERAND>(row);
+        k[i] = c * kEpc<T>;
+        const bool second = row >= split;
+        const int r = second ? row - split : row;
+        off[i] = r < (second ? valid2 : valid) ? unsigned(r * ld_bytes + (second ? jump : 0) + c * 16) : kOutside;
+      }
+    }
+  }
+  // base: the tile's first byte at this K step; left: K entries that remain
+  __device__ __forceinline__ void load(const char* base, int left, char* lds, int wave) const {
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), short(0), int(kOutside), 0x00027000);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const unsigned o = k[i] < left ? off[i] : kOutside;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (LdsPtr)(lds + (wave * kLoads + i) * 1024), 16, o, 0, 0, 0);
+    }
+  }
+};
+
+// The 16-byte K piece kk (of 2) of a fragment.  row operand: group base + frag_row(r16, j); column operand: base + 16 j
+// + r16.  16-bit types: k = 32 kk + 8 g + i; fp32: k = 16 kk + 4 g + i.
+template <typename T, bool KOUT, bool ROW_OPERAND, int EXT>
+__device__ __forceinline__ typename Mma<T>::Frag read_frag(const char* lds, int base, int j, int kk, int lane) {
+  using Frag = typename Mma<T>::Frag;
+  const int g = lane >> 4, r = lane & 15;
+  if constexpr (!KOUT) {
+    const int row = base + (ROW_OPERAND ? frag_row(r, j) : 16 * j + r);
+    return *reinterpret_cast<const Frag*>(lds + row * kRowBytes + (((kk * 4 + g) ^ (r & 7)) << 4));
+  } else if constexpr (sizeof(T) == 2) {
+    // lane 4 e + a of a 16-lane group addresses 4 elements of row k = .. + e; the transposing read gives lane
+    // 4 a + c element c of the pieces of rows e = 0..3
+    const int e = r >> 2, a = r & 3;
+    const int col = base + (ROW_OPERAND ? 16 * a + 4 * j : 16 * j + 4 * a);
+    typedef __attribute__((__vector_size__(4 * sizeof(T)))) T Op4;
+    Op4 h[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int k = 32 * kk + 8 * g + 4 * s + e;
+      h[s] = read_tr16(reinterpret_cast<const T*>(lds + k * (EXT * 2) + (((col >> 3) ^ swz_k<T, ROW_OPERAND>(k)) << 4) +
+                                                  (col & 4) * 2));
+    }
+    return __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+  } else {
+    const int col = base + (ROW_OPERAND ? frag_row(r, j) : 16 * j + r);
+    Frag f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int k = 16 * kk + 4 * g + e;
+      f[e] = *reinterpret_cast<const float*>(lds + k * (EXT * 4) + (((col >> 2) ^ swz_k<T, ROW_OPERAND>(k)) << 4) +
+                                             (col & 3) * 4);
+    }
+    return f;
+  }
+}
+
+struct Params {
+  const char* a;      // row operand: W (kFwd, kBwd, kDx), x (kDw)
+  const char* b;      // column operand: x (kFwd, kBwd), [dA dB] (kDx, kDw)
+  int64_t lda, ldb;   // bytes between their rows
+  int M, N, K;        // output columns (kFwd, kBwd: F), output rows (kDw: 2 Fp), K extent
+  int F, Fp;          // hidden width, and its multiple of 64 that [dA dB] is laid out by
+  int act;
+  int mt, nt, splits, steps;  // tiles along M and N, K splits, K steps of one split
+  void* out;          // h, [dA dB], dx or dW
+  int64_t ldo;        // elements between its rows
+  float* part;        // kDx, kDw with splits > 1: fp32 [splits][N][M]; kBwd: bias sums [column tiles' waves][2 Fp]
+  const void* bias;   // [2F] or null
+  const void* go;     // kBwd: [N, F]
+  int vec;            // rows of out (and go) are 16-byte aligned
+};
+
+// 16 consecutive elements, of which the first n exist
+template <typename T>
+__device__ __forceinline__ void store16(T* p, const float (&v)[16], int n, bool vec) {
+  typedef T V __attribute__((ext_vector_type(16 / sizeof(T))));
+  constexpr int E = kEpc<T>;
+  if (vec && n >= 16) {
+#pragma unroll
+    for (int i = 0; i < 16 / E; ++i) {
+      V o;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = Elem<T>::from_f32(v[i * E + e]);
+      reinterpret_cast<V*>(p)[i] = o;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i < n) p[i] = Elem<T>::from_f32(v[i]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void load16(const T* p, float (&v)[16], int n, bool vec) {
+  typedef T V __attribute__((ext_vector_type(16 / sizeof(T))));
+  constexpr int E = kEpc<T>;
+  if (vec && n >= 16) {
+#pragma unroll
+    for (int i = 0; i < 16 / E; ++i) {
+      const V o = reinterpret_cast<const V*>(p)[i];
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[i * E + e] = Elem<T>::to_f32(o[e]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = i < n ? Elem<T>::to_f32(p[i]) : 0.0f;
+  }
+}
+
+// WM waves of 128 rows (two groups of 64: gate and up of the same 64 hidden columns in kFwd and kBwd) by WN waves of
+// 16 NT columns.
+template <typename T, int MODE, int WM, int WN, int NT>
+__global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) gemm_kernel(Params p) {
+  constexpr int NW = WM * WN;
+  constexpr int BM = WM * 128, BN = WN * NT * 16, BK = kBK<T>;
+  constexpr bool kGated = MODE == kFwd || MODE == kBwd;
+  constexpr bool kAOut = MODE == kDx || MODE == kDw;  // K is the outer axis of the row operand
+  constexpr bool kBOut = MODE == kDw;
+  constexpr int TM = kGated ? BM / 2 : BM;            // output columns per tile
+  using TileA = Tile<T, kAOut, true, BM, NW>;
+  using TileB = Tile<T, kBOut, false, BN, NW>;
+  using Frag = typename Mma<T>::Frag;
+  // two objects per operand, so that a load into one is known not to touch the reads of the other
+  __shared__ __attribute__((aligned(1024))) char a0[TileA::kBytes];
+  __shared__ __attribute__((aligned(1024))) char b0[TileB::kBytes];
+  __shared__ __attribute__((aligned(1024))) char a1[TileA::kBytes];
+  __shared__ __attribute__((aligned(1024))) char b1[TileB::kBytes];
+
+  // XCD-aware order: blockIdx.x % 8 is the XCD; each gets a contiguous range of tiles, walked in groups of 8 column
+  // tiles so that the tiles resident together share rows of both operands
+  const int total = p.mt * p.nt * p.splits;
+  const int per = (total + 7) >> 3;
+  const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= per || id >= total) return;
+  const int split = id / (p.mt * p.nt);
+  int t = id - split * p.mt * p.nt;
+  const int group = t / (8 * p.mt);
+  t -= group * 8 * p.mt;
+  const int gn = min(8, p.nt - group * 8);
+  const int tm = t / gn, tn = group * 8 + (t - tm * gn);
+  const int m0 = tm * TM, n0 = tn * BN;
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % WM, wn = wave / WM;
+  TileA ta;
+  TileB tb;
+  const char* pa = p.a;
+  const char* pb = p.b;
+  if constexpr (kGated) {
+    ta.init(wave, lane, p.lda, p.F - m0, BM / 2, p.F - m0, int64_t(p.F) * p.lda);
+    pa += int64_t(m0) * p.lda;
+  } else {
+    ta.init(wave, lane, p.lda, p.M - m0, BM, 0, 0);
+    pa += int64_t(m0) * sizeof(T);
+  }
+  tb.init(wave, lane, p.ldb, p.N - n0, BN, 0, 0);
+  pb += kBOut ? int64_t(n0) * sizeof(T) : int64_t(n0) * p.ldb;
+
+  const int steps_all = (p.K + BK - 1) / BK;
+  const int s0 = split * p.steps, s1 = min(steps_all, s0 + p.steps);
+  auto load = [&](int s, char* la, char* lb) {
+    const int k0 = s * BK;
+    const int left = p.K - k0;
+    const char* xa;
+    int left_a = left;
+    if constexpr (MODE == kDx) {
+      // k runs over [dA dB]'s columns; each half of Fp has F rows of W
+      const int half = k0 >= p.Fp ? p.Fp : 0;
+      xa = pa + int64_t(k0 - half + (half ? p.F : 0)) * p.lda;
+      left_a = p.F - (k0 - half);
+    } else {
+      xa = kAOut ? pa + int64_t(k0) * p.lda : pa + int64_t(k0) * int(sizeof(T));
+    }
+    const char* xb = kBOut ? pb + int64_t(k0) * p.ldb : pb + int64_t(k0) * int(sizeof(T));
+    ta.load(xa, left_a, la, wave);
+    tb.load(xb, left, lb, wave);
+  };
+
+  mf_f32x4 acc[2][4][NT];
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) acc[q][j][i] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
+
+  auto multiply = [&](const char* la, const char* lb) {
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      Frag fb[NT];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) fb[i] = read_frag<T, kBOut, false, BN>(lb, wn * NT * 16, i, kk, lane);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int base = kGated ? q * (BM / 2) + wm * 64 : wm * 128 + q * 64;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const Frag fa = read_frag<T, kAOut, true, BM>(la, base, j, kk, lane);
+#pragma unroll
+          for (int i = 0; i < NT; ++i) Mma<T>::run(fa, fb[i], acc[q][j][i]);
+        }
+      }
+    }
+  };
+  auto ready = [] {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+  if (s0 < s1) load(s0, a0, b0);
+  for (int s = s0; s < s1; s += 2) {
+    ready();
+    if (s + 1 < s1) load(s + 1, a1, b1);
+    multiply(a0, b0);
+    if (s + 1 < s1) {
+      ready();
+      if (s + 2 < s1) load(s + 2, a0, b0);
+      multiply(a1, b1);
+    }
+  }
+
+  // lane (g, r16) holds, for column n0 + .. + 16 i + r16 of the tile, group rows 16 g .. 16 g + 15
+  const int g = lane >> 4, r16 = lane & 15;
+  constexpr bool kFast = sizeof(T) == 2;
+  if constexpr (kGated) {
+    const int f0 = m0 + wm * 64 + 16 * g;
+    const int left = p.F - f0;
+    float ba[16], bb[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) ba[e] = bb[e] = 0.0f;
+    if (p.bias) {
+      const T* bias = static_cast<const T*>(p.bias);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if (e < left) {
+          ba[e] = Elem<T>::to_f32(bias[f0 + e]);
+          bb[e] = Elem<T>::to_f32(bias[p.F + f0 + e]);
+        }
+      }
+    }
+    if constexpr (MODE == kFwd) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const int n = n0 + (wn * NT + i) * 16 + r16;
+        float h[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float a = acc[0][e >> 2][i][e & 3] + ba[e], b = acc[1][e >> 2][i][e & 3] + bb[e];
+          h[e] = act_value<kFast>(p.act, a) * b;
+        }
+        if (n < p.N) store16(static_cast<T*>(p.out) + int64_t(n) * p.ldo + f0, h, left, p.vec);
+      }
+    } else {
+      float sa[16], sb[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sa[e] = sb[e] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const int n = n0 + (wn * NT + i) * 16 + r16;
+        float go[16], da[16], db[16];
+        if (n < p.N) load16(static_cast<const T*>(p.go) + int64_t(n) * p.F + f0, go, left, p.vec);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float a = acc[0][e >> 2][i][e & 3] + ba[e], b = acc[1][e >> 2][i][e & 3] + bb[e];
+          float y, dy;
+          act_both<kFast>(p.act, a, y, dy);
+          const bool in = n < p.N && e < left;  // columns past F are zero, whatever x holds
+          da[e] = in ? go[e] * b * dy : 0.0f;
+          db[e] = in ? go[e] * y : 0.0f;
+          sa[e] += da[e];
+          sb[e] += db[e];
+        }
+        if (n < p.N && f0 < p.Fp) {
+          T* o = static_cast<T*>(p.out) + int64_t(n) * p.ldo + f0;
+          store16(o, da, 16, true);
+          store16(o + p.Fp, db, 16, true);
+        }
+      }
+      if (p.part) {
+        float* row = p.part + int64_t(tn * WN + wn) * 2 * p.Fp + f0;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          sa[e] = group16_sum(sa[e]);
+          sb[e] = group16_sum(sb[e]);
+        }
+        if (r16 == 0 && f0 < p.Fp) {
+          store16(row, sa, 16, true);
+          store16(row + p.Fp, sb, 16, true);
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int m = m0 + wm * 128 + q * 64 + 16 * g;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        int n = n0 + (wn * NT + i) * 16 + r16;
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = acc[q][e >> 2][i][e & 3];
+        bool in = n < p.N;
+        if constexpr (MODE == kDw) {
+          const int f = n >= p.Fp ? n - p.Fp : n;
+          in = in && f < p.F;
+          n = n >= p.Fp ? p.F + f : f;
+        }
+        if (!in || m >= p.M) continue;
+        if (p.splits > 1) {
+          const int64_t rows = MODE == kDw ? 2 * p.F : p.N;
+          store16(p.part + (split * rows + n) * int64_t(p.M) + m, v, p.M - m, true);
+        } else {
+          store16(static_cast<T*>(p.out) + int64_t(n) * p.ldo + m, v, min(p.M, int(p.ldo)) - m, p.vec);
+        }
+      }
+    }
+  }
+}
+
+// out[i] = sum over splits of part[s][i], in order; `cols` of every `ld` columns are kept.
+template <typename T>
+__global__ void __launch_bounds__(256) sum_kernel(const float* part, T* out, int splits, int64_t rows, int ld, int cols) {
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t n = rows * cols;
+  if (i >= n) return;
+  const int64_t r = i / cols;
+  const float* src = part + r * ld + (i - r * cols);
+  const int64_t plane = rows * ld;
+  float v = 0.0f;
+  for (int s = 0; s < splits; ++s) v += src[s * plane];
+  out[i] = Elem<T>::from_f32(v);
+}
+
+// dbias: column sums of `rows` partial rows of [2 Fp], one wave per 16 columns, four row strands each.
+template <typename T>
+__global__ void __launch_bounds__(256) bias_kernel(const float* part, T* out, int rows, int F, int Fp) {
+  __shared__ float sums[16][17];
+  const int c = threadIdx.x & 15, strand = threadIdx.x >> 4;
+  const int col = blockIdx.x * 16 + c;  // of the 2 Fp
+  float v = 0.0f;
+  for (int r = strand; r < rows; r += 16) v += part[int64_t(r) * 2 * Fp + col];
+  sums[strand][c] = v;
+  __syncthreads();
+  if (strand == 0) {
+    float s = 0.0f;
+    for (int k = 0; k < 16; ++k) s += sums[k][c];
+    const int f = col >= Fp ? col - Fp : col;
+    if (f < F) out[(col >= Fp ? F : 0) + f] = Elem<T>::from_f32(s);
+  }
+}
+
+// Rows of `cols` elements, `ld` apart, into rows of `pitch`, zero behind: the aligned copy of an operand whose rows
+// are no multiple of 16 bytes.
+template <typename T>
+__global__ void __launch_bounds__(256) pad_kernel(const T* src, T* dst, int64_t rows, int cols, int64_t ld, int pitch) {
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= rows * pitch) return;
+  const int64_t r = i / pitch;
+  const int c = int(i - r * pitch);
+  dst[i] = c < cols ? src[r * ld + c] : T(0.0f);
+}
+
+// -- host ----------------------------------------------------------------------------------------------------
+struct Plan {
+  int64_t T, C, F, Fp, Cp;  // Cp: channels of the padded copies (C when none is needed)
+  int esize;
+  bool pad_x, pad_w;
+  size_t x_bytes, w_bytes, dab_bytes, bias_bytes, dx_bytes, dw_bytes;
+  int dx_splits, dw_splits;
+};
+
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Tiles of 256 x 256 when they are enough to give every CU one, else of 128 x 128.
+bool large_tiles(int64_t m, int64_t n, int num_cus) {
+  return ((m + 255) / 256) * ((n + 255) / 256) >= num_cus;
+}
+
+// K splits of a product with few tiles: enough workgroups for two a CU, at least four K steps each.
+int k_splits(int64_t m, int64_t n, int64_t k, int bk, bool large, int num_cus) {
+  const int64_t b = large ? 256 : 128;
+  const int64_t tiles = ((m + b - 1) / b) * ((n + b - 1) / b);
+  const int64_t steps = (k + bk - 1) / bk;
+  const int64_t want = (2 * num_cus) / std::max<int64_t>(tiles, 1);
+  return int(std::max<int64_t>(1, std::min<int64_t>(want, steps / 4)));
+}
+
+void make_plan(Plan* q, int64_t T, int64_t C, int64_t F, int64_t x_stride, const void* x, const void* w, int dtype,
+               bool need_dx, bool need_dw, bool need_db, int num_cus) {
+  q->T = T;
+  q->C = C;
+  q->F = F;
+  q->esize = dtype == MF_DTYPE_F32 ? 4 : 2;
+  q->Fp = (F + 63) / 64 * 64;
+  const bool odd = C * q->esize % 16 != 0;
+  q->pad_x = odd || x_stride * q->esize % 16 != 0 || reinterpret_cast<uintptr_t>(x) % 16 != 0;
+  q->pad_w = odd || reinterpret_cast<uintptr_t>(w) % 16 != 0;
+  q->Cp = (C * q->esize + 15) / 16 * 16 / q->esize;
+  q->x_bytes = q->pad_x ? round256(size_t(T) * q->Cp * q->esize) : 0;
+  q->w_bytes = q->pad_w ? round256(size_t(2) * F * q->Cp * q->esize) : 0;
+  q->dab_bytes = need_dx || need_dw ? round256(size_t(T) * 2 * q->Fp * q->esize) : 0;
+  // bias sums of every column wave: 128-row tiles have 4 waves of 32, 256-row tiles 4 of 64
+  q->bias_bytes = need_db ? round256(size_t((T + 127) / 128) * 4 * 2 * q->Fp * 4) : 0;
+  const int bk = 128 / q->esize;
+  q->dx_splits = k_splits(q->Cp, T, 2 * q->Fp, bk, large_tiles(q->Cp, T, num_cus), num_cus);
+  q->dw_splits = k_splits(q->Cp, 2 * q->Fp, T, bk, large_tiles(q->Cp, 2 * q->Fp, num_cus), num_cus);
+  q->dx_bytes = need_dx && q->dx_splits > 1 ? round256(size_t(q->dx_splits) * T * q->Cp * 4) : 0;
+  q->dw_bytes = need_dw && q->dw_splits > 1 ? round256(size_t(q->dw_splits) * 2 * F * q->Cp * 4) : 0;
+}
+
+template <typename T, int MODE>
+void launch_gemm(Params p, bool large, hipStream_t s) {
+  const int tm = (MODE == kFwd || MODE == kBwd) ? (large ? 128 : 64) : (large ? 256 : 128);
+  const int tn = large ? 256 : 128;
+  p.mt = (p.M + tm - 1) / tm;
+  p.nt = (p.N + tn - 1) / tn;
+  const int bk = kBK<T>;
+  const int steps = (p.K + bk - 1) / bk;
+  p.steps = (steps + p.splits - 1) / p.splits;
+  const int64_t total = int64_t(p.mt) * p.nt * p.splits;
+  const dim3 grid(unsigned((total + 7) / 8 * 8));
+  if (large) hipLaunchKernelGGL((gemm_kernel<T, MODE, 2, 4, 4>), grid, dim3(512), 0, s, p);
+  else hipLaunchKernelGGL((gemm_kernel<T, MODE, 1, 4, 2>), grid, dim3(256), 0, s, p);
+}
+
+template <typename T>
+void pad_rows(const void* src, void* dst, int64_t rows, int64_t cols, int64_t ld, int64_t pitch, hipStream_t s) {
+  const int64_t n = rows * pitch;
+  if (n > 0)
+    hipLaunchKernelGGL(pad_kernel<T>, dim3(unsigned((n + 255) / 256)), dim3(256), 0, s, static_cast<const T*>(src),
+                       static_cast<T*>(dst), rows, int(cols), ld, int(pitch));
+}
+
+// x and W, as the tile kernel reads them: in place, or their aligned copies at ws
+template <typename T>
+char* operands(const Plan& q, const void* x, int64_t x_stride, const void* w, char* ws, Params* p, hipStream_t s) {
+  p->a = static_cast<const char*>(w);
+  p->lda = q.C * sizeof(T);
+  p->b = static_cast<const char*>(x);
+  p->ldb = x_stride * sizeof(T);
+  if (q.pad_x) {
+    pad_rows<T>(x, ws, q.T, q.C, x_stride, q.Cp, s);
+    p->b = ws;
+    p->ldb = q.Cp * sizeof(T);
+    ws += q.x_bytes;
+  }
+  if (q.pad_w) {
+    pad_rows<T>(w, ws, 2 * q.F, q.C, q.C, q.Cp, s);
+    p->a = ws;
+    p->lda = q.Cp * sizeof(T);
+    ws += q.w_bytes;
+  }
+  p->F = int(q.F);
+  p->Fp = int(q.Fp);
+  p->splits = 1;
+  return ws;
+}
+
+bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
+
+template <typename T>
+int forward(const mf_gated_linear_args* a, const Plan& q, int num_cus, hipStream_t s) {
+  Params p = {};
+  operands<T>(q, a->x, a->x_stride, a->weight, static_cast<char*>(a->workspace), &p, s);
+  p.M = int(q.F);
+  p.N = int(q.T);
+  p.K = int(q.Cp);
+  p.act = a->activation;
+  p.out = a->out;
+  p.ldo = q.F;
+  p.bias = a->bias;
+  p.vec = q.F * q.esize % 16 == 0 && aligned16(a->out);
+  launch_gemm<T, kFwd>(p, large_tiles(2 * q.F, q.T, num_cus), s);
+  MF_HIP_CHECK(hipGetLastError());
+  return MF_OK;
+}
+
+template <typename T>
+int backward(const mf_gated_linear_bwd_args* a, const Plan& q, int num_cus, hipStream_t s) {
+  const mf_gated_linear_args& f = a->fwd;
+  Params p = {};
+  char* ws = operands<T>(q, f.x, f.x_stride, f.weight, static_cast<char*>(a->workspace), &p, s);
+  const char *w = p.a, *x = p.b;
+  const int64_t ldw = p.lda, ldx = p.ldb;
+  T* dab = reinterpret_cast<T*>(ws);
+  ws += round256(size_t(q.T) * 2 * q.Fp * sizeof(T));
+  float* sums = a->dbias ? reinterpret_cast<float*>(ws) : nullptr;
+  ws += q.bias_bytes;
+  const bool big = large_tiles(2 * q.F, q.T, num_cus);
+  p.M = int(q.F);
+  p.N = int(q.T);
+  p.K = int(q.Cp);
+  p.act = f.activation;
+  p.out = dab;
+  p.ldo = 2 * q.Fp;
+  p.bias = f.bias;
+  p.go = a->grad_out;
+  p.part = sums;
+  p.vec = q.F * q.esize % 16 == 0 && aligned16(a->grad_out);
+  if (q.T > 0) launch_gemm<T, kBwd>(p, big, s);
+  MF_HIP_CHECK(hipGetLastError());
+  if (a->dbias) {
+    const int rows = q.T == 0 ? 0 : int((q.T + (big ? 255 : 127)) / (big ? 256 : 128)) * 4;
+    hipLaunchKernelGGL(bias_kernel<T>, dim3(unsigned(2 * q.Fp / 16)), dim3(256), 0, s, sums, static_cast<T*>(a->dbias),
+                       rows, int(q.F), int(q.Fp));
+    MF_HIP_CHECK(hipGetLastError());
+  }
+  if (a->dx && q.T > 0) {
+    Params d = p;
+    d.a = w;
+    d.lda = ldw;
+    d.b = reinterpret_cast<const char*>(dab);
+    d.ldb = 2 * q.Fp * sizeof(T);
+    d.M = int(q.Cp);
+    d.N = int(q.T);
+    d.K = int(2 * q.Fp);
+    d.out = a->dx;
+    d.ldo = q.C;
+    d.splits = q.dx_splits;
+    d.part = reinterpret_cast<float*>(ws);
+    d.vec = q.C * q.esize % 16 == 0 && aligned16(a->dx);
+    launch_gemm<T, kDx>(d, large_tiles(q.Cp, q.T, num_cus), s);
+    MF_HIP_CHECK(hipGetLastError());
+    if (d.splits > 1) {
+      hipLaunchKernelGGL(sum_kernel<T>, dim3(unsigned((q.T * q.C + 255) / 256)), dim3(256), 0, s, d.part,
+                         static_cast<T*>(a->dx), d.splits, q.T, int(q.Cp), int(q.C));
+      MF_HIP_CHECK(hipGetLastError());
+    }
+    ws += q.dx_bytes;
+  }
+  if (a->dweight) {
+    Params d = p;
+    d.a = x;
+    d.lda = ldx;
+    d.b = reinterpret_cast<const char*>(dab);
+    d.ldb = 2 * q.Fp * sizeof(T);
+    d.M = int(q.Cp);
+    d.N = int(2 * q.Fp);
+    d.K = int(q.T);
+    d.out = a->dweight;
+    d.ldo = q.C;
+    d.splits = q.dw_splits;
+    d.part = reinterpret_cast<float*>(ws);
+    d.vec = q.C * q.esize % 16 == 0 && aligned16(a->dweight);
+    launch_gemm<T, kDw>(d, large_tiles(q.Cp, 2 * q.Fp, num_cus), s);
+    MF_HIP_CHECK(hipGetLastError());
+    if (d.splits > 1) {
+      hipLaunchKernelGGL(sum_kernel<T>, dim3(unsigned((2 * q.F * q.C + 255) / 256)), dim3(256), 0, s, d.part,
+                         static_cast<T*>(a->dweight), d.splits, 2 * q.F, int(q.Cp), int(q.C));
+      MF_HIP_CHECK(hipGetLastError());
+    }
+  }
+  return MF_OK;
+}
+
+int check(const char* name, const mf_gated_linear_args* a) {
+  const std::string n(name);
+  if (!a->x || !a->weight) return fail(MF_ERR_INVALID_ARGUMENT, n + ": x and weight must be non-NULL");
+  if (a->tokens < 0 || a->channels <= 0 || a->hidden <= 0 || a->x_stride < a->channels)
+    return fail(MF_ERR_INVALID_ARGUMENT, n + ": tokens must be non-negative, channels and hidden positive, x_stride >= channels");
+  if (a->dtype != MF_DTYPE_F32 && a->dtype != MF_DTYPE_F16 && a->dtype != MF_DTYPE_BF16)
+    return fail(MF_ERR_INVALID_ARGUMENT, n + ": bad dtype");
+  if (a->activation < MF_ACT_SILU || a->activation > MF_ACT_SIGMOID)
+    return fail(MF_ERR_INVALID_ARGUMENT, n + ": bad activation");
+  // tile-relative byte offsets are 32 bits: the weight below 2^31 bytes, 256 rows of x and of [dA dB] too
+  const int64_t esize = a->dtype == MF_DTYPE_F32 ? 4 : 2;
+  if ((a->channels + 8) * int64_t(a->hidden) * 2 * esize >= (int64_t(1) << 31) ||
+      a->x_stride * 256 * esize >= (int64_t(1) << 31) || int64_t(a->hidden + 64) * 512 * esize >= (int64_t(1) << 31) ||
+      a->tokens > (1 << 30))
+    return fail(MF_ERR_UNSUPPORTED, n + ": weight of 2^31 bytes, rows of 2^22 elements or 2^30 tokens and more are not supported");
+  return MF_OK;
+}
+
+}  // namespace gated
+}  // namespace mf
+
+extern "C" uint64_t mf_gated_linear_workspace_size(const mf_gated_linear_args* a) {
+  using namespace mf;
+  using namespace mf::gated;
+  if (a == nullptr || check("mf_gated_linear_workspace_size", a) != MF_OK) return 0;
+  Plan q;
+  make_plan(&q, a->tokens, a->channels, a->hidden, a->x_stride, a->x, a->weight, a->dtype, false, false, false, 256);
+  return q.x_bytes + q.w_bytes;
+}
+
+extern "C" int mf_gated_linear(const mf_gated_linear_args* a, void* stream) {
+  using namespace mf;
+  using namespace mf::gated;
+  if (a == nullptr) return fail(MF_ERR_INVALID_ARGUMENT, "mf_gated_linear: args is NULL");
+  int st = check("mf_gated_linear", a);
+  if (st != MF_OK) return st;
+  if (!a->out) return fail(MF_ERR_INVALID_ARGUMENT, "mf_gated_linear: out must be non-NULL");
+  if (a->tokens == 0) return MF_OK;
+  DeviceInfo info;
+  st = device_info(&info);
+  if (st != MF_OK) return st;
+  Plan q;
+  make_plan(&q, a->tokens, a->channels, a->hidden, a->x_stride, a->x, a->weight, a->dtype, false, false, false,
+            info.num_cus);
+  if (q.x_bytes + q.w_bytes > 0 && (!a->workspace || a->workspace_bytes < q.x_bytes + q.w_bytes))
+    return fail(MF_ERR_INVALID_ARGUMENT, "mf_gated_linear: workspace is smaller than mf_gated_linear_workspace_size");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (a->dtype) {
+    case MF_DTYPE_BF16: return forward<__bf16>(a, q, info.num_cus, s);
+    case MF_DTYPE_F16: return forward<_Float16>(a, q, info.num_cus, s);
+    default: return forward<float>(a, q, info.num_cus, s);
+  }
+}
+
+static int bwd_plan(const mf_gated_linear_bwd_args* a, mf::gated::Plan* q, int num_cus) {
+  using namespace mf;
+  using namespace mf::gated;
+  const int st = check("mf_gated_linear_bwd", &a->fwd);
+  if (st != MF_OK) return st;
+  const mf_gated_linear_args& f = a->fwd;
+  make_plan(q, f.tokens, f.channels, f.hidden, f.x_stride, f.x, f.weight, f.dtype, a->dx != nullptr,
+            a->dweight != nullptr, a->dbias != nullptr, num_cus);
+  q->dab_bytes = round256(size_t(q->T) * 2 * q->Fp * q->esize);
+  return MF_OK;
+}
+
+extern "C" uint64_t mf_gated_linear_bwd_workspace_size(const mf_gated_linear_bwd_args* a) {
+  using namespace mf;
+  using namespace mf::gated;
+  DeviceInfo info;
+  Plan q;
+  if (a == nullptr || check("mf_gated_linear_bwd_workspace_size", &a->fwd) != MF_OK) return 0;
+  if (device_info(&info) != MF_OK || bwd_plan(a, &q, info.num_cus) != MF_OK) return 0;
+  return q.x_bytes + q.w_bytes + q.dab_bytes + q.bias_bytes + q.dx_bytes + q.dw_bytes;
+}
+
+extern "C" int mf_gated_linear_bwd(const mf_gated_linear_bwd_args* a, void* stream) {
+  using namespace mf;
+  using namespace mf::gated;
+  if (a == nullptr) return fail(MF_ERR_INVALID_ARGUMENT, "mf_gated_linear_bwd: args is NULL");
+  int st = check("mf_gated_linear_bwd", &a->fwd);
+  if (st != MF_OK) return st;
+  if (!a->grad_out) return fail(MF_ERR_INVALID_ARGUMENT, "mf_gated_linear_bwd: grad_out must be non-NULL");
+  if (!a->dx && !a->dweight && !a->dbias)
+    return fail(MF_ERR_INVALID_ARGUMENT, "mf_gated_linear_bwd: nothing to compute");
+  DeviceInfo info;
+  st = device_info(&info);
+  if (st != MF_OK) return st;
+  Plan q;
+  st = bwd_plan(a, &q, info.num_cus);
+  if (st != MF_OK) return st;
+  const size_t need = q.x_bytes + q.w_bytes + q.dab_bytes + q.bias_bytes + q.dx_bytes + q.dw_bytes;
+  if (need > 0 && (!a->workspace || a->workspace_bytes < need))
+    return fail(MF_ERR_INVALID_ARGUMENT,
+                "mf_gated_linear_bwd: workspace is smaller than mf_gated_linear_bwd_workspace_size");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (a->fwd.dtype) {
+    case MF_DTYPE_BF16: return backward<__bf16>(a, q, info.num_cus, s);
+    case MF_DTYPE_F16: return backward<_Float16>(a, q, info.num_cus, s);
+    default: return backward<float>(a, q, info.num_cus, s);
+  }
+}

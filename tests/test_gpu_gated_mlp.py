@@ -1,0 +1,245 @@
+"""mf_gated_linear and mf_gated_linear_bwd against float64, element by element.
+
+Tolerances, from the arithmetic.  u = 2^-24.  A sum of n products in fp32, in any order, is within n u sum|x w| of the
+exact one (n products and n - 1 additions; the matrix cores add exactly or in fp32); with the bias one more.  So a and
+b are within ea = (C + 1) u (|x| |Wg|^T + |bg|) and eb alike.  The activations have |act'| <= 1.13 (gelu) and
+|act''| <= 0.8; evaluated in fp32 they are off by a few u (16-bit types: a few units of hardware exp2 and reciprocal and
+the rounding of the exponent, below |x| u per exponent: 64 u covers |a| <= 30, where the inputs here lie; fp32: 16 u).
+With y = act(a):
+  |dh| <= 1.13 ea |b| + |y| eb + k u (|y b|)                                    k = 64 or 16
+  |dA - exact| <= |go| (1.13 eb + 0.8 ea |b| + k u |b act'| + k u |b|),  |dB - exact| <= |go| (1.13 ea + k u |y| + k u)
+and dA, dB are rounded to the type (eps / 2 relative) before the two products, which add their own fp32 sums: with
+E = the error of [dA dB] just named,
+  |dx - exact| <= E |W| + (2F + 1) u |[dA dB]| |W|,   |dW - exact| <= E^T |x| + (T + 1) u |[dA dB]|^T |x|.
+dbias sums the unrounded values.  Each output rounds once more, eps / 2 relative or half the smallest subnormal."""
+
+import math
+
+import pytest
+import torch
+
+from matterformer_amd.gated_mlp import ACTIVATIONS, gated_linear
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+U = 2.0 ** -24
+
+
+def _act64(a, name):
+    """Value and derivative in float64."""
+    sig = torch.sigmoid(a)
+    if name == "relu":
+        return a.clamp_min(0), (a > 0).double()
+    if name == "sigmoid":
+        return sig, sig * (1 - sig)
+    if name == "silu":
+        return a * sig, sig * (1 + a * (1 - sig))
+    if name == "gelu":
+        cdf = 0.5 * torch.erfc(-a / math.sqrt(2.0))
+        return a * cdf, cdf + a * torch.exp(-0.5 * a * a) / math.sqrt(2 * math.pi)
+    c = 2 * math.sqrt(2 / math.pi)
+    s = torch.sigmoid(c * (a + 0.044715 * a ** 3))
+    return a * s, s + a * s * (1 - s) * c * (1 + 3 * 0.044715 * a * a)
+
+
+def _inputs(T, C, F, dtype, bias, seed, device, scale=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    x = (torch.randn(T, C, generator=gen) * scale).to(dtype)
+    w = ((torch.rand(2 * F, C, generator=gen) * 2 - 1) * C ** -0.5).to(dtype)
+    b = (torch.rand(2 * F, generator=gen) - 0.5).to(dtype) if bias else None
+    go = (torch.randn(T, F, generator=gen) * 0.1).to(dtype)
+    return [None if t is None else t.to(device) for t in (x, w, b, go)]
+
+
+def _reference(x, w, b, go, name):
+    """Outputs in float64 and their bounds before the last rounding."""
+    x, w, go = x.double(), w.double(), go.double()
+    C, F, T = x.shape[1], w.shape[0] // 2, x.shape[0]
+    b = torch.zeros(2 * F, dtype=torch.float64, device=x.device) if b is None else b.double()
+    both = x @ w.T + b
+    e = (C + 1) * U * (x.abs() @ w.abs().T + b.abs())
+    (a, up), (ea, eb) = both.chunk(2, -1), e.chunk(2, -1)
+    y, dy = _act64(a, name)
+    return x, w, go, a, up, ea, eb, y, dy, C, F, T
+
+
+def _close(got, want, bound, what):
+    fi = torch.finfo(got.dtype)
+    tol = bound + (want.abs() + bound) * fi.eps / 2 + fi.smallest_normal * fi.eps / 2
+    err = (got.double() - want).abs()
+    over = err - tol
+    assert torch.all(over <= 0), f"{what}: off by {float(err.max()):.3e}, {float(over.max()):.3e} past the bound"
+
+
+def _check(x, w, b, go, name, got, grads=None):
+    dtype = x.dtype
+    k = 16 if dtype == torch.float32 else 64
+    half = torch.finfo(dtype).eps / 2
+    X, W, GO, a, up, ea, eb, y, dy, C, F, T = _reference(x, w, b, go, name)
+    _close(got, y * up, 1.13 * ea * up.abs() + y.abs() * eb + k * U * (y * up).abs(), "h")
+    if grads is None:
+        return
+    da, db = GO * up * dy, GO * y
+    fa = GO.abs() * (1.13 * eb + 0.8 * ea * up.abs() + k * U * (up * dy).abs() + k * U * up.abs())
+    fb = GO.abs() * (1.13 * ea + k * U * y.abs() + k * U)
+    dab, fab = torch.cat([da, db], -1), torch.cat([fa, fb], -1)
+    tiny = torch.finfo(dtype).smallest_normal * half
+    rounded = fab + (dab.abs() + fab) * half + tiny
+    dx, dw, dbias = grads
+    mag = dab.abs() + rounded
+    _close(dx, dab @ W, rounded @ W.abs() + (2 * F + 1) * U * (mag @ W.abs()), "dx")
+    _close(dw, dab.T @ X, rounded.T @ X.abs() + (T + 1) * U * (mag.T @ X.abs()), "dW")
+    if b is not None:
+        _close(dbias, dab.sum(0), fab.sum(0) + (T + 1) * U * (dab.abs() + fab).sum(0), "dbias")
+
+
+def _run(x, w, b, go, name):
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b) if t is not None]
+    out = gated_linear(*leaves, activation=name)
+    grads = torch.autograd.grad(out, leaves, go)
+    return out.detach(), [*grads, *([None] if b is None else [])]
+
+
+SIZES = [
+    # T, C, F
+    (1, 8, 1), (1, 512, 256), (3, 17, 5), (16, 64, 64), (17, 72, 65), (33, 200, 100), (64, 128, 129), (65, 63, 200),
+    (129, 136, 64), (300, 512, 341), (1000, 96, 128), (257, 1000, 70),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,C,F", SIZES)
+def test_sizes(cuda, dtype, T, C, F):
+    print(f"gated T={T} C={C} F={F} {dtype}", flush=True)
+    x, w, b, go = _inputs(T, C, F, dtype, (T + C) % 2 == 0, T * 7 + C, cuda)
+    out, grads = _run(x, w, b, go, "silu")
+    _check(x, w, b, go, "silu", out, grads)
+    with torch.no_grad():
+        again = gated_linear(x, w, b)
+    assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+def test_activations(cuda, dtype, activation):
+    x, w, b, go = _inputs(130, 96, 80, dtype, True, 5, cuda, scale=4.0)
+    _check(x, w, b, go, activation, *_run(x, w, b, go, activation))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_large_tiles(cuda, dtype):
+    """Enough tiles of 256 for every CU in each of the three products, rows and columns that end inside one."""
+    T, C, F = (4000, 1096, 1025) if dtype == torch.bfloat16 else (4000, 1096, 1025)
+    x, w, b, go = _inputs(T, C, F, dtype, True, 11, cuda)
+    _check(x, w, b, go, "gelu_tanh", *_run(x, w, b, go, "gelu_tanh"))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_two_calls_give_identical_bits(cuda, dtype):
+    x, w, b, go = _inputs(700, 256, 192, dtype, True, 12, cuda)
+    one, two = _run(x, w, b, go, "silu"), _run(x, w, b, go, "silu")
+    assert torch.equal(one[0], two[0]) and all(torch.equal(p, q) for p, q in zip(one[1], two[1]))
+
+
+def test_views(cuda):
+    """Rows apart (a slice of wider rows), more leading axes, a transposed weight, an expanded gradient."""
+    x, w, b, go = _inputs(60, 80, 48, torch.bfloat16, True, 13, cuda)
+    wide = torch.full((60, 120), float("nan"), dtype=torch.bfloat16, device=cuda)
+    for start in (0, 8, 3):  # aligned twice, then not
+        part = wide[:, start:start + 80]
+        part.copy_(x)
+        assert torch.equal(gated_linear(part, w, b), gated_linear(x, w, b))
+    assert torch.equal(gated_linear(x.view(3, 4, 5, 80), w, b).view(60, 48), gated_linear(x, w, b))
+    assert torch.equal(gated_linear(x, w.t().contiguous().t(), b), gated_linear(x, w, b))
+    assert torch.equal(gated_linear(x[0], w, b), gated_linear(x[:1], w, b)[0])
+    one = x[:1].expand(60, 80)
+    assert torch.equal(gated_linear(one, w, b), gated_linear(one.contiguous(), w, b))
+    leaf = x.clone().requires_grad_(True)
+    gated_linear(leaf, w, b).sum().backward()
+    _check(x, w, b, torch.ones_like(go), "silu", gated_linear(x, w, b),
+           [leaf.grad, *_run(x, w, b, torch.ones_like(go), "silu")[1][1:]])
+
+
+def test_gradients_of_some_inputs(cuda):
+    x, w, b, go = _inputs(40, 64, 32, torch.bfloat16, True, 14, cuda)
+    _, full = _run(x, w, b, go, "silu")
+    for needs in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1)):
+        leaves = [t.detach().requires_grad_(bool(n)) for t, n in zip((x, w, b), needs)]
+        grads = torch.autograd.grad(gated_linear(*leaves), [t for t, n in zip(leaves, needs) if n], go)
+        assert all(torch.equal(g, f) for g, f in zip(grads, [f for f, n in zip(full, needs) if n]))
+
+
+def test_gradient_against_differences(cuda):
+    x, w, b, go = _inputs(9, 24, 12, torch.float32, True, 15, cuda)
+    _, grads = _run(x, w, b, go, "gelu")
+    gen = torch.Generator().manual_seed(16)
+    for leaf, grad in zip((x, w, b), grads):
+        step = torch.randn(leaf.shape, generator=gen).to(cuda)
+        ends = []
+        for s in (1.0, -1.0):
+            t = [v.double() for v in (x, w, b)]
+            t = [v + s * 1e-4 * step.double() if v.shape == leaf.shape else v for v in t]
+            both = t[0] @ t[1].T + t[2]
+            ends.append(float((_act64(both[:, :12], "gelu")[0] * both[:, 12:] * go.double()).sum()))
+        slope = float((grad.double() * step.double()).sum())
+        size = float((grad.double() * step.double()).abs().sum())
+        # central differences of step 1e-4 in float64: third derivatives of order 10 leave 1e-8 relative to the sum;
+        # the gradient's own sums carry about 60 roundings
+        assert abs((ends[0] - ends[1]) / 2e-4 - slope) <= size * 200 * U + 1e-6
+
+
+def test_rows_of_other_tokens_stay_apart(cuda):
+    """NaN and infinity in one token's row reach that row only (and every weight gradient)."""
+    x, w, b, go = _inputs(130, 64, 70, torch.bfloat16, True, 17, cuda)
+    bad = x.clone()
+    bad[129, 3] = float("nan")
+    bad[5, 7] = float("inf")
+    out, (dx, _, _) = _run(bad, w, b, go, "silu")
+    ref, (rx, _, _) = _run(x, w, b, go, "silu")
+    keep = torch.ones(130, dtype=torch.bool, device=cuda)
+    keep[[5, 129]] = False
+    assert torch.equal(out[keep], ref[keep]) and torch.equal(dx[keep], rx[keep])
+    assert torch.isnan(out[129]).all()
+
+
+def test_empty(cuda):
+    w = torch.zeros(8, 16, device=cuda, requires_grad=True)
+    b = torch.zeros(8, device=cuda, requires_grad=True)
+    x = torch.zeros(0, 16, device=cuda, requires_grad=True)
+    out = gated_linear(x, w, b)
+    assert out.shape == (0, 4)
+    dx, dw, db = torch.autograd.grad(out, (x, w, b), torch.zeros(0, 4, device=cuda))
+    assert dx.shape == (0, 16) and torch.equal(dw, torch.zeros_like(w)) and torch.equal(db, torch.zeros_like(b))
+
+
+def test_gpu_refusals(cuda):
+    with pytest.raises(RuntimeError, match="bfloat16, float16 and float32"):
+        gated_linear(torch.zeros(2, 8, device=cuda).double(), torch.zeros(4, 8, device=cuda).double())
+    with pytest.raises(RuntimeError, match="share a dtype and a device"):
+        gated_linear(torch.zeros(2, 8, device=cuda), torch.zeros(4, 8))
+
+
+@pytest.mark.parametrize("C", [128, 100, 77])
+def test_stream_and_graph(cuda, C):
+    """Forward and backward on a side stream, then captured and replayed with eager work in between; with C = 77 the
+    aligned copies are part of the graph."""
+    x, w, b, go = _inputs(300, C, 96, torch.bfloat16, True, 18, cuda)
+    want = _run(x, w, b, go, "silu")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _run(x, w, b, go, "silu")
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and all(torch.equal(p, q) for p, q in zip(got[1], want[1]))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = _run(x, w, b, go, "silu")
+    gen = torch.Generator().manual_seed(19)
+    for turn in range(3):
+        x.copy_(torch.randn(300, C, generator=gen).to(torch.bfloat16))
+        graph.replay()
+        torch.cuda.synchronize()
+        now = _run(x, w, b, go, "silu")
+        assert torch.equal(held[0], now[0]) and all(torch.equal(p, q) for p, q in zip(held[1], now[1])), turn
