@@ -475,6 +475,8 @@ typedef struct mf_radius_attn_args {
   int32_t atoms;
   int32_t head_dim;            /* 32, 64 or 128                              */
   int32_t dtype;               /* MF_DTYPE_BF16 or MF_DTYPE_F16              */
+  const uint64_t* key_any;     /* ABI 12: of mf_radius_tables, or NULL.  With it, keys that no query of a */
+                               /* tile attends count as zeros, whatever they hold (NaN).                  */
 } mf_radius_attn_args;
 
 int mf_radius_attn(const mf_radius_attn_args* args, void* stream);
@@ -641,6 +643,65 @@ typedef struct mf_pair_mlp_bwd_args {
 
 uint64_t mf_pair_mlp_bias_bwd_workspace_size(int32_t hidden);
 int mf_pair_mlp_bias_bwd(const mf_pair_mlp_bwd_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Tables of a neighbour bit mask (ABI 12), for mf_radius_attn_bwd and, its  */
+/* key_any, mf_radius_attn: the transposed mask and, for every 64 x 64 tile, */
+/* the keys that a query of the tile attends and the queries with a key in   */
+/* it (bit t: row t of the tile).  Tiles whose block_mask entry is 0 count   */
+/* as empty.  One launch, shared by every head and layer that uses the mask. */
+/* ------------------------------------------------------------------------ */
+typedef struct mf_radius_tables_args {
+  const uint32_t* mask_bits;   /* [B, N, ceil(N/32)]                         */
+  const uint8_t* block_mask;   /* [B, NB, NB] for block 64, or NULL          */
+  uint32_t* mask_bits_t;       /* [B, N, ceil(N/32)]                         */
+  uint64_t* key_any;           /* [B, NB query tiles, NB key tiles]          */
+  uint64_t* query_any;         /* [B, NB key tiles, NB query tiles]          */
+  int32_t batch;
+  int32_t atoms;
+} mf_radius_tables_args;
+
+int mf_radius_tables(const mf_radius_tables_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Gradients of mf_radius_attn (ABI 12), from its q, k, v, out, lse and mask: */
+/* with P = exp(scale q_i . k_j - lse_i) on the allowed pairs and            */
+/* delta_i = grad_out_i . out_i - grad_lse_i,                                */
+/*   dv_j = sum_i P_ij grad_out_i,  dS_ij = P_ij (grad_out_i . v_j - delta_i), */
+/*   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i.            */
+/* Rows without an allowed partner get zeros, and what they hold reaches no  */
+/* other row.  Sums in fp32 in a fixed order (two calls give identical bits); */
+/* P and dS rounded to dtype in between (dS of fp16 times a power of two per */
+/* molecule and head, so that it neither overflows nor loses small values).  */
+/* The workspace needs no fill and is 16-byte aligned.                       */
+/* ------------------------------------------------------------------------ */
+typedef struct mf_radius_attn_bwd_args {
+  const void* q;               /* [B, H, N, D], dtype bf16 or fp16           */
+  const void* k;
+  const void* v;
+  const void* out;             /* [B, H, N, D] the forward's out             */
+  const float* lse;            /* [B, H, N] the forward's lse                */
+  const void* grad_out;        /* [B, H, N, D]                               */
+  const float* grad_lse;       /* [B, H, N] fp32, or NULL (none)             */
+  const uint32_t* mask_bits;   /* as in the forward                          */
+  const uint32_t* mask_bits_t; /* and its mf_radius_tables                   */
+  const uint64_t* key_any;
+  const uint64_t* query_any;
+  void* dq;                    /* [B, H, N, D] dtype, every entry written    */
+  void* dk;
+  void* dv;
+  void* workspace;
+  uint64_t workspace_bytes;
+  float scale;
+  int32_t batch;
+  int32_t heads;
+  int32_t atoms;
+  int32_t head_dim;            /* 32, 64 or 128                              */
+  int32_t dtype;               /* MF_DTYPE_BF16 or MF_DTYPE_F16              */
+} mf_radius_attn_bwd_args;
+
+uint64_t mf_radius_attn_bwd_workspace_size(int32_t batch, int32_t heads, int32_t atoms, int32_t dtype);
+int mf_radius_attn_bwd(const mf_radius_attn_bwd_args* args, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* Rotary positions (ABI 12).  Every pair (x0, x1) of a head's first         */

@@ -66,6 +66,9 @@ EXPORTED_SYMBOLS = (
     "mf_lattice_terms",
     "mf_pair_mlp_bias_bwd",
     "mf_pair_mlp_bias_bwd_workspace_size",
+    "mf_radius_tables",
+    "mf_radius_attn_bwd",
+    "mf_radius_attn_bwd_workspace_size",
     "mf_rotary",
     "mf_gated_linear",
     "mf_gated_linear_workspace_size",
@@ -207,7 +210,13 @@ class MfRadiusAttnArgs(ctypes.Structure):
         ("atoms", ctypes.c_int32),
         ("head_dim", ctypes.c_int32),
         ("dtype", ctypes.c_int32),
+        ("key_any", ctypes.c_void_p),
     ]
+
+
+class MfRadiusTablesArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("mask_bits", "block_mask", "mask_bits_t", "key_any", "query_any")] + [
+        (n, ctypes.c_int32) for n in ("batch", "atoms")]
 
 
 class MfAdalnRowsArgs(ctypes.Structure):
@@ -238,6 +247,13 @@ class MfPairMlpBwdArgs(ctypes.Structure):
     _fields_ = [("fwd", MfPairMlpArgs)] + [(f"{m}_grad", ctypes.c_void_p) for m in "uvw"] + [
         (f"{m}_{t}", ctypes.c_void_p) for m in "uvw" for t in ("dw1", "db1", "dw2", "db2")] + [
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class MfRadiusAttnBwdArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "lse", "grad_out", "grad_lse", "mask_bits",
+                                               "mask_bits_t", "key_any", "query_any", "dq", "dk", "dv", "workspace")] + [
+        ("workspace_bytes", ctypes.c_uint64), ("scale", ctypes.c_float)] + [
+        (n, ctypes.c_int32) for n in ("batch", "heads", "atoms", "head_dim", "dtype")]
 
 
 class MfRotaryArgs(ctypes.Structure):
@@ -296,6 +312,8 @@ def _load() -> ctypes.CDLL | None:
         ("mf_heads_to_rows", MfHeadsToRowsArgs),
         ("mf_pair_mlp_bias", MfPairMlpArgs),
         ("mf_pair_mlp_bias_bwd", MfPairMlpBwdArgs),
+        ("mf_radius_tables", MfRadiusTablesArgs),
+        ("mf_radius_attn_bwd", MfRadiusAttnBwdArgs),
         ("mf_rotary", MfRotaryArgs),
         ("mf_gated_linear", MfGatedLinearArgs),
         ("mf_gated_linear_bwd", MfGatedLinearBwdArgs),
@@ -327,6 +345,9 @@ def _load() -> ctypes.CDLL | None:
         if fn is not None:
             fn.argtypes = [ctypes.POINTER(argtype)]
             fn.restype = ctypes.c_uint64
+    if getattr(lib, "mf_radius_attn_bwd_workspace_size", None) is not None:
+        lib.mf_radius_attn_bwd_workspace_size.argtypes = [ctypes.c_int32] * 4
+        lib.mf_radius_attn_bwd_workspace_size.restype = ctypes.c_uint64
     version = lib.mf_abi_version()
     if version != EXPECTED_ABI_VERSION:
         _LOAD_ERROR = f"{path} has ABI version {version}, expected {EXPECTED_ABI_VERSION}"

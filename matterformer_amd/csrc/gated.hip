@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) gemm_kernel(Params 
     }
   };
   auto ready = [] {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's loads into LDS have landed
     __syncthreads();
   };
   if (s0 < s1) load(s0, a0, b0);

@@ -5,7 +5,9 @@
 // masked softmax an additive 0/-inf attn_mask gives in nn.MultiheadAttention /
 // scaled_dot_product_attention (src/matterformer/models/transformer.py:256-268,
 // src/matterformer/models/regular_attention.py:262-268,303-308).  Rows without
-// an allowed key give out = 0, lse = 0.
+// an allowed key give out = 0, lse = 0.  With the tables of mf_radius_tables,
+// keys that no query of a tile attends are staged as zeros (a NaN behind the
+// last atom stays there).
 //
 // One workgroup (4 waves) per (cell, head, 64-query tile); wave w owns the 16
 // queries 16w..16w+15 of the tile.  Key tiles of 64 whose block-mask entry is
@@ -41,6 +43,7 @@ struct Params {
   float scale_log2;  // scale * log2(e)
   int B, H, N, W, NB;
   int units;         // B * H * query tiles (the grid is rounded up to a multiple of 8)
+  const uint64_t* key_any;  // [B, NB, NB] keys of a tile that a query of the row's tile attends, or null
 };
 
 template <typename T>
@@ -143,7 +146,11 @@ __global__ void __launch_bounds__(kThreads) radius_attn_kernel(Params p) {
     uint32_t mok;     // bit 0 / 1: m0 / m1 are real words of a real query
     uint32_t valid;   // bit t: K chunk t is a real key; bit CPT + t: V chunk t
   };
+  // keys no query of this tile attends are staged as zeros, so that what they hold (NaN too) reaches no sum
+  const uint64_t* kany = p.key_any ? p.key_any + (size_t(b) * p.NB + qt) * p.NB : nullptr;
+  uint32_t seen = 0u;  // the query has a key
   auto load_tile = [&](int jt, Stage& st) {
+    const uint64_t set = kany ? kany[jt] : ~uint64_t(0);
     // the words are selected when used (a step later), so that nothing
     // waits for these loads now
     const int w0 = 2 * jt;
@@ -163,7 +170,8 @@ __global__ void __launch_bounds__(kThreads) radius_attn_kernel(Params p) {
       const int vd0 = (c / kTile) * 8;
       st.k[t] = *reinterpret_cast<const Op8*>(gk + size_t(min(key, N - 1)) * D + d0);
       st.v[t] = *reinterpret_cast<const Op8*>(gv + size_t(min(vkey, N - 1)) * D + vd0);
-      st.valid |= (key < N ? 1u << t : 0u) | (vkey < N ? 1u << (CPT + t) : 0u);
+      const bool kuse = key < N && ((set >> (c / CPR)) & 1u), vuse = vkey < N && ((set >> (c % kTile)) & 1u);
+      st.valid |= (kuse ? 1u << t : 0u) | (vuse ? 1u << (CPT + t) : 0u);
     }
   };
   auto store_tile = [&](const Stage& st, int buf) {
@@ -197,6 +205,7 @@ __global__ void __launch_bounds__(kThreads) radius_attn_kernel(Params p) {
     store_tile(sa, 0);
     mw0 = (sa.mok & 1u) ? sa.m0 : 0u;
     mw1 = (sa.mok & 2u) ? sa.m1 : 0u;
+    seen |= mw0 | mw1;
     __syncthreads();
   }
   auto step = [&](int it, Stage& freed, const Stage& next) {
@@ -283,6 +292,7 @@ __global__ void __launch_bounds__(kThreads) radius_attn_kernel(Params p) {
     __syncthreads();
     mw0 = (next.mok & 1u) ? next.m0 : 0u;
     mw1 = (next.mok & 2u) ? next.m1 : 0u;
+    if (it + 1 < ntiles) seen |= mw0 | mw1;
   };
   for (int it = 0; it < ntiles; it += 2) {
     step(it, sa, sb);
@@ -301,7 +311,7 @@ __global__ void __launch_bounds__(kThreads) radius_attn_kernel(Params p) {
     const int d0 = 16 * nd + 4 * g;
     float o[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) o[r] = acc[nd][r] * inv;
+    for (int r = 0; r < 4; ++r) o[r] = seen ? acc[nd][r] * inv : 0.0f;  // a NaN query without a key too
     if (p.out) {
       Op4 ov;
 #pragma unroll
@@ -455,9 +465,14 @@ __global__ void __launch_bounds__(kThreads2, 3 - QW) radius_attn_pair_kernel(Par
     uint32_t m0[QW], m1[QW];  // mask words as loaded
     uint32_t mok[QW];         // bit 0 / 1: m0 / m1 are real words of a real query
     int key0;                 // first key of the tile
-    bool full;                // every key of the tile is < N (uniform)
+    bool full;                // every key of the tile is < N and attended by a query of the workgroup (uniform)
+    uint64_t set;             // the attended ones
   };
+  const int row0 = qt * QW;  // first 64-query block row of the workgroup
+  const uint64_t* kany = p.key_any ? p.key_any + (size_t(b) * p.NB + row0) * p.NB : nullptr;
+  const bool second = QW == 2 && row0 + 1 < p.NB;
   auto load_tile = [&](int jt, Stage& st) {
+    st.set = kany ? kany[jt] | (second ? kany[p.NB + jt] : 0) : ~uint64_t(0);
     // the words are selected when used (a step later), so that nothing
     // waits for these loads now
     const int w0 = 2 * jt;
@@ -469,7 +484,7 @@ __global__ void __launch_bounds__(kThreads2, 3 - QW) radius_attn_pair_kernel(Par
     }
     const int key0 = jt * kTile;
     st.key0 = key0;
-    st.full = key0 + kTile <= N;
+    st.full = key0 + kTile <= N && st.set == ~uint64_t(0);
     const T* kb = gk + size_t(key0) * D;
     const T* vb = gv + size_t(key0) * D;
     if (st.full) {
@@ -501,7 +516,7 @@ __global__ void __launch_bounds__(kThreads2, 3 - QW) radius_attn_pair_kernel(Par
 #pragma unroll
       for (int t = 0; t < CPT; ++t) {
         Op8 kz = st.k[t], vz = st.v[t];
-        if (st.key0 + krow[t] >= N) {
+        if (st.key0 + krow[t] >= N || !((st.set >> krow[t]) & 1u)) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) kz[e] = vz[e] = T(0.0f);
         }
@@ -515,14 +530,15 @@ __global__ void __launch_bounds__(kThreads2, 3 - QW) radius_attn_pair_kernel(Par
   // the loads of step s + 1 (issued after the previous step's store) and
   // goes to the other buffer at the end of the step.
   Stage st;
-  uint32_t mw0[QW], mw1[QW];
+  uint32_t mw0[QW], mw1[QW], seen[QW];  // seen: the query has a key in this stream
 #pragma unroll
-  for (int t = 0; t < QW; ++t) mw0[t] = mw1[t] = 0u;
+  for (int t = 0; t < QW; ++t) mw0[t] = mw1[t] = seen[t] = 0u;
   auto take_words = [&](const Stage& x) {
 #pragma unroll
     for (int t = 0; t < QW; ++t) {
       mw0[t] = (x.mok[t] & 1u) ? x.m0[t] : 0u;
       mw1[t] = (x.mok[t] & 2u) ? x.m1[t] : 0u;
+      seen[t] |= mw0[t] | mw1[t];
     }
   };
   if (0 < ntiles) {
@@ -677,6 +693,12 @@ __global__ void __launch_bounds__(kThreads2, 3 - QW) radius_attn_pair_kernel(Par
       l[t] += __shfl_xor(l[t], 16, 64);
       l[t] += __shfl_xor(l[t], 32, 64);
     }
+    if (!seen[t]) {  // nothing from this stream, whatever the query holds
+      m[t] = -INFINITY;
+      l[t] = 0.0f;
+#pragma unroll
+      for (int nd = 0; nd < ND; ++nd) acc[t][nd] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
+    }
   }
   // (after the last barrier: the K tiles are no longer read)
   mf_f32x4* cmb_o = reinterpret_cast<mf_f32x4*>(&Ks[0][0][0]);  // [QW][ND][4 query groups x 64 lanes]
@@ -784,7 +806,7 @@ extern "C" int mf_radius_attn(const mf_radius_attn_args* a, void* stream) {
   const long long units = (long long)a->batch * a->heads * nb;
   if (units > 0x7fffffffLL - 8) return fail(MF_ERR_UNSUPPORTED, "mf_radius_attn: batch * heads * tiles too large");
   rattn::Params p{a->q, a->k, a->v, a->mask_bits, a->block_mask, a->out, a->out_f32, a->lse,
-                  a->scale * kLog2e, a->batch, a->heads, a->atoms, (a->atoms + 31) / 32, nb, int(units)};
+                  a->scale * kLog2e, a->batch, a->heads, a->atoms, (a->atoms + 31) / 32, nb, int(units), a->key_any};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (a->dtype == MF_DTYPE_BF16) return rattn::dispatch_dim<__bf16>(p, a->head_dim, s);
   return rattn::dispatch_dim<_Float16>(p, a->head_dim, s);

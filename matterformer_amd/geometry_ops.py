@@ -29,6 +29,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from matterformer_amd import _native
 
@@ -224,15 +225,115 @@ def radius_mask(coords: torch.Tensor, cutoff: float, *, gram: torch.Tensor | Non
     return bits, blocks
 
 
+class RadiusTables:
+    """What the gradients of radius_attention read of a mask, and its forward may: the transposed bits and, for every
+    64 x 64 tile, which keys are attended and which queries attend (radius_tables).  One serves every layer that uses
+    the mask."""
+
+    def __init__(self, bits_t: torch.Tensor, key_any: torch.Tensor, query_any: torch.Tensor) -> None:
+        self.bits_t = bits_t
+        self.key_any = key_any
+        self.query_any = query_any
+
+
+def radius_tables(mask_bits: torch.Tensor, block_mask: torch.Tensor | None = None) -> RadiusTables:
+    """The tables of a neighbour mask (mask_bits int32 (B, N, ceil(N/32)), block_mask uint8 (B, NB, NB) for block 64
+    or None), in one launch."""
+    if mask_bits.ndim != 3 or mask_bits.dtype != torch.int32 or mask_bits.shape[2] != (mask_bits.shape[1] + 31) // 32:
+        raise ValueError(f"mask_bits must be int32 of shape (B, N, ceil(N/32)), got {mask_bits.dtype} "
+                         f"{tuple(mask_bits.shape)}")
+    B, N, W = mask_bits.shape
+    NB = (N + MASK_BLOCK - 1) // MASK_BLOCK
+    if block_mask is not None and block_mask.shape != (B, NB, NB):
+        raise ValueError(f"block_mask must have shape ({B}, {NB}, {NB}) (block {MASK_BLOCK})")
+    dev = _require_device(mask_bits, block_mask)
+    bits = mask_bits.contiguous()
+    bm = None if block_mask is None else block_mask.to(torch.uint8).contiguous()
+    tables = RadiusTables(torch.empty(B, N, W, dtype=torch.int32, device=dev),
+                          *(torch.empty(B, NB, NB, dtype=torch.int64, device=dev) for _ in range(2)))
+    if B * N > 0:
+        args = _native.MfRadiusTablesArgs(
+            mask_bits=bits.data_ptr(), block_mask=_native.ptr(bm), mask_bits_t=tables.bits_t.data_ptr(),
+            key_any=tables.key_any.data_ptr(), query_any=tables.query_any.data_ptr(), batch=B, atoms=N)
+        with torch.cuda.device(dev):
+            _native.check(_native.lib().mf_radius_tables(args, _native.current_stream(dev)), "mf_radius_tables")
+    return tables
+
+
+def _radius_forward(q, k, v, bits, bm, tables, scale, *, lse: bool, fp32: bool):
+    """out, lse and the fp32 output (None where not asked) of contiguous operands."""
+    B, H, N, D = q.shape
+    out = torch.empty_like(q)
+    out32 = torch.empty(B, H, N, D, dtype=torch.float32, device=q.device) if fp32 else None
+    lse_out = torch.empty(B, H, N, dtype=torch.float32, device=q.device) if lse else None
+    args = _native.MfRadiusAttnArgs(
+        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), mask_bits=bits.data_ptr(), block_mask=_native.ptr(bm),
+        out=out.data_ptr(), out_f32=_native.ptr(out32), lse=_native.ptr(lse_out), scale=scale, batch=B, heads=H,
+        atoms=N, head_dim=D, dtype=_native.dtype_code(q.dtype),
+        key_any=None if tables is None else tables.key_any.data_ptr())
+    with torch.cuda.device(q.device):
+        _native.check(_native.lib().mf_radius_attn(args, _native.current_stream(q.device)), "mf_radius_attn")
+    return out, lse_out, out32
+
+
+class _RadiusAttentionFunction(torch.autograd.Function):
+    """mf_radius_attn with mf_radius_attn_bwd: differentiable in q, k and v through out and lse."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, bits, bm, tables, scale, fp32):
+        out, lse, out32 = _radius_forward(q, k, v, bits, bm, tables, scale, lse=True, fp32=fp32)
+        ctx.save_for_backward(q, k, v, bits, out, lse)
+        ctx.tables, ctx.scale = tables, scale
+        ctx.set_materialize_grads(False)
+        if out32 is not None:
+            ctx.mark_non_differentiable(out32)
+        return out, lse, out32
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out, grad_lse, _):
+        q, k, v, bits, out, lse = ctx.saved_tensors
+        if grad_out is None and grad_lse is None:
+            return (None,) * 8
+        B, H, N, D = q.shape
+        go = torch.zeros_like(out) if grad_out is None else grad_out.contiguous()
+        if go.data_ptr() % 16 != 0:
+            go = go.clone()
+        gl = None if grad_lse is None else grad_lse.contiguous()
+        grads = [torch.empty_like(t) for t in (q, k, v)]
+        if q.numel() > 0:
+            t = ctx.tables
+            lib = _native.lib()
+            nbytes = int(lib.mf_radius_attn_bwd_workspace_size(B, H, N, _native.dtype_code(q.dtype)))
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+            args = _native.MfRadiusAttnBwdArgs(
+                q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), lse=lse.data_ptr(),
+                grad_out=go.data_ptr(), grad_lse=_native.ptr(gl), mask_bits=bits.data_ptr(),
+                mask_bits_t=t.bits_t.data_ptr(), key_any=t.key_any.data_ptr(), query_any=t.query_any.data_ptr(),
+                dq=grads[0].data_ptr(), dk=grads[1].data_ptr(), dv=grads[2].data_ptr(),
+                workspace=workspace.data_ptr(), workspace_bytes=nbytes, scale=ctx.scale, batch=B, heads=H, atoms=N,
+                head_dim=D, dtype=_native.dtype_code(q.dtype))
+            with torch.cuda.device(q.device):
+                _native.check(lib.mf_radius_attn_bwd(args, _native.current_stream(q.device)), "mf_radius_attn_bwd")
+        return (*grads, None, None, None, None, None)
+
+
 def radius_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bits: torch.Tensor,
                      block_mask: torch.Tensor | None = None, *, scale: float | None = None,
-                     return_lse: bool = False, return_fp32: bool = False):
+                     return_lse: bool = False, return_fp32: bool = False, tables: RadiusTables | None = None):
     """softmax_j(scale q_i . k_j over the neighbours j of i) v_j.
 
     q, k, v (B, H, N, D) bf16/fp16 with D in {32, 64, 128}; mask_bits from
     radius_mask; block_mask from radius_mask with block=64 (or None: every
     tile is visited).  Rows without a neighbour are 0 (lse 0).  Returns out in
     q's dtype, plus lse (B, H, N) fp32 and/or the fp32 output when asked.
+
+    Differentiable in q, k and v through out and lse (mf_radius_attn_bwd, the
+    same tiles; rows without a neighbour get zeros); the fp32 output takes no
+    gradient.  ``tables`` = radius_tables of the same masks: a call that takes
+    gradients makes its own otherwise.  With tables, and so in every such call,
+    atoms that are nobody's neighbour may hold anything (NaN); without, their
+    k and v must be finite.
     """
     if q.ndim != 4 or k.shape != q.shape or v.shape != q.shape:
         raise ValueError("q, k, v must share the shape (B, H, N, D)")
@@ -251,18 +352,19 @@ def radius_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bit
     qc, kc, vc = q.contiguous(), k.contiguous(), v.contiguous()
     bits = mask_bits.contiguous()
     bm = None if block_mask is None else block_mask.to(torch.uint8).contiguous()
-    out = torch.empty_like(qc)
-    out32 = torch.empty(B, H, N, D, dtype=torch.float32, device=dev) if return_fp32 else None
-    lse = torch.empty(B, H, N, dtype=torch.float32, device=dev) if return_lse else None
     s = float(D ** -0.5 if scale is None else scale)
     if not math.isfinite(s):
         raise ValueError("scale must be finite")
-    args = _native.MfRadiusAttnArgs(
-        q=qc.data_ptr(), k=kc.data_ptr(), v=vc.data_ptr(), mask_bits=bits.data_ptr(), block_mask=_native.ptr(bm),
-        out=out.data_ptr(), out_f32=_native.ptr(out32), lse=_native.ptr(lse), scale=s, batch=B, heads=H, atoms=N,
-        head_dim=D, dtype=_native.dtype_code(q.dtype))
-    with torch.cuda.device(dev):
-        _native.check(_native.lib().mf_radius_attn(args, _native.current_stream(dev)), "mf_radius_attn")
+    if tables is not None:
+        if tables.bits_t.shape != bits.shape or tables.key_any.shape != (B, NB, NB):
+            raise ValueError("tables must be radius_tables of this call's masks")
+        _require_device(bits, tables.bits_t)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+        if tables is None:
+            tables = radius_tables(bits, bm)
+        out, lse, out32 = _RadiusAttentionFunction.apply(qc, kc, vc, bits, bm, tables, s, return_fp32)
+    else:
+        out, lse, out32 = _radius_forward(qc, kc, vc, bits, bm, tables, s, lse=return_lse, fp32=return_fp32)
     result = (out,)
     if return_lse:
         result += (lse,)
