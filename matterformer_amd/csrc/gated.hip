@@ -28,6 +28,7 @@
 // outer one (W in dx, both in dW) are stored as they lie and read transposed.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "mf_common.h"
 
@@ -52,51 +53,54 @@ __device__ __forceinline__ float sigmoid_(float x) {
 }
 
 // FAST (16-bit outputs): hardware exp2 and reciprocal, one unit in the last place of fp32 each.
-template <bool FAST>
-__device__ __forceinline__ float act_value(int act, float a) {
-  switch (act) {
-    case MF_ACT_GELU: return 0.5f * a * erfcf(-0.70710678118654752f * a);
-    case MF_ACT_GELU_TANH: {
-      // 0.5 (1 + tanh u) = sigmoid(2 u): no cancellation for negative u
-      const float u2 = 1.5957691216057308f * (a + 0.044715f * a * a * a);
-      return a * sigmoid_<FAST>(u2);
-    }
-    case MF_ACT_RELU: return a > 0.0f ? a : (a == a ? 0.0f : a);
-    case MF_ACT_SIGMOID: return sigmoid_<FAST>(a);
-    default: return a * sigmoid_<FAST>(a);
+template <int ACT, bool FAST>
+__device__ __forceinline__ float act_value(float a) {
+  if constexpr (ACT == MF_ACT_GELU) {
+    return 0.5f * a * erfcf(-0.70710678118654752f * a);
+  } else if constexpr (ACT == MF_ACT_GELU_TANH) {
+    // 0.5 (1 + tanh u) = sigmoid(2 u): no cancellation for negative u
+    return a * sigmoid_<FAST>(1.5957691216057308f * (a + 0.044715f * a * a * a));
+  } else if constexpr (ACT == MF_ACT_RELU) {
+    return a > 0.0f ? a : (a == a ? 0.0f : a);
+  } else if constexpr (ACT == MF_ACT_SIGMOID) {
+    return sigmoid_<FAST>(a);
+  } else {
+    return a * sigmoid_<FAST>(a);
   }
 }
-template <bool FAST>
-__device__ __forceinline__ void act_both(int act, float a, float& y, float& dy) {
+template <int ACT, bool FAST>
+__device__ __forceinline__ void act_both(float a, float& y, float& dy) {
+  if constexpr (ACT == MF_ACT_GELU) {
+    const float cdf = 0.5f * erfcf(-0.70710678118654752f * a);
+    y = a * cdf;
+    dy = cdf + a * 0.3989422804014327f * exp_<FAST>(-0.5f * a * a);
+  } else if constexpr (ACT == MF_ACT_GELU_TANH) {
+    const float a2 = a * a;
+    const float u2 = 1.5957691216057308f * (a + 0.044715f * a * a2);
+    const float s = sigmoid_<FAST>(u2), ns = sigmoid_<FAST>(-u2);
+    y = a * s;
+    dy = s + a * s * ns * 1.5957691216057308f * (1.0f + 0.134145f * a2);
+  } else if constexpr (ACT == MF_ACT_RELU) {
+    y = a > 0.0f ? a : (a == a ? 0.0f : a);
+    dy = a > 0.0f ? 1.0f : 0.0f;
+  } else if constexpr (ACT == MF_ACT_SIGMOID) {
+    y = sigmoid_<FAST>(a);
+    dy = y * sigmoid_<FAST>(-a);
+  } else {
+    const float s = sigmoid_<FAST>(a);
+    y = a * s;
+    dy = s * (1.0f + a * sigmoid_<FAST>(-a));
+  }
+}
+// f(integral constant of the activation): one branch around an epilogue instead of one per element
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F&& f) {
   switch (act) {
-    case MF_ACT_GELU: {
-      const float cdf = 0.5f * erfcf(-0.70710678118654752f * a);
-      y = a * cdf;
-      dy = cdf + a * 0.3989422804014327f * exp_<FAST>(-0.5f * a * a);
-      return;
-    }
-    case MF_ACT_GELU_TANH: {
-      const float a2 = a * a;
-      const float u2 = 1.5957691216057308f * (a + 0.044715f * a * a2);
-      const float s = sigmoid_<FAST>(u2), ns = sigmoid_<FAST>(-u2);
-      y = a * s;
-      dy = s + a * s * ns * 1.5957691216057308f * (1.0f + 0.134145f * a2);
-      return;
-    }
-    case MF_ACT_RELU:
-      y = a > 0.0f ? a : (a == a ? 0.0f : a);
-      dy = a > 0.0f ? 1.0f : 0.0f;
-      return;
-    case MF_ACT_SIGMOID:
-      y = sigmoid_<FAST>(a);
-      dy = y * sigmoid_<FAST>(-a);
-      return;
-    default: {
-      const float s = sigmoid_<FAST>(a);
-      y = a * s;
-      dy = s * (1.0f + a * sigmoid_<FAST>(-a));
-      return;
-    }
+    case MF_ACT_GELU: f(std::integral_constant<int, MF_ACT_GELU>()); break;
+    case MF_ACT_GELU_TANH: f(std::integral_constant<int, MF_ACT_GELU_TANH>()); break;
+    case MF_ACT_RELU: f(std::integral_constant<int, MF_ACT_RELU>()); break;
+    case MF_ACT_SIGMOID: f(std::integral_constant<int, MF_ACT_SIGMOID>()); break;
+    default: f(std::integral_constant<int, MF_ACT_SILU>()); break;
   }
 }
 
@@ -274,7 +278,7 @@ __device__ __forceinline__ void load16(const T* p, float (&v)[16], int n, bool v
 // WM waves of 128 rows (two groups of 64: gate and up of the same 64 hidden columns in kFwd and kBwd) by WN waves of
 // 16 NT columns.
 template <typename T, int MODE, int WM, int WN, int NT>
-__global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) gemm_kernel(Params p) {
+__global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
   constexpr int NW = WM * WN;
   constexpr int BM = WM * 128, BN = WN * NT * 16, BK = kBK<T>;
   constexpr bool kGated = MODE == kFwd || MODE == kBwd;
@@ -349,37 +353,63 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) gemm_kernel(Params 
 #pragma unroll
       for (int i = 0; i < NT; ++i) acc[q][j][i] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
 
-  auto multiply = [&](const char* la, const char* lb) {
+  // A K step is two 16-byte pieces of every fragment.  While one piece is multiplied the next is read from LDS into the
+  // other registers; the barrier sits between the two, where the second piece of a tile is in registers, so its buffer
+  // is free for the copy of the tile after next and the next tile has had a whole step to land.
+  struct Frags {
+    Frag a[2][4], b[NT];
+  };
+  auto read = [&](Frags& f, const char* la, const char* lb, int kk) {
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      Frag fb[NT];
+    for (int i = 0; i < NT; ++i) f.b[i] = read_frag<T, kBOut, false, BN>(lb, wn * NT * 16, i, kk, lane);
 #pragma unroll
-      for (int i = 0; i < NT; ++i) fb[i] = read_frag<T, kBOut, false, BN>(lb, wn * NT * 16, i, kk, lane);
+    for (int q = 0; q < 2; ++q) {
+      const int base = kGated ? q * (BM / 2) + wm * 64 : wm * 128 + q * 64;
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int base = kGated ? q * (BM / 2) + wm * 64 : wm * 128 + q * 64;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const Frag fa = read_frag<T, kAOut, true, BM>(la, base, j, kk, lane);
-#pragma unroll
-          for (int i = 0; i < NT; ++i) Mma<T>::run(fa, fb[i], acc[q][j][i]);
-        }
-      }
+      for (int j = 0; j < 4; ++j) f.a[q][j] = read_frag<T, kAOut, true, BM>(la, base, j, kk, lane);
     }
   };
-  auto ready = [] {
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's loads into LDS have landed
-    __syncthreads();
+  auto multiply = [&](const Frags& f) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) Mma<T>::run(f.a[q][j], f.b[i], acc[q][j][i]);
   };
-  if (s0 < s1) load(s0, a0, b0);
-  for (int s = s0; s < s1; s += 2) {
-    ready();
-    if (s + 1 < s1) load(s + 1, a1, b1);
-    multiply(a0, b0);
-    if (s + 1 < s1) {
-      ready();
-      if (s + 2 < s1) load(s + 2, a0, b0);
-      multiply(a1, b1);
+  // the order of the instructions of half a step: reads spread over the products
+  auto interleave = [] {
+    constexpr int kReads = (kAOut ? (sizeof(T) == 2 ? 16 : 32) : 8) + (kBOut ? (sizeof(T) == 2 ? 2 : 4) * NT : NT);
+    constexpr int kMul = 8 * NT * (sizeof(T) == 2 ? 1 : 4);
+    constexpr int kEach = kMul / kReads > 0 ? kMul / kReads : 1;
+#pragma unroll
+    for (int i = 0; i < kReads; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);      // one LDS read
+      __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);  // products
+    }
+  };
+  auto half = [&](Frags& f0, Frags& f1, const char* ca, const char* cb, int s, char* fa, char* fb, const char* na,
+                  const char* nb) {
+    read(f1, ca, cb, 1);
+    multiply(f0);
+    interleave();
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) and lgkmcnt(0): the next tile has landed, this one is read
+    __syncthreads();
+    if (s + 2 < s1) load(s + 2, fa, fb);
+    read(f0, na, nb, 0);  // after the last step: stale, not used
+    multiply(f1);
+    interleave();
+  };
+  if (s0 < s1) {
+    Frags f0, f1;
+    load(s0, a0, b0);
+    if (s0 + 1 < s1) load(s0 + 1, a1, b1);
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    __syncthreads();
+    read(f0, a0, b0, 0);
+    for (int s = s0; s < s1; s += 2) {
+      half(f0, f1, a0, b0, s, a0, b0, a1, b1);
+      if (s + 1 < s1) half(f0, f1, a1, b1, s + 1, a1, b1, a0, b0);
     }
   }
 
@@ -403,43 +433,47 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) gemm_kernel(Params 
       }
     }
     if constexpr (MODE == kFwd) {
+      with_activation(p.act, [&](auto act) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const int n = n0 + (wn * NT + i) * 16 + r16;
-        float h[16];
+        for (int i = 0; i < NT; ++i) {
+          const int n = n0 + (wn * NT + i) * 16 + r16;
+          float h[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float a = acc[0][e >> 2][i][e & 3] + ba[e], b = acc[1][e >> 2][i][e & 3] + bb[e];
-          h[e] = act_value<kFast>(p.act, a) * b;
+          for (int e = 0; e < 16; ++e) {
+            const float a = acc[0][e >> 2][i][e & 3] + ba[e], b = acc[1][e >> 2][i][e & 3] + bb[e];
+            h[e] = act_value<decltype(act)::value, kFast>(a) * b;
+          }
+          if (n < p.N) store16(static_cast<T*>(p.out) + int64_t(n) * p.ldo + f0, h, left, p.vec);
         }
-        if (n < p.N) store16(static_cast<T*>(p.out) + int64_t(n) * p.ldo + f0, h, left, p.vec);
-      }
+      });
     } else {
       float sa[16], sb[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) sa[e] = sb[e] = 0.0f;
+      with_activation(p.act, [&](auto act) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const int n = n0 + (wn * NT + i) * 16 + r16;
-        float go[16], da[16], db[16];
-        if (n < p.N) load16(static_cast<const T*>(p.go) + int64_t(n) * p.F + f0, go, left, p.vec);
+        for (int i = 0; i < NT; ++i) {
+          const int n = n0 + (wn * NT + i) * 16 + r16;
+          float go[16], da[16], db[16];
+          if (n < p.N) load16(static_cast<const T*>(p.go) + int64_t(n) * p.F + f0, go, left, p.vec);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float a = acc[0][e >> 2][i][e & 3] + ba[e], b = acc[1][e >> 2][i][e & 3] + bb[e];
-          float y, dy;
-          act_both<kFast>(p.act, a, y, dy);
-          const bool in = n < p.N && e < left;  // columns past F are zero, whatever x holds
-          da[e] = in ? go[e] * b * dy : 0.0f;
-          db[e] = in ? go[e] * y : 0.0f;
-          sa[e] += da[e];
-          sb[e] += db[e];
+          for (int e = 0; e < 16; ++e) {
+            const float a = acc[0][e >> 2][i][e & 3] + ba[e], b = acc[1][e >> 2][i][e & 3] + bb[e];
+            float y, dy;
+            act_both<decltype(act)::value, kFast>(a, y, dy);
+            const bool in = n < p.N && e < left;  // columns past F are zero, whatever x holds
+            da[e] = in ? go[e] * b * dy : 0.0f;
+            db[e] = in ? go[e] * y : 0.0f;
+            sa[e] += da[e];
+            sb[e] += db[e];
+          }
+          if (n < p.N && f0 < p.Fp) {
+            T* o = static_cast<T*>(p.out) + int64_t(n) * p.ldo + f0;
+            store16(o, da, 16, true);
+            store16(o + p.Fp, db, 16, true);
+          }
         }
-        if (n < p.N && f0 < p.Fp) {
-          T* o = static_cast<T*>(p.out) + int64_t(n) * p.ldo + f0;
-          store16(o, da, 16, true);
-          store16(o + p.Fp, db, 16, true);
-        }
-      }
+      });
       if (p.part) {
         float* row = p.part + int64_t(tn * WN + wn) * 2 * p.Fp + f0;
 #pragma unroll
@@ -535,8 +569,10 @@ struct Plan {
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Tiles of 256 x 256 when they are enough to give every CU one, else of 128 x 128.
-bool large_tiles(int64_t m, int64_t n, int num_cus) {
+// Tiles of 256 x 256 when they are enough to give every CU one, else of 128 x 128; fp32, whose matrix rate is a
+// sixteenth, always the latter.
+bool large_tiles(int64_t m, int64_t n, int num_cus, int esize) {
+  if (esize == 4) return false;
   return ((m + 255) / 256) * ((n + 255) / 256) >= num_cus;
 }
 
@@ -566,8 +602,8 @@ void make_plan(Plan* q, int64_t T, int64_t C, int64_t F, int64_t x_stride, const
   // bias sums of every column wave: 128-row tiles have 4 waves of 32, 256-row tiles 4 of 64
   q->bias_bytes = need_db ? round256(size_t((T + 127) / 128) * 4 * 2 * q->Fp * 4) : 0;
   const int bk = 128 / q->esize;
-  q->dx_splits = k_splits(q->Cp, T, 2 * q->Fp, bk, large_tiles(q->Cp, T, num_cus), num_cus);
-  q->dw_splits = k_splits(q->Cp, 2 * q->Fp, T, bk, large_tiles(q->Cp, 2 * q->Fp, num_cus), num_cus);
+  q->dx_splits = k_splits(q->Cp, T, 2 * q->Fp, bk, large_tiles(q->Cp, T, num_cus, q->esize), num_cus);
+  q->dw_splits = k_splits(q->Cp, 2 * q->Fp, T, bk, large_tiles(q->Cp, 2 * q->Fp, num_cus, q->esize), num_cus);
   q->dx_bytes = need_dx && q->dx_splits > 1 ? round256(size_t(q->dx_splits) * T * q->Cp * 4) : 0;
   q->dw_bytes = need_dw && q->dw_splits > 1 ? round256(size_t(q->dw_splits) * 2 * F * q->Cp * 4) : 0;
 }
@@ -583,8 +619,13 @@ void launch_gemm(Params p, bool large, hipStream_t s) {
   p.steps = (steps + p.splits - 1) / p.splits;
   const int64_t total = int64_t(p.mt) * p.nt * p.splits;
   const dim3 grid(unsigned((total + 7) / 8 * 8));
-  if (large) hipLaunchKernelGGL((gemm_kernel<T, MODE, 2, 4, 4>), grid, dim3(512), 0, s, p);
-  else hipLaunchKernelGGL((gemm_kernel<T, MODE, 1, 4, 2>), grid, dim3(256), 0, s, p);
+  if constexpr (sizeof(T) == 2) {
+    if (large) {
+      hipLaunchKernelGGL((gemm_kernel<T, MODE, 2, 4, 4>), grid, dim3(512), 0, s, p);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((gemm_kernel<T, MODE, 1, 4, 2>), grid, dim3(256), 0, s, p);
 }
 
 template <typename T>
@@ -634,7 +675,7 @@ int forward(const mf_gated_linear_args* a, const Plan& q, int num_cus, hipStream
   p.ldo = q.F;
   p.bias = a->bias;
   p.vec = q.F * q.esize % 16 == 0 && aligned16(a->out);
-  launch_gemm<T, kFwd>(p, large_tiles(2 * q.F, q.T, num_cus), s);
+  launch_gemm<T, kFwd>(p, large_tiles(2 * q.F, q.T, num_cus, q.esize), s);
   MF_HIP_CHECK(hipGetLastError());
   return MF_OK;
 }
@@ -650,7 +691,7 @@ int backward(const mf_gated_linear_bwd_args* a, const Plan& q, int num_cus, hipS
   ws += round256(size_t(q.T) * 2 * q.Fp * sizeof(T));
   float* sums = a->dbias ? reinterpret_cast<float*>(ws) : nullptr;
   ws += q.bias_bytes;
-  const bool big = large_tiles(2 * q.F, q.T, num_cus);
+  const bool big = large_tiles(2 * q.F, q.T, num_cus, q.esize);
   p.M = int(q.F);
   p.N = int(q.T);
   p.K = int(q.Cp);
@@ -683,7 +724,7 @@ int backward(const mf_gated_linear_bwd_args* a, const Plan& q, int num_cus, hipS
     d.splits = q.dx_splits;
     d.part = reinterpret_cast<float*>(ws);
     d.vec = q.C * q.esize % 16 == 0 && aligned16(a->dx);
-    launch_gemm<T, kDx>(d, large_tiles(q.Cp, q.T, num_cus), s);
+    launch_gemm<T, kDx>(d, large_tiles(q.Cp, q.T, num_cus, q.esize), s);
     MF_HIP_CHECK(hipGetLastError());
     if (d.splits > 1) {
       hipLaunchKernelGGL(sum_kernel<T>, dim3(unsigned((q.T * q.C + 255) / 256)), dim3(256), 0, s, d.part,
@@ -706,7 +747,7 @@ int backward(const mf_gated_linear_bwd_args* a, const Plan& q, int num_cus, hipS
     d.splits = q.dw_splits;
     d.part = reinterpret_cast<float*>(ws);
     d.vec = q.C * q.esize % 16 == 0 && aligned16(a->dweight);
-    launch_gemm<T, kDw>(d, large_tiles(q.Cp, 2 * q.Fp, num_cus), s);
+    launch_gemm<T, kDw>(d, large_tiles(q.Cp, 2 * q.Fp, num_cus, q.esize), s);
     MF_HIP_CHECK(hipGetLastError());
     if (d.splits > 1) {
       hipLaunchKernelGGL(sum_kernel<T>, dim3(unsigned((2 * q.F * q.C + 255) / 256)), dim3(256), 0, s, d.part,
