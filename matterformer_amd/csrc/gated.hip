@@ -230,10 +230,13 @@ struct Params {
   int M, N, K;        // output columns (kFwd, kBwd: F), output rows (kDw: 2 Fp), K extent
   int F, Fp;          // hidden width, and its multiple of 64 that [dA dB] is laid out by
   int act;
-  int mt, nt, splits, steps;  // tiles along M and N, K splits, K steps of one split
+  int mt, nt;         // tiles along M and N
+  int full, tail;     // tiles computed whole, and tiles after them whose K is split
+  int splits, steps;  // K splits of a tail tile, K steps of one
   void* out;          // h, [dA dB], dx or dW
   int64_t ldo;        // elements between its rows
-  float* part;        // kDx, kDw with splits > 1: fp32 [splits][N][M]; kBwd: bias sums [column tiles' waves][2 Fp]
+  float* part;        // kDx, kDw: sums of the tail tiles' splits, fp32 [tail][splits][BN][BM]; kBwd: bias sums
+                      // [column tiles' waves][2 Fp]
   const void* bias;   // [2F] or null
   const void* go;     // kBwd: [N, F]
   int vec;            // rows of out (and go) are 16-byte aligned
@@ -275,6 +278,27 @@ __device__ __forceinline__ void load16(const T* p, float (&v)[16], int n, bool v
   }
 }
 
+// Row n of the product as a row of the output: kDw's run over [dA dB]'s columns, each half padded to Fp.
+template <int MODE>
+__device__ __forceinline__ bool out_row(const Params& p, int& n) {
+  if (n >= p.N) return false;
+  if constexpr (MODE == kDw) {
+    const int f = n >= p.Fp ? n - p.Fp : n;
+    n = n >= p.Fp ? p.F + f : f;
+    return f < p.F;
+  }
+  return true;
+}
+
+// Tile t of the walk: groups of 8 column tiles, so that the tiles resident together share rows of both operands.
+__device__ __forceinline__ void tile_of(const Params& p, int t, int& tm, int& tn) {
+  const int group = t / (8 * p.mt);
+  t -= group * 8 * p.mt;
+  const int gn = min(8, p.nt - group * 8);
+  tm = t / gn;
+  tn = group * 8 + (t - tm * gn);
+}
+
 // WM waves of 128 rows (two groups of 64: gate and up of the same 64 hidden columns in kFwd and kBwd) by WN waves of
 // 16 NT columns.
 template <typename T, int MODE, int WM, int WN, int NT>
@@ -294,18 +318,23 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
   __shared__ __attribute__((aligned(1024))) char a1[TileA::kBytes];
   __shared__ __attribute__((aligned(1024))) char b1[TileB::kBytes];
 
-  // XCD-aware order: blockIdx.x % 8 is the XCD; each gets a contiguous range of tiles, walked in groups of 8 column
-  // tiles so that the tiles resident together share rows of both operands
-  const int total = p.mt * p.nt * p.splits;
-  const int per = (total + 7) >> 3;
-  const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if ((blockIdx.x >> 3) >= per || id >= total) return;
-  const int split = id / (p.mt * p.nt);
-  int t = id - split * p.mt * p.nt;
-  const int group = t / (8 * p.mt);
-  t -= group * 8 * p.mt;
-  const int gn = min(8, p.nt - group * 8);
-  const int tm = t / gn, tn = group * 8 + (t - tm * gn);
+  // XCD-aware order: blockIdx.x % 8 is the XCD; each gets a contiguous range of the whole tiles, then of the tail's
+  // splits
+  const int xcd = blockIdx.x & 7, turn = blockIdx.x >> 3;
+  const int full_per = (p.full + 7) >> 3, tail_per = (p.tail * p.splits + 7) >> 3;
+  int t, split = 0;
+  const bool whole = turn < full_per;
+  if (whole) {
+    t = xcd * full_per + turn;
+    if (t >= p.full) return;
+  } else {
+    const int k = xcd * tail_per + turn - full_per;
+    if (turn - full_per >= tail_per || k >= p.tail * p.splits) return;
+    t = p.full + k / p.splits;
+    split = k % p.splits;
+  }
+  int tm, tn;
+  tile_of(p, t, tm, tn);
   const int m0 = tm * TM, n0 = tn * BN;
 
   const int lane = threadIdx.x & 63;
@@ -326,7 +355,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
   pb += kBOut ? int64_t(n0) * sizeof(T) : int64_t(n0) * p.ldb;
 
   const int steps_all = (p.K + BK - 1) / BK;
-  const int s0 = split * p.steps, s1 = min(steps_all, s0 + p.steps);
+  const int s0 = split * p.steps, s1 = whole ? steps_all : min(steps_all, s0 + p.steps);
   auto load = [&](int s, char* la, char* lb) {
     const int k0 = s * BK;
     const int left = p.K - k0;
@@ -345,13 +374,30 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
     tb.load(xb, left, lb, wave);
   };
 
+  if (s0 < s1) load(s0, a0, b0);
+  if (s0 + 1 < s1) load(s0 + 1, a1, b1);
+
+  // lane (g, r16) holds, for column n0 + .. + 16 i + r16 of the tile, group rows 16 g .. 16 g + 15; the bias is the
+  // sums' start
+  const int g = lane >> 4, r16 = lane & 15;
   mf_f32x4 acc[2][4][NT];
 #pragma unroll
   for (int q = 0; q < 2; ++q)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 4; ++j) {
+      mf_f32x4 start = {0.f, 0.f, 0.f, 0.f};
+      if constexpr (kGated) {
+        if (p.bias) {
+          const int f = m0 + wm * 64 + 16 * g + 4 * j;
+          const T* bias = static_cast<const T*>(p.bias) + q * p.F + f;
 #pragma unroll
-      for (int i = 0; i < NT; ++i) acc[q][j][i] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int r = 0; r < 4; ++r)
+            if (f + r < p.F) start[r] = Elem<T>::to_f32(bias[r]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NT; ++i) acc[q][j][i] = start;
+    }
 
   // A K step is two 16-byte pieces of every fragment.  While one piece is multiplied the next is read from LDS into the
   // other registers; the barrier sits between the two, where the second piece of a tile is in registers, so its buffer
@@ -402,8 +448,6 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
   };
   if (s0 < s1) {
     Frags f0, f1;
-    load(s0, a0, b0);
-    if (s0 + 1 < s1) load(s0 + 1, a1, b1);
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
     __syncthreads();
     read(f0, a0, b0, 0);
@@ -413,25 +457,10 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
     }
   }
 
-  // lane (g, r16) holds, for column n0 + .. + 16 i + r16 of the tile, group rows 16 g .. 16 g + 15
-  const int g = lane >> 4, r16 = lane & 15;
   constexpr bool kFast = sizeof(T) == 2;
   if constexpr (kGated) {
     const int f0 = m0 + wm * 64 + 16 * g;
     const int left = p.F - f0;
-    float ba[16], bb[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) ba[e] = bb[e] = 0.0f;
-    if (p.bias) {
-      const T* bias = static_cast<const T*>(p.bias);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        if (e < left) {
-          ba[e] = Elem<T>::to_f32(bias[f0 + e]);
-          bb[e] = Elem<T>::to_f32(bias[p.F + f0 + e]);
-        }
-      }
-    }
     if constexpr (MODE == kFwd) {
       with_activation(p.act, [&](auto act) {
 #pragma unroll
@@ -439,17 +468,13 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
           const int n = n0 + (wn * NT + i) * 16 + r16;
           float h[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float a = acc[0][e >> 2][i][e & 3] + ba[e], b = acc[1][e >> 2][i][e & 3] + bb[e];
-            h[e] = act_value<decltype(act)::value, kFast>(a) * b;
-          }
+          for (int e = 0; e < 16; ++e)
+            h[e] = act_value<decltype(act)::value, kFast>(acc[0][e >> 2][i][e & 3]) * acc[1][e >> 2][i][e & 3];
           if (n < p.N) store16(static_cast<T*>(p.out) + int64_t(n) * p.ldo + f0, h, left, p.vec);
         }
       });
     } else {
-      float sa[16], sb[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) sa[e] = sb[e] = 0.0f;
+      // dA and dB take the place of a and b
       with_activation(p.act, [&](auto act) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
@@ -458,14 +483,13 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
           if (n < p.N) load16(static_cast<const T*>(p.go) + int64_t(n) * p.F + f0, go, left, p.vec);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const float a = acc[0][e >> 2][i][e & 3] + ba[e], b = acc[1][e >> 2][i][e & 3] + bb[e];
             float y, dy;
-            act_both<decltype(act)::value, kFast>(a, y, dy);
+            act_both<decltype(act)::value, kFast>(acc[0][e >> 2][i][e & 3], y, dy);
             const bool in = n < p.N && e < left;  // columns past F are zero, whatever x holds
-            da[e] = in ? go[e] * b * dy : 0.0f;
+            da[e] = in ? go[e] * acc[1][e >> 2][i][e & 3] * dy : 0.0f;
             db[e] = in ? go[e] * y : 0.0f;
-            sa[e] += da[e];
-            sb[e] += db[e];
+            acc[0][e >> 2][i][e & 3] = da[e];
+            acc[1][e >> 2][i][e & 3] = db[e];
           }
           if (n < p.N && f0 < p.Fp) {
             T* o = static_cast<T*>(p.out) + int64_t(n) * p.ldo + f0;
@@ -477,56 +501,70 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
       if (p.part) {
         float* row = p.part + int64_t(tn * WN + wn) * 2 * p.Fp + f0;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          sa[e] = group16_sum(sa[e]);
-          sb[e] = group16_sum(sb[e]);
-        }
-        if (r16 == 0 && f0 < p.Fp) {
-          store16(row, sa, 16, true);
-          store16(row + p.Fp, sb, 16, true);
+        for (int q = 0; q < 2; ++q) {
+          float sum[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float v = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) v += acc[q][e >> 2][i][e & 3];
+            sum[e] = group16_sum(v);
+          }
+          if (r16 == 0 && f0 < p.Fp) store16(row + q * p.Fp, sum, 16, true);
         }
       }
     }
   } else {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const int m = m0 + wm * 128 + q * 64 + 16 * g;
+      const int ml = wm * 128 + q * 64 + 16 * g;
+      const int m = m0 + ml;
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        int n = n0 + (wn * NT + i) * 16 + r16;
+        const int nl = (wn * NT + i) * 16 + r16;
+        int n = n0 + nl;
         float v[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = acc[q][e >> 2][i][e & 3];
-        bool in = n < p.N;
-        if constexpr (MODE == kDw) {
-          const int f = n >= p.Fp ? n - p.Fp : n;
-          in = in && f < p.F;
-          n = n >= p.Fp ? p.F + f : f;
-        }
-        if (!in || m >= p.M) continue;
-        if (p.splits > 1) {
-          const int64_t rows = MODE == kDw ? 2 * p.F : p.N;
-          store16(p.part + (split * rows + n) * int64_t(p.M) + m, v, p.M - m, true);
-        } else {
-          store16(static_cast<T*>(p.out) + int64_t(n) * p.ldo + m, v, min(p.M, int(p.ldo)) - m, p.vec);
+        if (!whole) {
+          store16(p.part + ((int64_t(t - p.full) * p.splits + split) * BN + nl) * BM + ml, v, 16, true);
+        } else if (out_row<MODE>(p, n) && m < p.ldo) {
+          store16(static_cast<T*>(p.out) + int64_t(n) * p.ldo + m, v, int(p.ldo) - m, p.vec);
         }
       }
     }
   }
 }
 
-// out[i] = sum over splits of part[s][i], in order; `cols` of every `ld` columns are kept.
-template <typename T>
-__global__ void __launch_bounds__(256) sum_kernel(const float* part, T* out, int splits, int64_t rows, int ld, int cols) {
-  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t n = rows * cols;
-  if (i >= n) return;
-  const int64_t r = i / cols;
-  const float* src = part + r * ld + (i - r * cols);
-  const int64_t plane = rows * ld;
-  float v = 0.0f;
-  for (int s = 0; s < splits; ++s) v += src[s * plane];
-  out[i] = Elem<T>::from_f32(v);
+// The tail tiles' outputs: each the sum of its splits, in order.  Four columns a thread.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(256) tail_kernel(Params p, int bm, int bn) {
+  const int cols = bm / 4;
+  const int rows_block = 256 / cols;
+  const int blocks_tile = bn / rows_block;
+  const int tile = blockIdx.x / blocks_tile;
+  const int nl = (blockIdx.x - tile * blocks_tile) * rows_block + threadIdx.x / cols;
+  const int ml = (threadIdx.x % cols) * 4;
+  int tm, tn;
+  tile_of(p, p.full + tile, tm, tn);
+  int n = tn * bn + nl;
+  const int m = tm * bm + ml;
+  if (!out_row<MODE>(p, n) || m >= p.ldo) return;
+  const float* src = p.part + (int64_t(tile) * p.splits * bn + nl) * bm + ml;
+  mf_f32x4 v = *reinterpret_cast<const mf_f32x4*>(src);
+  for (int s = 1; s < p.splits; ++s) v += *reinterpret_cast<const mf_f32x4*>(src + int64_t(s) * bn * bm);
+  T* out = static_cast<T*>(p.out) + int64_t(n) * p.ldo + m;
+  if (p.vec) {
+    typedef T V __attribute__((ext_vector_type(4)));
+    V o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = Elem<T>::from_f32(v[e]);
+    *reinterpret_cast<V*>(out) = o;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (m + e < p.ldo) out[e] = Elem<T>::from_f32(v[e]);
+  }
 }
 
 // dbias: column sums of `rows` partial rows of [2 Fp], one wave per 16 columns, four row strands each.
@@ -559,31 +597,58 @@ __global__ void __launch_bounds__(256) pad_kernel(const T* src, T* dst, int64_t 
 }
 
 // -- host ----------------------------------------------------------------------------------------------------
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+// How a product is cut.  Tiles of 256 x 256 (16-bit types) run one workgroup per CU, tiles of 128 x 128 two; `slots` is
+// what is resident at once.  Tiles that fill every slot are computed whole; the rest, which would leave slots idle for
+// a whole tile's time, are cut along K so that their pieces fill the slots, where K is long enough to pay for writing
+// and adding the pieces' fp32 sums.
+struct Cut {
+  bool large;
+  int full, tail, splits, steps;
+  size_t bytes;
+};
+Cut cut_tiles(int64_t m, int64_t n, int64_t k, int esize, bool large, bool split, int num_cus) {
+  Cut c;
+  c.large = large;
+  const int b = large ? 256 : 128;
+  const int64_t tiles = ((m + b - 1) / b) * ((n + b - 1) / b);
+  const int64_t slots = large ? num_cus : 2 * num_cus;
+  const int64_t steps = (k * esize + kRowBytes - 1) / kRowBytes;
+  const int64_t tail = tiles % slots;
+  int64_t s = tail > 0 ? std::min(slots / tail, steps / 4) : 1;
+  if (!split || s < 2 || steps - steps / s < 16) s = 1;
+  c.tail = s > 1 ? int(tail) : 0;
+  c.full = int(tiles - c.tail);
+  c.steps = int((steps + s - 1) / s);
+  c.splits = s > 1 ? int((steps + c.steps - 1) / c.steps) : 1;
+  c.bytes = round256(size_t(c.tail) * c.splits * b * b * 4);
+  return c;
+}
+// kFwd and kBwd: large tiles when every CU gets one.  fp32, whose matrix rate is a sixteenth, takes small ones.
+Cut cut_gated(int64_t f, int64_t t, int64_t k, int esize, int num_cus) {
+  const bool large = esize == 2 && ((2 * f + 255) / 256) * ((t + 255) / 256) >= num_cus;
+  // a large tile is 128 of f and their gate and up rows, a small one 64
+  Cut c = cut_tiles(2 * f, t, k, esize, large, false, num_cus);
+  const int64_t fb = large ? 128 : 64;
+  c.full = int(((f + fb - 1) / fb) * ((t + 2 * fb - 1) / (2 * fb)));
+  return c;
+}
+// kDx and kDw: large tiles when their K pieces can fill the CUs with at least 16 steps each.
+Cut cut_product(int64_t m, int64_t n, int64_t k, int esize, int num_cus) {
+  const int64_t tiles = ((m + 255) / 256) * ((n + 255) / 256);
+  const int64_t steps = (k * esize + kRowBytes - 1) / kRowBytes;
+  const bool large = esize == 2 && tiles * std::max<int64_t>(1, steps / 16) >= num_cus;
+  return cut_tiles(m, n, k, esize, large, true, num_cus);
+}
+
 struct Plan {
   int64_t T, C, F, Fp, Cp;  // Cp: channels of the padded copies (C when none is needed)
   int esize;
   bool pad_x, pad_w;
-  size_t x_bytes, w_bytes, dab_bytes, bias_bytes, dx_bytes, dw_bytes;
-  int dx_splits, dw_splits;
+  size_t x_bytes, w_bytes, dab_bytes, bias_bytes;
+  Cut gated, dx, dw;
 };
-
-size_t round256(size_t n) { return (n + 255) / 256 * 256; }
-
-// Tiles of 256 x 256 when they are enough to give every CU one, else of 128 x 128; fp32, whose matrix rate is a
-// sixteenth, always the latter.
-bool large_tiles(int64_t m, int64_t n, int num_cus, int esize) {
-  if (esize == 4) return false;
-  return ((m + 255) / 256) * ((n + 255) / 256) >= num_cus;
-}
-
-// K splits of a product with few tiles: enough workgroups for two a CU, at least four K steps each.
-int k_splits(int64_t m, int64_t n, int64_t k, int bk, bool large, int num_cus) {
-  const int64_t b = large ? 256 : 128;
-  const int64_t tiles = ((m + b - 1) / b) * ((n + b - 1) / b);
-  const int64_t steps = (k + bk - 1) / bk;
-  const int64_t want = (2 * num_cus) / std::max<int64_t>(tiles, 1);
-  return int(std::max<int64_t>(1, std::min<int64_t>(want, steps / 4)));
-}
 
 void make_plan(Plan* q, int64_t T, int64_t C, int64_t F, int64_t x_stride, const void* x, const void* w, int dtype,
                bool need_dx, bool need_dw, bool need_db, int num_cus) {
@@ -601,31 +666,34 @@ void make_plan(Plan* q, int64_t T, int64_t C, int64_t F, int64_t x_stride, const
   q->dab_bytes = need_dx || need_dw ? round256(size_t(T) * 2 * q->Fp * q->esize) : 0;
   // bias sums of every column wave: 128-row tiles have 4 waves of 32, 256-row tiles 4 of 64
   q->bias_bytes = need_db ? round256(size_t((T + 127) / 128) * 4 * 2 * q->Fp * 4) : 0;
-  const int bk = 128 / q->esize;
-  q->dx_splits = k_splits(q->Cp, T, 2 * q->Fp, bk, large_tiles(q->Cp, T, num_cus, q->esize), num_cus);
-  q->dw_splits = k_splits(q->Cp, 2 * q->Fp, T, bk, large_tiles(q->Cp, 2 * q->Fp, num_cus, q->esize), num_cus);
-  q->dx_bytes = need_dx && q->dx_splits > 1 ? round256(size_t(q->dx_splits) * T * q->Cp * 4) : 0;
-  q->dw_bytes = need_dw && q->dw_splits > 1 ? round256(size_t(q->dw_splits) * 2 * F * q->Cp * 4) : 0;
+  q->gated = cut_gated(F, T, q->Cp, q->esize, num_cus);
+  q->dx = cut_product(q->Cp, T, 2 * q->Fp, q->esize, num_cus);
+  q->dw = cut_product(q->Cp, 2 * q->Fp, T, q->esize, num_cus);
+  if (!need_dx) q->dx.bytes = 0;
+  if (!need_dw) q->dw.bytes = 0;
 }
 
 template <typename T, int MODE>
-void launch_gemm(Params p, bool large, hipStream_t s) {
-  const int tm = (MODE == kFwd || MODE == kBwd) ? (large ? 128 : 64) : (large ? 256 : 128);
-  const int tn = large ? 256 : 128;
+void launch_gemm(Params p, const Cut& c, hipStream_t s) {
+  const bool gated = MODE == kFwd || MODE == kBwd;
+  const int b = c.large ? 256 : 128;
+  const int tm = gated ? b / 2 : b;
   p.mt = (p.M + tm - 1) / tm;
-  p.nt = (p.N + tn - 1) / tn;
-  const int bk = kBK<T>;
-  const int steps = (p.K + bk - 1) / bk;
-  p.steps = (steps + p.splits - 1) / p.splits;
-  const int64_t total = int64_t(p.mt) * p.nt * p.splits;
-  const dim3 grid(unsigned((total + 7) / 8 * 8));
+  p.nt = (p.N + b - 1) / b;
+  p.full = c.full;
+  p.tail = c.tail;
+  p.splits = c.splits;
+  p.steps = c.steps;
+  const int64_t per = (c.full + 7) / 8 + (int64_t(c.tail) * c.splits + 7) / 8;
+  const dim3 grid(unsigned(per * 8));
   if constexpr (sizeof(T) == 2) {
-    if (large) {
-      hipLaunchKernelGGL((gemm_kernel<T, MODE, 2, 4, 4>), grid, dim3(512), 0, s, p);
-      return;
-    }
+    if (c.large) hipLaunchKernelGGL((gemm_kernel<T, MODE, 2, 4, 4>), grid, dim3(512), 0, s, p);
   }
-  hipLaunchKernelGGL((gemm_kernel<T, MODE, 1, 4, 2>), grid, dim3(256), 0, s, p);
+  if (!c.large) hipLaunchKernelGGL((gemm_kernel<T, MODE, 1, 4, 2>), grid, dim3(256), 0, s, p);
+  if constexpr (MODE == kDx || MODE == kDw) {
+    if (c.tail > 0)
+      hipLaunchKernelGGL((tail_kernel<T, MODE>), dim3(unsigned(c.tail * (b * b / 1024))), dim3(256), 0, s, p, b, b);
+  }
 }
 
 template <typename T>
@@ -657,14 +725,13 @@ char* operands(const Plan& q, const void* x, int64_t x_stride, const void* w, ch
   }
   p->F = int(q.F);
   p->Fp = int(q.Fp);
-  p->splits = 1;
   return ws;
 }
 
 bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
 
 template <typename T>
-int forward(const mf_gated_linear_args* a, const Plan& q, int num_cus, hipStream_t s) {
+int forward(const mf_gated_linear_args* a, const Plan& q, hipStream_t s) {
   Params p = {};
   operands<T>(q, a->x, a->x_stride, a->weight, static_cast<char*>(a->workspace), &p, s);
   p.M = int(q.F);
@@ -675,13 +742,13 @@ int forward(const mf_gated_linear_args* a, const Plan& q, int num_cus, hipStream
   p.ldo = q.F;
   p.bias = a->bias;
   p.vec = q.F * q.esize % 16 == 0 && aligned16(a->out);
-  launch_gemm<T, kFwd>(p, large_tiles(2 * q.F, q.T, num_cus, q.esize), s);
+  launch_gemm<T, kFwd>(p, q.gated, s);
   MF_HIP_CHECK(hipGetLastError());
   return MF_OK;
 }
 
 template <typename T>
-int backward(const mf_gated_linear_bwd_args* a, const Plan& q, int num_cus, hipStream_t s) {
+int backward(const mf_gated_linear_bwd_args* a, const Plan& q, hipStream_t s) {
   const mf_gated_linear_args& f = a->fwd;
   Params p = {};
   char* ws = operands<T>(q, f.x, f.x_stride, f.weight, static_cast<char*>(a->workspace), &p, s);
@@ -691,7 +758,7 @@ int backward(const mf_gated_linear_bwd_args* a, const Plan& q, int num_cus, hipS
   ws += round256(size_t(q.T) * 2 * q.Fp * sizeof(T));
   float* sums = a->dbias ? reinterpret_cast<float*>(ws) : nullptr;
   ws += q.bias_bytes;
-  const bool big = large_tiles(2 * q.F, q.T, num_cus, q.esize);
+  const int tile = q.gated.large ? 256 : 128;
   p.M = int(q.F);
   p.N = int(q.T);
   p.K = int(q.Cp);
@@ -702,10 +769,10 @@ int backward(const mf_gated_linear_bwd_args* a, const Plan& q, int num_cus, hipS
   p.go = a->grad_out;
   p.part = sums;
   p.vec = q.F * q.esize % 16 == 0 && aligned16(a->grad_out);
-  if (q.T > 0) launch_gemm<T, kBwd>(p, big, s);
+  if (q.T > 0) launch_gemm<T, kBwd>(p, q.gated, s);
   MF_HIP_CHECK(hipGetLastError());
   if (a->dbias) {
-    const int rows = q.T == 0 ? 0 : int((q.T + (big ? 255 : 127)) / (big ? 256 : 128)) * 4;
+    const int rows = int((q.T + tile - 1) / tile) * 4;
     hipLaunchKernelGGL(bias_kernel<T>, dim3(unsigned(2 * q.Fp / 16)), dim3(256), 0, s, sums, static_cast<T*>(a->dbias),
                        rows, int(q.F), int(q.Fp));
     MF_HIP_CHECK(hipGetLastError());
@@ -721,17 +788,11 @@ int backward(const mf_gated_linear_bwd_args* a, const Plan& q, int num_cus, hipS
     d.K = int(2 * q.Fp);
     d.out = a->dx;
     d.ldo = q.C;
-    d.splits = q.dx_splits;
     d.part = reinterpret_cast<float*>(ws);
     d.vec = q.C * q.esize % 16 == 0 && aligned16(a->dx);
-    launch_gemm<T, kDx>(d, large_tiles(q.Cp, q.T, num_cus, q.esize), s);
+    launch_gemm<T, kDx>(d, q.dx, s);
     MF_HIP_CHECK(hipGetLastError());
-    if (d.splits > 1) {
-      hipLaunchKernelGGL(sum_kernel<T>, dim3(unsigned((q.T * q.C + 255) / 256)), dim3(256), 0, s, d.part,
-                         static_cast<T*>(a->dx), d.splits, q.T, int(q.Cp), int(q.C));
-      MF_HIP_CHECK(hipGetLastError());
-    }
-    ws += q.dx_bytes;
+    ws += q.dx.bytes;
   }
   if (a->dweight) {
     Params d = p;
@@ -744,16 +805,10 @@ int backward(const mf_gated_linear_bwd_args* a, const Plan& q, int num_cus, hipS
     d.K = int(q.T);
     d.out = a->dweight;
     d.ldo = q.C;
-    d.splits = q.dw_splits;
     d.part = reinterpret_cast<float*>(ws);
     d.vec = q.C * q.esize % 16 == 0 && aligned16(a->dweight);
-    launch_gemm<T, kDw>(d, large_tiles(q.Cp, 2 * q.Fp, num_cus, q.esize), s);
+    launch_gemm<T, kDw>(d, q.dw, s);
     MF_HIP_CHECK(hipGetLastError());
-    if (d.splits > 1) {
-      hipLaunchKernelGGL(sum_kernel<T>, dim3(unsigned((2 * q.F * q.C + 255) / 256)), dim3(256), 0, s, d.part,
-                         static_cast<T*>(a->dweight), d.splits, 2 * q.F, int(q.Cp), int(q.C));
-      MF_HIP_CHECK(hipGetLastError());
-    }
   }
   return MF_OK;
 }
@@ -806,9 +861,9 @@ extern "C" int mf_gated_linear(const mf_gated_linear_args* a, void* stream) {
     return fail(MF_ERR_INVALID_ARGUMENT, "mf_gated_linear: workspace is smaller than mf_gated_linear_workspace_size");
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (a->dtype) {
-    case MF_DTYPE_BF16: return forward<__bf16>(a, q, info.num_cus, s);
-    case MF_DTYPE_F16: return forward<_Float16>(a, q, info.num_cus, s);
-    default: return forward<float>(a, q, info.num_cus, s);
+    case MF_DTYPE_BF16: return forward<__bf16>(a, q, s);
+    case MF_DTYPE_F16: return forward<_Float16>(a, q, s);
+    default: return forward<float>(a, q, s);
   }
 }
 
@@ -831,7 +886,7 @@ extern "C" uint64_t mf_gated_linear_bwd_workspace_size(const mf_gated_linear_bwd
   Plan q;
   if (a == nullptr || check("mf_gated_linear_bwd_workspace_size", &a->fwd) != MF_OK) return 0;
   if (device_info(&info) != MF_OK || bwd_plan(a, &q, info.num_cus) != MF_OK) return 0;
-  return q.x_bytes + q.w_bytes + q.dab_bytes + q.bias_bytes + q.dx_bytes + q.dw_bytes;
+  return q.x_bytes + q.w_bytes + q.dab_bytes + q.bias_bytes + q.dx.bytes + q.dw.bytes;
 }
 
 extern "C" int mf_gated_linear_bwd(const mf_gated_linear_bwd_args* a, void* stream) {
@@ -849,14 +904,14 @@ extern "C" int mf_gated_linear_bwd(const mf_gated_linear_bwd_args* a, void* stre
   Plan q;
   st = bwd_plan(a, &q, info.num_cus);
   if (st != MF_OK) return st;
-  const size_t need = q.x_bytes + q.w_bytes + q.dab_bytes + q.bias_bytes + q.dx_bytes + q.dw_bytes;
+  const size_t need = q.x_bytes + q.w_bytes + q.dab_bytes + q.bias_bytes + q.dx.bytes + q.dw.bytes;
   if (need > 0 && (!a->workspace || a->workspace_bytes < need))
     return fail(MF_ERR_INVALID_ARGUMENT,
                 "mf_gated_linear_bwd: workspace is smaller than mf_gated_linear_bwd_workspace_size");
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (a->fwd.dtype) {
-    case MF_DTYPE_BF16: return backward<__bf16>(a, q, info.num_cus, s);
-    case MF_DTYPE_F16: return backward<_Float16>(a, q, info.num_cus, s);
-    default: return backward<float>(a, q, info.num_cus, s);
+    case MF_DTYPE_BF16: return backward<__bf16>(a, q, s);
+    case MF_DTYPE_F16: return backward<_Float16>(a, q, s);
+    default: return backward<float>(a, q, s);
   }
 }

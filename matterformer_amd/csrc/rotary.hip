@@ -100,13 +100,31 @@ __device__ __forceinline__ double position(const Params& p, int64_t at) {
   }
 }
 
+// The workgroup's first token, and its others: a token is few steps behind it, so the molecule is found by counting on
+// (a 64-bit division per chunk costs more than the rest of its arithmetic).
+struct First {
+  int b, n;
+};
+__device__ __forceinline__ First first_token(const Params& p, unsigned g0) {
+  const unsigned b = g0 / unsigned(p.N);
+  return {int(b), int(g0 - b * unsigned(p.N))};
+}
+__device__ __forceinline__ void token_at(const Params& p, First f, int t, int& b, int& n) {
+  b = f.b;
+  n = f.n + t;
+  while (n >= p.N) {
+    n -= p.N;
+    ++b;
+  }
+}
+
 // cos and sin (times gain) of every (token, pair) of the workgroup
-__device__ __forceinline__ void fill_table(const Params& p, int64_t g0, int nt, float2* table) {
-  const int P = p.R >> 1, per = P / p.axes;
-  for (int i = threadIdx.x; i < nt * P; i += kThreads) {
-    const int t = i / P, pr = i - t * P;
-    const int64_t g = g0 + t;
-    const int64_t b = g / p.N, n = g - b * p.N;
+__device__ __forceinline__ void fill_table(const Params& p, First f, int nt, float2* table) {
+  const unsigned P = unsigned(p.R) >> 1, per = P / unsigned(p.axes);
+  for (unsigned i = threadIdx.x; i < nt * P; i += kThreads) {
+    const unsigned t = i / P, pr = i - t * P;
+    int b, n;
+    token_at(p, f, int(t), b, n);
     const double turns = position(p, b * p.ps[0] + n * p.ps[1] + (pr / per) * p.ps[2]) * p.freq[pr] *
                          0.15915494309189533577;
     const double half = 2.0 * (turns - rint(turns));  // the angle in units of pi, in [-1, 1]
@@ -126,7 +144,7 @@ struct Where {
   int turn;
 };
 
-__device__ __forceinline__ Where locate(const Params& p, int64_t g0, int t, int hh, int ssize, int dsize) {
+__device__ __forceinline__ Where locate(const Params& p, First f, int t, int hh, int ssize, int dsize) {
   Where w;
   w.t = t;
   // the part by comparison: an index into the arguments would put them in scratch memory
@@ -134,13 +152,13 @@ __device__ __forceinline__ Where locate(const Params& p, int64_t g0, int t, int 
   const bool two = p.nparts > 2 && hh >= p.part[0].heads + p.part[1].heads;
   const int h = hh - (one ? p.part[0].heads : 0) - (two ? p.part[1].heads : 0);
 #define MF_PICK(field) (two ? p.part[2].field : one ? p.part[1].field : p.part[0].field)
-  const int64_t g = g0 + t;
-  const int64_t b = g / p.N, n = g - b * p.N;
+  int b, n;
+  token_at(p, f, t, b, n);
   int64_t so = b * MF_PICK(ss[0]) + n * MF_PICK(ss[2]);
   int64_t dst = b * MF_PICK(ds[0]) + n * MF_PICK(ds[2]);
   bool src_ok = true, dst_ok = true;
   if (p.slot_side != MF_SLOT_NONE) {
-    const int64_t row = p.slot[g];
+    const int64_t row = p.slot[int64_t(b) * p.N + n];
     if (p.slot_side == MF_SLOT_SRC) {
       src_ok = row >= 0;
       so = row * MF_PICK(ss[2]);
@@ -163,13 +181,14 @@ template <typename TS, typename TD>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(Params p) {
   __shared__ float2 table[kMaxTokens * kMaxPairs];
   __shared__ __attribute__((aligned(16))) TS raw[kBlockChunks * 8];
-  const int64_t tokens = int64_t(p.B) * p.N;
-  const int64_t g0 = int64_t(blockIdx.x) * p.TT;
-  const int nt = int(min(int64_t(p.TT), tokens - g0));
+  const unsigned g0 = blockIdx.x * unsigned(p.TT);  // below 2^31 tokens
+  const int nt = min(p.TT, int(unsigned(p.B) * unsigned(p.N) - g0));
+  const First first = first_token(p, g0);
   const int h0 = blockIdx.y * p.HS;
   const int nh = min(p.HS, p.heads - h0);
   const int DC = p.D >> 3;
   const int total = nt * nh * DC;
+  const int rdc = (65536 + DC - 1) / DC, rnt = (65536 + nt - 1) / nt;
   Chunk<TS> v[kChunks];
   Where w[kChunks];
   int col[kChunks];
@@ -177,14 +196,15 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(Params p) {
   for (int k = 0; k < kChunks; ++k) {
     const int i = threadIdx.x + k * kThreads;
     if (i >= total) continue;
-    const int r = i / DC;
-    const int hh = r / nt;
+    // i < 1024, DC <= 32, nt <= 16: the products with the reciprocals' ceilings below are exact quotients
+    const int r = (i * rdc) >> 16;
+    const int hh = (r * rnt) >> 16;
     col[k] = (i - r * DC) * 8;
-    w[k] = locate(p, g0, r - hh * nt, h0 + hh, sizeof(TS), sizeof(TD));
+    w[k] = locate(p, first, r - hh * nt, h0 + hh, sizeof(TS), sizeof(TD));
     if (w[k].src) v[k].load(reinterpret_cast<const TS*>(w[k].src) + col[k]);
     else v[k].clear();
   }
-  fill_table(p, g0, nt, table);
+  fill_table(p, first, nt, table);
   if (!p.interleaved) {
 #pragma unroll
     for (int k = 0; k < kChunks; ++k) {
@@ -236,20 +256,20 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(Params p) {
 template <typename TS, typename TD>
 __global__ void __launch_bounds__(kThreads) rotary_scalar_kernel(Params p) {
   __shared__ float2 table[kMaxTokens * kMaxPairs];
-  const int64_t tokens = int64_t(p.B) * p.N;
-  const int64_t g0 = int64_t(blockIdx.x) * p.TT;
-  const int nt = int(min(int64_t(p.TT), tokens - g0));
+  const unsigned g0 = blockIdx.x * unsigned(p.TT);  // below 2^31 tokens
+  const int nt = min(p.TT, int(unsigned(p.B) * unsigned(p.N) - g0));
+  const First first = first_token(p, g0);
   const int h0 = blockIdx.y * p.HS;
   const int nh = min(p.HS, p.heads - h0);
   const int total = nt * nh * p.D;
-  fill_table(p, g0, nt, table);
+  fill_table(p, first, nt, table);
   __syncthreads();
   const int P = p.R >> 1;
   for (int i = threadIdx.x; i < total; i += kThreads) {
     const int r = i / p.D;
     const int hh = r / nt;
     const int j = i - r * p.D;
-    const Where w = locate(p, g0, r - hh * nt, h0 + hh, sizeof(TS), sizeof(TD));
+    const Where w = locate(p, first, r - hh * nt, h0 + hh, sizeof(TS), sizeof(TD));
     if (!w.dst) continue;
     const TS* src = reinterpret_cast<const TS*>(w.src);
     float y = src ? Elem<TS>::to_f32(src[j]) : 0.0f;

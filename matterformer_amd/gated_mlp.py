@@ -44,8 +44,7 @@ def _forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, a
     nbytes = int(lib.mf_gated_linear_workspace_size(args))
     scratch = _scratch(nbytes, x.device)
     args.workspace, args.workspace_bytes = _native.ptr(scratch), nbytes
-    with torch.cuda.device(x.device):
-        _native.check(lib.mf_gated_linear(args, _native.current_stream(x.device)), "mf_gated_linear")
+    _native.launch("mf_gated_linear", args, x.device)
     return out
 
 
@@ -67,15 +66,13 @@ class _GatedLinearFunction(torch.autograd.Function):
         db = torch.empty_like(bias) if bias is not None and need[2] else None
         if x.shape[0] == 0:
             return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None
-        lib = _native.lib()
-        with torch.cuda.device(x.device):
-            args = _native.MfGatedLinearBwdArgs(
-                fwd=_arguments(x, weight, bias, ctx.activation, None), grad_out=grad.data_ptr(), dx=_native.ptr(dx),
-                dweight=_native.ptr(dw), dbias=_native.ptr(db))
-            nbytes = int(lib.mf_gated_linear_bwd_workspace_size(args))
-            scratch = _scratch(nbytes, x.device)
-            args.workspace, args.workspace_bytes = _native.ptr(scratch), nbytes
-            _native.check(lib.mf_gated_linear_bwd(args, _native.current_stream(x.device)), "mf_gated_linear_bwd")
+        args = _native.MfGatedLinearBwdArgs(
+            fwd=_arguments(x, weight, bias, ctx.activation, None), grad_out=grad.data_ptr(), dx=_native.ptr(dx),
+            dweight=_native.ptr(dw), dbias=_native.ptr(db))
+        nbytes = int(_native.lib().mf_gated_linear_bwd_workspace_size(args))
+        scratch = _scratch(nbytes, x.device)
+        args.workspace, args.workspace_bytes = _native.ptr(scratch), nbytes
+        _native.launch("mf_gated_linear_bwd", args, x.device)
         return dx, dw, db, None
 
 
@@ -92,16 +89,20 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
         raise ValueError(f"x must have shape (..., {weight.shape[1]}), got {tuple(x.shape)}")
     if bias is not None and bias.shape != weight.shape[:1]:
         raise ValueError(f"bias must have shape ({weight.shape[0]},), got {tuple(bias.shape)}")
-    tensors = [t for t in (x, weight, bias) if t is not None]
-    if any(t.dtype != x.dtype or t.device != x.device for t in tensors):
+    if any(t is not None and (t.dtype != x.dtype or t.device != x.device) for t in (weight, bias)):
         raise RuntimeError("x, weight and bias must share a dtype and a device")
     if x.device.type != "cuda":
         gate, up = F.linear(x, weight, bias).chunk(2, dim=-1)
         return _TORCH_ACT[activation](gate) * up
     if x.dtype not in _DTYPES:
         raise RuntimeError(f"gated_linear supports bfloat16, float16 and float32 on the GPU, got {x.dtype}")
-    rows = x.reshape(-1, x.shape[-1])
+    rows = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
     if rows.stride(-1) != 1 or (rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]):
         rows = rows.contiguous()
-    out = _GatedLinearFunction.apply(rows, weight.contiguous(), None if bias is None else bias.contiguous(), activation)
-    return out.reshape(*x.shape[:-1], out.shape[-1])
+    weight = weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    if _native.takes_gradient(rows, weight, bias):
+        out = _GatedLinearFunction.apply(rows, weight, bias, activation)
+    else:
+        out = _forward(rows, weight, bias, activation)
+    return out if x.ndim == 2 else out.reshape(*x.shape[:-1], out.shape[-1])

@@ -249,14 +249,13 @@ def radius_tables(mask_bits: torch.Tensor, block_mask: torch.Tensor | None = Non
     dev = _require_device(mask_bits, block_mask)
     bits = mask_bits.contiguous()
     bm = None if block_mask is None else block_mask.to(torch.uint8).contiguous()
-    tables = RadiusTables(torch.empty(B, N, W, dtype=torch.int32, device=dev),
-                          *(torch.empty(B, NB, NB, dtype=torch.int64, device=dev) for _ in range(2)))
+    any_bits = torch.empty(2, B, NB, NB, dtype=torch.int64, device=dev)
+    tables = RadiusTables(torch.empty_like(bits), any_bits[0], any_bits[1])
     if B * N > 0:
         args = _native.MfRadiusTablesArgs(
             mask_bits=bits.data_ptr(), block_mask=_native.ptr(bm), mask_bits_t=tables.bits_t.data_ptr(),
             key_any=tables.key_any.data_ptr(), query_any=tables.query_any.data_ptr(), batch=B, atoms=N)
-        with torch.cuda.device(dev):
-            _native.check(_native.lib().mf_radius_tables(args, _native.current_stream(dev)), "mf_radius_tables")
+        _native.launch("mf_radius_tables", args, dev)
     return tables
 
 
@@ -271,8 +270,7 @@ def _radius_forward(q, k, v, bits, bm, tables, scale, *, lse: bool, fp32: bool):
         out=out.data_ptr(), out_f32=_native.ptr(out32), lse=_native.ptr(lse_out), scale=scale, batch=B, heads=H,
         atoms=N, head_dim=D, dtype=_native.dtype_code(q.dtype),
         key_any=None if tables is None else tables.key_any.data_ptr())
-    with torch.cuda.device(q.device):
-        _native.check(_native.lib().mf_radius_attn(args, _native.current_stream(q.device)), "mf_radius_attn")
+    _native.launch("mf_radius_attn", args, q.device)
     return out, lse_out, out32
 
 
@@ -303,8 +301,7 @@ class _RadiusAttentionFunction(torch.autograd.Function):
         grads = [torch.empty_like(t) for t in (q, k, v)]
         if q.numel() > 0:
             t = ctx.tables
-            lib = _native.lib()
-            nbytes = int(lib.mf_radius_attn_bwd_workspace_size(B, H, N, _native.dtype_code(q.dtype)))
+            nbytes = int(_native.lib().mf_radius_attn_bwd_workspace_size(B, H, N, _native.dtype_code(q.dtype)))
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
             args = _native.MfRadiusAttnBwdArgs(
                 q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), lse=lse.data_ptr(),
@@ -313,8 +310,7 @@ class _RadiusAttentionFunction(torch.autograd.Function):
                 dq=grads[0].data_ptr(), dk=grads[1].data_ptr(), dv=grads[2].data_ptr(),
                 workspace=workspace.data_ptr(), workspace_bytes=nbytes, scale=ctx.scale, batch=B, heads=H, atoms=N,
                 head_dim=D, dtype=_native.dtype_code(q.dtype))
-            with torch.cuda.device(q.device):
-                _native.check(lib.mf_radius_attn_bwd(args, _native.current_stream(q.device)), "mf_radius_attn_bwd")
+            _native.launch("mf_radius_attn_bwd", args, q.device)
         return (*grads, None, None, None, None, None)
 
 
@@ -359,7 +355,7 @@ def radius_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bit
         if tables.bits_t.shape != bits.shape or tables.key_any.shape != (B, NB, NB):
             raise ValueError("tables must be radius_tables of this call's masks")
         _require_device(bits, tables.bits_t)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+    if _native.takes_gradient(q, k, v):
         if tables is None:
             tables = radius_tables(bits, bm)
         out, lse, out32 = _RadiusAttentionFunction.apply(qc, kc, vc, bits, bm, tables, s, return_fp32)

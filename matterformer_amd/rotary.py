@@ -17,6 +17,7 @@ frequencies take none); a missing library raises.  CPU tensors take the torch fo
 
 from __future__ import annotations
 
+import ctypes
 import math
 from dataclasses import dataclass
 
@@ -51,6 +52,8 @@ class RotaryFrequencies:
             raise ValueError("the pairs must be a positive multiple of axes")
         if not math.isfinite(float(self.gain)):
             raise ValueError("gain must be finite")
+        object.__setattr__(self, "axes", int(self.axes))
+        object.__setattr__(self, "gain", float(self.gain))
 
     @property
     def rotary_dim(self) -> int:
@@ -104,20 +107,23 @@ def rotary_frequencies(rotary_dim: int, *, axes: int = 1, base: float = 10000.0,
 
 def _check_positions(positions: torch.Tensor, batch: int, tokens: int, frequencies: RotaryFrequencies,
                      device: torch.device) -> torch.Tensor:
-    """(B, N, axes) view of the positions; one row for the batch is expanded."""
-    axes = int(frequencies.axes)
-    if positions.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("rotary positions take no gradient: detach them")
+    """The positions as (B or 1, N, axes)."""
+    axes = frequencies.axes
+    if positions.requires_grad:
+        if torch.is_grad_enabled():
+            raise RuntimeError("rotary positions take no gradient: detach them")
+        positions = positions.detach()
     if positions.dtype not in _POSITION_TYPES:
         raise RuntimeError(f"rotary positions must be float32, float64, int32 or int64, got {positions.dtype}")
     if frequencies.table.device != device or positions.device != device:
         raise RuntimeError("positions and frequencies must be on the device of the heads")
     if axes == 1 and positions.ndim == 2:
         positions = positions[..., None]
-    if positions.ndim != 3 or positions.shape[0] not in (1, batch) or tuple(positions.shape[1:]) != (tokens, axes):
+    shape = positions.shape
+    if len(shape) != 3 or shape[0] not in (1, batch) or shape[1] != tokens or shape[2] != axes:
         want = f"({batch}, {tokens})" if axes == 1 else f"({batch}, {tokens}, {axes})"
-        raise ValueError(f"positions must have shape {want} (or one row for the batch), got {tuple(positions.shape)}")
-    return positions.detach().expand(batch, tokens, axes)
+        raise ValueError(f"positions must have shape {want} (or one row for the batch), got {tuple(shape)}")
+    return positions
 
 
 def _check_layout(layout: str, head_dim: int, frequencies: RotaryFrequencies) -> bool:
@@ -148,7 +154,7 @@ def _rotate_torch(x: torch.Tensor, positions: torch.Tensor, frequencies: RotaryF
 
 
 class _Plan:
-    """What a launch and its gradient share: positions (B, N, axes), frequencies and the pairs' layout; for packed
+    """What a launch and its gradient share: positions (B or 1, N, axes), frequencies and the pairs' layout; for packed
     rows the slot map."""
 
     def __init__(self, positions, frequencies, interleaved, slot=None):
@@ -158,29 +164,28 @@ class _Plan:
         self.slot = slot
 
 
+_I32x3 = ctypes.c_int32 * 3
+_I64x3 = ctypes.c_int64 * 3
+_I64x3x3 = _I64x3 * 3
+_PTRx3 = ctypes.c_void_p * 3
+
+
 def _launch(plan: _Plan, parts, *, batch: int, tokens: int, head_dim: int, inverse: bool, slot_side: int) -> None:
     """parts: (src, src strides {batch, head, token}, dst, dst strides, heads, turned), src and dst (tensor, element
     offset); the dtypes are those of the first part."""
+    pos, f = plan.positions, plan.frequencies
+    ps = pos.stride()
+    src, dst = parts[0][0][0], parts[0][2][0]
+    ssize, dsize = src.element_size(), dst.element_size()
     args = _native.MfRotaryArgs(
-        positions=plan.positions.data_ptr(), frequencies=plan.frequencies.table.data_ptr(),
-        slot=_native.ptr(plan.slot), gain=float(plan.frequencies.gain),
-        position_type=_POSITION_TYPES[plan.positions.dtype], slot_side=slot_side, parts=len(parts), batch=batch,
-        tokens=tokens, head_dim=head_dim, rotary_dim=plan.frequencies.rotary_dim, axes=int(plan.frequencies.axes),
-        interleaved=int(plan.interleaved), inverse=int(inverse), src_dtype=_native.dtype_code(parts[0][0][0].dtype),
-        dst_dtype=_native.dtype_code(parts[0][2][0].dtype))
-    for i, stride in enumerate(plan.positions.stride()):
-        args.position_stride[i] = stride
-    for k, ((src, s0), ss, (dst, d0), ds, heads, turn) in enumerate(parts):
-        args.src[k] = src.data_ptr() + s0 * src.element_size()
-        args.dst[k] = dst.data_ptr() + d0 * dst.element_size()
-        args.heads[k] = heads
-        args.turn[k] = int(turn)
-        for i in range(3):
-            args.src_stride[k][i] = ss[i]
-            args.dst_stride[k][i] = ds[i]
-    dev = parts[0][0][0].device
-    with torch.cuda.device(dev):
-        _native.check(_native.lib().mf_rotary(args, _native.current_stream(dev)), "mf_rotary")
+        _PTRx3(*[t.data_ptr() + at * ssize for (t, at), *_ in parts]),
+        _PTRx3(*[t.data_ptr() + at * dsize for _, _, (t, at), *_ in parts]),
+        _I64x3x3(*[p[1] for p in parts]), _I64x3x3(*[p[3] for p in parts]), _I32x3(*[p[4] for p in parts]),
+        _I32x3(*[p[5] for p in parts]), pos.data_ptr(), _I64x3(ps[0] if pos.shape[0] > 1 else 0, ps[1], ps[2]),
+        f.table.data_ptr(), _native.ptr(plan.slot), f.gain, _POSITION_TYPES[pos.dtype], slot_side, len(parts), batch,
+        tokens, head_dim, 2 * f.table.shape[0], f.axes, plan.interleaved, inverse, _native.dtype_code(src.dtype),
+        _native.dtype_code(dst.dtype))
+    _native.launch("mf_rotary", args, src.device)
 
 
 def _unit(t: torch.Tensor) -> torch.Tensor:
@@ -189,17 +194,19 @@ def _unit(t: torch.Tensor) -> torch.Tensor:
 
 def _strides(t: torch.Tensor) -> tuple:
     """{batch, head, token} strides of (B, H, N, D) heads; 0 for an axis of one entry, whose stride means nothing."""
-    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3]))
+    (b, h, n, _), (sb, sh, sn, _) = t.shape, t.stride()
+    return (sb if b > 1 else 0, sh if h > 1 else 0, sn if n > 1 else 0)
 
 
-def _turn_heads(plan: _Plan, heads: list[torch.Tensor], inverse: bool) -> list[torch.Tensor]:
+def _turn_heads(plan: _Plan, heads, inverse: bool) -> tuple[torch.Tensor, ...]:
     """(B, H, N, D) heads -> turned contiguous heads, in one launch."""
-    outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in heads]
+    outs = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in heads)
     B, _, N, D = heads[0].shape
-    parts = []
-    for t, o in zip((_unit(t) for t in heads), outs):
-        parts.append(((t, 0), _strides(t), (o, 0), _strides(o), t.shape[1], True))
     if B * N > 0:
+        parts = []
+        for t, o in zip(heads, outs):
+            t = _unit(t)
+            parts.append(((t, 0), _strides(t), (o, 0), _strides(o), t.shape[1], True))
         _launch(plan, parts, batch=B, tokens=N, head_dim=D, inverse=inverse, slot_side=_native.MF_SLOT_NONE)
     return outs
 
@@ -208,12 +215,12 @@ class _HeadsFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, plan, *heads):
         ctx.plan = plan
-        return tuple(_turn_heads(plan, list(heads), False))
+        return _turn_heads(plan, heads, False)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
-        return (None, *_turn_heads(ctx.plan, list(grads), True))
+        return (None, *_turn_heads(ctx.plan, grads, True))
 
 
 def _head_parts(counts, head_dim: int, batch_stride: int, row_stride: int):
@@ -227,7 +234,7 @@ def _head_parts(counts, head_dim: int, batch_stride: int, row_stride: int):
 
 def _rows_to_heads(plan: _Plan, rows: torch.Tensor, counts, batch: int, tokens: int, head_dim: int, dtype):
     """rows (B, N, columns), or packed (T, columns) through plan.slot -> one (B, heads, N, D) tensor a part."""
-    outs = [torch.empty(batch, h, tokens, head_dim, dtype=dtype, device=rows.device) for h in counts]
+    outs = tuple(torch.empty(batch, h, tokens, head_dim, dtype=dtype, device=rows.device) for h in counts)
     packed = plan.slot is not None
     rows = _unit(rows)
     layout = _head_parts(counts, head_dim, 0 if packed else rows.stride(0), rows.stride(-2))
@@ -244,7 +251,7 @@ class _RowsFunction(torch.autograd.Function):
     def forward(ctx, plan, rows, counts, batch, tokens, head_dim, dtype):
         ctx.plan, ctx.counts, ctx.sizes = plan, counts, (batch, tokens, head_dim)
         ctx.rows = (rows.shape, rows.dtype)
-        return tuple(_rows_to_heads(plan, rows, counts, batch, tokens, head_dim, dtype))
+        return _rows_to_heads(plan, rows, counts, batch, tokens, head_dim, dtype)
 
     @staticmethod
     @once_differentiable
@@ -289,7 +296,8 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         out = [_rotate_torch(t, pos, frequencies, interleaved).contiguous() for t in heads]
     else:
         _check_kernel(D, q.dtype)
-        out = _HeadsFunction.apply(_Plan(pos, frequencies, interleaved), *heads)
+        plan = _Plan(pos, frequencies, interleaved)
+        out = _HeadsFunction.apply(plan, *heads) if _native.takes_gradient(q, k) else _turn_heads(plan, heads, False)
     return (out[0], None) if k is None else (out[0], out[1])
 
 
@@ -321,7 +329,8 @@ def rotary_heads(rows: torch.Tensor, positions: torch.Tensor, frequencies: Rotar
     if rows.device.type != "cuda":
         return _rows_torch(rows, pos, frequencies, interleaved, counts, D, rows.dtype)
     _check_kernel(D, rows.dtype)
-    return _RowsFunction.apply(_Plan(pos, frequencies, interleaved), rows, counts, B, N, D, rows.dtype)
+    run = _RowsFunction.apply if _native.takes_gradient(rows) else _rows_to_heads
+    return run(_Plan(pos, frequencies, interleaved), rows, counts, B, N, D, rows.dtype)
 
 
 def _packed_rotary_heads(rows: torch.Tensor, slot: torch.Tensor, positions: torch.Tensor,
@@ -340,4 +349,5 @@ def _packed_rotary_heads(rows: torch.Tensor, slot: torch.Tensor, positions: torc
     _check_kernel(head_dim, rows.dtype)
     _check_kernel(head_dim, dtype)
     plan = _Plan(pos, frequencies, interleaved, slot.contiguous())
-    return _RowsFunction.apply(plan, rows, (heads, heads, heads), B, W, head_dim, dtype)
+    run = _RowsFunction.apply if _native.takes_gradient(rows) else _rows_to_heads
+    return run(plan, rows, (heads, heads, heads), B, W, head_dim, dtype)
