@@ -10,16 +10,16 @@
 // once and the bytes are what bounds it.
 //
 // Angles: pos * f is formed in fp64 and reduced to a fraction of a turn there
-// (a position of 10^6 in fp32 would be off by 0.06 rad), then sincospi in fp32
-// with the fraction's own rounding carried as a first-order correction.  They
-// are computed once per token and pair into LDS and serve every head of every
-// part.
+// (a position of 10^6 in fp32 would be off by 0.06 rad); sine and cosine of what
+// is left are fp32.
 //
-// A workgroup takes TT tokens of a range of heads: at most 1024 chunks of 8
-// consecutive elements, four a thread, all loaded before the first is used.
-// With the half layout the partner of an element lies rotary_dim / 2 away, at
-// any alignment, so the raw chunks go through LDS and partners are read there
-// one by one; reading them from global memory costs eight 2-byte loads a chunk.
+// A thread owns eight pairs of one token: it computes their sines and cosines
+// once, into registers, and walks the heads of every part, four at a time (eight
+// 16-byte loads in flight).  Its pairs are two pieces of eight consecutive
+// entries, 16 bytes each at any alignment (the second half of the half layout
+// starts at rotary_dim / 2, which need be no multiple of 8); the last unit of
+// pairs starts at P - 8 and computes some pairs a second time, with equal
+// results, rather than masking.  More threads of a token copy what is not turned.
 #include <algorithm>
 #include <cmath>
 
@@ -29,10 +29,9 @@ namespace mf {
 namespace rot {
 
 constexpr int kThreads = 256;
-constexpr int kChunks = 4;                       // chunks of 8 elements per thread
-constexpr int kBlockChunks = kThreads * kChunks;
-constexpr int kMaxTokens = 16;                   // tokens per workgroup
-constexpr int kMaxPairs = 128;                   // head_dim <= 256
+constexpr int kHeads = 4;         // heads in flight per thread
+constexpr int kMaxDim = 256;
+constexpr int kScalarTokens = 16; // tokens per workgroup of the scalar kernel
 
 struct Part {
   const void* src;
@@ -52,21 +51,17 @@ struct Params {
   int pos_type, slot_side, axes, inverse;
   int nparts, B, N, D, R, interleaved;
   int TT, HS, heads;     // tokens and heads per workgroup, heads of all parts
+  int units, turned;     // threads of a token, and those of them that turn pairs
 };
 
-// 8 consecutive elements in registers: one 16-byte load for 16-bit types, two for fp32.
+// 8 consecutive elements in registers: one 16-byte access for 16-bit types, two for fp32.
 template <typename T>
 struct Chunk {
   static constexpr int kLoads = sizeof(T) / 2;
   uint4 u[kLoads];
-  __device__ __forceinline__ void load(const T* p) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
-  }
-  __device__ __forceinline__ void store(T* p) const {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) reinterpret_cast<uint4*>(p)[i] = u[i];
-  }
+  // any alignment: global memory takes 16-byte accesses at every byte
+  __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(u, p, sizeof(u)); }
+  __device__ __forceinline__ void store(T* p) const { __builtin_memcpy(p, u, sizeof(u)); }
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) u[i] = make_uint4(0, 0, 0, 0);
@@ -100,202 +95,205 @@ __device__ __forceinline__ double position(const Params& p, int64_t at) {
   }
 }
 
-// The workgroup's first token, and its others: a token is few steps behind it, so the molecule is found by counting on
-// (a 64-bit division per chunk costs more than the rest of its arithmetic).
-struct First {
-  int b, n;
-};
-__device__ __forceinline__ First first_token(const Params& p, unsigned g0) {
-  const unsigned b = g0 / unsigned(p.N);
-  return {int(b), int(g0 - b * unsigned(p.N))};
+// cos and sin of pair pr at a position, times gain.  In fp64 the angle becomes quarter turns q and a rest x of at most
+// pi / 4; their Taylor sums to x^9 and x^10 leave less than 2^-25.
+__device__ __forceinline__ float2 turn_of(const Params& p, int64_t at, int pr) {
+  const double turns = position(p, at) * p.freq[pr] * 0.15915494309189533577;
+  const double quarters = 4.0 * (turns - rint(turns));  // in [-2, 2]
+  const double whole = rint(quarters);
+  const float x = float((quarters - whole) * 1.57079632679489661923);
+  const int q = int(whole) & 3;
+  const float z = x * x;
+  const float s = x + x * z * (-1.0f / 6 + z * (1.0f / 120 + z * (-1.0f / 5040 + z * (1.0f / 362880))));
+  const float c = 1.0f + z * (-0.5f + z * (1.0f / 24 + z * (-1.0f / 720 + z * (1.0f / 40320 + z * (-1.0f / 3628800)))));
+  const float cc = q & 1 ? s : c, sc = q & 1 ? c : s;
+  const float cos = q == 1 || q == 2 ? -cc : cc, sin = q >= 2 ? -sc : sc;
+  return make_float2(p.gain * cos, p.gain * (p.inverse ? -sin : sin));
 }
-__device__ __forceinline__ void token_at(const Params& p, First f, int t, int& b, int& n) {
-  b = f.b;
-  n = f.n + t;
-  while (n >= p.N) {
-    n -= p.N;
-    ++b;
+
+// n < 16 elements at any alignment, in pieces of 8, 4, 2 and 1
+template <typename TS, typename TD>
+__device__ __forceinline__ void copy_some(const TS* src, TD* dst, int n, bool zero) {
+  int at = 0;
+#pragma unroll
+  for (int size = 8; size >= 1; size >>= 1) {
+    if (!(n & size)) continue;
+    TS v[8];
+    if (zero) {
+#pragma unroll
+      for (int e = 0; e < size; ++e) v[e] = TS(0.0f);
+    } else {
+      __builtin_memcpy(v, src + at, size * sizeof(TS));
+    }
+    TD o[8];
+#pragma unroll
+    for (int e = 0; e < size; ++e) o[e] = Elem<TD>::from_f32(Elem<TS>::to_f32(v[e]));
+    __builtin_memcpy(dst + at, o, size * sizeof(TD));
+    at += size;
   }
 }
 
-// cos and sin (times gain) of every (token, pair) of the workgroup
-__device__ __forceinline__ void fill_table(const Params& p, First f, int nt, float2* table) {
+template <typename TS, typename TD, bool INTERLEAVED>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(Params p) {
+  const unsigned t = threadIdx.x / unsigned(p.units);
+  const int u = int(threadIdx.x - t * unsigned(p.units));
+  const unsigned g = blockIdx.x * unsigned(p.TT) + t;  // below 2^31
+  if (int(t) >= p.TT || g >= unsigned(p.B) * unsigned(p.N)) return;
+  const unsigned b = g / unsigned(p.N), n = g - b * unsigned(p.N);
+  const int P = p.R >> 1;
+  const bool turner = u < p.turned;
+  const int p0 = min(8 * u, P - 8);  // first pair (turners)
+  int64_t row = 0;
+  if (p.slot_side != MF_SLOT_NONE) row = p.slot[g];
+  const bool zero = p.slot_side == MF_SLOT_SRC && row < 0;
+  if (p.slot_side == MF_SLOT_DST && row < 0) return;
+  float2 cs[8];
+  if (turner && !zero) {
+    const int per = P / p.axes;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      cs[j] = turn_of(p, b * p.ps[0] + n * p.ps[1] + ((p0 + j) / per) * p.ps[2], p0 + j);
+  }
+  const int h0 = blockIdx.y * p.HS, h1 = min(p.heads, h0 + p.HS);
+  int base = 0;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    if (k >= p.nparts) break;
+    const Part& part = p.part[k];
+    const int lo = max(h0 - base, 0), hi = min(h1 - base, part.heads);
+    base += part.heads;
+    if (lo >= hi) continue;
+    const bool turning = part.turn != 0 && turner;
+    // the thread's entries: two pieces of 8, or fewer than 16 entries from e0 on
+    int e0, e1, some = 16;
+    if (turning) {
+      e0 = INTERLEAVED ? 2 * p0 : p0;
+      e1 = INTERLEAVED ? e0 + 8 : P + p0;
+    } else if (part.turn) {
+      e0 = p.R + 16 * (u - p.turned);
+      e1 = e0 + 8;
+      some = p.D - e0;
+    } else {
+      e0 = min(16 * u, p.D - 16);
+      e1 = e0 + 8;
+      if (16 * u >= p.D) continue;
+    }
+    const int64_t so = p.slot_side == MF_SLOT_SRC ? row * part.ss[2] : b * part.ss[0] + n * part.ss[2];
+    const int64_t dst = p.slot_side == MF_SLOT_DST ? row * part.ds[2] : b * part.ds[0] + n * part.ds[2];
+    const TS* s = static_cast<const TS*>(part.src) + so + lo * part.ss[1];
+    TD* d = static_cast<TD*>(part.dst) + dst + lo * part.ds[1];
+    if (some < 16) {
+      for (int h = lo; h < hi; ++h, s += part.ss[1], d += part.ds[1]) copy_some(s + e0, d + e0, some, zero);
+      continue;
+    }
+    for (int h = lo; h < hi; h += kHeads, s += kHeads * part.ss[1], d += kHeads * part.ds[1]) {
+      Chunk<TS> a[kHeads], c[kHeads];
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i) {
+        if (zero || h + i >= hi) {
+          a[i].clear();
+          c[i].clear();
+        } else {
+          a[i].load(s + i * part.ss[1] + e0);
+          c[i].load(s + i * part.ss[1] + e1);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i) {
+        if (h + i >= hi) break;
+        float x[8], y[8];
+        a[i].unpack(x);
+        c[i].unpack(y);
+        if (turning && !zero) {
+          if constexpr (INTERLEAVED) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float x0 = x[2 * j], x1 = x[2 * j + 1], y0 = y[2 * j], y1 = y[2 * j + 1];
+              x[2 * j] = x0 * cs[j].x - x1 * cs[j].y;
+              x[2 * j + 1] = x0 * cs[j].y + x1 * cs[j].x;
+              y[2 * j] = y0 * cs[j + 4].x - y1 * cs[j + 4].y;
+              y[2 * j + 1] = y0 * cs[j + 4].y + y1 * cs[j + 4].x;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float x0 = x[j], x1 = y[j];
+              x[j] = x0 * cs[j].x - x1 * cs[j].y;
+              y[j] = x0 * cs[j].y + x1 * cs[j].x;
+            }
+          }
+        }
+        Chunk<TD> o;
+        o.pack(x);
+        o.store(d + i * part.ds[1] + e0);
+        o.pack(y);
+        o.store(d + i * part.ds[1] + e1);
+      }
+    }
+  }
+}
+
+// Heads too short for a thread's pieces (fewer than 8 pairs or 16 entries): one element at a time.
+template <typename TS, typename TD>
+__global__ void __launch_bounds__(kThreads) rotary_scalar_kernel(Params p) {
+  __shared__ float2 table[kScalarTokens * 8];
+  const unsigned g0 = blockIdx.x * unsigned(p.TT);  // below 2^31 tokens
+  const unsigned nt = min(unsigned(p.TT), unsigned(p.B) * unsigned(p.N) - g0);
   const unsigned P = unsigned(p.R) >> 1, per = P / unsigned(p.axes);
   for (unsigned i = threadIdx.x; i < nt * P; i += kThreads) {
     const unsigned t = i / P, pr = i - t * P;
-    int b, n;
-    token_at(p, f, int(t), b, n);
-    const double turns = position(p, b * p.ps[0] + n * p.ps[1] + (pr / per) * p.ps[2]) * p.freq[pr] *
-                         0.15915494309189533577;
-    const double half = 2.0 * (turns - rint(turns));  // the angle in units of pi, in [-1, 1]
-    const float a = float(half);
-    const float d = float(half - double(a)) * 3.14159265f;
-    float s, c;
-    sincospif(a, &s, &c);
-    const float cc = c - d * s, sc = s + d * c;
-    table[i] = make_float2(p.gain * cc, p.gain * (p.inverse ? -sc : sc));
-  }
-}
-
-struct Where {
-  const char* src;  // the head row, or null where the source has none
-  char* dst;        // the head row, or null where the destination has none
-  int t;            // token within the workgroup
-  int turn;
-};
-
-__device__ __forceinline__ Where locate(const Params& p, First f, int t, int hh, int ssize, int dsize) {
-  Where w;
-  w.t = t;
-  // the part by comparison: an index into the arguments would put them in scratch memory
-  const bool one = hh >= p.part[0].heads;
-  const bool two = p.nparts > 2 && hh >= p.part[0].heads + p.part[1].heads;
-  const int h = hh - (one ? p.part[0].heads : 0) - (two ? p.part[1].heads : 0);
-#define MF_PICK(field) (two ? p.part[2].field : one ? p.part[1].field : p.part[0].field)
-  int b, n;
-  token_at(p, f, t, b, n);
-  int64_t so = b * MF_PICK(ss[0]) + n * MF_PICK(ss[2]);
-  int64_t dst = b * MF_PICK(ds[0]) + n * MF_PICK(ds[2]);
-  bool src_ok = true, dst_ok = true;
-  if (p.slot_side != MF_SLOT_NONE) {
-    const int64_t row = p.slot[int64_t(b) * p.N + n];
-    if (p.slot_side == MF_SLOT_SRC) {
-      src_ok = row >= 0;
-      so = row * MF_PICK(ss[2]);
-    } else {
-      dst_ok = row >= 0;
-      dst = row * MF_PICK(ds[2]);
-    }
-  }
-  so += h * MF_PICK(ss[1]);
-  dst += h * MF_PICK(ds[1]);
-  w.src = src_ok ? static_cast<const char*>(MF_PICK(src)) + so * ssize : nullptr;
-  w.dst = dst_ok ? static_cast<char*>(MF_PICK(dst)) + dst * dsize : nullptr;
-  w.turn = MF_PICK(turn);
-#undef MF_PICK
-  return w;
-}
-
-// Rows of 16-byte aligned chunks of 8 elements.
-template <typename TS, typename TD>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(Params p) {
-  __shared__ float2 table[kMaxTokens * kMaxPairs];
-  __shared__ __attribute__((aligned(16))) TS raw[kBlockChunks * 8];
-  const unsigned g0 = blockIdx.x * unsigned(p.TT);  // below 2^31 tokens
-  const int nt = min(p.TT, int(unsigned(p.B) * unsigned(p.N) - g0));
-  const First first = first_token(p, g0);
-  const int h0 = blockIdx.y * p.HS;
-  const int nh = min(p.HS, p.heads - h0);
-  const int DC = p.D >> 3;
-  const int total = nt * nh * DC;
-  const int rdc = (65536 + DC - 1) / DC, rnt = (65536 + nt - 1) / nt;
-  Chunk<TS> v[kChunks];
-  Where w[kChunks];
-  int col[kChunks];
-#pragma unroll
-  for (int k = 0; k < kChunks; ++k) {
-    const int i = threadIdx.x + k * kThreads;
-    if (i >= total) continue;
-    // i < 1024, DC <= 32, nt <= 16: the products with the reciprocals' ceilings below are exact quotients
-    const int r = (i * rdc) >> 16;
-    const int hh = (r * rnt) >> 16;
-    col[k] = (i - r * DC) * 8;
-    w[k] = locate(p, first, r - hh * nt, h0 + hh, sizeof(TS), sizeof(TD));
-    if (w[k].src) v[k].load(reinterpret_cast<const TS*>(w[k].src) + col[k]);
-    else v[k].clear();
-  }
-  fill_table(p, first, nt, table);
-  if (!p.interleaved) {
-#pragma unroll
-    for (int k = 0; k < kChunks; ++k) {
-      const int i = threadIdx.x + k * kThreads;
-      if (i < total) v[k].store(raw + i * 8);
-    }
+    const unsigned b = (g0 + t) / unsigned(p.N), n = g0 + t - b * unsigned(p.N);
+    table[i] = turn_of(p, b * p.ps[0] + n * p.ps[1] + (pr / per) * p.ps[2], int(pr));
   }
   __syncthreads();
-  const int P = p.R >> 1;
+  const int h0 = blockIdx.y * p.HS, h1 = min(p.heads, h0 + p.HS);
+  int base = 0;
 #pragma unroll
-  for (int k = 0; k < kChunks; ++k) {
-    const int i = threadIdx.x + k * kThreads;
-    if (i >= total || !w[k].dst) continue;
-    float x[8];
-    v[k].unpack(x);
-    if (w[k].turn && w[k].src) {
-      const float2* cs = table + w[k].t * P;
-      if (p.interleaved) {
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          if (col[k] + e < p.R) {
-            const float2 c = cs[(col[k] + e) >> 1];
-            const float a = x[e], b = x[e + 1];
-            x[e] = a * c.x - b * c.y;
-            x[e + 1] = a * c.y + b * c.x;
-          }
-        }
-      } else {
-        const TS* row = raw + (i * 8 - col[k]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int j = col[k] + e;
-          if (j < p.R) {
-            const bool first = j < P;
-            const float2 c = cs[first ? j : j - P];
-            const float o = Elem<TS>::to_f32(row[first ? j + P : j - P]);
-            x[e] = x[e] * c.x + o * (first ? -c.y : c.y);
-          }
-        }
+  for (int k = 0; k < 3; ++k) {
+    if (k >= p.nparts) break;
+    const Part& part = p.part[k];
+    const int lo = max(h0 - base, 0), hi = min(h1 - base, part.heads);
+    base += part.heads;
+    if (lo >= hi) continue;
+    const unsigned D = unsigned(p.D), total = nt * unsigned(hi - lo) * D;
+    for (unsigned i = threadIdx.x; i < total; i += kThreads) {
+      const unsigned r = i / D, h = r / nt, t = r - h * nt;
+      const int j = int(i - r * D);
+      const unsigned g = g0 + t, b = g / unsigned(p.N), n = g - b * unsigned(p.N);
+      const int64_t row = p.slot_side != MF_SLOT_NONE ? p.slot[g] : 0;
+      const bool zero = p.slot_side == MF_SLOT_SRC && row < 0;
+      if (p.slot_side == MF_SLOT_DST && row < 0) continue;
+      const TS* s = static_cast<const TS*>(part.src) + (lo + h) * part.ss[1] +
+                    (p.slot_side == MF_SLOT_SRC ? row * part.ss[2] : b * part.ss[0] + n * part.ss[2]);
+      TD* d = static_cast<TD*>(part.dst) + (lo + h) * part.ds[1] +
+              (p.slot_side == MF_SLOT_DST ? row * part.ds[2] : b * part.ds[0] + n * part.ds[2]);
+      float y = zero ? 0.0f : Elem<TS>::to_f32(s[j]);
+      if (part.turn && j < p.R && !zero) {
+        const int Pi = int(P);
+        const bool first = p.interleaved ? (j & 1) == 0 : j < Pi;
+        const int other = p.interleaved ? (j ^ 1) : first ? j + Pi : j - Pi;
+        const float2 c = table[t * P + (p.interleaved ? j >> 1 : first ? j : j - Pi)];
+        const float o = Elem<TS>::to_f32(s[other]);
+        y = y * c.x + o * (first ? -c.y : c.y);
       }
+      d[j] = Elem<TD>::from_f32(y);
     }
-    Chunk<TD> o;
-    o.pack(x);
-    o.store(reinterpret_cast<TD*>(w[k].dst) + col[k]);
-  }
-}
-
-// Any head_dim, strides and alignment: one element at a time.
-template <typename TS, typename TD>
-__global__ void __launch_bounds__(kThreads) rotary_scalar_kernel(Params p) {
-  __shared__ float2 table[kMaxTokens * kMaxPairs];
-  const unsigned g0 = blockIdx.x * unsigned(p.TT);  // below 2^31 tokens
-  const int nt = min(p.TT, int(unsigned(p.B) * unsigned(p.N) - g0));
-  const First first = first_token(p, g0);
-  const int h0 = blockIdx.y * p.HS;
-  const int nh = min(p.HS, p.heads - h0);
-  const int total = nt * nh * p.D;
-  fill_table(p, first, nt, table);
-  __syncthreads();
-  const int P = p.R >> 1;
-  for (int i = threadIdx.x; i < total; i += kThreads) {
-    const int r = i / p.D;
-    const int hh = r / nt;
-    const int j = i - r * p.D;
-    const Where w = locate(p, first, r - hh * nt, h0 + hh, sizeof(TS), sizeof(TD));
-    if (!w.dst) continue;
-    const TS* src = reinterpret_cast<const TS*>(w.src);
-    float y = src ? Elem<TS>::to_f32(src[j]) : 0.0f;
-    if (w.turn && j < p.R && src) {
-      const bool first = p.interleaved ? (j & 1) == 0 : j < P;
-      const int other = p.interleaved ? (j ^ 1) : first ? j + P : j - P;
-      const float2 c = table[w.t * P + (p.interleaved ? j >> 1 : first ? j : j - P)];
-      const float o = Elem<TS>::to_f32(src[other]);
-      y = y * c.x + o * (first ? -c.y : c.y);
-    }
-    reinterpret_cast<TD*>(w.dst)[j] = Elem<TD>::from_f32(y);
   }
 }
 
 template <typename TS, typename TD>
-void launch(bool vec, dim3 grid, hipStream_t s, const Params& p) {
-  if (vec) hipLaunchKernelGGL((rotary_kernel<TS, TD>), grid, dim3(kThreads), 0, s, p);
-  else hipLaunchKernelGGL((rotary_scalar_kernel<TS, TD>), grid, dim3(kThreads), 0, s, p);
+void launch(bool pieces, dim3 grid, hipStream_t s, const Params& p) {
+  if (!pieces) hipLaunchKernelGGL((rotary_scalar_kernel<TS, TD>), grid, dim3(kThreads), 0, s, p);
+  else if (p.interleaved) hipLaunchKernelGGL((rotary_kernel<TS, TD, true>), grid, dim3(kThreads), 0, s, p);
+  else hipLaunchKernelGGL((rotary_kernel<TS, TD, false>), grid, dim3(kThreads), 0, s, p);
 }
 
 template <typename TS>
-void launch_to(int dst, bool vec, dim3 grid, hipStream_t s, const Params& p) {
+void launch_to(int dst, bool pieces, dim3 grid, hipStream_t s, const Params& p) {
   switch (dst) {
-    case MF_DTYPE_BF16: launch<TS, __bf16>(vec, grid, s, p); break;
-    case MF_DTYPE_F16: launch<TS, _Float16>(vec, grid, s, p); break;
-    default: launch<TS, float>(vec, grid, s, p); break;
+    case MF_DTYPE_BF16: launch<TS, __bf16>(pieces, grid, s, p); break;
+    case MF_DTYPE_F16: launch<TS, _Float16>(pieces, grid, s, p); break;
+    default: launch<TS, float>(pieces, grid, s, p); break;
   }
 }
 
@@ -313,7 +311,7 @@ extern "C" int mf_rotary(const mf_rotary_args* a, void* stream) {
     return fail(MF_ERR_INVALID_ARGUMENT, "mf_rotary: positions and frequencies must be non-NULL");
   if (a->batch < 0 || a->tokens < 0 || a->head_dim <= 0)
     return fail(MF_ERR_INVALID_ARGUMENT, "mf_rotary: sizes must be non-negative (head_dim positive)");
-  if (a->head_dim > 2 * kMaxPairs) return fail(MF_ERR_UNSUPPORTED, "mf_rotary: head_dim must be at most 256");
+  if (a->head_dim > kMaxDim) return fail(MF_ERR_UNSUPPORTED, "mf_rotary: head_dim must be at most 256");
   if (a->axes < 1 || a->axes > 3) return fail(MF_ERR_INVALID_ARGUMENT, "mf_rotary: axes must be 1, 2 or 3");
   if (a->rotary_dim <= 0 || a->rotary_dim > a->head_dim || a->rotary_dim % (2 * a->axes) != 0)
     return fail(MF_ERR_INVALID_ARGUMENT, "mf_rotary: rotary_dim must be a positive multiple of 2 * axes, at most head_dim");
@@ -327,8 +325,6 @@ extern "C" int mf_rotary(const mf_rotary_args* a, void* stream) {
     return fail(MF_ERR_INVALID_ARGUMENT, "mf_rotary: a slot_side needs a slot map");
   if (!std::isfinite(a->gain)) return fail(MF_ERR_INVALID_ARGUMENT, "mf_rotary: gain must be finite");
   Params p = {};
-  const int ssize = a->src_dtype == MF_DTYPE_F32 ? 4 : 2, dsize = a->dst_dtype == MF_DTYPE_F32 ? 4 : 2;
-  bool vec = a->head_dim % 8 == 0;
   int64_t heads = 0;
   for (int k = 0; k < a->parts; ++k) {
     if (!a->src[k] || !a->dst[k]) return fail(MF_ERR_INVALID_ARGUMENT, "mf_rotary: every part needs src and dst");
@@ -339,12 +335,10 @@ extern "C" int mf_rotary(const mf_rotary_args* a, void* stream) {
     t.heads = a->heads[k];
     t.turn = a->turn[k];
     heads += t.heads;
-    vec = vec && reinterpret_cast<uintptr_t>(t.src) % 16 == 0 && reinterpret_cast<uintptr_t>(t.dst) % 16 == 0;
     for (int i = 0; i < 3; ++i) {
       t.ss[i] = a->src_stride[k][i];
       t.ds[i] = a->dst_stride[k][i];
       if (t.ss[i] < 0 || t.ds[i] < 0) return fail(MF_ERR_INVALID_ARGUMENT, "mf_rotary: strides must be non-negative");
-      vec = vec && t.ss[i] * ssize % 16 == 0 && t.ds[i] * dsize % 16 == 0;
     }
   }
   const int64_t tokens = int64_t(a->batch) * a->tokens;
@@ -367,22 +361,22 @@ extern "C" int mf_rotary(const mf_rotary_args* a, void* stream) {
   p.R = a->rotary_dim;
   p.interleaved = a->interleaved;
   p.heads = int(heads);
-  // Heads per workgroup: all that fit with one token; tokens: what fills the
-  // workgroup's chunks, fewer while the grid would leave CUs without work.
-  const int dc = (a->head_dim + 7) / 8;
-  p.HS = std::min(p.heads, kBlockChunks / dc);
-  const int slices = (p.heads + p.HS - 1) / p.HS;
-  p.HS = (p.heads + slices - 1) / slices;
-  int tt = std::min(kMaxTokens, kBlockChunks / (dc * p.HS));
-  while (tt > 1 && (tokens + tt - 1) / tt * slices < 512) tt = (tt + 1) / 2;
-  p.TT = tt;
-  const dim3 grid(unsigned((tokens + tt - 1) / tt), unsigned(slices));
-  if (grid.y > 65535) return fail(MF_ERR_UNSUPPORTED, "mf_rotary: too many heads");
+  const bool pieces = a->rotary_dim >= 16;
+  p.turned = (a->rotary_dim / 2 + 7) / 8;
+  p.units = p.turned + (a->head_dim - a->rotary_dim + 15) / 16;
+  p.TT = pieces ? kThreads / p.units : kScalarTokens;
+  // All heads in one workgroup, so that a token's angles are computed once; fewer while the grid would leave CUs
+  // without work (a molecule of 19 atoms and 16 heads is one workgroup else), but not below the heads in flight.
+  const int64_t blocks = (tokens + p.TT - 1) / p.TT;
+  int64_t slices = std::max<int64_t>(1, std::min<int64_t>((heads + kHeads - 1) / kHeads, 1024 / blocks));
+  p.HS = int((heads + slices - 1) / slices);
+  slices = (heads + p.HS - 1) / p.HS;
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(slices));
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (a->src_dtype) {
-    case MF_DTYPE_BF16: launch_to<__bf16>(a->dst_dtype, vec, grid, s, p); break;
-    case MF_DTYPE_F16: launch_to<_Float16>(a->dst_dtype, vec, grid, s, p); break;
-    default: launch_to<float>(a->dst_dtype, vec, grid, s, p); break;
+    case MF_DTYPE_BF16: launch_to<__bf16>(a->dst_dtype, pieces, grid, s, p); break;
+    case MF_DTYPE_F16: launch_to<_Float16>(a->dst_dtype, pieces, grid, s, p); break;
+    default: launch_to<float>(a->dst_dtype, pieces, grid, s, p); break;
   }
   MF_HIP_CHECK(hipGetLastError());
   return MF_OK;

@@ -27,9 +27,8 @@ def rotate64(x, positions, table, axes, gain, layout, *, inverse=False):
 def assert_turned(got, want, bound, what):
     """|got - want| <= bound * 7 * 2^-24 + half a step of got's dtype.
 
-    cos and sin come within 4 units in the last place (at most 2^-24 each below 1), the product with gain and the
-    correction of the angle's rounding add one more, and y = x0 c - x1 s rounds twice: in all
-    (|x0| + |x1|) gain (4 + 1 + 2) 2^-24.  Then one rounding to the output's type, half a step relative (or half the
+    cos and sin come within 4 units of 2^-24 (the rounded rest of the angle, their sums' cut and roundings), the product
+    with gain adds one more, and y = x0 c - x1 s rounds twice: in all (|x0| + |x1|) gain (4 + 1 + 2) 2^-24.  Then one rounding to the output's type, half a step relative (or half the
     smallest subnormal)."""
     fi = torch.finfo(got.dtype)
     tol = bound * 7 * 2.0 ** -24 + want.abs() * fi.eps / 2 * (1 + 2.0 ** -20) + fi.smallest_normal * fi.eps / 2
