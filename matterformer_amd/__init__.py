@@ -7,7 +7,9 @@ Public modules:
                                              matterformer.models.triton_simplicial_attention)
   matterformer_amd.attention / attention_triton / triton_regular_attention
                                              re-export shims of the reference
-  matterformer_amd.geometry_ops              kNN top-k, radius mask, radius attention
+  matterformer_amd.geometry_ops              kNN top-k, radius mask, radius attention (with gradients)
+  matterformer_amd.rotary                    rotary positions of heads or in_proj rows
+  matterformer_amd.gated_mlp                 gated linear layer (both projections, activation, product)
 The kernels live in libmf_hip.so (C ABI: include/mf_capi.h), built by
 ``python -m matterformer_amd.build``.
 
@@ -16,6 +18,11 @@ The package root exports lazily, so ``matterformer_amd.build`` can be imported
 """
 
 _LAZY = {
+    "RotaryFrequencies": "matterformer_amd.rotary",
+    "apply_rotary": "matterformer_amd.rotary",
+    "gated_linear": "matterformer_amd.gated_mlp",
+    "rotary_frequencies": "matterformer_amd.rotary",
+    "rotary_heads": "matterformer_amd.rotary",
     "SimplicialAttention": "matterformer_amd.simplicial_attention",
     "SimplicialAttentionMask": "matterformer_amd.simplicial_types",
     "SimplicialFactorizedBias": "matterformer_amd.simplicial_types",

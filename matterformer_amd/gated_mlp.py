@@ -79,7 +79,7 @@ class _GatedLinearFunction(torch.autograd.Function):
 def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
                  activation: str = "silu") -> torch.Tensor:
     """act(x Wg^T + bg) * (x Wu^T + bu): x (..., C); weight (2F, C), Wg its first F rows and Wu its last; bias (2F,) or
-    None; one dtype.  ``activation``: silu, gelu, gelu_tanh, relu or sigmoid.  Returns (..., F), differentiable in x,
+    None; one dtype (under autocast, its dtype).  ``activation``: silu, gelu, gelu_tanh, relu or sigmoid.  Returns (..., F), differentiable in x,
     weight and bias.  Sums, activation and product are fp32 on the GPU, rounded once."""
     if activation not in _native.MF_ACT:
         raise ValueError(f"Unsupported activation: {activation}; expected one of {ACTIVATIONS}")
@@ -89,6 +89,9 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
         raise ValueError(f"x must have shape (..., {weight.shape[1]}), got {tuple(x.shape)}")
     if bias is not None and bias.shape != weight.shape[:1]:
         raise ValueError(f"bias must have shape ({weight.shape[0]},), got {tuple(bias.shape)}")
+    if torch.is_autocast_enabled(x.device.type):
+        dtype = torch.get_autocast_dtype(x.device.type)
+        x, weight, bias = (t if t is None else t.to(dtype) for t in (x, weight, bias))
     if any(t is not None and (t.dtype != x.dtype or t.device != x.device) for t in (weight, bias)):
         raise RuntimeError("x, weight and bias must share a dtype and a device")
     if x.device.type != "cuda":

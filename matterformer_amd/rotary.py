@@ -126,7 +126,8 @@ def _check_positions(positions: torch.Tensor, batch: int, tokens: int, frequenci
     return positions
 
 
-def _check_layout(layout: str, head_dim: int, frequencies: RotaryFrequencies) -> bool:
+def check_layout(layout: str, head_dim: int, frequencies: RotaryFrequencies) -> bool:
+    """Whether the layout is the interleaved one, after the checks of both against the head."""
     if layout not in LAYOUTS:
         raise ValueError(f"Unsupported rotary layout: {layout}; expected one of {LAYOUTS}")
     if frequencies.rotary_dim > head_dim:
@@ -290,7 +291,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     if any(t.dtype != q.dtype or t.device != q.device for t in heads):
         raise RuntimeError("q and k must share a dtype and a device")
     B, _, N, D = q.shape
-    interleaved = _check_layout(layout, D, frequencies)
+    interleaved = check_layout(layout, D, frequencies)
     pos = _check_positions(positions, B, N, frequencies, q.device)
     if q.device.type != "cuda":
         out = [_rotate_torch(t, pos, frequencies, interleaved).contiguous() for t in heads]
@@ -301,20 +302,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     return (out[0], None) if k is None else (out[0], out[1])
 
 
-def _rows_torch(rows, pos, frequencies, interleaved, counts, head_dim, dtype):
-    """rows (B, N, columns) -> heads by torch expressions."""
-    B, N, _ = rows.shape
-    outs = []
-    for k, part in enumerate(rows.split([h * head_dim for h in counts], dim=-1)):
-        t = part.reshape(B, N, counts[k], head_dim).transpose(1, 2)
-        outs.append((_rotate_torch(t, pos, frequencies, interleaved) if k < 2 else t).to(dtype).contiguous())
-    return tuple(outs)
-
-
-def rotary_heads(rows: torch.Tensor, positions: torch.Tensor, frequencies: RotaryFrequencies, *, heads: int,
-                 kv_heads: int | None = None, layout: str = "half"):
-    """The heads of in_proj rows (B, N, (heads + 2 kv_heads) D), q and k turned as apply_rotary turns them: contiguous
-    q (B, heads, N, D), k and v (B, kv_heads, N, D), in one pass.  Differentiable in rows."""
+def _check_rows(rows, positions, frequencies, heads, kv_heads, layout):
     heads = int(heads)
     kv_heads = heads if kv_heads is None else int(kv_heads)
     if heads < 1 or kv_heads < 1:
@@ -323,11 +311,31 @@ def rotary_heads(rows: torch.Tensor, positions: torch.Tensor, frequencies: Rotar
         raise ValueError(f"rows must have shape (B, N, {heads + 2 * kv_heads} * head_dim), got {tuple(rows.shape)}")
     B, N, columns = rows.shape
     D = columns // (heads + 2 * kv_heads)
-    interleaved = _check_layout(layout, D, frequencies)
+    interleaved = check_layout(layout, D, frequencies)
     pos = _check_positions(positions, B, N, frequencies, rows.device)
-    counts = (heads, kv_heads, kv_heads)
+    return (heads, kv_heads, kv_heads), D, interleaved, pos
+
+
+def rotary_heads_torch(rows: torch.Tensor, positions: torch.Tensor, frequencies: RotaryFrequencies, *, heads: int,
+                       kv_heads: int | None = None, layout: str = "half"):
+    """rotary_heads by torch expressions, on any device."""
+    counts, D, interleaved, pos = _check_rows(rows, positions, frequencies, heads, kv_heads, layout)
+    B, N, _ = rows.shape
+    outs = []
+    for k, part in enumerate(rows.split([h * D for h in counts], dim=-1)):
+        t = part.reshape(B, N, counts[k], D).transpose(1, 2)
+        outs.append((_rotate_torch(t, pos, frequencies, interleaved) if k < 2 else t).contiguous())
+    return tuple(outs)
+
+
+def rotary_heads(rows: torch.Tensor, positions: torch.Tensor, frequencies: RotaryFrequencies, *, heads: int,
+                 kv_heads: int | None = None, layout: str = "half"):
+    """The heads of in_proj rows (B, N, (heads + 2 kv_heads) D), q and k turned as apply_rotary turns them: contiguous
+    q (B, heads, N, D), k and v (B, kv_heads, N, D), in one pass.  Differentiable in rows."""
     if rows.device.type != "cuda":
-        return _rows_torch(rows, pos, frequencies, interleaved, counts, D, rows.dtype)
+        return rotary_heads_torch(rows, positions, frequencies, heads=heads, kv_heads=kv_heads, layout=layout)
+    counts, D, interleaved, pos = _check_rows(rows, positions, frequencies, heads, kv_heads, layout)
+    B, N, _ = rows.shape
     _check_kernel(D, rows.dtype)
     run = _RowsFunction.apply if _native.takes_gradient(rows) else _rows_to_heads
     return run(_Plan(pos, frequencies, interleaved), rows, counts, B, N, D, rows.dtype)
@@ -344,7 +352,7 @@ def _packed_rotary_heads(rows: torch.Tensor, slot: torch.Tensor, positions: torc
         raise ValueError(f"rows must have shape (T, {3 * heads * head_dim}) and slot hold {B * W} int32 entries")
     if rows.device.type != "cuda" or slot.device != rows.device:
         raise RuntimeError("packed rotary heads need CUDA (ROCm) tensors on one device")
-    interleaved = _check_layout(layout, head_dim, frequencies)
+    interleaved = check_layout(layout, head_dim, frequencies)
     pos = _check_positions(positions, B, W, frequencies, rows.device)
     _check_kernel(head_dim, rows.dtype)
     _check_kernel(head_dim, dtype)

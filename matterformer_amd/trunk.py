@@ -32,6 +32,8 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from matterformer_amd.gated_mlp import ACTIVATIONS, gated_linear
+from matterformer_amd.rotary import RotaryFrequencies, check_layout, rotary_heads, rotary_heads_torch
 from matterformer_amd.simplicial_attention import SimplicialAttention
 from matterformer_amd.simplicial_types import SimplicialAttentionMask, coerce_attention_mask
 from matterformer_amd.token_packing import TokenPacking, adaln_rows
@@ -44,18 +46,26 @@ def _modulate(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor) -> torc
 
 
 class Mlp(nn.Module):
-    """fc1 -> tanh-GELU -> fc2 (transformer.py:129-148)."""
+    """fc1 -> tanh-GELU -> fc2 (transformer.py:129-148).  With ``gate`` (an activation of gated_mlp) the gated form:
+    fc1 holds the gate's and the up projection's rows (2 hidden of them) and fc2 reads act(gate) * up, one kernel
+    (gated_linear) with its gradients on the GPU."""
 
-    def __init__(self, d_model: int, mlp_ratio: float = 4.0, dropout: float = 0.0) -> None:
+    def __init__(self, d_model: int, mlp_ratio: float = 4.0, dropout: float = 0.0, gate: str | None = None) -> None:
         super().__init__()
         hidden = int(d_model * mlp_ratio)
-        self.fc1 = nn.Linear(d_model, hidden)
-        self.act = nn.GELU(approximate="tanh")
+        if gate is not None and gate not in ACTIVATIONS:
+            raise ValueError(f"Unsupported mlp gate: {gate}; expected one of {ACTIVATIONS}")
+        self.gate = gate
+        self.fc1 = nn.Linear(d_model, hidden if gate is None else 2 * hidden)
+        self.act = nn.GELU(approximate="tanh") if gate is None else None
         self.drop1 = nn.Dropout(dropout)
         self.fc2 = nn.Linear(hidden, d_model)
         self.drop2 = nn.Dropout(dropout)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.gate is not None:
+            h = gated_linear(x, self.fc1.weight, self.fc1.bias, activation=self.gate)
+            return self.drop2(self.fc2(self.drop1(h)))
         if self._fused_gelu_ok(x):
             # fc1 with the tanh-GELU in the GEMM epilogue (hipBLASLt), applied to the fp32 accumulator
             h = torch._addmm_activation(self.fc1.bias, x, self.fc1.weight.t(), use_gelu=True)
@@ -105,13 +115,23 @@ def knn_allowed_torch(idx: torch.Tensor, pad_mask: torch.Tensor | None) -> torch
 
 class KnnLocalMask:
     """The local blocks' mask, built once per forward: kNN lists plus bit / block masks (GPU) or the
-    boolean matrix (CPU)."""
+    boolean matrix (CPU); the coordinates they were built from, which rotary blocks turn by."""
 
-    def __init__(self, idx: torch.Tensor, bits=None, blocks=None, allowed=None):
+    def __init__(self, idx: torch.Tensor, bits=None, blocks=None, allowed=None, positions=None):
         self.idx = idx
         self.bits = bits
         self.blocks = blocks
         self.allowed = allowed
+        self.positions = positions
+        self._tables = None
+
+    def tables(self):
+        """radius_tables of the mask, made by the first block that takes gradients and shared by the others."""
+        if self._tables is None:
+            from matterformer_amd.geometry_ops import radius_tables
+
+            self._tables = radius_tables(self.bits, self.blocks)
+        return self._tables
 
 
 def build_knn_mask(coords: torch.Tensor, k: int, pad_mask: torch.Tensor | None, *, use_hip: bool) -> KnnLocalMask:
@@ -120,17 +140,34 @@ def build_knn_mask(coords: torch.Tensor, k: int, pad_mask: torch.Tensor | None, 
 
         idx = knn_graph(coords, k, pad_mask, exclude_self=True, return_dist=False)
         bits, blocks = knn_mask(idx, pad_mask, include_self=True)
-        return KnnLocalMask(idx, bits=bits, blocks=blocks)
+        return KnnLocalMask(idx, bits=bits, blocks=blocks, positions=coords.float())
     idx = knn_lists_torch(coords, k, pad_mask)
-    return KnnLocalMask(idx, allowed=knn_allowed_torch(idx, pad_mask))
+    return KnnLocalMask(idx, allowed=knn_allowed_torch(idx, pad_mask), positions=coords.float())
 
 
 class KnnLocalAttention(nn.Module):
     """MHA of every atom over its kNN mask.  Parameters are nn.MultiheadAttention's, held as ``attn``
-    like the reference's RegularAttention (regular_attention.py:275-338), so state dicts match."""
+    like the reference's RegularAttention (regular_attention.py:275-338), so state dicts match.
 
-    def __init__(self, d_model: int, n_heads: int, *, dropout: float = 0.0, impl: str = "auto") -> None:
+    ``rotary`` (RotaryFrequencies of three axes) turns q and k by the atoms' coordinates, as the reference's
+    RotaryMultiheadAttention does (regular_attention.py:112-271), here with any table of frequencies; a logit then
+    depends on the atoms' difference vector.  The coordinates take no gradient there: under autograd they are refused
+    when they ask for one.  ``hip_backward``: autograd follows the HIP kernels where the
+    projections are 16-bit (radius_attention's and rotary_heads' gradients); otherwise training takes the torch
+    path, as fp32 projections always do."""
+
+    def __init__(self, d_model: int, n_heads: int, *, dropout: float = 0.0, impl: str = "auto",
+                 rotary: RotaryFrequencies | None = None, rotary_layout: str = "half",
+                 hip_backward: bool = False) -> None:
         super().__init__()
+        if rotary is not None:
+            if rotary.axes != 3:
+                raise ValueError(f"local attention turns by three coordinates: rotary.axes must be 3, got {rotary.axes}")
+            check_layout(rotary_layout, d_model // n_heads, rotary)
+        self.rotary = rotary
+        self.rotary_layout = rotary_layout
+        self.hip_backward = bool(hip_backward)
+        self._rotary_on: dict = {}  # device -> rotary there
         impl = impl.lower()
         if impl == "hip":
             impl = "triton"
@@ -146,8 +183,11 @@ class KnnLocalAttention(nn.Module):
         if self.training and self.attn.dropout > 0.0:
             return "the HIP local attention does not support attention dropout in training mode"
         if torch.is_grad_enabled() and (h.requires_grad or any(p.requires_grad for p in self.attn.parameters())):
-            # mf_radius_attn is a forward kernel with no autograd Function: the torch path keeps the graph
-            return "the HIP local attention has no backward; autograd takes the torch path"
+            if not self.hip_backward:
+                return "the HIP local attention has no backward; autograd takes the torch path"
+            dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else h.dtype
+            if dtype not in (torch.bfloat16, torch.float16):
+                return "the HIP local attention's backward needs float16/bfloat16 projections"
         head_dim = self.attn.embed_dim // self.attn.num_heads
         if head_dim not in (32, 64, 128):
             return f"the HIP local attention supports head_dim 32, 64 or 128, got {head_dim}"
@@ -161,10 +201,31 @@ class KnnLocalAttention(nn.Module):
             raise RuntimeError(reason)
         return reason is None
 
+    def _core_dtype(self, h: torch.Tensor, rows: torch.Tensor) -> torch.dtype:
+        """The 16-bit type of the attention core: the block's input's, or, under autograd and in rotary blocks, the
+        projections' (which differ under autocast)."""
+        dtype = rows.dtype if self.hip_backward or self.rotary is not None else h.dtype
+        return dtype if dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
+
+    def _rotary(self, device: torch.device) -> RotaryFrequencies:
+        if device not in self._rotary_on:
+            self._rotary_on[device] = self.rotary.to(device)
+        return self._rotary_on[device]
+
+    def _positions(self, mask: KnnLocalMask) -> torch.Tensor:
+        if mask.positions is None:
+            raise ValueError("rotary local attention needs the mask's positions (build_knn_mask keeps them)")
+        return mask.positions
+
+    def _attend(self, q, k, v, mask: KnnLocalMask) -> torch.Tensor:
+        from matterformer_amd.geometry_ops import radius_attention
+
+        grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+        return radius_attention(q, k, v, mask.bits, mask.blocks, scale=q.shape[-1] ** -0.5,
+                                tables=mask.tables() if grad else None)
+
     def forward(self, h: torch.Tensor, mask: KnnLocalMask, pad_mask: torch.Tensor | None = None) -> torch.Tensor:
         if self._use_hip(h):
-            from matterformer_amd.geometry_ops import radius_attention
-
             if mask.bits is None:
                 raise RuntimeError("the HIP local attention needs the kNN bit mask (build_knn_mask(use_hip=True))")
             self._last_impl_used = "triton"
@@ -173,9 +234,13 @@ class KnnLocalAttention(nn.Module):
             H = mha.num_heads
             D = C // H
             qkv = F.linear(h, mha.in_proj_weight, mha.in_proj_bias)
-            cdt = h.dtype if h.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
-            q, k, v = (t.reshape(B, T, H, D).transpose(1, 2).to(cdt).contiguous() for t in qkv.chunk(3, dim=-1))
-            out = radius_attention(q, k, v, mask.bits, mask.blocks, scale=D ** -0.5)
+            cdt = self._core_dtype(h, qkv)
+            if self.rotary is not None:
+                q, k, v = rotary_heads(qkv.to(cdt), self._positions(mask), self._rotary(h.device), heads=H,
+                                       layout=self.rotary_layout)
+            else:
+                q, k, v = (t.reshape(B, T, H, D).transpose(1, 2).to(cdt).contiguous() for t in qkv.chunk(3, dim=-1))
+            out = self._attend(q, k, v, mask)
             out = out.transpose(1, 2).reshape(B, T, C).to(h.dtype)
             return F.linear(out, mha.out_proj.weight, mha.out_proj.bias)
         self._last_impl_used = "torch"
@@ -187,21 +252,34 @@ class KnnLocalAttention(nn.Module):
             raise RuntimeError("packed local attention runs on the HIP kernels only")
         if mask.bits is None:
             raise RuntimeError("the HIP local attention needs the kNN bit mask (build_knn_mask(use_hip=True))")
-        from matterformer_amd.geometry_ops import radius_attention
-
         self._last_impl_used = "triton"
         mha = self.attn
         H = mha.num_heads
         D = hp.shape[-1] // H
-        cdt = hp.dtype if hp.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
-        qkv = packing.to_heads(F.linear(hp, mha.in_proj_weight, mha.in_proj_bias), 3, H, D, cdt)
-        out = radius_attention(qkv[0], qkv[1], qkv[2], mask.bits, mask.blocks, scale=D ** -0.5)
+        rows = F.linear(hp, mha.in_proj_weight, mha.in_proj_bias)
+        cdt = self._core_dtype(hp, rows)
+        if self.rotary is not None:
+            qkv = packing.to_rotary_heads(rows, H, D, cdt, self._positions(mask), self._rotary(hp.device),
+                                          self.rotary_layout)
+        else:
+            qkv = packing.to_heads(rows, 3, H, D, cdt)
+        out = self._attend(qkv[0], qkv[1], qkv[2], mask)
         return F.linear(packing.from_heads(out, hp.dtype), mha.out_proj.weight, mha.out_proj.bias)
 
     def _forward_torch(self, h: torch.Tensor, mask: KnnLocalMask, pad_mask: torch.Tensor | None) -> torch.Tensor:
         allowed = mask.allowed if mask.allowed is not None else knn_allowed_torch(mask.idx, pad_mask)
         B, T, _ = h.shape
         H = self.attn.num_heads
+        if self.rotary is not None:
+            # the same mask on turned heads; a padded query keeps itself, as below
+            allowed = allowed | torch.eye(T, dtype=torch.bool, device=h.device)[None]
+            rows = F.linear(h, self.attn.in_proj_weight, self.attn.in_proj_bias)
+            q, k, v = rotary_heads_torch(rows, self._positions(mask), self._rotary(h.device), heads=H,
+                                         layout=self.rotary_layout)
+            out = F.scaled_dot_product_attention(q, k, v, attn_mask=allowed[:, None],
+                                                 dropout_p=self.attn.dropout if self.training else 0.0)
+            out = out.transpose(1, 2).reshape(B, T, -1)
+            return F.linear(out, self.attn.out_proj.weight, self.attn.out_proj.bias)
         # the reference's attn_head_bias route (transformer.py:256-268): 0 / -inf, padded keys at finfo.min;
         # a padded query keeps itself so its softmax row is defined (its output is never read by valid rows)
         allowed = allowed | torch.eye(T, dtype=torch.bool, device=h.device)[None]
@@ -296,6 +374,10 @@ class AdaLNBlock(nn.Module):
         local_impl: str = "auto",
         use_adaln_conditioning: bool = True,
         norm_affine_when_no_adaln: bool = False,
+        mlp_gate: str | None = None,
+        local_rotary: RotaryFrequencies | None = None,
+        local_rotary_layout: str = "half",
+        local_hip_backward: bool = False,
     ) -> None:
         super().__init__()
         attn_type = attn_type.lower()
@@ -315,14 +397,16 @@ class AdaLNBlock(nn.Module):
         else:
             self.ada_ln = None
         if attn_type == "knn_local":
-            self.attn = KnnLocalAttention(d_model, self.n_heads, dropout=attn_dropout, impl=local_impl)
+            self.attn = KnnLocalAttention(d_model, self.n_heads, dropout=attn_dropout, impl=local_impl,
+                                          rotary=local_rotary, rotary_layout=local_rotary_layout,
+                                          hip_backward=local_hip_backward)
         else:
             self.attn = SimplicialAttention(
                 dim=d_model, num_heads=self.n_heads, head_dim=simplicial_head_dim, dropout=attn_dropout,
                 chunk_size=simplicial_chunk_size, bias=True, out_proj=True, impl=simplicial_impl,
                 precision=simplicial_precision, message_mode=simplicial_message_mode,
                 message_rank=simplicial_message_rank, content_logits=simplicial_content_logits)
-        self.mlp = Mlp(d_model=d_model, mlp_ratio=mlp_ratio, dropout=dropout)
+        self.mlp = Mlp(d_model=d_model, mlp_ratio=mlp_ratio, dropout=dropout, gate=mlp_gate)
 
     def forward(self, x: torch.Tensor, cond_emb: torch.Tensor | None, pad_mask: torch.Tensor | None = None, *,
                 knn_mask: KnnLocalMask | None = None,
@@ -385,14 +469,18 @@ class AdaLNBlock(nn.Module):
 
 
 class AlternatingTrunk(nn.Module):
-    """n_layers AdaLN blocks, simplicial on even and kNN-local (k = knn_k) on odd layers by default."""
+    """n_layers AdaLN blocks, simplicial on even and kNN-local (k = knn_k) on odd layers by default.  ``mlp_gate``: the
+    blocks' MLPs gated by that activation (Mlp); ``local_rotary``, ``local_rotary_layout``, ``local_hip_backward``: the
+    local blocks' rotary positions and training on the HIP kernels (KnnLocalAttention)."""
 
     def __init__(self, d_model: int = 512, n_heads: int = 8, n_layers: int = 12, *, mlp_ratio: float = 4.0,
                  knn_k: int = 32, schedule: list[str] | None = None, simplicial_impl: str = "auto",
                  simplicial_precision: str = "bf16_tc", simplicial_message_mode: str = "none",
                  simplicial_message_rank: int = 16, simplicial_content_logits: str = "on", local_impl: str = "auto",
                  eps: float = 1e-6, use_adaln_conditioning: bool = True, geometry_adapter: nn.Module | None = None,
-                 simplicial_geometry_bias: nn.Module | None = None, pack_tokens: bool = True) -> None:
+                 simplicial_geometry_bias: nn.Module | None = None, pack_tokens: bool = True,
+                 mlp_gate: str | None = None, local_rotary: RotaryFrequencies | None = None,
+                 local_rotary_layout: str = "half", local_hip_backward: bool = False) -> None:
         super().__init__()
         self.pack_tokens = bool(pack_tokens)
         # registered before the blocks, as in TransformerTrunk.__init__ (transformer.py:1137-1139)
@@ -409,7 +497,8 @@ class AlternatingTrunk(nn.Module):
                        simplicial_precision=simplicial_precision, simplicial_message_mode=simplicial_message_mode,
                        simplicial_message_rank=simplicial_message_rank,
                        simplicial_content_logits=simplicial_content_logits, local_impl=local_impl,
-                       use_adaln_conditioning=use_adaln_conditioning)
+                       use_adaln_conditioning=use_adaln_conditioning, mlp_gate=mlp_gate, local_rotary=local_rotary,
+                       local_rotary_layout=local_rotary_layout, local_hip_backward=local_hip_backward)
             for t in self.schedule])
 
     def _use_hip(self, x: torch.Tensor) -> bool:

@@ -1,0 +1,156 @@
+"""The rotary local block with a gated MLP as it is used: trunks of local and simplicial blocks, padded and packed, in
+inference and training, against the same trunk in float64 on the CPU.
+
+Bars: every operation of a block rounds to bf16, off by at most 2^-8 and by 2^-8 / sqrt(3) in the mean square; about 15
+roundings lie between a block's input and its output, so two blocks leave sqrt(30) 2^-8 / sqrt(3) = 1.2e-2 of the norm
+(bar 2e-2, that of the trunk's other bf16 tests), and a gradient passes as many again: sqrt(60) 2^-8 / sqrt(3) = 1.7e-2,
+times three for sums that cancel (a bias's over tokens): 5e-2."""
+
+import copy
+
+import pytest
+import torch
+
+from matterformer_amd.rotary import rotary_frequencies
+from matterformer_amd.token_packing import TokenPacking
+from matterformer_amd.trunk import AlternatingTrunk
+
+pytestmark = pytest.mark.gpu
+
+
+def build(schedule, *, d=128, heads=2, gate="silu", layout="half", axes_dim=60, seed=0, dtype=torch.bfloat16):
+    torch.manual_seed(seed)
+    trunk = AlternatingTrunk(d, heads, len(schedule), knn_k=8, schedule=schedule, mlp_gate=gate, mlp_ratio=2.0,
+                             local_rotary=rotary_frequencies(axes_dim, axes=3, base=30.0), local_rotary_layout=layout,
+                             local_hip_backward=True, simplicial_precision="bf16_tc")
+    for block in trunk.blocks:
+        torch.nn.init.normal_(block.ada_ln[-1].weight, std=0.05)
+        torch.nn.init.normal_(block.ada_ln[-1].bias, std=0.3)
+    return trunk.to(dtype)
+
+
+def inputs(B=3, N=40, d=128, seed=1):
+    gen = torch.Generator().manual_seed(seed)
+    counts = torch.tensor([N, 7, 23][:B])
+    pad = torch.arange(N)[None] >= counts[:, None]
+    x = torch.randn(B, N, d, generator=gen).to(torch.bfloat16)
+    cond = torch.randn(B, d, generator=gen).to(torch.bfloat16)
+    coords = torch.randn(B, N, 3, generator=gen) * 1.4
+    weight = torch.randn(B, N, d, generator=gen).to(torch.bfloat16)
+    return x, cond, coords, pad, weight
+
+
+def reference(trunk, x, cond, coords, pad, weight):
+    ref = copy.deepcopy(trunk).cpu().double()
+    leaf = x.double().requires_grad_(True)
+    out = ref(leaf, cond.double(), coords, pad)
+    (out * weight.double()).sum().backward()
+    return out.detach(), leaf.grad, {n: p.grad for n, p in ref.named_parameters()}
+
+
+def rel(got, want):
+    return float((got.detach().cpu().double() - want).norm() / want.norm())
+
+
+@pytest.mark.parametrize("schedule,layout,gate", [(["knn_local", "knn_local"], "half", "silu"),
+                                                  (["simplicial", "knn_local"], "interleaved", "gelu_tanh")])
+@pytest.mark.parametrize("packed", [False, True])
+def test_forward_and_training(cuda, schedule, layout, gate, packed):
+    trunk = build(schedule, layout=layout, gate=gate)
+    x, cond, coords, pad, weight = inputs()
+    want, want_dx, want_grads = reference(trunk, x, cond, coords, pad, weight)
+    trunk = trunk.to(cuda)
+    trunk.pack_tokens = packed
+    args = [t.to(cuda) for t in (cond, coords, pad)]
+    with torch.no_grad():
+        assert trunk.packable(x.to(cuda)) == packed
+        out = trunk(x.to(cuda), *args)
+    assert rel(out, want) <= 2e-2
+    assert torch.equal(out[pad.to(cuda)], torch.zeros_like(out[pad.to(cuda)]))
+    leaf = x.to(cuda).requires_grad_(True)
+    out = trunk(leaf, *args)
+    (out.float() * weight.to(cuda).float()).sum().backward()
+    torch.cuda.synchronize()
+    assert all(b.attn._last_impl_used == "triton" for b in trunk.blocks)
+    assert rel(out, want) <= 2e-2
+    assert rel(leaf.grad, want_dx) <= 5e-2
+    for name, param in trunk.named_parameters():
+        if want_grads[name] is None:
+            continue
+        # a key bias shifts a row's logits alike: its gradient is zero but for rounding
+        if name.endswith("in_proj_bias") or name.endswith("in_proj.bias"):
+            scale = want_grads[name].norm()
+            assert float((param.grad.cpu().double() - want_grads[name]).norm()) <= 5e-2 * float(scale), name
+            continue
+        assert rel(param.grad, want_grads[name]) <= 5e-2, name
+
+
+def test_packed_equals_padded(cuda):
+    """The same rows through both layouts: attention cores see the same operands, so only the summation of the linears
+    differs, and with it the bf16 roundings."""
+    trunk = build(["knn_local", "knn_local"]).to(cuda)
+    x, cond, coords, pad, _ = (t.to(cuda) for t in inputs())
+    with torch.no_grad():
+        packed = trunk(x, cond, coords, pad)
+        trunk.pack_tokens = False
+        padded = trunk(x, cond, coords, pad)
+    assert rel(packed, padded.cpu().double()) <= 2e-2
+
+
+def test_float32_training_takes_the_torch_path(cuda):
+    trunk = build(["knn_local", "knn_local"], dtype=torch.float32)
+    x, cond, coords, pad, weight = inputs()
+    want, want_dx, want_grads = reference(trunk, x, cond, coords, pad, weight)
+    trunk = trunk.to(cuda)
+    leaf = x.to(cuda).float().requires_grad_(True)
+    out = trunk(leaf, cond.to(cuda).float(), coords.to(cuda), pad.to(cuda))
+    (out * weight.to(cuda).float()).sum().backward()
+    assert all(b.attn._last_impl_used == "torch" for b in trunk.blocks)
+    # fp32 sums of at most a few hundred terms over two blocks, forward and back
+    assert rel(out, want) <= 1e-4 and rel(leaf.grad, want_dx) <= 1e-4
+    for name, param in trunk.named_parameters():
+        if want_grads[name] is not None:
+            assert rel(param.grad, want_grads[name]) <= 1e-3, name
+
+
+def test_autocast_training_runs_the_kernels(cuda):
+    trunk = build(["knn_local", "knn_local"], dtype=torch.float32)
+    x, cond, coords, pad, weight = inputs()
+    want, want_dx, _ = reference(trunk, x, cond, coords, pad, weight)
+    trunk = trunk.to(cuda)
+    leaf = x.to(cuda).float().requires_grad_(True)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        out = trunk(leaf, cond.to(cuda).float(), coords.to(cuda), pad.to(cuda))
+    (out.float() * weight.to(cuda).float()).sum().backward()
+    assert all(b.attn._last_impl_used == "triton" for b in trunk.blocks)
+    assert rel(out, want) <= 2e-2 and rel(leaf.grad, want_dx) <= 5e-2
+
+
+def test_coordinates_that_ask_for_a_gradient_are_refused(cuda):
+    trunk = build(["knn_local"]).to(cuda)
+    x, cond, coords, pad, _ = (t.to(cuda) for t in inputs())
+    with pytest.raises(RuntimeError, match="no gradient"):
+        trunk(x, cond, coords.requires_grad_(True), pad)
+
+
+def test_captured_inference(cuda):
+    trunk = build(["knn_local", "knn_local"]).to(cuda).eval()
+    x, cond, coords, pad, _ = (t.to(cuda) for t in inputs())
+    packing = TokenPacking(pad)
+    gen = torch.Generator().manual_seed(9)
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(2):
+                trunk(x, cond, coords, pad, packing=packing)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = trunk(x, cond, coords, pad, packing=packing)
+        for turn in range(3):
+            x.copy_(torch.randn(x.shape, generator=gen).to(torch.bfloat16))
+            coords.copy_(torch.randn(coords.shape, generator=gen))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(held, trunk(x, cond, coords, pad, packing=packing)), f"replay {turn}"
