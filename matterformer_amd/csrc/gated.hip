@@ -536,6 +536,80 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
   }
 }
 
+// The forward of few tokens (N <= 16 NT <= 64): the weights are read once, straight into the matrix operands, and the
+// tile kernel's copies and barriers would only add to the latency.  A workgroup owns 16 hidden columns (their gate and
+// up rows); its four waves take a quarter of K each and meet in LDS.
+template <typename T, int NT>
+__global__ void __launch_bounds__(256) few_kernel(Params p) {
+  using Frag = typename Mma<T>::Frag;
+  constexpr int E = kEpc<T>, KS = 4 * E;  // K entries of a fragment's four lane groups
+  constexpr int kAhead = NT == 4 ? 2 : 4;  // steps in flight
+  __shared__ mf_f32x4 part[4][2][NT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int g = lane >> 4, r16 = lane & 15;
+  const int f0 = blockIdx.x * 16;
+  const int fr = min(f0 + r16, p.F - 1);  // rows past the end repeat the last: their results are not stored
+  const T* wg = reinterpret_cast<const T*>(p.a + int64_t(fr) * p.lda) + g * E;
+  const T* wu = reinterpret_cast<const T*>(p.a + (int64_t(p.F) + fr) * p.lda) + g * E;
+  const T* x[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+    x[i] = reinterpret_cast<const T*>(p.b + int64_t(min(16 * i + r16, p.N - 1)) * p.ldb) + g * E;
+  mf_f32x4 acc[2][NT];
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int i = 0; i < NT; ++i) acc[q][i] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
+  const int steps = (p.K + KS - 1) / KS;
+  const int quarter = (steps + 3) / 4;
+  const int s1 = min(steps, (wave + 1) * quarter);
+  for (int s = wave * quarter; s < s1; s += kAhead) {
+    Frag a[kAhead], u[kAhead], b[kAhead][NT];
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d) {
+      const int k = (s + d) * KS;
+      const bool in = s + d < s1 && k + g * E < p.K;  // K is a multiple of E
+      // (one zero on each side: what lies behind a row could be NaN)
+      Frag zero = {};
+      a[d] = in ? *reinterpret_cast<const Frag*>(wg + k) : zero;
+      u[d] = in ? *reinterpret_cast<const Frag*>(wu + k) : zero;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) b[d][i] = in ? *reinterpret_cast<const Frag*>(x[i] + k) : zero;
+    }
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        Mma<T>::run(a[d], b[d][i], acc[0][i]);
+        Mma<T>::run(u[d], b[d][i], acc[1][i]);
+      }
+  }
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int i = 0; i < NT; ++i) part[wave][q][i][lane] = acc[q][i];
+  __syncthreads();
+  // wave i finishes tokens 16 i ..: lane (g, r16) holds columns 4 g .. + 3 of token 16 i + r16
+  const int i = wave, n = 16 * i + r16;
+  if (i >= NT || n >= p.N) return;
+  const T* bias = static_cast<const T*>(p.bias);
+  with_activation(p.act, [&](auto act) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int f = f0 + 4 * g + r;
+      if (f >= p.F) break;
+      float a = bias ? Elem<T>::to_f32(bias[f]) : 0.0f, b = bias ? Elem<T>::to_f32(bias[p.F + f]) : 0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        a += part[w][0][i][lane][r];
+        b += part[w][1][i][lane][r];
+      }
+      static_cast<T*>(p.out)[int64_t(n) * p.ldo + f] =
+          Elem<T>::from_f32(act_value<decltype(act)::value, sizeof(T) == 2>(a) * b);
+    }
+  });
+}
+
 // The tail tiles' outputs: each the sum of its splits, in order.  Four columns a thread.
 template <typename T, int MODE>
 __global__ void __launch_bounds__(256) tail_kernel(Params p, int bm, int bn) {
@@ -605,6 +679,7 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 // and adding the pieces' fp32 sums.
 struct Cut {
   bool large;
+  int bn;  // columns of a tile: 256 (large), 128 or 64
   int full, tail, splits, steps;
   size_t bytes;
 };
@@ -612,6 +687,7 @@ Cut cut_tiles(int64_t m, int64_t n, int64_t k, int esize, bool large, bool split
   Cut c;
   c.large = large;
   const int b = large ? 256 : 128;
+  c.bn = b;
   const int64_t tiles = ((m + b - 1) / b) * ((n + b - 1) / b);
   const int64_t slots = large ? num_cus : 2 * num_cus;
   const int64_t steps = (k * esize + kRowBytes - 1) / kRowBytes;
@@ -625,13 +701,19 @@ Cut cut_tiles(int64_t m, int64_t n, int64_t k, int esize, bool large, bool split
   c.bytes = round256(size_t(c.tail) * c.splits * b * b * 4);
   return c;
 }
+constexpr int kFewTokens = 64;  // the forward of few_kernel
 // kFwd and kBwd: large tiles when every CU gets one.  fp32, whose matrix rate is a sixteenth, takes small ones.
 Cut cut_gated(int64_t f, int64_t t, int64_t k, int esize, int num_cus) {
   const bool large = esize == 2 && ((2 * f + 255) / 256) * ((t + 255) / 256) >= num_cus;
   // a large tile is 128 of f and their gate and up rows, a small one 64
   Cut c = cut_tiles(2 * f, t, k, esize, large, false, num_cus);
   const int64_t fb = large ? 128 : 64;
-  c.full = int(((f + fb - 1) / fb) * ((t + 2 * fb - 1) / (2 * fb)));
+  auto tiles = [&](int64_t bn) { return (f + fb - 1) / fb * ((t + bn - 1) / bn); };
+  // fp32 products fill the matrix cores from one workgroup, so what counts is the tiles of the busiest CU: half as wide
+  // ones where those add up to less (2432 rows, 1024 hidden: 3 of 64 columns instead of 2 of 128, 58 -> 47 us)
+  auto busiest = [&](int64_t bn) { return (tiles(bn) + num_cus - 1) / num_cus * bn; };
+  if (esize == 4 && busiest(64) < busiest(128)) c.bn = 64;
+  c.full = int(tiles(c.bn));
   return c;
 }
 // kDx and kDw: large tiles when their K pieces can fill the CUs with at least 16 steps each.
@@ -664,9 +746,9 @@ void make_plan(Plan* q, int64_t T, int64_t C, int64_t F, int64_t x_stride, const
   q->x_bytes = q->pad_x ? round256(size_t(T) * q->Cp * q->esize) : 0;
   q->w_bytes = q->pad_w ? round256(size_t(2) * F * q->Cp * q->esize) : 0;
   q->dab_bytes = need_dx || need_dw ? round256(size_t(T) * 2 * q->Fp * q->esize) : 0;
-  // bias sums of every column wave: 128-row tiles have 4 waves of 32, 256-row tiles 4 of 64
-  q->bias_bytes = need_db ? round256(size_t((T + 127) / 128) * 4 * 2 * q->Fp * 4) : 0;
   q->gated = cut_gated(F, T, q->Cp, q->esize, num_cus);
+  // bias sums of every column wave, four a tile
+  q->bias_bytes = need_db ? round256(size_t((T + q->gated.bn - 1) / q->gated.bn) * 4 * 2 * q->Fp * 4) : 0;
   q->dx = cut_product(q->Cp, T, 2 * q->Fp, q->esize, num_cus);
   q->dw = cut_product(q->Cp, 2 * q->Fp, T, q->esize, num_cus);
   if (!need_dx) q->dx.bytes = 0;
@@ -679,7 +761,7 @@ void launch_gemm(Params p, const Cut& c, hipStream_t s) {
   const int b = c.large ? 256 : 128;
   const int tm = gated ? b / 2 : b;
   p.mt = (p.M + tm - 1) / tm;
-  p.nt = (p.N + b - 1) / b;
+  p.nt = (p.N + c.bn - 1) / c.bn;
   p.full = c.full;
   p.tail = c.tail;
   p.splits = c.splits;
@@ -689,7 +771,10 @@ void launch_gemm(Params p, const Cut& c, hipStream_t s) {
   if constexpr (sizeof(T) == 2) {
     if (c.large) hipLaunchKernelGGL((gemm_kernel<T, MODE, 2, 4, 4>), grid, dim3(512), 0, s, p);
   }
-  if (!c.large) hipLaunchKernelGGL((gemm_kernel<T, MODE, 1, 4, 2>), grid, dim3(256), 0, s, p);
+  if constexpr (sizeof(T) == 4 && (MODE == kFwd || MODE == kBwd)) {
+    if (c.bn == 64) hipLaunchKernelGGL((gemm_kernel<T, MODE, 1, 4, 1>), grid, dim3(256), 0, s, p);
+  }
+  if (c.bn == 128) hipLaunchKernelGGL((gemm_kernel<T, MODE, 1, 4, 2>), grid, dim3(256), 0, s, p);
   if constexpr (MODE == kDx || MODE == kDw) {
     if (c.tail > 0)
       hipLaunchKernelGGL((tail_kernel<T, MODE>), dim3(unsigned(c.tail * (b * b / 1024))), dim3(256), 0, s, p, b, b);
@@ -742,7 +827,11 @@ int forward(const mf_gated_linear_args* a, const Plan& q, hipStream_t s) {
   p.ldo = q.F;
   p.bias = a->bias;
   p.vec = q.F * q.esize % 16 == 0 && aligned16(a->out);
-  launch_gemm<T, kFwd>(p, q.gated, s);
+  const dim3 few(unsigned((q.F + 15) / 16));
+  if (q.T <= 16) hipLaunchKernelGGL((few_kernel<T, 1>), few, dim3(256), 0, s, p);
+  else if (q.T <= 32) hipLaunchKernelGGL((few_kernel<T, 2>), few, dim3(256), 0, s, p);
+  else if (q.T <= kFewTokens) hipLaunchKernelGGL((few_kernel<T, 4>), few, dim3(256), 0, s, p);
+  else launch_gemm<T, kFwd>(p, q.gated, s);
   MF_HIP_CHECK(hipGetLastError());
   return MF_OK;
 }
@@ -758,7 +847,6 @@ int backward(const mf_gated_linear_bwd_args* a, const Plan& q, hipStream_t s) {
   ws += round256(size_t(q.T) * 2 * q.Fp * sizeof(T));
   float* sums = a->dbias ? reinterpret_cast<float*>(ws) : nullptr;
   ws += q.bias_bytes;
-  const int tile = q.gated.large ? 256 : 128;
   p.M = int(q.F);
   p.N = int(q.T);
   p.K = int(q.Cp);
@@ -772,7 +860,7 @@ int backward(const mf_gated_linear_bwd_args* a, const Plan& q, hipStream_t s) {
   if (q.T > 0) launch_gemm<T, kBwd>(p, q.gated, s);
   MF_HIP_CHECK(hipGetLastError());
   if (a->dbias) {
-    const int rows = int((q.T + tile - 1) / tile) * 4;
+    const int rows = int((q.T + q.gated.bn - 1) / q.gated.bn) * 4;
     hipLaunchKernelGGL(bias_kernel<T>, dim3(unsigned(2 * q.Fp / 16)), dim3(256), 0, s, sums, static_cast<T*>(a->dbias),
                        rows, int(q.F), int(q.Fp));
     MF_HIP_CHECK(hipGetLastError());
