@@ -477,6 +477,7 @@ typedef struct mf_radius_attn_args {
   int32_t dtype;               /* MF_DTYPE_BF16 or MF_DTYPE_F16              */
   const uint64_t* key_any;     /* ABI 12: of mf_radius_tables, or NULL.  With it, keys that no query of a */
                                /* tile attends count as zeros, whatever they hold (NaN).                  */
+  void* out_lo;                /* ABI 12: [B, H, N, D] dtype, the fp32 output less out, rounded; or NULL   */
 } mf_radius_attn_args;
 
 int mf_radius_attn(const mf_radius_attn_args* args, void* stream);
@@ -680,6 +681,7 @@ typedef struct mf_radius_attn_bwd_args {
   const void* k;
   const void* v;
   const void* out;             /* [B, H, N, D] the forward's out             */
+  const void* out_lo;          /* and out_lo, or NULL: delta without out's rounding */
   const float* lse;            /* [B, H, N] the forward's lse                */
   const void* grad_out;        /* [B, H, N, D]                               */
   const float* grad_lse;       /* [B, H, N] fp32, or NULL (none)             */

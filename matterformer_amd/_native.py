@@ -211,6 +211,7 @@ class MfRadiusAttnArgs(ctypes.Structure):
         ("head_dim", ctypes.c_int32),
         ("dtype", ctypes.c_int32),
         ("key_any", ctypes.c_void_p),
+        ("out_lo", ctypes.c_void_p),
     ]
 
 
@@ -250,7 +251,7 @@ class MfPairMlpBwdArgs(ctypes.Structure):
 
 
 class MfRadiusAttnBwdArgs(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "lse", "grad_out", "grad_lse", "mask_bits",
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "out_lo", "lse", "grad_out", "grad_lse", "mask_bits",
                                                "mask_bits_t", "key_any", "query_any", "dq", "dk", "dv", "workspace")] + [
         ("workspace_bytes", ctypes.c_uint64), ("scale", ctypes.c_float)] + [
         (n, ctypes.c_int32) for n in ("batch", "heads", "atoms", "head_dim", "dtype")]

@@ -122,7 +122,6 @@ struct Mma<float> {
 constexpr int kRowBytes = 128;                        // K bytes of a tile
 template <typename T> constexpr int kBK = kRowBytes / int(sizeof(T));
 template <typename T> constexpr int kEpc = 16 / int(sizeof(T));  // elements per 16-byte chunk
-constexpr unsigned kOutside = 0x80000000u;            // a buffer offset that is out of range: reads 0
 
 // Row operand ("A", M axis): lane r of fragment j in a group of 64 holds group row 16 (r >> 2) + 4 j + (r & 3),
 // so accumulator register q of fragment j in lane group g is row 16 g + 4 j + q: over j and q, 16 rows in order.
@@ -141,8 +140,6 @@ __device__ __forceinline__ int swz_k(int k) {
   else return ROW_OPERAND ? (k >> 2) & 3 : ((k >> 2) & 3) << 2;
 }
 
-typedef __attribute__((address_space(3))) void* LdsPtr;
-
 // One operand's tile: EXT rows (or columns) of the M or N axis by 128 bytes of K, loaded by NW waves.
 // KOUT: K is the outer axis in memory.
 template <typename T, bool KOUT, bool ROW_OPERAND, int EXT, int NW>
@@ -152,7 +149,7 @@ struct Tile {
   static_assert(kLoads * 64 * 16 * NW == kBytes, "tile shape");
   static constexpr int kPitch = KOUT ? EXT * int(sizeof(T)) : kRowBytes;
   static_assert(!KOUT || EXT >= 128, "the swizzle of K-outer rows needs 16 chunks");
-  unsigned off[kLoads];  // buffer offset of the lane's chunk, or kOutside for a row or column past the end
+  unsigned off[kLoads];  // buffer offset of the lane's chunk, or kLdsCopyOutside for a row or column past the end
   int k[kLoads];         // its first k within the tile
 
   // `valid`: rows (columns) of the tile that exist; K-contiguous rows r >= split continue at +jump bytes
@@ -165,25 +162,23 @@ struct Tile {
         const int row = q / (kPitch / 16), pos = q % (kPitch / 16);
         const int c = pos ^ swz_k<T, ROW_OPERAND>(row);
         k[i] = row;
-        off[i] = c * kEpc<T> < valid ? unsigned(row * ld_bytes + c * 16) : kOutside;
+        off[i] = c * kEpc<T> < valid ? unsigned(row * ld_bytes + c * 16) : kLdsCopyOutside;
       } else {
         const int row = q >> 3, pos = q & 7;
         const int c = pos ^ swz_row<ROW_OPERAND>(row);
         k[i] = c * kEpc<T>;
         const bool second = row >= split;
         const int r = second ? row - split : row;
-        off[i] = r < (second ? valid2 : valid) ? unsigned(r * ld_bytes + (second ? jump : 0) + c * 16) : kOutside;
+        off[i] = r < (second ? valid2 : valid) ? unsigned(r * ld_bytes + (second ? jump : 0) + c * 16) : kLdsCopyOutside;
       }
     }
   }
   // base: the tile's first byte at this K step; left: K entries that remain
   __device__ __forceinline__ void load(const char* base, int left, char* lds, int wave) const {
-    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), short(0), int(kOutside), 0x00027000);
+    const mf_i32x4 source = lds_copy_source(base);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const unsigned o = k[i] < left ? off[i] : kOutside;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (LdsPtr)(lds + (wave * kLoads + i) * 1024), 16, o, 0, 0, 0);
-    }
+    for (int i = 0; i < kLoads; ++i)
+      lds_copy16(source, k[i] < left ? off[i] : kLdsCopyOutside, lds + (wave * kLoads + i) * 1024);
   }
 };
 

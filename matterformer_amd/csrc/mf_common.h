@@ -120,6 +120,37 @@ __device__ __forceinline__ auto read_tr16(const T* p) {
   return __builtin_bit_cast(Op4, v);
 }
 
+// Copies from global memory straight into LDS (buffer_load .. lds): lane l's 16 (or 4) bytes at base + offset land at
+// lds + 16 l (4 l); `lds` is wave-uniform.  An offset of kLdsCopyOutside is out of the buffer's range and reads zeros.
+// The instruction is written out, not the builtin: behind the builtin the compiler makes every transposing LDS read
+// wait for all copies in flight, which it cannot tell apart by address, and with that no copy would overlap a product.
+// So the caller waits: s_waitcnt vmcnt(0) and a barrier between a copy and the reads of what it brought, and the reads
+// of what it overwrites before it.  No register is written, so none can be taken for ready too early.
+constexpr unsigned kLdsCopyOutside = 0x80000000u;
+typedef int mf_i32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ mf_i32x4 lds_copy_source(const void* base) {
+  const uint64_t a = reinterpret_cast<uint64_t>(base);
+  mf_i32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane(int(uint32_t(a)));
+  r[1] = __builtin_amdgcn_readfirstlane(int(uint32_t(a >> 32) & 0xffffu));
+  r[2] = int(kLdsCopyOutside);  // bytes in range
+  r[3] = 0x00027000;
+  return r;
+}
+__device__ __forceinline__ void lds_copy16(mf_i32x4 source, unsigned offset, void* lds) {
+  const int to = __builtin_amdgcn_readfirstlane(
+      int(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(lds))));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :: "s"(to), "v"(offset), "s"(source) : "memory");  // (m0 is reserved: the compiler keeps nothing in it)
+}
+__device__ __forceinline__ void lds_copy4(mf_i32x4 source, unsigned offset, void* lds) {
+  const int to = __builtin_amdgcn_readfirstlane(
+      int(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(lds))));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :: "s"(to), "v"(offset), "s"(source) : "memory");  // (m0 is reserved: the compiler keeps nothing in it)
+}
+
 // Element traits: 16-bit types use the K=32 MFMA (8 K-elements per lane),
 // fp32 uses the K=4 MFMA (1 K-element per lane).  Both produce the same
 // 16x16 fp32 accumulator layout: lane l holds C[4*(l>>4)+r][l&15], r=0..3.

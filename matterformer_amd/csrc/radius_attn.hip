@@ -9,17 +9,17 @@
 // keys that no query of a tile attends are staged as zeros (a NaN behind the
 // last atom stays there).
 //
-// One workgroup (4 waves) per (cell, head, 64-query tile); wave w owns the 16
-// queries 16w..16w+15 of the tile.  Key tiles of 64 whose block-mask entry is
-// set are staged in LDS (K row-major, V transposed), the next one prefetched
-// into registers during the current one's compute.  Per key tile and wave:
+// A workgroup takes a tile of 64 or 128 queries of one (cell, head).  Key tiles
+// of 64 whose block-mask entry is set are staged in LDS (K and V row-major), the
+// next one prefetched into registers during the current one's compute.  Per key
+// tile and wave (16 or 32 queries):
 //   S^T[key][q] = K Q^T        (MFMA 16x16x32, K rows = A operand from LDS,
 //                               Q^T = B operand held in registers)
 //   masked online softmax per query column (base 2, scale*log2 e folded in)
 //   O^T[d][q]  += V^T P^T      (P^T straight from the S^T accumulators as
 //                               the B operand, keys of a 32-key step taken in
 //                               the order {4g+r, 16+4g+r}; V^T rows read from
-//                               LDS in the same key order)
+//                               LDS by transposing reads in the same key order)
 #include <cmath>
 
 #include "mf_common.h"
@@ -43,6 +43,7 @@ struct Params {
   float scale_log2;  // scale * log2(e)
   int B, H, N, W, NB;
   int units;         // B * H * query tiles (the grid is rounded up to a multiple of 8)
+  void* out_lo;      // [B, H, N, D] what out's rounding left, or null
   const uint64_t* key_any;  // [B, NB, NB] keys of a tile that a query of the row's tile attends, or null
 };
 
@@ -63,6 +64,8 @@ struct Ops<_Float16> {
   }
 };
 
+// One key-tile stream: 4 waves per (cell, head, 64-query tile), V staged transposed.  For cells of one tile at head_dim
+// 128, where a second stream would only idle (256 molecules of 30 atoms, 8 heads: 36 us, with two streams 39).
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) radius_attn_kernel(Params p) {
   using Op8 = typename Ops<T>::Op8;
@@ -317,6 +320,11 @@ __global__ void __launch_bounds__(kThreads) radius_attn_kernel(Params p) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) ov[r] = T(o[r]);
       *reinterpret_cast<Op4*>(static_cast<T*>(p.out) + row * D + d0) = ov;
+      if (p.out_lo) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) ov[r] = T(o[r] - float(ov[r]));
+        *reinterpret_cast<Op4*>(static_cast<T*>(p.out_lo) + row * D + d0) = ov;
+      }
     }
     if (p.out_f32) *reinterpret_cast<float4*>(p.out_f32 + row * D + d0) = float4{o[0], o[1], o[2], o[3]};
   }
@@ -324,14 +332,15 @@ __global__ void __launch_bounds__(kThreads) radius_attn_kernel(Params p) {
 }
 
 // ---------------------------------------------------------------------------
-// Two key-tile streams (head_dim 32 and 64): 8 waves per (cell, head,
-// 64-query tile).  Waves w and w + 4 own the 16 queries 16 (w & 3) .. +15;
+// Two key-tile streams: 8 waves per (cell, head, 64-query tile).  Waves w and w + 4 own the 16 queries 16 (w & 3) .. +15;
 // stream e (waves 4e .. 4e + 3) takes the active key tiles of parity e, one
 // per step, each staged in LDS by the 256 threads of its stream.  (The
 // parity, not the position in the active list, picks the stream, so the
-// sums are the same whether or not empty tiles are skipped.)  Per step and wave the work is that of the kernel
-// above; with twice the waves per workgroup and half the steps per wave,
-// four waves share each SIMD.  At the end the two streams' (O, m, l) of a
+// sums are the same whether or not empty tiles are skipped.)  With twice the
+// waves per workgroup and half the steps per wave, up to four waves share each
+// SIMD.  (head_dim 128 too, where the two streams' double buffers take 143 KB of
+// LDS: one 64-query tile by four waves, with V staged transposed, took 133 us on
+// four cells of 1997 atoms and 8 heads, this 60.)  At the end the two streams' (O, m, l) of a
 // query meet in LDS:
 //   out = (2^(m0 - M) O0 + 2^(m1 - M) O1) / (2^(m0 - M) l0 + 2^(m1 - M) l1).
 // ---------------------------------------------------------------------------
@@ -738,6 +747,11 @@ __global__ void __launch_bounds__(kThreads2, 3 - QW) radius_attn_pair_kernel(Par
 #pragma unroll
         for (int r = 0; r < 4; ++r) ov[r] = T(o[r]);
         *reinterpret_cast<Op4*>(static_cast<T*>(p.out) + row * D + d0) = ov;
+        if (p.out_lo) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) ov[r] = T(o[r] - float(ov[r]));
+          *reinterpret_cast<Op4*>(static_cast<T*>(p.out_lo) + row * D + d0) = ov;
+        }
       }
       if (p.out_f32) *reinterpret_cast<float4*>(p.out_f32 + row * D + d0) = float4{o[0], o[1], o[2], o[3]};
     }
@@ -777,7 +791,8 @@ template <typename T>
 int dispatch_dim(const Params& p, int D, hipStream_t stream) {
   if (D == 32) return launch_pair<T, 32>(p, stream);
   if (D == 64) return launch_pair<T, 64>(p, stream);
-  return launch<T, 128>(p, stream);
+  if (p.N <= kTile) return launch<T, 128>(p, stream);
+  return launch_pair<T, 128>(p, stream);
 }
 
 }  // namespace rattn
@@ -797,16 +812,18 @@ extern "C" int mf_radius_attn(const mf_radius_attn_args* a, void* stream) {
   if (a->head_dim != 32 && a->head_dim != 64 && a->head_dim != 128)
     return fail(MF_ERR_UNSUPPORTED, "mf_radius_attn: head_dim must be 32, 64 or 128");
   if (!std::isfinite(a->scale)) return fail(MF_ERR_INVALID_ARGUMENT, "mf_radius_attn: scale must be finite");
-  for (const void* ptr : {a->q, a->k, a->v, static_cast<const void*>(a->out), static_cast<const void*>(a->out_f32)})
+  for (const void* ptr : {a->q, a->k, a->v, static_cast<const void*>(a->out), static_cast<const void*>(a->out_f32),
+                          static_cast<const void*>(a->out_lo)})
     if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0)
       return fail(MF_ERR_INVALID_ARGUMENT, "mf_radius_attn: q, k, v, out and out_f32 must be 16-byte aligned");
+  if (a->out_lo && !a->out) return fail(MF_ERR_INVALID_ARGUMENT, "mf_radius_attn: out_lo needs out");
   if (a->batch == 0 || a->heads == 0 || a->atoms == 0) return MF_OK;
   const int nb = (a->atoms + rattn::kTile - 1) / rattn::kTile;
   if (nb > rattn::kMaxTiles) return fail(MF_ERR_UNSUPPORTED, "mf_radius_attn: atoms must be <= 65536");
   const long long units = (long long)a->batch * a->heads * nb;
   if (units > 0x7fffffffLL - 8) return fail(MF_ERR_UNSUPPORTED, "mf_radius_attn: batch * heads * tiles too large");
   rattn::Params p{a->q, a->k, a->v, a->mask_bits, a->block_mask, a->out, a->out_f32, a->lse,
-                  a->scale * kLog2e, a->batch, a->heads, a->atoms, (a->atoms + 31) / 32, nb, int(units), a->key_any};
+                  a->scale * kLog2e, a->batch, a->heads, a->atoms, (a->atoms + 31) / 32, nb, int(units), a->out_lo, a->key_any};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (a->dtype == MF_DTYPE_BF16) return rattn::dispatch_dim<__bf16>(p, a->head_dim, s);
   return rattn::dispatch_dim<_Float16>(p, a->head_dim, s);

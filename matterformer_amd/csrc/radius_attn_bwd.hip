@@ -12,10 +12,10 @@
 //    (words per key instead of per query), and for every 64 x 64 tile which of
 //    its queries have a key in it and which of its keys a query, 64 bits each:
 //    also the list of tiles with an entry at all.  The forward takes the keys'.
-//  - radius_rows_kernel: per row lse in log2 units and delta.
-//  - radius_bwd_kernel: a workgroup owns 64 CW queries (dq) or keys (dk, dv) as
-//    the columns of its products, a wave 16 CW of them, and streams 64-row tiles
-//    of the other side, X and Y = (K, V) or (Q, go), from global memory straight
+//  - radius_rows_kernel: per row lse in log2 units and -delta.
+//  - radius_bwd_kernel: a workgroup owns 64 queries (dq) or keys (dk, dv) as the
+//    columns of its products, a wave 16 of them, and streams 64-row tiles of the
+//    other side, X and Y = (K, V) or (Q, go), from global memory straight
 //    to LDS, the next tile while the current one is multiplied.  Per 32 rows:
 //      S = X cX^T, dP = Y cY^T   (rows from LDS, columns cX, cY = (Q, go) or
 //                                 (K, V) in registers)
@@ -24,6 +24,11 @@
 //    operands of the second without leaving the lane; X^T and Y^T are read from
 //    the same rows by transposing LDS reads, in the row order the operands have.
 //
+// delta enters every pair of a row alike, so a rounded `out` would show in dq and
+// dk most of all their inputs; with out_lo, what that rounding left, it does not
+// (17 neighbours, head_dim 32: error 2.6e-3 -> 2.4e-3 of the norm, where rounding
+// dS and the result alone leave 2.35e-3).
+//
 // Sums are fp32.  P and dS are rounded to the operands' type for the second
 // products, as any 16-bit matrix product's input is.  fp16 has no room for dS of
 // small or large gradients, so there dS is kept times 2^e, e per (molecule,
@@ -31,8 +36,8 @@
 // stays below 2^14; bf16 has fp32's range and needs none.
 //
 // Rows that no column of the tile is paired with (padding, atoms without a
-// neighbour) are staged as zeros: whatever they hold, NaN too, meets only the
-// zeros of P and dS.
+// neighbour) are staged as zeros, so that whatever they hold, NaN too, reaches
+// no column; a column without a pair is stored as zeros.
 #include <algorithm>
 #include <cmath>
 
@@ -43,14 +48,13 @@ namespace rattn_bwd {
 
 constexpr int kTile = 64;
 constexpr int kThreads = 256;
-constexpr unsigned kOutside = 0x80000000u;  // a buffer offset that is out of range: reads 0
-typedef __attribute__((address_space(3))) void* LdsPtr;
 
 struct Params {
   const void* q;
   const void* k;
   const void* v;
   const void* out;
+  const void* out_lo;
   const void* go;
   const uint32_t* bits;
   const float* lse;
@@ -61,11 +65,11 @@ struct Params {
   const uint32_t* bits_t;   // [B, N, W] the transposed mask
   const uint64_t* key_any;  // [B, NB query tiles, NB key tiles] keys of the tile with a query
   const uint64_t* qry_any;  // [B, NB key tiles, NB query tiles] queries of the tile with a key
-  float* rows;        // [B H, NB, 2, 64]: lse log2(e), then delta, of every query tile
+  float* rows;        // [B H, NB, 2, 64]: lse log2(e), then -delta, of every query tile
   float4* peak;       // fp16: [B H, NB] max |go|^2, |v|^2 and |dlse| of a tile
   float scale;
   int B, H, N, W, NB;
-  int ntc, units;     // column tiles per (molecule, head); workgroups of one role
+  int units;          // workgroups of one role
 };
 
 // -- the mask's tables: one wave per 64 x 64 tile, lane i its query row -------------------------------------------
@@ -145,6 +149,11 @@ __global__ void __launch_bounds__(kThreads) radius_rows_kernel(Params p) {
       const T8 o = *reinterpret_cast<const T8*>(static_cast<const T*>(p.out) + at);
 #pragma unroll
       for (int e = 0; e < 8; ++e) dot += Elem<T>::to_f32(g[e]) * Elem<T>::to_f32(o[e]);
+      if (p.out_lo) {
+        const T8 lo = *reinterpret_cast<const T8*>(static_cast<const T*>(p.out_lo) + at);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dot += Elem<T>::to_f32(g[e]) * Elem<T>::to_f32(lo[e]);
+      }
       if constexpr (sizeof(T) == 2 && !__is_same(T, __bf16)) {
         const T8 v = *reinterpret_cast<const T8*>(static_cast<const T*>(p.v) + at);
 #pragma unroll
@@ -168,7 +177,7 @@ __global__ void __launch_bounds__(kThreads) radius_rows_kernel(Params p) {
       const float dl = in && p.dlse ? p.dlse[bh * p.N + row] : 0.0f;
       lmax = fmaxf(lmax, fabsf(dl) <= 3.0e38f ? fabsf(dl) : 0.0f);
       dst[r] = in ? p.lse[bh * p.N + row] * kLog2e : 0.0f;
-      dst[kTile + r] = in ? dot - dl : 0.0f;
+      dst[kTile + r] = in ? dl - dot : 0.0f;
     }
   }
   if (p.peak) {
@@ -196,20 +205,19 @@ __device__ __forceinline__ int swz(int row) {
   else return ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
 }
 
-template <typename T, int D, bool KEYS, int CW>
+template <typename T, int D, bool KEYS>
 __device__ __forceinline__ void bwd_unit(const Params& p, int unit, char* x0, char* y0, float* r0, char* x1, char* y1,
                                          float* r1) {
   using Op = typename Elem<T>::Operand;
   typedef __attribute__((__vector_size__(4 * sizeof(T)))) T Op4;
   constexpr int DK = D / 32, ND = D / 16, CPR = D / 8;
   constexpr int kLoads = kTile * CPR / kThreads;  // 16-byte chunks per thread and tile
-  constexpr int CT = kTile * CW;                  // columns per workgroup
   constexpr bool kHalf = __is_same(T, _Float16);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, r16 = lane & 15;
-  const int ct = unit % p.ntc;
-  const int64_t bh = unit / p.ntc;
+  const int ct = unit % p.NB;  // column tile
+  const int64_t bh = unit / p.NB;
   const int64_t b = bh / p.H;
   const int N = p.N;
   const int64_t base = bh * N * D;
@@ -218,32 +226,26 @@ __device__ __forceinline__ void bwd_unit(const Params& p, int unit, char* x0, ch
   const char* gx = reinterpret_cast<const char*>(static_cast<const T*>(KEYS ? p.q : p.k) + base);
   const char* gy = reinterpret_cast<const char*>(static_cast<const T*>(KEYS ? p.go : p.v) + base);
   const char* grow = reinterpret_cast<const char*>(p.rows + bh * p.NB * 2 * kTile);
-  const uint32_t* cbits = (KEYS ? p.bits_t : p.bits) + b * N * p.W;
-  // which rows of a streamed tile have a partner in 64-column tile c: any[c][tile]
-  const uint64_t* any = (KEYS ? p.qry_any : p.key_any) + b * p.NB * p.NB;
-  const int c64 = ct * CW;  // first 64-column tile
-  const bool two = CW == 2 && c64 + 1 < p.NB;
+  // which rows of a streamed tile have a partner among these columns
+  const uint64_t* any = (KEYS ? p.qry_any : p.key_any) + (b * p.NB + ct) * p.NB;
 
-  // columns: lane holds column 16 t + r16 of the wave's 16 CW, d = 32 kk + 8 g .. + 7
-  int col[CW];
-  Op bx[CW][DK], by[CW][DK];
-  float clse[CW], cdelta[CW];
+  // columns: lane holds column r16 of the wave's 16, d = 32 kk + 8 g .. + 7
+  const int col = ct * kTile + wave * 16 + r16;
+  const bool col_in = col < N;
+  const uint32_t* cbits = (KEYS ? p.bits_t : p.bits) + (b * N + (col_in ? col : 0)) * p.W;
+  const uint32_t col_mask = col_in ? ~0u : 0u;
+  Op bx[DK], by[DK];
 #pragma unroll
-  for (int t = 0; t < CW; ++t) {
-    col[t] = ct * CT + (wave * CW + t) * 16 + r16;
-    const bool in = col[t] < N;
-    const int64_t at = int64_t(in ? col[t] : 0) * D + 8 * g;
-#pragma unroll
-    for (int kk = 0; kk < DK; ++kk) {
-      bx[t][kk] = *reinterpret_cast<const Op*>(cx + at + 32 * kk);
-      by[t][kk] = *reinterpret_cast<const Op*>(cy + at + 32 * kk);
-    }
-    clse[t] = cdelta[t] = 0.0f;
-    if (!KEYS && in) {
-      const float* r = p.rows + (bh * p.NB + (col[t] >> 6)) * 2 * kTile + (col[t] & 63);
-      clse[t] = r[0];
-      cdelta[t] = r[kTile];
-    }
+  for (int kk = 0; kk < DK; ++kk) {
+    const int64_t at = int64_t(col_in ? col : 0) * D + 8 * g + 32 * kk;
+    bx[kk] = *reinterpret_cast<const Op*>(cx + at);
+    by[kk] = *reinterpret_cast<const Op*>(cy + at);
+  }
+  float clse = 0.0f, cdelta = 0.0f;
+  if (!KEYS && col_in) {
+    const float* r = p.rows + (bh * p.NB + ct) * 2 * kTile + (col & 63);
+    clse = r[0];
+    cdelta = r[kTile];
   }
   float up = 1.0f, down = p.scale;  // dS is kept times `up`
   if constexpr (kHalf) {
@@ -277,100 +279,84 @@ __device__ __forceinline__ void bwd_unit(const Params& p, int unit, char* x0, ch
 
   // tiles with an entry, in order: 64 tiles' row sets a time in the lanes
   int tbase = -64;
-  uint64_t active = 0, part0 = 0, part1 = 0;
-  auto next = [&](int& tile, uint64_t& s0, uint64_t& s1) -> bool {
+  uint64_t active = 0, sets = 0;
+  auto next = [&](int& tile, uint64_t& set) -> bool {
     while (active == 0) {
       tbase += 64;
       if (tbase >= p.NB) return false;
       const int t = tbase + lane;
-      part0 = t < p.NB ? any[int64_t(c64) * p.NB + t] : 0;
-      part1 = two && t < p.NB ? any[int64_t(c64 + 1) * p.NB + t] : 0;
-      active = __ballot((part0 | part1) != 0);
+      sets = t < p.NB ? any[t] : 0;
+      active = __ballot(sets != 0);
     }
     const int l = __builtin_ctzll(active);
     active &= active - 1;
     tile = tbase + l;
-    auto at = [l](uint64_t v) {
-      return uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v)), l))) |
-             uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(v >> 32)), l))) << 32;
-    };
-    s0 = at(part0);
-    s1 = at(part1);
+    set = uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(sets)), l))) |
+          uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(sets >> 32)), l))) << 32;
     return true;
   };
-  auto load = [&](int tile, uint64_t set, char* lx, char* ly, float* lr, uint32_t (&w)[CW][2]) {
+  auto load = [&](int tile, uint64_t set, char* lx, char* ly, float* lr, uint32_t (&w)[2]) {
     const int64_t first = int64_t(tile) * kTile * D * 2;
-    const auto rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(gx + first), short(0), int(kOutside), 0x00027000);
-    const auto ry = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(gy + first), short(0), int(kOutside), 0x00027000);
+    const mf_i32x4 rx = lds_copy_source(gx + first), ry = lds_copy_source(gy + first);
+    const bool all = set == ~uint64_t(0);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const unsigned o = (set >> srow[i]) & 1 ? off[i] : kOutside;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (LdsPtr)(lx + (wave * kLoads + i) * 1024), 16, o, 0, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ry, (LdsPtr)(ly + (wave * kLoads + i) * 1024), 16, o, 0, 0, 0);
+      unsigned o = off[i];
+      if (!all) o = (set >> srow[i]) & 1 ? o : kLdsCopyOutside;
+      lds_copy16(rx, o, lx + (wave * kLoads + i) * 1024);
+      lds_copy16(ry, o, ly + (wave * kLoads + i) * 1024);
     }
     if (KEYS && wave == 0) {
-      const auto rr = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(grow + int64_t(tile) * 512), short(0),
-                                                        int(kOutside), 0x00027000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rr, (LdsPtr)lr, 16, lane < 32 ? lane * 16u : kOutside, 0, 0, 0);
+      const mf_i32x4 rr = lds_copy_source(grow + int64_t(tile) * 512);
+      const bool on = (set >> lane) & 1;  // zeros for rows without a partner here too
+      lds_copy4(rr, on ? lane * 4u : kLdsCopyOutside, lr);
+      lds_copy4(rr, on ? lane * 4u + kTile * 4u : kLdsCopyOutside, lr + kTile);
     }
-#pragma unroll
-    for (int t = 0; t < CW; ++t) {
-      const bool in = col[t] < N;
-      const uint32_t* src = cbits + int64_t(in ? col[t] : 0) * p.W + 2 * tile;
-      w[t][0] = in ? src[0] : 0u;
-      w[t][1] = in && 2 * tile + 1 < p.W ? src[1] : 0u;
-    }
+    // (columns past the end read the first one's words, cleared where they are used)
+    w[0] = cbits[2 * tile];
+    w[1] = 2 * tile + 1 < p.W ? cbits[2 * tile + 1] : 0u;
   };
 
-  mf_f32x4 ax[CW][ND], ay[KEYS ? CW : 1][ND];
+  uint32_t seen = 0u;  // the column has a pair
+  mf_f32x4 ax[ND], ay[ND];
 #pragma unroll
-  for (int t = 0; t < CW; ++t)
-#pragma unroll
-    for (int n = 0; n < ND; ++n) {
-      ax[t][n] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
-      if constexpr (KEYS) ay[t][n] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+  for (int n = 0; n < ND; ++n) ax[n] = ay[n] = mf_f32x4{0.f, 0.f, 0.f, 0.f};
 
-  auto compute = [&](const char* lx, const char* ly, const float* lr, uint64_t s0, uint64_t s1,
-                     const uint32_t (&w)[CW][2]) {
-    const uint64_t set = s0 | s1;
+  auto compute = [&](const char* lx, const char* ly, const float* lr, uint64_t set, const uint32_t (&words)[2]) {
 #pragma unroll
     for (int pr = 0; pr < 2; ++pr) {
       if (uint32_t(set >> (32 * pr)) == 0) continue;  // no pair in these 32 rows
-      Op pb[CW], sb[CW];
+      const uint32_t word = words[pr] & col_mask;
+      seen |= word;
+      Op pb, sb;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int row = 32 * pr + 16 * h + r16;
-        Op fx[DK], fy[DK];
+        mf_f32x4 rl, d;  // d: dP - delta, -delta as the sum's start
+        if constexpr (KEYS) {
+          rl = *reinterpret_cast<const mf_f32x4*>(lr + 32 * pr + 16 * h + 4 * g);
+          d = *reinterpret_cast<const mf_f32x4*>(lr + kTile + 32 * pr + 16 * h + 4 * g);
+        } else {
+          d = mf_f32x4{cdelta, cdelta, cdelta, cdelta};
+        }
+        mf_f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kk = 0; kk < DK; ++kk) {
           const int at = row * (D * 2) + (((4 * kk + g) ^ swz<D>(row)) << 4);
-          fx[kk] = *reinterpret_cast<const Op*>(lx + at);
-          fy[kk] = *reinterpret_cast<const Op*>(ly + at);
+          s = Elem<T>::mma(*reinterpret_cast<const Op*>(lx + at), bx[kk], s);
+          d = Elem<T>::mma(*reinterpret_cast<const Op*>(ly + at), by[kk], d);
         }
-        mf_f32x4 rl, rd;
-        if constexpr (KEYS) {
-          rl = *reinterpret_cast<const mf_f32x4*>(lr + 32 * pr + 16 * h + 4 * g);
-          rd = *reinterpret_cast<const mf_f32x4*>(lr + kTile + 32 * pr + 16 * h + 4 * g);
-        }
+        const uint32_t bits = word >> (16 * h + 4 * g);
 #pragma unroll
-        for (int t = 0; t < CW; ++t) {
-          mf_f32x4 s = {0.f, 0.f, 0.f, 0.f}, d = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int kk = 0; kk < DK; ++kk) {
-            s = Elem<T>::mma(fx[kk], bx[t][kk], s);
-            d = Elem<T>::mma(fy[kk], by[t][kk], d);
-          }
-          const uint32_t bits = w[t][pr] >> (16 * h + 4 * g);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const bool on = (bits >> r) & 1u;
-            const float l = KEYS ? rl[r] : clse[t], dl = KEYS ? rd[r] : cdelta[t];
-            const float pv = on ? fast_exp2(s[r] * slog - l) : 0.0f;
-            const float ds = on ? pv * (d[r] - dl) * up : 0.0f;
-            pb[t][4 * h + r] = Elem<T>::from_f32(pv);
-            sb[t][4 * h + r] = Elem<T>::from_f32(ds);
-          }
+        for (int r = 0; r < 4; ++r) {
+          // pairs outside the mask: P's bits are cleared (its exponent may be anything), and dS = 0 with it
+          int on;
+          asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(on) : "v"(bits), "n"(r));
+          const float e = fast_exp2(fmaf(s[r], slog, KEYS ? -rl[r] : -clse));
+          const float pv = __int_as_float(__float_as_int(e) & on);
+          const float ds = kHalf ? pv * d[r] * up : pv * d[r];
+          pb[4 * h + r] = Elem<T>::from_f32(pv);
+          sb[4 * h + r] = Elem<T>::from_f32(ds);
         }
       }
       // operand entry 4 h + r of lane group g is row 32 pr + 16 h + 4 g + r
@@ -383,76 +369,70 @@ __device__ __forceinline__ void bwd_unit(const Params& p, int unit, char* x0, ch
         const int hi = (row + 16) * (D * 2) + ((chunk ^ swz<D>(row + 16)) << 4) + sub;
         const Op xt = __builtin_shufflevector(read_tr16(reinterpret_cast<const T*>(lx + lo)),
                                               read_tr16(reinterpret_cast<const T*>(lx + hi)), 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-        for (int t = 0; t < CW; ++t) ax[t][n] = Elem<T>::mma(xt, sb[t], ax[t][n]);
+        ax[n] = Elem<T>::mma(xt, sb, ax[n]);
         if constexpr (KEYS) {
           const Op yt = __builtin_shufflevector(read_tr16(reinterpret_cast<const T*>(ly + lo)),
                                                 read_tr16(reinterpret_cast<const T*>(ly + hi)), 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-          for (int t = 0; t < CW; ++t) ay[t][n] = Elem<T>::mma(yt, pb[t], ay[t][n]);
+          ay[n] = Elem<T>::mma(yt, pb, ay[n]);
         }
       }
     }
   };
 
   auto ready = [] {
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's loads into LDS have landed
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's copies into LDS have landed
     __syncthreads();
   };
   int tile = 0;
-  uint64_t s0a = 0, s1a = 0, s0b = 0, s1b = 0;
-  uint32_t wa[CW][2], wb[CW][2];
-  bool more = next(tile, s0a, s1a);
-  if (more) load(tile, s0a | s1a, x0, y0, r0, wa);
+  uint64_t sa = 0, sb = 0;
+  uint32_t wa[2], wb[2];
+  bool more = next(tile, sa);
+  if (more) load(tile, sa, x0, y0, r0, wa);
   while (more) {
     ready();
-    more = next(tile, s0b, s1b);
-    if (more) load(tile, s0b | s1b, x1, y1, r1, wb);
-    compute(x0, y0, r0, s0a, s1a, wa);
+    more = next(tile, sb);
+    if (more) load(tile, sb, x1, y1, r1, wb);
+    compute(x0, y0, r0, sa, wa);
     if (!more) break;
     ready();
-    more = next(tile, s0a, s1a);
-    if (more) load(tile, s0a | s1a, x0, y0, r0, wa);
-    compute(x1, y1, r1, s0b, s1b, wb);
+    more = next(tile, sa);
+    if (more) load(tile, sa, x0, y0, r0, wa);
+    compute(x1, y1, r1, sb, wb);
   }
 
+  if (!col_in) return;
   T* ox = static_cast<T*>(KEYS ? p.dk : p.dq) + base;
   T* oy = static_cast<T*>(p.dv) + base;
 #pragma unroll
-  for (int t = 0; t < CW; ++t) {
-    if (col[t] >= N) continue;
+  for (int n = 0; n < ND; ++n) {
+    Op4 vx, vy;
 #pragma unroll
-    for (int n = 0; n < ND; ++n) {
-      Op4 vx, vy;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        vx[r] = Elem<T>::from_f32(ax[t][n][r] * down);
-        if constexpr (KEYS) vy[r] = Elem<T>::from_f32(ay[t][n][r]);
-      }
-      const int64_t at = int64_t(col[t]) * D + 16 * n + 4 * g;
-      *reinterpret_cast<Op4*>(ox + at) = vx;
-      if constexpr (KEYS) *reinterpret_cast<Op4*>(oy + at) = vy;
+    for (int r = 0; r < 4; ++r) {
+      vx[r] = Elem<T>::from_f32(seen ? ax[n][r] * down : 0.0f);  // a NaN row without a pair too
+      if constexpr (KEYS) vy[r] = Elem<T>::from_f32(ay[n][r]);
     }
+    const int64_t at = int64_t(col) * D + 16 * n + 4 * g;
+    *reinterpret_cast<Op4*>(ox + at) = vx;
+    if constexpr (KEYS) *reinterpret_cast<Op4*>(oy + at) = vy;
   }
 }
 
-template <typename T, int D, int CW>
-__global__ void __launch_bounds__(kThreads, D == 128 || CW == 2 ? 2 : 3) radius_bwd_kernel(Params p) {
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, D == 128 ? 2 : 4) radius_bwd_kernel(Params p) {
   constexpr int kBytes = kTile * D * 2;
   __shared__ __attribute__((aligned(1024))) char x0[kBytes];
   __shared__ __attribute__((aligned(1024))) char y0[kBytes];
   __shared__ __attribute__((aligned(1024))) char x1[kBytes];
   __shared__ __attribute__((aligned(1024))) char y1[kBytes];
-  // 64 lanes of the row values' load write 16 bytes each; the upper half's land behind the 512 used
-  __shared__ __attribute__((aligned(1024))) float r0[256];
-  __shared__ __attribute__((aligned(1024))) float r1[256];
+  __shared__ __attribute__((aligned(1024))) float r0[2 * kTile];
+  __shared__ __attribute__((aligned(1024))) float r1[2 * kTile];
   // XCD-aware order: the column tiles of one (molecule, head), keys and queries, on one XCD and its L2
   const int per = gridDim.x >> 3;
   const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if (id >= 2 * p.units) return;
-  const int bh = id / (2 * p.ntc), r = id - bh * 2 * p.ntc;
-  if (r < p.ntc) bwd_unit<T, D, true, CW>(p, bh * p.ntc + r, x0, y0, r0, x1, y1, r1);
-  else bwd_unit<T, D, false, CW>(p, bh * p.ntc + r - p.ntc, x0, y0, r0, x1, y1, r1);
+  const int bh = id / (2 * p.NB), r = id - bh * 2 * p.NB;
+  if (r < p.NB) bwd_unit<T, D, true>(p, bh * p.NB + r, x0, y0, r0, x1, y1, r1);
+  else bwd_unit<T, D, false>(p, bh * p.NB + r - p.NB, x0, y0, r0, x1, y1, r1);
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
@@ -475,9 +455,9 @@ template <typename T, int D>
 int launch(Params p, hipStream_t s) {
   hipLaunchKernelGGL((radius_rows_kernel<T, D>), dim3(unsigned(p.B * p.H * p.NB)), dim3(kThreads), 0, s, p);
   MF_HIP_CHECK(hipGetLastError());
-  p.ntc = p.NB;
-  p.units = p.B * p.H * p.ntc;
-  hipLaunchKernelGGL((radius_bwd_kernel<T, D, 1>), dim3(unsigned((2 * p.units + 7) / 8 * 8)), dim3(kThreads), 0, s, p);
+  p.units = p.B * p.H * p.NB;
+  const dim3 grid(unsigned((2 * p.units + 7) / 8 * 8));
+  hipLaunchKernelGGL((radius_bwd_kernel<T, D>), grid, dim3(kThreads), 0, s, p);
   MF_HIP_CHECK(hipGetLastError());
   return MF_OK;
 }
@@ -533,7 +513,7 @@ extern "C" int mf_radius_attn_bwd(const mf_radius_attn_bwd_args* a, void* stream
   if (a->head_dim != 32 && a->head_dim != 64 && a->head_dim != 128)
     return fail(MF_ERR_UNSUPPORTED, "mf_radius_attn_bwd: head_dim must be 32, 64 or 128");
   if (!std::isfinite(a->scale)) return fail(MF_ERR_INVALID_ARGUMENT, "mf_radius_attn_bwd: scale must be finite");
-  for (const void* ptr : {a->q, a->k, a->v, a->out, a->grad_out, static_cast<const void*>(a->dq),
+  for (const void* ptr : {a->q, a->k, a->v, a->out, a->out_lo, a->grad_out, static_cast<const void*>(a->dq),
                           static_cast<const void*>(a->dk), static_cast<const void*>(a->dv)})
     if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0)
       return fail(MF_ERR_INVALID_ARGUMENT, "mf_radius_attn_bwd: operands and gradients must be 16-byte aligned");
@@ -551,6 +531,7 @@ extern "C" int mf_radius_attn_bwd(const mf_radius_attn_bwd_args* a, void* stream
   p.k = a->k;
   p.v = a->v;
   p.out = a->out;
+  p.out_lo = a->out_lo;
   p.go = a->grad_out;
   p.bits = a->mask_bits;
   p.lse = a->lse;

@@ -259,8 +259,9 @@ def radius_tables(mask_bits: torch.Tensor, block_mask: torch.Tensor | None = Non
     return tables
 
 
-def _radius_forward(q, k, v, bits, bm, tables, scale, *, lse: bool, fp32: bool):
-    """out, lse and the fp32 output (None where not asked) of contiguous operands."""
+def _radius_forward(q, k, v, bits, bm, tables, scale, *, lse: bool, fp32: bool, out_lo: torch.Tensor | None = None):
+    """out, lse and the fp32 output (None where not asked) of contiguous operands; out_lo takes what out's rounding
+    leaves."""
     B, H, N, D = q.shape
     out = torch.empty_like(q)
     out32 = torch.empty(B, H, N, D, dtype=torch.float32, device=q.device) if fp32 else None
@@ -269,7 +270,7 @@ def _radius_forward(q, k, v, bits, bm, tables, scale, *, lse: bool, fp32: bool):
         q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), mask_bits=bits.data_ptr(), block_mask=_native.ptr(bm),
         out=out.data_ptr(), out_f32=_native.ptr(out32), lse=_native.ptr(lse_out), scale=scale, batch=B, heads=H,
         atoms=N, head_dim=D, dtype=_native.dtype_code(q.dtype),
-        key_any=None if tables is None else tables.key_any.data_ptr())
+        key_any=None if tables is None else tables.key_any.data_ptr(), out_lo=_native.ptr(out_lo))
     _native.launch("mf_radius_attn", args, q.device)
     return out, lse_out, out32
 
@@ -279,8 +280,9 @@ class _RadiusAttentionFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, bits, bm, tables, scale, fp32):
-        out, lse, out32 = _radius_forward(q, k, v, bits, bm, tables, scale, lse=True, fp32=fp32)
-        ctx.save_for_backward(q, k, v, bits, out, lse)
+        lo = torch.empty_like(q)
+        out, lse, out32 = _radius_forward(q, k, v, bits, bm, tables, scale, lse=True, fp32=fp32, out_lo=lo)
+        ctx.save_for_backward(q, k, v, bits, out, lse, lo)
         ctx.tables, ctx.scale = tables, scale
         ctx.set_materialize_grads(False)
         if out32 is not None:
@@ -290,7 +292,7 @@ class _RadiusAttentionFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out, grad_lse, _):
-        q, k, v, bits, out, lse = ctx.saved_tensors
+        q, k, v, bits, out, lse, lo = ctx.saved_tensors
         if grad_out is None and grad_lse is None:
             return (None,) * 8
         B, H, N, D = q.shape
@@ -304,8 +306,8 @@ class _RadiusAttentionFunction(torch.autograd.Function):
             nbytes = int(_native.lib().mf_radius_attn_bwd_workspace_size(B, H, N, _native.dtype_code(q.dtype)))
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
             args = _native.MfRadiusAttnBwdArgs(
-                q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), lse=lse.data_ptr(),
-                grad_out=go.data_ptr(), grad_lse=_native.ptr(gl), mask_bits=bits.data_ptr(),
+                q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), out_lo=lo.data_ptr(),
+                lse=lse.data_ptr(), grad_out=go.data_ptr(), grad_lse=_native.ptr(gl), mask_bits=bits.data_ptr(),
                 mask_bits_t=t.bits_t.data_ptr(), key_any=t.key_any.data_ptr(), query_any=t.query_any.data_ptr(),
                 dq=grads[0].data_ptr(), dk=grads[1].data_ptr(), dv=grads[2].data_ptr(),
                 workspace=workspace.data_ptr(), workspace_bytes=nbytes, scale=ctx.scale, batch=B, heads=H, atoms=N,
