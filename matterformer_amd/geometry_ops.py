@@ -282,8 +282,8 @@ class _RadiusAttentionFunction(torch.autograd.Function):
     def forward(ctx, q, k, v, bits, bm, tables, scale, fp32):
         lo = torch.empty_like(q)
         out, lse, out32 = _radius_forward(q, k, v, bits, bm, tables, scale, lse=True, fp32=fp32, out_lo=lo)
-        ctx.save_for_backward(q, k, v, bits, out, lse, lo)
-        ctx.tables, ctx.scale = tables, scale
+        ctx.save_for_backward(q, k, v, bits, out, lse, lo, tables.bits_t, tables.key_any, tables.query_any)
+        ctx.scale = scale
         ctx.set_materialize_grads(False)
         if out32 is not None:
             ctx.mark_non_differentiable(out32)
@@ -292,7 +292,7 @@ class _RadiusAttentionFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out, grad_lse, _):
-        q, k, v, bits, out, lse, lo = ctx.saved_tensors
+        q, k, v, bits, out, lse, lo, bits_t, key_any, query_any = ctx.saved_tensors
         if grad_out is None and grad_lse is None:
             return (None,) * 8
         B, H, N, D = q.shape
@@ -302,13 +302,12 @@ class _RadiusAttentionFunction(torch.autograd.Function):
         gl = None if grad_lse is None else grad_lse.contiguous()
         grads = [torch.empty_like(t) for t in (q, k, v)]
         if q.numel() > 0:
-            t = ctx.tables
             nbytes = int(_native.lib().mf_radius_attn_bwd_workspace_size(B, H, N, _native.dtype_code(q.dtype)))
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
             args = _native.MfRadiusAttnBwdArgs(
                 q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), out_lo=lo.data_ptr(),
                 lse=lse.data_ptr(), grad_out=go.data_ptr(), grad_lse=_native.ptr(gl), mask_bits=bits.data_ptr(),
-                mask_bits_t=t.bits_t.data_ptr(), key_any=t.key_any.data_ptr(), query_any=t.query_any.data_ptr(),
+                mask_bits_t=bits_t.data_ptr(), key_any=key_any.data_ptr(), query_any=query_any.data_ptr(),
                 dq=grads[0].data_ptr(), dk=grads[1].data_ptr(), dv=grads[2].data_ptr(),
                 workspace=workspace.data_ptr(), workspace_bytes=nbytes, scale=ctx.scale, batch=B, heads=H, atoms=N,
                 head_dim=D, dtype=_native.dtype_code(q.dtype))

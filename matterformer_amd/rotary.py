@@ -212,16 +212,28 @@ def _turn_heads(plan: _Plan, heads, inverse: bool) -> tuple[torch.Tensor, ...]:
     return outs
 
 
+def _keep(ctx, plan: _Plan) -> None:
+    """The plan for the gradient; its tensors as saved ones, so that a change in place before it is an error."""
+    ctx.save_for_backward(plan.positions, plan.frequencies.table, plan.slot)
+    ctx.plan = (plan.frequencies.axes, plan.frequencies.gain, plan.interleaved)
+
+
+def _kept(ctx) -> _Plan:
+    positions, table, slot = ctx.saved_tensors
+    axes, gain, interleaved = ctx.plan
+    return _Plan(positions, RotaryFrequencies(table, axes, gain), interleaved, slot)
+
+
 class _HeadsFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, plan, *heads):
-        ctx.plan = plan
+        _keep(ctx, plan)
         return _turn_heads(plan, heads, False)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
-        return (None, *_turn_heads(ctx.plan, grads, True))
+        return (None, *_turn_heads(_kept(ctx), grads, True))
 
 
 def _head_parts(counts, head_dim: int, batch_stride: int, row_stride: int):
@@ -250,14 +262,15 @@ def _rows_to_heads(plan: _Plan, rows: torch.Tensor, counts, batch: int, tokens: 
 class _RowsFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, plan, rows, counts, batch, tokens, head_dim, dtype):
-        ctx.plan, ctx.counts, ctx.sizes = plan, counts, (batch, tokens, head_dim)
+        _keep(ctx, plan)
+        ctx.counts, ctx.sizes = counts, (batch, tokens, head_dim)
         ctx.rows = (rows.shape, rows.dtype)
         return _rows_to_heads(plan, rows, counts, batch, tokens, head_dim, dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
-        plan, (batch, tokens, head_dim), (shape, dtype) = ctx.plan, ctx.sizes, ctx.rows
+        plan, (batch, tokens, head_dim), (shape, dtype) = _kept(ctx), ctx.sizes, ctx.rows
         packed = plan.slot is not None
         out = torch.empty(shape, dtype=dtype, device=grads[0].device)
         layout = _head_parts(ctx.counts, head_dim, 0 if packed else out.stride(0), out.stride(-2))

@@ -243,3 +243,21 @@ def test_stream_and_graph(cuda, C):
         torch.cuda.synchronize()
         now = _run(x, w, b, go, "silu")
         assert torch.equal(held[0], now[0]) and all(torch.equal(p, q) for p, q in zip(held[1], now[1])), turn
+
+
+def test_many_rows_pass_32_bit_offsets(cuda):
+    """1.1e6 rows of 2048 hidden columns: 2.25e9 output elements; the last rows against a call of their own."""
+    x, w, b, _ = _inputs(1100000, 64, 2048, torch.bfloat16, True, 20, cuda)
+    with torch.no_grad():
+        out = gated_linear(x, w, b)
+        tail = gated_linear(x[-512:], w, b)
+    assert torch.equal(out[-512:], tail)
+
+
+def test_two_calls_in_flight(cuda):
+    x, w, b, go = _inputs(70, 64, 40, torch.bfloat16, True, 21, cuda)
+    leaf = x.clone().requires_grad_(True)
+    one, two = gated_linear(leaf, w, b), gated_linear(leaf, w, b, activation="relu")
+    g2 = torch.autograd.grad(two, leaf, go)[0]
+    g1 = torch.autograd.grad(one, leaf, go)[0]
+    assert torch.equal(g1, _run(x, w, b, go, "silu")[1][0]) and torch.equal(g2, _run(x, w, b, go, "relu")[1][0])

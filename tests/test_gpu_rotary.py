@@ -216,3 +216,34 @@ def test_stream_and_graph(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, once())), f"replay {turn}"
+
+
+def test_positions_changed_before_the_gradient_are_an_error(cuda):
+    f = rotary_frequencies(16).to(cuda)
+    rows = torch.randn(1, 4, 3 * 16, device=cuda, requires_grad=True)
+    pos = torch.arange(4, device=cuda)[None].float()
+    out = rotary_heads(rows, pos, f, heads=1)
+    pos += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out[0].sum().backward()
+
+
+def test_two_calls_in_flight_and_long_rows(cuda):
+    """Two graphs of one leaf, their gradients in either order; a batch whose elements pass 2^31."""
+    f = rotary_frequencies(16).to(cuda)
+    rows = torch.randn(2, 5, 3 * 16, device=cuda, requires_grad=True)
+    a = rotary_heads(rows, torch.arange(5, device=cuda)[None], f, heads=1)
+    b = rotary_heads(rows, torch.arange(5, device=cuda)[None] + 7, f, heads=1)
+    one = [torch.ones_like(t) for t in a]
+    (gb,) = torch.autograd.grad(b, rows, one)
+    (ga,) = torch.autograd.grad(a, rows, one)
+    again = rotary_heads(rows, torch.arange(5, device=cuda)[None], f, heads=1)
+    assert torch.equal(torch.autograd.grad(again, rows, one)[0], ga) and not torch.equal(ga, gb)
+    big = torch.zeros(2, 700000, 3 * 2 * 256, dtype=torch.bfloat16, device=cuda)  # 2.15e9 elements
+    big[1, -1] = 1.0
+    f = rotary_frequencies(256).to(cuda)
+    pos = torch.zeros(1, 700000, dtype=torch.int32, device=cuda)
+    q, k, v = rotary_heads(big, pos, f, heads=2)
+    for t in (q, k, v):
+        assert torch.equal(t[1, :, -1], torch.ones(2, 256, dtype=torch.bfloat16, device=cuda))
+        assert float(t[0, :, -1].abs().max()) == 0.0 and float(t[1, :, -2].abs().max()) == 0.0
