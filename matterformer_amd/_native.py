@@ -258,10 +258,14 @@ class MfRadiusAttnBwdArgs(ctypes.Structure):
 
 
 class MfRotaryArgs(ctypes.Structure):
-    _fields_ = [("src", ctypes.c_void_p * 3), ("dst", ctypes.c_void_p * 3), ("src_stride", ctypes.c_int64 * 3 * 3),
-                ("dst_stride", ctypes.c_int64 * 3 * 3), ("heads", ctypes.c_int32 * 3), ("turn", ctypes.c_int32 * 3),
-                ("positions", ctypes.c_void_p), ("position_stride", ctypes.c_int64 * 3),
-                ("frequencies", ctypes.c_void_p), ("slot", ctypes.c_void_p), ("gain", ctypes.c_float)] + [
+    """mf_rotary_args with its small arrays as fields of their own (src0, src1, ..; src_stride is src_stride0 .. 8, part
+    by part): building ctypes arrays takes four times as long as the rest of the call."""
+
+    _fields_ = [(f"{n}{i}", ctypes.c_void_p) for n in ("src", "dst") for i in range(3)] + [
+        (f"{n}{i}", ctypes.c_int64) for n in ("src_stride", "dst_stride") for i in range(9)] + [
+        (f"{n}{i}", ctypes.c_int32) for n in ("heads", "turn") for i in range(3)] + [
+        ("positions", ctypes.c_void_p)] + [(f"position_stride{i}", ctypes.c_int64) for i in range(3)] + [
+        ("frequencies", ctypes.c_void_p), ("slot", ctypes.c_void_p), ("gain", ctypes.c_float)] + [
         (n, ctypes.c_int32) for n in ("position_type", "slot_side", "parts", "batch", "tokens", "head_dim",
                                       "rotary_dim", "axes", "interleaved", "inverse", "src_dtype", "dst_dtype")]
 

@@ -249,8 +249,8 @@ def radius_tables(mask_bits: torch.Tensor, block_mask: torch.Tensor | None = Non
     dev = _require_device(mask_bits, block_mask)
     bits = mask_bits.contiguous()
     bm = None if block_mask is None else block_mask.to(torch.uint8).contiguous()
-    any_bits = torch.empty(2, B, NB, NB, dtype=torch.int64, device=dev)
-    tables = RadiusTables(torch.empty_like(bits), any_bits[0], any_bits[1])
+    tables = RadiusTables(torch.empty_like(bits), torch.empty(B, NB, NB, dtype=torch.int64, device=dev),
+                          torch.empty(B, NB, NB, dtype=torch.int64, device=dev))
     if B * N > 0:
         args = _native.MfRadiusTablesArgs(
             mask_bits=bits.data_ptr(), block_mask=_native.ptr(bm), mask_bits_t=tables.bits_t.data_ptr(),

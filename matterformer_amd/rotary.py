@@ -17,7 +17,6 @@ frequencies take none); a missing library raises.  CPU tensors take the torch fo
 
 from __future__ import annotations
 
-import ctypes
 import math
 from dataclasses import dataclass
 
@@ -155,38 +154,32 @@ def _rotate_torch(x: torch.Tensor, positions: torch.Tensor, frequencies: RotaryF
 
 
 class _Plan:
-    """What a launch and its gradient share: positions (B or 1, N, axes), frequencies and the pairs' layout; for packed
-    rows the slot map."""
+    """What a launch and its gradient share: positions (B or 1, N, axes), the table of frequencies with its axes and
+    gain, the pairs' layout; for packed rows the slot map."""
 
-    def __init__(self, positions, frequencies, interleaved, slot=None):
+    def __init__(self, positions, table, axes, gain, interleaved, slot=None):
         self.positions = positions
-        self.frequencies = frequencies
-        self.interleaved = interleaved
+        self.table = table
+        self.settings = (axes, gain, interleaved)
         self.slot = slot
 
 
-_I32x3 = ctypes.c_int32 * 3
-_I64x3 = ctypes.c_int64 * 3
-_I64x3x3 = _I64x3 * 3
-_PTRx3 = ctypes.c_void_p * 3
+_TURN = (1, 1, 0)  # q and k turn, v is copied
 
 
-def _launch(plan: _Plan, parts, *, batch: int, tokens: int, head_dim: int, inverse: bool, slot_side: int) -> None:
-    """parts: (src, src strides {batch, head, token}, dst, dst strides, heads, turned), src and dst (tensor, element
-    offset); the dtypes are those of the first part."""
-    pos, f = plan.positions, plan.frequencies
-    ps = pos.stride()
-    src, dst = parts[0][0][0], parts[0][2][0]
-    ssize, dsize = src.element_size(), dst.element_size()
+def _launch(plan: _Plan, src, src_strides, dst, dst_strides, heads, *, batch: int, tokens: int, head_dim: int,
+            inverse: bool, slot_side: int, src_dtype: torch.dtype, dst_dtype: torch.dtype,
+            device: torch.device) -> None:
+    """src, dst: three addresses (None past the last part); strides: nine, {batch, head, token} of each part."""
+    pos = plan.positions
+    axes, gain, interleaved = plan.settings
+    sb, sn, sa = pos.stride()
     args = _native.MfRotaryArgs(
-        _PTRx3(*[t.data_ptr() + at * ssize for (t, at), *_ in parts]),
-        _PTRx3(*[t.data_ptr() + at * dsize for _, _, (t, at), *_ in parts]),
-        _I64x3x3(*[p[1] for p in parts]), _I64x3x3(*[p[3] for p in parts]), _I32x3(*[p[4] for p in parts]),
-        _I32x3(*[p[5] for p in parts]), pos.data_ptr(), _I64x3(ps[0] if pos.shape[0] > 1 else 0, ps[1], ps[2]),
-        f.table.data_ptr(), _native.ptr(plan.slot), f.gain, _POSITION_TYPES[pos.dtype], slot_side, len(parts), batch,
-        tokens, head_dim, 2 * f.table.shape[0], f.axes, plan.interleaved, inverse, _native.dtype_code(src.dtype),
-        _native.dtype_code(dst.dtype))
-    _native.launch("mf_rotary", args, src.device)
+        *src, *dst, *src_strides, *dst_strides, *heads, *_TURN, pos.data_ptr(), sb if pos.shape[0] > 1 else 0, sn, sa,
+        plan.table.data_ptr(), _native.ptr(plan.slot), gain, _POSITION_TYPES[pos.dtype], slot_side,
+        3 if src[2] is not None else 2 if src[1] is not None else 1, batch, tokens, head_dim, 2 * plan.table.shape[0],
+        axes, interleaved, inverse, _native.dtype_code(src_dtype), _native.dtype_code(dst_dtype))
+    _native.launch("mf_rotary", args, device)
 
 
 def _unit(t: torch.Tensor) -> torch.Tensor:
@@ -200,28 +193,30 @@ def _strides(t: torch.Tensor) -> tuple:
 
 
 def _turn_heads(plan: _Plan, heads, inverse: bool) -> tuple[torch.Tensor, ...]:
-    """(B, H, N, D) heads -> turned contiguous heads, in one launch."""
+    """One or two (B, H, N, D) heads -> turned contiguous heads, in one launch."""
     outs = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in heads)
-    B, _, N, D = heads[0].shape
+    first = heads[0]
+    B, _, N, D = first.shape
     if B * N > 0:
-        parts = []
-        for t, o in zip(heads, outs):
-            t = _unit(t)
-            parts.append(((t, 0), _strides(t), (o, 0), _strides(o), t.shape[1], True))
-        _launch(plan, parts, batch=B, tokens=N, head_dim=D, inverse=inverse, slot_side=_native.MF_SLOT_NONE)
+        units = [_unit(t) for t in heads]
+        pad = 3 - len(units)
+        zeros = (0, 0, 0) * pad
+        _launch(plan, (*(t.data_ptr() for t in units), *(None,) * pad), (*(s for t in units for s in _strides(t)), *zeros),
+                (*(o.data_ptr() for o in outs), *(None,) * pad), (*(s for o in outs for s in o.stride()[:3]), *zeros),
+                (*(t.shape[1] for t in units), *(0,) * pad), batch=B, tokens=N, head_dim=D, inverse=inverse,
+                slot_side=_native.MF_SLOT_NONE, src_dtype=first.dtype, dst_dtype=first.dtype, device=first.device)
     return outs
 
 
 def _keep(ctx, plan: _Plan) -> None:
     """The plan for the gradient; its tensors as saved ones, so that a change in place before it is an error."""
-    ctx.save_for_backward(plan.positions, plan.frequencies.table, plan.slot)
-    ctx.plan = (plan.frequencies.axes, plan.frequencies.gain, plan.interleaved)
+    ctx.save_for_backward(plan.positions, plan.table, plan.slot)
+    ctx.settings = plan.settings
 
 
 def _kept(ctx) -> _Plan:
     positions, table, slot = ctx.saved_tensors
-    axes, gain, interleaved = ctx.plan
-    return _Plan(positions, RotaryFrequencies(table, axes, gain), interleaved, slot)
+    return _Plan(positions, table, *ctx.settings, slot)
 
 
 class _HeadsFunction(torch.autograd.Function):
@@ -236,26 +231,25 @@ class _HeadsFunction(torch.autograd.Function):
         return (None, *_turn_heads(_kept(ctx), grads, True))
 
 
-def _head_parts(counts, head_dim: int, batch_stride: int, row_stride: int):
-    """Offset, {batch, head, token} strides of each part inside rows of (H + 2 KV) head_dim columns."""
-    out, offset = [], 0
-    for heads in counts:
-        out.append((offset, (batch_stride, head_dim, row_stride), heads))
-        offset += heads * head_dim
-    return out
+def _row_parts(rows: torch.Tensor, counts, head_dim: int, packed: bool):
+    """Addresses and strides of q, k and v inside rows of (H + 2 KV) head_dim columns."""
+    at, size = rows.data_ptr(), rows.element_size() * head_dim
+    one = (0 if packed else rows.stride(0), head_dim, rows.stride(-2))
+    return (at, at + counts[0] * size, at + (counts[0] + counts[1]) * size), one * 3
 
 
 def _rows_to_heads(plan: _Plan, rows: torch.Tensor, counts, batch: int, tokens: int, head_dim: int, dtype):
     """rows (B, N, columns), or packed (T, columns) through plan.slot -> one (B, heads, N, D) tensor a part."""
     outs = tuple(torch.empty(batch, h, tokens, head_dim, dtype=dtype, device=rows.device) for h in counts)
-    packed = plan.slot is not None
-    rows = _unit(rows)
-    layout = _head_parts(counts, head_dim, 0 if packed else rows.stride(0), rows.stride(-2))
-    parts = [((rows, offset), strides, (o, 0), _strides(o), h, k < 2)
-             for k, ((offset, strides, h), o) in enumerate(zip(layout, outs))]
     if batch * tokens > 0:
-        _launch(plan, parts, batch=batch, tokens=tokens, head_dim=head_dim, inverse=False,
-                slot_side=_native.MF_SLOT_SRC if packed else _native.MF_SLOT_NONE)
+        packed = plan.slot is not None
+        rows = _unit(rows)
+        src, src_strides = _row_parts(rows, counts, head_dim, packed)
+        q, k, v = outs
+        _launch(plan, src, src_strides, (q.data_ptr(), k.data_ptr(), v.data_ptr()),
+                (*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]), counts, batch=batch, tokens=tokens,
+                head_dim=head_dim, inverse=False, slot_side=_native.MF_SLOT_SRC if packed else _native.MF_SLOT_NONE,
+                src_dtype=rows.dtype, dst_dtype=dtype, device=rows.device)
     return outs
 
 
@@ -273,13 +267,13 @@ class _RowsFunction(torch.autograd.Function):
         plan, (batch, tokens, head_dim), (shape, dtype) = _kept(ctx), ctx.sizes, ctx.rows
         packed = plan.slot is not None
         out = torch.empty(shape, dtype=dtype, device=grads[0].device)
-        layout = _head_parts(ctx.counts, head_dim, 0 if packed else out.stride(0), out.stride(-2))
-        parts = []
-        for k, ((offset, strides, h), g) in enumerate(zip(layout, (_unit(g) for g in grads))):
-            parts.append(((g, 0), _strides(g), (out, offset), strides, h, k < 2))
         if out.numel() > 0:
-            _launch(plan, parts, batch=batch, tokens=tokens, head_dim=head_dim, inverse=True,
-                    slot_side=_native.MF_SLOT_DST if packed else _native.MF_SLOT_NONE)
+            q, k, v = (_unit(g) for g in grads)
+            dst, dst_strides = _row_parts(out, ctx.counts, head_dim, packed)
+            _launch(plan, (q.data_ptr(), k.data_ptr(), v.data_ptr()), (*_strides(q), *_strides(k), *_strides(v)), dst,
+                    dst_strides, ctx.counts, batch=batch, tokens=tokens, head_dim=head_dim, inverse=True,
+                    slot_side=_native.MF_SLOT_DST if packed else _native.MF_SLOT_NONE, src_dtype=q.dtype,
+                    dst_dtype=dtype, device=out.device)
         return (None, out, None, None, None, None, None)
 
 
@@ -310,7 +304,7 @@ def apply_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         out = [_rotate_torch(t, pos, frequencies, interleaved).contiguous() for t in heads]
     else:
         _check_kernel(D, q.dtype)
-        plan = _Plan(pos, frequencies, interleaved)
+        plan = _Plan(pos, frequencies.table, frequencies.axes, frequencies.gain, interleaved)
         out = _HeadsFunction.apply(plan, *heads) if _native.takes_gradient(q, k) else _turn_heads(plan, heads, False)
     return (out[0], None) if k is None else (out[0], out[1])
 
@@ -351,7 +345,8 @@ def rotary_heads(rows: torch.Tensor, positions: torch.Tensor, frequencies: Rotar
     B, N, _ = rows.shape
     _check_kernel(D, rows.dtype)
     run = _RowsFunction.apply if _native.takes_gradient(rows) else _rows_to_heads
-    return run(_Plan(pos, frequencies, interleaved), rows, counts, B, N, D, rows.dtype)
+    plan = _Plan(pos, frequencies.table, frequencies.axes, frequencies.gain, interleaved)
+    return run(plan, rows, counts, B, N, D, rows.dtype)
 
 
 def _packed_rotary_heads(rows: torch.Tensor, slot: torch.Tensor, positions: torch.Tensor,
@@ -369,6 +364,6 @@ def _packed_rotary_heads(rows: torch.Tensor, slot: torch.Tensor, positions: torc
     pos = _check_positions(positions, B, W, frequencies, rows.device)
     _check_kernel(head_dim, rows.dtype)
     _check_kernel(head_dim, dtype)
-    plan = _Plan(pos, frequencies, interleaved, slot.contiguous())
+    plan = _Plan(pos, frequencies.table, frequencies.axes, frequencies.gain, interleaved, slot.contiguous())
     run = _RowsFunction.apply if _native.takes_gradient(rows) else _rows_to_heads
     return run(plan, rows, (heads, heads, heads), B, W, head_dim, dtype)

@@ -128,8 +128,8 @@ def test_c_entry_refuses_before_any_device_call():
     def args(**kw):
         a = _native.MfRotaryArgs(positions=fake, frequencies=fake, gain=1.0, parts=1, batch=1, tokens=4, head_dim=8,
                                  rotary_dim=8, axes=1, src_dtype=_native.MF_DTYPE_F32, dst_dtype=_native.MF_DTYPE_F32)
-        a.src[0] = a.dst[0] = fake
-        a.heads[0] = 1
+        a.src0 = a.dst0 = fake
+        a.heads0 = 1
         for key, value in kw.items():
             setattr(a, key, value)
         return a
@@ -144,6 +144,63 @@ def test_c_entry_refuses_before_any_device_call():
         assert match in _native.last_error()
     assert lib.mf_rotary(args(head_dim=264), None) == _native.MF_ERR_UNSUPPORTED
     bad = args()
-    bad.src_stride[0][0] = -8
+    bad.src_stride0 = -8
     assert lib.mf_rotary(bad, None) == _native.MF_ERR_INVALID_ARGUMENT and "strides" in _native.last_error()
     assert lib.mf_rotary(args(tokens=0), None) == _native.MF_OK
+
+
+def test_struct_has_the_header_layout(tmp_path):
+    """The flat fields lie where the C compiler puts the arrays' elements."""
+    import shutil
+    import subprocess
+    from pathlib import Path
+
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "mf_capi.h"', "int main(void) {"]
+    want = {}
+    for name, *_ in _native.MfRotaryArgs._fields_:
+        base = name.rstrip("0123456789")
+        field = name
+        if base != name:
+            i = int(name[len(base):])
+            field = f"{base}[{i // 3}][{i % 3}]" if base in ("src_stride", "dst_stride") else f"{base}[{i}]"
+        lines.append(f'  printf("{name} %zu\\n", offsetof(mf_rotary_args, {field}));')
+        want[name] = getattr(_native.MfRotaryArgs, name).offset
+    lines += ['  printf("size %zu\\n", sizeof(mf_rotary_args));', "  return 0;", "}"]
+    (tmp_path / "t.c").write_text("\n".join(lines))
+    include = Path(__file__).resolve().parents[1] / "include"
+    subprocess.run([cc, f"-I{include}", str(tmp_path / "t.c"), "-o", str(tmp_path / "t")], check=True)
+    out = subprocess.run([str(tmp_path / "t")], check=True, capture_output=True, text=True).stdout
+    got = {line.split()[0]: int(line.split()[1]) for line in out.splitlines()}
+    import ctypes
+
+    assert got.pop("size") == ctypes.sizeof(_native.MfRotaryArgs)
+    assert got == want
+
+
+@pytest.mark.parametrize("name,argtype", [("mf_radius_attn_args", _native.MfRadiusAttnArgs),
+                                          ("mf_radius_tables_args", _native.MfRadiusTablesArgs),
+                                          ("mf_radius_attn_bwd_args", _native.MfRadiusAttnBwdArgs),
+                                          ("mf_gated_linear_args", _native.MfGatedLinearArgs),
+                                          ("mf_gated_linear_bwd_args", _native.MfGatedLinearBwdArgs)])
+def test_the_other_new_structs_have_the_header_layout(tmp_path, name, argtype):
+    import ctypes
+    import shutil
+    import subprocess
+    from pathlib import Path
+
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "mf_capi.h"', "int main(void) {"]
+    lines += [f'  printf("{f} %zu\\n", offsetof({name}, {f}));' for f, *_ in argtype._fields_]
+    lines += [f'  printf("size %zu\\n", sizeof({name}));', "  return 0;", "}"]
+    (tmp_path / "t.c").write_text("\n".join(lines))
+    include = Path(__file__).resolve().parents[1] / "include"
+    subprocess.run([cc, f"-I{include}", str(tmp_path / "t.c"), "-o", str(tmp_path / "t")], check=True)
+    out = subprocess.run([str(tmp_path / "t")], check=True, capture_output=True, text=True).stdout
+    got = {line.split()[0]: int(line.split()[1]) for line in out.splitlines()}
+    assert got.pop("size") == ctypes.sizeof(argtype)
+    assert got == {f: getattr(argtype, f).offset for f, *_ in argtype._fields_}
