@@ -694,9 +694,9 @@ __global__ void __launch_bounds__(256) pad_kernel(const T* src, T* dst, int64_t 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 // How a product is cut.  Tiles of 256 x 256 (16-bit types) run one workgroup per CU, tiles of 128 x 128 two (fp32: one
-// fills the matrix cores); `slots` is what is to be resident at once.  Tiles that fill every slot are computed whole; the rest, which would leave slots idle for
-// a whole tile's time, are cut along K so that their pieces fill the slots, where K is long enough to pay for writing
-// and adding the pieces' fp32 sums.
+// fills the matrix cores); `slots` is what is to be resident at once.  Tiles that fill every slot are computed whole;
+// the rest, which would leave slots idle for a whole tile's time, are cut along K so that their pieces fill the slots,
+// where K is long enough to pay for writing and adding the pieces' fp32 sums.
 struct Cut {
   bool large;
   int bn;  // columns of a tile: 256 (large), 128 or 64
@@ -722,9 +722,12 @@ Cut cut_tiles(int64_t m, int64_t n, int64_t k, int esize, bool large, bool split
   return c;
 }
 constexpr int kFewTokens = 64;  // the forward of few_kernel
-// kFwd and kBwd: large tiles when every CU gets one.  fp32, whose matrix rate is a sixteenth, takes small ones.
+// kFwd and kBwd: large tiles once the small ones need more than one round of two a CU, that is when more than half the
+// CUs get a large one.  bf16, C 512, F 2048, large against small: 1400 tokens (96 large tiles) 17.6 and 13.6 us, 2000
+// (128) 17.9 and 14.2, 2304 (144) 18.9 and 22.6, 3500 (224) 20.5 and 26.0.  fp32, whose matrix rate is a sixteenth,
+// takes small ones.
 Cut cut_gated(int64_t f, int64_t t, int64_t k, int esize, int num_cus) {
-  const bool large = esize == 2 && ((2 * f + 255) / 256) * ((t + 255) / 256) >= num_cus;
+  const bool large = esize == 2 && 2 * ((2 * f + 255) / 256) * ((t + 255) / 256) > num_cus;
   // a large tile is 128 of f and their gate and up rows, a small one 64
   Cut c = cut_tiles(2 * f, t, k, esize, large, false, num_cus);
   const int64_t fb = large ? 128 : 64;

@@ -261,3 +261,11 @@ def test_two_calls_in_flight(cuda):
     g2 = torch.autograd.grad(two, leaf, go)[0]
     g1 = torch.autograd.grad(one, leaf, go)[0]
     assert torch.equal(g1, _run(x, w, b, go, "silu")[1][0]) and torch.equal(g2, _run(x, w, b, go, "relu")[1][0])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T", [2047, 2305])
+def test_either_side_of_the_tile_rule(cuda, dtype, T):
+    """Half as many large tiles as CUs and a few more, rows that end inside a tile."""
+    x, w, b, go = _inputs(T, 72, 2040, dtype, True, 22, cuda)
+    _check(x, w, b, go, "silu", *_run(x, w, b, go, "silu"))
