@@ -683,11 +683,12 @@ __global__ void __launch_bounds__(256) bias_kernel(const float* part, T* out, in
 // are no multiple of 16 bytes.
 template <typename T>
 __global__ void __launch_bounds__(256) pad_kernel(const T* src, T* dst, int64_t rows, int cols, int64_t ld, int pitch) {
-  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= rows * pitch) return;
-  const int64_t r = i / pitch;
-  const int c = int(i - r * pitch);
-  dst[i] = c < cols ? src[r * ld + c] : T(0.0f);
+  // a grid of 2^32 threads and more is no launch: every thread goes on by the grid's size
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < rows * pitch; i += int64_t(gridDim.x) * 256) {
+    const int64_t r = i / pitch;
+    const int c = int(i - r * pitch);
+    dst[i] = c < cols ? src[r * ld + c] : T(0.0f);
+  }
 }
 
 // -- host ----------------------------------------------------------------------------------------------------
@@ -808,8 +809,8 @@ template <typename T>
 void pad_rows(const void* src, void* dst, int64_t rows, int64_t cols, int64_t ld, int64_t pitch, hipStream_t s) {
   const int64_t n = rows * pitch;
   if (n > 0)
-    hipLaunchKernelGGL(pad_kernel<T>, dim3(unsigned((n + 255) / 256)), dim3(256), 0, s, static_cast<const T*>(src),
-                       static_cast<T*>(dst), rows, int(cols), ld, int(pitch));
+    hipLaunchKernelGGL(pad_kernel<T>, dim3(unsigned(std::min<int64_t>((n + 255) / 256, 1 << 20))), dim3(256), 0, s,
+                       static_cast<const T*>(src), static_cast<T*>(dst), rows, int(cols), ld, int(pitch));
 }
 
 // x and W, as the tile kernel reads them: in place, or their aligned copies at ws

@@ -485,7 +485,8 @@ extern "C" int mf_radius_tables(const mf_radius_tables_args* a, void* stream) {
   TableParams p = {a->mask_bits, a->block_mask, a->mask_bits_t, a->key_any, a->query_any, a->batch, a->atoms,
                    (a->atoms + 31) / 32, (a->atoms + kTile - 1) / kTile};
   const int64_t blocks = (int64_t(p.B) * p.NB * p.NB + 3) / 4;
-  if (blocks > 0x7fffffffLL) return fail(MF_ERR_UNSUPPORTED, "mf_radius_tables: batch * tiles too large");
+  if (blocks * kThreads > 0xffffffffLL)  // threads of a launch
+    return fail(MF_ERR_UNSUPPORTED, "mf_radius_tables: batch * tiles too large");
   hipLaunchKernelGGL(radius_tables_kernel, dim3(unsigned(blocks)), dim3(kThreads), 0, static_cast<hipStream_t>(stream), p);
   MF_HIP_CHECK(hipGetLastError());
   return MF_OK;
@@ -521,7 +522,7 @@ extern "C" int mf_radius_attn_bwd(const mf_radius_attn_bwd_args* a, void* stream
   if (a->atoms > 65536) return fail(MF_ERR_UNSUPPORTED, "mf_radius_attn_bwd: atoms must be <= 65536");
   const Sizes z = sizes(a->batch, a->heads, a->atoms, a->dtype);
   const int64_t units = int64_t(a->batch) * a->heads * z.NB;
-  if (2 * units > 0x7fffffffLL - 8)
+  if ((2 * units + 7) / 8 * 8 * kThreads > 0xffffffffLL)  // threads of a launch
     return fail(MF_ERR_UNSUPPORTED, "mf_radius_attn_bwd: batch * heads * tiles too large");
   if (!a->workspace || a->workspace_bytes < z.total() || reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0)
     return fail(MF_ERR_INVALID_ARGUMENT, "mf_radius_attn_bwd: the workspace must be 16-byte aligned and hold "

@@ -371,6 +371,8 @@ extern "C" int mf_rotary(const mf_rotary_args* a, void* stream) {
   int64_t slices = std::max<int64_t>(1, std::min<int64_t>((heads + kHeads - 1) / kHeads, 1024 / blocks));
   p.HS = int((heads + slices - 1) / slices);
   slices = (heads + p.HS - 1) / p.HS;
+  if (blocks * kThreads > 0xffffffffLL)  // threads of a launch
+    return fail(MF_ERR_UNSUPPORTED, "mf_rotary: too many tokens for one launch");
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(slices));
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (a->src_dtype) {

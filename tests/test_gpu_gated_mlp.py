@@ -269,3 +269,29 @@ def test_either_side_of_the_tile_rule(cuda, dtype, T):
     """Half as many large tiles as CUs and a few more, rows that end inside a tile."""
     x, w, b, go = _inputs(T, 72, 2040, dtype, True, 22, cuda)
     _check(x, w, b, go, "silu", *_run(x, w, b, go, "silu"))
+
+
+def test_aligned_copy_of_2_32_elements(cuda):
+    """Rows of 255 channels are copied into rows of 256: 2^32 + 2^14 elements, more than a launch has threads."""
+    x = torch.empty(2 ** 24 + 64, 255, dtype=torch.bfloat16, device=cuda).normal_()
+    _, w, b, _ = _inputs(1, 255, 4, torch.bfloat16, True, 23, cuda)
+    with torch.no_grad():
+        out = gated_linear(x, w, b)
+    for rows in (slice(0, 128), slice(2 ** 24 - 64, 2 ** 24 + 64)):
+        _check(x[rows], w, b, x[rows, :4], "silu", out[rows])
+
+
+def test_c_entries_refuse_a_workspace_off_16_bytes(cuda):
+    from matterformer_amd import _native
+
+    x, w, _, go = _inputs(4, 63, 32, torch.bfloat16, False, 24, cuda)
+    out, work = torch.zeros(4, 32, dtype=x.dtype, device=cuda), torch.zeros(1 << 20, dtype=torch.uint8, device=cuda)
+    a = _native.MfGatedLinearArgs(x=x.data_ptr(), weight=w.data_ptr(), out=out.data_ptr(), workspace=work.data_ptr() + 8,
+                                  workspace_bytes=work.numel() - 8, x_stride=63, tokens=4, channels=63, hidden=32,
+                                  dtype=_native.MF_DTYPE_BF16)
+    b = _native.MfGatedLinearBwdArgs(fwd=a, grad_out=go.data_ptr(), dx=x.data_ptr(), workspace=work.data_ptr() + 8,
+                                     workspace_bytes=work.numel() - 8)
+    for name, args in (("mf_gated_linear", a), ("mf_gated_linear_bwd", b)):
+        assert getattr(_native.lib(), name)(args, None) == _native.MF_ERR_INVALID_ARGUMENT
+        assert "16-byte aligned" in _native.last_error()
+    assert not out.any() and not work.any()

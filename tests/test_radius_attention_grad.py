@@ -49,3 +49,16 @@ def test_tables_entry_refuses_before_any_device_call():
     assert lib.mf_radius_tables(args(atoms=-1), None) == invalid
     assert lib.mf_radius_tables(args(atoms=65537), None) == _native.MF_ERR_UNSUPPORTED
     assert lib.mf_radius_tables(args(batch=0), None) == _native.MF_OK
+
+
+def test_entries_refuse_more_threads_than_a_launch_has():
+    lib = _native.lib()
+    fake = 1 << 20
+    names = ("q", "k", "v", "out", "lse", "grad_out", "mask_bits", "mask_bits_t", "key_any", "query_any", "dq", "dk", "dv",
+             "workspace")
+    a = _native.MfRadiusAttnBwdArgs(**{n: fake for n in names}, workspace_bytes=2 ** 60, scale=0.125, batch=2 ** 23, heads=1,
+                                    atoms=1, head_dim=32, dtype=_native.MF_DTYPE_BF16)
+    assert lib.mf_radius_attn_bwd(a, None) == _native.MF_ERR_UNSUPPORTED and "too large" in _native.last_error()
+    t = _native.MfRadiusTablesArgs(**{n: fake for n in ("mask_bits", "mask_bits_t", "key_any", "query_any")}, batch=2 ** 26,
+                                   atoms=1)
+    assert lib.mf_radius_tables(t, None) == _native.MF_ERR_UNSUPPORTED and "too large" in _native.last_error()

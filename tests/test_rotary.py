@@ -204,3 +204,12 @@ def test_the_other_new_structs_have_the_header_layout(tmp_path, name, argtype):
     got = {line.split()[0]: int(line.split()[1]) for line in out.splitlines()}
     assert got.pop("size") == ctypes.sizeof(argtype)
     assert got == {f: getattr(argtype, f).offset for f, *_ in argtype._fields_}
+
+
+def test_c_entry_refuses_more_threads_than_a_launch_has():
+    fake = 1 << 20
+    a = _native.MfRotaryArgs(positions=fake, frequencies=fake, gain=1.0, parts=1, batch=1, tokens=2 ** 28, head_dim=2,
+                             rotary_dim=2, axes=1, src_dtype=_native.MF_DTYPE_BF16, dst_dtype=_native.MF_DTYPE_BF16)
+    a.src0 = a.dst0 = fake
+    a.heads0 = 1
+    assert _native.lib().mf_rotary(a, None) == _native.MF_ERR_UNSUPPORTED and "too many tokens" in _native.last_error()
