@@ -253,15 +253,14 @@ struct Params {
                       // [column tiles' waves][2 Fp]
   const void* bias;   // [2F] or null
   const void* go;     // kBwd: [N, F]
-  int vec;            // rows of out (and go) are 16-byte aligned
 };
 
-// 16 consecutive elements, of which the first n exist
+// 16 consecutive elements, of which the first n exist; rows of odd lengths start off 16 bytes, which wide accesses may
 template <typename T>
-__device__ __forceinline__ void store16(T* p, const float (&v)[16], int n, bool vec) {
-  typedef T V __attribute__((ext_vector_type(16 / sizeof(T))));
+__device__ __forceinline__ void store16(T* p, const float (&v)[16], int n) {
+  typedef T V __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
   constexpr int E = kEpc<T>;
-  if (vec && n >= 16) {
+  if (n >= 16) {
 #pragma unroll
     for (int i = 0; i < 16 / E; ++i) {
       V o;
@@ -276,10 +275,10 @@ __device__ __forceinline__ void store16(T* p, const float (&v)[16], int n, bool 
   }
 }
 template <typename T>
-__device__ __forceinline__ void load16(const T* p, float (&v)[16], int n, bool vec) {
-  typedef T V __attribute__((ext_vector_type(16 / sizeof(T))));
+__device__ __forceinline__ void load16(const T* p, float (&v)[16], int n) {
+  typedef T V __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
   constexpr int E = kEpc<T>;
-  if (vec && n >= 16) {
+  if (n >= 16) {
 #pragma unroll
     for (int i = 0; i < 16 / E; ++i) {
       const V o = reinterpret_cast<const V*>(p)[i];
@@ -487,7 +486,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             h[e] = act_value<decltype(act)::value, kFast>(acc[0][e >> 2][i][e & 3]) * acc[1][e >> 2][i][e & 3];
-          if (n < p.N) store16(static_cast<T*>(p.out) + int64_t(n) * p.ldo + f0, h, left, p.vec);
+          if (n < p.N) store16(static_cast<T*>(p.out) + int64_t(n) * p.ldo + f0, h, left);
         }
       });
     } else {
@@ -497,7 +496,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
         for (int i = 0; i < NT; ++i) {
           const int n = n0 + (wn * NT + i) * 16 + r16;
           float go[16], da[16], db[16];
-          if (n < p.N) load16(static_cast<const T*>(p.go) + int64_t(n) * p.F + f0, go, left, p.vec);
+          if (n < p.N) load16(static_cast<const T*>(p.go) + int64_t(n) * p.F + f0, go, left);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float y, dy;
@@ -510,8 +509,8 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
           }
           if (n < p.N && f0 < p.Fp) {
             T* o = static_cast<T*>(p.out) + int64_t(n) * p.ldo + f0;
-            store16(o, da, 16, true);
-            store16(o + p.Fp, db, 16, true);
+            store16(o, da, 16);
+            store16(o + p.Fp, db, 16);
           }
         }
       });
@@ -527,7 +526,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
             for (int i = 0; i < NT; ++i) v += acc[q][e >> 2][i][e & 3];
             sum[e] = group16_sum(v);
           }
-          if (r16 == 0 && f0 < p.Fp) store16(row + q * p.Fp, sum, 16, true);
+          if (r16 == 0 && f0 < p.Fp) store16(row + q * p.Fp, sum, 16);
         }
       }
     }
@@ -544,9 +543,9 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = acc[q][e >> 2][i][e & 3];
         if (!whole) {
-          store16(p.part + ((int64_t(t - p.full) * p.splits + split) * BN + nl) * BM + ml, v, 16, true);
+          store16(p.part + ((int64_t(t - p.full) * p.splits + split) * BN + nl) * BM + ml, v, 16);
         } else if (out_row<MODE>(p, n) && m < p.ldo) {
-          store16(static_cast<T*>(p.out) + int64_t(n) * p.ldo + m, v, int(p.ldo) - m, p.vec);
+          store16(static_cast<T*>(p.out) + int64_t(n) * p.ldo + m, v, int(p.ldo) - m);
         }
       }
     }
@@ -647,8 +646,8 @@ __global__ void __launch_bounds__(256) tail_kernel(Params p, int bm, int bn) {
   mf_f32x4 v = *reinterpret_cast<const mf_f32x4*>(src);
   for (int s = 1; s < p.splits; ++s) v += *reinterpret_cast<const mf_f32x4*>(src + int64_t(s) * bn * bm);
   T* out = static_cast<T*>(p.out) + int64_t(n) * p.ldo + m;
-  if (p.vec) {
-    typedef T V __attribute__((ext_vector_type(4)));
+  if (m + 4 <= p.ldo) {
+    typedef T V __attribute__((ext_vector_type(4), aligned(sizeof(T))));
     V o;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = Elem<T>::from_f32(v[e]);
@@ -850,7 +849,6 @@ int forward(const mf_gated_linear_args* a, const Plan& q, hipStream_t s) {
   p.out = a->out;
   p.ldo = q.F;
   p.bias = a->bias;
-  p.vec = q.F * q.esize % 16 == 0 && aligned16(a->out);
   const dim3 few(unsigned((q.F + 15) / 16));
   if (q.T <= 16) hipLaunchKernelGGL((few_kernel<T, 1>), few, dim3(256), 0, s, p);
   else if (q.T <= 32) hipLaunchKernelGGL((few_kernel<T, 2>), few, dim3(256), 0, s, p);
@@ -880,7 +878,6 @@ int backward(const mf_gated_linear_bwd_args* a, const Plan& q, hipStream_t s) {
   p.bias = f.bias;
   p.go = a->grad_out;
   p.part = sums;
-  p.vec = q.F * q.esize % 16 == 0 && aligned16(a->grad_out);
   if (q.T > 0) launch_gemm<T, kBwd>(p, q.gated, s);
   MF_HIP_CHECK(hipGetLastError());
   if (a->dbias) {
@@ -901,7 +898,6 @@ int backward(const mf_gated_linear_bwd_args* a, const Plan& q, hipStream_t s) {
     d.out = a->dx;
     d.ldo = q.C;
     d.part = reinterpret_cast<float*>(ws);
-    d.vec = q.C * q.esize % 16 == 0 && aligned16(a->dx);
     launch_gemm<T, kDx>(d, q.dx, s);
     MF_HIP_CHECK(hipGetLastError());
     ws += q.dx.bytes;
@@ -918,7 +914,6 @@ int backward(const mf_gated_linear_bwd_args* a, const Plan& q, hipStream_t s) {
     d.out = a->dweight;
     d.ldo = q.C;
     d.part = reinterpret_cast<float*>(ws);
-    d.vec = q.C * q.esize % 16 == 0 && aligned16(a->dweight);
     launch_gemm<T, kDw>(d, q.dw, s);
     MF_HIP_CHECK(hipGetLastError());
   }
