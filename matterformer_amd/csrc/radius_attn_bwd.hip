@@ -32,8 +32,9 @@
 // Sums are fp32.  P and dS are rounded to the operands' type for the second
 // products, as any 16-bit matrix product's input is.  fp16 has no room for dS of
 // small or large gradients, so there dS is kept times 2^e, e per (molecule,
-// head) from |dP - delta| <= 2 max|go| max|v| + max|dlse| (Cauchy-Schwarz) so that it
-// stays below 2^14; bf16 has fp32's range and needs none.
+// head) from |dP - delta| <= 2 max|go| max|v| + max|dlse| (Cauchy-Schwarz, over the
+// rows that have a partner) so that it stays below 2^14; bf16 has fp32's range and
+// needs none.
 //
 // Rows that no column of the tile is paired with (padding, atoms without a
 // neighbour) are staged as zeros, so that whatever they hold, NaN too, reaches
@@ -138,6 +139,20 @@ __global__ void __launch_bounds__(kThreads) radius_rows_kernel(Params p) {
   typedef T T8 __attribute__((ext_vector_type(8)));
   float gmax = 0.0f, vmax = 0.0f, lmax = 0.0f;
   float* dst = p.rows + (bh * p.NB + tile) * 2 * kTile;
+  // rows of the tile that a pair reads, as queries (go, dlse) and as keys (v): only they decide the scale
+  unsigned long long queries = 0, keys = 0;
+  if (p.peak) {
+    const int64_t first = bh / p.H * p.NB * p.NB + tile;
+    for (int t = lane; t < p.NB; t += 64) {
+      queries |= p.qry_any[first + int64_t(t) * p.NB];
+      keys |= p.key_any[first + int64_t(t) * p.NB];
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) {
+      queries |= __shfl_xor(queries, off, 64);
+      keys |= __shfl_xor(keys, off, 64);
+    }
+  }
 #pragma unroll
   for (int pass = 0; pass < kTile / (4 * RPW); ++pass) {
     const int r = (pass * 4 + wave) * RPW + lane / L;
@@ -169,13 +184,14 @@ __global__ void __launch_bounds__(kThreads) radius_rows_kernel(Params p) {
       gg += __shfl_xor(gg, off, 64);
       vv += __shfl_xor(vv, off, 64);
     }
-    // rows that are not finite do not decide the other rows' scale
-    gmax = fmaxf(gmax, gg <= 3.0e38f ? gg : 0.0f);
-    vmax = fmaxf(vmax, vv <= 3.0e38f ? vv : 0.0f);
+    // nor do rows that are not finite
+    const bool query = (queries >> r) & 1, key = (keys >> r) & 1;
+    gmax = fmaxf(gmax, query && gg <= 3.0e38f ? gg : 0.0f);
+    vmax = fmaxf(vmax, key && vv <= 3.0e38f ? vv : 0.0f);
     if (lane % L == 0) {
       const bool in = row < p.N;
       const float dl = in && p.dlse ? p.dlse[bh * p.N + row] : 0.0f;
-      lmax = fmaxf(lmax, fabsf(dl) <= 3.0e38f ? fabsf(dl) : 0.0f);
+      lmax = fmaxf(lmax, query && fabsf(dl) <= 3.0e38f ? fabsf(dl) : 0.0f);
       dst[r] = in ? p.lse[bh * p.N + row] * kLog2e : 0.0f;
       dst[kTile + r] = in ? dl - dot : 0.0f;
     }

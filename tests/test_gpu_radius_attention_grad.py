@@ -306,3 +306,26 @@ def test_forward_with_tables(cuda, D, scale, N):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     with pytest.raises(ValueError, match="radius_tables of this call"):
         radius_attention(q[:1], k[:1], v[:1], bits[:1], tables=tables)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N", [100, 300])
+def test_large_finite_rows_without_a_partner_reach_nothing(cuda, dtype, N):
+    """6e4 (near fp16's largest number) where nobody is paired: the scale of fp16's dS must not follow it."""
+    q, k, v, go, gen = operands(2, 2, N, 64, dtype, 13, cuda)
+    allowed = mask_of("ragged", 2, N, gen)
+    bits = pack(allowed).to(cuda)
+    no_key = ~allowed.any(2).to(cuda)[:, None, :]
+    no_query = ~allowed.any(1).to(cuda)[:, None, :]
+    assert no_key[1].any() and no_query[1].any()
+    glse = torch.randn(2, 2, N, generator=gen).to(cuda)
+
+    def grads(q, k, v, go, glse):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        return torch.autograd.grad(radius_attention(*leaves, bits, return_lse=True), leaves, (go, glse))
+
+    want = grads(q, k, v, go, glse)
+    bad = [t.masked_fill(m[..., None], 6e4) for t, m in ((q, no_key), (k, no_query), (v, no_query), (go, no_key))]
+    got = grads(*bad, glse.masked_fill(no_key, 1e30))
+    for g, w, name in zip(got, want, ("dq", "dk", "dv")):
+        assert torch.equal(g, w), name
