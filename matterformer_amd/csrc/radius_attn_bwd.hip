@@ -424,8 +424,9 @@ __device__ __forceinline__ void bwd_unit(const Params& p, int unit, char* x0, ch
     Op4 vx, vy;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      vx[r] = Elem<T>::from_f32(seen ? ax[n][r] * down : 0.0f);  // a NaN row without a pair too
-      if constexpr (KEYS) vy[r] = Elem<T>::from_f32(ay[n][r]);
+      // a column without a pair: zeros, whatever it holds and whatever the tile's other rows hold
+      vx[r] = Elem<T>::from_f32(seen ? ax[n][r] * down : 0.0f);
+      if constexpr (KEYS) vy[r] = Elem<T>::from_f32(seen ? ay[n][r] : 0.0f);
     }
     const int64_t at = int64_t(col) * D + 16 * n + 4 * g;
     *reinterpret_cast<Op4*>(ox + at) = vx;

@@ -329,3 +329,15 @@ def test_large_finite_rows_without_a_partner_reach_nothing(cuda, dtype, N):
     got = grads(*bad, glse.masked_fill(no_key, 1e30))
     for g, w, name in zip(got, want, ("dq", "dk", "dv")):
         assert torch.equal(g, w), name
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_keys_without_a_query_get_zeros_beside_a_row_that_is_not_finite(cuda, dtype):
+    """Where a paired row's gradient is not finite, keys of its tile that nobody attends still get zeros."""
+    q, k, v, go, gen = operands(1, 2, 60, 32, dtype, 14, cuda)
+    allowed = mask_of("random", 1, 60, gen)
+    allowed[:, :, [3, 40]] = False
+    go[0, 1, 7, 5] = float("inf")
+    dq, dk, dv = gradients(q, k, v, go, pack(allowed).to(cuda), None)
+    for t in (dk, dv):
+        assert torch.equal(t[:, :, [3, 40]], torch.zeros_like(t[:, :, [3, 40]]))
