@@ -33,8 +33,9 @@
 // products, as any 16-bit matrix product's input is.  fp16 has no room for dS of
 // small or large gradients, so there dS is kept times 2^e, e per (molecule,
 // head) from |dP - delta| <= 2 max|go| max|v| + max|dlse| (Cauchy-Schwarz, over the
-// rows that have a partner) so that it stays below 2^14; bf16 has fp32's range and
-// needs none.
+// rows that have a partner) so that it stays below 2^14, and P times 2^12 (a key of
+// weight 3e-9 still counts), which the stored lse carries; bf16 has fp32's range and
+// needs neither.
 //
 // Rows that no column of the tile is paired with (padding, atoms without a
 // neighbour) are staged as zeros, so that whatever they hold, NaN too, reaches
@@ -49,6 +50,7 @@ namespace rattn_bwd {
 
 constexpr int kTile = 64;
 constexpr int kThreads = 256;
+constexpr float kProbBits = 12.0f;  // fp16: P is kept times 2^12; it is at most 1 but for the roundings of lse
 
 struct Params {
   const void* q;
@@ -66,7 +68,7 @@ struct Params {
   const uint32_t* bits_t;   // [B, N, W] the transposed mask
   const uint64_t* key_any;  // [B, NB query tiles, NB key tiles] keys of the tile with a query
   const uint64_t* qry_any;  // [B, NB key tiles, NB query tiles] queries of the tile with a key
-  float* rows;        // [B H, NB, 2, 64]: lse log2(e), then -delta, of every query tile
+  float* rows;        // [B H, NB, 2, 64]: lse log2(e) (fp16: less kProbBits), then -delta, of every query tile
   float4* peak;       // fp16: [B H, NB] max |go|^2, |v|^2 and |dlse| of a tile
   float scale;
   int B, H, N, W, NB;
@@ -192,7 +194,8 @@ __global__ void __launch_bounds__(kThreads) radius_rows_kernel(Params p) {
       const bool in = row < p.N;
       const float dl = in && p.dlse ? p.dlse[bh * p.N + row] : 0.0f;
       lmax = fmaxf(lmax, query && fabsf(dl) <= 3.0e38f ? fabsf(dl) : 0.0f);
-      dst[r] = in ? p.lse[bh * p.N + row] * kLog2e : 0.0f;
+      constexpr float kLess = __is_same(T, _Float16) ? kProbBits : 0.0f;
+      dst[r] = in ? fmaf(p.lse[bh * p.N + row], kLog2e, -kLess) : 0.0f;
       dst[kTile + r] = in ? dl - dot : 0.0f;
     }
   }
@@ -263,7 +266,7 @@ __device__ __forceinline__ void bwd_unit(const Params& p, int unit, char* x0, ch
     clse = r[0];
     cdelta = r[kTile];
   }
-  float up = 1.0f, down = p.scale;  // dS is kept times `up`
+  float up = 1.0f, down = p.scale;  // dS is kept times `up` (fp16: P comes times 2^kProbBits)
   if constexpr (kHalf) {
     float gm = 0.0f, vm = 0.0f, lm = 0.0f;
     for (int i = lane; i < p.NB; i += 64) {
@@ -281,6 +284,7 @@ __device__ __forceinline__ void bwd_unit(const Params& p, int unit, char* x0, ch
       up = ldexpf(1.0f, e);
       down = p.scale * ldexpf(1.0f, -e);
     }
+    up *= exp2f(-kProbBits);
   }
   const float slog = p.scale * kLog2e;
 
@@ -426,7 +430,7 @@ __device__ __forceinline__ void bwd_unit(const Params& p, int unit, char* x0, ch
     for (int r = 0; r < 4; ++r) {
       // a column without a pair: zeros, whatever it holds and whatever the tile's other rows hold
       vx[r] = Elem<T>::from_f32(seen ? ax[n][r] * down : 0.0f);
-      if constexpr (KEYS) vy[r] = Elem<T>::from_f32(seen ? ay[n][r] : 0.0f);
+      if constexpr (KEYS) vy[r] = Elem<T>::from_f32(seen ? ay[n][r] * (kHalf ? exp2f(-kProbBits) : 1.0f) : 0.0f);
     }
     const int64_t at = int64_t(col) * D + 16 * n + 4 * g;
     *reinterpret_cast<Op4*>(ox + at) = vx;

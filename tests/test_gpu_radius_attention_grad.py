@@ -341,3 +341,27 @@ def test_keys_without_a_query_get_zeros_beside_a_row_that_is_not_finite(cuda, dt
     dq, dk, dv = gradients(q, k, v, go, pack(allowed).to(cuda), None)
     for t in (dk, dv):
         assert torch.equal(t[:, :, [3, 40]], torch.zeros_like(t[:, :, [3, 40]]))
+
+
+def test_value_gradients_of_keys_with_little_weight(cuda):
+    """fp16: a key of weight 3e-9 in every row, gradients of 1e3: its dv of 1.2e-4 is within the type, though the weight
+    by itself is below the type's smallest number.
+
+    P is kept times 2^12, so what rounding it leaves is half a step: t relative, or 2^-25 2^-12 below the normal numbers;
+    the logits here are sums of one exact product, so P's own error is the exponential's and lse's: 2^-20 + t + N u."""
+    N, t = 40, 2.0 ** -11
+    gen = torch.Generator().manual_seed(15)
+    q = torch.zeros(1, 1, N, 32)
+    k = torch.zeros(1, 1, N, 32)
+    q[..., 0] = 4.0
+    k[0, 0, 1, 0] = -4.0  # logit -16 against 0
+    v = torch.randn(1, 1, N, 32, generator=gen)
+    go = torch.randn(1, 1, N, 32, generator=gen).abs() * 1e3
+    q, k, v, go = (x.to(torch.float16).to(cuda) for x in (q, k, v, go))
+    allowed = torch.ones(1, N, N, dtype=torch.bool)
+    got = gradients(q, k, v, go, pack(allowed).to(cuda), None, scale=1.0)[2]
+    P = torch.softmax(q.double() @ k.double().mT, -1)
+    want = P.mT @ go.double()
+    slack = (P * (2 * t + 2 * N * U + 2.0 ** -20) + 2.0 ** -37).mT @ go.double().abs()
+    assert float(want[0, 0, 1].min()) > 5e-5
+    check(got, want, slack, "dv")
