@@ -763,7 +763,9 @@ int mf_rotary(const mf_rotary_args* args, void* stream);
 /*   out = activation(a) * b                                                 */
 /* in one kernel: sums, activation and product in fp32, out rounded once.    */
 /* Backward, for grad_out = dL/dout (a and b are formed again):              */
-/*   dA = grad_out b act'(a),  dB = grad_out act(a)   (rounded to dtype)     */
+/*   dA = grad_out b act'(a),  dB = grad_out act(a)   (rounded to dtype;     */
+/*     fp16: a token's values times a power of two, so that none overflows   */
+/*     and small ones keep their bits)                                       */
 /*   dx = [dA dB] weight,  dweight = [dA dB]^T x,  dbias = column sums of    */
 /* the unrounded [dA dB]; any of the three may be NULL.  Every sum is in a   */
 /* fixed order (two calls give identical bits).  Workspaces need no fill:    */

@@ -15,6 +15,13 @@
 // them to the 16-bit type before the derivative.  [dA dB] is rounded to the operands' type for the two
 // products that follow, as any 16-bit matrix product's input is.
 //
+// fp16 has no room for [dA dB] of large or small gradients (go of 3e4 times b of 4 overflows although dx may be small), so
+// there row n is kept times 2^e_n, e_n from |dA|, |dB| <= 1.25 max|go_n| max(|x_n| max|W| + max|bias|, 1), the norms Euclidean
+// (Cauchy-Schwarz; 1.25 covers the activations' derivatives, at most 1.13), so that the bound lies in [2^13, 2^14).  By row,
+// because rows of dx have nothing to do with each other; dW, a sum over them, multiplies its operand by 2^(E - e_n), E the
+// smallest of all.  Two launches before the products (7 and 47 us of 32768 x 768 x 2048, 7 and 9 of 2738 x 512 x 2048) and
+// what it adds to them: the backward takes 888 and 120 us there, without the scales 766 and 102.
+//
 // All three products run on one tile kernel.  Its matrix-core "row" operand is
 // the output's contiguous axis (h's columns, dx's and dW's channels), the
 // "column" operand the output's rows, so that a lane ends with 16 consecutive
@@ -253,6 +260,11 @@ struct Params {
                       // [column tiles' waves][2 Fp]
   const void* bias;   // [2F] or null
   const void* go;     // kBwd: [N, F]
+  // fp16's [dA dB]: row n is kept times 2^exps[n] (kBwd, kDx); *lowest is the smallest of them (kBwd, kDw) and factors[n]
+  // 2^(*lowest - exps[n]), zero up to a multiple of 64 (written by kBwd, read by kDw)
+  int* exps;
+  int* lowest;
+  _Float16* factors;
 };
 
 // 16 consecutive elements, of which the first n exist; rows of odd lengths start off 16 bytes, which wide accesses may
@@ -322,6 +334,8 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
   constexpr bool kAOut = MODE == kDx || MODE == kDw;  // K is the outer axis of the row operand
   constexpr bool kBOut = MODE == kDw;
   constexpr int TM = kGated ? BM / 2 : BM;            // output columns per tile
+  constexpr bool kScaled = std::is_same<T, _Float16>::value && MODE != kFwd;
+  constexpr bool kFactors = kScaled && MODE == kDw;
   using TileA = Tile<T, kAOut, true, BM, NW>;
   using TileB = Tile<T, kBOut, false, BN, NW>;
   using Frag = typename Mma<T>::Frag;
@@ -330,6 +344,9 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
   __shared__ __attribute__((aligned(1024))) char b0[TileB::kBytes];
   __shared__ __attribute__((aligned(1024))) char a1[TileA::kBytes];
   __shared__ __attribute__((aligned(1024))) char b1[TileB::kBytes];
+  // kFactors: a K step's 64 factors (128 bytes; a copy by a wave writes 256)
+  __shared__ __attribute__((aligned(1024))) char fac0[kFactors ? 256 : 16];
+  __shared__ __attribute__((aligned(1024))) char fac1[kFactors ? 256 : 16];
 
   // XCD-aware order: blockIdx.x % 8 is the XCD; each gets a contiguous range of the whole tiles, then of the tail's
   // splits
@@ -369,7 +386,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
 
   const int steps_all = (p.K + BK - 1) / BK;
   const int s0 = split * p.steps, s1 = whole ? steps_all : min(steps_all, s0 + p.steps);
-  auto load = [&](int s, char* la, char* lb) {
+  auto load = [&](int s, char* la, char* lb, char* lf) {
     const int k0 = s * BK;
     const int left = p.K - k0;
     const char* xa;
@@ -385,10 +402,20 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
     const char* xb = kBOut ? pb + int64_t(k0) * p.ldb : pb + int64_t(k0) * int(sizeof(T));
     ta.load(xa, left_a, la, wave);
     tb.load(xb, left, lb, wave);
+    if (kFactors && wave == 0)
+      lds_copy4(lds_copy_source(p.factors + k0), lane < 32 ? lane * 4u : kLdsCopyOutside, lf);
   };
 
-  if (s0 < s1) load(s0, a0, b0);
-  if (s0 + 1 < s1) load(s0 + 1, a1, b1);
+  if constexpr (kScaled && MODE == kBwd) {
+    static_assert(BN <= 64 * NW, "a thread per column");
+    if (m0 == 0) {
+      const int n = n0 + int(threadIdx.x);
+      if (n < min(n0 + BN, (p.N + 63) / 64 * 64))
+        p.factors[n] = _Float16(n < p.N ? ldexpf(1.0f, *p.lowest - p.exps[n]) : 0.0f);
+    }
+  }
+  if (s0 < s1) load(s0, a0, b0, fac0);
+  if (s0 + 1 < s1) load(s0 + 1, a1, b1, fac1);
 
   // lane (g, r16) holds, for column n0 + .. + 16 i + r16 of the tile, group rows 16 g .. 16 g + 15; the bias is the
   // sums' start
@@ -417,8 +444,10 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
   // is free for the copy of the tile after next and the next tile has had a whole step to land.
   struct Frags {
     Frag a[2][4], b[NT];
+    Frag factor;  // kFactors: of the piece's eight K rows
   };
-  auto read = [&](Frags& f, const char* la, const char* lb, int kk) {
+  auto read = [&](Frags& f, const char* la, const char* lb, const char* lf, int kk) {
+    if constexpr (kFactors) f.factor = *reinterpret_cast<const Frag*>(lf + kk * 64 + g * 16);
 #pragma unroll
     for (int i = 0; i < NT; ++i) f.b[i] = read_frag<T, kBOut, false, BN>(lb, wn * NT * 16, i, kk, lane);
 #pragma unroll
@@ -429,6 +458,12 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
     }
   };
   auto multiply = [&](const Frags& f) {
+    Frag b[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      if constexpr (kFactors) b[i] = f.b[i] * f.factor;
+      else b[i] = f.b[i];
+    }
     // fp32: one of the four K entries at a time, so that no product waits for the one before it
 #pragma unroll
     for (int e = 0; e < Mma<T>::kParts; ++e)
@@ -437,11 +472,12 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int i = 0; i < NT; ++i) Mma<T>::run(f.a[q][j], f.b[i], acc[q][j][i], e);
+          for (int i = 0; i < NT; ++i) Mma<T>::run(f.a[q][j], b[i], acc[q][j][i], e);
   };
   // the order of the instructions of half a step: reads spread over the products
   auto interleave = [] {
-    constexpr int kReads = (kAOut ? (sizeof(T) == 2 ? 16 : 32) : 8) + (kBOut ? (sizeof(T) == 2 ? 2 : 4) * NT : NT);
+    constexpr int kReads = (kAOut ? (sizeof(T) == 2 ? 16 : 32) : 8) + (kBOut ? (sizeof(T) == 2 ? 2 : 4) * NT : NT) +
+                           (kFactors ? 1 : 0);
     constexpr int kMul = 8 * NT * (sizeof(T) == 2 ? 1 : 4);
     constexpr int kEach = kMul / kReads > 0 ? kMul / kReads : 1;
 #pragma unroll
@@ -450,15 +486,15 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
       __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);  // products
     }
   };
-  auto half = [&](Frags& f0, Frags& f1, const char* ca, const char* cb, int s, char* fa, char* fb, const char* na,
-                  const char* nb) {
-    read(f1, ca, cb, 1);
+  auto half = [&](Frags& f0, Frags& f1, char* ca, char* cb, char* cf, int s, const char* na, const char* nb,
+                  const char* nf) {
+    read(f1, ca, cb, cf, 1);
     multiply(f0);
     interleave();
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) and lgkmcnt(0): the next tile has landed, this one is read
     __syncthreads();
-    if (s + 2 < s1) load(s + 2, fa, fb);
-    read(f0, na, nb, 0);  // after the last step: stale, not used
+    if (s + 2 < s1) load(s + 2, ca, cb, cf);
+    read(f0, na, nb, nf, 0);  // after the last step: stale, not used
     multiply(f1);
     interleave();
   };
@@ -466,10 +502,10 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
     Frags f0, f1;
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
     __syncthreads();
-    read(f0, a0, b0, 0);
+    read(f0, a0, b0, fac0, 0);
     for (int s = s0; s < s1; s += 2) {
-      half(f0, f1, a0, b0, s, a0, b0, a1, b1);
-      if (s + 1 < s1) half(f0, f1, a1, b1, s + 1, a1, b1, a0, b0);
+      half(f0, f1, a0, b0, fac0, s, a1, b1, fac1);
+      if (s + 1 < s1) half(f0, f1, a1, b1, fac1, s + 1, a0, b0, fac0);
     }
   }
 
@@ -497,15 +533,17 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
           const int n = n0 + (wn * NT + i) * 16 + r16;
           float go[16], da[16], db[16];
           if (n < p.N) load16(static_cast<const T*>(p.go) + int64_t(n) * p.F + f0, go, left);
+          const int kept = kScaled && n < p.N ? p.exps[n] : 0;
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float y, dy;
             act_both<decltype(act)::value, kFast>(acc[0][e >> 2][i][e & 3], y, dy);
+            if constexpr (kScaled) go[e] = ldexpf(go[e], kept);
             const bool in = n < p.N && e < left;  // columns past F are zero, whatever x holds
             da[e] = in ? go[e] * acc[1][e >> 2][i][e & 3] * dy : 0.0f;
             db[e] = in ? go[e] * y : 0.0f;
-            acc[0][e >> 2][i][e & 3] = da[e];
-            acc[1][e >> 2][i][e & 3] = db[e];
+            acc[0][e >> 2][i][e & 3] = kScaled ? ldexpf(da[e], -kept) : da[e];
+            acc[1][e >> 2][i][e & 3] = kScaled ? ldexpf(db[e], -kept) : db[e];
           }
           if (n < p.N && f0 < p.Fp) {
             T* o = static_cast<T*>(p.out) + int64_t(n) * p.ldo + f0;
@@ -542,6 +580,11 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) gemm_kernel(Params p) {
         float v[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = acc[q][e >> 2][i][e & 3];
+        if constexpr (kScaled) {
+          const int e_n = MODE == kDw ? *p.lowest : n < p.N ? p.exps[n] : 0;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] = ldexpf(v[e], -e_n);
+        }
         if (!whole) {
           store16(p.part + ((int64_t(t - p.full) * p.splits + split) * BN + nl) * BM + ml, v, 16);
         } else if (out_row<MODE>(p, n) && m < p.ldo) {
@@ -659,6 +702,96 @@ __global__ void __launch_bounds__(256) tail_kernel(Params p, int bm, int bn) {
   }
 }
 
+// fp16's [dA dB]: how large it can get (see the top).  Two launches: of every workgroup's rows of W the largest norms and
+// biases, (gate, up) each; then of every token its exponent, and the smallest of all, a minimum of integers (its order does
+// not matter).  What is not finite decides nothing: a row of x or W with such an entry has no finite value in [dA dB]'s
+// row or column anyway.
+constexpr int kTopExp = 40;       // of a token without a gradient: 2^-24 <= B_n, so that e_n <= 37 elsewhere
+constexpr int kNormBlocks = 256;  // workgroups of the first launch at most
+
+__device__ __forceinline__ float finite_or_zero(float v) { return fabsf(v) <= 3.0e38f ? fabsf(v) : 0.0f; }
+
+__global__ void __launch_bounds__(256) weight_reach_kernel(const char* w, int64_t ldw, const _Float16* bias, int F, int K,
+                                                           float4* reach, int* lowest) {
+  __shared__ float4 waves[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float4 top = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int f = blockIdx.x * 4 + wave; f < 2 * F; f += gridDim.x * 4) {
+    const _Float16* row = reinterpret_cast<const _Float16*>(w + int64_t(f) * ldw);
+    float sum = 0.0f;
+    for (int c = lane * 8; c < K; c += 512) {  // K is a multiple of 8, the rows are aligned
+      const mf_f16x8 v = *reinterpret_cast<const mf_f16x8*>(row + c);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += float(v[e]) * float(v[e]);
+    }
+    const float norm = sqrtf(finite_or_zero(wave_sum(sum)));
+    const float b = bias ? finite_or_zero(float(bias[f])) : 0.0f;
+    if (f < F) {
+      top.x = fmaxf(top.x, norm);
+      top.z = fmaxf(top.z, b);
+    } else {
+      top.y = fmaxf(top.y, norm);
+      top.w = fmaxf(top.w, b);
+    }
+  }
+  if (lane == 0) waves[wave] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 4; ++i)
+      top = make_float4(fmaxf(top.x, waves[i].x), fmaxf(top.y, waves[i].y), fmaxf(top.z, waves[i].z), fmaxf(top.w, waves[i].w));
+    reach[blockIdx.x] = top;
+    if (blockIdx.x == 0) *lowest = kTopExp;
+  }
+}
+
+// A wave per token; sixteen waves a workgroup and one workgroup a CU, because the minimum's atomics take their time (32768 x
+// 768 x 2048, 184 MB: 47 us, with 4096 workgroups of four waves 65).
+constexpr int kExpWaves = 16;
+__global__ void __launch_bounds__(64 * kExpWaves) token_exp_kernel(const char* x, int64_t ldx, const _Float16* go, int T, int F, int K,
+                                                        const float4* reach, int blocks, int* exps, int* lowest) {
+  typedef _Float16 U __attribute__((ext_vector_type(8), aligned(2)));
+  __shared__ int low[kExpWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float4 top = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = lane; i < blocks; i += 64) {
+    const float4 r = reach[i];
+    top = make_float4(fmaxf(top.x, r.x), fmaxf(top.y, r.y), fmaxf(top.z, r.z), fmaxf(top.w, r.w));
+  }
+  top = make_float4(wave_max(top.x), wave_max(top.y), wave_max(top.z), wave_max(top.w));
+  int least = kTopExp;
+  for (int64_t n = int64_t(blockIdx.x) * kExpWaves + wave; n < T; n += int64_t(gridDim.x) * kExpWaves) {
+    const _Float16* row = reinterpret_cast<const _Float16*>(x + n * ldx);
+    float sum = 0.0f, peak = 0.0f;
+    for (int c = lane * 8; c < K; c += 512) {
+      const mf_f16x8 v = *reinterpret_cast<const mf_f16x8*>(row + c);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += float(v[e]) * float(v[e]);
+    }
+    const _Float16* grad = go + n * F;
+    for (int f = lane * 8; f < F; f += 512) {
+      if (f + 8 <= F) {
+        const U v = *reinterpret_cast<const U*>(grad + f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) peak = fmaxf(peak, finite_or_zero(float(v[e])));
+      } else {
+        for (int e = f; e < F; ++e) peak = fmaxf(peak, finite_or_zero(float(grad[e])));
+      }
+    }
+    const float norm = sqrtf(finite_or_zero(wave_sum(sum)));
+    peak = wave_max(peak);
+    const float bound = 1.25f * peak * fmaxf(fmaxf(norm * top.x + top.z, norm * top.y + top.w), 1.0f);
+    const int e = peak > 0.0f ? 13 - ilogbf(bound) : kTopExp;
+    least = min(least, e);
+    if (lane == 0) exps[n] = e;
+  }
+  if (lane == 0) low[wave] = least;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < kExpWaves; ++i) least = min(least, low[i]);
+    atomicMin(lowest, least);
+  }
+}
+
 // dbias: column sums of `rows` partial rows of [2 Fp], 16 columns a workgroup, 16 strands of rows each.
 template <typename T>
 __global__ void __launch_bounds__(256) bias_kernel(const float* part, T* out, int rows, int F, int Fp) {
@@ -772,7 +905,11 @@ struct Plan {
   int esize;
   bool pad_x, pad_w;
   size_t x_bytes, w_bytes, dab_bytes, bias_bytes;
+  size_t reach_bytes, exps_bytes, factors_bytes;  // fp16's backward
   Cut gated, dx, dw;
+  size_t bwd_bytes() const {
+    return x_bytes + w_bytes + dab_bytes + bias_bytes + reach_bytes + exps_bytes + factors_bytes + dx.bytes + dw.bytes;
+  }
 };
 
 void make_plan(Plan* q, int64_t T, int64_t C, int64_t F, int64_t x_stride, const void* x, const void* w, int dtype,
@@ -789,6 +926,10 @@ void make_plan(Plan* q, int64_t T, int64_t C, int64_t F, int64_t x_stride, const
   q->x_bytes = q->pad_x ? round256(size_t(T) * q->Cp * q->esize) : 0;
   q->w_bytes = q->pad_w ? round256(size_t(2) * F * q->Cp * q->esize) : 0;
   q->dab_bytes = need_dx || need_dw ? round256(size_t(T) * 2 * q->Fp * q->esize) : 0;
+  const bool scaled = dtype == MF_DTYPE_F16 && (need_dx || need_dw || need_db);
+  q->reach_bytes = scaled ? 256 + kNormBlocks * sizeof(float4) : 0;  // the smallest exponent, the weights' reach
+  q->exps_bytes = scaled ? round256(size_t(T) * 4) : 0;
+  q->factors_bytes = scaled ? round256(size_t((T + 63) / 64 * 64) * 2) : 0;
   q->gated = cut_gated(F, T, q->Cp, q->esize, num_cus);
   // bias sums of every column wave, four a tile
   q->bias_bytes = need_db ? round256(size_t((T + q->gated.bn - 1) / q->gated.bn) * 4 * 2 * q->Fp * 4) : 0;
@@ -866,7 +1007,7 @@ int forward(const mf_gated_linear_args* a, const Plan& q, hipStream_t s) {
 }
 
 template <typename T>
-int backward(const mf_gated_linear_bwd_args* a, const Plan& q, hipStream_t s) {
+int backward(const mf_gated_linear_bwd_args* a, const Plan& q, int num_cus, hipStream_t s) {
   const mf_gated_linear_args& f = a->fwd;
   Params p = {};
   char* ws = operands<T>(q, f.x, f.x_stride, f.weight, static_cast<char*>(a->workspace), &p, s);
@@ -885,6 +1026,23 @@ int backward(const mf_gated_linear_bwd_args* a, const Plan& q, hipStream_t s) {
   p.bias = f.bias;
   p.go = a->grad_out;
   p.part = sums;
+  if constexpr (std::is_same<T, _Float16>::value) {
+    p.lowest = reinterpret_cast<int*>(ws);
+    float4* reach = reinterpret_cast<float4*>(ws + 256);
+    ws += q.reach_bytes;
+    p.exps = reinterpret_cast<int*>(ws);
+    ws += q.exps_bytes;
+    p.factors = reinterpret_cast<_Float16*>(ws);
+    ws += q.factors_bytes;
+    const int blocks = int(std::min<int64_t>((2 * q.F + 3) / 4, kNormBlocks));
+    hipLaunchKernelGGL(weight_reach_kernel, dim3(unsigned(blocks)), dim3(256), 0, s, w, ldw,
+                       static_cast<const _Float16*>(f.bias), p.F, p.K, reach, p.lowest);
+    if (q.T > 0) {
+      const int64_t groups = std::min<int64_t>((q.T + kExpWaves - 1) / kExpWaves, num_cus);
+      hipLaunchKernelGGL(token_exp_kernel, dim3(unsigned(groups)), dim3(64 * kExpWaves), 0, s, x, ldx,
+                         static_cast<const _Float16*>(a->grad_out), p.N, p.F, p.K, reach, blocks, p.exps, p.lowest);
+    }
+  }
   if (q.T > 0) launch_gemm<T, kBwd>(p, q.gated, s);
   MF_HIP_CHECK(hipGetLastError());
   if (a->dbias) {
@@ -1002,7 +1160,7 @@ extern "C" uint64_t mf_gated_linear_bwd_workspace_size(const mf_gated_linear_bwd
   Plan q;
   if (a == nullptr || check("mf_gated_linear_bwd_workspace_size", &a->fwd) != MF_OK) return 0;
   if (device_info(&info) != MF_OK || bwd_plan(a, &q, info.num_cus) != MF_OK) return 0;
-  return q.x_bytes + q.w_bytes + q.dab_bytes + q.bias_bytes + q.dx.bytes + q.dw.bytes;
+  return q.bwd_bytes();
 }
 
 extern "C" int mf_gated_linear_bwd(const mf_gated_linear_bwd_args* a, void* stream) {
@@ -1020,14 +1178,14 @@ extern "C" int mf_gated_linear_bwd(const mf_gated_linear_bwd_args* a, void* stre
   Plan q;
   st = bwd_plan(a, &q, info.num_cus);
   if (st != MF_OK) return st;
-  const size_t need = q.x_bytes + q.w_bytes + q.dab_bytes + q.bias_bytes + q.dx.bytes + q.dw.bytes;
+  const size_t need = q.bwd_bytes();
   if (need > 0 && (!a->workspace || !aligned16(a->workspace) || a->workspace_bytes < need))
     return fail(MF_ERR_INVALID_ARGUMENT, "mf_gated_linear_bwd: the workspace must be 16-byte aligned and hold "
                                          "mf_gated_linear_bwd_workspace_size bytes");
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (a->fwd.dtype) {
-    case MF_DTYPE_BF16: return backward<__bf16>(a, q, s);
-    case MF_DTYPE_F16: return backward<_Float16>(a, q, s);
-    default: return backward<float>(a, q, s);
+    case MF_DTYPE_BF16: return backward<__bf16>(a, q, info.num_cus, s);
+    case MF_DTYPE_F16: return backward<_Float16>(a, q, info.num_cus, s);
+    default: return backward<float>(a, q, info.num_cus, s);
   }
 }

@@ -295,3 +295,83 @@ def test_c_entries_refuse_a_workspace_off_16_bytes(cuda):
         assert getattr(_native.lib(), name)(args, None) == _native.MF_ERR_INVALID_ARGUMENT
         assert "16-byte aligned" in _native.last_error()
     assert not out.any() and not work.any()
+
+
+# float16's [dA dB] is kept times a power of two per token, chosen from the bound
+#   B_n = 1.25 max|go_n| max(|x_n| max|Wu| + max|bu|, |x_n| max|Wg| + max|bg|, 1)     (Euclidean norms of rows)
+# so that B_n 2^e_n lies in [2^13, 2^14): no value overflows, and what rounding leaves below the normal numbers, 2^-25
+# 2^-e_n, is at most 2^-38 B_n.  For dW the rows come to the smallest e of all: the same with max B, once more rounded.
+def _half_check(x, w, b, go, name, grads):
+    X, W, GO, a, up, ea, eb, y, dy, C, F, T = _reference(x, w, b, go, name)
+    t = 2.0 ** -11
+    da, db = GO * up * dy, GO * y
+    fa = GO.abs() * (1.13 * eb + 0.8 * ea * up.abs() + 64 * U * (up * dy).abs() + 64 * U * up.abs())
+    fb = GO.abs() * (1.13 * ea + 64 * U * y.abs() + 64 * U)
+    dab, fab = torch.cat([da, db], -1), torch.cat([fa, fb], -1)
+    norm, size = X.norm(dim=1, keepdim=True), W.norm(dim=1)
+    bias = torch.zeros(2 * F, dtype=torch.float64, device=x.device) if b is None else b.double().abs()
+    reach = [norm * size[h].max() + bias[h].max() for h in (slice(0, F), slice(F, None))]
+    bound = 1.25 * GO.abs().amax(1, keepdim=True) * torch.maximum(*reach).clamp_min(1.0)
+    rounded = fab + (dab.abs() + fab) * t
+    by_row = rounded + 2.0 ** -38 * bound
+    by_all = rounded + 2.0 ** -37 * bound.max()
+    for got, want, slack, what in (
+            (grads[0], dab @ W, by_row @ W.abs() + (2 * F + 1) * U * ((dab.abs() + by_row) @ W.abs()), "dx"),
+            (grads[1], dab.T @ X, by_all.T @ X.abs() + (T + 1) * U * ((dab.abs() + by_all).T @ X.abs()), "dW")):
+        # a value past float16's range rounds to infinity (65520 and more), one within its bound of that may
+        over, near = want.abs() - slack * (1 + t) >= 65520, want.abs() + slack * (1 + t) >= 65504
+        assert torch.equal(got[over].double(), torch.sign(want[over]) * math.inf), what
+        _close(torch.where(near, 0, got), torch.where(near, 0.0, want), torch.where(near, 0.0, slack), what)
+
+
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+@pytest.mark.parametrize("T,C,F", [(40, 64, 48), (150, 80, 70)])
+@pytest.mark.parametrize("sizes", [(30.0, 0.02, 3e4), (0.02, 30.0, 3e4), (0.02, 30.0, 1e-6), (1.0, 1.0, 1e-6)])
+def test_half_gradients_near_the_ends_of_the_type(cuda, activation, T, C, F, sizes):
+    """Intermediate gradients of 1e5 (past float16's largest number) and of 1e-6 (below its normal ones) whose dx or dW
+    is within it."""
+    gen = torch.Generator().manual_seed(T)
+    x, w, go = (((torch.rand(*s, generator=gen) * 2 - 1) * m).half().to(cuda)
+                for s, m in zip(((T, C), (2 * F, C), (T, F)), sizes))
+    out, grads = _run(x, w, None, go, activation)
+    assert torch.isfinite(out).all()
+    X, W, GO, a, up, _, _, y, dy, *_ = _reference(x, w, None, go, activation)
+    if sizes[2] > 1:
+        assert float(torch.maximum((GO * up * dy).abs().max(), (GO * y).abs().max())) > 65504 or activation == "sigmoid"
+    _half_check(x, w, None, go, activation, grads)
+
+
+@pytest.mark.parametrize("T", [40, 300, 2500])
+def test_half_gradients_of_other_tokens_stay_apart(cuda, T):
+    """One token of 6e4 (its gradients overflow) changes no other token's dx; dW follows its formula with a token of 1e3."""
+    x, w, b, go = _inputs(T, 64, 520, torch.float16, True, 25, cuda)
+    big_x, big_go = x.clone(), go.clone()
+    big_x[7], big_go[7] = 6e4, 6e4
+    ref, got = _run(x, w, b, go, "silu")[1], _run(big_x, w, b, big_go, "silu")[1]
+    keep = torch.arange(T, device=cuda) != 7
+    assert torch.equal(got[0][keep], ref[0][keep])
+    x[7] *= 8
+    go[7] *= 1e3
+    _half_check(x, w, b, go, "silu", _run(x, w, b, go, "silu")[1])
+    want = _run(x, w, b, go, "silu")[1][0]
+    go[T - 1] = float("inf")  # nor does a token that is not finite
+    assert torch.equal(_run(x, w, b, go, "silu")[1][0][:T - 1], want[:T - 1])
+
+
+@pytest.mark.parametrize("C", [128, 77])
+def test_half_gradients_in_a_graph(cuda, C):
+    """The scales are found anew at every replay: inputs of other magnitudes, checked against eager calls."""
+    x, w, b, go = _inputs(300, C, 96, torch.float16, True, 26, cuda)
+    _run(x, w, b, go, "silu")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = _run(x, w, b, go, "silu")
+    gen = torch.Generator().manual_seed(27)
+    for size in (1e-4, 1e3, 1.0, 1e-6):
+        go.copy_((torch.randn(300, 96, generator=gen) * size).half())
+        x.copy_(torch.randn(300, C, generator=gen).half())
+        graph.replay()
+        torch.cuda.synchronize()
+        now = _run(x, w, b, go, "silu")
+        assert torch.equal(held[0], now[0]) and all(torch.equal(p, q) for p, q in zip(held[1], now[1])), size
+        _half_check(x, w, b, go, "silu", now[1])
