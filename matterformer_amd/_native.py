@@ -16,6 +16,7 @@ import os
 from pathlib import Path
 
 import torch  # noqa: F401  (loads the HIP runtime the library must share)
+from torch.autograd import forward_ad
 
 from matterformer_amd.build import LIB_PATH
 
@@ -420,9 +421,21 @@ def launch(name: str, args: ctypes.Structure, device: torch.device) -> None:
         check(status, name)
 
 
+def in_forward_mode() -> bool:
+    """Some tensor may carry a forward-mode tangent."""
+    return forward_ad._current_level >= 0
+
+
+def has_tangent(*tensors: torch.Tensor | None) -> bool:
+    """One of these tensors carries a forward-mode tangent."""
+    return in_forward_mode() and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def takes_gradient(*tensors: torch.Tensor | None) -> bool:
-    """Autograd follows a call on these tensors."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Autograd follows a call on these tensors: backward, or by tangents, for which the autograd functions have no rule
+    and raise NotImplementedError (also where gradients are off)."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or has_tangent(*tensors)
 
 
 _WORKSPACES: dict = {}

@@ -108,6 +108,8 @@ def _check_positions(positions: torch.Tensor, batch: int, tokens: int, frequenci
                      device: torch.device) -> torch.Tensor:
     """The positions as (B or 1, N, axes)."""
     axes = frequencies.axes
+    if _native.has_tangent(positions, frequencies.table):
+        raise RuntimeError("rotary positions and frequencies take no derivative: detach them")
     if positions.requires_grad:
         if torch.is_grad_enabled():
             raise RuntimeError("rotary positions take no gradient: detach them")

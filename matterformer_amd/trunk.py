@@ -32,6 +32,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from matterformer_amd import _native
 from matterformer_amd.gated_mlp import ACTIVATIONS, gated_linear
 from matterformer_amd.rotary import RotaryFrequencies, check_layout, rotary_heads, rotary_heads_torch
 from matterformer_amd.simplicial_attention import SimplicialAttention
@@ -182,6 +183,8 @@ class KnnLocalAttention(nn.Module):
             return "the HIP local attention requires GPU tensors"
         if self.training and self.attn.dropout > 0.0:
             return "the HIP local attention does not support attention dropout in training mode"
+        if _native.in_forward_mode() and _native.has_tangent(h, *self.attn.parameters()):
+            return "the HIP local attention has no forward-mode derivative"
         if torch.is_grad_enabled() and (h.requires_grad or any(p.requires_grad for p in self.attn.parameters())):
             if not self.hip_backward:
                 return "the HIP local attention has no backward; autograd takes the torch path"
