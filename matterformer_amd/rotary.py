@@ -110,6 +110,8 @@ def _check_positions(positions: torch.Tensor, batch: int, tokens: int, frequenci
     axes = frequencies.axes
     if _native.has_tangent(positions, frequencies.table):
         raise RuntimeError("rotary positions and frequencies take no derivative: detach them")
+    if frequencies.table.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("a rotary frequency table takes no gradient: detach it")
     if positions.requires_grad:
         if torch.is_grad_enabled():
             raise RuntimeError("rotary positions take no gradient: detach them")

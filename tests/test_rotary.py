@@ -121,6 +121,16 @@ def test_argument_refusals():
         rotary_heads(torch.zeros(2, 5, 48), pos, f, heads=4, kv_heads=0)
 
 
+def test_a_table_that_asks_for_a_gradient_is_refused():
+    f = RotaryFrequencies(torch.ones(4, dtype=torch.float64, requires_grad=True))
+    for call in (lambda: apply_rotary(torch.zeros(1, 1, 5, 8), None, torch.zeros(1, 5), f),
+                 lambda: rotary_heads(torch.zeros(1, 5, 24), torch.zeros(1, 5), f, heads=1)):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+        with torch.no_grad():
+            call()
+
+
 def test_c_entry_refuses_before_any_device_call():
     lib = _native.lib()
     fake = 1 << 20  # never dereferenced: every call below fails validation first
