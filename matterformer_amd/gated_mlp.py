@@ -25,6 +25,9 @@ _TORCH_ACT = {"silu": F.silu, "gelu": F.gelu, "gelu_tanh": lambda t: F.gelu(t, a
 
 def _arguments(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, activation: str,
                out: torch.Tensor | None) -> _native.MfGatedLinearArgs:
+    if x.shape[0] > 1 << 30 or weight.numel() >= 1 << 31:  # before they are cut to 32 bits
+        raise RuntimeError(f"gated_linear supports up to 2^30 tokens and weights below 2^31 bytes, got {x.shape[0]} tokens "
+                           f"and a weight of {tuple(weight.shape)}")
     return _native.MfGatedLinearArgs(
         x=x.data_ptr(), weight=weight.data_ptr(), bias=_native.ptr(bias), out=_native.ptr(out),
         x_stride=x.stride(0) if x.shape[0] > 1 else x.shape[1], tokens=x.shape[0], channels=x.shape[1],

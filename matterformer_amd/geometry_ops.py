@@ -243,6 +243,8 @@ def radius_tables(mask_bits: torch.Tensor, block_mask: torch.Tensor | None = Non
         raise ValueError(f"mask_bits must be int32 of shape (B, N, ceil(N/32)), got {mask_bits.dtype} "
                          f"{tuple(mask_bits.shape)}")
     B, N, W = mask_bits.shape
+    if B >= 1 << 31:  # before it is cut to 32 bits
+        raise RuntimeError(f"radius_tables supports batches below 2^31, got {B}")
     NB = (N + MASK_BLOCK - 1) // MASK_BLOCK
     if block_mask is not None and block_mask.shape != (B, NB, NB):
         raise ValueError(f"block_mask must have shape ({B}, {NB}, {NB}) (block {MASK_BLOCK})")
@@ -339,6 +341,8 @@ def radius_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bit
     B, H, N, D = q.shape
     if D not in (32, 64, 128):
         raise RuntimeError(f"radius_attention supports head_dim 32, 64 or 128, got {D}")
+    if B * H >= 1 << 31:  # before they are cut to 32 bits
+        raise RuntimeError(f"radius_attention supports below 2^31 cells times heads, got {B} x {H}")
     W = (N + 31) // 32
     if mask_bits.shape != (B, N, W) or mask_bits.dtype != torch.int32:
         raise ValueError(f"mask_bits must be int32 of shape ({B}, {N}, {W})")

@@ -175,6 +175,9 @@ def _launch(plan: _Plan, src, src_strides, dst, dst_strides, heads, *, batch: in
             inverse: bool, slot_side: int, src_dtype: torch.dtype, dst_dtype: torch.dtype,
             device: torch.device) -> None:
     """src, dst: three addresses (None past the last part); strides: nine, {batch, head, token} of each part."""
+    if batch * tokens >= 1 << 31 or sum(heads) * head_dim >= 1 << 24:  # before they are cut to 32 bits
+        raise RuntimeError(f"rotary positions support up to 2^31 tokens of 2^24 elements, got {batch} x {tokens} of "
+                           f"{sum(heads)} x {head_dim}")
     pos = plan.positions
     axes, gain, interleaved = plan.settings
     sb, sn, sa = pos.stride()
