@@ -168,7 +168,7 @@ class KnnLocalAttention(nn.Module):
         self.rotary = rotary
         self.rotary_layout = rotary_layout
         self.hip_backward = bool(hip_backward)
-        self._rotary_on: dict = {}  # device -> rotary there
+        self._rotary_on: dict = {}  # device -> [(rotary, its table's version, rotary there)], the last one in use
         impl = impl.lower()
         if impl == "hip":
             impl = "triton"
@@ -211,9 +211,19 @@ class KnnLocalAttention(nn.Module):
         return dtype if dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
 
     def _rotary(self, device: torch.device) -> RotaryFrequencies:
-        if device not in self._rotary_on:
-            self._rotary_on[device] = self.rotary.to(device)
-        return self._rotary_on[device]
+        """``rotary`` on the device: copied once, into the same copy when its table changed in place, into another when
+        it is another object (the copies before it stay: a captured graph may read them)."""
+        table = self.rotary.table
+        if table.device == device:
+            return self.rotary
+        version = 0 if table.is_inference() else table._version
+        held = self._rotary_on.setdefault(device, [])
+        if not held or held[-1][0] is not self.rotary:
+            held.append((self.rotary, version, self.rotary.to(device)))
+        elif held[-1][1] != version:
+            held[-1][2].table.copy_(table)
+            held[-1] = (self.rotary, version, held[-1][2])
+        return held[-1][2]
 
     def _positions(self, mask: KnnLocalMask) -> torch.Tensor:
         if mask.positions is None:

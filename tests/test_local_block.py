@@ -80,3 +80,62 @@ def test_trunk_with_every_option_trains_on_the_cpu():
     assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in trunk.parameters())
     assert trunk.blocks[1].attn._last_impl_used == "torch"
     assert isinstance(trunk.blocks[0], AdaLNBlock) and trunk.blocks[0].mlp.gate == "silu"
+
+
+def test_another_table_of_frequencies_takes_effect():
+    """Assigned, or changed in place, after a forward: the next one turns by it (its copy on the device too)."""
+    torch.manual_seed(4)
+    attn = KnnLocalAttention(64, 2, rotary=rotary_frequencies(24, axes=3, base=20.0)).double()
+    h, coords = torch.randn(1, 9, 64, dtype=torch.float64), torch.randn(1, 9, 3) * 3
+    mask = build_knn_mask(coords, 4, None, use_hip=False)
+    meta = torch.device("meta")  # another device than the table's
+
+    def fresh():
+        other = KnnLocalAttention(64, 2, rotary=rotary_frequencies(24, axes=3, base=20.0)).double()
+        other.load_state_dict(attn.state_dict())
+        other.rotary = attn.rotary
+        return other(h, mask)
+
+    first, held = attn(h, mask), attn._rotary(meta)
+    assert attn._rotary(meta) is held  # one copy a device, while the table stays
+    attn.rotary = rotary_frequencies(24, axes=3, base=500.0)
+    second = attn(h, mask)
+    assert not torch.allclose(first, second) and torch.equal(second, fresh())
+    assert attn._rotary(meta) is not held
+    held = attn._rotary(meta)
+    attn.rotary.table.mul_(0.5)
+    third = attn(h, mask)
+    assert not torch.allclose(second, third) and torch.equal(third, fresh())
+    assert attn._rotary(meta) is held  # the same copy, changed with it (a captured graph reads it)
+
+
+@pytest.mark.gpu
+def test_another_table_of_frequencies_takes_effect_on_the_gpu(cuda):
+    """The module's copy there follows an assignment and a change in place, also one behind a captured graph."""
+    torch.manual_seed(5)
+    attn = KnnLocalAttention(64, 2, rotary=rotary_frequencies(24, axes=3, base=20.0)).to(cuda, torch.bfloat16)
+    h, coords = torch.randn(1, 9, 64).to(cuda, torch.bfloat16), torch.randn(1, 9, 3, device=cuda) * 3
+    mask = build_knn_mask(coords, 4, None, use_hip=True)
+
+    def fresh():
+        other = KnnLocalAttention(64, 2, rotary=attn.rotary).to(cuda, torch.bfloat16)
+        other.load_state_dict(attn.state_dict())
+        return other(h, mask)
+
+    with torch.no_grad():
+        first = attn(h, mask)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = attn(h, mask)
+        attn.rotary.table.mul_(2.0)
+        second = attn(h, mask)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert not torch.equal(first, second) and torch.equal(second, fresh()) and torch.equal(out, second)
+        attn.rotary = rotary_frequencies(24, axes=3, base=500.0)
+        third = attn(h, mask)
+        assert not torch.equal(second, third) and torch.equal(third, fresh())
+        filler = [torch.full((12,), 7.0, dtype=torch.float64, device=cuda) for _ in range(64)]
+        graph.replay()  # as it was captured
+        torch.cuda.synchronize()
+        assert torch.equal(out, second) and len(filler) == 64
