@@ -116,32 +116,42 @@ def knn_allowed_torch(idx: torch.Tensor, pad_mask: torch.Tensor | None) -> torch
 
 class KnnLocalMask:
     """The local blocks' mask, built once per forward: kNN lists plus bit / block masks (GPU) or the
-    boolean matrix (CPU); the coordinates they were built from, which rotary blocks turn by."""
+    boolean matrix (CPU); the coordinates they were built from, which rotary blocks turn by.  ``with_tables``: the
+    radius_tables of the bits with them, for blocks that take gradients."""
 
-    def __init__(self, idx: torch.Tensor, bits=None, blocks=None, allowed=None, positions=None):
+    def __init__(self, idx: torch.Tensor, bits=None, blocks=None, allowed=None, positions=None, with_tables: bool = False):
         self.idx = idx
         self.bits = bits
         self.blocks = blocks
         self.allowed = allowed
         self.positions = positions
-        self._tables = None
+        self._tables = self._tables_of = None
+        if with_tables:
+            of = self._source()
+            self._tables, self._tables_of = self.tables(), of
+
+    def _source(self) -> tuple:
+        return tuple((t, None if t is None or t.is_inference() else t._version) for t in (self.bits, self.blocks))
 
     def tables(self):
-        """radius_tables of the mask, made by the first block that takes gradients and shared by the others."""
-        if self._tables is None:
-            from matterformer_amd.geometry_ops import radius_tables
+        """radius_tables of the mask: those it was built with, shared by its blocks, while its bits are as they were;
+        else of a call's own, and not kept (that call may be captured into a graph or run on another stream)."""
+        if self._tables is not None and all(
+                a is b and va == vb for (a, va), (b, vb) in zip(self._source(), self._tables_of)):
+            return self._tables
+        from matterformer_amd.geometry_ops import radius_tables
 
-            self._tables = radius_tables(self.bits, self.blocks)
-        return self._tables
+        return radius_tables(self.bits, self.blocks)
 
 
-def build_knn_mask(coords: torch.Tensor, k: int, pad_mask: torch.Tensor | None, *, use_hip: bool) -> KnnLocalMask:
+def build_knn_mask(coords: torch.Tensor, k: int, pad_mask: torch.Tensor | None, *, use_hip: bool,
+                   with_tables: bool = False) -> KnnLocalMask:
     if use_hip:
         from matterformer_amd.geometry_ops import knn_graph, knn_mask
 
         idx = knn_graph(coords, k, pad_mask, exclude_self=True, return_dist=False)
         bits, blocks = knn_mask(idx, pad_mask, include_self=True)
-        return KnnLocalMask(idx, bits=bits, blocks=blocks, positions=coords.float())
+        return KnnLocalMask(idx, bits=bits, blocks=blocks, positions=coords.float(), with_tables=with_tables)
     idx = knn_lists_torch(coords, k, pad_mask)
     return KnnLocalMask(idx, allowed=knn_allowed_torch(idx, pad_mask), positions=coords.float())
 
@@ -519,6 +529,11 @@ class AlternatingTrunk(nn.Module):
         return x.device.type == "cuda" and any(a.impl != "torch" and a._hip_unavailable_reason(x) is None
                                                for a in local)
 
+    def _trains_local(self, x: torch.Tensor) -> bool:
+        """Some local block takes gradients on the HIP kernels."""
+        return (torch.is_grad_enabled() and any(b.attn_type == "knn_local" and b.attn.hip_backward for b in self.blocks)
+                and (x.requires_grad or any(p.requires_grad for p in self.parameters())))
+
     def packable(self, x: torch.Tensor, terms: SimplicialTerms | None = None) -> bool:
         """True when every block would run its HIP kernels on x (with the simplicial terms of this call), which
         the packed forward requires."""
@@ -583,7 +598,8 @@ class AlternatingTrunk(nn.Module):
         terms = self.simplicial_terms(coords, pad_mask, lattice, sigma)
         mask = None
         if "knn_local" in self.schedule:
-            mask = build_knn_mask(coords, self.knn_k, pad_mask, use_hip=self._use_hip(x))
+            mask = build_knn_mask(coords, self.knn_k, pad_mask, use_hip=self._use_hip(x),
+                                  with_tables=self._trains_local(x))
         kwargs = terms.block_kwargs() if terms is not None else {}
         # transformer.py:1298-1316: padded atoms are zeroed before every block and in the output
         for block in self.blocks:
@@ -618,7 +634,8 @@ class AlternatingTrunk(nn.Module):
         cpad = packing.compact_pad_mask
         mask = None
         if "knn_local" in self.schedule:
-            mask = build_knn_mask(packing.compact(coords.float()), self.knn_k, cpad, use_hip=True)
+            mask = build_knn_mask(packing.compact(coords.float()), self.knn_k, cpad, use_hip=True,
+                                  with_tables=self._trains_local(x))
         if terms is None:
             terms = SimplicialTerms(coerce_attention_mask(None, key_padding_mask=cpad, batch_size=B, num_tokens=W,
                                                           device=x.device))

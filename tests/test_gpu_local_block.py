@@ -154,3 +154,50 @@ def test_captured_inference(cuda):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(held, trunk(x, cond, coords, pad, packing=packing)), f"replay {turn}"
+
+
+def test_one_mask_in_a_captured_step_and_outside_it(cuda):
+    """A mask built beforehand, first used by a captured training step: an eager step on it before any replay is right,
+    and so is every replay."""
+    from matterformer_amd.trunk import KnnLocalAttention, build_knn_mask
+
+    torch.manual_seed(6)
+    attn = KnnLocalAttention(64, 2, hip_backward=True).to(cuda, torch.bfloat16)
+    gen = torch.Generator().manual_seed(7)
+    h = torch.randn(2, 70, 64, generator=gen).to(cuda, torch.bfloat16).requires_grad_(True)
+    go = torch.randn(2, 70, 64, generator=gen).to(cuda, torch.bfloat16)
+    coords = torch.randn(2, 70, 3, generator=gen).to(cuda)
+    leaves = [h, *attn.parameters()]
+
+    def step(mask):
+        return torch.autograd.grad(attn(h, mask), leaves, go)
+
+    want = step(build_knn_mask(coords, 8, None, use_hip=True))
+    for with_tables in (False, True):
+        mask = build_knn_mask(coords, 8, None, use_hip=True, with_tables=with_tables)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = step(mask)
+        assert all(torch.equal(a, b) for a, b in zip(step(mask), want))
+        for turn in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(held, want)), turn
+            assert all(torch.equal(a, b) for a, b in zip(step(mask), want)), turn
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_a_training_trunk_makes_its_tables_once(cuda, packed, monkeypatch):
+    from matterformer_amd import geometry_ops
+
+    made, real = [], geometry_ops.radius_tables
+    monkeypatch.setattr(geometry_ops, "radius_tables", lambda *a: made.append(a) or real(*a))
+    trunk = build(["knn_local", "knn_local", "knn_local"]).to(cuda)
+    trunk.pack_tokens = packed
+    x, cond, coords, pad, _ = (t.to(cuda) for t in inputs())
+    trunk(x, cond, coords, pad).float().sum().backward()
+    assert len(made) == 1
+    with torch.no_grad():
+        trunk(x, cond, coords, pad)
+    assert len(made) == 1

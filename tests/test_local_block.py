@@ -139,3 +139,27 @@ def test_another_table_of_frequencies_takes_effect_on_the_gpu(cuda):
         graph.replay()  # as it was captured
         torch.cuda.synchronize()
         assert torch.equal(out, second) and len(filler) == 64
+
+
+def test_tables_are_kept_only_by_a_mask_built_with_them(monkeypatch):
+    """A mask keeps no tables of a call on it (which may have been captured, or on another stream), and drops those it was
+    built with when its bits change."""
+    from matterformer_amd import geometry_ops
+
+    made = []
+
+    def make(bits, blocks):
+        made.append(bits)
+        return object()
+
+    monkeypatch.setattr(geometry_ops, "radius_tables", make)
+    bits = torch.ones(1, 3, 1, dtype=torch.int32)
+    mask = KnnLocalMask(torch.zeros(1, 3, 1, dtype=torch.int32), bits=bits)
+    assert mask.tables() is not mask.tables() and len(made) == 2
+    mask = KnnLocalMask(mask.idx, bits=bits, with_tables=True)
+    assert len(made) == 3 and mask.tables() is mask.tables() and len(made) == 3
+    bits.zero_()
+    assert mask.tables() is not mask.tables() and len(made) == 5
+    mask = KnnLocalMask(mask.idx, bits=bits, with_tables=True)
+    mask.bits = torch.ones(1, 3, 1, dtype=torch.int32)
+    assert mask.tables() is not mask.tables() and made[-1] is mask.bits
