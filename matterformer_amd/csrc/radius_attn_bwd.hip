@@ -298,6 +298,7 @@ __device__ __forceinline__ void bwd_unit(const Params& p, int unit, char* x0, ch
   }
 
   // tiles with an entry, in order: 64 tiles' row sets a time in the lanes
+  const uint64_t last = ~uint64_t(0) >> (p.NB * kTile - N);  // the last tile's rows
   int tbase = -64;
   uint64_t active = 0, sets = 0;
   auto next = [&](int& tile, uint64_t& set) -> bool {
@@ -306,6 +307,7 @@ __device__ __forceinline__ void bwd_unit(const Params& p, int unit, char* x0, ch
       if (tbase >= p.NB) return false;
       const int t = tbase + lane;
       sets = t < p.NB ? any[t] : 0;
+      if (t == p.NB - 1) sets &= last;  // rows past N are read by no table
       active = __ballot(sets != 0);
     }
     const int l = __builtin_ctzll(active);

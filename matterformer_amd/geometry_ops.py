@@ -261,6 +261,14 @@ def radius_tables(mask_bits: torch.Tensor, block_mask: torch.Tensor | None = Non
     return tables
 
 
+def _check_tables(tables: RadiusTables, bits: torch.Tensor, tiles: tuple) -> None:
+    """The kernels read the three by address: their shapes, types, layout and device."""
+    for t, shape, dtype in ((tables.bits_t, bits.shape, torch.int32), (tables.key_any, tiles, torch.int64),
+                            (tables.query_any, tiles, torch.int64)):
+        if t.shape != shape or t.dtype != dtype or t.device != bits.device or not t.is_contiguous():
+            raise ValueError("tables must be radius_tables of this call's masks")
+
+
 def _radius_forward(q, k, v, bits, bm, tables, scale, *, lse: bool, fp32: bool, out_lo: torch.Tensor | None = None):
     """out, lse and the fp32 output (None where not asked) of contiguous operands; out_lo takes what out's rounding
     leaves."""
@@ -357,9 +365,7 @@ def radius_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask_bit
     if not math.isfinite(s):
         raise ValueError("scale must be finite")
     if tables is not None:
-        if tables.bits_t.shape != bits.shape or tables.key_any.shape != (B, NB, NB):
-            raise ValueError("tables must be radius_tables of this call's masks")
-        _require_device(bits, tables.bits_t)
+        _check_tables(tables, bits, (B, NB, NB))
     if _native.takes_gradient(q, k, v):
         if tables is None:
             tables = radius_tables(bits, bm)

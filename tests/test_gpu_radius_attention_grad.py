@@ -365,3 +365,18 @@ def test_value_gradients_of_keys_with_little_weight(cuda):
     slack = (P * (2 * t + 2 * N * U + 2.0 ** -20) + 2.0 ** -37).mT @ go.double().abs()
     assert float(want[0, 0, 1].min()) > 5e-5
     check(got, want, slack, "dv")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N,D", [(70, 64), (30, 128), (129, 32), (128, 64)])
+def test_tables_that_name_every_row(cuda, dtype, N, D):
+    """Tables whose tiles are all marked, rows past the last atom too: the same gradients, none of those rows read."""
+    from matterformer_amd.geometry_ops import RadiusTables
+
+    q, k, v, go, gen = operands(2, 2, N, D, dtype, 16, cuda)
+    allowed = mask_of("random", 2, N, gen)
+    bits = pack(allowed).to(cuda)
+    t = radius_tables(bits)
+    every = RadiusTables(t.bits_t, torch.full_like(t.key_any, -1), torch.full_like(t.query_any, -1))
+    want, got = gradients(q, k, v, go, bits, None, tables=t), gradients(q, k, v, go, bits, None, tables=every)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

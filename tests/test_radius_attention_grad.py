@@ -1,6 +1,10 @@
 """mf_radius_attn_bwd on the CPU: the C entry's checks and its struct."""
 
+import pytest
+import torch
+
 from matterformer_amd import _native
+from matterformer_amd.geometry_ops import RadiusTables, _check_tables
 
 
 def test_c_entry_refuses_before_any_device_call():
@@ -62,3 +66,21 @@ def test_entries_refuse_more_threads_than_a_launch_has():
     t = _native.MfRadiusTablesArgs(**{n: fake for n in ("mask_bits", "mask_bits_t", "key_any", "query_any")}, batch=2 ** 26,
                                    atoms=1)
     assert lib.mf_radius_tables(t, None) == _native.MF_ERR_UNSUPPORTED and "too large" in _native.last_error()
+
+
+def test_tables_of_another_form_are_refused():
+    bits = torch.zeros(2, 70, 3, dtype=torch.int32)
+
+    def tables(**kw):
+        t = dict(bits_t=bits.clone(), key_any=torch.zeros(2, 2, 2, dtype=torch.int64),
+                 query_any=torch.zeros(2, 2, 2, dtype=torch.int64))
+        t.update(kw)
+        return RadiusTables(**t)
+
+    _check_tables(tables(), bits, (2, 2, 2))
+    for kw in (dict(bits_t=bits[:1]), dict(bits_t=bits.long()), dict(key_any=torch.zeros(2, 1, 2, dtype=torch.int64)),
+               dict(query_any=torch.zeros(2, 2, 1, dtype=torch.int64)), dict(query_any=torch.zeros(2, 2, 2)),
+               dict(query_any=torch.zeros(2, 2, 2, dtype=torch.int64, device="meta")),
+               dict(key_any=torch.zeros(2, 2, 2, dtype=torch.int64).transpose(0, 1))):
+        with pytest.raises(ValueError, match="radius_tables of this call"):
+            _check_tables(tables(**kw), bits, (2, 2, 2))
