@@ -139,8 +139,10 @@ def check_layout(layout: str, head_dim: int, frequencies: RotaryFrequencies) -> 
 
 
 def _rotate_torch(x: torch.Tensor, positions: torch.Tensor, frequencies: RotaryFrequencies,
-                  interleaved: bool) -> torch.Tensor:
-    """(B, H, N, D) heads turned by torch expressions: angles in fp64, products in fp32 (fp64 for fp64 heads)."""
+                  interleaved: bool, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """(B, H, N, D) heads turned by torch expressions, in ``dtype`` (default: x's): angles in fp64, products in fp32
+    (fp64 for fp64 heads)."""
+    dtype = x.dtype if dtype is None else dtype
     per = frequencies.table.numel() // frequencies.axes
     angle = positions.double().repeat_interleave(per, dim=-1) * frequencies.table
     wide = torch.float64 if x.dtype == torch.float64 else torch.float32
@@ -154,7 +156,7 @@ def _rotate_torch(x: torch.Tensor, positions: torch.Tensor, frequencies: RotaryF
     else:
         a, b = xr[..., :R // 2], xr[..., R // 2:]
         y = torch.cat([a * cos - b * sin, a * sin + b * cos], dim=-1)
-    return torch.cat([y.to(x.dtype), x[..., R:]], dim=-1)
+    return torch.cat([y.to(dtype), x[..., R:].to(dtype)], dim=-1)
 
 
 class _Plan:
@@ -331,29 +333,35 @@ def _check_rows(rows, positions, frequencies, heads, kv_heads, layout):
 
 
 def rotary_heads_torch(rows: torch.Tensor, positions: torch.Tensor, frequencies: RotaryFrequencies, *, heads: int,
-                       kv_heads: int | None = None, layout: str = "half"):
+                       kv_heads: int | None = None, layout: str = "half", dtype: torch.dtype | None = None):
     """rotary_heads by torch expressions, on any device."""
     counts, D, interleaved, pos = _check_rows(rows, positions, frequencies, heads, kv_heads, layout)
     B, N, _ = rows.shape
+    dtype = rows.dtype if dtype is None else dtype
+    if not dtype.is_floating_point:
+        raise RuntimeError(f"rotary positions need heads of a floating type, got {dtype}")
     outs = []
     for k, part in enumerate(rows.split([h * D for h in counts], dim=-1)):
         t = part.reshape(B, N, counts[k], D).transpose(1, 2)
-        outs.append((_rotate_torch(t, pos, frequencies, interleaved) if k < 2 else t).contiguous())
+        outs.append((_rotate_torch(t, pos, frequencies, interleaved, dtype) if k < 2 else t.to(dtype)).contiguous())
     return tuple(outs)
 
 
 def rotary_heads(rows: torch.Tensor, positions: torch.Tensor, frequencies: RotaryFrequencies, *, heads: int,
-                 kv_heads: int | None = None, layout: str = "half"):
+                 kv_heads: int | None = None, layout: str = "half", dtype: torch.dtype | None = None):
     """The heads of in_proj rows (B, N, (heads + 2 kv_heads) D), q and k turned as apply_rotary turns them: contiguous
-    q (B, heads, N, D), k and v (B, kv_heads, N, D), in one pass.  Differentiable in rows."""
+    q (B, heads, N, D), k and v (B, kv_heads, N, D) in ``dtype`` (default: rows'), in one pass, rounded once.
+    Differentiable in rows."""
     if rows.device.type != "cuda":
-        return rotary_heads_torch(rows, positions, frequencies, heads=heads, kv_heads=kv_heads, layout=layout)
+        return rotary_heads_torch(rows, positions, frequencies, heads=heads, kv_heads=kv_heads, layout=layout, dtype=dtype)
     counts, D, interleaved, pos = _check_rows(rows, positions, frequencies, heads, kv_heads, layout)
     B, N, _ = rows.shape
+    dtype = rows.dtype if dtype is None else dtype
     _check_kernel(D, rows.dtype)
+    _check_kernel(D, dtype)
     run = _RowsFunction.apply if _native.takes_gradient(rows) else _rows_to_heads
     plan = _Plan(pos, frequencies.table, frequencies.axes, frequencies.gain, interleaved)
-    return run(plan, rows, counts, B, N, D, rows.dtype)
+    return run(plan, rows, counts, B, N, D, dtype)
 
 
 def _packed_rotary_heads(rows: torch.Tensor, slot: torch.Tensor, positions: torch.Tensor,

@@ -259,8 +259,9 @@ class KnnLocalAttention(nn.Module):
             qkv = F.linear(h, mha.in_proj_weight, mha.in_proj_bias)
             cdt = self._core_dtype(h, qkv)
             if self.rotary is not None:
-                q, k, v = rotary_heads(qkv.to(cdt), self._positions(mask), self._rotary(h.device), heads=H,
-                                       layout=self.rotary_layout)
+                rows = qkv.float() if qkv.dtype == torch.float64 else qkv  # fp64 is no type of the kernel's
+                q, k, v = rotary_heads(rows, self._positions(mask), self._rotary(h.device), heads=H,
+                                       layout=self.rotary_layout, dtype=cdt)
             else:
                 q, k, v = (t.reshape(B, T, H, D).transpose(1, 2).to(cdt).contiguous() for t in qkv.chunk(3, dim=-1))
             out = self._attend(q, k, v, mask)

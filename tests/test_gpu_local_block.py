@@ -201,3 +201,54 @@ def test_a_training_trunk_makes_its_tables_once(cuda, packed, monkeypatch):
     with torch.no_grad():
         trunk(x, cond, coords, pad)
     assert len(made) == 1
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_float32_heads_round_once(cuda, packed, monkeypatch):
+    """fp32 projections in inference: the 16-bit heads are the turned fp32 rows rounded once, padded or packed."""
+    import torch.nn.functional as F
+
+    from matterformer_amd.rotary import rotary_frequencies
+    from matterformer_amd.trunk import KnnLocalAttention, build_knn_mask
+    from rotary_reference import assert_turned, rotate64
+
+    torch.manual_seed(8)
+    f = rotary_frequencies(60, axes=3, base=30.0)
+    attn = KnnLocalAttention(128, 2, rotary=f).to(cuda).eval()
+    gen = torch.Generator().manual_seed(9)
+    h, coords = torch.randn(1, 40, 128, generator=gen).to(cuda), torch.randn(1, 40, 3, generator=gen).to(cuda)
+    seen = []
+    real = attn._attend
+    monkeypatch.setattr(attn, "_attend", lambda q, k, v, mask: seen.extend((q, k, v)) or real(q, k, v, mask))
+    with torch.no_grad():
+        mask = build_knn_mask(coords, 8, None, use_hip=True)
+        if packed:
+            hp = h.view(40, 128)
+            rows = F.linear(hp, attn.attn.in_proj_weight, attn.attn.in_proj_bias).view(1, 40, 384)
+            attn.forward_packed(hp, mask, TokenPacking(torch.zeros(1, 40, dtype=torch.bool, device=cuda)))
+        else:
+            rows = F.linear(h, attn.attn.in_proj_weight, attn.attn.in_proj_bias)
+            attn(h, mask)
+    heads = [t.view(1, 40, 2, 64).transpose(1, 2) for t in rows.split(128, dim=-1)]
+    assert all(t.dtype == torch.bfloat16 for t in seen) and attn._last_impl_used == "triton"
+    for got, part, name in zip(seen[:2], heads[:2], "qk"):
+        assert_turned(got, *rotate64(part, coords, f.table, 3, 1.0, "half"), name)
+    assert torch.equal(seen[2], heads[2].bfloat16())
+
+
+def test_float64_modules_in_inference(cuda):
+    """The core runs in 16 bits, as it does without rotary positions."""
+    from matterformer_amd.trunk import KnnLocalAttention, build_knn_mask
+
+    torch.manual_seed(10)
+    attn = KnnLocalAttention(128, 2, rotary=rotary_frequencies(60, axes=3, base=30.0)).to(cuda).double().eval()
+    h, coords = torch.randn(1, 40, 128, device=cuda).double(), torch.randn(1, 40, 3, device=cuda)
+    with torch.no_grad():
+        mask = build_knn_mask(coords, 8, None, use_hip=True)
+        out = attn(h, mask)
+        assert attn._last_impl_used == "triton"
+        attn.impl = "torch"
+        want = attn(h, mask)
+    assert out.dtype == torch.float64
+    # heads, P and the core's output round to bf16 (three roundings of 2^-8 / sqrt(3) in the mean square): 4e-3 of the norm
+    assert rel(out, want.cpu()) <= 1e-2

@@ -7,7 +7,7 @@ import torch
 
 from matterformer_amd import _native
 from matterformer_amd.rotary import RotaryFrequencies, apply_rotary, rotary_frequencies, rotary_heads
-from rotary_reference import rotate64
+from rotary_reference import assert_turned, rotate64
 
 
 def test_table_of_each_scaling():
@@ -91,6 +91,24 @@ def test_rows_equal_heads():
                         pos.expand(2, 7), f, layout="interleaved")
     assert torch.equal(q, a) and torch.equal(k, b) and torch.equal(v, hv.view(2, 7, 1, 10).transpose(1, 2))
     assert all(t.is_contiguous() for t in (q, k, v))
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_heads_in_another_dtype(layout):
+    """Rounded once, from the rows' own type; the gradient comes in theirs."""
+    gen = torch.Generator().manual_seed(5)
+    rows = torch.randn(2, 7, 3 * 2 * 10, generator=gen, requires_grad=True)
+    pos, f = torch.arange(7)[None] * 3, rotary_frequencies(8)
+    q, k, v = rotary_heads(rows, pos, f, heads=2, layout=layout, dtype=torch.bfloat16)
+    assert all(t.dtype == torch.bfloat16 for t in (q, k, v))
+    for got, part in zip((q, k), rows.split(20, dim=-1)):
+        part = part.reshape(2, 7, 2, 10).transpose(1, 2)
+        assert_turned(got, *rotate64(part, pos.expand(2, 7), f.table, 1, 1.0, layout), layout)
+    assert torch.equal(v, rows[..., 40:].reshape(2, 7, 2, 10).transpose(1, 2).bfloat16())
+    (g,) = torch.autograd.grad((q, k, v), rows, [torch.ones_like(t) for t in (q, k, v)])
+    assert g.dtype == torch.float32
+    with pytest.raises(RuntimeError, match="heads"):
+        rotary_heads(rows, pos, f, heads=2, dtype=torch.int32)
 
 
 def test_argument_refusals():
