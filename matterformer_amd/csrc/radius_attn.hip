@@ -64,10 +64,16 @@ struct Ops<_Float16> {
   }
 };
 
-// One key-tile stream: 4 waves per (cell, head, 64-query tile), V staged transposed.  For cells of one tile at head_dim
-// 128, where a second stream would only idle (256 molecules of 30 atoms, 8 heads: 36 us, with two streams 39).
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) radius_attn_kernel(Params p) {
+// One key-tile stream: 4 waves per (cell, head, 64-query tile), V staged transposed, two workgroups a CU.  At head_dim 128
+// for cells of one tile, where a second stream would only idle, and of up to three once there is more than a workgroup per
+// CU, of which two streams leave room for one (8 heads, one stream and two: 256 molecules of 19 atoms 20 and 35 us, of 64 30
+// and 42, of 96 65 and 90, of 181 143 and 175; 16 of 96 8.0 and 6.9, of 181 14.0 and 14.3; 64 of 181 at 4 heads, the worst of
+// the rule, 22.8 and 21.6; 64 of 256 60 and 50).
+//
+// TAB: the call has key_any or out_lo.  Compiled apart, because their registers cost a plain forward up to 1.7 times its time
+// (head_dim 128, one wave a SIMD instead of two) and 20-30 % at head_dim 32.
+template <typename T, int D, bool TAB>
+__global__ void __launch_bounds__(kThreads, 2) radius_attn_kernel(Params p) {
   using Op8 = typename Ops<T>::Op8;
   typedef __attribute__((__vector_size__(4 * sizeof(T)))) T Op4;
   constexpr int KS = D + 8;         // K row stride in LDS (elements)
@@ -150,7 +156,7 @@ __global__ void __launch_bounds__(kThreads) radius_attn_kernel(Params p) {
     uint32_t valid;   // bit t: K chunk t is a real key; bit CPT + t: V chunk t
   };
   // keys no query of this tile attends are staged as zeros, so that what they hold (NaN too) reaches no sum
-  const uint64_t* kany = p.key_any ? p.key_any + (size_t(b) * p.NB + qt) * p.NB : nullptr;
+  const uint64_t* kany = TAB && p.key_any ? p.key_any + (size_t(b) * p.NB + qt) * p.NB : nullptr;
   uint32_t seen = 0u;  // the query has a key
   auto load_tile = [&](int jt, Stage& st) {
     const uint64_t set = kany ? kany[jt] : ~uint64_t(0);
@@ -173,7 +179,8 @@ __global__ void __launch_bounds__(kThreads) radius_attn_kernel(Params p) {
       const int vd0 = (c / kTile) * 8;
       st.k[t] = *reinterpret_cast<const Op8*>(gk + size_t(min(key, N - 1)) * D + d0);
       st.v[t] = *reinterpret_cast<const Op8*>(gv + size_t(min(vkey, N - 1)) * D + vd0);
-      const bool kuse = key < N && ((set >> (c / CPR)) & 1u), vuse = vkey < N && ((set >> (c % kTile)) & 1u);
+      const bool kuse = key < N && (!TAB || ((set >> (c / CPR)) & 1u));
+      const bool vuse = vkey < N && (!TAB || ((set >> (c % kTile)) & 1u));
       st.valid |= (kuse ? 1u << t : 0u) | (vuse ? 1u << (CPT + t) : 0u);
     }
   };
@@ -320,7 +327,7 @@ __global__ void __launch_bounds__(kThreads) radius_attn_kernel(Params p) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) ov[r] = T(o[r]);
       *reinterpret_cast<Op4*>(static_cast<T*>(p.out) + row * D + d0) = ov;
-      if (p.out_lo) {
+      if (TAB && p.out_lo) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) ov[r] = T(o[r] - float(ov[r]));
         *reinterpret_cast<Op4*>(static_cast<T*>(p.out_lo) + row * D + d0) = ov;
@@ -338,9 +345,8 @@ __global__ void __launch_bounds__(kThreads) radius_attn_kernel(Params p) {
 // parity, not the position in the active list, picks the stream, so the
 // sums are the same whether or not empty tiles are skipped.)  With twice the
 // waves per workgroup and half the steps per wave, up to four waves share each
-// SIMD.  (head_dim 128 too, where the two streams' double buffers take 143 KB of
-// LDS: one 64-query tile by four waves, with V staged transposed, took 133 us on
-// four cells of 1997 atoms and 8 heads, this 60.)  At the end the two streams' (O, m, l) of a
+// SIMD.  (At head_dim 128 the two streams' double buffers take 143 KB of LDS: four
+// cells of 1997 atoms and 8 heads, every tile active, 101 us, by one stream 175.)  At the end the two streams' (O, m, l) of a
 // query meet in LDS:
 //   out = (2^(m0 - M) O0 + 2^(m1 - M) O1) / (2^(m0 - M) l0 + 2^(m1 - M) l1).
 // ---------------------------------------------------------------------------
@@ -356,7 +362,7 @@ constexpr int kThreads2 = 512;
 // the LDS reads per query), and the workgroup's key tiles are those active in
 // either of its two 64-query block rows (a key tile none of a query's keys
 // are allowed in adds exactly 0 to that query's sums).
-template <typename T, int D, bool POS, int QW>
+template <typename T, int D, bool POS, int QW, bool TAB>
 __global__ void __launch_bounds__(kThreads2, 3 - QW) radius_attn_pair_kernel(Params p) {
   using Op8 = typename Ops<T>::Op8;
   typedef __attribute__((__vector_size__(4 * sizeof(T)))) T Op4;
@@ -478,7 +484,7 @@ __global__ void __launch_bounds__(kThreads2, 3 - QW) radius_attn_pair_kernel(Par
     uint64_t set;             // the attended ones
   };
   const int row0 = qt * QW;  // first 64-query block row of the workgroup
-  const uint64_t* kany = p.key_any ? p.key_any + (size_t(b) * p.NB + row0) * p.NB : nullptr;
+  const uint64_t* kany = TAB && p.key_any ? p.key_any + (size_t(b) * p.NB + row0) * p.NB : nullptr;
   const bool second = QW == 2 && row0 + 1 < p.NB;
   auto load_tile = [&](int jt, Stage& st) {
     st.set = kany ? kany[jt] | (second ? kany[p.NB + jt] : 0) : ~uint64_t(0);
@@ -493,7 +499,7 @@ __global__ void __launch_bounds__(kThreads2, 3 - QW) radius_attn_pair_kernel(Par
     }
     const int key0 = jt * kTile;
     st.key0 = key0;
-    st.full = key0 + kTile <= N && st.set == ~uint64_t(0);
+    st.full = key0 + kTile <= N && (!TAB || st.set == ~uint64_t(0));
     const T* kb = gk + size_t(key0) * D;
     const T* vb = gv + size_t(key0) * D;
     if (st.full) {
@@ -525,7 +531,7 @@ __global__ void __launch_bounds__(kThreads2, 3 - QW) radius_attn_pair_kernel(Par
 #pragma unroll
       for (int t = 0; t < CPT; ++t) {
         Op8 kz = st.k[t], vz = st.v[t];
-        if (st.key0 + krow[t] >= N || !((st.set >> krow[t]) & 1u)) {
+        if (st.key0 + krow[t] >= N || (TAB && !((st.set >> krow[t]) & 1u))) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) kz[e] = vz[e] = T(0.0f);
         }
@@ -747,7 +753,7 @@ __global__ void __launch_bounds__(kThreads2, 3 - QW) radius_attn_pair_kernel(Par
 #pragma unroll
         for (int r = 0; r < 4; ++r) ov[r] = T(o[r]);
         *reinterpret_cast<Op4*>(static_cast<T*>(p.out) + row * D + d0) = ov;
-        if (p.out_lo) {
+        if (TAB && p.out_lo) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) ov[r] = T(o[r] - float(ov[r]));
           *reinterpret_cast<Op4*>(static_cast<T*>(p.out_lo) + row * D + d0) = ov;
@@ -759,10 +765,10 @@ __global__ void __launch_bounds__(kThreads2, 3 - QW) radius_attn_pair_kernel(Par
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool TAB>
 int launch(const Params& p, hipStream_t stream) {
   const dim3 grid((p.units + 7) / 8 * 8);
-  hipLaunchKernelGGL((radius_attn_kernel<T, D>), grid, dim3(kThreads), 0, stream, p);
+  hipLaunchKernelGGL((radius_attn_kernel<T, D, TAB>), grid, dim3(kThreads), 0, stream, p);
   MF_HIP_CHECK(hipGetLastError());
   return MF_OK;
 }
@@ -770,29 +776,29 @@ int launch(const Params& p, hipStream_t stream) {
 // Two query tiles per wave once a (cell, head) spans more than three 64-query
 // tiles (the 128-query workgroups then waste at most a quarter of a tile's
 // queries to padding) and the launch still has a workgroup per CU.
-template <typename T, int D>
+template <typename T, int D, bool TAB>
 int launch_pair(const Params& p, hipStream_t stream) {
   const bool wide = p.N > 3 * kTile && (long long)p.B * p.H * ((p.N + 2 * kTile - 1) / (2 * kTile)) >= 256;
   Params q = p;
   if (wide) q.units = p.B * p.H * ((p.N + 2 * kTile - 1) / (2 * kTile));
   const dim3 grid((q.units + 7) / 8 * 8);
   if (p.scale_log2 > 0.0f) {
-    if (wide) hipLaunchKernelGGL((radius_attn_pair_kernel<T, D, true, 2>), grid, dim3(kThreads2), 0, stream, q);
-    else hipLaunchKernelGGL((radius_attn_pair_kernel<T, D, true, 1>), grid, dim3(kThreads2), 0, stream, q);
+    if (wide) hipLaunchKernelGGL((radius_attn_pair_kernel<T, D, true, 2, TAB>), grid, dim3(kThreads2), 0, stream, q);
+    else hipLaunchKernelGGL((radius_attn_pair_kernel<T, D, true, 1, TAB>), grid, dim3(kThreads2), 0, stream, q);
   } else {
-    if (wide) hipLaunchKernelGGL((radius_attn_pair_kernel<T, D, false, 2>), grid, dim3(kThreads2), 0, stream, q);
-    else hipLaunchKernelGGL((radius_attn_pair_kernel<T, D, false, 1>), grid, dim3(kThreads2), 0, stream, q);
+    if (wide) hipLaunchKernelGGL((radius_attn_pair_kernel<T, D, false, 2, TAB>), grid, dim3(kThreads2), 0, stream, q);
+    else hipLaunchKernelGGL((radius_attn_pair_kernel<T, D, false, 1, TAB>), grid, dim3(kThreads2), 0, stream, q);
   }
   MF_HIP_CHECK(hipGetLastError());
   return MF_OK;
 }
 
-template <typename T>
+template <typename T, bool TAB>
 int dispatch_dim(const Params& p, int D, hipStream_t stream) {
-  if (D == 32) return launch_pair<T, 32>(p, stream);
-  if (D == 64) return launch_pair<T, 64>(p, stream);
-  if (p.N <= kTile) return launch<T, 128>(p, stream);
-  return launch_pair<T, 128>(p, stream);
+  if (D == 32) return launch_pair<T, 32, TAB>(p, stream);
+  if (D == 64) return launch_pair<T, 64, TAB>(p, stream);
+  if (p.N <= kTile || (p.N <= 3 * kTile && p.units > 256)) return launch<T, 128, TAB>(p, stream);
+  return launch_pair<T, 128, TAB>(p, stream);
 }
 
 }  // namespace rattn
@@ -825,6 +831,10 @@ extern "C" int mf_radius_attn(const mf_radius_attn_args* a, void* stream) {
   rattn::Params p{a->q, a->k, a->v, a->mask_bits, a->block_mask, a->out, a->out_f32, a->lse,
                   a->scale * kLog2e, a->batch, a->heads, a->atoms, (a->atoms + 31) / 32, nb, int(units), a->out_lo, a->key_any};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a->dtype == MF_DTYPE_BF16) return rattn::dispatch_dim<__bf16>(p, a->head_dim, s);
-  return rattn::dispatch_dim<_Float16>(p, a->head_dim, s);
+  const bool tables = a->key_any || a->out_lo;
+  if (a->dtype == MF_DTYPE_BF16)
+    return tables ? rattn::dispatch_dim<__bf16, true>(p, a->head_dim, s)
+                  : rattn::dispatch_dim<__bf16, false>(p, a->head_dim, s);
+  return tables ? rattn::dispatch_dim<_Float16, true>(p, a->head_dim, s)
+                : rattn::dispatch_dim<_Float16, false>(p, a->head_dim, s);
 }

@@ -380,3 +380,33 @@ def test_tables_that_name_every_row(cuda, dtype, N, D):
     every = RadiusTables(t.bits_t, torch.full_like(t.key_any, -1), torch.full_like(t.query_any, -1))
     want, got = gradients(q, k, v, go, bits, None, tables=t), gradients(q, k, v, go, bits, None, tables=every)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N", [65, 100, 192])
+@pytest.mark.parametrize("scale", [0.1, -0.1])
+def test_head_dim_128_of_few_tiles_and_many_cells(cuda, dtype, N, scale):
+    """Two and three tiles a cell, by the kernel of many workgroups and by that of few: each against float64, with and
+    without tables, with NaN where nobody is paired, and the gradients of many.
+
+    |out' - out| <= (2 es + 2 t + N u + 2^-20) sum P|v| + t |out| as above (P rounded, the sum, the last rounding)."""
+    t = torch.finfo(dtype).eps / 2
+    for B, H in ((40, 8), (3, 2)):
+        q, k, v, go, gen = operands(B, H, N, 128, dtype, 17, cuda)
+        allowed = mask_of("ragged", B, N, gen)
+        bits = pack(allowed).to(cuda)
+        tables = radius_tables(bits)
+        out = radius_attention(q, k, v, bits, scale=scale)
+        assert torch.equal(radius_attention(q, k, v, bits, scale=scale, tables=tables), out)
+        want, _, grads, bounds = reference(q, k, v, go, allowed, scale)
+        Q, K, V, A = q.double(), k.double(), v.double(), allowed.to(cuda)[:, None]
+        s = (scale * (Q @ K.mT)).masked_fill(~A, -math.inf)
+        P = torch.nan_to_num(torch.softmax(s, -1))
+        es = 132 * U * abs(scale) * torch.where(A, Q.abs() @ K.abs().mT, 0.0).amax(-1, keepdim=True)
+        check(out, want, (2 * es + 2 * t + N * U + 2.0 ** -20) * (P @ V.abs()), "out")
+        no_key, no_query = ~allowed.any(2).to(cuda), ~allowed.any(1).to(cuda)
+        bad = [x.masked_fill(m[:, None, :, None], float("nan")) for x, m in zip((q, k, v), (no_key, no_query, no_query))]
+        assert torch.equal(radius_attention(*bad, bits, scale=scale, tables=tables), out)
+        assert torch.equal(radius_attention(bad[0], k, v, bits, scale=scale), out)
+        for g, w, b, name in zip(gradients(q, k, v, go, bits, None, scale=scale), grads, bounds, ("dq", "dk", "dv")):
+            check(g, w, b, name)
