@@ -1096,10 +1096,14 @@ int check(const char* name, const mf_gated_linear_args* a) {
     return fail(MF_ERR_INVALID_ARGUMENT, n + ": bad activation");
   // tile-relative byte offsets are 32 bits: the weight below 2^31 bytes, 256 rows of x and of [dA dB] too
   const int64_t esize = a->dtype == MF_DTYPE_F32 ? 4 : 2;
-  if ((a->channels + 8) * int64_t(a->hidden) * 2 * esize >= (int64_t(1) << 31) ||
-      a->x_stride * 256 * esize >= (int64_t(1) << 31) || int64_t(a->hidden + 64) * 512 * esize >= (int64_t(1) << 31) ||
-      a->tokens > (1 << 30))
-    return fail(MF_ERR_UNSUPPORTED, n + ": weight of 2^31 bytes, rows of 2^22 elements or 2^30 tokens and more are not supported");
+  const int64_t reach = (int64_t(1) << 31) / (256 * esize);  // elements between rows: 2^22, of fp32 2^21
+  if (a->tokens > (1 << 30)) return fail(MF_ERR_UNSUPPORTED, n + ": at most 2^30 tokens");
+  if (a->x_stride >= reach)
+    return fail(MF_ERR_UNSUPPORTED, n + ": rows of x " + std::to_string(reach) + " elements apart and more are not supported");
+  if ((a->channels + 8) * int64_t(a->hidden) * 2 * esize >= (int64_t(1) << 31))
+    return fail(MF_ERR_UNSUPPORTED, n + ": a weight of 2^31 bytes and more is not supported");
+  if (2 * (int64_t(a->hidden) + 64) >= reach)
+    return fail(MF_ERR_UNSUPPORTED, n + ": hidden above " + std::to_string(reach / 2 - 65) + " is not supported");
   return MF_OK;
 }
 

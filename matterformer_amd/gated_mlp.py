@@ -34,6 +34,15 @@ def _arguments(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None,
         hidden=weight.shape[0] // 2, activation=_native.MF_ACT[activation], dtype=_native.dtype_code(x.dtype))
 
 
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """Rows as the kernels take them: copied unless their entries lie side by side and the rows apart, but not so far
+    that a tile of 256 reaches 2^31 bytes."""
+    apart = x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    if x.stride(-1) != 1 or apart < x.shape[1] or apart * 256 * x.element_size() >= 1 << 31:
+        return x.contiguous()
+    return x
+
+
 def _scratch(nbytes: int, device: torch.device) -> torch.Tensor | None:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
@@ -102,9 +111,7 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
         return _TORCH_ACT[activation](gate) * up
     if x.dtype not in _DTYPES:
         raise RuntimeError(f"gated_linear supports bfloat16, float16 and float32 on the GPU, got {x.dtype}")
-    rows = x if x.ndim == 2 else x.reshape(-1, x.shape[-1])
-    if rows.stride(-1) != 1 or (rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]):
-        rows = rows.contiguous()
+    rows = _rows(x if x.ndim == 2 else x.reshape(-1, x.shape[-1]))
     weight = weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     if _native.takes_gradient(rows, weight, bias):

@@ -67,3 +67,36 @@ def test_c_entries_refuse_before_any_device_call():
     assert lib.mf_gated_linear_bwd(b, None) == invalid and "nothing to compute" in _native.last_error()
     b.grad_out = None
     assert lib.mf_gated_linear_bwd(b, None) == invalid and "grad_out" in _native.last_error()
+
+
+def test_c_entries_name_the_limit_that_a_call_passes():
+    """Offsets within a tile are 32 bits: each limit with its size, which half as many elements of fp32 reach."""
+    lib = _native.lib()
+    fake = 1 << 20
+
+    def refusal(**kw):
+        a = dict(x=fake, weight=fake, out=fake, x_stride=64, tokens=4, channels=8, hidden=32, dtype=2)
+        a.update(kw)
+        a["x_stride"] = max(a["x_stride"], a["channels"])
+        assert lib.mf_gated_linear(_native.MfGatedLinearArgs(**a), None) == _native.MF_ERR_UNSUPPORTED
+        return _native.last_error()
+
+    assert "tokens" in refusal(tokens=(1 << 30) + 1)
+    assert "weight" in refusal(channels=16384, hidden=53248)
+    for dtype, most in ((2, 1 << 22), (0, 1 << 21)):
+        assert f"rows of x {most} elements apart" in refusal(x_stride=most, dtype=dtype)
+        assert f"hidden above {most // 2 - 65}" in refusal(channels=1, hidden=most // 2 - 64, dtype=dtype)
+
+
+def test_rows_far_apart_are_copied():
+    from matterformer_amd.gated_mlp import _rows
+
+    assert _rows(torch.zeros(8).expand(3, 8)).is_contiguous()  # rows on top of each other
+    near = torch.zeros(2, 16)[:, :8]
+    assert _rows(near) is near
+    one = torch.empty(1, 8).as_strided((1, 8), (1 << 40, 1))
+    assert _rows(one) is one  # one row's stride means nothing
+    for dtype, most in ((torch.bfloat16, 1 << 22), (torch.float32, 1 << 21)):
+        base = torch.zeros(most + 8, dtype=dtype)
+        assert _rows(base.as_strided((2, 8), (most - 8, 1))).stride(0) == most - 8
+        assert _rows(base.as_strided((2, 8), (most, 1))).is_contiguous()

@@ -375,3 +375,13 @@ def test_half_gradients_in_a_graph(cuda, C):
         now = _run(x, w, b, go, "silu")
         assert torch.equal(held[0], now[0]) and all(torch.equal(p, q) for p, q in zip(held[1], now[1])), size
         _half_check(x, w, b, go, "silu", now[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_far_apart(cuda, dtype):
+    """Rows 2^22 elements apart, past what a tile's offsets reach: copied, not refused."""
+    x, w, b, go = _inputs(5, 64, 40, dtype, True, 28, cuda)
+    wide = torch.zeros(5, 1 << 22, dtype=dtype, device=cuda)
+    wide[:, :64] = x
+    out, grads = _run(wide[:, :64], w, b, go, "silu")
+    _check(x, w, b, go, "silu", out, grads)
