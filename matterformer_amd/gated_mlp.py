@@ -91,8 +91,9 @@ class _GatedLinearFunction(torch.autograd.Function):
 def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
                  activation: str = "silu") -> torch.Tensor:
     """act(x Wg^T + bg) * (x Wu^T + bu): x (..., C); weight (2F, C), Wg its first F rows and Wu its last; bias (2F,) or
-    None; one dtype (under autocast, its dtype).  ``activation``: silu, gelu, gelu_tanh, relu or sigmoid.  Returns (..., F), differentiable in x,
-    weight and bias.  Sums, activation and product are fp32 on the GPU, rounded once."""
+    None; one dtype (under autocast, its dtype, unless they are float64).  ``activation``: silu, gelu, gelu_tanh, relu or
+    sigmoid.  Returns (..., F), differentiable in x, weight and bias.  Sums, activation and product are fp32 on the GPU,
+    rounded once.  Up to 2^30 tokens and weights below 2^31 bytes there; hidden below 2^21 (float32 2^20)."""
     if activation not in _native.MF_ACT:
         raise ValueError(f"Unsupported activation: {activation}; expected one of {ACTIVATIONS}")
     if weight.ndim != 2 or weight.shape[0] == 0 or weight.shape[0] % 2 != 0 or weight.shape[1] == 0:
@@ -103,7 +104,7 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
         raise ValueError(f"bias must have shape ({weight.shape[0]},), got {tuple(bias.shape)}")
     if torch.is_autocast_enabled(x.device.type):
         dtype = torch.get_autocast_dtype(x.device.type)
-        x, weight, bias = (t if t is None else t.to(dtype) for t in (x, weight, bias))
+        x, weight, bias = (t if t is None or t.dtype == torch.float64 else t.to(dtype) for t in (x, weight, bias))
     if any(t is not None and (t.dtype != x.dtype or t.device != x.device) for t in (weight, bias)):
         raise RuntimeError("x, weight and bias must share a dtype and a device")
     if x.device.type != "cuda":

@@ -100,3 +100,14 @@ def test_rows_far_apart_are_copied():
         base = torch.zeros(most + 8, dtype=dtype)
         assert _rows(base.as_strided((2, 8), (most - 8, 1))).stride(0) == most - 8
         assert _rows(base.as_strided((2, 8), (most, 1))).is_contiguous()
+
+
+def test_autocast_leaves_float64_alone():
+    """As it does F.linear; other types come to its own."""
+    x, w = torch.randn(3, 5, dtype=torch.float64), torch.randn(8, 5, dtype=torch.float64)
+    want = gated_linear(x, w)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        assert torch.nn.functional.linear(x, w).dtype == torch.float64
+        got = gated_linear(x, w)
+        assert gated_linear(x.float(), w.float()).dtype == torch.bfloat16
+    assert got.dtype == torch.float64 and torch.equal(got, want)
