@@ -385,3 +385,32 @@ def test_rows_far_apart(cuda, dtype):
     wide[:, :64] = x
     out, grads = _run(wide[:, :64], w, b, go, "silu")
     _check(x, w, b, go, "silu", out, grads)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T,C,F", [(4100, 1096, 2047), (8200, 2104, 600)])
+def test_large_tiles_of_both_gradients(cuda, dtype, T, C, F):
+    """Sizes whose dx and dW are cut into tiles of 256 (tiles times pieces of 16 K steps reach the 256 CUs): 85 and 80
+    tiles in three pieces each; 297 tiles, 256 whole and 41 in five pieces, and 45 tiles in five.  Every edge is ragged."""
+    x, w, b, go = _inputs(T, C, F, dtype, True, 29, cuda)
+    out, grads = _run(x, w, b, go, "silu")
+    _check(x, w, b, go, "silu", out, grads)
+    again = _run(x, w, b, go, "silu")[1]
+    assert all(torch.equal(p, q) for p, q in zip(grads, again))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradients_past_2_31_intermediate_elements(cuda, dtype):
+    """2^24 + 300 tokens of 2 x 64 intermediate values: dx of the first and last tokens, and dW, to which only those
+    contribute (x is zero between them)."""
+    T = 2 ** 24 + 300
+    _, w, _, _ = _inputs(1, 8, 64, dtype, False, 30, cuda)
+    gen = torch.Generator().manual_seed(31)
+    x = torch.zeros(T, 8, dtype=dtype, device=cuda)
+    rows = torch.cat([torch.arange(200), torch.arange(T - 400, T)]).to(cuda)
+    x[rows] = torch.randn(600, 8, generator=gen).to(dtype).to(cuda)
+    go = torch.empty(T, 64, dtype=dtype, device=cuda).normal_().mul_(0.1)
+    leaves = [x.requires_grad_(True), w.requires_grad_(True)]
+    out = gated_linear(*leaves)
+    dx, dw = torch.autograd.grad(out, leaves, go)
+    _check(x.detach()[rows], w.detach(), None, go[rows], "silu", out.detach()[rows], (dx[rows], dw, None))
