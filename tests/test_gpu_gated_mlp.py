@@ -414,3 +414,13 @@ def test_gradients_past_2_31_intermediate_elements(cuda, dtype):
     out = gated_linear(*leaves)
     dx, dw = torch.autograd.grad(out, leaves, go)
     _check(x.detach()[rows], w.detach(), None, go[rows], "silu", out.detach()[rows], (dx[rows], dw, None))
+
+
+def test_gelu_keeps_its_relative_accuracy_in_the_tail(cuda):
+    """fp32, one channel, weights of one: h = gelu(a) a for a from -12 to 12.  The normal distribution comes within 10 units
+    of 2^-24 (the fit 1, t, its last steps and the product 7, the exponential 2) and the three products that follow round
+    once each: 16 units, relative also where gelu is 1e-32."""
+    a = torch.cat([torch.linspace(-12.0, 12.0, 100001), torch.tensor([0.0, -1e-20, 1e-20])]).to(cuda)
+    out = gated_linear(a[:, None], torch.ones(2, 1, device=cuda), activation="gelu")[:, 0]
+    want = _act64(a.double(), "gelu")[0] * a.double()
+    assert torch.all((out.double() - want).abs() <= 16 * U * want.abs() + 2.0 ** -126)
