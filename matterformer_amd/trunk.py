@@ -165,7 +165,8 @@ class KnnLocalAttention(nn.Module):
     depends on the atoms' difference vector.  The coordinates take no gradient there: under autograd they are refused
     when they ask for one.  ``hip_backward``: autograd follows the HIP kernels where the
     projections are 16-bit (radius_attention's and rotary_heads' gradients); otherwise training takes the torch
-    path, as fp32 projections always do."""
+    path, as fp32 projections always do.  (In inference the HIP core of fp32 projections runs in bfloat16, with rotary
+    positions or without.)"""
 
     def __init__(self, d_model: int, n_heads: int, *, dropout: float = 0.0, impl: str = "auto",
                  rotary: RotaryFrequencies | None = None, rotary_layout: str = "half",
@@ -197,7 +198,7 @@ class KnnLocalAttention(nn.Module):
             return "the HIP local attention has no forward-mode derivative"
         if torch.is_grad_enabled() and (h.requires_grad or any(p.requires_grad for p in self.attn.parameters())):
             if not self.hip_backward:
-                return "the HIP local attention has no backward; autograd takes the torch path"
+                return "the HIP local attention's backward is off (hip_backward); autograd takes the torch path"
             dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else h.dtype
             if dtype not in (torch.bfloat16, torch.float16):
                 return "the HIP local attention's backward needs float16/bfloat16 projections"
