@@ -206,12 +206,13 @@ def _turn_heads(plan: _Plan, heads, inverse: bool) -> tuple[torch.Tensor, ...]:
     outs = tuple(torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in heads)
     first = heads[0]
     B, _, N, D = first.shape
-    if B * N > 0:
-        units = [_unit(t) for t in heads]
+    units = [_unit(t) for t in heads if t.numel() > 0]
+    if units:
+        to = [o for o in outs if o.numel() > 0]
         pad = 3 - len(units)
         zeros = (0, 0, 0) * pad
         _launch(plan, (*(t.data_ptr() for t in units), *(None,) * pad), (*(s for t in units for s in _strides(t)), *zeros),
-                (*(o.data_ptr() for o in outs), *(None,) * pad), (*(s for o in outs for s in o.stride()[:3]), *zeros),
+                (*(o.data_ptr() for o in to), *(None,) * pad), (*(s for o in to for s in o.stride()[:3]), *zeros),
                 (*(t.shape[1] for t in units), *(0,) * pad), batch=B, tokens=N, head_dim=D, inverse=inverse,
                 slot_side=_native.MF_SLOT_NONE, src_dtype=first.dtype, dst_dtype=first.dtype, device=first.device)
     return outs

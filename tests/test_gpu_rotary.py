@@ -247,3 +247,14 @@ def test_two_calls_in_flight_and_long_rows(cuda):
     for t in (q, k, v):
         assert torch.equal(t[1, :, -1], torch.ones(2, 256, dtype=torch.bfloat16, device=cuda))
         assert float(t[0, :, -1].abs().max()) == 0.0 and float(t[1, :, -2].abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("H,KV", [(0, 2), (2, 0), (0, 0)])
+def test_no_heads(cuda, H, KV):
+    f = rotary_frequencies(8).to(cuda)
+    q, k = (torch.ones(2, h, 5, 8, device=cuda, requires_grad=True) for h in (H, KV))
+    pos = torch.zeros(2, 5, device=cuda)
+    out = apply_rotary(q, k, pos, f)
+    grads = torch.autograd.grad(out, (q, k), [torch.ones_like(t) for t in out])
+    for t, o, g in zip((q, k), out, grads):
+        assert torch.equal(o, t.detach()) and torch.equal(g, t.detach())
