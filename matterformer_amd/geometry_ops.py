@@ -276,6 +276,8 @@ def _radius_forward(q, k, v, bits, bm, tables, scale, *, lse: bool, fp32: bool, 
     out = torch.empty_like(q)
     out32 = torch.empty(B, H, N, D, dtype=torch.float32, device=q.device) if fp32 else None
     lse_out = torch.empty(B, H, N, dtype=torch.float32, device=q.device) if lse else None
+    if q.numel() == 0:
+        return out, lse_out, out32
     args = _native.MfRadiusAttnArgs(
         q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), mask_bits=bits.data_ptr(), block_mask=_native.ptr(bm),
         out=out.data_ptr(), out_f32=_native.ptr(out32), lse=_native.ptr(lse_out), scale=scale, batch=B, heads=H,

@@ -410,3 +410,15 @@ def test_head_dim_128_of_few_tiles_and_many_cells(cuda, dtype, N, scale):
         assert torch.equal(radius_attention(bad[0], k, v, bits, scale=scale), out)
         for g, w, b, name in zip(gradients(q, k, v, go, bits, None, scale=scale), grads, bounds, ("dq", "dk", "dv")):
             check(g, w, b, name)
+
+
+@pytest.mark.parametrize("B,H,N", [(0, 2, 5), (2, 0, 5), (2, 2, 0)])
+def test_empty(cuda, B, H, N):
+    bits = torch.zeros(B, N, (N + 31) // 32, dtype=torch.int32, device=cuda)
+    leaves = [torch.zeros(B, H, N, 32, dtype=torch.bfloat16, device=cuda, requires_grad=True) for _ in range(3)]
+    with torch.no_grad():
+        out, lse, out32 = radius_attention(*leaves, bits, return_lse=True, return_fp32=True)
+    assert out.shape == (B, H, N, 32) and lse.shape == (B, H, N) and out32.dtype == torch.float32
+    out = radius_attention(*leaves, bits)
+    grads = torch.autograd.grad(out, leaves, torch.zeros_like(out))
+    assert all(g.shape == t.shape for g, t in zip(grads, leaves))
