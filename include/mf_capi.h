@@ -672,8 +672,9 @@ int mf_radius_tables(const mf_radius_tables_args* args, void* stream);
 /*   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i.            */
 /* Rows without an allowed partner get zeros, and what they hold reaches no  */
 /* other row.  Sums in fp32 in a fixed order (two calls give identical bits); */
-/* P and dS rounded to dtype in between (dS of fp16 times a power of two per */
-/* molecule and head, so that it neither overflows nor loses small values).  */
+/* P and dS rounded to dtype in between (of fp16 P times 2^12 and dS times a */
+/* power of two per molecule and head, found from the rows with a partner,   */
+/* so that neither overflows nor loses small values).                        */
 /* The workspace needs no fill and is 16-byte aligned.                       */
 /* ------------------------------------------------------------------------ */
 typedef struct mf_radius_attn_bwd_args {

@@ -884,8 +884,8 @@ Cut cut_tiles(int64_t m, int64_t n, int64_t k, int esize, bool large, bool split
 constexpr int kFewTokens = 64;  // the forward of few_kernel
 // kFwd and kBwd: large tiles once the small ones need more than one round of two a CU, that is when more than half the
 // CUs get a large one.  bf16, C 512, F 2048, large against small: 1400 tokens (96 large tiles) 17.6 and 13.6 us, 2000
-// (128) 17.9 and 14.2, 2304 (144) 18.9 and 22.6, 3500 (224) 20.5 and 26.0.  fp32, whose matrix rate is a sixteenth,
-// takes small ones.
+// (128) 17.9 and 14.2, 2304 (144) 18.9 and 22.6, 3500 (224) 20.5 and 26.0 (at this width only: the rule leaves out K, and
+// at 176 large tiles, 2738 tokens, 31 % of the CUs idle).  fp32, whose matrix rate is a sixteenth, takes small ones.
 Cut cut_gated(int64_t f, int64_t t, int64_t k, int esize, int num_cus) {
   const bool large = esize == 2 && 2 * ((2 * f + 255) / 256) * ((t + 255) / 256) > num_cus;
   // a large tile is 128 of f and their gate and up rows, a small one 64
