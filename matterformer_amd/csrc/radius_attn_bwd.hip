@@ -30,7 +30,10 @@
 // dS and the result alone leave 2.35e-3).
 //
 // Sums are fp32.  P and dS are rounded to the operands' type for the second
-// products, as any 16-bit matrix product's input is.  fp16 has no room for dS of
+// products, as any 16-bit matrix product's input is: bf16 gradients are off by
+// 2.4e-3 of the norm, where rounding them alone leaves 1.7e-3.  (Tried: the low
+// parts of P and dS as further products, 1.75e-3, for 113 us instead of 92 on 32
+// cells of 512 atoms, 167 instead of 144 on four of 1997 at head_dim 128.)  fp16 has no room for dS of
 // small or large gradients, so there dS is kept times 2^e, e per (molecule,
 // head) from |dP - delta| <= 2 max|go| max|v| + max|dlse| (Cauchy-Schwarz, over the
 // rows that have a partner) so that it stays below 2^14, and P times 2^12 (a key of
