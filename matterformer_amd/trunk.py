@@ -230,7 +230,8 @@ class KnnLocalAttention(nn.Module):
         version = 0 if table.is_inference() else table._version
         held = self._rotary_on.setdefault(device, [])
         if not held or held[-1][0] is not self.rotary:
-            held.append((self.rotary, version, self.rotary.to(device)))
+            with torch.inference_mode(False):  # a gradient may be taken through it later
+                held.append((self.rotary, version, self.rotary.to(device)))
         elif held[-1][1] != version:
             held[-1][2].table.copy_(table)
             held[-1] = (self.rotary, version, held[-1][2])

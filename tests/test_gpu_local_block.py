@@ -252,3 +252,15 @@ def test_float64_modules_in_inference(cuda):
     assert out.dtype == torch.float64
     # heads, P and the core's output round to bf16 (three roundings of 2^-8 / sqrt(3) in the mean square): 4e-3 of the norm
     assert rel(out, want.cpu()) <= 1e-2
+
+
+def test_training_after_inference_mode(cuda):
+    """A first forward under inference_mode leaves nothing that a gradient cannot be taken through."""
+    trunk = build(["knn_local", "knn_local"]).to(cuda)
+    x, cond, coords, pad, weight = (t.to(cuda) for t in inputs())
+    with torch.inference_mode():
+        first = trunk(x, cond, coords, pad)
+    leaf = x.clone().requires_grad_(True)
+    out = trunk(leaf, cond, coords, pad)
+    (out.float() * weight.float()).sum().backward()
+    assert leaf.grad is not None and rel(out, first.cpu().double()) <= 2e-2
