@@ -39,7 +39,7 @@
 extern "C" {
 #endif
 
-#define MF_ABI_VERSION 12
+#define MF_ABI_VERSION 13
 
 typedef enum mf_status {
   MF_OK = 0,
@@ -807,6 +807,166 @@ uint64_t mf_gated_linear_workspace_size(const mf_gated_linear_args* args);
 int mf_gated_linear(const mf_gated_linear_args* args, void* stream);
 uint64_t mf_gated_linear_bwd_workspace_size(const mf_gated_linear_bwd_args* args);
 int mf_gated_linear_bwd(const mf_gated_linear_bwd_args* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Attention over all pairs with a learned bias by buckets (ABI 13).         */
+/*                                                                          */
+/* A pair (i, j) of a query and a key has a bucket 0 .. buckets - 1 (at most */
+/* MF_MAX_BUCKETS) or MF_BUCKET_MASKED, which leaves it out.  The buckets of */
+/* a batch, shared by its heads and layers:                                  */
+/*   index     [B, queries, S(keys)] bytes, S(n) = n rounded up to 64; the   */
+/*             bytes past the last key are MF_BUCKET_MASKED                  */
+/*   index_t   [B, keys, S(queries)] the same transposed                     */
+/*   key_any   [B, TQ, TK], T = tiles of 64: bit t of a tile's word: key t   */
+/*             of the tile has a query in it                                 */
+/*   query_any [B, TK, TQ]: bit t: query t of the tile has a key in it       */
+/* mf_pair_buckets writes them, in one launch.  bucket = how many of the     */
+/* rising edges are at or below the pair's value: with buckets = num_edges + */
+/* 1.  By source, the value is                                               */
+/*   MF_BUCKETS_DISTANCE  the distance of query_pos [B, queries, 3] and      */
+/*                        key_pos [B, keys, 3], fp32; d^2 in fp64 without    */
+/*                        contraction, compared with the edges' squares      */
+/*   MF_BUCKETS_OFFSET    key_pos [B, keys] - query_pos [B, queries], int64  */
+/*   MF_BUCKETS_VALUE     values [B, queries, keys], fp32                    */
+/* and MF_BUCKETS_INDEX takes the bucket itself from values (int32; below 0  */
+/* or from `buckets` on: masked).  Masked besides: pairs of a padded query   */
+/* or key, above the cutoff (distance, value; negative: none), causal: with  */
+/* a positive offset.                                                        */
+/* index_t may be NULL (it is for gradients).  With DISTANCE over one set of */
+/* atoms index_t and query_any may equal index and key_any, both: the matrix */
+/* is its own transpose.                                                     */
+/* ------------------------------------------------------------------------ */
+#define MF_MAX_BUCKETS 64
+#define MF_BUCKET_MASKED 64
+#define MF_BUCKETS_DISTANCE 0
+#define MF_BUCKETS_OFFSET 1
+#define MF_BUCKETS_VALUE 2
+#define MF_BUCKETS_INDEX 3
+typedef struct mf_pair_buckets_args {
+  const void* query_pos;
+  const void* key_pos;
+  const void* values;
+  const uint8_t* query_pad;    /* [B, queries], nonzero = padding, or NULL    */
+  const uint8_t* key_pad;      /* [B, keys] or NULL                          */
+  const double* edges;         /* [num_edges] in host memory, rising         */
+  uint8_t* index;
+  uint8_t* index_t;
+  uint64_t* key_any;
+  uint64_t* query_any;
+  int64_t query_step;          /* elements of query_pos from one batch entry to the next (0: shared) */
+  int64_t key_step;
+  double cutoff;
+  int32_t source;              /* MF_BUCKETS_*                               */
+  int32_t num_edges;           /* <= 63                                      */
+  int32_t buckets;             /* 1 .. MF_MAX_BUCKETS                        */
+  int32_t causal;              /* OFFSET only                                */
+  int32_t batch;
+  int32_t queries;
+  int32_t keys;
+} mf_pair_buckets_args;
+
+int mf_pair_buckets(const mf_pair_buckets_args* args, void* stream);
+
+/* The bias itself: bias[b, h, i, j] = table[index[b, i, j], h], -inf where  */
+/* the pair is masked; table [buckets, H].  Its gradient:                    */
+/*   dtable[c, h] = sum of dbias[b, h, i, j] over the pairs of bucket c,     */
+/* fp32 sums in a fixed order (two calls give identical bits), rounded once  */
+/* to table_dtype; the workspace needs no fill.                              */
+typedef struct mf_bucket_bias_args {
+  const uint8_t* index;        /* [B or 1, queries, S(keys)]                 */
+  const void* table;           /* forward: [buckets, H]                      */
+  void* bias;                  /* [B, H, queries, keys]: written, or, by the gradient, its upstream gradient */
+  void* dtable;                /* gradient: [buckets, H]                     */
+  void* workspace;
+  uint64_t workspace_bytes;
+  int32_t index_batch;         /* 1 or batch                                 */
+  int32_t batch;
+  int32_t heads;               /* <= 128                                     */
+  int32_t queries;
+  int32_t keys;
+  int32_t buckets;
+  int32_t table_dtype;         /* MF_DTYPE_*                                 */
+  int32_t bias_dtype;
+} mf_bucket_bias_args;
+
+int mf_bucket_bias(const mf_bucket_bias_args* args, void* stream);
+uint64_t mf_bucket_bias_bwd_workspace_size(const mf_bucket_bias_args* args);
+int mf_bucket_bias_bwd(const mf_bucket_bias_args* args, void* stream);
+
+/* Attention: S_ij = scale q_i . k_j + table[index_ij, h] over the pairs that */
+/* are not masked, out_i = softmax_j(S_i) v, lse_i = log sum_j exp S_ij.      */
+/* q, k, v bf16 or fp16, element d of (b, h, n) at stride[0] b + stride[1] h */
+/* + stride[2] n + d, the strides multiples of 8 and the bases 16-byte       */
+/* aligned; head h reads key head h / (heads / kv_heads).  head_dim: a       */
+/* multiple of 8 up to 128.  A query without a pair, or all of whose pairs   */
+/* have a bias of -inf, gets out 0 and lse 0.  What keys and queries without */
+/* a pair hold reaches nothing.  Few queries over many keys are split over   */
+/* the keys and joined (workspace, no fill needed).                          */
+/* Softmax and sums in fp32; P rounded to dtype for its product with v.      */
+typedef struct mf_bucket_attn_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* table;           /* [buckets, heads] table_dtype               */
+  const uint8_t* index;        /* mf_pair_buckets' of index_batch            */
+  const uint64_t* key_any;
+  const uint64_t* query_any;
+  void* out;                   /* out_stride                                 */
+  void* out_lo;                /* what out's rounding left, contiguous [B, H, queries, head_dim], or NULL */
+  float* lse;                  /* [B, H, queries] or NULL                    */
+  float* stats;                /* [2, B, H, queries]: of each query the maximum of log2(e) S and 1 / sum, or NULL */
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t out_stride[3];
+  float scale;
+  int32_t index_batch;         /* 1 or batch                                 */
+  int32_t batch;
+  int32_t heads;
+  int32_t kv_heads;            /* divides heads; heads / kv_heads <= 32      */
+  int32_t queries;
+  int32_t keys;
+  int32_t head_dim;
+  int32_t buckets;
+  int32_t dtype;               /* MF_DTYPE_BF16 or MF_DTYPE_F16              */
+  int32_t table_dtype;         /* MF_DTYPE_*                                 */
+} mf_bucket_attn_args;
+
+uint64_t mf_bucket_attn_workspace_size(const mf_bucket_attn_args* args);
+int mf_bucket_attn(const mf_bucket_attn_args* args, void* stream);
+
+/* Its gradients, P formed again from stats:                                 */
+/*   dP_ij = grad_out_i . v_j,  dS_ij = P_ij (dP_ij - delta_i),              */
+/*   delta_i = grad_out_i . out_i - grad_lse_i,                              */
+/*   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,            */
+/*   dv_j = sum_i P_ij grad_out_i,  dtable[c, h] = sum dS_ij over bucket c   */
+/* (dk, dv over the query heads of a key head too, dtable over the batch).   */
+/* Every gradient is written in full (zeros where there is no pair); sums in */
+/* fp32 in a fixed order (two calls give identical bits), P and dS rounded   */
+/* to dtype for their products (of fp16 P times 2^12 and dS times a power of */
+/* two per molecule and key head).  fwd: the forward's operands, out, out_lo */
+/* and stats; its workspace and lse are not used.                            */
+typedef struct mf_bucket_attn_bwd_args {
+  mf_bucket_attn_args fwd;
+  const uint8_t* index_t;
+  const void* grad_out;        /* grad_out_stride                            */
+  const float* grad_lse;       /* [B, H, queries] or NULL                    */
+  void* dq;                    /* strides as the operands have them          */
+  void* dk;
+  void* dv;
+  void* dtable;                /* [buckets, heads] table_dtype, or NULL      */
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t grad_out_stride[3];
+  int64_t dq_stride[3];
+  int64_t dk_stride[3];
+  int64_t dv_stride[3];
+} mf_bucket_attn_bwd_args;
+
+uint64_t mf_bucket_attn_bwd_workspace_size(const mf_bucket_attn_bwd_args* args);
+int mf_bucket_attn_bwd(const mf_bucket_attn_bwd_args* args, void* stream);
 
 #ifdef __cplusplus
 }

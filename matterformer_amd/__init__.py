@@ -9,6 +9,8 @@ Public modules:
                                              re-export shims of the reference
   matterformer_amd.geometry_ops              kNN top-k, radius mask, radius attention (with gradients)
   matterformer_amd.rotary                    rotary positions of heads or in_proj rows
+  matterformer_amd.pair_buckets              buckets of pairs (distance, offset) and their learned bias
+  matterformer_amd.bucket_attention          attention over all pairs with that bias (with gradients)
   matterformer_amd.gated_mlp                 gated linear layer (both projections, activation, product)
 The kernels live in libmf_hip.so (C ABI: include/mf_capi.h), built by
 ``python -m matterformer_amd.build``.
@@ -18,6 +20,13 @@ The package root exports lazily, so ``matterformer_amd.build`` can be imported
 """
 
 _LAZY = {
+    "PairBuckets": "matterformer_amd.pair_buckets",
+    "bucket_bias": "matterformer_amd.pair_buckets",
+    "distance_buckets": "matterformer_amd.pair_buckets",
+    "index_buckets": "matterformer_amd.pair_buckets",
+    "offset_buckets": "matterformer_amd.pair_buckets",
+    "offset_edges": "matterformer_amd.pair_buckets",
+    "value_buckets": "matterformer_amd.pair_buckets",
     "RotaryFrequencies": "matterformer_amd.rotary",
     "apply_rotary": "matterformer_amd.rotary",
     "gated_linear": "matterformer_amd.gated_mlp",

@@ -37,6 +37,13 @@ MF_SLOT_NONE = 0
 MF_SLOT_SRC = 1
 MF_SLOT_DST = 2
 
+MF_MAX_BUCKETS = 64
+MF_BUCKET_MASKED = 64
+MF_BUCKETS_DISTANCE = 0
+MF_BUCKETS_OFFSET = 1
+MF_BUCKETS_VALUE = 2
+MF_BUCKETS_INDEX = 3
+
 MF_ACT = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3, "sigmoid": 4}
 
 MF_PREC = {"bf16_tc": 0, "tf32": 1, "ieee_fp32": 2}
@@ -75,9 +82,17 @@ EXPORTED_SYMBOLS = (
     "mf_gated_linear_workspace_size",
     "mf_gated_linear_bwd",
     "mf_gated_linear_bwd_workspace_size",
+    "mf_pair_buckets",
+    "mf_bucket_bias",
+    "mf_bucket_bias_bwd",
+    "mf_bucket_bias_bwd_workspace_size",
+    "mf_bucket_attn",
+    "mf_bucket_attn_workspace_size",
+    "mf_bucket_attn_bwd",
+    "mf_bucket_attn_bwd_workspace_size",
 )
 
-EXPECTED_ABI_VERSION = 12
+EXPECTED_ABI_VERSION = 13
 
 _DTYPE_CODE = {
     torch.float32: MF_DTYPE_F32,
@@ -283,6 +298,37 @@ class MfGatedLinearBwdArgs(ctypes.Structure):
         ("workspace_bytes", ctypes.c_uint64)]
 
 
+class MfPairBucketsArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("query_pos", "key_pos", "values", "query_pad", "key_pad", "edges", "index",
+                                               "index_t", "key_any", "query_any")] + [
+        ("query_step", ctypes.c_int64), ("key_step", ctypes.c_int64), ("cutoff", ctypes.c_double)] + [
+        (n, ctypes.c_int32) for n in ("source", "num_edges", "buckets", "causal", "batch", "queries", "keys")]
+
+
+class MfBucketBiasArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("index", "table", "bias", "dtable", "workspace")] + [
+        ("workspace_bytes", ctypes.c_uint64)] + [
+        (n, ctypes.c_int32) for n in ("index_batch", "batch", "heads", "queries", "keys", "buckets", "table_dtype",
+                                      "bias_dtype")]
+
+
+class MfBucketAttnArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "table", "index", "key_any", "query_any", "out", "out_lo",
+                                               "lse", "stats", "workspace")] + [
+        ("workspace_bytes", ctypes.c_uint64)] + [
+        (n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] + [
+        ("scale", ctypes.c_float)] + [
+        (n, ctypes.c_int32) for n in ("index_batch", "batch", "heads", "kv_heads", "queries", "keys", "head_dim",
+                                      "buckets", "dtype", "table_dtype")]
+
+
+class MfBucketAttnBwdArgs(ctypes.Structure):
+    _fields_ = [("fwd", MfBucketAttnArgs)] + [
+        (n, ctypes.c_void_p) for n in ("index_t", "grad_out", "grad_lse", "dq", "dk", "dv", "dtable", "workspace")] + [
+        ("workspace_bytes", ctypes.c_uint64)] + [
+        (n, ctypes.c_int64 * 3) for n in ("grad_out_stride", "dq_stride", "dk_stride", "dv_stride")]
+
+
 _LIB: ctypes.CDLL | None = None
 _LOAD_ERROR: str | None = None
 
@@ -323,6 +369,11 @@ def _load() -> ctypes.CDLL | None:
         ("mf_rotary", MfRotaryArgs),
         ("mf_gated_linear", MfGatedLinearArgs),
         ("mf_gated_linear_bwd", MfGatedLinearBwdArgs),
+        ("mf_pair_buckets", MfPairBucketsArgs),
+        ("mf_bucket_bias", MfBucketBiasArgs),
+        ("mf_bucket_bias_bwd", MfBucketBiasArgs),
+        ("mf_bucket_attn", MfBucketAttnArgs),
+        ("mf_bucket_attn_bwd", MfBucketAttnBwdArgs),
     ):
         fn = getattr(lib, name, None)
         if fn is not None:
@@ -346,7 +397,10 @@ def _load() -> ctypes.CDLL | None:
                                          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
         lib.mf_lattice_terms.restype = ctypes.c_int
     for name, argtype in (("mf_gated_linear_workspace_size", MfGatedLinearArgs),
-                          ("mf_gated_linear_bwd_workspace_size", MfGatedLinearBwdArgs)):
+                          ("mf_gated_linear_bwd_workspace_size", MfGatedLinearBwdArgs),
+                          ("mf_bucket_bias_bwd_workspace_size", MfBucketBiasArgs),
+                          ("mf_bucket_attn_workspace_size", MfBucketAttnArgs),
+                          ("mf_bucket_attn_bwd_workspace_size", MfBucketAttnBwdArgs)):
         fn = getattr(lib, name, None)
         if fn is not None:
             fn.argtypes = [ctypes.POINTER(argtype)]

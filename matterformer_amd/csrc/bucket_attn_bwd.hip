@@ -1,0 +1,563 @@
+// Gradients of attention with a bias by buckets (mf_bucket_attn_bwd) on gfx950.
+// With the forward's row maximum m_i and 1 / sum of it,
+//   e_ij = 2^(log2(e) (scale q_i . k_j + bias_ij) - m_i),  P_ij = e_ij / l_i,
+//   dv_j = sum_i P_ij go_i,           dP_ij = go_i . v_j,
+//   dS_ij = P_ij (dP_ij - delta_i),   delta_i = go_i . out_i - dlse_i,
+//   dq_i = scale sum_j dS_ij k_j,     dk_j = scale sum_i dS_ij q_i,
+//   dtable[c, h] = sum of dS_ij over the pairs of bucket c
+// (10 D flops a pair).  m and 1 / l are kept apart, and x - m is formed as the
+// forward forms it: a row all of whose biases are huge and negative (a finite
+// mask value) has P of one all the same, where exp(x - lse) would lose it in
+// lse's rounding.
+//
+// Three kernels; the last two have workgroups of 128 columns, a wave 32, and
+// stream 64-row tiles X and Y of the other side through LDS:
+//   rows:    delta from the forward's out (and what its rounding left)
+//   queries: columns are queries (Q, go in registers), rows keys (X = K, Y = V):
+//            dq^T += K^T dS.  A column is one query, so dS is kept without 1 / l,
+//            which the sum gets at the end.  The sum of a query's dS, which is
+//            dlse_i but for delta's error (out is a product of rounded P), corrects
+//            delta for the next kernel.
+//   keys:    columns are keys (K, V in registers), rows the queries of every head
+//            of the key head (X = Q, Y = go): dk^T += Q^T dS, dv^T += go^T P, and
+//            the table's gradient, in which delta's error would not cancel (with it
+//            dtable is off by 2e-3 of the largest entry, without by 1e-6)
+// P and dS go from the accumulators of the first pair of products into the
+// operands of the second without leaving the lane (bucket_tiles.h).
+//
+// The table's gradient needs no atomics between lanes: every lane adds dS to a
+// sum per bucket of its own in LDS ([bucket][thread], one bank a lane), in the
+// order of its pairs; the threads' sums are joined at the end in a fixed order
+// and the workgroups' by table_sum_kernel.  Two calls give identical bits.
+//
+// Sums are fp32; P and dS are rounded to the operands' type for the second
+// products, as any 16-bit matrix product's input is.  fp16 has no room for dS of
+// small or large gradients: there it is kept times 2^e, e per (batch entry, key
+// head) from |dP - delta| <= 2 max|go| max|v| + max|dlse| over the rows that have
+// a partner, so that it stays below 2^14, and P times 2^12; bf16 has fp32's range
+// and needs neither.
+#include <algorithm>
+#include <cmath>
+
+#include "bucket_tiles.h"
+
+namespace mf {
+namespace bucket {
+
+int check_attn(const mf_bucket_attn_args* a, const char* what);
+int launch_table_sum(const float* parts, void* dtable, int heads, int buckets, int pieces, int dtype, hipStream_t s);
+
+constexpr int kRowThreads = 256;
+constexpr float kProb = 4096.0f;  // fp16: P is kept times this
+
+struct BwdParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* table;
+  const void* out;
+  const void* out_lo;
+  const void* go;
+  const uint8_t* index;
+  const uint8_t* index_t;
+  const uint64_t* key_any;
+  const uint64_t* query_any;
+  const float* stats;  // [2, B H Nq]
+  const float* dlse;
+  void* dq;
+  void* dk;
+  void* dv;
+  float* rows;    // [B H, TQ, 3, 64] m, 1 / l (fp16: times kProb), -delta
+  float4* peak;   // fp16: [B H, TQ] max |go|^2 and |dlse|, then [B KV, TK] max |v|^2
+  float* parts;   // [H, K, B CK] sums of dS by bucket, or null
+  int64_t qs[3], ks[3], vs[3], os[3], gs[3], dqs[3], dks[3], dvs[3];
+  int64_t index_step, index_t_step, any_step;
+  float scale;
+  int B, H, KV, G, Nq, Nk, D, S, St, TQ, TK, K, table_dtype;
+  int CT;  // column tiles of a head, of the kernel at hand
+  int64_t units;
+};
+
+// -- delta, and the peaks ----------------------------------------------------------------------------------------
+// A workgroup takes 64 rows of one head: the first B H TQ of them queries, the others (fp16) rows of v.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kRowThreads) bucket_rows_kernel(BwdParams p) {
+  typedef T T8 __attribute__((ext_vector_type(8)));
+  constexpr int L = DP / 8, RPW = 64 / L;  // lanes a row, rows a wave and pass
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t queries = int64_t(p.B) * p.H * p.TQ;
+  const int64_t id = blockIdx.x;
+  const bool is_query = id < queries;
+  const int64_t unit = is_query ? id : id - queries;
+  const int tiles = is_query ? p.TQ : p.TK, heads = is_query ? p.H : p.KV, N = is_query ? p.Nq : p.Nk;
+  const int64_t bh = unit / tiles;
+  const int tile = int(unit - bh * tiles);
+  const int64_t b = bh / heads;
+  const int h = int(bh - b * heads);
+  uint64_t used = 0;  // rows with a partner: only they decide the scale
+  if (p.peak)
+    used = is_query ? union_of(p.query_any + b * p.any_step, p.TQ, tile, 0, p.TK)
+                    : union_of(p.key_any + b * p.any_step, p.TK, tile, 0, p.TQ);
+  float top = 0.0f, ltop = 0.0f;
+  const int d = (lane % L) * 8;
+#pragma unroll
+  for (int pass = 0; pass < kTile / (4 * RPW); ++pass) {
+    const int r = (pass * 4 + wave) * RPW + lane / L;
+    const int row = tile * kTile + r;
+    const bool in = row < N;
+    float dot = 0.0f, norm = 0.0f;
+    if (in && d < p.D) {
+      if (is_query) {
+        const T8 g = *reinterpret_cast<const T8*>(static_cast<const T*>(p.go) + b * p.gs[0] + h * p.gs[1] + row * p.gs[2] + d);
+        const T8 o = *reinterpret_cast<const T8*>(static_cast<const T*>(p.out) + b * p.os[0] + h * p.os[1] + row * p.os[2] + d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          dot += float(g[e]) * float(o[e]);
+          norm += float(g[e]) * float(g[e]);
+        }
+        if (p.out_lo) {
+          const T8 lo = *reinterpret_cast<const T8*>(static_cast<const T*>(p.out_lo) + (bh * p.Nq + row) * p.D + d);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) dot += float(g[e]) * float(lo[e]);
+        }
+      } else {
+        const T8 v = *reinterpret_cast<const T8*>(static_cast<const T*>(p.v) + b * p.vs[0] + h * p.vs[1] + row * p.vs[2] + d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) norm += float(v[e]) * float(v[e]);
+      }
+    }
+#pragma unroll
+    for (int off = L / 2; off >= 1; off >>= 1) {
+      dot += __shfl_xor(dot, off, 64);
+      norm += __shfl_xor(norm, off, 64);
+    }
+    const bool counts = (used >> r) & 1;
+    top = fmaxf(top, counts && norm <= 3.0e38f ? norm : 0.0f);  // (nor do rows that are not finite)
+    if (is_query && lane % L == 0) {
+      const float dl = in && p.dlse ? p.dlse[bh * p.Nq + row] : 0.0f;
+      ltop = fmaxf(ltop, counts && fabsf(dl) <= 3.0e38f ? fabsf(dl) : 0.0f);
+      float* dst = p.rows + (bh * p.TQ + tile) * 3 * kTile + r;
+      const int64_t at = bh * p.Nq + row;
+      const float inv = in ? p.stats[int64_t(p.B) * p.H * p.Nq + at] : 0.0f;
+      dst[0] = in ? p.stats[at] : 0.0f;
+      dst[kTile] = __is_same(T, _Float16) ? inv * kProb : inv;
+      dst[2 * kTile] = in ? dl - dot : 0.0f;
+    }
+  }
+  if (p.peak) {
+    __shared__ float2 s[4];
+    top = wave_max(top);
+    ltop = wave_max(ltop);
+    if (lane == 0) s[wave] = make_float2(top, ltop);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const float a = fmaxf(fmaxf(s[0].x, s[1].x), fmaxf(s[2].x, s[3].x));
+      const float c = fmaxf(fmaxf(s[0].y, s[1].y), fmaxf(s[2].y, s[3].y));
+      p.peak[id] = make_float4(a, c, 0.0f, 0.0f);
+    }
+  }
+}
+
+// fp16: the exponent of dS for the heads of a key head, which share dk.
+__device__ __forceinline__ int scale_bits(const BwdParams& p, int64_t b, int kv) {
+  const int lane = threadIdx.x & 63;
+  float gm = 0.0f, vm = 0.0f, lm = 0.0f;
+  const float4* g = p.peak + (b * p.H + int64_t(kv) * p.G) * p.TQ;
+  for (int i = lane; i < p.G * p.TQ; i += 64) {
+    gm = fmaxf(gm, g[i].x);
+    lm = fmaxf(lm, g[i].y);
+  }
+  const float4* v = p.peak + int64_t(p.B) * p.H * p.TQ + (b * p.KV + kv) * p.TK;
+  for (int i = lane; i < p.TK; i += 64) vm = fmaxf(vm, v[i].x);
+  const float bound = 2.0f * sqrtf(wave_max(gm)) * sqrtf(wave_max(vm)) + wave_max(lm);
+  return bound > 0.0f && bound < 3.0e38f ? min(60, max(-60, 13 - ilogbf(bound))) : 0;
+}
+
+// -- the products ------------------------------------------------------------------------------------------------
+template <typename T, int DP, int W, bool KEYS, bool SUMS>
+__global__ void __launch_bounds__(64 * W, DP == 128 ? 1 : 2) bucket_bwd_kernel(BwdParams p) {
+  using Op = typename Elem<T>::Operand;
+  constexpr int NK = DP / 16, ND = DP / 32;
+  constexpr int kBytes = kTile * DP * 2;
+  constexpr int kRowFloats = KEYS ? 3 * kTile : 0;
+  constexpr bool kHalf = __is_same(T, _Float16);
+  extern __shared__ __attribute__((aligned(1024))) char smem[];  // X, Y of two tiles, their rows, the tables, the sums
+  float* s_rows = reinterpret_cast<float*>(smem + 4 * kBytes);   // KEYS: [2][3][64]
+  float* s_table = s_rows + 2 * kRowFloats;
+  float* s_bins = s_table + (KEYS ? p.G : 1) * kPitch;           // SUMS: [K + 1][64 W], the last one of masked pairs
+  static_assert(KEYS || !SUMS, "the table's gradient is the keys' kernel's");
+  const int64_t id = xcd_order(blockIdx.x, gridDim.x);
+  if (id >= p.units) return;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // units: the heads of a column tile follow one another (they read the same buckets)
+  const int UH = KEYS ? p.KV : p.H;
+  const int uh = int(id % UH), ct = int(id / UH % p.CT);
+  const int64_t b = id / (int64_t(UH) * p.CT);
+  const int kv = KEYS ? uh : uh / p.G;
+  const int N = KEYS ? p.Nk : p.Nq, rows = KEYS ? p.TQ : p.TK;
+  const int col = ct * 32 * W + wave * 32 + (lane & 31);
+  const bool in = col < N;
+  const int at = in ? col : 0;
+
+  load_tables(s_table, p.table, p.table_dtype, p.K, p.H, KEYS ? kv * p.G : uh, KEYS ? p.G : 1, 64 * W);
+
+  // which columns have a partner, and the tables of the row tiles that have
+  const uint64_t* by_col = (KEYS ? p.key_any : p.query_any) + b * p.any_step;  // rows of it: row tiles
+  const uint64_t* by_row = (KEYS ? p.query_any : p.key_any) + b * p.any_step;  // rows of it: column tiles
+  const int c0 = ct * 32 * W / kTile, col_tiles = KEYS ? p.TK : p.TQ;
+  const bool two = W == 4 && c0 + 1 < col_tiles;
+  uint64_t used = union_of(by_col, col_tiles, c0, 0, rows);
+  if (two) {
+    const uint64_t second = union_of(by_col, col_tiles, c0 + 1, 0, rows);
+    if (wave >= 2) used = second;
+  }
+  const bool mine = in && ((used >> (at & 63)) & 1);
+
+  // columns: (K, V) or (Q, go), zeros where there is no partner
+  Op bx[NK], by[NK];
+  const T* gx = KEYS ? static_cast<const T*>(p.k) + b * p.ks[0] + kv * p.ks[1] + at * p.ks[2]
+                     : static_cast<const T*>(p.q) + b * p.qs[0] + uh * p.qs[1] + at * p.qs[2];
+  const T* gy = KEYS ? static_cast<const T*>(p.v) + b * p.vs[0] + kv * p.vs[1] + at * p.vs[2]
+                     : static_cast<const T*>(p.go) + b * p.gs[0] + uh * p.gs[1] + at * p.gs[2];
+#pragma unroll
+  for (int kk = 0; kk < NK; ++kk) {
+    const int d = 16 * kk + 8 * half;
+    if (mine && d < p.D) {
+      bx[kk] = *reinterpret_cast<const Op*>(gx + d);
+      by[kk] = *reinterpret_cast<const Op*>(gy + d);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) bx[kk][e] = by[kk][e] = T(0.0f);
+    }
+  }
+  float cm = 0.0f, cinv = 0.0f, cdelta = 0.0f;  // the column's row statistics
+  if (!KEYS && mine) {
+    const float* r = p.rows + ((b * p.H + uh) * p.TQ + (at >> 6)) * 3 * kTile + (at & 63);
+    cm = r[0];
+    cinv = r[kTile];
+    cdelta = r[2 * kTile];
+  }
+  float up = 1.0f, down = p.scale;
+  if constexpr (kHalf) {
+    const int e = scale_bits(p, b, kv);
+    up = ldexpf(1.0f, e);
+    down = p.scale * ldexpf(1.0f, -e);
+    if (KEYS) up *= 1.0f / kProb;  // P comes times kProb
+  }
+  const float slog = p.scale * kLog2e;
+  const uint8_t* codes = (KEYS ? p.index_t + b * p.index_t_step + int64_t(at) * p.St
+                               : p.index + b * p.index_step + int64_t(at) * p.S) + 16 * half;
+
+  mf_f32x16 ax[ND], ay[ND];
+#pragma unroll
+  for (int n = 0; n < ND; ++n) ax[n] = ay[n] = zeros16();
+  float total = 0.0f;  // queries: of dS
+
+  const char *tx = nullptr, *ty = nullptr, *tr = nullptr;
+  unsigned xstride = 0, ystride = 0;
+  auto side = [&](int h) {  // the streamed side of query head h
+    if (KEYS) {
+      tx = reinterpret_cast<const char*>(static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[1]);
+      ty = reinterpret_cast<const char*>(static_cast<const T*>(p.go) + b * p.gs[0] + h * p.gs[1]);
+      tr = reinterpret_cast<const char*>(p.rows + (b * p.H + h) * p.TQ * 3 * kTile);
+      xstride = unsigned(p.qs[2]) * 2;
+      ystride = unsigned(p.gs[2]) * 2;
+    } else {
+      tx = reinterpret_cast<const char*>(static_cast<const T*>(p.k) + b * p.ks[0] + kv * p.ks[1]);
+      ty = reinterpret_cast<const char*>(static_cast<const T*>(p.v) + b * p.vs[0] + kv * p.vs[1]);
+      xstride = unsigned(p.ks[2]) * 2;
+      ystride = unsigned(p.vs[2]) * 2;
+    }
+  };
+  auto load = [&](int tile, uint64_t set, char* lx, char* ly, float* lr, uint4 (&w)[2]) {
+    copy_tile<DP, W>(tx + int64_t(tile) * kTile * xstride, xstride, p.D, set, lx, wave, lane);
+    copy_tile<DP, W>(ty + int64_t(tile) * kTile * ystride, ystride, p.D, set, ly, wave, lane);
+    if (KEYS && wave == 0) {
+      const mf_i32x4 src = lds_copy_source(tr + int64_t(tile) * (3 * kTile * 4));
+      const bool on = (set >> lane) & 1;  // zeros for rows without a partner here too
+#pragma unroll
+      for (int n = 0; n < 3; ++n) lds_copy4(src, on ? lane * 4u + n * kTile * 4u : kLdsCopyOutside, lr + n * kTile);
+    }
+    w[0] = *reinterpret_cast<const uint4*>(codes + int64_t(tile) * kTile);
+    w[1] = *reinterpret_cast<const uint4*>(codes + int64_t(tile) * kTile + 32);
+    if (KEYS && !in) w[0] = w[1] = make_uint4(0x40404040u, 0x40404040u, 0x40404040u, 0x40404040u);  // kMasked
+  };
+  auto compute = [&](const char* lx, const char* ly, const float* lr, uint64_t set, const uint4 (&w)[2],
+                     const float* table) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      if (uint32_t(set >> (32 * kb)) == 0) continue;  // no pair in these 32 rows
+      const int row = 32 * kb + block_row(lane & 31);
+      const uint32_t word[4] = {w[kb].x, w[kb].y, w[kb].z, w[kb].w};
+      mf_f32x16 s = zeros16(), d;  // d: dP - delta, -delta as the sum's start
+      const float* lrow = lr + 32 * kb + 16 * half;
+#pragma unroll
+      for (int t = 0; t < 16; ++t) d[t] = KEYS ? lrow[2 * kTile + t] : cdelta;
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) {
+        s = Mma32<T>::mma(row_operand<Op, DP>(lx, row, half, kk), bx[kk], s);
+        d = Mma32<T>::mma(row_operand<Op, DP>(ly, row, half, kk), by[kk], d);
+      }
+      Op pb[2], sb[2];
+#pragma unroll
+      for (int t = 0; t < 16; ++t) {
+        const unsigned code = byte_of(word, t);
+        const float x = fmaf(s[t], slog, table[code]);
+        float e = fast_exp2(x - (KEYS ? lrow[t] : cm));
+        if (KEYS) {
+          e *= lrow[kTile + t];
+          pb[t >> 3][t & 7] = static_cast<T>(e);
+        }
+        const float ds = e * d[t];
+        if (!KEYS) total += ds;
+        sb[t >> 3][t & 7] = static_cast<T>(kHalf ? ds * up : ds);
+        if constexpr (SUMS) unsafeAtomicAdd(s_bins + min(int(code), p.K) * 64 * W + int(threadIdx.x), ds);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int n = 0; n < ND; ++n) {
+          ax[n] = Mma32<T>::mma(column_operand<T, Op, DP>(lx, 32 * kb, u, n, lane), sb[u], ax[n]);
+          if (KEYS) ay[n] = Mma32<T>::mma(column_operand<T, Op, DP>(ly, 32 * kb, u, n, lane), pb[u], ay[n]);
+        }
+    }
+  };
+  auto ready = [] {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's copies into LDS have landed
+    __syncthreads();
+  };
+
+  char *x0 = smem, *y0 = smem + kBytes, *x1 = smem + 2 * kBytes, *y1 = smem + 3 * kBytes;
+  float *r0 = s_rows, *r1 = s_rows + kRowFloats;
+  for (int g = 0; g < (KEYS ? p.G : 1); ++g) {
+    side(KEYS ? kv * p.G + g : uh);
+    const float* table = s_table + (KEYS ? g : 0) * kPitch;
+    Tiles tiles(by_row + int64_t(c0) * rows, two ? by_row + int64_t(c0 + 1) * rows : nullptr, 0, rows);
+    int tile = 0;
+    uint64_t sa = 0, sb = 0;
+    uint4 wa[2], wb[2];
+    if constexpr (SUMS)
+      for (int c = 0; c <= p.K; ++c) s_bins[c * 64 * W + threadIdx.x] = 0.0f;
+    __syncthreads();  // the tables, and the last head's last tile and sums
+    bool more = tiles.next(tile, sa);
+    if (more) load(tile, sa, x0, y0, r0, wa);
+    while (more) {
+      ready();
+      more = tiles.next(tile, sb);
+      if (more) load(tile, sb, x1, y1, r1, wb);
+      compute(x0, y0, r0, sa, wa, table);
+      if (!more) break;
+      ready();
+      more = tiles.next(tile, sa);
+      if (more) load(tile, sa, x0, y0, r0, wa);
+      compute(x1, y1, r1, sb, wb, table);
+    }
+    if constexpr (SUMS) {
+      __syncthreads();
+      for (int c = wave; c < p.K; c += W) {
+        float v = 0.0f;
+#pragma unroll
+        for (int u = 0; u < W; ++u) v += s_bins[c * 64 * W + u * 64 + lane];
+        v = wave_sum(v) * (kHalf ? 1.0f / kProb : 1.0f);
+        if (lane == 0) p.parts[(int64_t(kv * p.G + g) * p.K + c) * (int64_t(p.B) * p.CT) + b * p.CT + ct] = v;
+      }
+      __syncthreads();  // read before the next head clears them
+    }
+  }
+
+  if (in) {
+    T* ox = KEYS ? static_cast<T*>(p.dk) + b * p.dks[0] + kv * p.dks[1] + at * p.dks[2]
+                 : static_cast<T*>(p.dq) + b * p.dqs[0] + uh * p.dqs[1] + at * p.dqs[2];
+    T* oy = static_cast<T*>(p.dv) + b * p.dvs[0] + kv * p.dvs[1] + at * p.dvs[2];
+    const float fx = KEYS ? down : down * (kHalf ? cinv * (1.0f / kProb) : cinv), fy = kHalf ? 1.0f / kProb : 1.0f;
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int d0 = 32 * n + 16 * half + 8 * u;
+        if (d0 >= p.D) continue;
+        Op x, y;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          // a column without a partner: zeros, whatever the tile's other rows hold
+          x[e] = static_cast<T>(mine ? ax[n][8 * u + e] * fx : 0.0f);
+          y[e] = static_cast<T>(mine ? ay[n][8 * u + e] * fy : 0.0f);
+        }
+        *reinterpret_cast<Op*>(ox + d0) = x;
+        if (KEYS) *reinterpret_cast<Op*>(oy + d0) = y;
+      }
+  }
+  if (!KEYS) {
+    total = pair_sum(total);
+    const float inv = kHalf ? cinv * (1.0f / kProb) : cinv;
+    if (mine && half == 0 && inv > 0.0f) {
+      const float left = p.dlse ? p.dlse[(b * p.H + uh) * p.Nq + at] : 0.0f;
+      p.rows[((b * p.H + uh) * p.TQ + (at >> 6)) * 3 * kTile + 2 * kTile + (at & 63)] = cdelta - (total * inv - left);
+    }
+  }
+}
+
+namespace {
+
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+struct BwdPlan {
+  int DP, TQ, TK, WQ, WK, CQ, CK;  // waves and column tiles of the queries' and the keys' kernel
+  size_t rows, peak, parts;
+  size_t total() const { return rows + peak + parts; }
+};
+
+int waves_of(int columns) { return columns <= 32 ? 1 : columns <= 64 ? 2 : 4; }
+
+BwdPlan bwd_plan(const mf_bucket_attn_bwd_args* a) {
+  const mf_bucket_attn_args* f = &a->fwd;
+  BwdPlan z = {};
+  z.DP = f->head_dim <= 32 ? 32 : f->head_dim <= 64 ? 64 : 128;
+  z.TQ = (f->queries + kTile - 1) / kTile;
+  z.TK = (f->keys + kTile - 1) / kTile;
+  z.WQ = waves_of(f->queries);
+  z.WK = waves_of(f->keys);
+  z.CQ = (f->queries + 32 * z.WQ - 1) / (32 * z.WQ);
+  z.CK = (f->keys + 32 * z.WK - 1) / (32 * z.WK);
+  const size_t qt = size_t(f->batch) * f->heads * z.TQ, kt = size_t(f->batch) * f->kv_heads * z.TK;
+  z.rows = round256(qt * 3 * kTile * sizeof(float));
+  z.peak = f->dtype == MF_DTYPE_F16 ? round256((qt + kt) * sizeof(float4)) : 0;
+  z.parts = a->dtable ? round256(size_t(f->heads) * f->buckets * f->batch * z.CK * sizeof(float)) : 0;
+  return z;
+}
+
+template <typename T, int DP, int W, bool KEYS, bool SUMS>
+int launch_bwd(const BwdParams& p, hipStream_t s) {
+  constexpr int kFixed = 4 * kTile * DP * 2 + (KEYS ? 2 * 3 * kTile * 4 : 0);
+  const int lds = kFixed + (KEYS ? p.G : 1) * kPitch * 4 + (SUMS ? (p.K + 1) * 64 * W * 4 : 0);
+  constexpr int kMost = kFixed + (KEYS ? 32 : 1) * kPitch * 4 + (SUMS ? (MF_MAX_BUCKETS + 1) * 64 * W * 4 : 0);
+  static_assert(kMost <= 160 * 1024, "LDS of a workgroup");
+  if (const int status = ensure_dynamic_lds(reinterpret_cast<const void*>(bucket_bwd_kernel<T, DP, W, KEYS, SUMS>), kMost))
+    return status;
+  hipLaunchKernelGGL((bucket_bwd_kernel<T, DP, W, KEYS, SUMS>), dim3(unsigned((p.units + 7) / 8 * 8)), dim3(64 * W), lds,
+                     s, p);
+  MF_HIP_CHECK(hipGetLastError());
+  return MF_OK;
+}
+
+template <typename T, int DP, bool KEYS, bool SUMS>
+int launch_bwd(const BwdParams& p, int W, hipStream_t s) {
+  if (W == 1) return launch_bwd<T, DP, 1, KEYS, SUMS>(p, s);
+  if (W == 2) return launch_bwd<T, DP, 2, KEYS, SUMS>(p, s);
+  return launch_bwd<T, DP, 4, KEYS, SUMS>(p, s);
+}
+
+template <typename T, int DP>
+int launch_all(BwdParams p, const BwdPlan& z, hipStream_t s) {
+  const int64_t blocks = int64_t(p.B) * p.H * z.TQ + (p.peak ? int64_t(p.B) * p.KV * z.TK : 0);
+  hipLaunchKernelGGL((bucket_rows_kernel<T, DP>), dim3(unsigned(blocks)), dim3(kRowThreads), 0, s, p);
+  MF_HIP_CHECK(hipGetLastError());
+  p.CT = z.CQ;
+  p.units = int64_t(p.B) * p.H * z.CQ;
+  if (const int status = launch_bwd<T, DP, false, false>(p, z.WQ, s)) return status;
+  p.CT = z.CK;
+  p.units = int64_t(p.B) * p.KV * z.CK;
+  return p.parts ? launch_bwd<T, DP, true, true>(p, z.WK, s) : launch_bwd<T, DP, true, false>(p, z.WK, s);
+}
+
+template <typename T>
+int launch_all(const BwdParams& p, const BwdPlan& z, hipStream_t s) {
+  if (z.DP == 32) return launch_all<T, 32>(p, z, s);
+  if (z.DP == 64) return launch_all<T, 64>(p, z, s);
+  return launch_all<T, 128>(p, z, s);
+}
+
+}  // namespace
+}  // namespace bucket
+}  // namespace mf
+
+extern "C" uint64_t mf_bucket_attn_bwd_workspace_size(const mf_bucket_attn_bwd_args* a) {
+  if (a == nullptr) return 0;
+  const mf_bucket_attn_args* f = &a->fwd;
+  if (f->batch <= 0 || f->heads <= 0 || f->kv_heads <= 0 || f->queries <= 0 || f->keys <= 0 || f->buckets <= 0) return 0;
+  return mf::bucket::bwd_plan(a).total();
+}
+
+extern "C" int mf_bucket_attn_bwd(const mf_bucket_attn_bwd_args* a, void* stream) {
+  using namespace mf;
+  using namespace mf::bucket;
+  if (a == nullptr) return fail(MF_ERR_INVALID_ARGUMENT, "mf_bucket_attn_bwd: args is NULL");
+  const mf_bucket_attn_args* f = &a->fwd;
+  if (const int status = check_attn(f, "mf_bucket_attn_bwd")) return status;
+  if (!f->stats || !a->index_t || !a->grad_out || !a->dq || !a->dk || !a->dv)
+    return fail(MF_ERR_INVALID_ARGUMENT, "mf_bucket_attn_bwd: stats, index_t, grad_out, dq, dk and dv must be non-NULL");
+  for (const void* ptr : {static_cast<const void*>(a->index_t), a->grad_out, static_cast<const void*>(a->dq),
+                          static_cast<const void*>(a->dk), static_cast<const void*>(a->dv)})
+    if (reinterpret_cast<uintptr_t>(ptr) % 16 != 0)
+      return fail(MF_ERR_INVALID_ARGUMENT, "mf_bucket_attn_bwd: operands and gradients must be 16-byte aligned");
+  for (const int64_t* s : {a->grad_out_stride, a->dq_stride, a->dk_stride, a->dv_stride})
+    for (int n = 0; n < 3; ++n)
+      if (s[n] % 8 != 0 || s[n] < 0)
+        return fail(MF_ERR_INVALID_ARGUMENT, "mf_bucket_attn_bwd: strides must be non-negative multiples of 8");
+  if (a->grad_out_stride[2] >= (1 << 23))
+    return fail(MF_ERR_UNSUPPORTED, "mf_bucket_attn_bwd: token strides must be below 2^23 elements");
+  if (f->batch == 0 || f->heads == 0) return MF_OK;
+  if (f->queries == 0 || f->keys == 0)
+    return fail(MF_ERR_UNSUPPORTED, "mf_bucket_attn_bwd: queries and keys must be positive");
+  const BwdPlan z = bwd_plan(a);
+  const int64_t B = f->batch;
+  const int64_t most = std::max({B * f->heads * z.TQ + B * f->kv_heads * z.TK, B * f->kv_heads * z.CK + 8, B * f->heads * z.CQ + 8});
+  if (most * 256 > 0xffffffffLL)  // threads of a launch
+    return fail(MF_ERR_UNSUPPORTED, "mf_bucket_attn_bwd: batch * heads * tiles too large");
+  if (!a->workspace || a->workspace_bytes < z.total() || reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0)
+    return fail(MF_ERR_INVALID_ARGUMENT, "mf_bucket_attn_bwd: the workspace must be 16-byte aligned and hold "
+                                         "mf_bucket_attn_bwd_workspace_size bytes");
+  BwdParams p = {};
+  p.q = f->q;
+  p.k = f->k;
+  p.v = f->v;
+  p.table = f->table;
+  p.out = f->out;
+  p.out_lo = f->out_lo;
+  p.go = a->grad_out;
+  p.index = f->index;
+  p.index_t = a->index_t;
+  p.key_any = f->key_any;
+  p.query_any = f->query_any;
+  p.stats = f->stats;
+  p.dlse = a->grad_lse;
+  p.dq = a->dq;
+  p.dk = a->dk;
+  p.dv = a->dv;
+  char* ws = static_cast<char*>(a->workspace);
+  p.rows = reinterpret_cast<float*>(ws);
+  p.peak = z.peak ? reinterpret_cast<float4*>(ws + z.rows) : nullptr;
+  p.parts = a->dtable ? reinterpret_cast<float*>(ws + z.rows + z.peak) : nullptr;
+  for (int n = 0; n < 3; ++n) {
+    p.qs[n] = f->q_stride[n];
+    p.ks[n] = f->k_stride[n];
+    p.vs[n] = f->v_stride[n];
+    p.os[n] = f->out_stride[n];
+    p.gs[n] = a->grad_out_stride[n];
+    p.dqs[n] = a->dq_stride[n];
+    p.dks[n] = a->dk_stride[n];
+    p.dvs[n] = a->dv_stride[n];
+  }
+  p.scale = f->scale;
+  p.B = f->batch;
+  p.H = f->heads;
+  p.KV = f->kv_heads;
+  p.G = f->heads / f->kv_heads;
+  p.Nq = f->queries;
+  p.Nk = f->keys;
+  p.D = f->head_dim;
+  p.S = (f->keys + 63) / 64 * 64;
+  p.St = (f->queries + 63) / 64 * 64;
+  p.TQ = z.TQ;
+  p.TK = z.TK;
+  p.K = f->buckets;
+  p.table_dtype = f->table_dtype;
+  p.index_step = f->index_batch == 1 ? 0 : int64_t(p.Nq) * p.S;
+  p.index_t_step = f->index_batch == 1 ? 0 : int64_t(p.Nk) * p.St;
+  p.any_step = f->index_batch == 1 ? 0 : int64_t(p.TQ) * p.TK;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int status = f->dtype == MF_DTYPE_BF16 ? launch_all<__bf16>(p, z, s) : launch_all<_Float16>(p, z, s);
+  if (status != MF_OK || !a->dtable) return status;
+  return launch_table_sum(p.parts, a->dtable, p.H, p.K, p.B * z.CK, p.table_dtype, s);
+}

@@ -1,0 +1,173 @@
+// What the kernels of attention with a bias by buckets share (bucket_attn.hip, bucket_attn_bwd.hip): 64-row tiles of a
+// head in LDS, products of 32 x 32, and the table of the bias.
+//
+// A product has rows (keys or queries, from LDS) and columns (32 a wave, one a lane and its partner 32 lanes on, in
+// registers): C = A B with A = 32 rows x 16, B = 16 x 32 columns a step (MFMA 32x32x16).  Lane l holds column l & 31 and
+// the accumulators' rows 8 (t >> 2) + 4 half + (t & 3), t = 0 .. 15, half = l >> 5.  The rows are taken from LDS in an
+// order in which these are the 16 rows 16 half + t of the block: then a lane's buckets are 16 consecutive bytes, its
+// row statistics 16 consecutive words, and the accumulators 8 s .. 8 s + 7, rounded, are the B operand of step s of the
+// second product, whose A operand (the tile transposed) is read by transposing reads in the same order.  Nothing goes
+// through LDS between the two products.
+#pragma once
+
+#include "mf_common.h"
+
+typedef __attribute__((__vector_size__(16 * sizeof(float)))) float mf_f32x16;
+
+namespace mf {
+namespace bucket {
+
+constexpr int kTile = 64;    // rows of a staged tile, and of a tile of the buckets' tables
+constexpr int kMasked = 64;  // the bucket of a pair that is left out; up to 64 buckets count
+constexpr int kPitch = 65;   // floats between the tables of two heads
+
+template <typename T>
+struct Mma32;
+template <>
+struct Mma32<__bf16> {
+  __device__ static __forceinline__ mf_f32x16 mma(mf_bf16x8 a, mf_bf16x8 b, mf_f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma32<_Float16> {
+  __device__ static __forceinline__ mf_f32x16 mma(mf_f16x8 a, mf_f16x8 b, mf_f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+__device__ __forceinline__ mf_f32x16 zeros16() {
+  mf_f32x16 z;
+#pragma unroll
+  for (int t = 0; t < 16; ++t) z[t] = 0.0f;
+  return z;
+}
+
+// The other half's value, and the larger and the sum of both, of a column's two lanes.
+__device__ __forceinline__ float pair_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pair_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Row of a 32-row block that lane m of an A operand stands for.
+__device__ __forceinline__ int block_row(int m) { return 16 * ((m >> 2) & 1) + 4 * (m >> 3) + (m & 3); }
+
+// Chunk swizzle of a staged row of DP entries (16-byte chunks).  The 16 rows that an access of 16 lanes reads at one
+// chunk (rows 0 - 7 and 16 - 23 of a block, or 8 - 15 and 24 - 31) fall on different banks, and so do the four rows by
+// four chunks of two transposing reads.
+template <int DP>
+__device__ __forceinline__ int swz(int row) {
+  const int b0 = row & 1, b1 = (row >> 1) & 1, b2 = (row >> 2) & 1, b4 = (row >> 4) & 1;
+  if constexpr (DP == 128) return b0 << 2 | b1 << 3 | b2 | b4 << 1;
+  else if constexpr (DP == 64) return b1 << 2 | b2 | b4 << 1;
+  else return b2 | b4 << 1;
+}
+
+// Copies the rows of a 64-row tile (those in `set`; the others and the entries past D become zeros) into LDS.
+// base: the tile's first row; stride: bytes between rows.  W waves take part.
+template <int DP, int W>
+__device__ __forceinline__ void copy_tile(const char* base, unsigned stride, int D, uint64_t set, char* lds, int wave,
+                                          int lane) {
+  constexpr int CPR = DP / 8, kLoads = CPR / W;
+  static_assert(kLoads >= 1, "a wave copies at least one chunk a lane");
+  const mf_i32x4 src = lds_copy_source(base);
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int q = (wave * kLoads + i) * 64 + lane;
+    const int row = q / CPR, chunk = (q % CPR) ^ swz<DP>(row);
+    const bool on = chunk * 8 < D && ((set >> row) & 1);
+    lds_copy16(src, on ? unsigned(row) * stride + unsigned(chunk) * 16 : kLdsCopyOutside,
+               lds + (wave * kLoads + i) * 1024);
+  }
+}
+
+// A operand of a 32-row block: entries 16 kk + 8 half .. + 7 of row block_row(lane & 31).
+template <typename Op, int DP>
+__device__ __forceinline__ Op row_operand(const char* lds, int row, int half, int kk) {
+  return *reinterpret_cast<const Op*>(lds + row * (DP * 2) + (((2 * kk + half) ^ swz<DP>(row)) << 4));
+}
+
+// A operand of the transposed tile: output rows 32 nd .. + 31 (lane m: entry 32 nd + block_row(m)), inputs the rows
+// block + 16 half + 8 s .. + 7.
+template <typename T, typename Op, int DP>
+__device__ __forceinline__ Op column_operand(const char* lds, int block, int s, int nd, int lane) {
+  const int half = lane >> 5, g = (lane >> 4) & 1, e = (lane >> 2) & 3, a = lane & 3;
+  const int row = block + 16 * half + 8 * s + e;
+  const int chunk = 4 * nd + 2 * (a & 1) + g, sub = (a >> 1) * 8;
+  const int lo = row * (DP * 2) + ((chunk ^ swz<DP>(row)) << 4) + sub;
+  const int hi = (row + 4) * (DP * 2) + ((chunk ^ swz<DP>(row + 4)) << 4) + sub;
+  return __builtin_shufflevector(read_tr16(reinterpret_cast<const T*>(lds + lo)),
+                                 read_tr16(reinterpret_cast<const T*>(lds + hi)), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// The tiles of a row of sets from `first` on, below `end`, whose set is not empty, in order, with their sets; 64 tiles'
+// sets at a time in the lanes.  A second row of sets (or null) is joined to the first.
+struct Tiles {
+  const uint64_t* a;
+  const uint64_t* b;
+  int at, end;
+  uint64_t active, sets;
+
+  __device__ __forceinline__ Tiles(const uint64_t* a_, const uint64_t* b_, int first, int end_)
+      : a(a_), b(b_), at(first - 64), end(end_), active(0), sets(0) {}
+
+  __device__ __forceinline__ bool next(int& tile, uint64_t& set) {
+    while (active == 0) {
+      at += 64;
+      if (at >= end) return false;
+      const int t = at + (threadIdx.x & 63);
+      sets = t < end ? a[t] : 0;
+      if (b != nullptr && t < end) sets |= b[t];
+      active = __ballot(sets != 0);
+    }
+    const int l = __builtin_ctzll(active);
+    active &= active - 1;
+    tile = at + l;
+    set = uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(sets)), l))) |
+          uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(sets >> 32)), l))) << 32;
+    return true;
+  }
+};
+
+// Which of the 64 rows of tile `column` have a partner in the tiles first .. end - 1: the union down a column of a table
+// whose rows are `pitch` apart.
+__device__ __forceinline__ uint64_t union_of(const uint64_t* table, int pitch, int column, int first, int end) {
+  uint64_t u = 0;
+  for (int t = first + int(threadIdx.x & 63); t < end; t += 64) u |= table[int64_t(t) * pitch + column];
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) u |= __shfl_xor((unsigned long long)u, off, 64);
+  return u;
+}
+
+// The bias tables of `heads` heads from `first` on, in log2 units: entries past the buckets are -inf, and a finite entry
+// stays finite, so that the lowest value of a type masks as it does in a softmax over it alone.
+__device__ __forceinline__ void load_tables(float* lds, const void* table, int dtype, int buckets, int all_heads,
+                                            int first, int heads, int threads) {
+  for (int n = threadIdx.x; n < heads * kPitch; n += threads) {
+    const int h = n / kPitch, c = n - h * kPitch;
+    float v = -INFINITY;
+    if (c < buckets) {
+      const int64_t at = int64_t(c) * all_heads + first + h;
+      if (dtype == MF_DTYPE_F32) v = static_cast<const float*>(table)[at];
+      else if (dtype == MF_DTYPE_BF16) v = float(static_cast<const __bf16*>(table)[at]);
+      else v = float(static_cast<const _Float16*>(table)[at]);
+      if (fabsf(v) < INFINITY) v = fminf(fmaxf(v * kLog2e, -3.4028234e38f), 3.4028234e38f);
+    }
+    lds[n] = v;
+  }
+}
+
+// Byte t of 16.
+__device__ __forceinline__ unsigned byte_of(const uint32_t (&w)[4], int t) { return (w[t >> 2] >> (8 * (t & 3))) & 255u; }
+
+// Workgroups of a launch in an order in which those that follow one another run on one XCD.  grid: a multiple of 8.
+__device__ __forceinline__ int64_t xcd_order(unsigned block, unsigned grid) {
+  return int64_t(block & 7) * (grid >> 3) + (block >> 3);
+}
+
+}  // namespace bucket
+}  // namespace mf

@@ -1,0 +1,362 @@
+"""mf_bucket_attn and mf_bucket_attn_bwd against the formulas in 64 bits (tests/bucket_reference.py)."""
+
+import math
+
+import pytest
+import torch
+
+from matterformer_amd.bucket_attention import bucket_attention
+from matterformer_amd.pair_buckets import MASKED, index_buckets, offset_buckets, offset_edges
+from tests.bucket_reference import attention, check
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def gen_of(cuda, seed):
+    g = torch.Generator(device=cuda)
+    g.manual_seed(seed)
+    return g
+
+
+def make(cuda, B, H, KV, Nq, Nk, D, dtype, *, K=17, mask="none", table=FP32, seed=0, batch=None):
+    """q, k, v, table, index (uint8), go."""
+    g = gen_of(cuda, seed)
+    rnd = lambda *s: torch.randn(*s, generator=g, device=cuda)
+    q, k, v, go = (rnd(B, h, n, D).to(dtype) for h, n in ((H, Nq), (KV, Nk), (KV, Nk), (H, Nq)))
+    batch = B if batch is None else batch
+    index = torch.randint(0, K, (batch, Nq, Nk), generator=g, device=cuda, dtype=torch.int32)
+    if mask == "holes":  # pairs left out at random, a query and a key without a pair
+        index[torch.rand(index.shape, generator=g, device=cuda) < 0.5] = -1
+        index[0, Nq // 2] = -1
+        index[-1, :, Nk // 3] = -1
+    elif mask == "padding":  # what padding holds reaches nothing
+        for b in range(batch):
+            cut_q, cut_k = max(1, Nq - 7 * b - 3), max(1, Nk - 13 * b - 5)
+            index[b, cut_q:], index[b, :, cut_k:] = -1, -1
+            q[b, :, cut_q:], go[b, :, cut_q:] = math.nan, math.inf
+            k[b, :, cut_k:], v[b, :, cut_k:] = math.nan, -math.inf
+    elif mask == "blocks":  # whole tiles without a pair
+        i, j = (torch.arange(n, device=cuda) // 64 for n in (Nq, Nk))
+        index[:, (i[:, None] + j[None]) % 3 != 0] = -1
+    elif mask == "all":
+        index.fill_(-1)
+    return q, k, v, rnd(K, H).to(table), index, go
+
+
+def run(q, k, v, table, index, go, *, glse=None, scale=None, K=None):
+    buckets = index_buckets(index, table.shape[0])
+    leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v, table)]
+    out, lse = bucket_attention(*leaves, buckets, scale=scale, return_lse=True)
+    ups = (go,) if glse is None else (go, glse)
+    grads = torch.autograd.grad((out,) if glse is None else (out, lse), leaves, ups)
+    return dict(zip(("out", "lse", "dq", "dk", "dv", "dtable"), (out.detach(), lse.detach(), *grads)))
+
+
+SHAPES = [(1, 1, 1, 1, 1, 8), (2, 4, 4, 29, 29, 48), (2, 8, 2, 1, 300, 64), (1, 4, 1, 33, 65, 128), (2, 4, 4, 181, 181, 64),
+          (1, 2, 2, 64, 128, 32), (1, 8, 8, 130, 257, 96), (3, 2, 1, 5, 1000, 40), (1, 12, 4, 100, 700, 128),
+          (1, 2, 2, 257, 64, 24), (5, 3, 3, 19, 19, 64), (1, 1, 1, 500, 3, 16)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("mask", ["none", "holes", "padding", "blocks"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_output_and_gradients(cuda, shape, mask, dtype):
+    B, H, KV, Nq, Nk, D = shape
+    q, k, v, table, index, go = make(cuda, *shape, dtype, mask=mask, seed=sum(shape))
+    r, bound = attention(q, k, v, table, index_buckets(index, table.shape[0]).index, D ** -0.5, go)
+    check(run(q, k, v, table, index, go), r, bound)
+    # without gradients: the same bits
+    plain, lse = bucket_attention(q, k, v, table, index_buckets(index, table.shape[0], gradients=False), return_lse=True)
+    check({"out": plain, "lse": lse}, r, bound)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("shape", [(2, 4, 2, 70, 130, 64), (1, 6, 6, 29, 29, 32)])
+def test_gradient_through_lse(cuda, shape, dtype):
+    q, k, v, table, index, go = make(cuda, *shape, dtype, mask="holes")
+    glse = torch.randn(shape[0], shape[1], shape[3], device=cuda) * 3.0
+    buckets = index_buckets(index, table.shape[0])
+    r, bound = attention(q, k, v, table, buckets.index, shape[-1] ** -0.5, go, glse)
+    check(run(q, k, v, table, index, go, glse=glse), r, bound)
+    # lse alone
+    leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v, table)]
+    _, lse = bucket_attention(*leaves, buckets, return_lse=True)
+    grads = torch.autograd.grad(lse, leaves, glse)
+    r, bound = attention(q, k, v, table, buckets.index, shape[-1] ** -0.5, torch.zeros_like(go), glse)
+    check(dict(zip(("dq", "dk", "dv", "dtable"), grads)), r, bound)
+    assert not grads[2].any()
+
+
+@pytest.mark.parametrize("table_dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("K", [1, 2, 32, 63, 64])
+def test_tables(cuda, K, table_dtype):
+    q, k, v, table, index, go = make(cuda, 2, 4, 2, 100, 70, 64, BF16, K=K, table=table_dtype)
+    r, bound = attention(q, k, v, table, index_buckets(index, K).index, 0.125, go)
+    check(run(q, k, v, table, index, go), r, bound)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1.0, 1e-30])
+def test_scales(cuda, scale):
+    q, k, v, table, index, go = make(cuda, 1, 2, 2, 70, 90, 32, BF16)
+    r, bound = attention(q, k, v, table, index_buckets(index, table.shape[0]).index, scale, go)
+    check(run(q, k, v, table, index, go, scale=scale), r, bound)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("Nq", [1, 40, 200])
+def test_entries_of_minus_infinity(cuda, dtype, Nq):
+    """A bucket whose bias is -inf leaves its pairs out; a row that has no other gives 0, and takes no gradient."""
+    q, k, v, table, index, go = make(cuda, 2, 4, 2, Nq, 150, 64, dtype, K=5)
+    table[2] = -math.inf
+    table[3, 1] = -math.inf
+    index[0, Nq // 2] = 2
+    index[1, 0] = 3
+    buckets = index_buckets(index, 5)
+    r, bound = attention(q, k, v, table, buckets.index, 0.125, go)
+    got = run(q, k, v, table, index, go)
+    check(got, r, bound)
+    assert not got["out"][0, :, Nq // 2].any() and not got["lse"][0, :, Nq // 2].any() and not got["dq"][0, :, Nq // 2].any()
+    assert not got["dtable"][2].any() and got["dtable"][3, 1] == 0
+
+
+@pytest.mark.parametrize("low", [-1e4, -65504.0, -1e9, torch.finfo(BF16).min, torch.finfo(FP32).min])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_finite_mask_values(cuda, low, dtype):
+    """A huge negative bias masks beside others; a row that has nothing else is an average of what its rounding leaves, as a
+    softmax over it alone is: of all keys alike once the value swallows the products."""
+    q, k, v, table, index, go = make(cuda, 1, 2, 2, 40, 100, 64, dtype, K=4)
+    table[1] = low
+    index[0, 5] = 1
+    index[0, 6] = 1
+    index[0, 6, 70:] = -1
+    buckets = index_buckets(index, 4)
+    got = run(q, k, v, table, index, go)
+    assert all(torch.isfinite(t).all() for t in got.values())
+    q2, go2, index2 = q.clone(), go.clone(), index.clone()
+    rest = [i for i in range(40) if i not in (5, 6)]
+    r, bound = attention(q2[:, :, rest].contiguous(), k, v, table.clamp_min(-3e38), index_buckets(index2[:, rest], 4).index, 0.125,
+                         go2[:, :, rest].contiguous())
+    check({n: got[n][:, :, rest] for n in ("out", "dq")}, r, bound)
+    if low < -1e8:
+        # x - m is 0 for every pair of the row but where a step of x is small beside the products: below -2^27 none is
+        for i, keys in ((5, 100), (6, 70)):
+            mean = v[0, :, :keys].double().mean(1)
+            off = (got["out"][0, :, i].double() - mean).abs()
+            assert (off <= (2 * 2.0 ** -9 if dtype == BF16 else 2 * 2.0 ** -12) * v[0].double().abs().amax(1) + 2.0 ** -8 * mean.abs()).all()
+
+
+def test_head_layouts_and_strides(cuda):
+    """Views of projected rows, sliced, transposed, misaligned and broadcast operands give what contiguous ones give, and
+    gradients in the operands' layout."""
+    B, N, H, KV, D = 2, 90, 4, 2, 48
+    g = gen_of(cuda, 4)
+    rows = torch.randn(B, N, (H + 2 * KV) * D, generator=g, device=cuda).to(BF16)
+    table = torch.randn(9, H, generator=g, device=cuda)
+    index = torch.randint(0, 9, (B, N, N), generator=g, device=cuda)
+    buckets = index_buckets(index, 9)
+    go = torch.randn(B, N, H, D, generator=g, device=cuda).to(BF16).transpose(1, 2)
+
+    def heads(r):
+        q, k, v = r.split((H * D, KV * D, KV * D), dim=-1)
+        return [t.view(B, N, -1, D).transpose(1, 2) for t in (q, k, v)]
+
+    leaf = rows.clone().requires_grad_(True)
+    out = bucket_attention(*heads(leaf), table, buckets)
+    (grad,) = torch.autograd.grad(out, leaf, go)
+    assert out.transpose(1, 2).is_contiguous()  # merged without a copy
+    plain = [t.contiguous().requires_grad_(True) for t in heads(rows)]
+    want = bucket_attention(*plain, table, buckets)
+    dq, dk, dv = torch.autograd.grad(want, plain, go.contiguous())
+    assert torch.equal(out, want)
+    assert torch.equal(grad, torch.cat([t.transpose(1, 2).flatten(2) for t in (dq, dk, dv)], dim=-1))
+
+    q, k, v = (t.contiguous() for t in heads(rows))
+    for change in (lambda t: t.transpose(2, 3).contiguous().transpose(2, 3),  # entries apart
+                   lambda t: torch.cat([t, t], dim=2)[:, :, :N],              # a slice
+                   lambda t: torch.cat([t, t], dim=3)[..., 8:8 + D].contiguous().flatten().clone().view_as(t),
+                   lambda t: torch.empty(t.numel() + 1, dtype=t.dtype, device=cuda)[1:].view_as(t).copy_(t)):  # misaligned
+        args = [change(t) for t in (q, k, v)]
+        fixed = [t.contiguous() for t in args]
+        assert torch.equal(bucket_attention(*args, table, buckets), bucket_attention(*fixed, table, buckets))
+    one = q[:1, :1].requires_grad_(True)
+    wide = bucket_attention(one.expand(B, H, N, D), k, v, table, buckets)
+    (summed,) = torch.autograd.grad(wide, one, go)
+    full = one.detach().expand(B, H, N, D).contiguous().requires_grad_(True)
+    (each,) = torch.autograd.grad(bucket_attention(full, k, v, table, buckets), full, go)
+    assert torch.equal(summed, each.sum((0, 1), keepdim=True))
+    # a gradient that is a broadcast view
+    (ones,) = torch.autograd.grad(bucket_attention(full, k, v, table, buckets).sum(), full)
+    (same,) = torch.autograd.grad(bucket_attention(full, k, v, table, buckets), full, torch.ones_like(full))
+    assert torch.equal(ones, same)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_buckets_of_one_entry_serve_a_batch(cuda, dtype):
+    q, k, v, table, index, go = make(cuda, 3, 4, 4, 100, 100, 32, dtype, mask="holes", batch=1)
+    r, bound = attention(q, k, v, table, index_buckets(index, table.shape[0]).index, 32 ** -0.5, go)
+    check(run(q, k, v, table, index, go), r, bound)
+
+
+@pytest.mark.parametrize("B,H,KV,Nq,Nk,D", [(1, 8, 8, 1, 5000, 64), (2, 12, 3, 1, 3001, 128), (1, 32, 1, 1, 700, 64),
+                                            (1, 32, 1, 4, 900, 32), (4, 4, 4, 3, 20000, 32), (1, 2, 1, 64, 4100, 128)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_few_queries_over_long_caches(cuda, B, H, KV, Nq, Nk, D, dtype):
+    """New tokens: positions at the end of caches of different lengths, what lies behind them is anything."""
+    g = gen_of(cuda, Nk)
+    rnd = lambda *s: torch.randn(*s, generator=g, device=cuda).to(dtype)
+    q, k, v = rnd(B, H, Nq, D), rnd(B, KV, Nk, D), rnd(B, KV, Nk, D)
+    length = torch.randint(Nq, Nk + 1, (B, 1), generator=g, device=cuda)
+    length[0] = Nk
+    pad = torch.arange(Nk, device=cuda)[None] >= length
+    k.masked_fill_(pad[:, None, :, None], math.nan)
+    v.masked_fill_(pad[:, None, :, None], math.inf)
+    places = length - Nq + torch.arange(Nq, device=cuda)[None]
+    buckets = offset_buckets(places, torch.arange(Nk, device=cuda), offset_edges(32, 512, causal=True), pad_mask=pad,
+                             causal=True, gradients=False)
+    table = torch.randn(32, H, generator=g, device=cuda)
+    out, lse = bucket_attention(q, k, v, table, buckets, return_lse=True)
+    r, bound = attention(q, k, v, table, buckets.index, D ** -0.5)
+    check({"out": out, "lse": lse}, r, bound)
+    assert torch.equal(out, bucket_attention(q, k, v, table, buckets))
+
+
+def test_small_weights_beside_a_large_one(cuda):
+    """fp16: 131072 keys of weight 2^-25 beside one of weight 1 are 0.4 % of the row, not nothing."""
+    Nk = 131073
+    q = torch.ones(1, 1, 1, 8, device=cuda, dtype=FP16)
+    k, v = torch.zeros(1, 1, Nk, 8, device=cuda, dtype=FP16), torch.ones(1, 1, Nk, 8, device=cuda, dtype=FP16)
+    v[:, :, 0] = 0
+    index = torch.ones(1, 1, Nk, dtype=torch.int32, device=cuda)
+    index[..., 0] = 0
+    table = torch.tensor([[25.0 * math.log(2.0)], [0.0]], device=cuda)
+    out = bucket_attention(q, k, v, table, index_buckets(index, 2, gradients=False))
+    want = 131072 * 2.0 ** -25 / (1 + 131072 * 2.0 ** -25)
+    assert (out.double() - want).abs().max() <= want * (2.0 ** -11 * 2 + 2.0 ** -15)
+
+
+def test_caches_past_2_31_elements(cuda):
+    """k and v of 2.2e9 elements each, the last request's rows past 2^31."""
+    B, KV, Nk, D = 17, 8, 131072, 128
+    k = torch.empty(B, KV, Nk, D, device=cuda, dtype=BF16)
+    v = torch.empty_like(k)
+    g = gen_of(cuda, 9)
+    for b in (0, B - 1):
+        k[b] = torch.randn(KV, Nk, D, generator=g, device=cuda).to(BF16)
+        v[b] = torch.randn(KV, Nk, D, generator=g, device=cuda).to(BF16)
+    k[1:-1], v[1:-1] = 0, 0
+    q = torch.randn(B, KV, 1, D, generator=g, device=cuda).to(BF16)
+    places = torch.arange(Nk, device=cuda)
+    buckets = offset_buckets(places[-1:], places, offset_edges(16, 1000, causal=True), causal=True, gradients=False)
+    table = torch.randn(16, KV, generator=g, device=cuda)
+    out = bucket_attention(q, k, v, table, buckets)
+    assert k.numel() > 2 ** 31
+    for b in (0, B - 1):
+        r, bound = attention(q[b:b + 1], k[b:b + 1], v[b:b + 1], table, buckets.index, D ** -0.5)
+        check({"out": out[b:b + 1]}, r, bound)
+
+
+def test_two_calls_give_identical_bits(cuda):
+    q, k, v, table, index, go = make(cuda, 3, 8, 2, 200, 333, 64, FP16, mask="holes")
+    a, b = run(q, k, v, table, index, go), run(q, k, v, table, index, go)
+    assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+def test_empty_calls(cuda):
+    for B, H, Nq, Nk in ((0, 2, 5, 5), (2, 0, 5, 5), (2, 2, 0, 5), (2, 2, 5, 0)):
+        q = torch.randn(B, H, Nq, 32, device=cuda, dtype=BF16, requires_grad=True)
+        k, v = (torch.randn(B, H, Nk, 32, device=cuda, dtype=BF16, requires_grad=True) for _ in range(2))
+        table = torch.randn(4, H, device=cuda, requires_grad=True)
+        out, lse = bucket_attention(q, k, v, table, index_buckets(torch.zeros(B, Nq, Nk, dtype=torch.int32, device=cuda), 4),
+                                    return_lse=True)
+        assert out.shape == q.shape and not out.any() and lse.shape == q.shape[:3] and not lse.any()
+        grads = torch.autograd.grad(out, (q, k, v, table), torch.ones_like(out))
+        assert all(g.shape == t.shape and not g.any() for g, t in zip(grads, (q, k, v, table)))
+
+
+def test_nobody_pairs(cuda):
+    q, k, v, table, index, go = make(cuda, 2, 4, 2, 70, 90, 64, BF16, mask="all")
+    q[:], k[:], v[:], go[:] = math.nan, math.inf, math.nan, math.nan
+    assert all(not t.any() for t in run(q, k, v, table, index, go).values())
+
+
+def test_differences(cuda):
+    """The gradients against differences of the kernel's own output: the loss is summed in 64 bits, and steps in which the
+    output's rounding is small are taken along the gradient."""
+    q, k, v, table, index, go = make(cuda, 1, 2, 1, 64, 64, 32, FP16, K=8)
+    got = run(q, k, v, table, index, go)
+    buckets = index_buckets(index, 8)
+    loss = lambda *a: (bucket_attention(*a, buckets).double() * go.double()).sum().item()
+    for n, name in ((3, "dtable"),):
+        args = [q, k, v, table]
+        direction = got[name].double()
+        h = 0.05 / direction.abs().max().item()
+        up, down = ((table.double() + s * h * direction).float() for s in (1, -1))
+        slope = (loss(q, k, v, up) - loss(q, k, v, down)) / (2 * h)
+        want = direction.square().sum().item()
+        # a rounding of every output entry, random in sign: 2^-12 of |out| <= 4 by |go| <= 4 over sqrt(entries), by 2 h
+        noise = 2.0 ** -12 * (go.double().square().sum().sqrt().item()) * 4 / h
+        assert abs(slope - want) <= 0.02 * want + noise
+
+
+def test_refused_calls(cuda):
+    b = index_buckets(torch.zeros(2, 3, 5, dtype=torch.int32, device=cuda), 4)
+    q, k, table = (torch.zeros(*s, device=cuda) for s in ((2, 4, 3, 8), (2, 2, 5, 8), (4, 4)))
+    h = lambda t: t.to(BF16)
+    for args, match in (((q, k, k, table, b), "float16/bfloat16"), ((h(q), h(k), h(k).half(), table, b), "one dtype"),
+                        ((h(q), h(k), h(k), table.double(), b), "table"), ((h(q).cpu(), h(k), h(k), table, b), "same device"),
+                        ((h(q)[..., :4], h(k)[..., :4], h(k)[..., :4], table, b), "multiples of 8"),
+                        ((h(q).repeat(1, 17, 1, 1), h(k), h(k), table.repeat(1, 17), b), "up to 32 heads")):
+        with pytest.raises(RuntimeError, match=match):
+            bucket_attention(*args)
+    wide = torch.zeros(2, 4, 3, 136, device=cuda, dtype=BF16)
+    with pytest.raises(RuntimeError, match="multiples of 8"):
+        bucket_attention(wide, wide[:, :2, :1].expand(2, 2, 5, 136), wide[:, :2, :1].expand(2, 2, 5, 136), table, b)
+    once = index_buckets(torch.zeros(2, 3, 5, dtype=torch.int32, device=cuda), 4, gradients=False)
+    with pytest.raises(ValueError, match="gradients=True"):
+        bucket_attention(h(q).requires_grad_(True), h(k), h(k), table, once)
+
+
+def test_another_stream(cuda):
+    q, k, v, table, index, go = make(cuda, 2, 8, 8, 300, 300, 64, BF16, mask="holes")
+    want = run(q, k, v, table, index, go)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got.append(run(q, k, v, table, index, go))
+    torch.cuda.synchronize()
+    assert all(torch.equal(want[n], g[n]) for g in got for n in want)
+
+
+@pytest.mark.parametrize("shape", [(2, 4, 2, 100, 130, 64), (1, 8, 2, 1, 3000, 64)])
+def test_replayed_graph(cuda, shape):
+    q, k, v, table, index, go = make(cuda, *shape, BF16)
+    buckets = index_buckets(index, table.shape[0])
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v, table)]
+
+    def step():
+        out = bucket_attention(*leaves, buckets)
+        return [out.detach(), *torch.autograd.grad(out, leaves, go)]
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    held = []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            held.append(step())
+    for n in range(3):
+        with torch.no_grad():
+            for t in leaves:
+                t.copy_(torch.randn_like(t))
+        want = step()
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for mine in held:
+            assert all(torch.equal(a, b) for a, b in zip(mine, want))

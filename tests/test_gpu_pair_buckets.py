@@ -1,0 +1,222 @@
+"""mf_pair_buckets, mf_bucket_bias and mf_bucket_bias_bwd on the GPU against the torch formulations on the CPU and 64-bit
+sums."""
+
+import math
+
+import pytest
+import torch
+
+from matterformer_amd.pair_buckets import (MASKED, bucket_bias, distance_buckets, index_buckets, offset_buckets, offset_edges,
+                                           value_buckets)
+from tests.bucket_reference import dense, step
+
+pytestmark = pytest.mark.gpu
+
+
+def same(got, want):
+    """The buckets of a GPU call and of the same call on the CPU, and what its tiles say of them."""
+    torch.cuda.synchronize()
+    B, Nq, Nk = want.index.shape
+    assert got.num_buckets == want.num_buckets
+    assert torch.equal(got.index.cpu(), want.index)
+    if want.index_t is not None:
+        assert torch.equal(got.index_t.cpu(), want.index_t)
+    pad_q, pad_k = -Nq % 64, -Nk % 64
+    on = torch.nn.functional.pad(want.index != MASKED, (0, pad_k, 0, pad_q))
+    tiles = on.view(B, (Nq + pad_q) // 64, 64, (Nk + pad_k) // 64, 64)
+    weights = torch.tensor([1 << t if t < 63 else -(1 << 63) for t in range(64)])
+    assert torch.equal(got.key_any.cpu(), (tiles.any(2).long() * weights).sum(-1))
+    assert torch.equal(got.query_any.cpu().transpose(1, 2), (tiles.any(4).long() * weights[:, None]).sum(2))
+    # the bytes behind the last key are masked: a row is read whole
+    for t, n in ((got.index, Nk), (got.index_t, Nq)):
+        if t is not None and t.numel():
+            whole = t.as_strided((*t.shape[:2], t.stride(1)), t.stride())
+            assert whole[:, :, n:].eq(MASKED).all()
+
+
+@pytest.mark.parametrize("B,N", [(1, 1), (3, 19), (2, 64), (2, 65), (5, 181), (1, 700)])
+@pytest.mark.parametrize("edges,cutoff", [([], None), ([0.0, 1.0], None), ([0.3 * i for i in range(1, 64)], 9.0)])
+def test_distance_buckets(cuda, B, N, edges, cutoff):
+    g = torch.Generator().manual_seed(N)
+    coords = torch.randn(B, N, 3, generator=g) * 4.0
+    pad = torch.arange(N)[None] >= torch.randint(1, N + 1, (B, 1), generator=g)
+    for mask in (None, pad):
+        same(distance_buckets(coords.to(cuda), edges, pad_mask=None if mask is None else mask.to(cuda), cutoff=cutoff),
+             distance_buckets(coords, edges, pad_mask=mask, cutoff=cutoff))
+
+
+def test_distances_at_and_beside_edges(cuda):
+    """Points on a lattice of eighths and a step of fp32 beside it: many distances equal an edge or miss it by a step."""
+    g = torch.Generator().manual_seed(1)
+    coords = torch.randint(-16, 17, (2, 150, 3), generator=g) / 8.0
+    up = torch.nextafter(coords, torch.full_like(coords, math.inf))
+    coords = torch.where(torch.rand(coords.shape, generator=g) < 0.2, up, coords)
+    edges = [i / 8.0 for i in range(1, 40)]
+    same(distance_buckets(coords.to(cuda), edges, cutoff=4.5), distance_buckets(coords, edges, cutoff=4.5))
+    # exact: the squares' sums in whole numbers of 2^-46
+    d = (coords[0, :, None].double() - coords[0, None].double()) * 2.0 ** 25
+    ok = 0
+    got = distance_buckets(coords.to(cuda), edges).index[0].cpu()
+    for i in range(0, 150, 13):
+        for j in range(0, 150, 7):
+            square = sum(int(x) ** 2 for x in d[i, j].tolist())
+            ok += int(got[i, j]) == sum(square >= (e * 2 ** 22) ** 2 for e in range(1, 40))
+    assert ok == len(range(0, 150, 13)) * len(range(0, 150, 7))
+
+
+def test_coordinates_that_are_not_finite_or_large(cuda):
+    coords = torch.tensor([[[0.0, 0, 0], [math.nan, 0, 0], [math.inf, 0, 0], [-math.inf, 0, 0], [3e38, 3e38, 0], [-3e38, 0, 0]]])
+    edges = [1.0, 1e30, 3e38]
+    same(distance_buckets(coords.to(cuda), edges), distance_buckets(coords, edges))
+
+
+@pytest.mark.parametrize("Nq,Nk", [(1, 1), (1, 500), (70, 3), (130, 257), (64, 64)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_offset_buckets(cuda, Nq, Nk, causal):
+    g = torch.Generator().manual_seed(Nq + Nk)
+    qp, kp = (torch.randint(-50, 2000, (3, n), generator=g) for n in (Nq, Nk))
+    qpad, kpad = (torch.rand(3, n, generator=g) < 0.2 for n in (Nq, Nk))
+    edges = offset_edges(33, 700)
+    for q, k, gradients in ((qp, kp, True), (qp[0], kp, False), (qp.int(), kp[:1], True), (qp[0], kp[0], True)):
+        masks = dict(pad_mask=kpad, query_pad_mask=qpad) if max(q.ndim, k.ndim) > 1 and k.shape[0] != 1 or q.ndim > 1 else {}
+        on = {n: m.to(cuda) for n, m in masks.items()}
+        same(offset_buckets(q.to(cuda), k.to(cuda), edges, causal=causal, gradients=gradients, **on),
+             offset_buckets(q, k, edges, causal=causal, gradients=gradients, **masks))
+    # a strided row of positions
+    same(offset_buckets(qp.to(cuda).t().contiguous().t(), kp.to(cuda), edges, causal=causal),
+         offset_buckets(qp, kp, edges, causal=causal))
+
+
+def test_far_positions(cuda):
+    p = torch.tensor([0, 1, 2 ** 31, 2 ** 31 + 1, 2 ** 53, 2 ** 53 + 1, 2 ** 61])
+    edges = [-(2 ** 53), -1, 0, 1, 2, 2 ** 31, 2 ** 53]
+    same(offset_buckets(p.to(cuda), p.to(cuda), edges), offset_buckets(p, p, edges))
+
+
+@pytest.mark.parametrize("B,Nq,Nk", [(1, 1, 1), (2, 33, 130), (3, 181, 181), (1, 64, 128)])
+def test_value_and_index_buckets(cuda, B, Nq, Nk):
+    g = torch.Generator().manual_seed(B * Nq)
+    values = torch.randn(B, Nq, Nk, generator=g) * 3.0
+    values[0, 0, 0] = math.nan
+    pad = torch.rand(B, Nk, generator=g) < 0.3
+    edges = sorted(set(values.flatten()[:40].tolist()) - {math.nan})[:39]
+    edges = [e for e in edges if e == e]
+    for gradients in (True, False):
+        same(value_buckets(values.to(cuda), edges, pad_mask=pad.to(cuda), cutoff=4.0, gradients=gradients),
+             value_buckets(values, edges, pad_mask=pad, cutoff=4.0, gradients=gradients))
+    index = torch.randint(-3, 70, (B, Nq, Nk), generator=g)
+    index[0, 0, 0] = 2 ** 32 + 1
+    for t in (index, index.int(), index.clamp_min(0).to(torch.uint8)):
+        same(index_buckets(t.to(cuda), 30, query_pad_mask=torch.zeros(B, Nq, dtype=torch.int64, device=cuda)), index_buckets(t, 30))
+
+
+def test_empty_calls(cuda):
+    for B, N in ((0, 5), (2, 0)):
+        b = distance_buckets(torch.zeros(B, N, 3, device=cuda), [1.0])
+        assert b.index.shape == (B, N, N)
+        table = torch.zeros(2, 3, device=cuda, requires_grad=True)
+        bias = bucket_bias(table, b)
+        assert bias.shape == (B, 3, N, N)
+        bias.sum().backward()
+        assert not table.grad.any()
+
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,H,Nq,Nk,K", [(1, 1, 1, 1, 1), (2, 8, 29, 29, 32), (3, 5, 64, 181, 64), (2, 12, 130, 257, 17),
+                                         (1, 3, 1, 1000, 8), (1, 128, 7, 15, 5)])
+def test_bias_and_its_gradient(cuda, B, H, Nq, Nk, K, dtype):
+    g = torch.Generator(device=cuda).manual_seed(H * Nk)
+    index = torch.randint(-1, K, (B, Nq, Nk), generator=g, device=cuda, dtype=torch.int32)
+    buckets = index_buckets(index, K)
+    for table_dtype in (dtype, torch.float32):
+        table = torch.randn(K, H, generator=g, device=cuda).to(table_dtype).requires_grad_(True)
+        bias = bucket_bias(table, buckets, dtype=dtype)
+        want = dense(buckets.index, table.detach())
+        assert bias.dtype == dtype and torch.equal(bias.double(), want.to(dtype).double())
+        go = torch.randn(bias.shape, generator=g, device=cuda).to(dtype)
+        go[0, :, :, 0] *= 1000.0
+        go[(index < 0)[:, None].expand_as(go)] = math.nan  # pairs that are left out count for nothing
+        (grad,) = torch.autograd.grad(bias, table, go)
+        masked = torch.where((index >= 0)[:, None], go.double(), 0.0)
+        for c in range(K):
+            terms = torch.where((index == c)[:, None], masked, 0.0)
+            exact, spread = terms.sum((0, 2, 3)), terms.abs().sum((0, 2, 3))
+            # fp32 sums of at most 4096 terms a lane and of 256 lanes: a step each, on partial sums below the spread
+            off = (grad[c].double() - exact).abs()
+            assert (off <= spread * 4096 * 2.0 ** -24 + step(table_dtype) * exact.abs()).all()
+        (again,) = torch.autograd.grad(bucket_bias(table, buckets, dtype=dtype), table, go)
+        assert torch.equal(grad, again)
+
+
+def test_bias_of_a_shared_batch(cuda):
+    index = torch.randint(0, 6, (1, 40, 40), device=cuda)
+    buckets = index_buckets(index, 6)
+    table = torch.randn(6, 4, device=cuda, requires_grad=True)
+    bias = bucket_bias(table, buckets, batch=3)
+    assert torch.equal(bias, dense(buckets.index, table.detach()).float().expand(3, 4, 40, 40))
+    go = torch.randn_like(bias)
+    (grad,) = torch.autograd.grad(bias, table, go)
+    for c in range(6):
+        assert torch.allclose(grad[c].double(), torch.where((index == c)[:, None], go.double(), 0.0).sum((0, 2, 3)), atol=1e-3)
+    # an upstream gradient that is itself a broadcast view
+    (ones,) = torch.autograd.grad(bucket_bias(table, buckets, batch=3).sum(), table)
+    assert torch.equal(ones, torch.stack([(index == c).sum().float().expand(4) * 3 for c in range(6)]))
+
+
+def test_bias_of_more_than_2_31_entries(cuda):
+    """(the index of one atom pair row is shared; 2.2e9 entries of bias)"""
+    N, H = 4700, 100
+    index = torch.randint(0, 8, (1, N, N), device=cuda, dtype=torch.int32)
+    buckets = index_buckets(index, 8)
+    table = torch.randn(8, H, device=cuda).bfloat16()
+    bias = bucket_bias(table, buckets)
+    assert bias.numel() > 2 ** 31
+    for h, i in ((0, 0), (H - 1, N - 1), (H - 3, 17)):
+        assert torch.equal(bias[0, h, i], table[:, h][index[0, i].long()])
+
+
+def test_tables_with_infinities_and_lowest_values(cuda):
+    index = torch.randint(0, 4, (1, 9, 30), device=cuda)
+    for dtype in DTYPES:
+        table = torch.tensor([[0.0], [-math.inf], [torch.finfo(dtype).min], [math.inf]], device=cuda, dtype=dtype)
+        assert torch.equal(bucket_bias(table, index_buckets(index, 4))[0, 0], table[:, 0][index[0]])
+
+
+def test_buckets_and_bias_in_a_graph(cuda):
+    coords = torch.randn(4, 70, 3, device=cuda)
+    table = torch.randn(9, 8, device=cuda)
+    edges = [0.3 * i for i in range(1, 9)]
+
+    def step():
+        b = distance_buckets(coords, edges)
+        return bucket_bias(table, b), b.key_any
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for n in range(4):
+        coords.copy_(torch.randn_like(coords))
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
+def test_two_streams_at_once(cuda):
+    index = [torch.randint(0, 16, (4, 300, 300), device=cuda) for _ in range(2)]
+    table = torch.randn(16, 8, device=cuda, requires_grad=True)
+    go = torch.randn(4, 8, 300, 300, device=cuda)
+    want = [torch.autograd.grad(bucket_bias(table, index_buckets(i, 16)), table, go)[0] for i in index]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in index]
+    got = []
+    for s, i in zip(streams, index):
+        with torch.cuda.stream(s):
+            got.append(torch.autograd.grad(bucket_bias(table, index_buckets(i, 16)), table, go)[0])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
