@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(64 * W, DP == 128 ? 1 : 2) bucket_bwd_kernel(B
         const float ds = e * d[t];
         if (!KEYS) total += ds;
         sb[t >> 3][t & 7] = static_cast<T>(kHalf ? ds * up : ds);
-        if constexpr (SUMS) unsafeAtomicAdd(s_bins + min(int(code), p.K) * 64 * W + int(threadIdx.x), ds);
+        if constexpr (SUMS) s_bins[min(int(code), p.K) * 64 * W + int(threadIdx.x)] += ds;
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u)

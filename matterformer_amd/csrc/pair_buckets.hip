@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kThreads) bucket_bias_bwd_kernel(BiasParams p)
       for (int t = 0; t < 16; ++t) x[t] = t < left ? float(in[t]) : 0.0f;
     }
 #pragma unroll
-    for (int t = 0; t < 16; ++t) unsafeAtomicAdd(s_bins + min(int(byte_of(w, t)), p.K) * kThreads + tid, x[t]);
+    for (int t = 0; t < 16; ++t) s_bins[min(int(byte_of(w, t)), p.K) * kThreads + tid] += x[t];
   }
   __syncthreads();
   for (int c = tid >> 6; c < p.K; c += kThreads / 64) {
