@@ -109,13 +109,13 @@ __device__ __forceinline__ void store_stats(const FwdParams& p, const Column& c,
   if (p.lse) p.lse[at] = l > 0.0f ? (m + __log2f(l)) * kLn2 : l;
 }
 
-template <typename T, int DP, int W>
-__global__ void __launch_bounds__(64 * W, DP == 128 ? 2 : 3) bucket_attn_kernel(FwdParams p) {
+template <typename T, int DP, int W, bool PACKED>
+__global__ void __launch_bounds__(64 * W, DP == 128 ? 2 : 4) bucket_attn_kernel(FwdParams p) {
   using Op = typename Elem<T>::Operand;
   constexpr int NK = DP / 16, ND = DP / 32;
   constexpr int kBytes = kTile * DP * 2;
-  extern __shared__ __attribute__((aligned(1024))) char smem[];  // K, V of two tiles, then the tables
-  float* s_table = reinterpret_cast<float*>(smem + 4 * kBytes);
+  __shared__ __attribute__((aligned(1024))) char s_tiles[4 * kBytes];  // K and V of two tiles
+  __shared__ float s_table[(PACKED ? 32 : 1) * kPitch];
   const int64_t id = xcd_order(blockIdx.x, gridDim.x);
   if (id >= p.units * p.splits) return;
   const int64_t unit = id / p.splits;
@@ -126,14 +126,15 @@ __global__ void __launch_bounds__(64 * W, DP == 128 ? 2 : 3) bucket_attn_kernel(
   const int column = ct * 32 * W + wave * 32 + (lane & 31);
   const Column me = column_of(p, unit, column);
   const int64_t b = unit / (int64_t(p.UH) * p.CT);
-  const int kv = p.packed ? uh : uh / p.G;
+  const int kv = PACKED ? uh : uh / p.G;
 
-  load_tables(s_table, p.table, p.table_dtype, p.K, p.H, p.packed ? uh * p.G : uh, p.packed ? p.G : 1, 64 * W);
-  const float* table = s_table + (p.packed ? me.h - uh * p.G : 0) * kPitch;
+  load_tables(s_table, p.table, p.table_dtype, p.K, p.H, PACKED ? uh * p.G : uh, PACKED ? p.G : 1, 64 * W);
+  const float* table = PACKED ? s_table + (me.h - uh * p.G) * kPitch : s_table;
+  const LaneReads<T, DP> reads(lane);
 
   // the query tiles of the unit's columns, and which of the lane's queries have a key among this split's
-  const int qt0 = p.packed ? 0 : (ct * 32 * W) / kTile;
-  const bool two = !p.packed && W == 4 && qt0 + 1 < p.TQ;
+  const int qt0 = PACKED ? 0 : (ct * 32 * W) / kTile;
+  const bool two = !PACKED && W == 4 && qt0 + 1 < p.TQ;
   const int t0 = split * p.tiles_per_split, t1 = min(p.TK, t0 + p.tiles_per_split);
   const uint64_t* any = p.key_any + b * p.any_step + int64_t(qt0) * p.TK;
   uint64_t used = union_of(p.query_any + b * p.any_step, p.TQ, qt0, t0, t1);
@@ -165,21 +166,35 @@ __global__ void __launch_bounds__(64 * W, DP == 128 ? 2 : 3) bucket_attn_kernel(
   for (int n = 0; n < ND; ++n) acc[n] = zeros16();
   float m = -INFINITY, l = 0.0f;
 
-  auto load = [&](int tile, uint64_t set, char* lk, char* lv, uint4 (&w)[2]) {
-    copy_tile<DP, W>(gk + int64_t(tile) * kTile * kstride, kstride, p.D, set, lk, wave, lane);
-    copy_tile<DP, W>(gv + int64_t(tile) * kTile * vstride, vstride, p.D, set, lv, wave, lane);
+  auto load = [&](int tile, uint64_t set, char* to, uint4 (&w)[2]) {
+    copy_tile<DP, W>(gk + int64_t(tile) * kTile * kstride, kstride, p.D, set, to, wave, lane);
+    copy_tile<DP, W>(gv + int64_t(tile) * kTile * vstride, vstride, p.D, set, to + kBytes, wave, lane);
     w[0] = *reinterpret_cast<const uint4*>(codes + int64_t(tile) * kTile);
     w[1] = *reinterpret_cast<const uint4*>(codes + int64_t(tile) * kTile + 32);
   };
-  auto compute = [&](const char* lk, const char* lv, const uint4 (&w)[2]) {
+
+  Tiles tiles(any, two ? any + p.TK : nullptr, t0, t1);
+  int tile = 0, buffer = 0;
+  uint64_t set = 0;
+  uint4 next[2];
+  bool more = tiles.next(tile, set);
+  if (more) load(tile, set, s_tiles, next);
+  while (more) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's copies into LDS have landed
+    __syncthreads();
+    const uint4 w[2] = {next[0], next[1]};
+    const LaneReads<T, DP> at = reads.shifted(buffer);
+    buffer ^= 2 * kBytes;
+    more = tiles.next(tile, set);
+    if (more) load(tile, set, s_tiles + buffer, next);
+
     mf_f32x16 x[2];
     float top = -INFINITY;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       mf_f32x16 s = zeros16();
-      const int row = 32 * kb + block_row(lane & 31);
 #pragma unroll
-      for (int kk = 0; kk < NK; ++kk) s = Mma32<T>::mma(row_operand<Op, DP>(lk, row, half, kk), qb[kk], s);
+      for (int kk = 0; kk < NK; ++kk) s = Mma32<T>::mma(at.rows(s_tiles, kb, kk), qb[kk], s);
       const uint32_t word[4] = {w[kb].x, w[kb].y, w[kb].z, w[kb].w};
 #pragma unroll
       for (int t = 0; t < 16; ++t) {
@@ -209,32 +224,8 @@ __global__ void __launch_bounds__(64 * W, DP == 128 ? 2 : 3) bucket_attn_kernel(
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int n = 0; n < ND; ++n)
-          acc[n] = Mma32<T>::mma(column_operand<T, Op, DP>(lv, 32 * kb, s, n, lane), pb[s], acc[n]);
+        for (int n = 0; n < ND; ++n) acc[n] = Mma32<T>::mma(at.columns(s_tiles + kBytes, kb, s, n), pb[s], acc[n]);
     }
-  };
-  auto ready = [] {
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's copies into LDS have landed
-    __syncthreads();
-  };
-
-  char *k0 = smem, *v0 = smem + kBytes, *k1 = smem + 2 * kBytes, *v1 = smem + 3 * kBytes;
-  Tiles tiles(any, two ? any + p.TK : nullptr, t0, t1);
-  int tile = 0;
-  uint64_t set = 0;
-  uint4 wa[2], wb[2];
-  bool more = tiles.next(tile, set);
-  if (more) load(tile, set, k0, v0, wa);
-  while (more) {
-    ready();
-    more = tiles.next(tile, set);
-    if (more) load(tile, set, k1, v1, wb);
-    compute(k0, v0, wa);
-    if (!more) break;
-    ready();
-    more = tiles.next(tile, set);
-    if (more) load(tile, set, k0, v0, wa);
-    compute(k1, v1, wb);
   }
 
   l = pair_sum(l);
@@ -391,13 +382,10 @@ int check_attn(const mf_bucket_attn_args* a, const char* what) {
   return MF_OK;
 }
 
-template <typename T, int DP, int W>
+template <typename T, int DP, int W, bool PACKED>
 int launch_fwd(const FwdParams& p, hipStream_t s) {
-  const int lds = 4 * kTile * DP * 2 + (p.packed ? p.G : 1) * kPitch * int(sizeof(float));
-  const void* fn = reinterpret_cast<const void*>(bucket_attn_kernel<T, DP, W>);
-  if (const int status = ensure_dynamic_lds(fn, 4 * kTile * DP * 2 + 32 * kPitch * int(sizeof(float)))) return status;
   const int64_t blocks = (p.units * p.splits + 7) / 8 * 8;
-  hipLaunchKernelGGL((bucket_attn_kernel<T, DP, W>), dim3(unsigned(blocks)), dim3(64 * W), lds, s, p);
+  hipLaunchKernelGGL((bucket_attn_kernel<T, DP, W, PACKED>), dim3(unsigned(blocks)), dim3(64 * W), 0, s, p);
   MF_HIP_CHECK(hipGetLastError());
   if (p.splits > 1) {
     const int64_t all = p.units * 32 * W;
@@ -409,9 +397,9 @@ int launch_fwd(const FwdParams& p, hipStream_t s) {
 
 template <typename T, int DP>
 int launch_fwd(const FwdParams& p, int W, hipStream_t s) {
-  if (W == 1) return launch_fwd<T, DP, 1>(p, s);
-  if (W == 2) return launch_fwd<T, DP, 2>(p, s);
-  return launch_fwd<T, DP, 4>(p, s);
+  if (W == 1) return p.packed ? launch_fwd<T, DP, 1, true>(p, s) : launch_fwd<T, DP, 1, false>(p, s);
+  if (W == 2) return p.packed ? launch_fwd<T, DP, 2, true>(p, s) : launch_fwd<T, DP, 2, false>(p, s);
+  return p.packed ? launch_fwd<T, DP, 4, true>(p, s) : launch_fwd<T, DP, 4, false>(p, s);
 }
 
 template <typename T>

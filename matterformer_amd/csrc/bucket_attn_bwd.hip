@@ -179,12 +179,12 @@ __global__ void __launch_bounds__(64 * W, DP == 128 ? 1 : 2) bucket_bwd_kernel(B
   using Op = typename Elem<T>::Operand;
   constexpr int NK = DP / 16, ND = DP / 32;
   constexpr int kBytes = kTile * DP * 2;
-  constexpr int kRowFloats = KEYS ? 3 * kTile : 0;
+  constexpr int kRowFloats = 3 * kTile;
   constexpr bool kHalf = __is_same(T, _Float16);
-  extern __shared__ __attribute__((aligned(1024))) char smem[];  // X, Y of two tiles, their rows, the tables, the sums
-  float* s_rows = reinterpret_cast<float*>(smem + 4 * kBytes);   // KEYS: [2][3][64]
-  float* s_table = s_rows + 2 * kRowFloats;
-  float* s_bins = s_table + (KEYS ? p.G : 1) * kPitch;           // SUMS: [K + 1][64 W], the last one of masked pairs
+  __shared__ __attribute__((aligned(1024))) char s_tiles[4 * kBytes];                  // X and Y of two tiles
+  __shared__ __attribute__((aligned(1024))) float s_rows[KEYS ? 2 * kRowFloats : 1];  // KEYS: m, 1 / l and -delta of them
+  __shared__ float s_table[kPitch];
+  extern __shared__ float s_bins[];  // SUMS: [K + 1][64 W], the last one of masked pairs
   static_assert(KEYS || !SUMS, "the table's gradient is the keys' kernel's");
   const int64_t id = xcd_order(blockIdx.x, gridDim.x);
   if (id >= p.units) return;
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(64 * W, DP == 128 ? 1 : 2) bucket_bwd_kernel(B
   const bool in = col < N;
   const int at = in ? col : 0;
 
-  load_tables(s_table, p.table, p.table_dtype, p.K, p.H, KEYS ? kv * p.G : uh, KEYS ? p.G : 1, 64 * W);
+  const LaneReads<T, DP> reads(lane);
 
   // which columns have a partner, and the tables of the row tiles that have
   const uint64_t* by_col = (KEYS ? p.key_any : p.query_any) + b * p.any_step;  // rows of it: row tiles
@@ -270,12 +270,13 @@ __global__ void __launch_bounds__(64 * W, DP == 128 ? 1 : 2) bucket_bwd_kernel(B
       ystride = unsigned(p.vs[2]) * 2;
     }
   };
-  auto load = [&](int tile, uint64_t set, char* lx, char* ly, float* lr, uint4 (&w)[2]) {
-    copy_tile<DP, W>(tx + int64_t(tile) * kTile * xstride, xstride, p.D, set, lx, wave, lane);
-    copy_tile<DP, W>(ty + int64_t(tile) * kTile * ystride, ystride, p.D, set, ly, wave, lane);
+  auto load = [&](int tile, uint64_t set, int buffer, uint4 (&w)[2]) {
+    copy_tile<DP, W>(tx + int64_t(tile) * kTile * xstride, xstride, p.D, set, s_tiles + buffer, wave, lane);
+    copy_tile<DP, W>(ty + int64_t(tile) * kTile * ystride, ystride, p.D, set, s_tiles + buffer + kBytes, wave, lane);
     if (KEYS && wave == 0) {
-      const mf_i32x4 src = lds_copy_source(tr + int64_t(tile) * (3 * kTile * 4));
+      const mf_i32x4 src = lds_copy_source(tr + int64_t(tile) * (kRowFloats * 4));
       const bool on = (set >> lane) & 1;  // zeros for rows without a partner here too
+      float* lr = s_rows + (buffer ? kRowFloats : 0);
 #pragma unroll
       for (int n = 0; n < 3; ++n) lds_copy4(src, on ? lane * 4u + n * kTile * 4u : kLdsCopyOutside, lr + n * kTile);
     }
@@ -283,78 +284,69 @@ __global__ void __launch_bounds__(64 * W, DP == 128 ? 1 : 2) bucket_bwd_kernel(B
     w[1] = *reinterpret_cast<const uint4*>(codes + int64_t(tile) * kTile + 32);
     if (KEYS && !in) w[0] = w[1] = make_uint4(0x40404040u, 0x40404040u, 0x40404040u, 0x40404040u);  // kMasked
   };
-  auto compute = [&](const char* lx, const char* ly, const float* lr, uint64_t set, const uint4 (&w)[2],
-                     const float* table) {
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      if (uint32_t(set >> (32 * kb)) == 0) continue;  // no pair in these 32 rows
-      const int row = 32 * kb + block_row(lane & 31);
-      const uint32_t word[4] = {w[kb].x, w[kb].y, w[kb].z, w[kb].w};
-      mf_f32x16 s = zeros16(), d;  // d: dP - delta, -delta as the sum's start
-      const float* lrow = lr + 32 * kb + 16 * half;
-#pragma unroll
-      for (int t = 0; t < 16; ++t) d[t] = KEYS ? lrow[2 * kTile + t] : cdelta;
-#pragma unroll
-      for (int kk = 0; kk < NK; ++kk) {
-        s = Mma32<T>::mma(row_operand<Op, DP>(lx, row, half, kk), bx[kk], s);
-        d = Mma32<T>::mma(row_operand<Op, DP>(ly, row, half, kk), by[kk], d);
-      }
-      Op pb[2], sb[2];
-#pragma unroll
-      for (int t = 0; t < 16; ++t) {
-        const unsigned code = byte_of(word, t);
-        const float x = fmaf(s[t], slog, table[code]);
-        float e = fast_exp2(x - (KEYS ? lrow[t] : cm));
-        if (KEYS) {
-          e *= lrow[kTile + t];
-          pb[t >> 3][t & 7] = static_cast<T>(e);
-        }
-        const float ds = e * d[t];
-        if (!KEYS) total += ds;
-        sb[t >> 3][t & 7] = static_cast<T>(kHalf ? ds * up : ds);
-        if constexpr (SUMS) s_bins[min(int(code), p.K) * 64 * W + int(threadIdx.x)] += ds;
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int n = 0; n < ND; ++n) {
-          ax[n] = Mma32<T>::mma(column_operand<T, Op, DP>(lx, 32 * kb, u, n, lane), sb[u], ax[n]);
-          if (KEYS) ay[n] = Mma32<T>::mma(column_operand<T, Op, DP>(ly, 32 * kb, u, n, lane), pb[u], ay[n]);
-        }
-    }
-  };
-  auto ready = [] {
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's copies into LDS have landed
-    __syncthreads();
-  };
 
-  char *x0 = smem, *y0 = smem + kBytes, *x1 = smem + 2 * kBytes, *y1 = smem + 3 * kBytes;
-  float *r0 = s_rows, *r1 = s_rows + kRowFloats;
   for (int g = 0; g < (KEYS ? p.G : 1); ++g) {
     side(KEYS ? kv * p.G + g : uh);
-    const float* table = s_table + (KEYS ? g : 0) * kPitch;
-    Tiles tiles(by_row + int64_t(c0) * rows, two ? by_row + int64_t(c0 + 1) * rows : nullptr, 0, rows);
-    int tile = 0;
-    uint64_t sa = 0, sb = 0;
-    uint4 wa[2], wb[2];
+    load_tables(s_table, p.table, p.table_dtype, p.K, p.H, KEYS ? kv * p.G + g : uh, 1, 64 * W);
     if constexpr (SUMS)
       for (int c = 0; c <= p.K; ++c) s_bins[c * 64 * W + threadIdx.x] = 0.0f;
-    __syncthreads();  // the tables, and the last head's last tile and sums
-    bool more = tiles.next(tile, sa);
-    if (more) load(tile, sa, x0, y0, r0, wa);
+    Tiles tiles(by_row + int64_t(c0) * rows, two ? by_row + int64_t(c0 + 1) * rows : nullptr, 0, rows);
+    int tile = 0, buffer = 0;
+    uint64_t set = 0;
+    uint4 next[2];
+    bool more = tiles.next(tile, set);
+    if (more) load(tile, set, 0, next);
+    __syncthreads();  // the table and the sums
     while (more) {
-      ready();
-      more = tiles.next(tile, sb);
-      if (more) load(tile, sb, x1, y1, r1, wb);
-      compute(x0, y0, r0, sa, wa, table);
-      if (!more) break;
-      ready();
-      more = tiles.next(tile, sa);
-      if (more) load(tile, sa, x0, y0, r0, wa);
-      compute(x1, y1, r1, sb, wb, table);
-    }
-    if constexpr (SUMS) {
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's copies into LDS have landed
       __syncthreads();
+      const uint4 w[2] = {next[0], next[1]};
+      const uint64_t now = set;
+      const LaneReads<T, DP> at = reads.shifted(buffer);
+      const float* lr = s_rows + (buffer ? kRowFloats : 0) + 16 * half;
+      buffer ^= 2 * kBytes;
+      more = tiles.next(tile, set);
+      if (more) load(tile, set, buffer, next);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        if (uint32_t(now >> (32 * kb)) == 0) continue;  // no pair in these 32 rows
+        const uint32_t word[4] = {w[kb].x, w[kb].y, w[kb].z, w[kb].w};
+        mf_f32x16 s = zeros16(), d;  // d: dP - delta, -delta as the sum's start
+#pragma unroll
+        for (int t = 0; t < 16; ++t) d[t] = KEYS ? lr[2 * kTile + 32 * kb + t] : cdelta;
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+          s = Mma32<T>::mma(at.rows(s_tiles, kb, kk), bx[kk], s);
+          d = Mma32<T>::mma(at.rows(s_tiles + kBytes, kb, kk), by[kk], d);
+        }
+        Op pb[2], sb[2];
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+          const float x = fmaf(s[t], slog, s_table[byte_of(word, t)]);
+          float e = fast_exp2(x - (KEYS ? lr[32 * kb + t] : cm));
+          if (KEYS) {
+            e *= lr[kTile + 32 * kb + t];
+            pb[t >> 3][t & 7] = static_cast<T>(e);
+          }
+          d[t] *= e;
+          sb[t >> 3][t & 7] = static_cast<T>(kHalf ? d[t] * up : d[t]);
+          if (!KEYS) total += d[t];
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int n = 0; n < ND; ++n) {
+            ax[n] = Mma32<T>::mma(at.columns(s_tiles, kb, u, n), sb[u], ax[n]);
+            if (KEYS) ay[n] = Mma32<T>::mma(at.columns(s_tiles + kBytes, kb, u, n), pb[u], ay[n]);
+          }
+        if constexpr (SUMS) {
+#pragma unroll
+          for (int t = 0; t < 16; ++t) s_bins[min(int(byte_of(word, t)), p.K) * 64 * W + int(threadIdx.x)] += d[t];
+        }
+      }
+    }
+    __syncthreads();
+    if constexpr (SUMS) {
       for (int c = wave; c < p.K; c += W) {
         float v = 0.0f;
 #pragma unroll
@@ -362,7 +354,7 @@ __global__ void __launch_bounds__(64 * W, DP == 128 ? 1 : 2) bucket_bwd_kernel(B
         v = wave_sum(v) * (kHalf ? 1.0f / kProb : 1.0f);
         if (lane == 0) p.parts[(int64_t(kv * p.G + g) * p.K + c) * (int64_t(p.B) * p.CT) + b * p.CT + ct] = v;
       }
-      __syncthreads();  // read before the next head clears them
+      __syncthreads();  // the next head clears them
     }
   }
 
@@ -429,10 +421,9 @@ BwdPlan bwd_plan(const mf_bucket_attn_bwd_args* a) {
 
 template <typename T, int DP, int W, bool KEYS, bool SUMS>
 int launch_bwd(const BwdParams& p, hipStream_t s) {
-  constexpr int kFixed = 4 * kTile * DP * 2 + (KEYS ? 2 * 3 * kTile * 4 : 0);
-  const int lds = kFixed + (KEYS ? p.G : 1) * kPitch * 4 + (SUMS ? (p.K + 1) * 64 * W * 4 : 0);
-  constexpr int kMost = kFixed + (KEYS ? 32 : 1) * kPitch * 4 + (SUMS ? (MF_MAX_BUCKETS + 1) * 64 * W * 4 : 0);
-  static_assert(kMost <= 160 * 1024, "LDS of a workgroup");
+  const int lds = SUMS ? (p.K + 1) * 64 * W * 4 : 0;
+  constexpr int kMost = SUMS ? (MF_MAX_BUCKETS + 1) * 64 * W * 4 : 0;
+  static_assert(kMost + 4 * kTile * DP * 2 + 4096 <= 160 * 1024, "LDS of a workgroup");
   if (const int status = ensure_dynamic_lds(reinterpret_cast<const void*>(bucket_bwd_kernel<T, DP, W, KEYS, SUMS>), kMost))
     return status;
   hipLaunchKernelGGL((bucket_bwd_kernel<T, DP, W, KEYS, SUMS>), dim3(unsigned((p.units + 7) / 8 * 8)), dim3(64 * W), lds,

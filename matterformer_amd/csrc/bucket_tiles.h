@@ -85,24 +85,43 @@ __device__ __forceinline__ void copy_tile(const char* base, unsigned stride, int
   }
 }
 
-// A operand of a 32-row block: entries 16 kk + 8 half .. + 7 of row block_row(lane & 31).
-template <typename Op, int DP>
-__device__ __forceinline__ Op row_operand(const char* lds, int row, int half, int kk) {
-  return *reinterpret_cast<const Op*>(lds + row * (DP * 2) + (((2 * kk + half) ^ swz<DP>(row)) << 4));
-}
+// Where a lane reads a staged tile: byte offsets that 32-row blocks and eight-row steps shift by constants (the swizzle
+// takes no part of them).
+template <typename T, int DP>
+struct LaneReads {
+  using Op = typename Elem<T>::Operand;
+  int row;     // A operand: row block_row(lane & 31), chunk half; chunk 2 kk + half lies at row ^ (kk << 5)
+  int lo, hi;  // transposed: rows 16 half + e and 4 further, the lane's four entries; 32 nd entries on at ^ (nd << 6)
 
-// A operand of the transposed tile: output rows 32 nd .. + 31 (lane m: entry 32 nd + block_row(m)), inputs the rows
-// block + 16 half + 8 s .. + 7.
-template <typename T, typename Op, int DP>
-__device__ __forceinline__ Op column_operand(const char* lds, int block, int s, int nd, int lane) {
-  const int half = lane >> 5, g = (lane >> 4) & 1, e = (lane >> 2) & 3, a = lane & 3;
-  const int row = block + 16 * half + 8 * s + e;
-  const int chunk = 4 * nd + 2 * (a & 1) + g, sub = (a >> 1) * 8;
-  const int lo = row * (DP * 2) + ((chunk ^ swz<DP>(row)) << 4) + sub;
-  const int hi = (row + 4) * (DP * 2) + ((chunk ^ swz<DP>(row + 4)) << 4) + sub;
-  return __builtin_shufflevector(read_tr16(reinterpret_cast<const T*>(lds + lo)),
-                                 read_tr16(reinterpret_cast<const T*>(lds + hi)), 0, 1, 2, 3, 4, 5, 6, 7);
-}
+  __device__ __forceinline__ explicit LaneReads(int lane) {
+    const int half = lane >> 5, g = (lane >> 4) & 1, e = (lane >> 2) & 3, a = lane & 3;
+    const int r = block_row(lane & 31);
+    row = r * (DP * 2) + ((half ^ swz<DP>(r)) << 4);
+    const int t = 16 * half + e, chunk = 2 * (a & 1) + g, sub = (a >> 1) * 8;
+    lo = t * (DP * 2) + ((chunk ^ swz<DP>(t)) << 4) + sub;
+    hi = (t + 4) * (DP * 2) + ((chunk ^ swz<DP>(t + 4)) << 4) + sub;
+  }
+  // The same `bytes` further on (a multiple of 256).
+  __device__ __forceinline__ LaneReads shifted(int bytes) const {
+    LaneReads r = *this;
+    r.row += bytes;
+    r.lo += bytes;
+    r.hi += bytes;
+    return r;
+  }
+  // A operand of block kb: entries 16 kk + 8 half .. + 7 of the lane's row.
+  __device__ __forceinline__ Op rows(const char* lds, int kb, int kk) const {
+    return *reinterpret_cast<const Op*>(lds + (row ^ (kk << 5)) + kb * (32 * DP * 2));
+  }
+  // A operand of the transposed tile: output rows 32 nd .. + 31 (lane m: entry 32 nd + block_row(m)), inputs the rows
+  // 32 kb + 16 half + 8 s .. + 7.
+  __device__ __forceinline__ Op columns(const char* lds, int kb, int s, int nd) const {
+    const int at = (32 * kb + 8 * s) * (DP * 2);
+    return __builtin_shufflevector(read_tr16(reinterpret_cast<const T*>(lds + (lo ^ (nd << 6)) + at)),
+                                   read_tr16(reinterpret_cast<const T*>(lds + (hi ^ (nd << 6)) + at)), 0, 1, 2, 3, 4, 5, 6,
+                                   7);
+  }
+};
 
 // The tiles of a row of sets from `first` on, below `end`, whose set is not empty, in order, with their sets; 64 tiles'
 // sets at a time in the lanes.  A second row of sets (or null) is joined to the first.
