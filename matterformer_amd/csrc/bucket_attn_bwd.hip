@@ -332,16 +332,34 @@ __global__ void __launch_bounds__(64 * W, DP == 128 ? 1 : 2) bucket_bwd_kernel(B
           sb[t >> 3][t & 7] = static_cast<T>(kHalf ? d[t] * up : d[t]);
           if (!KEYS) total += d[t];
         }
+        // the second products, and between them the sums by bucket, two of a lane's at a time: where both go to one
+        // bucket the first takes both values and the second adds to the masked pairs' row
+        constexpr int kProducts = 2 * ND * (KEYS ? 2 : 1), kSteps = SUMS ? 8 : 1;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int n = 0; n < ND; ++n) {
-            ax[n] = Mma32<T>::mma(at.columns(s_tiles, kb, u, n), sb[u], ax[n]);
-            if (KEYS) ay[n] = Mma32<T>::mma(at.columns(s_tiles + kBytes, kb, u, n), pb[u], ay[n]);
+        for (int step = 0; step < kSteps; ++step) {
+          float* b0 = nullptr;
+          float* b1 = nullptr;
+          float v0 = 0.0f, v1 = 0.0f, s0 = 0.0f, s1 = 0.0f;
+          if constexpr (SUMS) {
+            const int c0 = min(int(byte_of(word, 2 * step)), p.K), c1 = min(int(byte_of(word, 2 * step + 1)), p.K);
+            const bool same = c0 == c1;
+            b0 = s_bins + c0 * 64 * W + threadIdx.x;
+            b1 = s_bins + (same ? p.K : c1) * 64 * W + threadIdx.x;
+            v0 = same ? d[2 * step] + d[2 * step + 1] : d[2 * step];
+            v1 = d[2 * step + 1];
+            s0 = *b0;
+            s1 = *b1;
           }
-        if constexpr (SUMS) {
 #pragma unroll
-          for (int t = 0; t < 16; ++t) s_bins[min(int(byte_of(word, t)), p.K) * 64 * W + int(threadIdx.x)] += d[t];
+          for (int i = step * kProducts / kSteps; i < (step + 1) * kProducts / kSteps; ++i) {
+            const int n = KEYS ? (i >> 1) % ND : i % ND, u = KEYS ? (i >> 1) / ND : i / ND;
+            if (KEYS && (i & 1)) ay[n] = Mma32<T>::mma(at.columns(s_tiles + kBytes, kb, u, n), pb[u], ay[n]);
+            else ax[n] = Mma32<T>::mma(at.columns(s_tiles, kb, u, n), sb[u], ax[n]);
+          }
+          if constexpr (SUMS) {
+            *b0 = s0 + v0;
+            *b1 = s1 + v1;
+          }
         }
       }
     }
