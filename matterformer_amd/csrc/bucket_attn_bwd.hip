@@ -173,14 +173,78 @@ __device__ __forceinline__ int scale_bits(const BwdParams& p, int64_t b, int kv)
   return bound > 0.0f && bound < 3.0e38f ? min(60, max(-60, 13 - ilogbf(bound))) : 0;
 }
 
+// -- the sums by bucket ------------------------------------------------------------------------------------------
+// A lane's 16 values of a block are added to its sums in LDS while the next block is computed: a pair of values a step,
+// fetched before two or more matrix instructions and put after them, so that nothing waits for LDS.  Where both values
+// of a pair go to one bucket the first takes their sum and the second adds to the masked pairs' row.
+template <bool ON>
+struct BlockSums {
+  __device__ __forceinline__ BlockSums(float*, int, int) {}
+  __device__ __forceinline__ void fetch(int, int) {}
+  __device__ __forceinline__ void put(int, int) {}
+  __device__ __forceinline__ void take(const mf_f32x16&, const uint32_t (&)[4]) {}
+};
+template <>
+struct BlockSums<true> {
+  float* bins;
+  int pitch, K;
+  mf_f32x16 d;
+  uint32_t word[4];
+  float *b0[2], *b1[2];
+  float v0[2], v1[2], s0[2], s1[2];
+  __device__ __forceinline__ BlockSums(float* bins_, int pitch_, int K_) : bins(bins_), pitch(pitch_), K(K_), d(zeros16()) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) word[n] = 0x40404040u;
+  }
+  __device__ __forceinline__ void fetch(int from, int to) {  // at most two steps
+#pragma unroll
+    for (int step = from; step < to; ++step) {
+      const int c0 = min(int(byte_of(word, 2 * step)), K), c1 = min(int(byte_of(word, 2 * step + 1)), K);
+      const bool same = c0 == c1;
+      const int i = step - from;
+      b0[i] = bins + c0 * pitch;
+      b1[i] = bins + (same ? K : c1) * pitch;
+      v0[i] = same ? d[2 * step] + d[2 * step + 1] : d[2 * step];
+      v1[i] = d[2 * step + 1];
+      if (i == 0) {
+        s0[i] = *b0[i];
+        s1[i] = *b1[i];
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __device__ __forceinline__ void put(int from, int to) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int step = from; step < to; ++step) {
+      const int i = step - from;
+      if (i > 0) {  // the first one's may be the same places
+        s0[i] = *b0[i];
+        s1[i] = *b1[i];
+      }
+      *b0[i] = s0[i] + v0[i];
+      *b1[i] = s1[i] + v1[i];
+    }
+  }
+  __device__ __forceinline__ void take(const mf_f32x16& d_, const uint32_t (&w)[4]) {
+    d = d_;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) word[n] = w[n];
+  }
+};
+
 // -- the products ------------------------------------------------------------------------------------------------
 template <typename T, int DP, int W, bool KEYS, bool SUMS>
-__global__ void __launch_bounds__(64 * W, DP == 128 ? 1 : 2) bucket_bwd_kernel(BwdParams p) {
+__global__ void __launch_bounds__(64 * W, DP == 128 && KEYS ? 1 : 2) bucket_bwd_kernel(BwdParams p) {
   using Op = typename Elem<T>::Operand;
   constexpr int NK = DP / 16, ND = DP / 32;
   constexpr int kBytes = kTile * DP * 2;
   constexpr int kRowFloats = 3 * kTile;
   constexpr bool kHalf = __is_same(T, _Float16);
+  // Reads of LDS are asked for a group at a time, ahead of the products or of the exp2s, where the registers allow it: left
+  // to itself the compiler waits for each beside its use (head_dim 128, keys: 319 -> 292 us on four cells of 1997 atoms).
+  // The queries' kernel of head_dim 128 fits two waves a SIMD without (144 us, with it and one wave 168 and more).
+  constexpr bool kAhead = KEYS || DP < 128;
   __shared__ __attribute__((aligned(1024))) char s_tiles[4 * kBytes];                  // X and Y of two tiles
   __shared__ __attribute__((aligned(1024))) float s_rows[KEYS ? 2 * kRowFloats : 1];  // KEYS: m, 1 / l and -delta of them
   __shared__ float s_table[kPitch];
@@ -294,6 +358,7 @@ __global__ void __launch_bounds__(64 * W, DP == 128 ? 1 : 2) bucket_bwd_kernel(B
     int tile = 0, buffer = 0;
     uint64_t set = 0;
     uint4 next[2];
+    BlockSums<SUMS> sums(s_bins + threadIdx.x, 64 * W, p.K);
     bool more = tiles.next(tile, set);
     if (more) load(tile, set, 0, next);
     __syncthreads();  // the table and the sums
@@ -311,56 +376,79 @@ __global__ void __launch_bounds__(64 * W, DP == 128 ? 1 : 2) bucket_bwd_kernel(B
       for (int kb = 0; kb < 2; ++kb) {
         if (uint32_t(now >> (32 * kb)) == 0) continue;  // no pair in these 32 rows
         const uint32_t word[4] = {w[kb].x, w[kb].y, w[kb].z, w[kb].w};
+        Op xa[NK], ya[NK], xt[2][ND], yt[2][ND];
+        float bias[16];
         mf_f32x16 s = zeros16(), d;  // d: dP - delta, -delta as the sum's start
+#pragma unroll
+        for (int kk = 0; kk < (kAhead ? NK : 0); ++kk) {
+          xa[kk] = at.rows(s_tiles, kb, kk);
+          ya[kk] = at.rows(s_tiles + kBytes, kb, kk);
+        }
 #pragma unroll
         for (int t = 0; t < 16; ++t) d[t] = KEYS ? lr[2 * kTile + 32 * kb + t] : cdelta;
 #pragma unroll
+        for (int t = 0; t < (kAhead ? 16 : 0); ++t) bias[t] = s_table[byte_of(word, t)];
+        if constexpr (kAhead) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
         for (int kk = 0; kk < NK; ++kk) {
-          s = Mma32<T>::mma(at.rows(s_tiles, kb, kk), bx[kk], s);
-          d = Mma32<T>::mma(at.rows(s_tiles + kBytes, kb, kk), by[kk], d);
+          sums.fetch(4 * kk / NK, 4 * (kk + 1) / NK);
+          s = Mma32<T>::mma(kAhead ? xa[kk] : at.rows(s_tiles, kb, kk), bx[kk], s);
+          d = Mma32<T>::mma(kAhead ? ya[kk] : at.rows(s_tiles + kBytes, kb, kk), by[kk], d);
+          sums.put(4 * kk / NK, 4 * (kk + 1) / NK);
         }
+        float m[16], inv[16];
+        if (KEYS) {
+#pragma unroll
+          for (int t = 0; t < 16; ++t) {
+            m[t] = lr[32 * kb + t];
+            inv[t] = lr[kTile + 32 * kb + t];
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < (kAhead ? ND : 0); ++n) {
+          xt[0][n] = at.columns(s_tiles, kb, 0, n);
+          if (KEYS) yt[0][n] = at.columns(s_tiles + kBytes, kb, 0, n);
+        }
+        if constexpr (kAhead) __builtin_amdgcn_sched_barrier(0);
         Op pb[2], sb[2];
 #pragma unroll
         for (int t = 0; t < 16; ++t) {
-          const float x = fmaf(s[t], slog, s_table[byte_of(word, t)]);
-          float e = fast_exp2(x - (KEYS ? lr[32 * kb + t] : cm));
+          float e = fast_exp2(fmaf(s[t], slog, kAhead ? bias[t] : s_table[byte_of(word, t)]) - (KEYS ? m[t] : cm));
           if (KEYS) {
-            e *= lr[kTile + 32 * kb + t];
+            e *= inv[t];
             pb[t >> 3][t & 7] = static_cast<T>(e);
           }
           d[t] *= e;
           sb[t >> 3][t & 7] = static_cast<T>(kHalf ? d[t] * up : d[t]);
           if (!KEYS) total += d[t];
         }
-        // the second products, and between them the sums by bucket, two of a lane's at a time: where both go to one
-        // bucket the first takes both values and the second adds to the masked pairs' row
-        constexpr int kProducts = 2 * ND * (KEYS ? 2 : 1), kSteps = SUMS ? 8 : 1;
+        if constexpr (kAhead) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int step = 0; step < kSteps; ++step) {
-          float* b0 = nullptr;
-          float* b1 = nullptr;
-          float v0 = 0.0f, v1 = 0.0f, s0 = 0.0f, s1 = 0.0f;
-          if constexpr (SUMS) {
-            const int c0 = min(int(byte_of(word, 2 * step)), p.K), c1 = min(int(byte_of(word, 2 * step + 1)), p.K);
-            const bool same = c0 == c1;
-            b0 = s_bins + c0 * 64 * W + threadIdx.x;
-            b1 = s_bins + (same ? p.K : c1) * 64 * W + threadIdx.x;
-            v0 = same ? d[2 * step] + d[2 * step + 1] : d[2 * step];
-            v1 = d[2 * step + 1];
-            s0 = *b0;
-            s1 = *b1;
-          }
+        for (int n = 0; n < (kAhead ? ND : 0); ++n) {
+          xt[1][n] = at.columns(s_tiles, kb, 1, n);
+          if (KEYS) yt[1][n] = at.columns(s_tiles + kBytes, kb, 1, n);
+        }
+        if constexpr (kAhead) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int i = step * kProducts / kSteps; i < (step + 1) * kProducts / kSteps; ++i) {
-            const int n = KEYS ? (i >> 1) % ND : i % ND, u = KEYS ? (i >> 1) / ND : i / ND;
-            if (KEYS && (i & 1)) ay[n] = Mma32<T>::mma(at.columns(s_tiles + kBytes, kb, u, n), pb[u], ay[n]);
-            else ax[n] = Mma32<T>::mma(at.columns(s_tiles, kb, u, n), sb[u], ax[n]);
-          }
-          if constexpr (SUMS) {
-            *b0 = s0 + v0;
-            *b1 = s1 + v1;
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+          for (int n = 0; n < ND; ++n) {
+            // two steps a half: one each before and after the middle, or both at once
+            const int step = 4 + 2 * u + (2 * n >= ND && n > 0);
+            if (n == 0 || 2 * n == ND) sums.fetch(step, ND > 1 ? step + 1 : step + 2);
+            ax[n] = Mma32<T>::mma(kAhead ? xt[u][n] : at.columns(s_tiles, kb, u, n), sb[u], ax[n]);
+            if (KEYS) ay[n] = Mma32<T>::mma(kAhead ? yt[u][n] : at.columns(s_tiles + kBytes, kb, u, n), pb[u], ay[n]);
+            if (2 * (n + 1) == ND || n + 1 == ND) sums.put(step, ND > 1 ? step + 1 : step + 2);
           }
         }
+        sums.take(d, word);
+      }
+    }
+    if constexpr (SUMS) {
+#pragma unroll
+      for (int step = 0; step < 8; ++step) {
+        sums.fetch(step, step + 1);
+        sums.put(step, step + 1);
       }
     }
     __syncthreads();
