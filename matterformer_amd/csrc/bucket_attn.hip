@@ -109,8 +109,15 @@ __device__ __forceinline__ void store_stats(const FwdParams& p, const Column& c,
   if (p.lse) p.lse[at] = l > 0.0f ? (m + __log2f(l)) * kLn2 : l;
 }
 
+// Waves a SIMD that the registers are to allow: four (head_dim 128: two), or what LDS has room for.
+constexpr int fwd_waves(int DP, int W, bool packed) {
+  const int lds = 4 * kTile * DP * 2 + (packed ? 32 : 1) * kPitch * 4;
+  const int fit = 160 * 1024 / lds * W / 4, most = DP == 128 ? 2 : 4;
+  return fit < 1 ? 1 : fit < most ? fit : most;
+}
+
 template <typename T, int DP, int W, bool PACKED>
-__global__ void __launch_bounds__(64 * W, DP == 128 ? 2 : 4) bucket_attn_kernel(FwdParams p) {
+__global__ void __launch_bounds__(64 * W, fwd_waves(DP, W, PACKED)) bucket_attn_kernel(FwdParams p) {
   using Op = typename Elem<T>::Operand;
   constexpr int NK = DP / 16, ND = DP / 32;
   constexpr int kBytes = kTile * DP * 2;
@@ -258,33 +265,36 @@ __global__ void __launch_bounds__(64 * W, DP == 128 ? 2 : 4) bucket_attn_kernel(
   if (half == 0) store_stats<T>(p, me, p.units / (int64_t(p.UH) * p.CT), m, l);
 }
 
-// Joins the splits: a wave per column, eight entries a lane.
+// Joins the splits: a workgroup per column, a quarter of the splits a wave (or as many waves as there are splits for),
+// DP / 8 lanes to a split's entries, the others taking the next splits.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) bucket_join_kernel(FwdParams p, int columns, int64_t all) {
-  const int64_t id = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (id >= all) return;
-  const int lane = threadIdx.x & 63;
-  const int64_t unit = id / columns;
-  const int c = int(id - unit * columns), ct = int(unit / p.UH % p.CT);
+__global__ void __launch_bounds__(256) bucket_join_kernel(FwdParams p, int columns, int in_use) {
+  constexpr int L = DP / 8, SG = 64 / L;
+  __shared__ float s_m[4], s_l[4], s_y[4][DP];
+  const int64_t unit = blockIdx.x / in_use;
+  const int c = int(blockIdx.x - unit * in_use), ct = int(unit / p.UH % p.CT);
   const Column me = column_of(p, unit, ct * columns + c);
   if (!me.in) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float* ml = p.part_ml + (unit * p.splits * columns + c) * 2;
   const float* po = p.part_out + (unit * p.splits * columns + c) * DP;
   const int64_t step = columns;
   float m = -INFINITY, l = 0.0f;
-  for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, ml[s * step * 2]);
+  for (int s = tid; s < p.splits; s += 256) m = fmaxf(m, ml[s * step * 2]);
   m = wave_max(m);
+  if (lane == 0) s_m[wave] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
   const float from = m == -INFINITY ? 0.0f : m;
-  // DP / 8 lanes take a split's entries, the others the next splits
-  constexpr int L = DP / 8, SG = 64 / L;
   const int d0 = (lane % L) * 8, g = lane / L;
   float y[8] = {};
-  for (int s = g; s < p.splits; s += SG) {
+#pragma unroll 4
+  for (int s = wave * SG + g; s < p.splits; s += 4 * SG) {
     const float2 one = *reinterpret_cast<const float2*>(ml + s * step * 2);
-    const float w = fast_exp2(one.x - from);
-    l += w * one.y;
     const float4 lo = *reinterpret_cast<const float4*>(po + s * step * DP + d0);
     const float4 hi = *reinterpret_cast<const float4*>(po + s * step * DP + d0 + 4);
+    const float w = fast_exp2(one.x - from);
+    l += w * one.y;
     y[0] += w * lo.x;
     y[1] += w * lo.y;
     y[2] += w * lo.z;
@@ -300,11 +310,20 @@ __global__ void __launch_bounds__(256) bucket_join_kernel(FwdParams p, int colum
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] += __shfl_xor(y[e], off, 64);
   }
+  if (g == 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s_y[wave][d0 + e] = y[e];
+    if (lane == 0) s_l[wave] = l;
+  }
+  __syncthreads();
+  if (tid >= L) return;
+  l = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
   const float inv = l > 0.0f ? 1.0f / l : l;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] *= inv;
-  if (g == 0 && d0 < p.D) store_row<T>(p, me, d0, y);
-  if (lane == 0) store_stats<T>(p, me, p.units / (int64_t(p.UH) * p.CT), m, l);
+  for (int e = 0; e < 8; ++e)
+    y[e] = ((s_y[0][d0 + e] + s_y[1][d0 + e]) + (s_y[2][d0 + e] + s_y[3][d0 + e])) * inv;
+  if (d0 < p.D) store_row<T>(p, me, d0, y);
+  if (tid == 0) store_stats<T>(p, me, p.units / (int64_t(p.UH) * p.CT), m, l);
 }
 
 namespace {
@@ -388,8 +407,9 @@ int launch_fwd(const FwdParams& p, hipStream_t s) {
   hipLaunchKernelGGL((bucket_attn_kernel<T, DP, W, PACKED>), dim3(unsigned(blocks)), dim3(64 * W), 0, s, p);
   MF_HIP_CHECK(hipGetLastError());
   if (p.splits > 1) {
-    const int64_t all = p.units * 32 * W;
-    hipLaunchKernelGGL((bucket_join_kernel<T, DP>), dim3(unsigned((all + 3) / 4)), dim3(256), 0, s, p, 32 * W, all);
+    // (columns past the last are left out)
+    const int columns = p.CT == 1 ? std::min(32 * W, p.packed ? p.G * p.Nq : p.Nq) : 32 * W;
+    hipLaunchKernelGGL((bucket_join_kernel<T, DP>), dim3(unsigned(p.units * columns)), dim3(256), 0, s, p, 32 * W, columns);
     MF_HIP_CHECK(hipGetLastError());
   }
   return MF_OK;

@@ -69,12 +69,14 @@ struct BwdParams {
   void* dv;
   float* rows;    // [B H, TQ, 3, 64] m, 1 / l (fp16: times kProb), -delta
   float4* peak;   // fp16: [B H, TQ] max |go|^2 and |dlse|, then [B KV, TK] max |v|^2
-  float* parts;   // [H, K, B CK] sums of dS by bucket, or null
+  float* parts;   // [H, K, B CK pieces] sums of dS by bucket, or null
+  float* split;   // pieces > 1: [units, pieces, columns, 2 or 1, DP] gradients, then the queries' sums [units, pieces, columns]
   int64_t qs[3], ks[3], vs[3], os[3], gs[3], dqs[3], dks[3], dvs[3];
   int64_t index_step, index_t_step, any_step;
   float scale;
   int B, H, KV, G, Nq, Nk, D, S, St, TQ, TK, K, table_dtype;
   int CT;  // column tiles of a head, of the kernel at hand
+  int pieces, per_piece;  // the streamed row tiles in pieces, one a workgroup
   int64_t units;
 };
 
@@ -233,9 +235,26 @@ struct BlockSums<true> {
   }
 };
 
+template <typename T>
+__device__ __forceinline__ void store8(T* to, const float (&x)[8]) {
+  typedef __attribute__((__vector_size__(8 * sizeof(T)))) T T8;
+  T8 y;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = static_cast<T>(x[e]);
+  *reinterpret_cast<T8*>(to) = y;
+}
+
+// delta of query `at`, corrected by the sum of its dS: that is dlse but for delta's error.
+__device__ __forceinline__ void correct_delta(const BwdParams& p, int64_t b, int h, int at, float total) {
+  const int64_t bh = b * p.H + h;
+  float* delta = p.rows + (bh * p.TQ + (at >> 6)) * 3 * kTile + 2 * kTile + (at & 63);  // (negative)
+  *delta -= total - (p.dlse ? p.dlse[bh * p.Nq + at] : 0.0f);
+}
+
 // -- the products ------------------------------------------------------------------------------------------------
 template <typename T, int DP, int W, bool KEYS, bool SUMS>
-__global__ void __launch_bounds__(64 * W, DP == 128 && KEYS ? 1 : 2) bucket_bwd_kernel(BwdParams p) {
+__global__ void __launch_bounds__(64 * W, (DP == 128 && (KEYS || W == 2)) || (W == 1 && DP > 32) ? 1 : 2)
+    bucket_bwd_kernel(BwdParams p) {
   using Op = typename Elem<T>::Operand;
   constexpr int NK = DP / 16, ND = DP / 32;
   constexpr int kBytes = kTile * DP * 2;
@@ -250,8 +269,10 @@ __global__ void __launch_bounds__(64 * W, DP == 128 && KEYS ? 1 : 2) bucket_bwd_
   __shared__ float s_table[kPitch];
   extern __shared__ float s_bins[];  // SUMS: [K + 1][64 W], the last one of masked pairs
   static_assert(KEYS || !SUMS, "the table's gradient is the keys' kernel's");
-  const int64_t id = xcd_order(blockIdx.x, gridDim.x);
-  if (id >= p.units) return;
+  const int64_t in_order = xcd_order(blockIdx.x, gridDim.x);
+  if (in_order >= p.units * p.pieces) return;
+  const int64_t id = in_order / p.pieces;
+  const int piece = int(in_order - id * p.pieces);
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // units: the heads of a column tile follow one another (they read the same buckets)
@@ -350,11 +371,18 @@ __global__ void __launch_bounds__(64 * W, DP == 128 && KEYS ? 1 : 2) bucket_bwd_
   };
 
   for (int g = 0; g < (KEYS ? p.G : 1); ++g) {
+    const int t0 = max(0, piece * p.per_piece - g * rows), t1 = min(rows, (piece + 1) * p.per_piece - g * rows);
+    const int64_t slots = int64_t(p.B) * p.CT * p.pieces;
+    float* slot = SUMS ? p.parts + int64_t(kv * p.G + g) * p.K * slots + (b * p.CT + ct) * p.pieces + piece : nullptr;
+    if (t0 >= t1) {  // none of this head's rows in the piece
+      if (SUMS && int(threadIdx.x) < p.K) slot[threadIdx.x * slots] = 0.0f;
+      continue;
+    }
     side(KEYS ? kv * p.G + g : uh);
     load_tables(s_table, p.table, p.table_dtype, p.K, p.H, KEYS ? kv * p.G + g : uh, 1, 64 * W);
     if constexpr (SUMS)
       for (int c = 0; c <= p.K; ++c) s_bins[c * 64 * W + threadIdx.x] = 0.0f;
-    Tiles tiles(by_row + int64_t(c0) * rows, two ? by_row + int64_t(c0 + 1) * rows : nullptr, 0, rows);
+    Tiles tiles(by_row + int64_t(c0) * rows, two ? by_row + int64_t(c0 + 1) * rows : nullptr, t0, t1);
     int tile = 0, buffer = 0;
     uint64_t set = 0;
     uint4 next[2];
@@ -458,41 +486,85 @@ __global__ void __launch_bounds__(64 * W, DP == 128 && KEYS ? 1 : 2) bucket_bwd_
 #pragma unroll
         for (int u = 0; u < W; ++u) v += s_bins[c * 64 * W + u * 64 + lane];
         v = wave_sum(v) * (kHalf ? 1.0f / kProb : 1.0f);
-        if (lane == 0) p.parts[(int64_t(kv * p.G + g) * p.K + c) * (int64_t(p.B) * p.CT) + b * p.CT + ct] = v;
+        if (lane == 0) slot[c * slots] = v;
       }
       __syncthreads();  // the next head clears them
     }
   }
 
-  if (in) {
-    T* ox = KEYS ? static_cast<T*>(p.dk) + b * p.dks[0] + kv * p.dks[1] + at * p.dks[2]
-                 : static_cast<T*>(p.dq) + b * p.dqs[0] + uh * p.dqs[1] + at * p.dqs[2];
-    T* oy = static_cast<T*>(p.dv) + b * p.dvs[0] + kv * p.dvs[1] + at * p.dvs[2];
-    const float fx = KEYS ? down : down * (kHalf ? cinv * (1.0f / kProb) : cinv), fy = kHalf ? 1.0f / kProb : 1.0f;
+  const float fx = KEYS ? down : down * (kHalf ? cinv * (1.0f / kProb) : cinv), fy = kHalf ? 1.0f / kProb : 1.0f;
+  if (!KEYS) total = pair_sum(total) * (kHalf ? cinv * (1.0f / kProb) : cinv);
+  if (!in) return;
+  const int64_t place = in_order * (32 * W) + wave * 32 + (lane & 31);  // pieces > 1
+  T* ox = KEYS ? static_cast<T*>(p.dk) + b * p.dks[0] + kv * p.dks[1] + at * p.dks[2]
+               : static_cast<T*>(p.dq) + b * p.dqs[0] + uh * p.dqs[1] + at * p.dqs[2];
+  T* oy = static_cast<T*>(p.dv) + b * p.dvs[0] + kv * p.dvs[1] + at * p.dvs[2];
 #pragma unroll
-    for (int n = 0; n < ND; ++n)
+  for (int n = 0; n < ND; ++n)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int d0 = 32 * n + 16 * half + 8 * u;
-        if (d0 >= p.D) continue;
-        Op x, y;
+    for (int u = 0; u < 2; ++u) {
+      const int d0 = 32 * n + 16 * half + 8 * u;
+      float x[8], y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          // a column without a partner: zeros, whatever the tile's other rows hold
-          x[e] = static_cast<T>(mine ? ax[n][8 * u + e] * fx : 0.0f);
-          y[e] = static_cast<T>(mine ? ay[n][8 * u + e] * fy : 0.0f);
-        }
-        *reinterpret_cast<Op*>(ox + d0) = x;
-        if (KEYS) *reinterpret_cast<Op*>(oy + d0) = y;
+      for (int e = 0; e < 8; ++e) {
+        // a column without a partner: zeros, whatever the tile's other rows hold
+        x[e] = mine ? ax[n][8 * u + e] * fx : 0.0f;
+        y[e] = mine ? ay[n][8 * u + e] * fy : 0.0f;
       }
+      if (p.pieces > 1) {
+        float* to = p.split + place * (KEYS ? 2 * DP : DP) + d0;
+        store8(to, x);
+        if (KEYS) store8(to + DP, y);
+      } else if (d0 < p.D) {
+        store8(ox + d0, x);
+        if (KEYS) store8(oy + d0, y);
+      }
+    }
+  if (!KEYS && half == 0) {
+    if (p.pieces > 1) p.split[p.units * p.pieces * (32 * W) * DP + place] = total;
+    else if (mine) correct_delta(p, b, uh, at, total);
+  }
+}
+
+// Joins the pieces in their order: eight entries of a column a thread.
+template <typename T, int DP, bool KEYS>
+__global__ void __launch_bounds__(256) bucket_bwd_join_kernel(BwdParams p, int columns) {
+  constexpr int L = (KEYS ? 2 : 1) * DP / 8;
+  const int64_t id = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int part = int(id % L), c = int(id / L % columns);
+  const int64_t unit = id / L / columns;
+  if (unit >= p.units) return;
+  const int UH = KEYS ? p.KV : p.H;
+  const int uh = int(unit % UH), ct = int(unit / UH % p.CT);
+  const int64_t b = unit / (int64_t(UH) * p.CT);
+  const int at = ct * columns + c, d0 = part * 8 % DP;
+  if (at >= (KEYS ? p.Nk : p.Nq) || d0 >= p.D) return;
+  const int64_t first = unit * p.pieces * columns + c;
+  float x[8] = {};
+  for (int n = 0; n < p.pieces; ++n) {
+    const float4* in = reinterpret_cast<const float4*>(p.split + ((first + int64_t(n) * columns) * L + part) * 8);
+    const float4 lo = in[0], hi = in[1];
+    x[0] += lo.x;
+    x[1] += lo.y;
+    x[2] += lo.z;
+    x[3] += lo.w;
+    x[4] += hi.x;
+    x[5] += hi.y;
+    x[6] += hi.z;
+    x[7] += hi.w;
   }
   if (!KEYS) {
-    total = pair_sum(total);
-    const float inv = kHalf ? cinv * (1.0f / kProb) : cinv;
-    if (mine && half == 0 && inv > 0.0f) {
-      const float left = p.dlse ? p.dlse[(b * p.H + uh) * p.Nq + at] : 0.0f;
-      p.rows[((b * p.H + uh) * p.TQ + (at >> 6)) * 3 * kTile + 2 * kTile + (at & 63)] = cdelta - (total * inv - left);
+    store8(static_cast<T*>(p.dq) + b * p.dqs[0] + uh * p.dqs[1] + at * p.dqs[2] + d0, x);
+    if (part == 0) {
+      float total = 0.0f;
+      for (int n = 0; n < p.pieces; ++n)
+        total += p.split[p.units * p.pieces * columns * DP + first + int64_t(n) * columns];
+      correct_delta(p, b, uh, at, total);
     }
+  } else if (part * 8 < DP) {
+    store8(static_cast<T*>(p.dk) + b * p.dks[0] + uh * p.dks[1] + at * p.dks[2] + d0, x);
+  } else {
+    store8(static_cast<T*>(p.dv) + b * p.dvs[0] + uh * p.dvs[1] + at * p.dvs[2] + d0, x);
   }
 }
 
@@ -500,13 +572,33 @@ namespace {
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
+struct Side {  // the queries' or the keys' kernel
+  int W, CT, pieces, per_piece;
+  int64_t units;
+  size_t split_bytes;
+};
 struct BwdPlan {
-  int DP, TQ, TK, WQ, WK, CQ, CK;  // waves and column tiles of the queries' and the keys' kernel
-  size_t rows, peak, parts;
-  size_t total() const { return rows + peak + parts; }
+  int DP, TQ, TK;
+  Side queries, keys;
+  size_t rows, peak, parts, split;
+  size_t total() const { return rows + peak + parts + split; }
 };
 
-int waves_of(int columns) { return columns <= 32 ? 1 : columns <= 64 ? 2 : 4; }
+// Few workgroups over many row tiles: the tiles in pieces, until the waves that fit (one a SIMD with head_dim 128's keys,
+// two otherwise) are there, so many that none is left over.
+Side side_of(int64_t batch_heads, int columns, int64_t tiles, int DP, bool keys) {
+  Side z = {};
+  z.W = columns <= 32 ? 1 : columns <= 64 ? 2 : 4;
+  z.CT = (columns + 32 * z.W - 1) / (32 * z.W);
+  z.units = batch_heads * z.CT;
+  const int64_t room = 1024 * (keys && DP == 128 ? 1 : 2);
+  const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>(tiles, room / std::max<int64_t>(1, z.units * z.W)));
+  z.per_piece = int((tiles + pieces - 1) / pieces);
+  z.pieces = int((tiles + z.per_piece - 1) / z.per_piece);
+  if (z.pieces > 1)
+    z.split_bytes = size_t(z.units) * z.pieces * 32 * z.W * (keys ? 2 * DP : DP + 1) * sizeof(float);
+  return z;
+}
 
 BwdPlan bwd_plan(const mf_bucket_attn_bwd_args* a) {
   const mf_bucket_attn_args* f = &a->fwd;
@@ -514,14 +606,14 @@ BwdPlan bwd_plan(const mf_bucket_attn_bwd_args* a) {
   z.DP = f->head_dim <= 32 ? 32 : f->head_dim <= 64 ? 64 : 128;
   z.TQ = (f->queries + kTile - 1) / kTile;
   z.TK = (f->keys + kTile - 1) / kTile;
-  z.WQ = waves_of(f->queries);
-  z.WK = waves_of(f->keys);
-  z.CQ = (f->queries + 32 * z.WQ - 1) / (32 * z.WQ);
-  z.CK = (f->keys + 32 * z.WK - 1) / (32 * z.WK);
-  const size_t qt = size_t(f->batch) * f->heads * z.TQ, kt = size_t(f->batch) * f->kv_heads * z.TK;
+  const int64_t B = f->batch;
+  z.queries = side_of(B * f->heads, f->queries, z.TK, z.DP, false);
+  z.keys = side_of(B * f->kv_heads, f->keys, int64_t(f->heads / f->kv_heads) * z.TQ, z.DP, true);
+  const size_t qt = size_t(B) * f->heads * z.TQ, kt = size_t(B) * f->kv_heads * z.TK;
   z.rows = round256(qt * 3 * kTile * sizeof(float));
   z.peak = f->dtype == MF_DTYPE_F16 ? round256((qt + kt) * sizeof(float4)) : 0;
-  z.parts = a->dtable ? round256(size_t(f->heads) * f->buckets * f->batch * z.CK * sizeof(float)) : 0;
+  z.parts = a->dtable ? round256(size_t(f->heads) * f->buckets * B * z.keys.CT * z.keys.pieces * sizeof(float)) : 0;
+  z.split = round256(std::max(z.queries.split_bytes, z.keys.split_bytes));  // one kernel's at a time
   return z;
 }
 
@@ -532,9 +624,15 @@ int launch_bwd(const BwdParams& p, hipStream_t s) {
   static_assert(kMost + 4 * kTile * DP * 2 + 4096 <= 160 * 1024, "LDS of a workgroup");
   if (const int status = ensure_dynamic_lds(reinterpret_cast<const void*>(bucket_bwd_kernel<T, DP, W, KEYS, SUMS>), kMost))
     return status;
-  hipLaunchKernelGGL((bucket_bwd_kernel<T, DP, W, KEYS, SUMS>), dim3(unsigned((p.units + 7) / 8 * 8)), dim3(64 * W), lds,
-                     s, p);
+  hipLaunchKernelGGL((bucket_bwd_kernel<T, DP, W, KEYS, SUMS>), dim3(unsigned((p.units * p.pieces + 7) / 8 * 8)), dim3(64 * W),
+                     lds, s, p);
   MF_HIP_CHECK(hipGetLastError());
+  if (p.pieces > 1) {
+    const int64_t threads = p.units * 32 * W * (KEYS ? 2 : 1) * (DP / 8);
+    hipLaunchKernelGGL((bucket_bwd_join_kernel<T, DP, KEYS>), dim3(unsigned((threads + 255) / 256)), dim3(256), 0, s, p,
+                       32 * W);
+    MF_HIP_CHECK(hipGetLastError());
+  }
   return MF_OK;
 }
 
@@ -550,12 +648,16 @@ int launch_all(BwdParams p, const BwdPlan& z, hipStream_t s) {
   const int64_t blocks = int64_t(p.B) * p.H * z.TQ + (p.peak ? int64_t(p.B) * p.KV * z.TK : 0);
   hipLaunchKernelGGL((bucket_rows_kernel<T, DP>), dim3(unsigned(blocks)), dim3(kRowThreads), 0, s, p);
   MF_HIP_CHECK(hipGetLastError());
-  p.CT = z.CQ;
-  p.units = int64_t(p.B) * p.H * z.CQ;
-  if (const int status = launch_bwd<T, DP, false, false>(p, z.WQ, s)) return status;
-  p.CT = z.CK;
-  p.units = int64_t(p.B) * p.KV * z.CK;
-  return p.parts ? launch_bwd<T, DP, true, true>(p, z.WK, s) : launch_bwd<T, DP, true, false>(p, z.WK, s);
+  auto take = [&p](const Side& z) {
+    p.CT = z.CT;
+    p.pieces = z.pieces;
+    p.per_piece = z.per_piece;
+    p.units = z.units;
+  };
+  take(z.queries);
+  if (const int status = launch_bwd<T, DP, false, false>(p, z.queries.W, s)) return status;
+  take(z.keys);
+  return p.parts ? launch_bwd<T, DP, true, true>(p, z.keys.W, s) : launch_bwd<T, DP, true, false>(p, z.keys.W, s);
 }
 
 template <typename T>
@@ -599,7 +701,9 @@ extern "C" int mf_bucket_attn_bwd(const mf_bucket_attn_bwd_args* a, void* stream
     return fail(MF_ERR_UNSUPPORTED, "mf_bucket_attn_bwd: queries and keys must be positive");
   const BwdPlan z = bwd_plan(a);
   const int64_t B = f->batch;
-  const int64_t most = std::max({B * f->heads * z.TQ + B * f->kv_heads * z.TK, B * f->kv_heads * z.CK + 8, B * f->heads * z.CQ + 8});
+  // (where there are pieces, there are few units)
+  const int64_t most = std::max({B * f->heads * z.TQ + B * f->kv_heads * z.TK, z.keys.units * z.keys.pieces + 8,
+                                 z.queries.units * z.queries.pieces + 8});
   if (most * 256 > 0xffffffffLL)  // threads of a launch
     return fail(MF_ERR_UNSUPPORTED, "mf_bucket_attn_bwd: batch * heads * tiles too large");
   if (!a->workspace || a->workspace_bytes < z.total() || reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0)
@@ -626,6 +730,7 @@ extern "C" int mf_bucket_attn_bwd(const mf_bucket_attn_bwd_args* a, void* stream
   p.rows = reinterpret_cast<float*>(ws);
   p.peak = z.peak ? reinterpret_cast<float4*>(ws + z.rows) : nullptr;
   p.parts = a->dtable ? reinterpret_cast<float*>(ws + z.rows + z.peak) : nullptr;
+  p.split = reinterpret_cast<float*>(ws + z.rows + z.peak + z.parts);
   for (int n = 0; n < 3; ++n) {
     p.qs[n] = f->q_stride[n];
     p.ks[n] = f->k_stride[n];
@@ -656,5 +761,5 @@ extern "C" int mf_bucket_attn_bwd(const mf_bucket_attn_bwd_args* a, void* stream
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int status = f->dtype == MF_DTYPE_BF16 ? launch_all<__bf16>(p, z, s) : launch_all<_Float16>(p, z, s);
   if (status != MF_OK || !a->dtable) return status;
-  return launch_table_sum(p.parts, a->dtable, p.H, p.K, p.B * z.CK, p.table_dtype, s);
+  return launch_table_sum(p.parts, a->dtable, p.H, p.K, p.B * z.keys.CT * z.keys.pieces, p.table_dtype, s);
 }

@@ -9,8 +9,8 @@
 // fp64 without contraction, so that the bucket is that of the exact distance of
 // the fp32 coordinates but for the roundings of fp64.
 //
-// bucket_bias_kernel: a thread reads 16 buckets once and writes their biases for
-// every head; the tables lie in LDS, one bank a bucket.  Bound by its writes.
+// bucket_bias_kernel: a thread reads the buckets of 16 bytes of bias once and
+// writes them for every head; the tables lie in LDS, one bank a bucket.  Bound by its writes.
 //
 // bucket_bias_bwd_kernel: sums by bucket without atomics between lanes.  Every
 // lane keeps a sum per bucket of its own in LDS ([bucket][thread]: one bank a
@@ -73,6 +73,8 @@ __global__ void __launch_bounds__(kThreads) pair_buckets_kernel(BucketParams p) 
   __shared__ __attribute__((aligned(16))) float s_pos[3][kTile];
   __shared__ Value s_edges[MF_MAX_BUCKETS];
   __shared__ uint32_t s_cells[kCells / 4];
+  __shared__ int64_t s_off[SOURCE == MF_BUCKETS_OFFSET ? kTile : 1];
+  __shared__ int s_off32[SOURCE == MF_BUCKETS_OFFSET ? kTile : 1];
   __shared__ uint8_t tile[kTile][kTile + 4];
   __shared__ uint64_t s_key[4], s_qry[4];
   int64_t id = xcd_order(blockIdx.x, gridDim.x) + p.first;
@@ -125,10 +127,65 @@ __global__ void __launch_bounds__(kThreads) pair_buckets_kernel(BucketParams p) 
       qo = static_cast<const int64_t*>(p.query_pos)[b * p.query_step + i];
     }
   }
+  // OFFSET: positions relative to the tile's first key; where all of a wave's are within 2^29 their differences are formed
+  // in 32 bits, and if the least and the greatest of those that count have one bucket the wave's rows have no other
+  bool near = true, whole = false;
+  int q32 = 0, whole_code = 0;
+  if constexpr (SOURCE == MF_BUCKETS_OFFSET) {
+    const int64_t* kp = static_cast<const int64_t*>(p.key_pos) + b * p.key_step;
+    const int64_t base = kp[kt * kTile], mine = jl < p.Nk ? kp[jl] : base;
+    const int64_t dk = mine - base, dq = i < p.Nq ? qo - base : 0;
+    constexpr int64_t kNear = int64_t(1) << 29;
+    const bool keys_near = !__any(!(dk > -kNear && dk < kNear));  // (one answer for the workgroup)
+    near = keys_near && !__any(!(dq > -kNear && dq < kNear));
+    if (wave == 0) {
+      s_off[lane] = mine;
+      if (keys_near) s_off32[lane] = int(dk);
+    }
+    if (near) {
+      q32 = int(dq);
+      const bool key_in = (keys >> lane) & 1;
+      int klo = key_in ? int(dk) : INT32_MAX, khi = key_in ? int(dk) : INT32_MIN;
+      int qlo = row_on ? q32 : INT32_MAX, qhi = row_on ? q32 : INT32_MIN;
+#pragma unroll
+      for (int off = 32; off >= 1; off >>= 1) {
+        klo = min(klo, __shfl_xor(klo, off, 64));
+        khi = max(khi, __shfl_xor(khi, off, 64));
+        qlo = min(qlo, __shfl_xor(qlo, off, 64));
+        qhi = max(qhi, __shfl_xor(qhi, off, 64));
+      }
+      if (klo <= khi && qlo <= qhi) {
+        const int low = klo - qhi, high = khi - qlo;  // the least and the greatest offset
+        if (p.causal && low > 0) {
+          whole = true;
+          whole_code = kMasked;
+        } else if (!(p.causal && high > 0)) {
+          int nl = 0, nh = 0;
+          for (int e = lane; e < p.buckets - 1; e += 64) {
+            nl += double(low) >= p.edges[e];
+            nh += double(high) >= p.edges[e];
+          }
+          nl = __popcll(__ballot(nl != 0));
+          nh = __popcll(__ballot(nh != 0));
+          whole = nl == nh;
+          whole_code = nl;
+        }
+      } else {
+        whole = true;
+        whole_code = kMasked;
+      }
+    }
+  }
   __syncthreads();
   uint32_t w[4] = {0x40404040u, 0x40404040u, 0x40404040u, 0x40404040u};  // kMasked
   const uint32_t mine = row_on ? uint32_t(keys >> c0) & 0xffffu : 0u;
-  if (mine != 0) {
+  if (SOURCE == MF_BUCKETS_OFFSET && whole) {
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+      const uint32_t code = (mine >> t) & 1 ? uint32_t(whole_code) : uint32_t(kMasked);
+      w[t >> 2] = (w[t >> 2] & ~(255u << (8 * (t & 3)))) | code << (8 * (t & 3));
+    }
+  } else if (mine != 0) {
 #pragma unroll
     for (int t = 0; t < 16; ++t) {
       const int j = kt * kTile + c0 + t;
@@ -137,27 +194,34 @@ __global__ void __launch_bounds__(kThreads) pair_buckets_kernel(BucketParams p) 
       if constexpr (SOURCE == MF_BUCKETS_INDEX) {
         const int v = in ? static_cast<const int32_t*>(p.values)[(b * p.Nq + i) * p.Nk + j] : -1;
         if (v >= 0 && v < p.buckets) code = unsigned(v);
+      } else if constexpr (SOURCE == MF_BUCKETS_OFFSET) {
+        bool on = in;
+        unsigned n;
+        if (near) {
+          const int x = s_off32[c0 + t] - q32;
+          on = on && !(p.causal && x > 0);
+          n = reinterpret_cast<const uint8_t*>(s_cells)[cell_of(float(x), p.base, p.shift)];
+          while (int64_t(x) >= s_edges[n]) ++n;  // (not past the greatest at the end)
+        } else {
+          const int64_t x = s_off[c0 + t] - qo;
+          on = on && !(p.causal && x > 0);
+          n = reinterpret_cast<const uint8_t*>(s_cells)[cell_of(float(x), p.base, p.shift)];
+          while (n + 1 < unsigned(p.buckets) && x >= s_edges[n]) ++n;
+        }
+        if (on) code = n;
       } else {
-        Value x;
+        double x;
         bool on = in;
         if constexpr (SOURCE == MF_BUCKETS_DISTANCE) {
           const double dx = qx - s_pos[0][c0 + t], dy = qy - s_pos[1][c0 + t], dz = qz - s_pos[2][c0 + t];
           x = (dx * dx + dy * dy) + dz * dz;
-          on = on && !(p.cutoff >= 0.0 && x > p.cutoff);
-        } else if constexpr (SOURCE == MF_BUCKETS_OFFSET) {
-          x = (in ? static_cast<const int64_t*>(p.key_pos)[b * p.key_step + j] : 0) - qo;
-          on = on && !(p.causal && x > 0);
         } else {
           x = in ? static_cast<const float*>(p.values)[(b * p.Nq + i) * p.Nk + j] : 0.0f;
-          on = on && !(p.cutoff >= 0.0 && x > p.cutoff);
         }
+        on = on && !(p.cutoff >= 0.0 && x > p.cutoff);
         unsigned n = reinterpret_cast<const uint8_t*>(s_cells)[cell_of(float(x), p.base, p.shift)];
         if (x != x) n = 0;
-        if constexpr (SOURCE == MF_BUCKETS_OFFSET) {
-          while (n + 1 < unsigned(p.buckets) && x >= s_edges[n]) ++n;
-        } else {
-          while (x >= s_edges[n]) ++n;  // (not past the NaN at the end)
-        }
+        while (x >= s_edges[n]) ++n;  // (not past the NaN at the end)
         if (on) code = n;
       }
       w[t >> 2] = (w[t >> 2] & ~(255u << (8 * (t & 3)))) | code << (8 * (t & 3));
@@ -204,12 +268,13 @@ struct BiasParams {
   const uint8_t* index;
   const void* table;
   void* bias;
-  float* parts;        // gradient: [H, K, pieces]
-  int64_t chunks;      // 16-key chunks of all rows
-  int64_t rows_index;  // rows of the index (the rows of a batch of one, or all)
-  int B, H, Nq, Nk, K, S, table_dtype;
-  int head_step;       // heads of a workgroup
-  int pieces;
+  float* parts;         // gradient: [H, K, pieces]
+  uint32_t rows;        // B Nq
+  uint32_t first_row;   // of this launch
+  uint32_t rows_index;  // rows of the index (the rows of a batch of one, or all)
+  int H, Nq, Nk, K, S, table_dtype;
+  int head_step;        // heads of a workgroup
+  int pieces, piece_rows;
 };
 
 template <typename T>
@@ -222,9 +287,11 @@ struct __attribute__((packed, aligned(sizeof(T)))) Wide {  // 16 bytes at any el
   T v[16 / sizeof(T)];
 };
 
+// V buckets of a row (16 bytes of bias) a thread.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) bucket_bias_kernel(BiasParams p) {
   extern __shared__ float s_table[];  // [head_step][kPitch]
+  constexpr int V = 16 / sizeof(T);
   const int h0 = blockIdx.y * p.head_step, heads = min(p.head_step, p.H - h0);
   for (int n = threadIdx.x; n < heads * kPitch; n += kThreads) {
     const int h = n / kPitch, c = n - h * kPitch;
@@ -238,69 +305,99 @@ __global__ void __launch_bounds__(kThreads) bucket_bias_kernel(BiasParams p) {
     s_table[n] = v;
   }
   __syncthreads();
-  const int64_t id = int64_t(blockIdx.x) * kThreads + threadIdx.x;
-  if (id >= p.chunks) return;
-  const int per = (p.Nk + 15) / 16;
-  const int64_t row = id / per;
-  const int c = int(id - row * per), b = int(row / p.Nq), i = int(row - int64_t(b) * p.Nq);
-  const uint4 packed = *reinterpret_cast<const uint4*>(p.index + (row % p.rows_index) * p.S + 16 * c);
-  const uint32_t w[4] = {packed.x, packed.y, packed.z, packed.w};
-  const int left = p.Nk - 16 * c;
-  constexpr int V = 16 / sizeof(T);
-  for (int h = 0; h < heads; ++h) {
-    T* out = static_cast<T*>(p.bias) + ((int64_t(b) * p.H + h0 + h) * p.Nq + i) * p.Nk + 16 * c;
+  const uint32_t id = blockIdx.x * uint32_t(kThreads) + threadIdx.x, per = (p.Nk + V - 1) / V;
+  const uint32_t row = p.first_row + id / per;
+  if (row >= p.rows) return;
+  const int c = int(id % per);
+  const uint32_t b = row / uint32_t(p.Nq), i = row - b * uint32_t(p.Nq);
+  const uint8_t* in = p.index + int64_t(row % p.rows_index) * p.S + V * c;
+  uint32_t w[4] = {};
+#pragma unroll
+  for (int t = 0; t < V / 4; ++t) w[t] = reinterpret_cast<const uint32_t*>(in)[t];
+  const int left = p.Nk - V * c;
+  T* out = static_cast<T*>(p.bias) + ((int64_t(b) * p.H + h0) * p.Nq + i) * p.Nk + V * c;
+  const int64_t step = int64_t(p.Nq) * p.Nk;
+  for (int h = 0; h < heads; ++h, out += step) {
     const float* table = s_table + h * kPitch;
-    if (left >= 16) {
+    Wide<T> x;
 #pragma unroll
-      for (int u = 0; u < 16 / V; ++u) {
-        Wide<T> x;
-#pragma unroll
-        for (int t = 0; t < V; ++t) x.v[t] = static_cast<T>(table[byte_of(w, V * u + t)]);
-        *reinterpret_cast<Wide<T>*>(out + V * u) = x;
-      }
+    for (int t = 0; t < V; ++t) x.v[t] = static_cast<T>(table[byte_of(w, t)]);
+    if (left >= V) {
+      *reinterpret_cast<Wide<T>*>(out) = x;
     } else {
 #pragma unroll
-      for (int t = 0; t < 16; ++t)
-        if (t < left) out[t] = static_cast<T>(table[byte_of(w, t)]);
+      for (int t = 0; t < V - 1; ++t)
+        if (t < left) out[t] = x.v[t];
     }
   }
 }
 
+// A workgroup sums one head's rows first .. + piece_rows: `across` threads to a row, each 16 keys at a time, the next ones
+// loaded while the last ones are added.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) bucket_bias_bwd_kernel(BiasParams p) {
   extern __shared__ float s_bins[];  // [K + 1][kThreads]; the last one takes the masked pairs
+  constexpr int V = 16 / sizeof(T), kKeys = 16;
   const int tid = threadIdx.x;
   for (int c = 0; c <= p.K; ++c) s_bins[c * kThreads + tid] = 0.0f;
   const int h = blockIdx.y;
-  const int per = (p.Nk + 15) / 16;
-  for (int64_t id = int64_t(blockIdx.x) * kThreads + tid; id < p.chunks; id += int64_t(p.pieces) * kThreads) {
-    const int64_t row = id / per;
-    const int c = int(id - row * per), b = int(row / p.Nq), i = int(row - int64_t(b) * p.Nq);
-    const uint4 packed = *reinterpret_cast<const uint4*>(p.index + (row % p.rows_index) * p.S + 16 * c);
-    const uint32_t w[4] = {packed.x, packed.y, packed.z, packed.w};
-    const int left = p.Nk - 16 * c;
-    const T* in = static_cast<const T*>(p.bias) + ((int64_t(b) * p.H + h) * p.Nq + i) * p.Nk + 16 * c;
-    float x[16];
-    if (left >= 16) {
-      constexpr int V = 16 / sizeof(T);
+  const int per = (p.Nk + kKeys - 1) / kKeys;
+  int across = 1;
+  while (across < per && across < kThreads) across *= 2;
+  const int down = kThreads / across, tx = tid & (across - 1), ty = tid / across;
+  const uint32_t end = min(p.rows, (blockIdx.x + 1u) * uint32_t(p.piece_rows));
+  float* bins = s_bins + tid;
+
+  uint4 packed = {};
+  Wide<T> x[kKeys / V];
+  int left = 0;
+  auto load = [&](uint32_t row, int c) {
+    const uint32_t b = row / uint32_t(p.Nq), i = row - b * uint32_t(p.Nq);
+    packed = *reinterpret_cast<const uint4*>(p.index + int64_t(row % p.rows_index) * p.S + kKeys * c);
+    left = p.Nk - kKeys * c;
+    const T* in = static_cast<const T*>(p.bias) + ((int64_t(b) * p.H + h) * p.Nq + i) * p.Nk + kKeys * c;
+    if (left >= kKeys) {
 #pragma unroll
-      for (int u = 0; u < 16 / V; ++u) {
-        const Wide<T> y = *reinterpret_cast<const Wide<T>*>(in + V * u);
-#pragma unroll
-        for (int t = 0; t < V; ++t) x[V * u + t] = float(y.v[t]);
-      }
+      for (int u = 0; u < kKeys / V; ++u) x[u] = reinterpret_cast<const Wide<T>*>(in)[u];
     } else {
 #pragma unroll
-      for (int t = 0; t < 16; ++t) x[t] = t < left ? float(in[t]) : 0.0f;
+      for (int t = 0; t < kKeys; ++t) x[t / V].v[t % V] = t < left ? in[t] : T(0.0f);
     }
+  };
+  uint32_t row = blockIdx.x * uint32_t(p.piece_rows) + ty;
+  int c = tx;
+  bool more = row < end && c < per;  // (a thread past the row's last keys has no row)
+  if (more) load(row, c);
+  while (more) {
+    const uint32_t w[4] = {packed.x, packed.y, packed.z, packed.w};
+    Wide<T> y[kKeys / V];
 #pragma unroll
-    for (int t = 0; t < 16; ++t) s_bins[min(int(byte_of(w, t)), p.K) * kThreads + tid] += x[t];
+    for (int u = 0; u < kKeys / V; ++u) y[u] = x[u];
+    c += across;
+    if (c >= per) {
+      c = tx;
+      row += down;
+    }
+    more = row < end;
+    if (more) load(row, c);
+    // two at a time: where both have one bucket the first takes both and the second adds to the masked pairs' row
+#pragma unroll
+    for (int t = 0; t < kKeys; t += 2) {
+      const int c0 = min(int(byte_of(w, t)), p.K), c1 = min(int(byte_of(w, t + 1)), p.K);
+      const float v0 = float(y[t / V].v[t % V]), v1 = float(y[(t + 1) / V].v[(t + 1) % V]);
+      const bool same = c0 == c1;
+      float* b0 = bins + c0 * kThreads;
+      float* b1 = bins + (same ? p.K : c1) * kThreads;
+      const float s0 = *b0, s1 = *b1;
+      *b0 = s0 + (same ? v0 + v1 : v0);
+      *b1 = s1 + v1;
+    }
   }
   __syncthreads();
-  for (int c = tid >> 6; c < p.K; c += kThreads / 64) {
-    const float* s = s_bins + c * kThreads + (tid & 63);
+  for (int n = tid >> 6; n < p.K; n += kThreads / 64) {
+    const float* s = s_bins + n * kThreads + (tid & 63);
     const float v = wave_sum((s[0] + s[64]) + (s[128] + s[192]));
-    if ((tid & 63) == 0) p.parts[(int64_t(h) * p.K + c) * p.pieces + blockIdx.x] = v;
+    if ((tid & 63) == 0) p.parts[(int64_t(h) * p.K + n) * p.pieces + blockIdx.x] = v;
   }
 }
 
@@ -352,6 +449,8 @@ int check_bias(const mf_bucket_bias_args* a, const char* what) {
     return fail(MF_ERR_UNSUPPORTED, name + ": queries and keys must be <= 2^24");
   if (!dtype_ok(a->table_dtype) || !dtype_ok(a->bias_dtype))
     return fail(MF_ERR_UNSUPPORTED, name + ": only supports float32/float16/bfloat16");
+  if (int64_t(a->batch) * a->queries >= (int64_t(1) << 31))
+    return fail(MF_ERR_UNSUPPORTED, name + ": batch * queries too large");
   if (reinterpret_cast<uintptr_t>(a->index) % 16 != 0)
     return fail(MF_ERR_INVALID_ARGUMENT, name + ": index must be 16-byte aligned");
   return MF_OK;
@@ -362,9 +461,8 @@ BiasParams bias_params(const mf_bucket_bias_args* a) {
   p.index = a->index;
   p.table = a->table;
   p.bias = a->bias;
-  p.chunks = int64_t(a->batch) * a->queries * ((a->keys + 15) / 16);
-  p.rows_index = int64_t(a->index_batch) * a->queries;
-  p.B = a->batch;
+  p.rows = uint32_t(a->batch) * uint32_t(a->queries);
+  p.rows_index = uint32_t(a->index_batch) * uint32_t(a->queries);
   p.H = a->heads;
   p.Nq = a->queries;
   p.Nk = a->keys;
@@ -374,12 +472,17 @@ BiasParams bias_params(const mf_bucket_bias_args* a) {
   return p;
 }
 
-// Pieces a head's pairs are summed in: four chunks a thread and more, and no more workgroups than are resident at two a
-// CU (66 KB of LDS each) twice over.
+// Rows of a piece of a head's pairs, each summed by a workgroup: four 16-key chunks a thread and more, and no more
+// workgroups than are resident at two a CU (66 KB of LDS each) twice over.
+int bias_piece_rows(const mf_bucket_bias_args* a) {
+  const int64_t rows = int64_t(a->batch) * a->queries, per = (a->keys + 15) / 16;
+  const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>((rows * per + 4 * kThreads - 1) / (4 * kThreads),
+                                                                std::max(1, 1024 / std::max(1, a->heads))));
+  return int((rows + pieces - 1) / pieces);
+}
 int bias_pieces(const mf_bucket_bias_args* a) {
-  const int64_t chunks = int64_t(a->batch) * a->queries * ((a->keys + 15) / 16);
-  return int(std::max<int64_t>(1, std::min<int64_t>((chunks + 4 * kThreads - 1) / (4 * kThreads),
-                                                    std::max(1, 1024 / std::max(1, a->heads)))));
+  const int64_t rows = int64_t(a->batch) * a->queries, step = bias_piece_rows(a);
+  return int((rows + step - 1) / step);
 }
 
 }  // namespace
@@ -483,18 +586,26 @@ extern "C" int mf_bucket_bias(const mf_bucket_bias_args* a, void* stream) {
   if (!a->table) return fail(MF_ERR_INVALID_ARGUMENT, "mf_bucket_bias: table must be non-NULL");
   if (a->batch == 0 || a->heads == 0 || a->queries == 0 || a->keys == 0) return MF_OK;
   BiasParams p = bias_params(a);
-  const int64_t blocks = (p.chunks + kThreads - 1) / kThreads;
-  if (blocks * kThreads > 0xffffffffLL) return fail(MF_ERR_UNSUPPORTED, "mf_bucket_bias: batch * queries * keys too large");
+  const int V = a->bias_dtype == MF_DTYPE_F32 ? 4 : 8;
+  const int64_t per = (a->keys + V - 1) / V, rows = p.rows;
   // a workgroup takes all heads (one read of the index) unless that leaves less than eight workgroups a CU
-  const int parts = int(std::min<int64_t>(a->heads, std::max<int64_t>(1, (2048 + blocks - 1) / blocks)));
+  const int64_t all = (rows * per + kThreads - 1) / kThreads;
+  const int parts = int(std::min<int64_t>(a->heads, std::max<int64_t>(1, (2048 + all - 1) / all)));
   p.head_step = (a->heads + parts - 1) / parts;
-  const dim3 grid(unsigned(blocks), unsigned((a->heads + p.head_step - 1) / p.head_step));
   const unsigned lds = unsigned(p.head_step * kPitch * sizeof(float));
+  const int64_t step = std::max<int64_t>(1, (int64_t(1) << 30) / per);  // rows of a launch
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a->bias_dtype == MF_DTYPE_F32) hipLaunchKernelGGL(bucket_bias_kernel<float>, grid, dim3(kThreads), lds, s, p);
-  else if (a->bias_dtype == MF_DTYPE_BF16) hipLaunchKernelGGL(bucket_bias_kernel<__bf16>, grid, dim3(kThreads), lds, s, p);
-  else hipLaunchKernelGGL(bucket_bias_kernel<_Float16>, grid, dim3(kThreads), lds, s, p);
-  MF_HIP_CHECK(hipGetLastError());
+  for (int64_t first = 0; first < rows; first += step) {
+    p.first_row = uint32_t(first);
+    const int64_t blocks = (std::min(step, rows - first) * per + kThreads - 1) / kThreads;
+    BiasParams q = p;
+    q.rows = uint32_t(std::min(rows, first + step));
+    const dim3 grid(unsigned(blocks), unsigned((a->heads + p.head_step - 1) / p.head_step));
+    if (a->bias_dtype == MF_DTYPE_F32) hipLaunchKernelGGL(bucket_bias_kernel<float>, grid, dim3(kThreads), lds, s, q);
+    else if (a->bias_dtype == MF_DTYPE_BF16) hipLaunchKernelGGL(bucket_bias_kernel<__bf16>, grid, dim3(kThreads), lds, s, q);
+    else hipLaunchKernelGGL(bucket_bias_kernel<_Float16>, grid, dim3(kThreads), lds, s, q);
+    MF_HIP_CHECK(hipGetLastError());
+  }
   return MF_OK;
 }
 
@@ -512,12 +623,13 @@ extern "C" int mf_bucket_bias_bwd(const mf_bucket_bias_args* a, void* stream) {
   BiasParams p = bias_params(a);
   hipStream_t s = static_cast<hipStream_t>(stream);
   // without a pair the sums are empty, and zero
-  if (p.chunks == 0) return launch_table_sum(nullptr, a->dtable, a->heads, a->buckets, 0, a->table_dtype, s);
+  if (a->batch == 0 || a->queries == 0 || a->keys == 0) return launch_table_sum(nullptr, a->dtable, a->heads, a->buckets, 0, a->table_dtype, s);
   if (!a->workspace || a->workspace_bytes < mf_bucket_bias_bwd_workspace_size(a) ||
       reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0)
     return fail(MF_ERR_INVALID_ARGUMENT, "mf_bucket_bias_bwd: the workspace must be 16-byte aligned and hold "
                                          "mf_bucket_bias_bwd_workspace_size bytes");
   p.pieces = bias_pieces(a);
+  p.piece_rows = bias_piece_rows(a);
   p.parts = static_cast<float*>(a->workspace);
   const dim3 grid(unsigned(p.pieces), unsigned(a->heads));
   const int lds = (a->buckets + 1) * kThreads * int(sizeof(float));

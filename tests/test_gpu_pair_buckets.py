@@ -93,6 +93,33 @@ def test_far_positions(cuda):
     same(offset_buckets(p.to(cuda), p.to(cuda), edges), offset_buckets(p, p, edges))
 
 
+@pytest.mark.parametrize("causal", [False, True])
+def test_near_and_far_positions_in_one_tile(cuda, causal):
+    """Rows whose queries are far from the tile's keys beside rows whose queries are near, padded ones among them."""
+    g = torch.Generator().manual_seed(8)
+    edges = offset_edges(24, 300)
+    for first, last, shift in ((0, 16, 2 ** 40), (0, 16, -(2 ** 29)), (40, 60, 2 ** 29 - 3), (5, 6, -(2 ** 35))):
+        qp, kp = torch.randint(0, 700, (2, 130), generator=g), torch.randint(0, 700, (2, 200), generator=g)
+        qp[:, first:last] += shift
+        kp[1, 70:90] += shift // 2
+        pad, qpad = (torch.rand(2, n, generator=g) < 0.3 for n in (200, 130))
+        masks = dict(pad_mask=pad, query_pad_mask=qpad)
+        same(offset_buckets(qp.to(cuda), kp.to(cuda), edges, causal=causal, **{n: m.to(cuda) for n, m in masks.items()}),
+             offset_buckets(qp, kp, edges, causal=causal, **masks))
+
+
+@pytest.mark.parametrize("B,N", [(1, 300), (2, 64)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_places_in_order(cuda, B, N, causal):
+    """Tiles far from the diagonal, which have one bucket."""
+    places = torch.arange(N)[None].expand(B, N) * 3
+    pad = torch.arange(N)[None] >= torch.tensor([[N - 37 * b] for b in range(B)])
+    for edges in ([], [0], offset_edges(9, 40), [-10 ** 6, -400, 5, 399, 10 ** 6]):
+        same(offset_buckets(places.to(cuda), places.to(cuda), edges, pad_mask=pad.to(cuda), query_pad_mask=pad.to(cuda),
+                            causal=causal),
+             offset_buckets(places, places, edges, pad_mask=pad, query_pad_mask=pad, causal=causal))
+
+
 @pytest.mark.parametrize("B,Nq,Nk", [(1, 1, 1), (2, 33, 130), (3, 181, 181), (1, 64, 128)])
 def test_value_and_index_buckets(cuda, B, Nq, Nk):
     g = torch.Generator().manual_seed(B * Nq)

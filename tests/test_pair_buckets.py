@@ -245,7 +245,8 @@ def test_bias_entries_refuse_before_any_device_call():
     refused(lib.mf_bucket_bias_bwd, args(), INVALID, "workspace")
     need = lib.mf_bucket_bias_bwd_workspace_size(args())
     refused(lib.mf_bucket_bias_bwd, args(workspace=FAKE, workspace_bytes=need - 1), INVALID, "workspace")
-    refused(lib.mf_bucket_bias, args(batch=2 ** 20, index_batch=1, queries=2 ** 13, keys=2 ** 10), UNSUPPORTED, "too large")
+    for fn in (lib.mf_bucket_bias, lib.mf_bucket_bias_bwd):
+        refused(fn, args(batch=2 ** 20, index_batch=1, queries=2 ** 13, keys=2 ** 10), UNSUPPORTED, "too large")
     assert lib.mf_bucket_bias(args(heads=0), None) == _native.MF_OK
     assert lib.mf_bucket_bias_bwd_workspace_size(args(queries=0)) == 0
 
