@@ -12,7 +12,7 @@
 // second.  A lane's 16 logits of a 32-key block belong to 16 consecutive bytes
 // of its query's row of buckets, loaded from global memory in one access and
 // looked up in the head's table in LDS, one bank a bucket.  fp16 keeps 2^(x - m)
-// times 2^15: many keys of small weight beside a large one still count (131072
+// times 2^7: many keys of small weight beside a large one still count (131072
 // of 2^-25 would be 0 each, 0.4 % of the row together).
 //
 // Where the query heads of a key head have few queries in all (a new token), the
@@ -52,25 +52,25 @@ struct FwdParams {
   int64_t units;
 };
 
-// What a unit's column stands for.
+// What column c of a unit's head stands for.
 struct Column {
   int64_t b;
-  int h, kv, i;
+  int h, i;
   bool in;
 };
-__device__ __forceinline__ Column column_of(const FwdParams& p, int64_t unit, int c) {
+__device__ __forceinline__ Unit unit_of(const FwdParams& p, int64_t unit) {
+  return unit_of(unit, p.UH, p.packed ? 1 : p.G, p.CT);
+}
+__device__ __forceinline__ Column column_of(const FwdParams& p, const Unit& u, int c) {
   Column r;
-  const int uh = int(unit % p.UH);
-  r.b = unit / (int64_t(p.UH) * p.CT);
+  r.b = u.b;
   if (p.packed) {
     const int g = c / p.Nq;
     r.in = g < p.G;
-    r.kv = uh;
-    r.h = uh * p.G + (r.in ? g : 0);
+    r.h = u.head * p.G + (r.in ? g : 0);
     r.i = r.in ? c - g * p.Nq : 0;
   } else {
-    r.h = uh;
-    r.kv = uh / p.G;
+    r.h = u.head;
     r.in = c < p.Nq;
     r.i = r.in ? c : 0;
   }
@@ -92,19 +92,29 @@ __device__ __forceinline__ void store_row(const FwdParams& p, const Column& c, i
   }
 }
 
+constexpr float kSlack = 8.0f;         // how far x may pass m, which is not always the maximum
+constexpr float kExact = 1048576.0f;   // |m| below which it may: up to there m + 8 and the like lose little
+
 // What 2^(x - m) is kept times, as a power of two.
 template <typename T>
 constexpr float shift_bits() {
-  return __is_same(T, _Float16) ? 15.0f : 0.0f;
+  return __is_same(T, _Float16) ? 15.0f - kSlack : 0.0f;
 }
+
 
 template <typename T>
 __device__ __forceinline__ void store_stats(const FwdParams& p, const Column& c, int64_t B, float m, float l) {
-  l *= __is_same(T, _Float16) ? 1.0f / 32768.0f : 1.0f;  // 2^-shift_bits
+  l *= __is_same(T, _Float16) ? 1.0f / 128.0f : 1.0f;  // 2^-shift_bits
   const int64_t at = (c.b * p.H + c.h) * p.Nq + c.i;
   if (p.stats) {
-    p.stats[at] = l > 0.0f ? m : 0.0f;
-    p.stats[B * p.H * p.Nq + at] = l > 0.0f ? 1.0f / l : l;  // (a NaN stays one)
+    // m is raised by the whole part of log2 l, so that 2^(x - m) <= 2 for every x of the row
+    float to = m, inv = l;  // (a NaN stays one)
+    if (l > 0.0f) {
+      if (fabsf(m) < kExact) to = m + float(ilogbf(l));
+      inv = fast_exp2(to - m) / l;
+    }
+    p.stats[at] = l > 0.0f ? to : 0.0f;
+    p.stats[B * p.H * p.Nq + at] = inv;
   }
   if (p.lse) p.lse[at] = l > 0.0f ? (m + __log2f(l)) * kLn2 : l;
 }
@@ -112,7 +122,7 @@ __device__ __forceinline__ void store_stats(const FwdParams& p, const Column& c,
 // Waves a SIMD that the registers are to allow: four (head_dim 128: two), or what LDS has room for.
 constexpr int fwd_waves(int DP, int W, bool packed) {
   const int lds = 4 * kTile * DP * 2 + (packed ? 32 : 1) * kPitch * 4;
-  const int fit = 160 * 1024 / lds * W / 4, most = DP == 128 ? 2 : 4;
+  const int fit = 160 * 1024 / lds * W / 4, most = DP == 128 ? 2 : 3;
   return fit < 1 ? 1 : fit < most ? fit : most;
 }
 
@@ -129,10 +139,10 @@ __global__ void __launch_bounds__(64 * W, fwd_waves(DP, W, PACKED)) bucket_attn_
   const int split = int(id - unit * p.splits);
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int uh = int(unit % p.UH), ct = int(unit / p.UH % p.CT);
-  const int column = ct * 32 * W + wave * 32 + (lane & 31);
-  const Column me = column_of(p, unit, column);
-  const int64_t b = unit / (int64_t(p.UH) * p.CT);
+  const Unit of = unit_of(p, unit);
+  const int uh = of.head, ct = of.tile;
+  const int64_t b = of.b;
+  const Column me = column_of(p, of, ct * 32 * W + wave * 32 + (lane & 31));
   const int kv = PACKED ? uh : uh / p.G;
 
   load_tables(s_table, p.table, p.table_dtype, p.K, p.H, PACKED ? uh * p.G : uh, PACKED ? p.G : 1, 64 * W);
@@ -171,11 +181,12 @@ __global__ void __launch_bounds__(64 * W, fwd_waves(DP, W, PACKED)) bucket_attn_
   mf_f32x16 acc[ND];
 #pragma unroll
   for (int n = 0; n < ND; ++n) acc[n] = zeros16();
-  float m = -INFINITY, l = 0.0f;
+  float m = -INFINITY, l = 0.0f, limit = -INFINITY;
 
+  const TileCopy<DP, W> kcopy(kstride, p.D, wave, lane), vcopy(vstride, p.D, wave, lane);
   auto load = [&](int tile, uint64_t set, char* to, uint4 (&w)[2]) {
-    copy_tile<DP, W>(gk + int64_t(tile) * kTile * kstride, kstride, p.D, set, to, wave, lane);
-    copy_tile<DP, W>(gv + int64_t(tile) * kTile * vstride, vstride, p.D, set, to + kBytes, wave, lane);
+    kcopy.copy(gk + int64_t(tile) * kTile * kstride, set, to, wave, lane);
+    vcopy.copy(gv + int64_t(tile) * kTile * vstride, set, to + kBytes, wave, lane);
     w[0] = *reinterpret_cast<const uint4*>(codes + int64_t(tile) * kTile);
     w[1] = *reinterpret_cast<const uint4*>(codes + int64_t(tile) * kTile + 32);
   };
@@ -209,13 +220,16 @@ __global__ void __launch_bounds__(64 * W, fwd_waves(DP, W, PACKED)) bucket_attn_
         top = fmaxf(top, x[kb][t]);
       }
     }
-    top = fmaxf(m, pair_max(top));
-    if (__any(top > m)) {
-      const float keep = top == -INFINITY ? 1.0f : fast_exp2(m - top);
+    // m follows the maximum only where that has grown by more than kSlack, so that most tiles leave the sums alone
+    top = pair_max(top);
+    if (__any(top > limit)) {
+      const float to = top > limit ? top : m;
+      const float keep = to == -INFINITY ? 1.0f : fast_exp2(m - to);
       l *= keep;
 #pragma unroll
       for (int n = 0; n < ND; ++n) acc[n] *= keep;
-      m = top;
+      m = to;
+      limit = fabsf(m) < kExact ? m + kSlack : m;
     }
     const float from = m == -INFINITY ? 0.0f : m;
 #pragma unroll
@@ -272,8 +286,9 @@ __global__ void __launch_bounds__(256) bucket_join_kernel(FwdParams p, int colum
   constexpr int L = DP / 8, SG = 64 / L;
   __shared__ float s_m[4], s_l[4], s_y[4][DP];
   const int64_t unit = blockIdx.x / in_use;
-  const int c = int(blockIdx.x - unit * in_use), ct = int(unit / p.UH % p.CT);
-  const Column me = column_of(p, unit, ct * columns + c);
+  const int c = int(blockIdx.x - unit * in_use);
+  const Unit of = unit_of(p, unit);
+  const Column me = column_of(p, of, of.tile * columns + c);
   if (!me.in) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float* ml = p.part_ml + (unit * p.splits * columns + c) * 2;

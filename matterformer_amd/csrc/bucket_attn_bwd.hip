@@ -34,7 +34,7 @@
 // products, as any 16-bit matrix product's input is.  fp16 has no room for dS of
 // small or large gradients: there it is kept times 2^e, e per (batch entry, key
 // head) from |dP - delta| <= 2 max|go| max|v| + max|dlse| over the rows that have
-// a partner, so that it stays below 2^14, and P times 2^12; bf16 has fp32's range
+// a partner, so that it stays below 2^14 (the queries' 2^(x - m) is at most 2), and P times 2^12; bf16 has fp32's range
 // and needs neither.
 #include <algorithm>
 #include <cmath>
@@ -172,7 +172,7 @@ __device__ __forceinline__ int scale_bits(const BwdParams& p, int64_t b, int kv)
   const float4* v = p.peak + int64_t(p.B) * p.H * p.TQ + (b * p.KV + kv) * p.TK;
   for (int i = lane; i < p.TK; i += 64) vm = fmaxf(vm, v[i].x);
   const float bound = 2.0f * sqrtf(wave_max(gm)) * sqrtf(wave_max(vm)) + wave_max(lm);
-  return bound > 0.0f && bound < 3.0e38f ? min(60, max(-60, 13 - ilogbf(bound))) : 0;
+  return bound > 0.0f && bound < 3.0e38f ? min(60, max(-60, 12 - ilogbf(bound))) : 0;
 }
 
 // -- the sums by bucket ------------------------------------------------------------------------------------------
@@ -275,10 +275,9 @@ __global__ void __launch_bounds__(64 * W, (DP == 128 && (KEYS || W == 2)) || (W 
   const int piece = int(in_order - id * p.pieces);
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // units: the heads of a column tile follow one another (they read the same buckets)
-  const int UH = KEYS ? p.KV : p.H;
-  const int uh = int(id % UH), ct = int(id / UH % p.CT);
-  const int64_t b = id / (int64_t(UH) * p.CT);
+  const Unit of = unit_of(id, KEYS ? p.KV : p.H, KEYS ? 1 : p.G, p.CT);
+  const int uh = of.head, ct = of.tile;
+  const int64_t b = of.b;
   const int kv = KEYS ? uh : uh / p.G;
   const int N = KEYS ? p.Nk : p.Nq, rows = KEYS ? p.TQ : p.TK;
   const int col = ct * 32 * W + wave * 32 + (lane & 31);
@@ -340,24 +339,21 @@ __global__ void __launch_bounds__(64 * W, (DP == 128 && (KEYS || W == 2)) || (W 
   float total = 0.0f;  // queries: of dS
 
   const char *tx = nullptr, *ty = nullptr, *tr = nullptr;
-  unsigned xstride = 0, ystride = 0;
+  const unsigned xstride = unsigned(KEYS ? p.qs[2] : p.ks[2]) * 2, ystride = unsigned(KEYS ? p.gs[2] : p.vs[2]) * 2;
+  const TileCopy<DP, W> xcopy(xstride, p.D, wave, lane), ycopy(ystride, p.D, wave, lane);
   auto side = [&](int h) {  // the streamed side of query head h
     if (KEYS) {
       tx = reinterpret_cast<const char*>(static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[1]);
       ty = reinterpret_cast<const char*>(static_cast<const T*>(p.go) + b * p.gs[0] + h * p.gs[1]);
       tr = reinterpret_cast<const char*>(p.rows + (b * p.H + h) * p.TQ * 3 * kTile);
-      xstride = unsigned(p.qs[2]) * 2;
-      ystride = unsigned(p.gs[2]) * 2;
     } else {
       tx = reinterpret_cast<const char*>(static_cast<const T*>(p.k) + b * p.ks[0] + kv * p.ks[1]);
       ty = reinterpret_cast<const char*>(static_cast<const T*>(p.v) + b * p.vs[0] + kv * p.vs[1]);
-      xstride = unsigned(p.ks[2]) * 2;
-      ystride = unsigned(p.vs[2]) * 2;
     }
   };
   auto load = [&](int tile, uint64_t set, int buffer, uint4 (&w)[2]) {
-    copy_tile<DP, W>(tx + int64_t(tile) * kTile * xstride, xstride, p.D, set, s_tiles + buffer, wave, lane);
-    copy_tile<DP, W>(ty + int64_t(tile) * kTile * ystride, ystride, p.D, set, s_tiles + buffer + kBytes, wave, lane);
+    xcopy.copy(tx + int64_t(tile) * kTile * xstride, set, s_tiles + buffer, wave, lane);
+    ycopy.copy(ty + int64_t(tile) * kTile * ystride, set, s_tiles + buffer + kBytes, wave, lane);
     if (KEYS && wave == 0) {
       const mf_i32x4 src = lds_copy_source(tr + int64_t(tile) * (kRowFloats * 4));
       const bool on = (set >> lane) & 1;  // zeros for rows without a partner here too
@@ -534,9 +530,9 @@ __global__ void __launch_bounds__(256) bucket_bwd_join_kernel(BwdParams p, int c
   const int part = int(id % L), c = int(id / L % columns);
   const int64_t unit = id / L / columns;
   if (unit >= p.units) return;
-  const int UH = KEYS ? p.KV : p.H;
-  const int uh = int(unit % UH), ct = int(unit / UH % p.CT);
-  const int64_t b = unit / (int64_t(UH) * p.CT);
+  const Unit of = unit_of(unit, KEYS ? p.KV : p.H, KEYS ? 1 : p.G, p.CT);
+  const int uh = of.head, ct = of.tile;
+  const int64_t b = of.b;
   const int at = ct * columns + c, d0 = part * 8 % DP;
   if (at >= (KEYS ? p.Nk : p.Nq) || d0 >= p.D) return;
   const int64_t first = unit * p.pieces * columns + c;

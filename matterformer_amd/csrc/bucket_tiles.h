@@ -67,23 +67,37 @@ __device__ __forceinline__ int swz(int row) {
   else return b2 | b4 << 1;
 }
 
-// Copies the rows of a 64-row tile (those in `set`; the others and the entries past D become zeros) into LDS.
-// base: the tile's first row; stride: bytes between rows.  W waves take part.
+// Copies the rows of a 64-row tile (those in a set; the others and the entries past D become zeros) into LDS.  W waves take
+// part; stride: bytes between rows.
 template <int DP, int W>
-__device__ __forceinline__ void copy_tile(const char* base, unsigned stride, int D, uint64_t set, char* lds, int wave,
-                                          int lane) {
-  constexpr int CPR = DP / 8, kLoads = CPR / W;
+struct TileCopy {
+  static constexpr int CPR = DP / 8, kLoads = CPR / W;
   static_assert(kLoads >= 1, "a wave copies at least one chunk a lane");
-  const mf_i32x4 src = lds_copy_source(base);
+  unsigned off[kLoads];  // of the lane's chunks from the tile's first row
+
+  __device__ __forceinline__ TileCopy(unsigned stride, int D, int wave, int lane) { start(stride, D, wave, lane); }
+  __device__ __forceinline__ void start(unsigned stride, int D, int wave, int lane) {
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int q = (wave * kLoads + i) * 64 + lane;
-    const int row = q / CPR, chunk = (q % CPR) ^ swz<DP>(row);
-    const bool on = chunk * 8 < D && ((set >> row) & 1);
-    lds_copy16(src, on ? unsigned(row) * stride + unsigned(chunk) * 16 : kLdsCopyOutside,
-               lds + (wave * kLoads + i) * 1024);
+    for (int i = 0; i < kLoads; ++i) {
+      const int q = (wave * kLoads + i) * 64 + lane, row = q / CPR, chunk = (q % CPR) ^ swz<DP>(row);
+      off[i] = chunk * 8 < D ? unsigned(row) * stride + unsigned(chunk) * 16 : kLdsCopyOutside;
+    }
   }
-}
+  __device__ __forceinline__ void copy(const char* base, uint64_t set, char* lds, int wave, int lane) const {
+    const mf_i32x4 src = lds_copy_source(base);
+    if (set == ~uint64_t(0)) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) lds_copy16(src, off[i], lds + (wave * kLoads + i) * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int row = ((wave * kLoads + i) * 64 + lane) / CPR;
+        const uint32_t word = row & 32 ? uint32_t(set >> 32) : uint32_t(set);
+        lds_copy16(src, (word >> (row & 31)) & 1 ? off[i] : kLdsCopyOutside, lds + (wave * kLoads + i) * 1024);
+      }
+    }
+  }
+};
 
 // Where a lane reads a staged tile: byte offsets that 32-row blocks and eight-row steps shift by constants (the swizzle
 // takes no part of them).
@@ -186,6 +200,26 @@ __device__ __forceinline__ unsigned byte_of(const uint32_t (&w)[4], int t) { ret
 // Workgroups of a launch in an order in which those that follow one another run on one XCD.  grid: a multiple of 8.
 __device__ __forceinline__ int64_t xcd_order(unsigned block, unsigned grid) {
   return int64_t(block & 7) * (grid >> 3) + (block >> 3);
+}
+
+// A unit is a tile of columns of a head: the tiles of a key head, its query heads inside, follow one another, for they
+// stream the same rows.  The last and the first tile take turns, so that where the work grows with the tile (earlier keys
+// only) any stretch of units, an XCD's for one, has the same share of it.
+struct Unit {
+  int64_t b;
+  int head, tile;  // head: of `heads`, `inside` of them to a key head
+};
+__device__ __forceinline__ Unit unit_of(int64_t id, int heads, int inside, int tiles) {
+  const int g = int(id % inside);
+  id /= inside;
+  const int i = int(id % tiles);
+  id /= tiles;
+  const int groups = heads / inside;
+  Unit u;
+  u.tile = i & 1 ? i >> 1 : tiles - 1 - (i >> 1);
+  u.head = int(id % groups) * inside + g;
+  u.b = id / groups;
+  return u;
 }
 
 }  // namespace bucket

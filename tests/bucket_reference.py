@@ -31,8 +31,9 @@ def attention(q, k, v, table, index, scale, go=None, glse=None):
     sums are fp32, where |x| < 128 leaves P a relative error below 128 * 2^-24 * 4 = 2^-15 (and delta's from out's two
     parts, 2^-18, is within the same share of its terms).  delta = go . out has the error of out's rounded P, at most
     (u + f) |go| . (P |v|), in dq; for dk and dtable it is corrected.
-    fp16's steps end at 2^-24: a result is off by up to 2^-25 besides, P (kept times 2^15 and 2^12, with 1 / l <= 1 in
-    the second) by 2^-40 and 2^-37, and dS, kept times 2^e >= 2^12 / (2 max|go| max|v| + max|dlse|), by 2^-25 - e."""
+    fp16's steps end at 2^-24: a result is off by up to 2^-25 besides; P by 2^-32 (it is kept times 2^7 over a sum of at
+    least 1) and, for dv, 2^-37 (kept times 2^12); and dS, kept times 2^e >= 2^12 / (2 max|go| max|v| + max|dlse|), by
+    2^-25 - e."""
     half = q.dtype == torch.float16
     grain = 2.0 ** -25 if half else 0.0
     B, H = q.shape[:2]
@@ -50,7 +51,7 @@ def attention(q, k, v, table, index, scale, go=None, glse=None):
     out = P @ v64
     r = {"out": out, "lse": torch.where(total > 0, torch.log(total) + top, 0.0)[..., 0]}
     spread = P @ v64.abs()
-    bound = {"out": u * out.abs() + (u + f) * spread + grain + 2.0 ** -15 * grain * v64.abs().sum(2, keepdim=True), "lse": 2.0 ** -15 + r["lse"].abs() * 2.0 ** -20}
+    bound = {"out": u * out.abs() + (u + f) * spread + grain + 2.0 ** -7 * grain * v64.abs().sum(2, keepdim=True), "lse": 2.0 ** -15 + r["lse"].abs() * 2.0 ** -20}
     if go is None:
         return r, bound
     g64 = clean(go, allowed.any(2))
