@@ -44,7 +44,7 @@ struct FwdParams {
   int64_t qs[3], ks[3], vs[3], os[3];
   int64_t index_step, any_step;  // from one batch entry to the next (0: shared)
   float slog;                    // scale * log2(e)
-  int H, KV, G, Nq, Nk, D, S, TQ, TK, K, table_dtype;
+  int B, H, KV, G, Nq, Nk, D, S, TQ, TK, K, table_dtype;
   int packed;    // the columns are the queries of all heads of a key head
   int UH;        // heads of the units: H, or KV when packed
   int CT;        // workgroups per (batch, unit head) and split
@@ -58,8 +58,8 @@ struct Column {
   int h, i;
   bool in;
 };
-__device__ __forceinline__ Unit unit_of(const FwdParams& p, int64_t unit) {
-  return unit_of(unit, p.UH, p.packed ? 1 : p.G, p.CT);
+__device__ __forceinline__ Unit unit_of(const FwdParams& p, uint32_t unit) {
+  return unit_of(unit, p.B, p.UH, p.packed ? 1 : p.G, p.CT);
 }
 __device__ __forceinline__ Column column_of(const FwdParams& p, const Unit& u, int c) {
   Column r;
@@ -103,7 +103,7 @@ constexpr float shift_bits() {
 
 
 template <typename T>
-__device__ __forceinline__ void store_stats(const FwdParams& p, const Column& c, int64_t B, float m, float l) {
+__device__ __forceinline__ void store_stats(const FwdParams& p, const Column& c, float m, float l) {
   l *= __is_same(T, _Float16) ? 1.0f / 128.0f : 1.0f;  // 2^-shift_bits
   const int64_t at = (c.b * p.H + c.h) * p.Nq + c.i;
   if (p.stats) {
@@ -114,7 +114,7 @@ __device__ __forceinline__ void store_stats(const FwdParams& p, const Column& c,
       inv = fast_exp2(to - m) / l;
     }
     p.stats[at] = l > 0.0f ? to : 0.0f;
-    p.stats[B * p.H * p.Nq + at] = inv;
+    p.stats[int64_t(p.B) * p.H * p.Nq + at] = inv;
   }
   if (p.lse) p.lse[at] = l > 0.0f ? (m + __log2f(l)) * kLn2 : l;
 }
@@ -133,9 +133,9 @@ __global__ void __launch_bounds__(64 * W, fwd_waves(DP, W, PACKED)) bucket_attn_
   constexpr int kBytes = kTile * DP * 2;
   __shared__ __attribute__((aligned(1024))) char s_tiles[4 * kBytes];  // K and V of two tiles
   __shared__ float s_table[(PACKED ? 32 : 1) * kPitch];
-  const int64_t id = xcd_order(blockIdx.x, gridDim.x);
+  const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
   if (id >= p.units * p.splits) return;
-  const int64_t unit = id / p.splits;
+  const uint32_t unit = id / uint32_t(p.splits);
   const int split = int(id - unit * p.splits);
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -145,43 +145,17 @@ __global__ void __launch_bounds__(64 * W, fwd_waves(DP, W, PACKED)) bucket_attn_
   const Column me = column_of(p, of, ct * 32 * W + wave * 32 + (lane & 31));
   const int kv = PACKED ? uh : uh / p.G;
 
-  load_tables(s_table, p.table, p.table_dtype, p.K, p.H, PACKED ? uh * p.G : uh, PACKED ? p.G : 1, 64 * W);
   const float* table = PACKED ? s_table + (me.h - uh * p.G) * kPitch : s_table;
   const LaneReads<T, DP> reads(lane);
-
-  // the query tiles of the unit's columns, and which of the lane's queries have a key among this split's
+  // the query tiles of the unit's columns
   const int qt0 = PACKED ? 0 : (ct * 32 * W) / kTile;
   const bool two = !PACKED && W == 4 && qt0 + 1 < p.TQ;
   const int t0 = split * p.tiles_per_split, t1 = min(p.TK, t0 + p.tiles_per_split);
   const uint64_t* any = p.key_any + b * p.any_step + int64_t(qt0) * p.TK;
-  uint64_t used = union_of(p.query_any + b * p.any_step, p.TQ, qt0, t0, t1);
-  if (two) {
-    const uint64_t second = union_of(p.query_any + b * p.any_step, p.TQ, qt0 + 1, t0, t1);
-    if (wave >= 2) used = second;
-  }
-  const bool mine = me.in && ((used >> (me.i & 63)) & 1);
-
-  Op qb[NK];
-  const T* gq = static_cast<const T*>(p.q) + me.b * p.qs[0] + me.h * p.qs[1] + me.i * p.qs[2];
-#pragma unroll
-  for (int kk = 0; kk < NK; ++kk) {
-    const int d = 16 * kk + 8 * half;
-    if (mine && d < p.D) {
-      qb[kk] = *reinterpret_cast<const Op*>(gq + d);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) qb[kk][e] = T(0.0f);
-    }
-  }
   const uint8_t* codes = p.index + me.b * p.index_step + int64_t(me.i) * p.S + 16 * half;
   const char* gk = reinterpret_cast<const char*>(static_cast<const T*>(p.k) + b * p.ks[0] + kv * p.ks[1]);
   const char* gv = reinterpret_cast<const char*>(static_cast<const T*>(p.v) + b * p.vs[0] + kv * p.vs[1]);
   const unsigned kstride = unsigned(p.ks[2]) * 2, vstride = unsigned(p.vs[2]) * 2;
-
-  mf_f32x16 acc[ND];
-#pragma unroll
-  for (int n = 0; n < ND; ++n) acc[n] = zeros16();
-  float m = -INFINITY, l = 0.0f, limit = -INFINITY;
 
   const TileCopy<DP, W> kcopy(kstride, p.D, wave, lane), vcopy(vstride, p.D, wave, lane);
   auto load = [&](int tile, uint64_t set, char* to, uint4 (&w)[2]) {
@@ -197,6 +171,35 @@ __global__ void __launch_bounds__(64 * W, fwd_waves(DP, W, PACKED)) bucket_attn_
   uint4 next[2];
   bool more = tiles.next(tile, set);
   if (more) load(tile, set, s_tiles, next);
+
+  // while the first tile is on its way: the tables, the lane's query, and which queries have a key among this split's
+  const T* gq = static_cast<const T*>(p.q) + me.b * p.qs[0] + me.h * p.qs[1] + me.i * p.qs[2];
+  Op qb[NK];
+#pragma unroll
+  for (int kk = 0; kk < NK; ++kk) {
+    const int d = 16 * kk + 8 * half;
+    qb[kk] = *reinterpret_cast<const Op*>(gq + (d < p.D ? d : 0));
+  }
+  uint64_t used = union_of(p.query_any + b * p.any_step, p.TQ, qt0, t0, t1);
+  if (two) {
+    const uint64_t second = union_of(p.query_any + b * p.any_step, p.TQ, qt0 + 1, t0, t1);
+    if (wave >= 2) used = second;
+  }
+  load_tables(s_table, p.table, p.table_dtype, p.K, p.H, PACKED ? uh * p.G : uh, PACKED ? p.G : 1, 64 * W);
+  const bool mine = me.in && ((used >> (me.i & 63)) & 1);
+#pragma unroll
+  for (int kk = 0; kk < NK; ++kk) {
+    if (!mine || 16 * kk + 8 * half >= p.D) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) qb[kk][e] = T(0.0f);
+    }
+  }
+  mf_f32x16 acc[ND];
+#pragma unroll
+  for (int n = 0; n < ND; ++n) acc[n] = zeros16();
+  float m = -INFINITY, l = 0.0f, limit = -INFINITY;
+
+
   while (more) {
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's copies into LDS have landed
     __syncthreads();
@@ -252,7 +255,7 @@ __global__ void __launch_bounds__(64 * W, fwd_waves(DP, W, PACKED)) bucket_attn_
   l = pair_sum(l);
   if (!me.in) return;
   if (p.splits > 1) {
-    const int64_t at = (unit * p.splits + split) * (32 * W) + wave * 32 + (lane & 31);
+    const int64_t at = int64_t(id) * (32 * W) + wave * 32 + (lane & 31);
     float* o = p.part_out + at * DP;
 #pragma unroll
     for (int n = 0; n < ND; ++n)
@@ -276,7 +279,7 @@ __global__ void __launch_bounds__(64 * W, fwd_waves(DP, W, PACKED)) bucket_attn_
       for (int e = 0; e < 8; ++e) y[e] = acc[n][8 * u + e] * inv;
       store_row<T>(p, me, d0, y);
     }
-  if (half == 0) store_stats<T>(p, me, p.units / (int64_t(p.UH) * p.CT), m, l);
+  if (half == 0) store_stats<T>(p, me, m, l);
 }
 
 // Joins the splits: a workgroup per column, a quarter of the splits a wave (or as many waves as there are splits for),
@@ -285,14 +288,14 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(256) bucket_join_kernel(FwdParams p, int columns, int in_use) {
   constexpr int L = DP / 8, SG = 64 / L;
   __shared__ float s_m[4], s_l[4], s_y[4][DP];
-  const int64_t unit = blockIdx.x / in_use;
+  const uint32_t unit = blockIdx.x / uint32_t(in_use);
   const int c = int(blockIdx.x - unit * in_use);
   const Unit of = unit_of(p, unit);
   const Column me = column_of(p, of, of.tile * columns + c);
   if (!me.in) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const float* ml = p.part_ml + (unit * p.splits * columns + c) * 2;
-  const float* po = p.part_out + (unit * p.splits * columns + c) * DP;
+  const float* ml = p.part_ml + (int64_t(unit) * p.splits * columns + c) * 2;
+  const float* po = p.part_out + (int64_t(unit) * p.splits * columns + c) * DP;
   const int64_t step = columns;
   float m = -INFINITY, l = 0.0f;
   for (int s = tid; s < p.splits; s += 256) m = fmaxf(m, ml[s * step * 2]);
@@ -338,7 +341,7 @@ __global__ void __launch_bounds__(256) bucket_join_kernel(FwdParams p, int colum
   for (int e = 0; e < 8; ++e)
     y[e] = ((s_y[0][d0 + e] + s_y[1][d0 + e]) + (s_y[2][d0 + e] + s_y[3][d0 + e])) * inv;
   if (d0 < p.D) store_row<T>(p, me, d0, y);
-  if (tid == 0) store_stats<T>(p, me, p.units / (int64_t(p.UH) * p.CT), m, l);
+  if (tid == 0) store_stats<T>(p, me, m, l);
 }
 
 namespace {
@@ -477,6 +480,7 @@ extern "C" int mf_bucket_attn(const mf_bucket_attn_args* a, void* stream) {
     p.os[n] = a->out_stride[n];
   }
   p.slog = a->scale * kLog2e;
+  p.B = a->batch;
   p.H = a->heads;
   p.KV = a->kv_heads;
   p.G = a->heads / a->kv_heads;

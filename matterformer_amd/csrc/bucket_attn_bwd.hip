@@ -269,13 +269,13 @@ __global__ void __launch_bounds__(64 * W, (DP == 128 && (KEYS || W == 2)) || (W 
   __shared__ float s_table[kPitch];
   extern __shared__ float s_bins[];  // SUMS: [K + 1][64 W], the last one of masked pairs
   static_assert(KEYS || !SUMS, "the table's gradient is the keys' kernel's");
-  const int64_t in_order = xcd_order(blockIdx.x, gridDim.x);
+  const uint32_t in_order = xcd_order(blockIdx.x, gridDim.x);
   if (in_order >= p.units * p.pieces) return;
-  const int64_t id = in_order / p.pieces;
+  const uint32_t id = in_order / uint32_t(p.pieces);
   const int piece = int(in_order - id * p.pieces);
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Unit of = unit_of(id, KEYS ? p.KV : p.H, KEYS ? 1 : p.G, p.CT);
+  const Unit of = unit_of(id, p.B, KEYS ? p.KV : p.H, KEYS ? 1 : p.G, p.CT);
   const int uh = of.head, ct = of.tile;
   const int64_t b = of.b;
   const int kv = KEYS ? uh : uh / p.G;
@@ -291,13 +291,6 @@ __global__ void __launch_bounds__(64 * W, (DP == 128 && (KEYS || W == 2)) || (W 
   const uint64_t* by_row = (KEYS ? p.query_any : p.key_any) + b * p.any_step;  // rows of it: column tiles
   const int c0 = ct * 32 * W / kTile, col_tiles = KEYS ? p.TK : p.TQ;
   const bool two = W == 4 && c0 + 1 < col_tiles;
-  uint64_t used = union_of(by_col, col_tiles, c0, 0, rows);
-  if (two) {
-    const uint64_t second = union_of(by_col, col_tiles, c0 + 1, 0, rows);
-    if (wave >= 2) used = second;
-  }
-  const bool mine = in && ((used >> (at & 63)) & 1);
-
   // columns: (K, V) or (Q, go), zeros where there is no partner
   Op bx[NK], by[NK];
   const T* gx = KEYS ? static_cast<const T*>(p.k) + b * p.ks[0] + kv * p.ks[1] + at * p.ks[2]
@@ -307,10 +300,18 @@ __global__ void __launch_bounds__(64 * W, (DP == 128 && (KEYS || W == 2)) || (W 
 #pragma unroll
   for (int kk = 0; kk < NK; ++kk) {
     const int d = 16 * kk + 8 * half;
-    if (mine && d < p.D) {
-      bx[kk] = *reinterpret_cast<const Op*>(gx + d);
-      by[kk] = *reinterpret_cast<const Op*>(gy + d);
-    } else {
+    bx[kk] = *reinterpret_cast<const Op*>(gx + (d < p.D ? d : 0));
+    by[kk] = *reinterpret_cast<const Op*>(gy + (d < p.D ? d : 0));
+  }
+  uint64_t used = union_of(by_col, col_tiles, c0, 0, rows);
+  if (two) {
+    const uint64_t second = union_of(by_col, col_tiles, c0 + 1, 0, rows);
+    if (wave >= 2) used = second;
+  }
+  const bool mine = in && ((used >> (at & 63)) & 1);
+#pragma unroll
+  for (int kk = 0; kk < NK; ++kk) {
+    if (!mine || 16 * kk + 8 * half >= p.D) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) bx[kk][e] = by[kk][e] = T(0.0f);
     }
@@ -370,21 +371,21 @@ __global__ void __launch_bounds__(64 * W, (DP == 128 && (KEYS || W == 2)) || (W 
     const int t0 = max(0, piece * p.per_piece - g * rows), t1 = min(rows, (piece + 1) * p.per_piece - g * rows);
     const int64_t slots = int64_t(p.B) * p.CT * p.pieces;
     float* slot = SUMS ? p.parts + int64_t(kv * p.G + g) * p.K * slots + (b * p.CT + ct) * p.pieces + piece : nullptr;
-    if (t0 >= t1) {  // none of this head's rows in the piece
-      if (SUMS && int(threadIdx.x) < p.K) slot[threadIdx.x * slots] = 0.0f;
-      continue;
-    }
     side(KEYS ? kv * p.G + g : uh);
-    load_tables(s_table, p.table, p.table_dtype, p.K, p.H, KEYS ? kv * p.G + g : uh, 1, 64 * W);
-    if constexpr (SUMS)
-      for (int c = 0; c <= p.K; ++c) s_bins[c * 64 * W + threadIdx.x] = 0.0f;
     Tiles tiles(by_row + int64_t(c0) * rows, two ? by_row + int64_t(c0 + 1) * rows : nullptr, t0, t1);
     int tile = 0, buffer = 0;
     uint64_t set = 0;
     uint4 next[2];
     BlockSums<SUMS> sums(s_bins + threadIdx.x, 64 * W, p.K);
     bool more = tiles.next(tile, set);
-    if (more) load(tile, set, 0, next);
+    if (!more) {  // no pair
+      if (SUMS && int(threadIdx.x) < p.K) slot[threadIdx.x * slots] = 0.0f;
+      continue;
+    }
+    load(tile, set, 0, next);
+    load_tables(s_table, p.table, p.table_dtype, p.K, p.H, KEYS ? kv * p.G + g : uh, 1, 64 * W);
+    if constexpr (SUMS)
+      for (int c = 0; c <= p.K; ++c) s_bins[c * 64 * W + threadIdx.x] = 0.0f;
     __syncthreads();  // the table and the sums
     while (more) {
       __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's copies into LDS have landed
@@ -491,7 +492,7 @@ __global__ void __launch_bounds__(64 * W, (DP == 128 && (KEYS || W == 2)) || (W 
   const float fx = KEYS ? down : down * (kHalf ? cinv * (1.0f / kProb) : cinv), fy = kHalf ? 1.0f / kProb : 1.0f;
   if (!KEYS) total = pair_sum(total) * (kHalf ? cinv * (1.0f / kProb) : cinv);
   if (!in) return;
-  const int64_t place = in_order * (32 * W) + wave * 32 + (lane & 31);  // pieces > 1
+  const int64_t place = int64_t(in_order) * (32 * W) + wave * 32 + (lane & 31);  // pieces > 1
   T* ox = KEYS ? static_cast<T*>(p.dk) + b * p.dks[0] + kv * p.dks[1] + at * p.dks[2]
                : static_cast<T*>(p.dq) + b * p.dqs[0] + uh * p.dqs[1] + at * p.dqs[2];
   T* oy = static_cast<T*>(p.dv) + b * p.dvs[0] + kv * p.dvs[1] + at * p.dvs[2];
@@ -530,7 +531,7 @@ __global__ void __launch_bounds__(256) bucket_bwd_join_kernel(BwdParams p, int c
   const int part = int(id % L), c = int(id / L % columns);
   const int64_t unit = id / L / columns;
   if (unit >= p.units) return;
-  const Unit of = unit_of(unit, KEYS ? p.KV : p.H, KEYS ? 1 : p.G, p.CT);
+  const Unit of = unit_of(unit, p.B, KEYS ? p.KV : p.H, KEYS ? 1 : p.G, p.CT);
   const int uh = of.head, ct = of.tile;
   const int64_t b = of.b;
   const int at = ct * columns + c, d0 = part * 8 % DP;
