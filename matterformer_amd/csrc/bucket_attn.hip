@@ -59,7 +59,7 @@ struct Column {
   bool in;
 };
 __device__ __forceinline__ Unit unit_of(const FwdParams& p, uint32_t unit) {
-  return unit_of(unit, p.B, p.UH, p.packed ? 1 : p.G, p.CT);
+  return unit_of(unit, p.B, p.UH, p.packed ? 1 : p.G, p.CT, false);
 }
 __device__ __forceinline__ Column column_of(const FwdParams& p, const Unit& u, int c) {
   Column r;
@@ -213,13 +213,20 @@ __global__ void __launch_bounds__(64 * W, fwd_waves(DP, W, PACKED)) bucket_attn_
     float top = -INFINITY;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
+      const uint32_t word[4] = {w[kb].x, w[kb].y, w[kb].z, w[kb].w};
+      Op ka[NK];
+      float bias[16];
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) ka[kk] = at.rows(s_tiles, kb, kk);
+#pragma unroll
+      for (int t = 0; t < 16; ++t) bias[t] = table[byte_of(word, t)];
+      __builtin_amdgcn_sched_barrier(0);
       mf_f32x16 s = zeros16();
 #pragma unroll
-      for (int kk = 0; kk < NK; ++kk) s = Mma32<T>::mma(at.rows(s_tiles, kb, kk), qb[kk], s);
-      const uint32_t word[4] = {w[kb].x, w[kb].y, w[kb].z, w[kb].w};
+      for (int kk = 0; kk < NK; ++kk) s = Mma32<T>::mma(ka[kk], qb[kk], s);
 #pragma unroll
       for (int t = 0; t < 16; ++t) {
-        x[kb][t] = fmaf(s[t], p.slog, table[byte_of(word, t)]);
+        x[kb][t] = fmaf(s[t], p.slog, bias[t]);
         top = fmaxf(top, x[kb][t]);
       }
     }
@@ -237,7 +244,12 @@ __global__ void __launch_bounds__(64 * W, fwd_waves(DP, W, PACKED)) bucket_attn_
     const float from = m == -INFINITY ? 0.0f : m;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      Op pb[2];
+      Op pb[2], va[2][ND];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int n = 0; n < ND; ++n) va[s][n] = at.columns(s_tiles + kBytes, kb, s, n);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int t = 0; t < 16; ++t) {
         // (the shift after the difference: beside a huge m it would be lost)
@@ -248,7 +260,7 @@ __global__ void __launch_bounds__(64 * W, fwd_waves(DP, W, PACKED)) bucket_attn_
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int n = 0; n < ND; ++n) acc[n] = Mma32<T>::mma(at.columns(s_tiles + kBytes, kb, s, n), pb[s], acc[n]);
+        for (int n = 0; n < ND; ++n) acc[n] = Mma32<T>::mma(va[s][n], pb[s], acc[n]);
     }
   }
 

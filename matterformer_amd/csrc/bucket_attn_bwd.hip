@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(64 * W, (DP == 128 && (KEYS || W == 2)) || (W 
   const int piece = int(in_order - id * p.pieces);
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Unit of = unit_of(id, p.B, KEYS ? p.KV : p.H, KEYS ? 1 : p.G, p.CT);
+  const Unit of = unit_of(id, p.B, KEYS ? p.KV : p.H, KEYS ? 1 : p.G, p.CT, KEYS);
   const int uh = of.head, ct = of.tile;
   const int64_t b = of.b;
   const int kv = KEYS ? uh : uh / p.G;
@@ -531,7 +531,7 @@ __global__ void __launch_bounds__(256) bucket_bwd_join_kernel(BwdParams p, int c
   const int part = int(id % L), c = int(id / L % columns);
   const int64_t unit = id / L / columns;
   if (unit >= p.units) return;
-  const Unit of = unit_of(unit, p.B, KEYS ? p.KV : p.H, KEYS ? 1 : p.G, p.CT);
+  const Unit of = unit_of(unit, p.B, KEYS ? p.KV : p.H, KEYS ? 1 : p.G, p.CT, KEYS);
   const int uh = of.head, ct = of.tile;
   const int64_t b = of.b;
   const int at = ct * columns + c, d0 = part * 8 % DP;

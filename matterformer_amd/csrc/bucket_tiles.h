@@ -206,33 +206,35 @@ __device__ __forceinline__ uint32_t xcd_order(unsigned block, unsigned grid) {
 // tile before they take the next, fewer where an XCD's share is fewer: the units of an XCD stream few heads' rows, and
 // the tiles past a padded batch's last atoms, which have nothing to do, come in runs instead of at every second place,
 // which the hardware's dealing of workgroups to CUs would turn into idle ones (64 x 181 atoms, 44 on average: 20.6 and
-// 33.6 us against 17.0 and 29.0).  The tiles come in eight descending sequences, so that where the work grows with the
-// tile (earlier keys only) an eighth of a head's units, which may be an XCD's, has its share of it.
+// 33.6 us against 17.0 and 29.0).  Where the work grows with the tile (earlier keys only: queries; for keys it falls), the
+// units with the most come first, and where an XCD's share is less than a key head's units, the tiles come in eight
+// sequences, so that each share has some of all.
 struct Unit {
   int64_t b;
   int head, tile;  // head: of `heads`, `inside` of them to a key head
 };
-__device__ __forceinline__ Unit unit_of(uint32_t id, uint32_t batch, uint32_t heads, uint32_t inside, uint32_t tiles) {
+__device__ __forceinline__ Unit unit_of(uint32_t id, uint32_t batch, uint32_t heads, uint32_t inside, uint32_t tiles,
+                                        bool rising) {
   const uint32_t key_heads = heads / inside, groups = batch * key_heads;
   const uint32_t block = groups >= 64 ? 8 : groups >= 8 ? groups >> 3 : 1;
   const uint32_t first = id / (block * tiles * inside) * block;
   const uint32_t r = id - first * tiles * inside, per = min(block, groups - first) * inside;
   const uint32_t i = r / per, in_tile = r - i * per;
-  const uint32_t q = tiles >> 3, longer = tiles & 7;  // `longer` sequences of q + 1 tiles, the others of q
-  uint32_t sequence = i, place = 0;
-  if (tiles > 8) {
+  uint32_t n = i;
+  if (groups < 8 && tiles > 8) {  // `longer` sequences of q + 1 tiles, the others of q
+    const uint32_t q = tiles >> 3, longer = tiles & 7;
     if (i < longer * (q + 1)) {
-      sequence = i / (q + 1);
-      place = i - sequence * (q + 1);
+      n = i / (q + 1);
+      n += (i - n * (q + 1)) * 8;
     } else {
       const uint32_t j = i - longer * (q + 1);
-      sequence = longer + j / q;
-      place = j - (sequence - longer) * q;
+      n = j / q;
+      n += longer + (j - n * q) * 8;
     }
   }
   const uint32_t in_block = in_tile / inside, group = first + in_block, b = group / key_heads;
   Unit u;
-  u.tile = int(tiles - 1 - (place * 8 + sequence));
+  u.tile = int(rising ? n : tiles - 1 - n);
   u.head = int((group - b * key_heads) * inside + in_tile - in_block * inside);
   u.b = b;
   return u;
