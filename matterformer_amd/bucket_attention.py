@@ -26,12 +26,18 @@ _TABLE_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 def _strides(t: torch.Tensor) -> tuple[int, int, int]:
     """Elements from one batch entry, head and token to the next (0 where there is only one)."""
-    return tuple(s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3]))
+    n, s = t.shape, t.stride()
+    return (s[0] if n[0] > 1 else 0, s[1] if n[1] > 1 else 0, s[2] if n[2] > 1 else 0)
+
+
+def _rows_apart(t: torch.Tensor) -> bool:
+    """A head's entries next to one another, the rest by steps that the kernels take."""
+    b, h, n = _strides(t)
+    return t.stride(3) == 1 and b % 8 == 0 and h % 8 == 0 and n % 8 == 0 and min(b, h, n) >= 0 and n < 1 << 23
 
 
 def _readable(t: torch.Tensor) -> bool:
-    return (t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 and s >= 0 for s in _strides(t))
-            and _strides(t)[2] < 1 << 23)
+    return t.data_ptr() % 16 == 0 and _rows_apart(t)
 
 
 def _operand(t: torch.Tensor) -> torch.Tensor:
@@ -44,8 +50,7 @@ def _operand(t: torch.Tensor) -> torch.Tensor:
 def _like(t: torch.Tensor) -> torch.Tensor:
     """An output in t's layout (heads of projected rows come back as such views)."""
     out = torch.empty_like(t)
-    dense = out.stride(3) == 1 and all(s % 8 == 0 for s in _strides(out)) and _strides(out)[2] < 1 << 23
-    return out if dense else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return out if _rows_apart(out) else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _arguments(q, k, v, table, buckets: PairBuckets, out, out_lo, lse, stats, scale: float):
@@ -60,7 +65,8 @@ def _arguments(q, k, v, table, buckets: PairBuckets, out, out_lo, lse, stats, sc
 
 
 def _forward(q, k, v, table, buckets, scale: float, *, lse: bool, training: bool):
-    """out, lse, and for gradients what out's rounding left and the rows' maxima and sums (None where not asked)."""
+    """out, lse, and for gradients what out's rounding left, the rows' maxima and sums and the call's arguments (None where
+    not asked)."""
     B, H, Nq, D = q.shape
     out = _like(q)
     lse_out = torch.empty(B, H, Nq, dtype=torch.float32, device=q.device) if lse else None
@@ -70,14 +76,14 @@ def _forward(q, k, v, table, buckets, scale: float, *, lse: bool, training: bool
         for t in (out, lse_out, lo, stats):
             if t is not None:
                 t.zero_()
-        return out, lse_out, lo, stats
+        return out, lse_out, lo, stats, None
     args = _arguments(q, k, v, table, buckets, out, lo, lse_out, stats, scale)
     nbytes = int(_native.lib().mf_bucket_attn_workspace_size(args))
     if nbytes > 0:
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         args.workspace, args.workspace_bytes = workspace.data_ptr(), nbytes
     _native.launch("mf_bucket_attn", args, q.device)
-    return out, lse_out, lo, stats
+    return out, lse_out, lo, stats, args
 
 
 class _BucketAttentionFunction(torch.autograd.Function):
@@ -85,9 +91,9 @@ class _BucketAttentionFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, table, buckets, scale):
-        out, lse, lo, stats = _forward(q, k, v, table, buckets, scale, lse=True, training=True)
+        out, lse, lo, stats, args = _forward(q, k, v, table, buckets, scale, lse=True, training=True)
         ctx.save_for_backward(q, k, v, table, out, lo, stats)
-        ctx.buckets, ctx.scale = buckets, scale
+        ctx.buckets, ctx.args = buckets, args
         ctx.set_materialize_grads(False)
         return out, lse
 
@@ -97,6 +103,7 @@ class _BucketAttentionFunction(torch.autograd.Function):
         if grad_out is None and grad_lse is None:
             return (None,) * 6
         q, k, v, table, out, lo, stats = ctx.saved_tensors
+        q, k, v, out = _operand(q), _operand(k), _operand(v), _operand(out)
         buckets = ctx.buckets
         go = torch.zeros_like(out) if grad_out is None else _operand(grad_out)
         gl = None if grad_lse is None else grad_lse.contiguous()
@@ -108,10 +115,13 @@ class _BucketAttentionFunction(torch.autograd.Function):
                     t.zero_()
             return dq, dk, dv, dtable, None, None
         args = _native.MfBucketAttnBwdArgs(
-            fwd=_arguments(q, k, v, table, buckets, out, lo, None, stats, ctx.scale),
-            index_t=buckets.index_t.data_ptr(), grad_out=go.data_ptr(), grad_lse=_native.ptr(gl), dq=dq.data_ptr(),
-            dk=dk.data_ptr(), dv=dv.data_ptr(), dtable=_native.ptr(dtable), grad_out_stride=_strides(go),
-            dq_stride=_strides(dq), dk_stride=_strides(dk), dv_stride=_strides(dv))
+            fwd=ctx.args, index_t=buckets.index_t.data_ptr(), grad_out=go.data_ptr(), grad_lse=_native.ptr(gl),
+            dq=dq.data_ptr(), dk=dk.data_ptr(), dv=dv.data_ptr(), dtable=_native.ptr(dtable),
+            grad_out_stride=_strides(go), dq_stride=_strides(dq), dk_stride=_strides(dk), dv_stride=_strides(dv))
+        f = args.fwd  # a copy; the saved tensors may have been moved meanwhile (saved tensor hooks), and laid out anew
+        f.q, f.k, f.v, f.table = q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr()
+        f.out, f.out_lo, f.stats = out.data_ptr(), lo.data_ptr(), stats.data_ptr()
+        f.q_stride, f.k_stride, f.v_stride, f.out_stride = _strides(q), _strides(k), _strides(v), _strides(out)
         nbytes = int(_native.lib().mf_bucket_attn_bwd_workspace_size(args))
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         args.workspace, args.workspace_bytes = workspace.data_ptr(), nbytes
@@ -185,5 +195,5 @@ def bucket_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: t
             raise ValueError("gradients need buckets made with gradients=True")
         out, lse = _BucketAttentionFunction.apply(qo, ko, vo, t, buckets, s)
     else:
-        out, lse, _, _ = _forward(qo, ko, vo, t, buckets, s, lse=return_lse, training=False)
+        out, lse, *_ = _forward(qo, ko, vo, t, buckets, s, lse=return_lse, training=False)
     return (out, lse) if return_lse else out

@@ -49,6 +49,7 @@ class PairBuckets:
         self.num_buckets = int(num_buckets)
         self.key_any = key_any
         self.query_any = query_any
+        self._laid_out = False  # as the kernels read it (check_layout)
 
     @property
     def batch(self) -> int:
@@ -312,6 +313,8 @@ def _check_table(table: torch.Tensor, buckets: PairBuckets) -> None:
 
 def check_layout(buckets: PairBuckets) -> None:
     """The kernels read the buckets by address: their types and layout."""
+    if buckets._laid_out:
+        return
     B, Nq, Nk = buckets.index.shape
     S, St = (Nk + 63) // 64 * 64, (Nq + 63) // 64 * 64
     TQ, TK = St // TILE, S // TILE
@@ -324,6 +327,7 @@ def check_layout(buckets: PairBuckets) -> None:
         ok = ok and t.dtype == torch.int64 and t.shape == shape and t.device == buckets.device and t.is_contiguous()
     if not ok:
         raise ValueError("buckets must be as distance_buckets, offset_buckets, value_buckets or index_buckets make them")
+    buckets._laid_out = True
 
 
 def table_with_masked(table: torch.Tensor) -> torch.Tensor:
