@@ -313,10 +313,12 @@ class MfBucketBiasArgs(ctypes.Structure):
 
 
 class MfBucketAttnArgs(ctypes.Structure):
+    """mf_bucket_attn_args with its strides as fields of their own (q_stride0 .. 2), as in MfRotaryArgs."""
+
     _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "table", "index", "key_any", "query_any", "out", "out_lo",
                                                "lse", "stats", "workspace")] + [
         ("workspace_bytes", ctypes.c_uint64)] + [
-        (n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] + [
+        (f"{n}{i}", ctypes.c_int64) for n in ("q_stride", "k_stride", "v_stride", "out_stride") for i in range(3)] + [
         ("scale", ctypes.c_float)] + [
         (n, ctypes.c_int32) for n in ("index_batch", "batch", "heads", "kv_heads", "queries", "keys", "head_dim",
                                       "buckets", "dtype", "table_dtype")]
@@ -326,7 +328,7 @@ class MfBucketAttnBwdArgs(ctypes.Structure):
     _fields_ = [("fwd", MfBucketAttnArgs)] + [
         (n, ctypes.c_void_p) for n in ("index_t", "grad_out", "grad_lse", "dq", "dk", "dv", "dtable", "workspace")] + [
         ("workspace_bytes", ctypes.c_uint64)] + [
-        (n, ctypes.c_int64 * 3) for n in ("grad_out_stride", "dq_stride", "dk_stride", "dv_stride")]
+        (f"{n}{i}", ctypes.c_int64) for n in ("grad_out_stride", "dq_stride", "dk_stride", "dv_stride") for i in range(3)]
 
 
 _LIB: ctypes.CDLL | None = None

@@ -55,13 +55,12 @@ def _like(t: torch.Tensor) -> torch.Tensor:
 
 def _arguments(q, k, v, table, buckets: PairBuckets, out, out_lo, lse, stats, scale: float):
     B, H, Nq, D = q.shape
-    return _native.MfBucketAttnArgs(
-        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), table=table.data_ptr(), index=buckets.index.data_ptr(),
-        key_any=buckets.key_any.data_ptr(), query_any=buckets.query_any.data_ptr(), out=out.data_ptr(),
-        out_lo=_native.ptr(out_lo), lse=_native.ptr(lse), stats=_native.ptr(stats), q_stride=_strides(q),
-        k_stride=_strides(k), v_stride=_strides(v), out_stride=_strides(out), scale=scale, index_batch=buckets.batch,
-        batch=B, heads=H, kv_heads=k.shape[1], queries=Nq, keys=k.shape[2], head_dim=D, buckets=buckets.num_buckets,
-        dtype=_native.dtype_code(q.dtype), table_dtype=_native.dtype_code(table.dtype))
+    ptr = _native.ptr
+    return _native.MfBucketAttnArgs(  # in the order of the fields, which is quicker than by name
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), buckets.index.data_ptr(),
+        buckets.key_any.data_ptr(), buckets.query_any.data_ptr(), out.data_ptr(), ptr(out_lo), ptr(lse), ptr(stats), None,
+        0, *_strides(q), *_strides(k), *_strides(v), *_strides(out), scale, buckets.index.shape[0], B, H, k.shape[1], Nq,
+        k.shape[2], D, buckets.num_buckets, _native.dtype_code(q.dtype), _native.dtype_code(table.dtype))
 
 
 def _forward(q, k, v, table, buckets, scale: float, *, lse: bool, training: bool):
@@ -115,13 +114,15 @@ class _BucketAttentionFunction(torch.autograd.Function):
                     t.zero_()
             return dq, dk, dv, dtable, None, None
         args = _native.MfBucketAttnBwdArgs(
-            fwd=ctx.args, index_t=buckets.index_t.data_ptr(), grad_out=go.data_ptr(), grad_lse=_native.ptr(gl),
-            dq=dq.data_ptr(), dk=dk.data_ptr(), dv=dv.data_ptr(), dtable=_native.ptr(dtable),
-            grad_out_stride=_strides(go), dq_stride=_strides(dq), dk_stride=_strides(dk), dv_stride=_strides(dv))
+            ctx.args, buckets.index_t.data_ptr(), go.data_ptr(), _native.ptr(gl), dq.data_ptr(), dk.data_ptr(),
+            dv.data_ptr(), _native.ptr(dtable), None, 0, *_strides(go), *_strides(dq), *_strides(dk), *_strides(dv))
         f = args.fwd  # a copy; the saved tensors may have been moved meanwhile (saved tensor hooks), and laid out anew
         f.q, f.k, f.v, f.table = q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr()
         f.out, f.out_lo, f.stats = out.data_ptr(), lo.data_ptr(), stats.data_ptr()
-        f.q_stride, f.k_stride, f.v_stride, f.out_stride = _strides(q), _strides(k), _strides(v), _strides(out)
+        f.q_stride0, f.q_stride1, f.q_stride2 = _strides(q)
+        f.k_stride0, f.k_stride1, f.k_stride2 = _strides(k)
+        f.v_stride0, f.v_stride1, f.v_stride2 = _strides(v)
+        f.out_stride0, f.out_stride1, f.out_stride2 = _strides(out)
         nbytes = int(_native.lib().mf_bucket_attn_bwd_workspace_size(args))
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         args.workspace, args.workspace_bytes = workspace.data_ptr(), nbytes

@@ -3,6 +3,7 @@ entries' checks and structs."""
 
 import ctypes
 import math
+import re
 import shutil
 import subprocess
 
@@ -177,7 +178,8 @@ def test_structs_match_the_header(tmp_path):
     lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "mf_capi.h"', "int main(void) {"]
     for name, py in structs.items():
         lines.append(f'  printf("%zu\\n", sizeof({name}));')
-        lines += [f'  printf("%zu\\n", offsetof({name}, {f[0]}));' for f in py._fields_]
+        member = lambda f: re.sub(r"^(.*_stride)(\d)$", r"\1[\2]", f)  # an array's elements are fields of their own
+        lines += [f'  printf("%zu\\n", offsetof({name}, {member(f[0])}));' for f in py._fields_]
     (tmp_path / "layout.c").write_text("\n".join(lines + ["  return 0;", "}"]))
     subprocess.run([cc, f"-I{HEADER.parent}", str(tmp_path / "layout.c"), "-o", str(tmp_path / "layout")], check=True)
     got = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.split()
@@ -252,7 +254,7 @@ def test_bias_entries_refuse_before_any_device_call():
 
 
 ATTN = dict(q=FAKE, k=FAKE, v=FAKE, table=FAKE, index=FAKE, key_any=FAKE, query_any=FAKE, out=FAKE, out_lo=FAKE,
-            stats=FAKE, q_stride=(64, 64, 64), k_stride=(64, 64, 64), v_stride=(64, 64, 64), out_stride=(64, 64, 64),
+            stats=FAKE, **{f"{n}_stride{i}": 64 for n in ("q", "k", "v", "out") for i in range(3)},
             scale=0.1, index_batch=2, batch=2, heads=4, kv_heads=2, queries=100, keys=100, head_dim=64, buckets=6,
             dtype=_native.MF_DTYPE_BF16, table_dtype=0)
 ATTN_REFUSALS = [(dict(q=None), INVALID, "non-NULL"), (dict(query_any=None), INVALID, "non-NULL"),
@@ -262,8 +264,8 @@ ATTN_REFUSALS = [(dict(q=None), INVALID, "non-NULL"), (dict(query_any=None), INV
                  (dict(scale=math.nan), INVALID, "finite"), (dict(index_batch=3), INVALID, "index_batch"),
                  (dict(keys=2 ** 24 + 1), UNSUPPORTED, "2^24"), (dict(kv_heads=3), UNSUPPORTED, "divide"),
                  (dict(kv_heads=0), UNSUPPORTED, "divide"), (dict(heads=66, kv_heads=2), UNSUPPORTED, "at most 32"),
-                 (dict(k=FAKE + 8), INVALID, "aligned"), (dict(v_stride=(64, 4, 64)), INVALID, "multiples of 8"),
-                 (dict(q_stride=(64, 64, -8)), INVALID, "multiples of 8"), (dict(k_stride=(8, 8, 2 ** 23)), UNSUPPORTED, "2^23")]
+                 (dict(k=FAKE + 8), INVALID, "aligned"), (dict(v_stride1=4), INVALID, "multiples of 8"),
+                 (dict(q_stride2=-8), INVALID, "multiples of 8"), (dict(k_stride2=2 ** 23), UNSUPPORTED, "2^23")]
 
 
 def test_attention_entries_refuse_before_any_device_call():
@@ -272,7 +274,7 @@ def test_attention_entries_refuse_before_any_device_call():
 
     def backward(bwd=None, **kw):
         a = dict(fwd=forward(**kw), index_t=FAKE, grad_out=FAKE, dq=FAKE, dk=FAKE, dv=FAKE, dtable=FAKE,
-                 grad_out_stride=(64, 64, 64), dq_stride=(64, 64, 64), dk_stride=(64, 64, 64), dv_stride=(64, 64, 64))
+                 **{f"{n}_stride{i}": 64 for n in ("grad_out", "dq", "dk", "dv") for i in range(3)})
         a.update(bwd or {})
         return _native.MfBucketAttnBwdArgs(**a)
 
@@ -288,8 +290,8 @@ def test_attention_entries_refuse_before_any_device_call():
     refused(lib.mf_bucket_attn, forward(**few, workspace=FAKE, workspace_bytes=need - 1), INVALID, "workspace")
     refused(lib.mf_bucket_attn, forward(batch=2 ** 24, index_batch=1, heads=32, kv_heads=32), UNSUPPORTED, "too large")
     for bwd, status, match in ((dict(index_t=None), INVALID, "non-NULL"), (dict(dv=None), INVALID, "non-NULL"),
-                               (dict(dq=FAKE + 8), INVALID, "aligned"), (dict(dk_stride=(64, 64, 7)), INVALID, "multiples of 8"),
-                               (dict(grad_out_stride=(8, 8, 2 ** 23)), UNSUPPORTED, "2^23"), (dict(), INVALID, "workspace")):
+                               (dict(dq=FAKE + 8), INVALID, "aligned"), (dict(dk_stride2=7), INVALID, "multiples of 8"),
+                               (dict(grad_out_stride2=2 ** 23), UNSUPPORTED, "2^23"), (dict(), INVALID, "workspace")):
         refused(lib.mf_bucket_attn_bwd, backward(bwd), status, match)
     refused(lib.mf_bucket_attn_bwd, backward(stats=None), INVALID, "non-NULL")
     refused(lib.mf_bucket_attn_bwd, backward(keys=0), UNSUPPORTED, "positive")
