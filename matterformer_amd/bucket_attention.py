@@ -130,8 +130,9 @@ class _BucketAttentionFunction(torch.autograd.Function):
         return dq, dk, dv, dtable, None, None
 
 
-def bucket_attention_torch(q, k, v, table, buckets: PairBuckets, scale: float):
-    """out and lse in torch, in fp32 (fp64 operands in fp64); rows without a pair are 0."""
+def bucket_attention_torch(q, k, v, table, buckets: PairBuckets, scale: float, *, dropout: float = 0.0):
+    """out and lse in torch, in fp32 (fp64 operands in fp64); rows without a pair are 0.  ``dropout`` of the
+    probabilities."""
     wide = torch.float64 if q.dtype == torch.float64 else torch.float32
     group = q.shape[1] // k.shape[1] if k.shape[1] else 1
     k, v = (t.to(wide).repeat_interleave(group, dim=1) for t in (k, v))
@@ -143,7 +144,8 @@ def bucket_attention_torch(q, k, v, table, buckets: PairBuckets, scale: float):
     p = torch.exp(s - torch.where(torch.isinf(top), torch.zeros_like(top), top))
     total = p.sum(-1, keepdim=True)
     some = total > 0
-    out = torch.matmul(p / torch.where(some, total, torch.ones_like(total)), v)
+    p = p / torch.where(some, total, torch.ones_like(total))
+    out = torch.matmul(torch.nn.functional.dropout(p, dropout) if dropout > 0.0 else p, v)
     lse = torch.where(some, torch.log(torch.where(some, total, torch.ones_like(total))) + top, torch.zeros_like(top))
     return out.to(q.dtype), lse[..., 0].to(torch.float32)
 

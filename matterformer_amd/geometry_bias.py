@@ -21,13 +21,14 @@ torch formulation never exist.  Other modes and CPU tensors take the torch formu
 
 from __future__ import annotations
 
-from typing import Callable
+from typing import Callable, Sequence
 
 import torch
 import torch.nn.functional as F
 from torch import nn
 
 from matterformer_amd.geometry import GeometryFeatures
+from matterformer_amd.pair_buckets import bucket_bias, value_buckets
 from matterformer_amd.simplicial_types import (
     SimplicialAttentionMask,
     SimplicialFactorizedBias,
@@ -385,3 +386,35 @@ class SimplicialGeometryBias(_GeometryBiasBase):
             return bias
 
         return bias_fn
+
+
+class BucketedGeometryBias(_GeometryBiasBase):
+    """The factorized bias u, v, w of simplicial attention as tables of learned numbers by distance bucket, in the place of
+    SimplicialGeometryBias's MLPs: u_ij = u_table[bucket(d_ij), h], and so v and w, with the same noise gate.  ``edges``:
+    rising distances (in the units of the geometry adapter's pair_dist, minimum-image ones on periodic geometry), one fewer
+    than buckets; the tables (buckets, heads) start at zero and take gradients (bucket_bias)."""
+
+    def __init__(self, n_heads: int, edges: Sequence[float], use_noise_gate: bool = True) -> None:
+        super().__init__(n_heads, use_noise_gate)
+        self.edges = [float(e) for e in edges]
+        for name in ("u_table", "v_table", "w_table"):
+            self.register_parameter(name, nn.Parameter(torch.zeros(len(self.edges) + 1, self.n_heads)))
+
+    def build_structured_bias_inputs(self, geom_features: GeometryFeatures, coords_len: int,
+                                     pad_mask: torch.Tensor | None = None, seq_len: int | None = None,
+                                     sigma: torch.Tensor | None = None):
+        """(factorized_bias, None, None, None, attention_mask), as SimplicialGeometryBias gives them."""
+        T = seq_len or coords_len
+        dist = geom_features.pair_dist
+        # every pair has a bucket: which ones count is the attention mask's
+        buckets = value_buckets(dist, self.edges, gradients=False)
+        u, v, w = (self._expand_atom_head_bias(bucket_bias(t, buckets), seq_len=T)
+                   for t in (self.u_table, self.v_table, self.w_table))
+        gate = self._sigma_gate(sigma=sigma, batch_size=dist.shape[0], dtype=u.dtype, device=u.device)
+        gate = gate.expand(-1, -1, T, -1).squeeze(-1)
+        if T > coords_len:
+            gate = gate * (torch.arange(T, device=gate.device) < coords_len).to(dtype=gate.dtype).view(1, 1, T)
+        mask = build_simplicial_attention_mask(coords_len=coords_len, seq_len=T, batch_size=gate.shape[0],
+                                               device=gate.device, pad_mask=pad_mask,
+                                               geom_pair_mask=geom_features.pair_mask)
+        return SimplicialFactorizedBias(u=u, v=v, w=w, gate=gate), None, None, None, mask

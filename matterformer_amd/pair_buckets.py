@@ -390,11 +390,11 @@ def bucket_bias(table: torch.Tensor, buckets: PairBuckets, *, batch: int | None 
     if B != buckets.batch and buckets.batch != 1:
         raise ValueError(f"batch must be {buckets.batch}, got {B}")
     dtype = table.dtype if dtype is None else dtype
-    if table.dtype not in _TABLE_DTYPES or dtype not in _TABLE_DTYPES:
-        raise RuntimeError(f"bucket_bias only supports float32/float16/bfloat16, got {table.dtype} and {dtype}")
     if table.device.type != "cuda":
         bias = table_with_masked(table)[table_rows(buckets)].permute(0, 3, 1, 2).to(dtype)
         return bias.expand(B, *bias.shape[1:]).contiguous()
+    if table.dtype not in _TABLE_DTYPES or dtype not in _TABLE_DTYPES:
+        raise RuntimeError(f"bucket_bias only supports float32/float16/bfloat16, got {table.dtype} and {dtype}")
     if table.shape[1] > 128:
         raise RuntimeError(f"bucket_bias supports up to 128 heads, got {table.shape[1]}")
     _check_counts(B, buckets.queries, buckets.keys)

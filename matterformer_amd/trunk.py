@@ -13,7 +13,11 @@ configs[4] trunk alternates
                (attn.attn.in_proj_weight, ...); on the GPU: in_proj, mf_radius_attn over the kNN bit
                mask (mf_knn -> mf_knn_mask), out_proj.
 
-The kNN lists and masks are built once per forward from the coordinates and shared by the local blocks.
+A schedule may name a third type, attn_type="bucket": multi-head attention of every atom over all atoms with a learned
+bias by distance bucket, the reference's attn_type="mha" block with an attn_head_bias that is a table by bucket.
+
+The kNN lists and masks are built once per forward from the coordinates and shared by the local blocks, and so are the
+bucket blocks' buckets.
 impl="auto" runs the HIP kernels for GPU tensors (a missing library raises) and the reference's own
 torch modules for CPU tensors; impl="torch" forces the latter.
 
@@ -28,18 +32,22 @@ packed projections are scattered into (padded rows zero) and gathered back from.
 
 from __future__ import annotations
 
+from typing import Sequence
+
 import torch
 import torch.nn.functional as F
 from torch import nn
 
 from matterformer_amd import _native
+from matterformer_amd.bucket_attention import bucket_attention, bucket_attention_torch
 from matterformer_amd.gated_mlp import ACTIVATIONS, gated_linear
+from matterformer_amd.pair_buckets import MAX_BUCKETS, PairBuckets, distance_buckets
 from matterformer_amd.rotary import RotaryFrequencies, check_layout, rotary_heads, rotary_heads_torch
 from matterformer_amd.simplicial_attention import SimplicialAttention
 from matterformer_amd.simplicial_types import SimplicialAttentionMask, coerce_attention_mask
 from matterformer_amd.token_packing import TokenPacking, adaln_rows
 
-ATTN_TYPES = ("simplicial", "knn_local")
+ATTN_TYPES = ("simplicial", "knn_local", "bucket")
 
 
 def _modulate(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
@@ -319,6 +327,86 @@ class KnnLocalAttention(nn.Module):
         return out
 
 
+class BucketAttention(nn.Module):
+    """MHA of every atom over all atoms with a learned bias by distance bucket (bucket_attention): ``bias_table``
+    (num_buckets, heads), zeros at first, beside nn.MultiheadAttention's parameters, held as ``attn`` like the reference's
+    RegularAttention (regular_attention.py:275-338).
+
+    impl="auto" runs the HIP kernels, training too, for GPU tensors whose projections are 16-bit (in inference fp32
+    projections as well, their core in bfloat16) and the torch formulation otherwise."""
+
+    def __init__(self, d_model: int, n_heads: int, num_buckets: int, *, dropout: float = 0.0, impl: str = "auto") -> None:
+        super().__init__()
+        impl = impl.lower()
+        if impl == "hip":
+            impl = "triton"
+        if impl not in {"auto", "torch", "triton"}:
+            raise ValueError(f"Unsupported bucket attention impl: {impl}")
+        if not 1 <= int(num_buckets) <= MAX_BUCKETS:
+            raise ValueError(f"num_buckets must be in [1, {MAX_BUCKETS}], got {num_buckets}")
+        self.impl = impl
+        self.attn = nn.MultiheadAttention(d_model, n_heads, dropout=dropout, batch_first=True)
+        self.bias_table = nn.Parameter(torch.zeros(int(num_buckets), n_heads))
+        self._last_impl_used = "torch"
+
+    def _hip_unavailable_reason(self, h: torch.Tensor) -> str | None:
+        if h.device.type != "cuda":
+            return "the HIP bucket attention requires GPU tensors"
+        if self.training and self.attn.dropout > 0.0:
+            return "the HIP bucket attention does not support attention dropout in training mode"
+        if _native.in_forward_mode() and _native.has_tangent(h, *self.parameters()):
+            return "the HIP bucket attention has no forward-mode derivative"
+        if self.bias_table.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            return "the HIP bucket attention needs a float32/float16/bfloat16 table"
+        if torch.is_grad_enabled() and (h.requires_grad or any(p.requires_grad for p in self.parameters())):
+            dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else h.dtype
+            if dtype not in (torch.bfloat16, torch.float16):
+                return "the HIP bucket attention's backward needs float16/bfloat16 projections"
+        head_dim = self.attn.embed_dim // self.attn.num_heads
+        if head_dim % 8 or head_dim > 128:
+            return f"the HIP bucket attention supports head_dim multiples of 8 up to 128, got {head_dim}"
+        return None
+
+    def _use_hip(self, h: torch.Tensor) -> bool:
+        if self.impl == "torch":
+            return False
+        reason = self._hip_unavailable_reason(h)
+        if reason is not None and self.impl == "triton":
+            raise RuntimeError(reason)
+        return reason is None
+
+    def forward(self, h: torch.Tensor, buckets: PairBuckets) -> torch.Tensor:
+        mha = self.attn
+        B, T, C = h.shape
+        H = mha.num_heads
+        rows = F.linear(h, mha.in_proj_weight, mha.in_proj_bias)
+        q, k, v = (t.view(B, T, H, C // H).transpose(1, 2) for t in rows.chunk(3, dim=-1))
+        if self._use_hip(h):
+            self._last_impl_used = "triton"
+            if rows.dtype not in (torch.bfloat16, torch.float16):
+                q, k, v = (t.to(torch.bfloat16) for t in (q, k, v))
+            out = bucket_attention(q, k, v, self.bias_table, buckets)
+        else:
+            self._last_impl_used = "torch"
+            p = self.attn.dropout if self.training else 0.0
+            out, _ = bucket_attention_torch(q, k, v, self.bias_table, buckets, (C // H) ** -0.5, dropout=p)
+        out = out.transpose(1, 2).reshape(B, T, C).to(rows.dtype)
+        return F.linear(out, mha.out_proj.weight, mha.out_proj.bias)
+
+    def forward_packed(self, hp: torch.Tensor, buckets: PairBuckets, packing: TokenPacking) -> torch.Tensor:
+        """The HIP path on packed rows: in_proj on (T, C), the kernel over the padded head layout, out_proj."""
+        if not self._use_hip(hp):
+            raise RuntimeError("packed bucket attention runs on the HIP kernels only")
+        self._last_impl_used = "triton"
+        mha = self.attn
+        H = mha.num_heads
+        rows = F.linear(hp, mha.in_proj_weight, mha.in_proj_bias)
+        cdt = rows.dtype if rows.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
+        q, k, v = packing.to_heads(rows, 3, H, hp.shape[-1] // H, cdt)
+        out = bucket_attention(q, k, v, self.bias_table, buckets)
+        return F.linear(packing.from_heads(out, hp.dtype), mha.out_proj.weight, mha.out_proj.bias)
+
+
 class SimplicialTerms:
     """The simplicial blocks' shared inputs: attention mask and the optional logit / message terms (the
     reference trunk builds them once per forward, transformer.py:1261-1296)."""
@@ -404,6 +492,8 @@ class AdaLNBlock(nn.Module):
         local_rotary: RotaryFrequencies | None = None,
         local_rotary_layout: str = "half",
         local_hip_backward: bool = False,
+        num_buckets: int | None = None,
+        bucket_impl: str = "auto",
     ) -> None:
         super().__init__()
         attn_type = attn_type.lower()
@@ -426,6 +516,10 @@ class AdaLNBlock(nn.Module):
             self.attn = KnnLocalAttention(d_model, self.n_heads, dropout=attn_dropout, impl=local_impl,
                                           rotary=local_rotary, rotary_layout=local_rotary_layout,
                                           hip_backward=local_hip_backward)
+        elif attn_type == "bucket":
+            if num_buckets is None:
+                raise ValueError("a bucket block needs num_buckets")
+            self.attn = BucketAttention(d_model, self.n_heads, num_buckets, dropout=attn_dropout, impl=bucket_impl)
         else:
             self.attn = SimplicialAttention(
                 dim=d_model, num_heads=self.n_heads, head_dim=simplicial_head_dim, dropout=attn_dropout,
@@ -438,7 +532,7 @@ class AdaLNBlock(nn.Module):
                 knn_mask: KnnLocalMask | None = None,
                 simplicial_attention_mask: SimplicialAttentionMask | None = None,
                 simplicial_factorized_bias=None, simplicial_angle_residual=None, simplicial_message_residual=None,
-                simplicial_logit_bias_fn=None) -> torch.Tensor:
+                simplicial_logit_bias_fn=None, pair_buckets: PairBuckets | None = None) -> torch.Tensor:
         if self.use_adaln_conditioning:
             if cond_emb is None or cond_emb.ndim != 2 or cond_emb.shape[-1] != x.shape[-1]:
                 raise ValueError(f"cond_emb must have shape (B, {x.shape[-1]})")
@@ -450,6 +544,10 @@ class AdaLNBlock(nn.Module):
             if knn_mask is None:
                 raise ValueError("a knn_local block needs knn_mask")
             attn_out = self.attn(h, knn_mask, pad_mask)
+        elif self.attn_type == "bucket":
+            if pair_buckets is None:
+                raise ValueError("a bucket block needs pair_buckets")
+            attn_out = self.attn(h, pair_buckets)
         else:
             attn_out = self.attn(h, key_padding_mask=pad_mask, attention_mask=simplicial_attention_mask,
                                  factorized_bias=simplicial_factorized_bias, angle_residual=simplicial_angle_residual,
@@ -468,27 +566,32 @@ class AdaLNBlock(nn.Module):
         return self.ada_ln(cond_emb).contiguous()
 
     def _attention_packed(self, h: torch.Tensor, packing: TokenPacking, knn_mask: KnnLocalMask | None,
-                          terms: "SimplicialTerms | None") -> torch.Tensor:
+                          terms: "SimplicialTerms | None", pair_buckets: PairBuckets | None = None) -> torch.Tensor:
         if self.attn_type == "knn_local":
             if knn_mask is None:
                 raise ValueError("a knn_local block needs knn_mask")
             return self.attn.forward_packed(h, knn_mask, packing)
+        if self.attn_type == "bucket":
+            if pair_buckets is None:
+                raise ValueError("a bucket block needs pair_buckets")
+            return self.attn.forward_packed(h, pair_buckets, packing)
         if terms is None or terms.attention_mask is None:
             raise ValueError("a packed simplicial block needs the attention mask of the compact batch")
         return _simplicial_packed(self.attn, h, packing, terms)
 
     def forward_packed(self, xp: torch.Tensor, cond_emb: torch.Tensor | None, packing: TokenPacking, *,
-                       knn_mask: KnnLocalMask | None = None, terms: "SimplicialTerms | None" = None) -> torch.Tensor:
-        """forward on the valid rows (T, C) of a batch (TokenPacking); masks and simplicial terms in the packing's
+                       knn_mask: KnnLocalMask | None = None, terms: "SimplicialTerms | None" = None,
+                       pair_buckets: PairBuckets | None = None) -> torch.Tensor:
+        """forward on the valid rows (T, C) of a batch (TokenPacking); masks, buckets and simplicial terms in the packing's
         compact layout.  The same operations in the same dtypes as forward."""
         if not self.use_adaln_conditioning:
             h = self.norm1(xp)
-            xp = xp + self._attention_packed(h, packing, knn_mask, terms)
+            xp = xp + self._attention_packed(h, packing, knn_mask, terms, pair_buckets)
             return xp + self.mlp(self.norm2(xp))
         C = xp.shape[-1]
         mods = self._mods(cond_emb, packing.batch)
         h = adaln_rows(packing, xp, shift=mods[:, :C], scale=mods[:, C:2 * C], eps=self.norm1.eps)
-        a = self._attention_packed(h, packing, knn_mask, terms)
+        a = self._attention_packed(h, packing, knn_mask, terms, pair_buckets)
         xp, h = adaln_rows(packing, xp, a, gate=mods[:, 2 * C:3 * C], shift=mods[:, 3 * C:4 * C],
                            scale=mods[:, 4 * C:5 * C], eps=self.norm2.eps)
         return adaln_rows(packing, xp, self.mlp(h), gate=mods[:, 5 * C:])
@@ -497,7 +600,9 @@ class AdaLNBlock(nn.Module):
 class AlternatingTrunk(nn.Module):
     """n_layers AdaLN blocks, simplicial on even and kNN-local (k = knn_k) on odd layers by default.  ``mlp_gate``: the
     blocks' MLPs gated by that activation (Mlp); ``local_rotary``, ``local_rotary_layout``, ``local_hip_backward``: the
-    local blocks' rotary positions and training on the HIP kernels (KnnLocalAttention)."""
+    local blocks' rotary positions and training on the HIP kernels (KnnLocalAttention).  ``bucket_edges`` (rising
+    distances, one fewer than buckets), ``bucket_cutoff``, ``bucket_impl``: of the "bucket" blocks that the schedule names
+    (BucketAttention)."""
 
     def __init__(self, d_model: int = 512, n_heads: int = 8, n_layers: int = 12, *, mlp_ratio: float = 4.0,
                  knn_k: int = 32, schedule: list[str] | None = None, simplicial_impl: str = "auto",
@@ -506,7 +611,9 @@ class AlternatingTrunk(nn.Module):
                  eps: float = 1e-6, use_adaln_conditioning: bool = True, geometry_adapter: nn.Module | None = None,
                  simplicial_geometry_bias: nn.Module | None = None, pack_tokens: bool = True,
                  mlp_gate: str | None = None, local_rotary: RotaryFrequencies | None = None,
-                 local_rotary_layout: str = "half", local_hip_backward: bool = False) -> None:
+                 local_rotary_layout: str = "half", local_hip_backward: bool = False,
+                 bucket_edges: Sequence[float] | None = None, bucket_cutoff: float | None = None,
+                 bucket_impl: str = "auto") -> None:
         super().__init__()
         self.pack_tokens = bool(pack_tokens)
         # registered before the blocks, as in TransformerTrunk.__init__ (transformer.py:1137-1139)
@@ -516,6 +623,10 @@ class AlternatingTrunk(nn.Module):
             schedule = ["simplicial" if layer % 2 == 0 else "knn_local" for layer in range(n_layers)]
         if len(schedule) != n_layers:
             raise ValueError("schedule must name one attention type per layer")
+        if "bucket" in schedule and bucket_edges is None:
+            raise ValueError("bucket blocks need bucket_edges")
+        self.bucket_edges = None if bucket_edges is None else [float(e) for e in bucket_edges]
+        self.bucket_cutoff = bucket_cutoff
         self.knn_k = int(knn_k)
         self.schedule = list(schedule)
         self.blocks = nn.ModuleList([
@@ -524,7 +635,8 @@ class AlternatingTrunk(nn.Module):
                        simplicial_message_rank=simplicial_message_rank,
                        simplicial_content_logits=simplicial_content_logits, local_impl=local_impl,
                        use_adaln_conditioning=use_adaln_conditioning, mlp_gate=mlp_gate, local_rotary=local_rotary,
-                       local_rotary_layout=local_rotary_layout, local_hip_backward=local_hip_backward)
+                       local_rotary_layout=local_rotary_layout, local_hip_backward=local_hip_backward,
+                       num_buckets=None if bucket_edges is None else len(bucket_edges) + 1, bucket_impl=bucket_impl)
             for t in self.schedule])
 
     def _use_hip(self, x: torch.Tensor) -> bool:
@@ -547,7 +659,7 @@ class AlternatingTrunk(nn.Module):
             a = block.attn
             if a.impl == "torch":
                 return False
-            if block.attn_type == "knn_local":
+            if block.attn_type in ("knn_local", "bucket"):
                 if a._hip_unavailable_reason(x) is not None:
                     return False
             elif a._triton_unavailable_reason(
@@ -557,6 +669,12 @@ class AlternatingTrunk(nn.Module):
                     logit_bias_fn=t.logit_bias_fn, return_attn=False) is not None:
                 return False
         return True
+
+    def _pair_buckets(self, coords: torch.Tensor, pad_mask: torch.Tensor | None) -> PairBuckets | None:
+        """The bucket blocks' buckets, built once per forward."""
+        if "bucket" not in self.schedule:
+            return None
+        return distance_buckets(coords, self.bucket_edges, pad_mask=pad_mask, cutoff=self.bucket_cutoff)
 
     def simplicial_terms(self, coords: torch.Tensor, pad_mask: torch.Tensor | None = None,
                          lattice: torch.Tensor | None = None, sigma: torch.Tensor | None = None
@@ -604,6 +722,7 @@ class AlternatingTrunk(nn.Module):
             mask = build_knn_mask(coords, self.knn_k, pad_mask, use_hip=self._use_hip(x),
                                   with_tables=self._trains_local(x))
         kwargs = terms.block_kwargs() if terms is not None else {}
+        kwargs["pair_buckets"] = self._pair_buckets(coords, pad_mask)
         # transformer.py:1298-1316: padded atoms are zeroed before every block and in the output
         for block in self.blocks:
             if pad_mask is not None:
@@ -639,13 +758,14 @@ class AlternatingTrunk(nn.Module):
         if "knn_local" in self.schedule:
             mask = build_knn_mask(packing.compact(coords.float()), self.knn_k, cpad, use_hip=True,
                                   with_tables=self._trains_local(x))
+        buckets = self._pair_buckets(packing.compact(coords.float()), cpad) if "bucket" in self.schedule else None
         if terms is None:
             terms = SimplicialTerms(coerce_attention_mask(None, key_padding_mask=cpad, batch_size=B, num_tokens=W,
                                                           device=x.device))
         xp = packing.pack(x)
         if not all(blk.use_adaln_conditioning for blk in self.blocks):
             for block in self.blocks:
-                xp = block.forward_packed(xp, cond_emb, packing, knn_mask=mask, terms=terms)
+                xp = block.forward_packed(xp, cond_emb, packing, knn_mask=mask, terms=terms, pair_buckets=buckets)
             return packing.unpack(xp)
         C = xp.shape[-1]
         mods = self._all_mods(cond_emb, B)
@@ -653,7 +773,7 @@ class AlternatingTrunk(nn.Module):
         h = adaln_rows(packing, xp, shift=mods[0][:, :C], scale=mods[0][:, C:2 * C], eps=blocks[0].norm1.eps)
         for layer, blk in enumerate(blocks):
             m = mods[layer]
-            a = blk._attention_packed(h, packing, mask, terms)
+            a = blk._attention_packed(h, packing, mask, terms, buckets)
             xp, h = adaln_rows(packing, xp, a, gate=m[:, 2 * C:3 * C], shift=m[:, 3 * C:4 * C],
                                scale=m[:, 4 * C:5 * C], eps=blk.norm2.eps, inplace=layer > 0)
             y = blk.mlp(h)

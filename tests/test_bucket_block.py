@@ -1,0 +1,101 @@
+"""Bucket blocks of the trunk and the bucketed simplicial bias on the CPU: construction, refusals, the torch path."""
+
+import pytest
+import torch
+
+from matterformer_amd.geometry import NonPeriodicGeometryAdapter
+from matterformer_amd.geometry_bias import BucketedGeometryBias, SimplicialGeometryBias
+from matterformer_amd.pair_buckets import distance_buckets
+from matterformer_amd.trunk import AdaLNBlock, AlternatingTrunk, BucketAttention
+
+EDGES = [0.5, 1.0, 1.5, 2.0, 3.0]
+
+
+def test_a_table_of_zeros_is_plain_attention():
+    torch.manual_seed(0)
+    attn = BucketAttention(32, 4, 6).double()
+    assert list(attn.state_dict()) == ["bias_table", "attn.in_proj_weight", "attn.in_proj_bias", "attn.out_proj.weight",
+                                       "attn.out_proj.bias"]
+    h = torch.randn(2, 9, 32, dtype=torch.float64)
+    pad = torch.zeros(2, 9, dtype=torch.bool)
+    pad[1, 6:] = True
+    buckets = distance_buckets(torch.randn(2, 9, 3), EDGES, pad_mask=pad)
+    out = attn(h, buckets)
+    want, _ = attn.attn(h, h, h, key_padding_mask=pad, need_weights=False)
+    assert torch.allclose(out[~pad], want[~pad], rtol=1e-10, atol=1e-12)
+
+
+def test_the_bias_is_the_additive_mask_of_the_reference():
+    torch.manual_seed(1)
+    attn = BucketAttention(32, 4, 6).double()
+    torch.nn.init.normal_(attn.bias_table)
+    h, coords = torch.randn(2, 7, 32, dtype=torch.float64), torch.randn(2, 7, 3)
+    buckets = distance_buckets(coords, EDGES)
+    bias = attn.bias_table[buckets.index.long()].permute(0, 3, 1, 2)
+    want, _ = attn.attn(h, h, h, need_weights=False, attn_mask=bias.reshape(8, 7, 7))
+    assert torch.allclose(attn(h, buckets), want, rtol=1e-10, atol=1e-12)
+
+
+def test_refusals():
+    for n in (0, 65):
+        with pytest.raises(ValueError, match="num_buckets"):
+            BucketAttention(32, 4, n)
+    with pytest.raises(ValueError, match="impl"):
+        BucketAttention(32, 4, 6, impl="cuda")
+    with pytest.raises(ValueError, match="num_buckets"):
+        AdaLNBlock(32, 4, attn_type="bucket")
+    with pytest.raises(ValueError, match="bucket_edges"):
+        AlternatingTrunk(32, 4, 2, schedule=["bucket", "simplicial"])
+    block = AdaLNBlock(32, 4, attn_type="bucket", num_buckets=6)
+    with pytest.raises(ValueError, match="pair_buckets"):
+        block(torch.zeros(1, 3, 32), torch.zeros(1, 32))
+    with pytest.raises(RuntimeError, match="GPU tensors"):
+        BucketAttention(32, 4, 6, impl="hip")(torch.zeros(1, 3, 32), distance_buckets(torch.zeros(1, 3, 3), EDGES))
+
+
+def test_padded_atoms_reach_nothing_and_every_parameter_trains():
+    torch.manual_seed(2)
+    trunk = AlternatingTrunk(32, 4, 3, schedule=["bucket", "simplicial", "bucket"], bucket_edges=EDGES, bucket_cutoff=4.0,
+                             simplicial_precision="ieee_fp32").double()
+    for block in trunk.blocks:
+        torch.nn.init.normal_(block.ada_ln[-1].weight, std=0.1)
+        if block.attn_type == "bucket":
+            torch.nn.init.normal_(block.attn.bias_table)
+    x, cond, coords = torch.randn(2, 8, 32, dtype=torch.float64), torch.randn(2, 32, dtype=torch.float64), torch.randn(2, 8, 3)
+    pad = torch.zeros(2, 8, dtype=torch.bool)
+    pad[0, 5:] = True
+    out = trunk(x, cond, coords, pad)
+    assert not out[0, 5:].any()
+    other = torch.where(pad[..., None], 100.0, x)
+    assert torch.allclose(trunk(other, cond, torch.where(pad[..., None], 50.0, coords), pad), out, rtol=1e-12, atol=1e-12)
+    out.square().sum().backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in trunk.parameters())
+    assert all(b.attn.bias_table.grad.abs().max() > 0 for b in trunk.blocks if b.attn_type == "bucket")
+
+
+def test_bucketed_geometry_bias():
+    torch.manual_seed(3)
+    bias = BucketedGeometryBias(4, EDGES)
+    for p in (bias.u_table, bias.v_table, bias.w_table):
+        torch.nn.init.normal_(p)
+    coords, pad = torch.randn(2, 6, 3), torch.zeros(2, 6, dtype=torch.bool)
+    pad[1, 4:] = True
+    geom = NonPeriodicGeometryAdapter()(coords=coords, pad_mask=pad)
+    sigma = torch.tensor([0.5, 2.0])
+    fb, fn, angle, message, mask = bias.build_structured_bias_inputs(geom, 6, pad, 6, sigma)
+    assert fn is None and angle is None and message is None
+    for i in range(6):
+        for j in range(6):
+            c = sum(float(geom.pair_dist[0, i, j]) >= e for e in EDGES)
+            assert torch.equal(fb.u[0, :, i, j], bias.u_table[c]) and torch.equal(fb.w[0, :, i, j], bias.w_table[c])
+    other = SimplicialGeometryBias(4).build_structured_bias_inputs(geom, 6, pad, 6, sigma)
+    assert torch.equal(fb.gate, other[0].gate) and torch.equal(mask.pair_key_valid, other[4].pair_key_valid)
+    wide = bias.build_structured_bias_inputs(geom, 6, torch.nn.functional.pad(pad, (0, 2)), 8, sigma)[0]
+    assert wide.u.shape == (2, 4, 8, 8) and torch.equal(wide.u[:, :, :6, :6], fb.u) and not wide.gate[:, :, 6:].any()
+    trunk = AlternatingTrunk(32, 4, 2, schedule=["simplicial", "bucket"], bucket_edges=EDGES,
+                             geometry_adapter=NonPeriodicGeometryAdapter(), simplicial_geometry_bias=bias,
+                             simplicial_precision="ieee_fp32")
+    for block in trunk.blocks:
+        torch.nn.init.normal_(block.ada_ln[-1].weight, std=0.1)
+    trunk(torch.randn(2, 6, 32), torch.randn(2, 32), coords, pad, sigma=sigma).square().sum().backward()
+    assert all(p.grad is not None and p.grad.abs().max() > 0 for p in bias.parameters())

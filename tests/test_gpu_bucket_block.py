@@ -1,0 +1,163 @@
+"""Bucket blocks of the trunk on the GPU: against the same modules in 64 bits, packed and padded, in training, in a graph."""
+
+import copy
+
+import pytest
+import torch
+
+from matterformer_amd.geometry import NonPeriodicGeometryAdapter, PeriodicGeometryAdapter
+from matterformer_amd.geometry_bias import BucketedGeometryBias
+from matterformer_amd.pair_buckets import distance_buckets
+from matterformer_amd.token_packing import TokenPacking
+from matterformer_amd.trunk import AlternatingTrunk, BucketAttention
+
+pytestmark = pytest.mark.gpu
+
+EDGES = [0.4 * i for i in range(1, 24)]
+
+
+def off(got, want):
+    """Error relative to the norm."""
+    got, want = got.detach().double(), want.detach().double().to(got.device)
+    return float((got - want).norm() / want.norm())
+
+
+def make_attn(cuda, d_model, heads, dtype):
+    torch.manual_seed(d_model + heads)
+    attn = BucketAttention(d_model, heads, len(EDGES) + 1)
+    torch.nn.init.normal_(attn.bias_table)
+    torch.nn.init.normal_(attn.attn.in_proj_bias, std=0.1)
+    return attn.to(cuda, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d_model,heads", [(256, 8), (384, 8), (128, 1)])
+def test_attention_module(cuda, d_model, heads, dtype):
+    attn = make_attn(cuda, d_model, heads, dtype)
+    exact = copy.deepcopy(attn).double()
+    exact.impl = "torch"
+    h = torch.randn(3, 70, d_model, device=cuda).to(dtype)
+    pad = torch.arange(70, device=cuda)[None] >= torch.tensor([[70], [41], [3]], device=cuda)
+    buckets = distance_buckets(torch.randn(3, 70, 3, device=cuda) * 3.0, EDGES, pad_mask=pad, cutoff=12.0)
+    x, y = h.clone().requires_grad_(True), h.double().requires_grad_(True)
+    got, want = attn(x, buckets), exact(y, buckets)
+    assert attn._last_impl_used == "triton" and exact._last_impl_used == "torch"
+    # a chain of at most eight roundings to the type, each half a step of what it rounds
+    u = torch.finfo(dtype).eps / 2
+    assert off(got, want) <= 8 * u
+    go = torch.randn_like(got)
+    grads = torch.autograd.grad(got, [x, *attn.parameters()], go)
+    exacts = torch.autograd.grad(want, [y, *exact.parameters()], go.double())
+    for (name, _), a, b in zip([("h", None), *attn.named_parameters()], grads, exacts):
+        assert off(a, b) <= 16 * u, name  # forward and backward
+    with torch.no_grad():
+        assert torch.equal(attn(h, buckets), got)
+
+
+def test_fp32_modules(cuda):
+    """Inference runs the core in bfloat16; training takes the torch path, autocast the kernels."""
+    attn = make_attn(cuda, 128, 2, torch.float32)
+    h = torch.randn(2, 50, 128, device=cuda)
+    buckets = distance_buckets(torch.randn(2, 50, 3, device=cuda), EDGES)
+    out = attn(h, buckets)
+    assert attn._last_impl_used == "torch"
+    with torch.no_grad():
+        assert off(attn(h, buckets), out) <= 8 * 2.0 ** -9 and attn._last_impl_used == "triton"
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        trained = attn(h, buckets)
+        assert attn._last_impl_used == "triton"
+    trained.float().square().mean().backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in attn.parameters())
+    attn.attn.dropout = 0.5
+    attn.train()(h, buckets)
+    assert attn._last_impl_used == "torch"
+    attn.impl = "triton"
+    with pytest.raises(RuntimeError, match="dropout"):
+        attn(h, buckets)
+
+
+def make_trunk(cuda, dtype, **kw):
+    torch.manual_seed(5)
+    trunk = AlternatingTrunk(256, 4, 3, schedule=["bucket", "simplicial", "bucket"], bucket_edges=EDGES, **kw)
+    for block in trunk.blocks:
+        torch.nn.init.normal_(block.ada_ln[-1].weight, std=0.05)
+        if block.attn_type == "bucket":
+            torch.nn.init.normal_(block.attn.bias_table)
+    return trunk.to(cuda, dtype)
+
+
+def batch(cuda, dtype, B=4, N=90):
+    g = torch.Generator(device=cuda).manual_seed(7)
+    x = torch.randn(B, N, 256, generator=g, device=cuda).to(dtype)
+    cond = torch.randn(B, 256, generator=g, device=cuda).to(dtype)
+    coords = torch.randn(B, N, 3, generator=g, device=cuda) * 2.0
+    pad = torch.arange(N, device=cuda)[None] >= torch.randint(20, N, (B, 1), generator=g, device=cuda)
+    return x, cond, coords, pad
+
+
+def test_trunk_packed_and_padded(cuda):
+    trunk = make_trunk(cuda, torch.bfloat16).eval()
+    x, cond, coords, pad = batch(cuda, torch.bfloat16)
+    with torch.no_grad():
+        packed = trunk(x, cond, coords, pad)
+        trunk.pack_tokens = False
+        padded = trunk(x, cond, coords, pad)
+        for block in trunk.blocks:  # the same trunk in 64 bits
+            block.attn.impl = "torch"
+        exact = trunk.double()(x.double(), cond.double(), coords, pad)
+    assert not packed[pad].any() and not padded[pad].any()
+    # three blocks of about ten roundings each
+    assert off(packed, exact) <= 30 * 2.0 ** -9 and off(padded, exact) <= 30 * 2.0 ** -9
+
+
+def test_trunk_trains(cuda):
+    """One step of everything together: buckets, their bias as simplicial terms, attention, gradients of all tables."""
+    bias = BucketedGeometryBias(4, EDGES)
+    for p in (bias.u_table, bias.v_table, bias.w_table):
+        torch.nn.init.normal_(p, std=0.3)
+    trunk = make_trunk(cuda, torch.bfloat16, geometry_adapter=NonPeriodicGeometryAdapter(), simplicial_geometry_bias=bias)
+    x, cond, coords, pad = batch(cuda, torch.bfloat16, N=60)
+    sigma = torch.tensor([0.5, 1.0, 2.0, 3.0], device=cuda)
+    exact = copy.deepcopy(trunk).cpu().double()
+    out = trunk(x, cond, coords, pad, sigma=sigma)
+    want = exact(x.cpu().double(), cond.cpu().double(), coords.cpu(), pad.cpu(), sigma=sigma.cpu())
+    assert all(b.attn._last_impl_used == "triton" for b in trunk.blocks if b.attn_type == "bucket")
+    go = torch.randn_like(out)
+    out.backward(go)
+    want.backward(go.cpu().double())
+    assert off(out, want) <= 30 * 2.0 ** -9
+    for (name, p), e in zip(trunk.named_parameters(), exact.parameters()):
+        assert p.grad is not None and torch.isfinite(p.grad).all(), name
+        if e.grad.norm() > 0 and "table" in name:
+            assert off(p.grad, e.grad) <= 60 * 2.0 ** -9, name
+
+
+def test_periodic_geometry(cuda):
+    """Minimum-image distances through the adapter's pair_dist: the bias on the GPU is that on the CPU."""
+    adapter, bias = PeriodicGeometryAdapter(), BucketedGeometryBias(4, EDGES, use_noise_gate=False)
+    torch.nn.init.normal_(bias.u_table)
+    frac, lattice = torch.rand(2, 30, 3), torch.tensor([[1.5, 1.6, 1.4, 0.1, 0.0, -0.1]] * 2)
+    geom = adapter.to(cuda)(coords=frac.to(cuda), lattice=lattice.to(cuda))
+    on_cpu = type(geom)(**{k: v.cpu() if torch.is_tensor(v) else v for k, v in vars(geom).items()})
+    want = bias.build_structured_bias_inputs(on_cpu, 30)[0]
+    got = bias.to(cuda).build_structured_bias_inputs(geom, 30)[0]
+    assert torch.equal(got.u.cpu(), want.u)
+
+
+def test_trunk_in_a_graph(cuda):
+    trunk = make_trunk(cuda, torch.bfloat16).eval()
+    x, cond, coords, pad = batch(cuda, torch.bfloat16)
+    packing = TokenPacking(pad)
+    with torch.no_grad():
+        trunk(x, cond, coords, pad, packing=packing)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = trunk(x, cond, coords, pad, packing=packing)
+        for _ in range(3):
+            x.copy_(torch.randn_like(x))
+            coords.copy_(torch.randn_like(coords) * 2.0)
+            want = trunk(x, cond, coords, pad, packing=packing)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(held, want)

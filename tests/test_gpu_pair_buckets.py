@@ -211,6 +211,18 @@ def test_tables_with_infinities_and_lowest_values(cuda):
         assert torch.equal(bucket_bias(table, index_buckets(index, 4))[0, 0], table[:, 0][index[0]])
 
 
+def test_refused_bias(cuda):
+    buckets = index_buckets(torch.zeros(1, 3, 3, dtype=torch.int32, device=cuda), 4)
+    with pytest.raises(RuntimeError, match="only supports"):
+        bucket_bias(torch.zeros(4, 2, dtype=torch.float64, device=cuda), buckets)
+    with pytest.raises(RuntimeError, match="only supports"):
+        bucket_bias(torch.zeros(4, 2, device=cuda), buckets, dtype=torch.float64)
+    with pytest.raises(RuntimeError, match="128 heads"):
+        bucket_bias(torch.zeros(4, 129, device=cuda), buckets)
+    with pytest.raises(RuntimeError, match="same device"):
+        bucket_bias(torch.zeros(4, 2), buckets)
+
+
 def test_buckets_and_bias_in_a_graph(cuda):
     coords = torch.randn(4, 70, 3, device=cuda)
     table = torch.randn(9, 8, device=cuda)
