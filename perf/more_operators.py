@@ -240,8 +240,10 @@ def _own_buckets(state):
     if "coords" in state:
         return distance_buckets(state["coords"], state["edges"], pad_mask=state["pad"],
                                 cutoff=state["case"].get("cutoff") or None)
-    return offset_buckets(state["places"], state["places"], state["edges"], pad_mask=state["pad"],
-                          query_pad_mask=state["pad"], causal=state["causal"])
+    # offsets to both sides of an even number of buckets leave the last one without an edge: one that no offset reaches
+    edges = state["edges"] + [2 ** 40 + i for i in range(state["case"]["buckets"] - 1 - len(state["edges"]))]
+    return offset_buckets(state["places"], state["places"], edges, pad_mask=state["pad"], query_pad_mask=state["pad"],
+                          causal=state["causal"])
 
 
 def _own_index(state):
