@@ -160,7 +160,7 @@ def bucket_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: t
     or of one for every entry; scale D^-1/2 unless given.  One new token is Nq = 1.
 
     Returns out like q and, with return_lse, lse (B, H, Nq) fp32.  Queries without a pair get 0 (lse 0); keys and
-    queries without a pair may hold anything (NaN).  Differentiable in q, k, v and the table through out and lse, for
+    queries without a pair may hold anything (NaN); a key that some query attends must be finite.  Differentiable in q, k, v and the table through out and lse, for
     which the buckets need their transpose (made with gradients=True); two calls give identical bits."""
     if q.ndim != 4 or k.ndim != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
         raise ValueError("q must have shape (B, H, Nq, D), k and v (B, KV, Nk, D)")

@@ -19,8 +19,8 @@ missing library raises.  CPU tensors take the torch formulation.
 
 from __future__ import annotations
 
-import ctypes
 import math
+import operator
 from array import array
 from typing import Sequence
 
@@ -72,7 +72,7 @@ class PairBuckets:
         return self.index != MASKED
 
 
-def _round_edges(edges, whole: bool) -> list:
+def _round_edges(edges, whole: bool) -> array:
     """The edges as host numbers: whole ones, or rounded to fp32 as the values they are compared with."""
     if isinstance(edges, torch.Tensor):
         if edges.device.type != "cpu" or edges.ndim != 1:
@@ -81,17 +81,20 @@ def _round_edges(edges, whole: bool) -> list:
     if len(edges) > MAX_BUCKETS - 1:
         raise ValueError(f"at most {MAX_BUCKETS - 1} edges, got {len(edges)}")
     if whole:
-        out = [int(e) for e in edges]
-        if any(a != b for a, b in zip(out, edges)):
-            raise ValueError("edges of offsets must be whole numbers")
-        if any(abs(e) > 2 ** 53 for e in out):
-            raise ValueError("edges of offsets must not pass 2^53")
+        try:
+            edges = array("q", edges)
+        except OverflowError:
+            raise ValueError("edges of offsets must not pass 2^53") from None
+        except TypeError:  # not integers: whole floats pass
+            if any(not math.isfinite(e) or e != math.floor(e) for e in edges):
+                raise ValueError("edges of offsets must be finite and whole numbers") from None
     else:
-        if any(abs(e) > 3.4028234663852886e38 for e in edges):
-            raise ValueError("edges must be finite")
-        out = array("f", edges).tolist()
-    if any(not (math.isfinite(e) and (i == 0 or e > out[i - 1])) for i, e in enumerate(out)):
+        edges = array("f", edges)  # (past fp32's range becomes infinite)
+    out = array("d", edges)
+    if out and not (all(map(operator.lt, out, out[1:])) and math.isfinite(out[0]) and math.isfinite(out[-1])):
         raise ValueError("edges must be finite and rise")
+    if whole and out and max(-edges[0], edges[-1]) > 2 ** 53:
+        raise ValueError("edges of offsets must not pass 2^53")
     return out
 
 
@@ -127,18 +130,19 @@ def _launch(source: int, B: int, Nq: int, Nk: int, device: torch.device, *, edge
     else:
         index_t, query_any = None, torch.empty(B, TK, TQ, dtype=torch.int64, device=device)
     if B * Nq * Nk > 0:
-        host = None if not edges else (ctypes.c_double * len(edges))(*edges)
         args = _native.MfPairBucketsArgs(
             query_pos=_native.ptr(query_pos), key_pos=_native.ptr(key_pos), values=_native.ptr(values),
             query_pad=_native.ptr(query_pad), key_pad=_native.ptr(key_pad),
-            edges=None if host is None else ctypes.addressof(host), index=index.data_ptr(),
+            edges=edges.buffer_info()[0] if edges else None, index=index.data_ptr(),
             index_t=_native.ptr(index_t), key_any=key_any.data_ptr(), query_any=query_any.data_ptr(),
             query_step=query_step, key_step=key_step, cutoff=cutoff, source=source,
             num_edges=0 if edges is None else len(edges), buckets=buckets, causal=int(causal), batch=B, queries=Nq,
             keys=Nk)
         _native.launch("mf_pair_buckets", args, device)
     view_t = None if index_t is None else index_t[:, :, :Nq]
-    return PairBuckets(index[:, :, :Nk], view_t, buckets, key_any, query_any)
+    made = PairBuckets(index[:, :, :Nk], view_t, buckets, key_any, query_any)
+    made._laid_out = True
+    return made
 
 
 def _from_torch(index: torch.Tensor, buckets: int, allowed: torch.Tensor | None, query_pad, key_pad,
@@ -203,7 +207,7 @@ def offset_buckets(query_positions: torch.Tensor, key_positions: torch.Tensor, e
     """Buckets of the offsets key position - query position: how many of the rising whole ``edges`` are at or below it.
     Positions are whole, (B, N) or (N,) for every batch entry, and need not follow one another.  pad_mask (B, Nk) and
     query_pad_mask (B, Nq), True = padding: their pairs are left out; ``causal``: so are keys at a later position than
-    the query's.  ``gradients`` = False leaves out what only gradients read (a new token's step).  Positions and pads
+    the query's.  Positions are 64-bit and their differences must be too.  ``gradients`` = False leaves out what only gradients read (a new token's step).  Positions and pads
     without a batch give buckets of a batch of one, which serve any batch."""
     host = _round_edges(edges, whole=True)
     positions = []

@@ -360,3 +360,52 @@ def test_replayed_graph(cuda, shape):
         torch.cuda.synchronize()
         for mine in held:
             assert all(torch.equal(a, b) for a, b in zip(mine, want))
+
+
+def test_saved_tensors_moved_meanwhile(cuda):
+    """Saved tensor hooks hand the backward pass other tensors than the forward saw."""
+    B, N, H, D = 2, 80, 4, 64
+    rows = torch.randn(B, N, 3 * H * D, device=cuda).to(BF16).requires_grad_(True)
+    q, k, v = (t.view(B, N, H, D).transpose(1, 2) for t in rows.chunk(3, dim=-1))
+    table = torch.randn(8, H, device=cuda, requires_grad=True)
+    buckets = index_buckets(torch.randint(0, 8, (B, N, N), device=cuda), 8)
+    go = torch.randn(B, H, N, D, device=cuda).to(BF16)
+    want = torch.autograd.grad(bucket_attention(q, k, v, table, buckets), (rows, table), go)
+    with torch.autograd.graph.save_on_cpu():
+        out = bucket_attention(*(t.view(B, N, H, D).transpose(1, 2) for t in rows.chunk(3, dim=-1)), table, buckets)
+    got = torch.autograd.grad(out, (rows, table), go)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_buckets_made_in_inference_mode(cuda):
+    q, k, v, table, index, go = make(cuda, 1, 2, 2, 40, 40, 32, BF16)
+    with torch.inference_mode():
+        buckets = index_buckets(index, table.shape[0])
+        plain = bucket_attention(q, k, v, table, buckets)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v, table)]
+    out = bucket_attention(*leaves, buckets)
+    assert torch.equal(out, plain)
+    assert all(torch.isfinite(g).all() for g in torch.autograd.grad(out, leaves, go))
+
+
+def test_two_layers_share_buckets_and_a_table(cuda):
+    """One table through two layers: its gradient is the sum of both."""
+    q, k, v, table, index, go = make(cuda, 2, 4, 4, 70, 70, 32, BF16)
+    buckets = index_buckets(index, table.shape[0])
+    t = table.clone().requires_grad_(True)
+    first = bucket_attention(q, k, v, t, buckets)
+    both = first + bucket_attention(v, k, q, t, buckets)
+    (together,) = torch.autograd.grad(both, t, go)
+    each = [torch.autograd.grad(bucket_attention(a, k, c, t, buckets), t, go)[0] for a, c in ((q, v), (v, q))]
+    assert torch.allclose(together, each[0] + each[1], rtol=1e-6, atol=1e-6)
+
+
+def test_forward_mode_is_refused(cuda):
+    from torch.autograd import forward_ad
+
+    q, k, v, table, index, _ = make(cuda, 1, 2, 2, 20, 20, 32, BF16)
+    buckets = index_buckets(index, table.shape[0])
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(q, torch.ones_like(q))
+        with pytest.raises(NotImplementedError):
+            bucket_attention(dual, k, v, table, buckets)

@@ -258,3 +258,31 @@ def test_two_streams_at_once(cuda):
             got.append(torch.autograd.grad(bucket_bias(table, index_buckets(i, 16)), table, go)[0])
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_distances_between_two_sets_through_the_c_entry(cuda):
+    import ctypes
+
+    from matterformer_amd import _native
+
+    g = torch.Generator().manual_seed(11)
+    B, Nq, Nk = 2, 70, 130
+    a, b = torch.randn(B, Nq, 3, generator=g), torch.randn(1, Nk, 3, generator=g)
+    edges = [0.5 * i for i in range(1, 8)]
+    values = torch.full((B, Nq, Nk), 0, dtype=torch.uint8)
+    d = a.double()[:, :, None] - b.double()[:, None]
+    d2 = (d[..., 0] * d[..., 0] + d[..., 1] * d[..., 1]) + d[..., 2] * d[..., 2]
+    for e in edges:
+        values += d2 >= e * e
+    values[d2 > 9.0] = MASKED
+    at, bt = a.to(cuda), b.to(cuda)
+    index = torch.zeros(B, Nq, 192, dtype=torch.uint8, device=cuda)
+    index_t = torch.zeros(B, Nk, 128, dtype=torch.uint8, device=cuda)
+    any_k, any_q = (torch.zeros(B, *s, dtype=torch.int64, device=cuda) for s in ((2, 3), (3, 2)))
+    host = (ctypes.c_double * 7)(*edges)
+    _native.launch("mf_pair_buckets", _native.MfPairBucketsArgs(
+        query_pos=at.data_ptr(), key_pos=bt.data_ptr(), edges=ctypes.addressof(host), index=index.data_ptr(),
+        index_t=index_t.data_ptr(), key_any=any_k.data_ptr(), query_any=any_q.data_ptr(), query_step=3 * Nq, key_step=0,
+        cutoff=3.0, source=_native.MF_BUCKETS_DISTANCE, num_edges=7, buckets=8, batch=B, queries=Nq, keys=Nk), at.device)
+    assert torch.equal(index[:, :, :Nk].cpu(), values) and index[:, :, Nk:].eq(MASKED).all()
+    assert torch.equal(index_t[:, :, :Nq].cpu(), values.transpose(1, 2))
