@@ -22,7 +22,7 @@ from __future__ import annotations
 import math
 import operator
 from array import array
-from typing import Sequence
+from typing import Iterable
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -158,7 +158,7 @@ def _from_torch(index: torch.Tensor, buckets: int, allowed: torch.Tensor | None,
     return PairBuckets(index, index.transpose(1, 2).contiguous() if gradients else None, buckets)
 
 
-def _count_edges(values: torch.Tensor, edges: Sequence[float]) -> torch.Tensor:
+def _count_edges(values: torch.Tensor, edges: Iterable[float]) -> torch.Tensor:
     index = torch.zeros(values.shape, dtype=torch.uint8, device=values.device)
     for e in edges:
         index += values >= e
@@ -238,7 +238,8 @@ def offset_buckets(query_positions: torch.Tensor, key_positions: torch.Tensor, e
                        key_step=kp.stride(0) if kp.shape[0] > 1 else 0, query_pad=qpad, key_pad=kpad, causal=causal,
                        gradients=gradients, symmetric=False)
     offset = (kp[:, None, :] - qp[:, :, None]).expand(B, Nq, Nk)
-    return _from_torch(_count_edges(offset, host), len(host) + 1, offset <= 0 if causal else None, qpad, kpad, gradients)
+    # (compared as whole numbers: a float would round the far ones)
+    return _from_torch(_count_edges(offset, map(int, host)), len(host) + 1, offset <= 0 if causal else None, qpad, kpad, gradients)
 
 
 def value_buckets(values: torch.Tensor, edges, *, pad_mask: torch.Tensor | None = None,
