@@ -131,9 +131,13 @@ class _BucketAttentionFunction(torch.autograd.Function):
 
 
 def bucket_attention_torch(q, k, v, table, buckets: PairBuckets, scale: float, *, dropout: float = 0.0):
-    """out and lse in torch, in fp32 (fp64 operands in fp64); rows without a pair are 0.  ``dropout`` of the
-    probabilities."""
+    """out and lse in torch, in fp32 (fp64 operands in fp64); rows without a pair are 0, whatever their operands hold.
+    ``dropout`` of the probabilities."""
     wide = torch.float64 if q.dtype == torch.float64 else torch.float32
+    allowed = buckets.allowed()
+    has_key, has_query = allowed.any(2)[:, None, :, None], allowed.any(1)[:, None, :, None]
+    none = torch.zeros((), dtype=q.dtype, device=q.device)
+    q, k, v = torch.where(has_key, q, none), torch.where(has_query, k, none), torch.where(has_query, v, none)
     group = q.shape[1] // k.shape[1] if k.shape[1] else 1
     k, v = (t.to(wide).repeat_interleave(group, dim=1) for t in (k, v))
     bias = table_with_masked(table.to(wide))[table_rows(buckets)].permute(0, 3, 1, 2)
@@ -146,6 +150,7 @@ def bucket_attention_torch(q, k, v, table, buckets: PairBuckets, scale: float, *
     some = total > 0
     p = p / torch.where(some, total, torch.ones_like(total))
     out = torch.matmul(torch.nn.functional.dropout(p, dropout) if dropout > 0.0 else p, v)
+    out = torch.where(has_key, out, torch.zeros_like(out))
     lse = torch.where(some, torch.log(torch.where(some, total, torch.ones_like(total))) + top, torch.zeros_like(top))
     return out.to(q.dtype), lse[..., 0].to(torch.float32)
 
@@ -160,8 +165,9 @@ def bucket_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: t
     or of one for every entry; scale D^-1/2 unless given.  One new token is Nq = 1.
 
     Returns out like q and, with return_lse, lse (B, H, Nq) fp32.  Queries without a pair get 0 (lse 0); keys and
-    queries without a pair may hold anything (NaN); a key that some query attends must be finite.  Differentiable in q, k, v and the table through out and lse, for
-    which the buckets need their transpose (made with gradients=True); two calls give identical bits."""
+    queries without a pair may hold anything (NaN); a key that some query attends must be finite.  Differentiable in q,
+    k, v and the table through out and lse, for which the buckets need their transpose (made with gradients=True); two
+    calls give identical bits."""
     if q.ndim != 4 or k.ndim != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
         raise ValueError("q must have shape (B, H, Nq, D), k and v (B, KV, Nk, D)")
     _check_table(table, buckets)

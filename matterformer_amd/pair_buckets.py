@@ -207,8 +207,9 @@ def offset_buckets(query_positions: torch.Tensor, key_positions: torch.Tensor, e
     """Buckets of the offsets key position - query position: how many of the rising whole ``edges`` are at or below it.
     Positions are whole, (B, N) or (N,) for every batch entry, and need not follow one another.  pad_mask (B, Nk) and
     query_pad_mask (B, Nq), True = padding: their pairs are left out; ``causal``: so are keys at a later position than
-    the query's.  Positions are 64-bit and their differences must be too.  ``gradients`` = False leaves out what only gradients read (a new token's step).  Positions and pads
-    without a batch give buckets of a batch of one, which serve any batch."""
+    the query's.  Positions are 64-bit and their differences must be too.  ``gradients`` = False leaves out what only
+    gradients read (a new token's step).  Positions and pads without a batch give buckets of a batch of one, which serve
+    any batch."""
     host = _round_edges(edges, whole=True)
     positions = []
     for name, p in (("query_positions", query_positions), ("key_positions", key_positions)):
@@ -239,7 +240,8 @@ def offset_buckets(query_positions: torch.Tensor, key_positions: torch.Tensor, e
                        gradients=gradients, symmetric=False)
     offset = (kp[:, None, :] - qp[:, :, None]).expand(B, Nq, Nk)
     # (compared as whole numbers: a float would round the far ones)
-    return _from_torch(_count_edges(offset, map(int, host)), len(host) + 1, offset <= 0 if causal else None, qpad, kpad, gradients)
+    return _from_torch(_count_edges(offset, map(int, host)), len(host) + 1, offset <= 0 if causal else None, qpad, kpad,
+                       gradients)
 
 
 def value_buckets(values: torch.Tensor, edges, *, pad_mask: torch.Tensor | None = None,

@@ -100,6 +100,25 @@ def test_bias_and_attention_follow_the_formulas():
     assert not out[0, :, 3].any() and not lse[0, :, 3].any()
 
 
+def test_rows_without_a_pair_may_hold_anything():
+    torch.manual_seed(11)
+    pad = torch.tensor([[False] * 5, [False, False, True, True, True]])
+    buckets = distance_buckets(torch.randn(2, 5, 3), [0.5, 1.0, 2.0], pad_mask=pad)
+    clean = [torch.randn(2, 4, 5, 8, dtype=torch.float64), torch.randn(2, 2, 5, 8, dtype=torch.float64),
+             torch.randn(2, 2, 5, 8, dtype=torch.float64)]
+    table, go = torch.randn(4, 4, dtype=torch.float64), torch.randn(2, 4, 5, 8, dtype=torch.float64)
+    results = []
+    for fill in (0.0, math.nan, math.inf):
+        q, k, v, g = (t.masked_fill(pad[:, None, :, None], fill) for t in (*clean, go))
+        leaves = [t.clone().requires_grad_() for t in (q, k, v, table)]
+        out, lse = bucket_attention(*leaves, buckets, return_lse=True)
+        out.backward(g)
+        results.append([out.detach(), lse.detach(), *(t.grad for t in leaves)])
+    for other in results[1:]:
+        for a, b in zip(results[0], other):
+            assert torch.equal(a, b)
+
+
 def test_refusals():
     c = torch.zeros(1, 4, 3)
     for edges in ([1.0, 1.0], [2.0, 1.0], [math.nan], [math.inf], [1e39], list(range(1, 65)), [-1.0, 2.0]):
