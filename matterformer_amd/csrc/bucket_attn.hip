@@ -101,7 +101,6 @@ constexpr float shift_bits() {
   return __is_same(T, _Float16) ? 15.0f - kSlack : 0.0f;
 }
 
-
 template <typename T>
 __device__ __forceinline__ void store_stats(const FwdParams& p, const Column& c, float m, float l) {
   l *= __is_same(T, _Float16) ? 1.0f / 128.0f : 1.0f;  // 2^-shift_bits
@@ -119,7 +118,7 @@ __device__ __forceinline__ void store_stats(const FwdParams& p, const Column& c,
   if (p.lse) p.lse[at] = l > 0.0f ? (m + __log2f(l)) * kLn2 : l;
 }
 
-// Waves a SIMD that the registers are to allow: four (head_dim 128: two), or what LDS has room for.
+// Waves a SIMD that the registers are to allow: three (head_dim 128: two), or what LDS has room for.
 constexpr int fwd_waves(int DP, int W, bool packed) {
   const int lds = 4 * kTile * DP * 2 + (packed ? 32 : 1) * kPitch * 4;
   const int fit = 160 * 1024 / lds * W / 4, most = DP == 128 ? 2 : 3;
@@ -198,7 +197,6 @@ __global__ void __launch_bounds__(64 * W, fwd_waves(DP, W, PACKED)) bucket_attn_
 #pragma unroll
   for (int n = 0; n < ND; ++n) acc[n] = zeros16();
   float m = -INFINITY, l = 0.0f, limit = -INFINITY;
-
 
   while (more) {
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this wave's copies into LDS have landed
