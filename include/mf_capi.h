@@ -875,7 +875,7 @@ int mf_pair_buckets(const mf_pair_buckets_args* args, void* stream);
 typedef struct mf_bucket_bias_args {
   const uint8_t* index;        /* [B or 1, queries, S(keys)]                 */
   const void* table;           /* forward: [buckets, H]                      */
-  void* bias;                  /* [B, H, queries, keys]: written, or, by the gradient, its upstream gradient */
+  void* bias;                  /* [B, H, queries, keys], 16-byte aligned: written, or, by the gradient, its upstream gradient */
   void* dtable;                /* gradient: [buckets, H]                     */
   void* workspace;
   uint64_t workspace_bytes;

@@ -264,17 +264,26 @@ __global__ void __launch_bounds__(kThreads) pair_buckets_kernel(BucketParams p) 
 }
 
 // -- the bias ----------------------------------------------------------------------------------------------------
+// Both kernels walk a plane (one batch entry and head, Nq Nk entries) in its flat order, so that their accesses to the bias
+// are 16 bytes and aligned whatever Nk is: where Nk is odd, planes and rows start off 16 bytes, and accesses that cross
+// such a boundary cost the memory pipeline twice.  The buckets' rows are padded, so a run of them may have to be put
+// together from the ends of two rows.
 struct BiasParams {
   const uint8_t* index;
   const void* table;
   void* bias;
-  float* parts;         // gradient: [H, K, pieces]
-  uint32_t rows;        // B Nq
-  uint32_t first_row;   // of this launch
-  uint32_t rows_index;  // rows of the index (the rows of a batch of one, or all)
+  float* parts;        // gradient: [H, K, pieces]
+  int64_t plane;       // Nq Nk
+  int64_t index_step;  // from one batch entry's buckets to the next (0: shared)
+  int64_t first;       // bias: this launch's first chunk of a plane
+  int64_t chunks;      // of a plane; bias: those of this launch
+  int64_t total;       // gradient: chunks of all batch entries
+  int64_t piece;       // gradient: chunks of a workgroup
+  uint32_t threads;    // bias: of this launch
+  int first_b;         // bias: this launch's first batch entry
   int H, Nq, Nk, K, S, table_dtype;
-  int head_step;        // heads of a workgroup
-  int pieces, piece_rows;
+  int head_step;       // bias: heads of a workgroup
+  int pieces;
 };
 
 template <typename T>
@@ -282,16 +291,60 @@ __device__ __forceinline__ float load_one(const void* p, int64_t at) {
   return float(static_cast<const T*>(p)[at]);
 }
 
-template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Wide {  // 16 bytes at any element
-  T v[16 / sizeof(T)];
+template <int N>
+struct __attribute__((packed, aligned(1))) Words {  // at any byte
+  uint32_t v[N];
 };
 
-// V buckets of a row (16 bytes of bias) a thread.
+__device__ __forceinline__ int64_t divide(int64_t x, int64_t by) {
+  if (((x | by) >> 32) == 0) return uint32_t(x) / uint32_t(by);
+  return x / by;
+}
+
+// 4 N bytes from byte `by` < 4 N on of two runs of words.
+__device__ __forceinline__ uint32_t pick(bool second, uint32_t a, uint32_t b) { return second ? b : a; }
+template <int N>
+__device__ __forceinline__ void bytes_from(const uint32_t (&lo)[N], const uint32_t (&hi)[N], int by, uint32_t (&w)[N]) {
+  const bool two = by & 8, one = by & 4;
+  if constexpr (N == 4) {
+    const uint32_t u0 = pick(two, lo[0], lo[2]), u1 = pick(two, lo[1], lo[3]), u2 = pick(two, lo[2], hi[0]),
+                   u3 = pick(two, lo[3], hi[1]), u4 = pick(two, hi[0], hi[2]), u5 = pick(two, hi[1], hi[3]);
+    const uint32_t v0 = pick(one, u0, u1), v1 = pick(one, u1, u2), v2 = pick(one, u2, u3), v3 = pick(one, u3, u4),
+                   v4 = pick(one, u4, u5);
+    w[0] = __builtin_amdgcn_alignbyte(v1, v0, by & 3);
+    w[1] = __builtin_amdgcn_alignbyte(v2, v1, by & 3);
+    w[2] = __builtin_amdgcn_alignbyte(v3, v2, by & 3);
+    w[3] = __builtin_amdgcn_alignbyte(v4, v3, by & 3);
+  } else {
+    const uint32_t v0 = pick(one, lo[0], lo[1]), v1 = pick(one, lo[1], hi[0]), v2 = pick(one, hi[0], hi[1]);
+    w[0] = __builtin_amdgcn_alignbyte(v1, v0, by & 3);
+    w[1] = __builtin_amdgcn_alignbyte(v2, v1, by & 3);
+  }
+}
+
+// Buckets one by one from (row, col) on of a batch entry; places before its first row or past its last are masked.
+template <int N>
+__device__ __forceinline__ void few_codes(const BiasParams& p, const uint8_t* in, int64_t row, int col, uint32_t (&w)[N]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) w[n] = 0;
+#pragma unroll
+  for (int t = 0; t < 4 * N; ++t) {
+    const uint32_t code = col >= 0 && row < p.Nq ? in[row * p.S + col] : uint32_t(kMasked);
+    w[t >> 2] |= code << (8 * (t & 3));
+    if (++col == p.Nk) {
+      col = 0;
+      ++row;
+    }
+  }
+}
+
+// A thread writes 16 aligned bytes of bias of every head from one window of buckets: head h's entries begin where its plane
+// is at a multiple of 16 bytes, V - 1 entries into the window at most.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) bucket_bias_kernel(BiasParams p) {
-  extern __shared__ float s_table[];  // [head_step][kPitch]
-  constexpr int V = 16 / sizeof(T);
+  extern __shared__ uint32_t s_table[];  // [head_step][kPitch]: entries in the bias's type, the others' bits zero
+  constexpr int V = 16 / sizeof(T), N = V / 2;
+  using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
   const int h0 = blockIdx.y * p.head_step, heads = min(p.head_step, p.H - h0);
   for (int n = threadIdx.x; n < heads * kPitch; n += kThreads) {
     const int h = n / kPitch, c = n - h * kPitch;
@@ -302,89 +355,180 @@ __global__ void __launch_bounds__(kThreads) bucket_bias_kernel(BiasParams p) {
           : p.table_dtype == MF_DTYPE_BF16 ? load_one<__bf16>(p.table, at)
                                            : load_one<_Float16>(p.table, at);
     }
-    s_table[n] = v;
+    s_table[n] = __builtin_bit_cast(Bits, static_cast<T>(v));
   }
   __syncthreads();
-  const uint32_t id = blockIdx.x * uint32_t(kThreads) + threadIdx.x, per = (p.Nk + V - 1) / V;
-  const uint32_t row = p.first_row + id / per;
-  if (row >= p.rows) return;
-  const int c = int(id % per);
-  const uint32_t b = row / uint32_t(p.Nq), i = row - b * uint32_t(p.Nq);
-  const uint8_t* in = p.index + int64_t(row % p.rows_index) * p.S + V * c;
-  uint32_t w[4] = {};
+  const uint32_t id = blockIdx.x * uint32_t(kThreads) + threadIdx.x;
+  if (id >= p.threads) return;
+  const uint32_t bl = id / uint32_t(p.chunks);
+  const int64_t b = p.first_b + int64_t(bl), n = p.first + (id - bl * uint32_t(p.chunks)), from = n * V;
+  const int64_t row = divide(from, p.Nk);
+  const int col = int(from - row * p.Nk);
+  const uint8_t* in = p.index + b * p.index_step;
+  uint32_t w[N] = {};
+  if (p.Nk % V == 0) {  // (every plane begins at a multiple of 16 bytes: the first V)
+    const uint8_t* at = in + row * p.S + col;
 #pragma unroll
-  for (int t = 0; t < V / 4; ++t) w[t] = reinterpret_cast<const uint32_t*>(in)[t];
-  const int left = p.Nk - V * c;
-  T* out = static_cast<T*>(p.bias) + ((int64_t(b) * p.H + h0) * p.Nq + i) * p.Nk + V * c;
-  const int64_t step = int64_t(p.Nq) * p.Nk;
-  for (int h = 0; h < heads; ++h, out += step) {
-    const float* table = s_table + h * kPitch;
-    Wide<T> x;
+    for (int t = 0; t < V / 4; ++t) w[t] = reinterpret_cast<const uint32_t*>(at)[t];
+  } else if (p.Nk >= 2 * V) {
+    const int start = min(col, p.Nk - 2 * V);
+    const Words<N> lo = *reinterpret_cast<const Words<N>*>(in + row * p.S + start);
+    uint32_t a[N], z[N];
 #pragma unroll
-    for (int t = 0; t < V; ++t) x.v[t] = static_cast<T>(table[byte_of(w, t)]);
-    if (left >= V) {
-      *reinterpret_cast<Wide<T>*>(out) = x;
+    for (int t = 0; t < N; ++t) {
+      w[t] = a[t] = lo.v[t];
+      z[t] = 0x40404040u;
+    }
+    if (col != start) {
+      if (row + 1 < p.Nq) {
+        const Words<N> hi = *reinterpret_cast<const Words<N>*>(in + (row + 1) * p.S);
+#pragma unroll
+        for (int t = 0; t < N; ++t) z[t] = hi.v[t];
+      }
+      bytes_from<N>(a, z, col - start, w);
+    }
+  } else {
+    few_codes<N>(p, in, row, col, w);
+  }
+  const int left = int(min(p.plane - from, int64_t(2 * V)));
+  Bits* out = static_cast<Bits*>(p.bias) + (b * p.H + h0) * p.plane;
+  unsigned begin = unsigned(b * p.H + h0) * unsigned(p.plane);  // of the plane, modulo V
+  for (int h = 0; h < heads; ++h, out += p.plane, begin += unsigned(p.plane)) {
+    const uint32_t* table = s_table + h * kPitch;
+    const int a = int(-begin & (V - 1));
+    uint32_t x[4] = {}, y[V];
+    if constexpr (V == 8) {
+      const uint32_t u0 = a & 4 ? w[1] : w[0], u1 = a & 4 ? w[2] : w[1], u2 = a & 4 ? w[3] : w[2];
+      x[0] = __builtin_amdgcn_alignbyte(u1, u0, a & 3);
+      x[1] = __builtin_amdgcn_alignbyte(u2, u1, a & 3);
+    } else {
+      x[0] = __builtin_amdgcn_alignbyte(w[1], w[0], a);
+    }
+#pragma unroll
+    for (int t = 0; t < V; ++t) y[t] = table[byte_of(x, t)];
+    if (a + V <= left) {
+      *reinterpret_cast<uint4*>(out + from + a) =
+          V == 4 ? make_uint4(y[0], y[1], y[2], y[3])
+                 : make_uint4(y[0] | y[1] << 16, y[2] | y[3] << 16, y[V - 4] | y[V - 3] << 16, y[V - 2] | y[V - 1] << 16);
     } else {
 #pragma unroll
       for (int t = 0; t < V - 1; ++t)
-        if (t < left) out[t] = x.v[t];
+        if (a + t < left) out[from + a + t] = Bits(y[t]);
+    }
+    if (n == 0 && a > 0) {  // the entries before the plane's first multiple
+#pragma unroll
+      for (int t = 0; t < V - 1; ++t)
+        if (t < a && t < left) out[t] = Bits(table[(w[t >> 2] >> (8 * (t & 3))) & 255u]);
     }
   }
 }
 
-// A workgroup sums one head's rows first .. + piece_rows: `across` threads to a row, each 16 keys at a time, the next ones
-// loaded while the last ones are added.
+// A workgroup sums a piece of one head's chunks, a thread 16 entries at a time, the next ones loaded while the last ones are
+// added.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) bucket_bias_bwd_kernel(BiasParams p) {
   extern __shared__ float s_bins[];  // [K + 1][kThreads]; the last one takes the masked pairs
   constexpr int V = 16 / sizeof(T), kKeys = 16;
+  using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+  auto value = [](const uint32_t* words, int t) {
+    return float(__builtin_bit_cast(T, Bits(sizeof(T) == 4 ? words[t] : words[t >> 1] >> (16 * (t & 1)))));
+  };
   const int tid = threadIdx.x;
   for (int c = 0; c <= p.K; ++c) s_bins[c * kThreads + tid] = 0.0f;
   const int h = blockIdx.y;
-  const int per = (p.Nk + kKeys - 1) / kKeys;
-  int across = 1;
-  while (across < per && across < kThreads) across *= 2;
-  const int down = kThreads / across, tx = tid & (across - 1), ty = tid / across;
-  const uint32_t end = min(p.rows, (blockIdx.x + 1u) * uint32_t(p.piece_rows));
   float* bins = s_bins + tid;
 
-  uint4 packed = {};
-  Wide<T> x[kKeys / V];
-  int left = 0;
-  auto load = [&](uint32_t row, int c) {
-    const uint32_t b = row / uint32_t(p.Nq), i = row - b * uint32_t(p.Nq);
-    packed = *reinterpret_cast<const uint4*>(p.index + int64_t(row % p.rows_index) * p.S + kKeys * c);
-    left = p.Nk - kKeys * c;
-    const T* in = static_cast<const T*>(p.bias) + ((int64_t(b) * p.H + h) * p.Nq + i) * p.Nk + kKeys * c;
-    if (left >= kKeys) {
-#pragma unroll
-      for (int u = 0; u < kKeys / V; ++u) x[u] = reinterpret_cast<const Wide<T>*>(in)[u];
+  // a plane's chunks begin at multiples of 16 bytes, the first one before the plane where that does not
+  const int64_t end = min(p.total, (blockIdx.x + int64_t(1)) * p.piece);
+  int64_t id = blockIdx.x * p.piece + tid, b = 0, n = id, from = 0, row = 0;
+  int col = 0;
+  auto enter = [&] {  // chunk n, past this batch entry's or the first
+    const int64_t more = divide(n, p.chunks);
+    b += more;
+    n -= more * p.chunks;
+    const int a = int(-(unsigned(b * p.H + h) * unsigned(p.plane)) & (V - 1));
+    from = n * kKeys + (a ? a - kKeys : 0);
+    row = from < 0 ? 0 : divide(from, p.Nk);
+    col = int(from - row * p.Nk);
+  };
+  const int rows_on = kThreads * kKeys / p.Nk, cols_on = kThreads * kKeys - rows_on * p.Nk;
+  auto advance = [&] {
+    id += kThreads;
+    n += kThreads;
+    if (n >= p.chunks) {
+      enter();
     } else {
-#pragma unroll
-      for (int t = 0; t < kKeys; ++t) x[t / V].v[t % V] = t < left ? in[t] : T(0.0f);
+      from += kThreads * kKeys;
+      row += rows_on;
+      col += cols_on;
+      if (col >= p.Nk) {
+        col -= p.Nk;
+        ++row;
+      }
+      while (col < 0) {  // (from the chunk before the plane)
+        col += p.Nk;
+        --row;
+      }
     }
   };
-  uint32_t row = blockIdx.x * uint32_t(p.piece_rows) + ty;
-  int c = tx;
-  bool more = row < end && c < per;  // (a thread past the row's last keys has no row)
-  if (more) load(row, c);
-  while (more) {
-    const uint32_t w[4] = {packed.x, packed.y, packed.z, packed.w};
-    Wide<T> y[kKeys / V];
+  uint32_t lo[4], hi[4];
+  int by = 0;
+  uint32_t x[kKeys / V * 4];  // (as words: halves would be taken apart, and waited for, where they are loaded)
+  auto load = [&] {
+    const uint8_t* in = p.index + b * p.index_step;
+    const T* values = static_cast<const T*>(p.bias) + (b * p.H + h) * p.plane + from;
+    by = 0;
+    if (from >= 0 && from + kKeys <= p.plane && p.Nk >= kKeys) {
+      const int start = min(col, p.Nk - kKeys);
+      const Words<4> one = *reinterpret_cast<const Words<4>*>(in + row * p.S + start);
 #pragma unroll
-    for (int u = 0; u < kKeys / V; ++u) y[u] = x[u];
-    c += across;
-    if (c >= per) {
-      c = tx;
-      row += down;
+      for (int t = 0; t < 4; ++t) lo[t] = one.v[t];
+      by = col - start;
+      if (by != 0) {
+        const uint4 two = *reinterpret_cast<const uint4*>(in + (row + 1) * p.S);
+        hi[0] = two.x;
+        hi[1] = two.y;
+        hi[2] = two.z;
+        hi[3] = two.w;
+      }
+#pragma unroll
+      for (int u = 0; u < kKeys / V; ++u) {
+        const uint4 one = reinterpret_cast<const uint4*>(values)[u];
+        x[4 * u] = one.x;
+        x[4 * u + 1] = one.y;
+        x[4 * u + 2] = one.z;
+        x[4 * u + 3] = one.w;
+      }
+    } else {
+      few_codes<4>(p, in, row, col, lo);
+#pragma unroll
+      for (int t = 0; t < kKeys; ++t) {
+        const uint32_t bits =
+            from + t >= 0 && from + t < p.plane ? reinterpret_cast<const Bits*>(values)[t] : Bits(0);
+        if (sizeof(T) == 4 || t % 2 == 0) x[t * sizeof(T) / 4] = bits;
+        else x[t * sizeof(T) / 4] |= bits << 16;
+      }
     }
-    more = row < end;
-    if (more) load(row, c);
+  };
+  bool more = id < end;
+  if (more) {
+    enter();
+    load();
+  }
+  while (more) {
+    uint32_t w[4] = {lo[0], lo[1], lo[2], lo[3]};
+    if (by != 0) bytes_from<4>(lo, hi, by, w);
+    uint32_t y[kKeys / V * 4];
+#pragma unroll
+    for (int u = 0; u < kKeys / V * 4; ++u) y[u] = x[u];
+    advance();
+    more = id < end;
+    if (more) load();
     // two at a time: where both have one bucket the first takes both and the second adds to the masked pairs' row
 #pragma unroll
     for (int t = 0; t < kKeys; t += 2) {
       const int c0 = min(int(byte_of(w, t)), p.K), c1 = min(int(byte_of(w, t + 1)), p.K);
-      const float v0 = float(y[t / V].v[t % V]), v1 = float(y[(t + 1) / V].v[(t + 1) % V]);
+      const float v0 = value(y, t), v1 = value(y, t + 1);
       const bool same = c0 == c1;
       float* b0 = bins + c0 * kThreads;
       float* b1 = bins + (same ? p.K : c1) * kThreads;
@@ -451,8 +595,8 @@ int check_bias(const mf_bucket_bias_args* a, const char* what) {
     return fail(MF_ERR_UNSUPPORTED, name + ": only supports float32/float16/bfloat16");
   if (int64_t(a->batch) * a->queries >= (int64_t(1) << 31))
     return fail(MF_ERR_UNSUPPORTED, name + ": batch * queries too large");
-  if (reinterpret_cast<uintptr_t>(a->index) % 16 != 0)
-    return fail(MF_ERR_INVALID_ARGUMENT, name + ": index must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(a->index) % 16 != 0 || reinterpret_cast<uintptr_t>(a->bias) % 16 != 0)
+    return fail(MF_ERR_INVALID_ARGUMENT, name + ": index and bias must be 16-byte aligned");
   return MF_OK;
 }
 
@@ -461,28 +605,28 @@ BiasParams bias_params(const mf_bucket_bias_args* a) {
   p.index = a->index;
   p.table = a->table;
   p.bias = a->bias;
-  p.rows = uint32_t(a->batch) * uint32_t(a->queries);
-  p.rows_index = uint32_t(a->index_batch) * uint32_t(a->queries);
   p.H = a->heads;
   p.Nq = a->queries;
   p.Nk = a->keys;
   p.K = a->buckets;
   p.S = (a->keys + 63) / 64 * 64;
+  p.plane = int64_t(a->queries) * a->keys;
+  p.index_step = a->index_batch == 1 ? 0 : int64_t(a->queries) * p.S;
   p.table_dtype = a->table_dtype;
   return p;
 }
 
-// Rows of a piece of a head's pairs, each summed by a workgroup: four 16-key chunks a thread and more, and no more
-// workgroups than are resident at two a CU (66 KB of LDS each) twice over.
-int bias_piece_rows(const mf_bucket_bias_args* a) {
-  const int64_t rows = int64_t(a->batch) * a->queries, per = (a->keys + 15) / 16;
-  const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>((rows * per + 4 * kThreads - 1) / (4 * kThreads),
+// The chunks of 16 entries of a head, and how many of them a workgroup sums: four a thread and more, and no more workgroups
+// than are resident at two a CU (66 KB of LDS each) twice over.
+void bias_pieces(const mf_bucket_bias_args* a, BiasParams& p) {
+  const int V = a->bias_dtype == MF_DTYPE_F32 ? 4 : 8;
+  p.plane = int64_t(a->queries) * a->keys;
+  p.chunks = (p.plane + 15) / 16 + (p.plane % V != 0);
+  p.total = p.chunks * a->batch;
+  const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>((p.total + 4 * kThreads - 1) / (4 * kThreads),
                                                                 std::max(1, 1024 / std::max(1, a->heads))));
-  return int((rows + pieces - 1) / pieces);
-}
-int bias_pieces(const mf_bucket_bias_args* a) {
-  const int64_t rows = int64_t(a->batch) * a->queries, step = bias_piece_rows(a);
-  return int((rows + step - 1) / step);
+  p.piece = ((p.total + pieces - 1) / pieces + kThreads - 1) / kThreads * kThreads;
+  p.pieces = int((p.total + p.piece - 1) / p.piece);
 }
 
 }  // namespace
@@ -587,31 +731,34 @@ extern "C" int mf_bucket_bias(const mf_bucket_bias_args* a, void* stream) {
   if (a->batch == 0 || a->heads == 0 || a->queries == 0 || a->keys == 0) return MF_OK;
   BiasParams p = bias_params(a);
   const int V = a->bias_dtype == MF_DTYPE_F32 ? 4 : 8;
-  const int64_t per = (a->keys + V - 1) / V, rows = p.rows;
+  const int64_t chunks = (p.plane + V - 1) / V;
   // a workgroup takes all heads (one read of the index) unless that leaves less than eight workgroups a CU
-  const int64_t all = (rows * per + kThreads - 1) / kThreads;
+  const int64_t all = (chunks * a->batch + kThreads - 1) / kThreads;
   const int parts = int(std::min<int64_t>(a->heads, std::max<int64_t>(1, (2048 + all - 1) / all)));
   p.head_step = (a->heads + parts - 1) / parts;
   const unsigned lds = unsigned(p.head_step * kPitch * sizeof(float));
-  const int64_t step = std::max<int64_t>(1, (int64_t(1) << 30) / per);  // rows of a launch
   hipStream_t s = static_cast<hipStream_t>(stream);
-  for (int64_t first = 0; first < rows; first += step) {
-    p.first_row = uint32_t(first);
-    const int64_t blocks = (std::min(step, rows - first) * per + kThreads - 1) / kThreads;
-    BiasParams q = p;
-    q.rows = uint32_t(std::min(rows, first + step));
-    const dim3 grid(unsigned(blocks), unsigned((a->heads + p.head_step - 1) / p.head_step));
-    if (a->bias_dtype == MF_DTYPE_F32) hipLaunchKernelGGL(bucket_bias_kernel<float>, grid, dim3(kThreads), lds, s, q);
-    else if (a->bias_dtype == MF_DTYPE_BF16) hipLaunchKernelGGL(bucket_bias_kernel<__bf16>, grid, dim3(kThreads), lds, s, q);
-    else hipLaunchKernelGGL(bucket_bias_kernel<_Float16>, grid, dim3(kThreads), lds, s, q);
-    MF_HIP_CHECK(hipGetLastError());
-  }
+  constexpr int64_t kMost = int64_t(1) << 30;  // threads of a launch: whole batch entries, or a part of one
+  const int64_t entries = std::max<int64_t>(1, kMost / chunks);
+  for (int64_t b = 0; b < a->batch; b += entries)
+    for (p.first = 0; p.first < chunks; p.first += kMost) {
+      p.first_b = int(b);
+      p.chunks = std::min(kMost, chunks - p.first);
+      p.threads = uint32_t(p.chunks * std::min(entries, a->batch - b));
+      const dim3 grid((p.threads + kThreads - 1) / kThreads, unsigned((a->heads + p.head_step - 1) / p.head_step));
+      if (a->bias_dtype == MF_DTYPE_F32) hipLaunchKernelGGL(bucket_bias_kernel<float>, grid, dim3(kThreads), lds, s, p);
+      else if (a->bias_dtype == MF_DTYPE_BF16) hipLaunchKernelGGL(bucket_bias_kernel<__bf16>, grid, dim3(kThreads), lds, s, p);
+      else hipLaunchKernelGGL(bucket_bias_kernel<_Float16>, grid, dim3(kThreads), lds, s, p);
+      MF_HIP_CHECK(hipGetLastError());
+    }
   return MF_OK;
 }
 
 extern "C" uint64_t mf_bucket_bias_bwd_workspace_size(const mf_bucket_bias_args* a) {
   if (a == nullptr || a->batch <= 0 || a->heads <= 0 || a->queries <= 0 || a->keys <= 0 || a->buckets <= 0) return 0;
-  return uint64_t(a->heads) * a->buckets * mf::bucket::bias_pieces(a) * sizeof(float);
+  mf::bucket::BiasParams p = {};
+  mf::bucket::bias_pieces(a, p);
+  return uint64_t(a->heads) * a->buckets * p.pieces * sizeof(float);
 }
 
 extern "C" int mf_bucket_bias_bwd(const mf_bucket_bias_args* a, void* stream) {
@@ -628,8 +775,7 @@ extern "C" int mf_bucket_bias_bwd(const mf_bucket_bias_args* a, void* stream) {
       reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0)
     return fail(MF_ERR_INVALID_ARGUMENT, "mf_bucket_bias_bwd: the workspace must be 16-byte aligned and hold "
                                          "mf_bucket_bias_bwd_workspace_size bytes");
-  p.pieces = bias_pieces(a);
-  p.piece_rows = bias_piece_rows(a);
+  bias_pieces(a, p);
   p.parts = static_cast<float*>(a->workspace);
   const dim3 grid(unsigned(p.pieces), unsigned(a->heads));
   const int lds = (a->buckets + 1) * kThreads * int(sizeof(float));

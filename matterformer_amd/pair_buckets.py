@@ -377,6 +377,8 @@ class _BucketBiasFunction(torch.autograd.Function):
         if grad.numel() == 0:
             return dtable.zero_(), None, None, None
         g = grad.contiguous()
+        if g.data_ptr() % 16:
+            g = g.clone()
         args = _bias_args(buckets, ctx.batch, ctx.heads, ctx.table_dtype, g, dtable=dtable.data_ptr())
         nbytes = int(_native.lib().mf_bucket_bias_bwd_workspace_size(args))
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=grad.device)

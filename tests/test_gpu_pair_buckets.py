@@ -286,3 +286,23 @@ def test_distances_between_two_sets_through_the_c_entry(cuda):
         cutoff=3.0, source=_native.MF_BUCKETS_DISTANCE, num_edges=7, buckets=8, batch=B, queries=Nq, keys=Nk), at.device)
     assert torch.equal(index[:, :, :Nk].cpu(), values) and index[:, :, Nk:].eq(MASKED).all()
     assert torch.equal(index_t[:, :, :Nq].cpu(), values.transpose(1, 2))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,H,Nq,Nk", [(2, 3, 900, 3), (2, 2, 700, 15), (1, 3, 5000, 1), (2, 3, 301, 17), (1, 3, 3, 4099), (1, 2, 1, 9001),
+                                       (3, 2, 13, 30), (2, 2, 200, 509)])
+def test_planes_that_begin_anywhere(cuda, B, H, Nq, Nk, dtype):
+    """Rows shorter than an access, longer than what a workgroup takes at once, and planes off 16 bytes."""
+    test_bias_and_its_gradient(cuda, B, H, Nq, Nk, 23, dtype)
+
+
+def test_a_gradient_off_16_bytes(cuda):
+    g = torch.Generator(device=cuda).manual_seed(2)
+    index = torch.randint(-1, 9, (2, 31, 33), generator=g, device=cuda, dtype=torch.int32)
+    table = torch.randn(9, 5, generator=g, device=cuda).requires_grad_(True)
+    bias = bucket_bias(table, index_buckets(index, 9))
+    go = torch.randn(bias.numel() + 1, generator=g, device=cuda)[1:].view(bias.shape)
+    assert go.data_ptr() % 16 and go.is_contiguous()
+    (grad,) = torch.autograd.grad(bias, table, go, retain_graph=True)
+    (same,) = torch.autograd.grad(bias, table, go.clone())
+    assert torch.equal(grad, same)

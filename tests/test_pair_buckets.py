@@ -257,7 +257,7 @@ def test_bias_entries_refuse_before_any_device_call():
                                   (dict(keys=-1), INVALID, "non-negative"), (dict(index_batch=3), INVALID, "index_batch"),
                                   (dict(buckets=0), UNSUPPORTED, "[1, 64]"), (dict(heads=129), UNSUPPORTED, "128"),
                                   (dict(queries=2 ** 24 + 1), UNSUPPORTED, "2^24"), (dict(bias_dtype=3), UNSUPPORTED, "float32"),
-                                  (dict(index=FAKE + 1), INVALID, "aligned")):
+                                  (dict(index=FAKE + 1), INVALID, "aligned"), (dict(bias=FAKE + 2), INVALID, "aligned")):
             refused(fn, args(**kw), status, match)
     refused(lib.mf_bucket_bias, args(table=None), INVALID, "non-NULL")
     refused(lib.mf_bucket_bias_bwd, args(dtable=None), INVALID, "non-NULL")
