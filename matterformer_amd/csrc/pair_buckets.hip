@@ -10,13 +10,17 @@
 // the fp32 coordinates but for the roundings of fp64.
 //
 // bucket_bias_kernel: a thread reads the buckets of 16 bytes of bias once and
-// writes them for every head; the tables lie in LDS, one bank a bucket.  Bound by its writes.
+// writes them for every head; the tables lie in LDS, one bank a bucket.  Bound
+// by its writes (4 x 12 planes of 1997^2 in bf16, 383 MB: 71 us).
 //
 // bucket_bias_bwd_kernel: sums by bucket without atomics between lanes.  Every
 // lane keeps a sum per bucket of its own in LDS ([bucket][thread]: one bank a
 // lane whatever the buckets), to which it adds in the order of its pairs; then
 // the threads' sums are joined in a fixed order, and table_sum_kernel joins the
-// workgroups' in fp64.  Two calls give identical bits.  Bound by reading dbias.
+// workgroups' in fp64.  Two calls give identical bits.  A sum is read, added to
+// and written: 9 clocks a wave, where an fp32 atomic of LDS takes 193.  Bound by
+// the time that takes at the eight waves a CU that the sums leave room for (bf16,
+// same planes: 149 us; fp32, twice the bytes, 150).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -266,7 +270,8 @@ __global__ void __launch_bounds__(kThreads) pair_buckets_kernel(BucketParams p) 
 // -- the bias ----------------------------------------------------------------------------------------------------
 // Both kernels walk a plane (one batch entry and head, Nq Nk entries) in its flat order, so that their accesses to the bias
 // are 16 bytes and aligned whatever Nk is: where Nk is odd, planes and rows start off 16 bytes, and accesses that cross
-// such a boundary cost the memory pipeline twice.  The buckets' rows are padded, so a run of them may have to be put
+// such a boundary cost the memory pipeline twice (by rows, 4 x 12 x 1997^2 in bf16: bias 114 us instead of 71, its
+// gradient 180 instead of 149).  The buckets' rows are padded, so a run of them may have to be put
 // together from the ends of two rows.
 struct BiasParams {
   const uint8_t* index;
