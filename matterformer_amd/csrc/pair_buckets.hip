@@ -36,6 +36,7 @@ constexpr int kThreads = 256;
 // lie in lower cells; those in the value's own cell, mostly none or one, are compared with it.  1024 cells over the
 // edges' range: 157 an octave for distances of 0.1 to 9, where a count of 32 compares takes four times as long.
 constexpr int kCells = 1024;
+constexpr int64_t kCounts = (int64_t(1) << 32) - 64;  // tiles of a call: they are counted in 32 bits
 
 struct BucketParams {
   const void* query_pos;
@@ -49,7 +50,8 @@ struct BucketParams {
   uint64_t* query_any;
   int64_t query_step, key_step;
   double cutoff;
-  int64_t first, tiles;  // workgroups before this launch's, and in all
+  uint32_t first, tiles;  // workgroups before this launch's, and in all
+  uint32_t per;           // symmetric: of a batch entry
   int symmetric;         // index_t is index: tiles on and above the diagonal, each written twice
   int buckets, causal, Nq, Nk, TQ, TK;
   int base, shift;
@@ -71,6 +73,31 @@ __host__ __device__ __forceinline__ int cell_of(float x, int base, int shift) {
   return c < 0 ? 0 : c >= kCells ? kCells - 1 : c;
 }
 
+// The least and the greatest of a wave's values.
+template <bool LEAST>
+__device__ __forceinline__ int wave_end(int v) {
+  constexpr int kNone = LEAST ? INT32_MAX : INT32_MIN;
+  auto join = [](int a, int b) { return LEAST ? min(a, b) : max(a, b); };
+  v = join(v, __builtin_amdgcn_update_dpp(kNone, v, 0x111, 0xf, 0xf, false));  // rows of 16 lanes: 1, 2, 4, 8 further on
+  v = join(v, __builtin_amdgcn_update_dpp(kNone, v, 0x112, 0xf, 0xf, false));
+  v = join(v, __builtin_amdgcn_update_dpp(kNone, v, 0x114, 0xf, 0xf, false));
+  v = join(v, __builtin_amdgcn_update_dpp(kNone, v, 0x118, 0xf, 0xf, false));
+  v = join(v, __builtin_amdgcn_update_dpp(kNone, v, 0x142, 0xa, 0xf, false));  // a row's last lane to the next row
+  v = join(v, __builtin_amdgcn_update_dpp(kNone, v, 0x143, 0xc, 0xf, false));  // the first half's to the second
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
+// 16 bytes: a code where the mask has a bit, kMasked where not.
+__device__ __forceinline__ uint4 masked_codes(uint32_t mask, uint32_t code) {
+  uint32_t w[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const uint32_t on = (((mask >> (4 * t)) & 15u) * 0x00204081u & 0x01010101u) * 255u;
+    w[t] = (on & (code * 0x01010101u)) | (~on & 0x40404040u);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 template <int SOURCE>
 __global__ void __launch_bounds__(kThreads) pair_buckets_kernel(BucketParams p) {
   using Value = std::conditional_t<SOURCE == MF_BUCKETS_OFFSET, int64_t, double>;
@@ -81,28 +108,83 @@ __global__ void __launch_bounds__(kThreads) pair_buckets_kernel(BucketParams p) 
   __shared__ int s_off32[SOURCE == MF_BUCKETS_OFFSET ? kTile : 1];
   __shared__ uint8_t tile[kTile][kTile + 4];
   __shared__ uint64_t s_key[4], s_qry[4];
-  int64_t id = xcd_order(blockIdx.x, gridDim.x) + p.first;
+  const uint32_t id = xcd_order(blockIdx.x, gridDim.x) + p.first;
   if (id >= p.tiles) return;
-  int qt, kt;
+  uint32_t qt, kt;
   int64_t b;
   if (p.symmetric) {
-    const int64_t per = int64_t(p.TK) * (p.TK + 1) / 2;
-    b = id / per;
-    const int64_t t = id - b * per;
-    kt = int((sqrt(8.0 * double(t) + 1.0) - 1.0) * 0.5);
-    while (int64_t(kt) * (kt + 1) / 2 > t) --kt;
-    while (int64_t(kt + 1) * (kt + 2) / 2 <= t) ++kt;
-    qt = int(t - int64_t(kt) * (kt + 1) / 2);
+    const uint32_t entry = id / p.per, t = id - entry * p.per;
+    b = entry;
+    kt = uint32_t((sqrtf(8.0f * float(t) + 1.0f) - 1.0f) * 0.5f);  // (off by one at most)
+    if (kt * (kt + 1) / 2 > t) --kt;
+    if ((kt + 1) * (kt + 2) / 2 <= t) ++kt;
+    qt = t - kt * (kt + 1) / 2;
   } else {
-    kt = int(id % p.TK);
-    qt = int(id / p.TK % p.TQ);
-    b = id / (int64_t(p.TK) * p.TQ);
+    const uint32_t row = id / uint32_t(p.TK), entry = row / uint32_t(p.TQ);
+    kt = id - row * uint32_t(p.TK);
+    qt = row - entry * uint32_t(p.TQ);
+    b = entry;
   }
   const int tid = threadIdx.x, r = tid >> 2, c0 = (tid & 3) * 16;
   const int lane = tid & 63, wave = tid >> 6;
   const int i = qt * kTile + r;
   const int64_t S = (int64_t(p.Nk) + 63) / 64 * 64, St = (int64_t(p.Nq) + 63) / 64 * 64;
 
+  // which of the tile's keys and queries count: lane t's key and query t
+  const int jl = kt * kTile + lane, il = qt * kTile + lane;
+  uint8_t key_out = jl >= p.Nk, query_out = il >= p.Nq;
+  if (p.key_pad != nullptr && jl < p.Nk) key_out = p.key_pad[b * p.Nk + jl];
+  if (p.query_pad != nullptr && il < p.Nq) query_out = p.query_pad[b * p.Nq + il];
+  // OFFSET: positions relative to the tile's first key; where all are within 2^29 their differences are formed in 32 bits,
+  // and if the least and the greatest of those that count have one bucket the tile has no other
+  int64_t qo = 0;
+  int q32 = 0;
+  bool near = true;
+  uint64_t keys, queries;
+  if constexpr (SOURCE == MF_BUCKETS_OFFSET) {
+    const int64_t* kp = static_cast<const int64_t*>(p.key_pos) + b * p.key_step;
+    const int64_t* qp = static_cast<const int64_t*>(p.query_pos) + b * p.query_step;
+    const int64_t base = kp[kt * kTile], key = jl < p.Nk ? kp[jl] : base, query = il < p.Nq ? qp[il] : base;
+    keys = __ballot(key_out == 0);
+    queries = __ballot(query_out == 0);
+    const int64_t dk = key - base, dq = query - base;
+    constexpr int64_t kNear = int64_t(1) << 29;
+    near = !__any(!(dk > -kNear && dk < kNear && dq > -kNear && dq < kNear));
+    if (near) {
+      const bool key_in = (keys >> lane) & 1, query_in = (queries >> lane) & 1;
+      const int low = wave_end<true>(key_in ? int(dk) : INT32_MAX), high = wave_end<false>(key_in ? int(dk) : INT32_MIN);
+      const int qlow = wave_end<true>(query_in ? int(dq) : INT32_MAX), qhigh = wave_end<false>(query_in ? int(dq) : INT32_MIN);
+      const bool none = keys == 0 || queries == 0 || (p.causal && low - qhigh > 0);  // no pair
+      int code = kMasked;
+      bool whole = none;
+      if (!none && !(p.causal && high - qlow > 0)) {
+        // (one value for the wave: its cell and edges come by scalar loads)
+        const int cell = __builtin_amdgcn_readfirstlane(cell_of(float(low - qhigh), p.base, p.shift));
+        code = (reinterpret_cast<const uint32_t*>(p.cells)[cell >> 2] >> (8 * (cell & 3))) & 255;
+        while (double(low - qhigh) >= p.edges[code]) ++code;  // (not past the NaN at the end)
+        whole = !(double(high - qlow) >= p.edges[code]);
+      }
+      if (whole) {
+        const uint32_t row = (queries >> r) & 1 ? uint32_t(keys >> c0) & 0xffffu : 0u;
+        const uint32_t column = (keys >> r) & 1 ? uint32_t(queries >> c0) & 0xffffu : 0u;
+        const int j = kt * kTile + r;
+        if (i < p.Nq) *reinterpret_cast<uint4*>(p.index + (b * p.Nq + i) * S + kt * kTile + c0) = masked_codes(row, code);
+        if (p.index_t && j < p.Nk)
+          *reinterpret_cast<uint4*>(p.index_t + (b * p.Nk + j) * St + qt * kTile + c0) = masked_codes(column, code);
+        if (tid == 0) {
+          p.key_any[(b * p.TQ + qt) * p.TK + kt] = none ? 0 : keys;
+          p.query_any[(b * p.TK + kt) * p.TQ + qt] = none ? 0 : queries;
+        }
+        return;
+      }
+    }
+    if (wave == 0) {
+      s_off[lane] = key;
+      s_off32[lane] = int(dk);  // (read where near)
+    }
+    if (near) q32 = __shfl(int(dq), r, 64);
+    else if (i < p.Nq) qo = qp[i];
+  }
   if constexpr (SOURCE != MF_BUCKETS_INDEX) {
     s_cells[tid] = reinterpret_cast<const uint32_t*>(p.cells)[tid];
     if (tid < MF_MAX_BUCKETS) {
@@ -115,81 +197,21 @@ __global__ void __launch_bounds__(kThreads) pair_buckets_kernel(BucketParams p) 
     const int j = kt * kTile + tid / 3;
     s_pos[tid % 3][tid / 3] = j < p.Nk ? static_cast<const float*>(p.key_pos)[b * p.key_step + int64_t(kt) * (3 * kTile) + tid] : 0.0f;
   }
-  const bool row_on = i < p.Nq && !(p.query_pad && p.query_pad[b * p.Nq + i]);
-  // which of the tile's keys count: lane t's key t
-  const int jl = kt * kTile + lane;
-  const uint64_t keys = __ballot(jl < p.Nk && !(p.key_pad && p.key_pad[b * p.Nk + jl]));
   double qx = 0.0, qy = 0.0, qz = 0.0;
-  int64_t qo = 0;
-  if (i < p.Nq) {
-    if constexpr (SOURCE == MF_BUCKETS_DISTANCE) {
-      const float* c = static_cast<const float*>(p.query_pos) + b * p.query_step + int64_t(i) * 3;
-      qx = c[0];
-      qy = c[1];
-      qz = c[2];
-    } else if constexpr (SOURCE == MF_BUCKETS_OFFSET) {
-      qo = static_cast<const int64_t*>(p.query_pos)[b * p.query_step + i];
-    }
+  if (SOURCE == MF_BUCKETS_DISTANCE && i < p.Nq) {
+    const float* c = static_cast<const float*>(p.query_pos) + b * p.query_step + int64_t(i) * 3;
+    qx = c[0];
+    qy = c[1];
+    qz = c[2];
   }
-  // OFFSET: positions relative to the tile's first key; where all of a wave's are within 2^29 their differences are formed
-  // in 32 bits, and if the least and the greatest of those that count have one bucket the wave's rows have no other
-  bool near = true, whole = false;
-  int q32 = 0, whole_code = 0;
-  if constexpr (SOURCE == MF_BUCKETS_OFFSET) {
-    const int64_t* kp = static_cast<const int64_t*>(p.key_pos) + b * p.key_step;
-    const int64_t base = kp[kt * kTile], mine = jl < p.Nk ? kp[jl] : base;
-    const int64_t dk = mine - base, dq = i < p.Nq ? qo - base : 0;
-    constexpr int64_t kNear = int64_t(1) << 29;
-    const bool keys_near = !__any(!(dk > -kNear && dk < kNear));  // (one answer for the workgroup)
-    near = keys_near && !__any(!(dq > -kNear && dq < kNear));
-    if (wave == 0) {
-      s_off[lane] = mine;
-      if (keys_near) s_off32[lane] = int(dk);
-    }
-    if (near) {
-      q32 = int(dq);
-      const bool key_in = (keys >> lane) & 1;
-      int klo = key_in ? int(dk) : INT32_MAX, khi = key_in ? int(dk) : INT32_MIN;
-      int qlo = row_on ? q32 : INT32_MAX, qhi = row_on ? q32 : INT32_MIN;
-#pragma unroll
-      for (int off = 32; off >= 1; off >>= 1) {
-        klo = min(klo, __shfl_xor(klo, off, 64));
-        khi = max(khi, __shfl_xor(khi, off, 64));
-        qlo = min(qlo, __shfl_xor(qlo, off, 64));
-        qhi = max(qhi, __shfl_xor(qhi, off, 64));
-      }
-      if (klo <= khi && qlo <= qhi) {
-        const int low = klo - qhi, high = khi - qlo;  // the least and the greatest offset
-        if (p.causal && low > 0) {
-          whole = true;
-          whole_code = kMasked;
-        } else if (!(p.causal && high > 0)) {
-          int nl = 0, nh = 0;
-          for (int e = lane; e < p.buckets - 1; e += 64) {
-            nl += double(low) >= p.edges[e];
-            nh += double(high) >= p.edges[e];
-          }
-          nl = __popcll(__ballot(nl != 0));
-          nh = __popcll(__ballot(nh != 0));
-          whole = nl == nh;
-          whole_code = nl;
-        }
-      } else {
-        whole = true;
-        whole_code = kMasked;
-      }
-    }
+  if constexpr (SOURCE != MF_BUCKETS_OFFSET) {
+    keys = __ballot(key_out == 0);
+    queries = __ballot(query_out == 0);
   }
   __syncthreads();
   uint32_t w[4] = {0x40404040u, 0x40404040u, 0x40404040u, 0x40404040u};  // kMasked
-  const uint32_t mine = row_on ? uint32_t(keys >> c0) & 0xffffu : 0u;
-  if (SOURCE == MF_BUCKETS_OFFSET && whole) {
-#pragma unroll
-    for (int t = 0; t < 16; ++t) {
-      const uint32_t code = (mine >> t) & 1 ? uint32_t(whole_code) : uint32_t(kMasked);
-      w[t >> 2] = (w[t >> 2] & ~(255u << (8 * (t & 3)))) | code << (8 * (t & 3));
-    }
-  } else if (mine != 0) {
+  const uint32_t mine = (queries >> r) & 1 ? uint32_t(keys >> c0) & 0xffffu : 0u;
+  if (mine != 0) {
 #pragma unroll
     for (int t = 0; t < 16; ++t) {
       const int j = kt * kTile + c0 + t;
@@ -710,10 +732,16 @@ extern "C" int mf_pair_buckets(const mf_pair_buckets_args* a, void* stream) {
       p.cells[c] = uint8_t(e);
     }
   }
-  p.tiles = p.symmetric ? int64_t(a->batch) * p.TK * (p.TK + 1) / 2 : int64_t(a->batch) * p.TQ * p.TK;
+  const int64_t per = p.symmetric ? int64_t(p.TK) * (p.TK + 1) / 2 : int64_t(p.TQ) * p.TK;
+  if (per >= (int64_t(1) << 30) || a->batch * per >= kCounts)  // (bytes past 2^42, and 80 a tile and more)
+    return fail(MF_ERR_UNSUPPORTED, "mf_pair_buckets: batch * queries * keys too large");
+  const int64_t tiles = a->batch * per;
+  p.tiles = uint32_t(tiles);
+  p.per = uint32_t(per);
   constexpr int64_t kMost = int64_t(1) << 23;  // workgroups of a launch
-  for (p.first = 0; p.first < p.tiles; p.first += kMost) {
-    const dim3 grid(unsigned((std::min(kMost, p.tiles - p.first) + 7) / 8 * 8));
+  for (int64_t first = 0; first < tiles; first += kMost) {
+    p.first = uint32_t(first);
+    const dim3 grid(unsigned((std::min(kMost, tiles - first) + 7) / 8 * 8));
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (a->source == MF_BUCKETS_DISTANCE)
       hipLaunchKernelGGL(pair_buckets_kernel<MF_BUCKETS_DISTANCE>, grid, dim3(kThreads), 0, s, p);
