@@ -7,7 +7,9 @@
 // through LDS the same tile transposed, with the words that say which of its
 // keys and queries have a pair at all.  Distances are compared as squares, in
 // fp64 without contraction, so that the bucket is that of the exact distance of
-// the fp32 coordinates but for the roundings of fp64.
+// the fp32 coordinates but for the roundings of fp64.  Bound by the vector
+// instructions of distances (8 cells of 1997 atoms: 25 us), by the writes of
+// offsets, most of whose tiles have one bucket (2 x 8192^2 in both layouts, 268 MB: 67).
 //
 // bucket_bias_kernel: a thread reads the buckets of 16 bytes of bias once and
 // writes them for every head; the tables lie in LDS, one bank a bucket.  Bound
@@ -51,7 +53,8 @@ struct BucketParams {
   int64_t query_step, key_step;
   double cutoff;
   uint32_t first, tiles;  // workgroups before this launch's, and in all
-  uint32_t per;           // symmetric: of a batch entry
+  uint32_t per;           // of a batch entry
+  uint32_t grid;          // of this launch
   int symmetric;         // index_t is index: tiles on and above the diagonal, each written twice
   int buckets, causal, Nq, Nk, TQ, TK;
   int base, shift;
@@ -108,7 +111,15 @@ __global__ void __launch_bounds__(kThreads) pair_buckets_kernel(BucketParams p) 
   __shared__ int s_off32[SOURCE == MF_BUCKETS_OFFSET ? kTile : 1];
   __shared__ uint8_t tile[kTile][kTile + 4];
   __shared__ uint64_t s_key[4], s_qry[4];
-  const uint32_t id = xcd_order(blockIdx.x, gridDim.x) + p.first;
+  // (asked for together: one by one, each waits for its own line of the arguments)
+  asm volatile("" ::"s"(p.index), "s"(p.key_pos), "s"(p.TK), "s"(p.base), "s"(p.tiles), "s"(p.grid), "s"(p.key_any));
+  uint32_t cells_in = 0;
+  double edge_in = 0.0;
+  if constexpr (SOURCE == MF_BUCKETS_DISTANCE || SOURCE == MF_BUCKETS_VALUE) {
+    cells_in = reinterpret_cast<const uint32_t*>(p.cells)[threadIdx.x];
+    edge_in = p.edges[threadIdx.x & (MF_MAX_BUCKETS - 1)];
+  }
+  const uint32_t id = xcd_order(blockIdx.x, p.grid) + p.first;
   if (id >= p.tiles) return;
   uint32_t qt, kt;
   int64_t b;
@@ -120,9 +131,13 @@ __global__ void __launch_bounds__(kThreads) pair_buckets_kernel(BucketParams p) 
     if ((kt + 1) * (kt + 2) / 2 <= t) ++kt;
     qt = t - kt * (kt + 1) / 2;
   } else {
-    const uint32_t row = id / uint32_t(p.TK), entry = row / uint32_t(p.TQ);
-    kt = id - row * uint32_t(p.TK);
-    qt = row - entry * uint32_t(p.TQ);
+    // two tiles by two follow one another: together they write whole lines of both layouts (two orders of 8192 places: 67 us;
+    // by rows 81, eight by one 73)
+    const uint32_t entry = id / p.per, in_entry = id - entry * p.per;
+    const uint32_t pair = in_entry / (2 * uint32_t(p.TK)), in_pair = in_entry - pair * 2 * uint32_t(p.TK);
+    const uint32_t both = 2 * pair + 1 < uint32_t(p.TQ);
+    kt = in_pair >> both;
+    qt = 2 * pair + (in_pair & both);
     b = entry;
   }
   const int tid = threadIdx.x, r = tid >> 2, c0 = (tid & 3) * 16;
@@ -186,11 +201,14 @@ __global__ void __launch_bounds__(kThreads) pair_buckets_kernel(BucketParams p) 
     else if (i < p.Nq) qo = qp[i];
   }
   if constexpr (SOURCE != MF_BUCKETS_INDEX) {
-    s_cells[tid] = reinterpret_cast<const uint32_t*>(p.cells)[tid];
+    if constexpr (SOURCE == MF_BUCKETS_OFFSET) {
+      cells_in = reinterpret_cast<const uint32_t*>(p.cells)[tid];
+      edge_in = p.edges[tid & (MF_MAX_BUCKETS - 1)];
+    }
+    s_cells[tid] = cells_in;
     if (tid < MF_MAX_BUCKETS) {
-      const double e = p.edges[tid];
-      if constexpr (SOURCE == MF_BUCKETS_OFFSET) s_edges[tid] = e == e ? int64_t(e) : INT64_MAX;
-      else s_edges[tid] = e;
+      if constexpr (SOURCE == MF_BUCKETS_OFFSET) s_edges[tid] = edge_in == edge_in ? int64_t(edge_in) : INT64_MAX;
+      else s_edges[tid] = edge_in;
     }
   }
   if (SOURCE == MF_BUCKETS_DISTANCE && tid < 3 * kTile) {
@@ -741,7 +759,8 @@ extern "C" int mf_pair_buckets(const mf_pair_buckets_args* a, void* stream) {
   constexpr int64_t kMost = int64_t(1) << 23;  // workgroups of a launch
   for (int64_t first = 0; first < tiles; first += kMost) {
     p.first = uint32_t(first);
-    const dim3 grid(unsigned((std::min(kMost, tiles - first) + 7) / 8 * 8));
+    p.grid = unsigned((std::min(kMost, tiles - first) + 7) / 8 * 8);
+    const dim3 grid(p.grid);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (a->source == MF_BUCKETS_DISTANCE)
       hipLaunchKernelGGL(pair_buckets_kernel<MF_BUCKETS_DISTANCE>, grid, dim3(kThreads), 0, s, p);
