@@ -331,8 +331,11 @@ __global__ void __launch_bounds__(64 * W, (DP == 128 && (KEYS || W == 2)) || (W 
     if (KEYS) up *= 1.0f / kProb;  // P comes times kProb
   }
   const float slog = p.scale * kLog2e;
-  const uint8_t* codes = (KEYS ? p.index_t + b * p.index_t_step + int64_t(at) * p.St
-                               : p.index + b * p.index_step + int64_t(at) * p.S) + 16 * half;
+  // the columns' buckets: rows of the workgroup's first column on, the lane's row below 2^31 bytes further
+  const int first = ct * 32 * W;
+  const uint8_t* codes = KEYS ? p.index_t + b * p.index_t_step + int64_t(first) * p.St
+                              : p.index + b * p.index_step + int64_t(first) * p.S;
+  const uint32_t code_row = uint32_t(min(col, N - 1) - first) * uint32_t(KEYS ? p.St : p.S) + 16 * half;
 
   mf_f32x16 ax[ND], ay[ND];
 #pragma unroll
@@ -341,7 +344,6 @@ __global__ void __launch_bounds__(64 * W, (DP == 128 && (KEYS || W == 2)) || (W 
 
   const char *tx = nullptr, *ty = nullptr, *tr = nullptr;
   const unsigned xstride = unsigned(KEYS ? p.qs[2] : p.ks[2]) * 2, ystride = unsigned(KEYS ? p.gs[2] : p.vs[2]) * 2;
-  const TileCopy<DP, W> xcopy(xstride, p.D, wave, lane), ycopy(ystride, p.D, wave, lane);
   auto side = [&](int h) {  // the streamed side of query head h
     if (KEYS) {
       tx = reinterpret_cast<const char*>(static_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[1]);
@@ -352,7 +354,21 @@ __global__ void __launch_bounds__(64 * W, (DP == 128 && (KEYS || W == 2)) || (W 
       ty = reinterpret_cast<const char*>(static_cast<const T*>(p.v) + b * p.vs[0] + kv * p.vs[1]);
     }
   };
+  // The copies' offsets are formed for every tile where registers are short: spilled, they came back in between the copies,
+  // each of which then waited for the one before.
+  constexpr bool kShort = KEYS && SUMS && DP == 64;
+  auto copies = [&] {
+    int l = lane;
+    if constexpr (kShort) asm volatile("" : "+v"(l));  // (not the ones of the last tile)
+    struct Both {
+      TileCopy<DP, W> x, y;
+    };
+    return Both{TileCopy<DP, W>(xstride, p.D, wave, l), TileCopy<DP, W>(ystride, p.D, wave, l)};
+  };
+  const auto kept = copies();
   auto load = [&](int tile, uint64_t set, int buffer, uint4 (&w)[2]) {
+    const auto now = kShort ? copies() : kept;
+    const TileCopy<DP, W>&xcopy = now.x, &ycopy = now.y;
     xcopy.copy(tx + int64_t(tile) * kTile * xstride, set, s_tiles + buffer, wave, lane);
     ycopy.copy(ty + int64_t(tile) * kTile * ystride, set, s_tiles + buffer + kBytes, wave, lane);
     if (KEYS && wave == 0) {
@@ -362,9 +378,8 @@ __global__ void __launch_bounds__(64 * W, (DP == 128 && (KEYS || W == 2)) || (W 
 #pragma unroll
       for (int n = 0; n < 3; ++n) lds_copy4(src, on ? lane * 4u + n * kTile * 4u : kLdsCopyOutside, lr + n * kTile);
     }
-    w[0] = *reinterpret_cast<const uint4*>(codes + int64_t(tile) * kTile);
-    w[1] = *reinterpret_cast<const uint4*>(codes + int64_t(tile) * kTile + 32);
-    if (KEYS && !in) w[0] = w[1] = make_uint4(0x40404040u, 0x40404040u, 0x40404040u, 0x40404040u);  // kMasked
+    w[0] = *reinterpret_cast<const uint4*>(codes + int64_t(tile) * kTile + code_row);
+    w[1] = *reinterpret_cast<const uint4*>(codes + int64_t(tile) * kTile + code_row + 32);
   };
 
   for (int g = 0; g < (KEYS ? p.G : 1); ++g) {
@@ -400,7 +415,8 @@ __global__ void __launch_bounds__(64 * W, (DP == 128 && (KEYS || W == 2)) || (W 
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
         if (uint32_t(now >> (32 * kb)) == 0) continue;  // no pair in these 32 rows
-        const uint32_t word[4] = {w[kb].x, w[kb].y, w[kb].z, w[kb].w};
+        uint32_t word[4] = {w[kb].x, w[kb].y, w[kb].z, w[kb].w};
+        if (KEYS && !in) word[0] = word[1] = word[2] = word[3] = 0x40404040u;  // kMasked (not in load, which would wait for them)
         Op xa[NK], ya[NK], xt[2][ND], yt[2][ND];
         float bias[16];
         mf_f32x16 s = zeros16(), d;  // d: dP - delta, -delta as the sum's start
