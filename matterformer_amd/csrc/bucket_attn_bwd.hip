@@ -148,8 +148,8 @@ __global__ void __launch_bounds__(kRowThreads) bucket_rows_kernel(BwdParams p) {
   }
   if (p.peak) {
     __shared__ float2 s[4];
-    top = wave_max(top);
-    ltop = wave_max(ltop);
+    top = wave_peak(top);
+    ltop = wave_peak(ltop);
     if (lane == 0) s[wave] = make_float2(top, ltop);
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -171,7 +171,7 @@ __device__ __forceinline__ int scale_bits(const BwdParams& p, int64_t b, int kv)
   }
   const float4* v = p.peak + int64_t(p.B) * p.H * p.TQ + (b * p.KV + kv) * p.TK;
   for (int i = lane; i < p.TK; i += 64) vm = fmaxf(vm, v[i].x);
-  const float bound = 2.0f * sqrtf(wave_max(gm)) * sqrtf(wave_max(vm)) + wave_max(lm);
+  const float bound = 2.0f * sqrtf(wave_peak(gm)) * sqrtf(wave_peak(vm)) + wave_peak(lm);
   return bound > 0.0f && bound < 3.0e38f ? min(60, max(-60, 12 - ilogbf(bound))) : 0;
 }
 
@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(64 * W, (DP == 128 && (KEYS || W == 2)) || (W 
         float v = 0.0f;
 #pragma unroll
         for (int u = 0; u < W; ++u) v += s_bins[c * 64 * W + u * 64 + lane];
-        v = wave_sum(v) * (kHalf ? 1.0f / kProb : 1.0f);
+        v = wave_total(v) * (kHalf ? 1.0f / kProb : 1.0f);
         if (lane == 0) slot[c * slots] = v;
       }
       __syncthreads();  // the next head clears them

@@ -53,6 +53,30 @@ __device__ __forceinline__ float pair_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// All lanes' values joined, in every lane; none: what joins to nothing.  Six instructions that hand values from lane to lane,
+// where shuffles go through LDS one after the other (a wave's sum: about 60 clocks instead of 800).
+template <typename Join>
+__device__ __forceinline__ int wave_join(int v, int none, Join join) {
+  v = join(v, __builtin_amdgcn_update_dpp(none, v, 0x111, 0xf, 0xf, false));  // rows of 16 lanes: 1, 2, 4, 8 further on
+  v = join(v, __builtin_amdgcn_update_dpp(none, v, 0x112, 0xf, 0xf, false));
+  v = join(v, __builtin_amdgcn_update_dpp(none, v, 0x114, 0xf, 0xf, false));
+  v = join(v, __builtin_amdgcn_update_dpp(none, v, 0x118, 0xf, 0xf, false));
+  v = join(v, __builtin_amdgcn_update_dpp(none, v, 0x142, 0xa, 0xf, false));  // a row's last lane to the next row
+  v = join(v, __builtin_amdgcn_update_dpp(none, v, 0x143, 0xc, 0xf, false));  // the first half's to the second
+  return __builtin_amdgcn_readlane(v, 63);
+}
+__device__ __forceinline__ float wave_total(float v) {
+  return __int_as_float(wave_join(__float_as_int(v), 0, [](int a, int b) {
+    return __float_as_int(__int_as_float(a) + __int_as_float(b));
+  }));
+}
+// Of values that are not negative.
+__device__ __forceinline__ float wave_peak(float v) {
+  return __int_as_float(wave_join(__float_as_int(v), 0, [](int a, int b) {
+    return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b)));
+  }));
+}
+
 // Row of a 32-row block that lane m of an A operand stands for.
 __device__ __forceinline__ int block_row(int m) { return 16 * ((m >> 2) & 1) + 4 * (m >> 3) + (m & 3); }
 
@@ -171,9 +195,9 @@ struct Tiles {
 __device__ __forceinline__ uint64_t union_of(const uint64_t* table, int pitch, int column, int first, int end) {
   uint64_t u = 0;
   for (int t = first + int(threadIdx.x & 63); t < end; t += 64) u |= table[int64_t(t) * pitch + column];
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) u |= __shfl_xor((unsigned long long)u, off, 64);
-  return u;
+  auto either = [](int a, int b) { return a | b; };
+  return uint64_t(uint32_t(wave_join(int(uint32_t(u)), 0, either))) |
+         uint64_t(uint32_t(wave_join(int(uint32_t(u >> 32)), 0, either))) << 32;
 }
 
 // The bias tables of `heads` heads from `first` on, in log2 units: entries past the buckets are -inf, and a finite entry

@@ -79,15 +79,7 @@ __host__ __device__ __forceinline__ int cell_of(float x, int base, int shift) {
 // The least and the greatest of a wave's values.
 template <bool LEAST>
 __device__ __forceinline__ int wave_end(int v) {
-  constexpr int kNone = LEAST ? INT32_MAX : INT32_MIN;
-  auto join = [](int a, int b) { return LEAST ? min(a, b) : max(a, b); };
-  v = join(v, __builtin_amdgcn_update_dpp(kNone, v, 0x111, 0xf, 0xf, false));  // rows of 16 lanes: 1, 2, 4, 8 further on
-  v = join(v, __builtin_amdgcn_update_dpp(kNone, v, 0x112, 0xf, 0xf, false));
-  v = join(v, __builtin_amdgcn_update_dpp(kNone, v, 0x114, 0xf, 0xf, false));
-  v = join(v, __builtin_amdgcn_update_dpp(kNone, v, 0x118, 0xf, 0xf, false));
-  v = join(v, __builtin_amdgcn_update_dpp(kNone, v, 0x142, 0xa, 0xf, false));  // a row's last lane to the next row
-  v = join(v, __builtin_amdgcn_update_dpp(kNone, v, 0x143, 0xc, 0xf, false));  // the first half's to the second
-  return __builtin_amdgcn_readlane(v, 63);
+  return wave_join(v, LEAST ? INT32_MAX : INT32_MIN, [](int a, int b) { return LEAST ? min(a, b) : max(a, b); });
 }
 
 // 16 bytes: a code where the mask has a bit, kMasked where not.
@@ -585,7 +577,7 @@ __global__ void __launch_bounds__(kThreads) bucket_bias_bwd_kernel(BiasParams p)
   __syncthreads();
   for (int n = tid >> 6; n < p.K; n += kThreads / 64) {
     const float* s = s_bins + n * kThreads + (tid & 63);
-    const float v = wave_sum((s[0] + s[64]) + (s[128] + s[192]));
+    const float v = wave_total((s[0] + s[64]) + (s[128] + s[192]));
     if ((tid & 63) == 0) p.parts[(int64_t(h) * p.K + n) * p.pieces + blockIdx.x] = v;
   }
 }
