@@ -13,7 +13,7 @@
 //
 // bucket_bias_kernel: a thread reads the buckets of 16 bytes of bias once and
 // writes them for every head; the tables lie in LDS, one bank a bucket.  Bound
-// by its writes (4 x 12 planes of 1997^2 in bf16, 383 MB: 71 us).
+// by its writes (4 x 12 planes of 1997^2 in bf16, 383 MB: 69 us).
 //
 // bucket_bias_bwd_kernel: sums by bucket without atomics between lanes.  Every
 // lane keeps a sum per bucket of its own in LDS ([bucket][thread]: one bank a
@@ -22,7 +22,7 @@
 // workgroups' in fp64.  Two calls give identical bits.  A sum is read, added to
 // and written: 9 clocks a wave, where an fp32 atomic of LDS takes 193.  Bound by
 // the time that takes at the eight waves a CU that the sums leave room for (bf16,
-// same planes: 149 us; fp32, twice the bytes, 150).
+// same planes: 140 us; fp32, twice the bytes, 150).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(kThreads) pair_buckets_kernel(BucketParams p) 
 // Both kernels walk a plane (one batch entry and head, Nq Nk entries) in its flat order, so that their accesses to the bias
 // are 16 bytes and aligned whatever Nk is: where Nk is odd, planes and rows start off 16 bytes, and accesses that cross
 // such a boundary cost the memory pipeline twice (by rows, 4 x 12 x 1997^2 in bf16: bias 114 us instead of 71, its
-// gradient 180 instead of 149).  The buckets' rows are padded, so a run of them may have to be put
+// gradient 180 instead of 163).  The buckets' rows are padded, so a run of them may have to be put
 // together from the ends of two rows.
 struct BiasParams {
   const uint8_t* index;
