@@ -222,6 +222,7 @@ __global__ void __launch_bounds__(kThreads) pair_buckets_kernel(BucketParams p) 
   uint32_t w[4] = {0x40404040u, 0x40404040u, 0x40404040u, 0x40404040u};  // kMasked
   const uint32_t mine = (queries >> r) & 1 ? uint32_t(keys >> c0) & 0xffffu : 0u;
   if (mine != 0) {
+    w[0] = w[1] = w[2] = w[3] = 0;
 #pragma unroll
     for (int t = 0; t < 16; ++t) {
       const int j = kt * kTile + c0 + t;
@@ -255,12 +256,16 @@ __global__ void __launch_bounds__(kThreads) pair_buckets_kernel(BucketParams p) 
           x = in ? static_cast<const float*>(p.values)[(b * p.Nq + i) * p.Nk + j] : 0.0f;
         }
         on = on && !(p.cutoff >= 0.0 && x > p.cutoff);
-        unsigned n = reinterpret_cast<const uint8_t*>(s_cells)[cell_of(float(x), p.base, p.shift)];
-        if (x != x) n = 0;
+        // (a NaN has the first cell and passes no edge; squares are their own order)
+        const float low = fmaxf(float(x), SOURCE == MF_BUCKETS_DISTANCE ? 0.0f : -INFINITY);
+        const int cell = SOURCE == MF_BUCKETS_DISTANCE
+                             ? min(max((__float_as_int(low) >> p.shift) - p.base, 0), kCells - 1)
+                             : cell_of(low, p.base, p.shift);
+        unsigned n = reinterpret_cast<const uint8_t*>(s_cells)[cell];
         while (x >= s_edges[n]) ++n;  // (not past the NaN at the end)
         if (on) code = n;
       }
-      w[t >> 2] = (w[t >> 2] & ~(255u << (8 * (t & 3)))) | code << (8 * (t & 3));
+      w[t >> 2] |= code << (8 * (t & 3));
     }
   }
   const bool any = (w[0] & w[1] & w[2] & w[3]) != 0x40404040u;  // (a bucket has no bit 6)
