@@ -8,7 +8,7 @@
 // keys and queries have a pair at all.  Distances are compared as squares, in
 // fp64 without contraction, so that the bucket is that of the exact distance of
 // the fp32 coordinates but for the roundings of fp64.  Bound by the vector
-// instructions of distances (8 cells of 1997 atoms: 25 us), by the writes of
+// instructions of distances (8 cells of 1997 atoms: 24 us), by the writes of
 // offsets, most of whose tiles have one bucket (2 x 8192^2 in both layouts, 268 MB: 67).
 //
 // bucket_bias_kernel: a thread reads the buckets of 16 bytes of bias once and
