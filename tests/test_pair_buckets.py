@@ -242,6 +242,14 @@ def test_buckets_entry_refuses_before_any_device_call():
     assert lib.mf_pair_buckets(args(batch=0), None) == _native.MF_OK
 
 
+def test_more_tiles_than_32_bits_count_are_refused():
+    args = _native.MfPairBucketsArgs(values=FAKE, index=FAKE, index_t=2 * FAKE, key_any=3 * FAKE, query_any=4 * FAKE,
+                                     source=_native.MF_BUCKETS_INDEX, buckets=4, batch=2 ** 30, queries=65, keys=65)
+    refused(_native.lib().mf_pair_buckets, args, UNSUPPORTED, "too large")
+    args.batch, args.queries, args.keys = 1, 2 ** 24, 2 ** 24
+    refused(_native.lib().mf_pair_buckets, args, UNSUPPORTED, "too large")
+
+
 def test_bias_entries_refuse_before_any_device_call():
     lib = _native.lib()
 
