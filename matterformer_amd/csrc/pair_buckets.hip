@@ -21,7 +21,7 @@
 // the threads' sums are joined in a fixed order, and table_sum_kernel joins the
 // workgroups' in fp64.  Two calls give identical bits.  A sum is read, added to
 // and written: 9 clocks a wave, where an fp32 atomic of LDS takes 193.  Bound by
-// the time that takes at the eight waves a CU that the sums leave room for (bf16,
+// the time that takes at the nine waves a CU that the sums leave room for (bf16,
 // same planes: 140 us; fp32, twice the bytes, 150).
 #include <algorithm>
 #include <cmath>
@@ -33,6 +33,9 @@ namespace mf {
 namespace bucket {
 
 constexpr int kThreads = 256;
+// Of bucket_bias_bwd_kernel: 50 KB of sums at 64 buckets, three workgroups and nine waves a CU.  (256, two and eight: bias and
+// gradient of 4 x 12 x 1997^2 in bf16 209 us instead of 207.)
+constexpr int kSumThreads = 192;
 
 // Bucket of a value: a table by the leading bits of its fp32 rounding (an order-preserving integer) gives how many edges
 // lie in lower cells; those in the value's own cell, mostly none or one, are compared with it.  1024 cells over the
@@ -468,15 +471,15 @@ __global__ void __launch_bounds__(kThreads) bucket_bias_kernel(BiasParams p) {
 // A workgroup sums a piece of one head's chunks, a thread 16 entries at a time, the next ones loaded while the last ones are
 // added.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) bucket_bias_bwd_kernel(BiasParams p) {
-  extern __shared__ float s_bins[];  // [K + 1][kThreads]; the last one takes the masked pairs
+__global__ void __launch_bounds__(kSumThreads) bucket_bias_bwd_kernel(BiasParams p) {
+  extern __shared__ float s_bins[];  // [K + 1][kSumThreads]; the last one takes the masked pairs
   constexpr int V = 16 / sizeof(T), kKeys = 16;
   using Bits = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
   auto value = [](const uint32_t* words, int t) {
     return float(__builtin_bit_cast(T, Bits(sizeof(T) == 4 ? words[t] : words[t >> 1] >> (16 * (t & 1)))));
   };
   const int tid = threadIdx.x;
-  for (int c = 0; c <= p.K; ++c) s_bins[c * kThreads + tid] = 0.0f;
+  for (int c = 0; c <= p.K; ++c) s_bins[c * kSumThreads + tid] = 0.0f;
   const int h = blockIdx.y;
   float* bins = s_bins + tid;
 
@@ -493,14 +496,14 @@ __global__ void __launch_bounds__(kThreads) bucket_bias_bwd_kernel(BiasParams p)
     row = from < 0 ? 0 : divide(from, p.Nk);
     col = int(from - row * p.Nk);
   };
-  const int rows_on = kThreads * kKeys / p.Nk, cols_on = kThreads * kKeys - rows_on * p.Nk;
+  const int rows_on = kSumThreads * kKeys / p.Nk, cols_on = kSumThreads * kKeys - rows_on * p.Nk;
   auto advance = [&] {
-    id += kThreads;
-    n += kThreads;
+    id += kSumThreads;
+    n += kSumThreads;
     if (n >= p.chunks) {
       enter();
     } else {
-      from += kThreads * kKeys;
+      from += kSumThreads * kKeys;
       row += rows_on;
       col += cols_on;
       if (col >= p.Nk) {
@@ -572,17 +575,17 @@ __global__ void __launch_bounds__(kThreads) bucket_bias_bwd_kernel(BiasParams p)
       const int c0 = min(int(byte_of(w, t)), p.K), c1 = min(int(byte_of(w, t + 1)), p.K);
       const float v0 = value(y, t), v1 = value(y, t + 1);
       const bool same = c0 == c1;
-      float* b0 = bins + c0 * kThreads;
-      float* b1 = bins + (same ? p.K : c1) * kThreads;
+      float* b0 = bins + c0 * kSumThreads;
+      float* b1 = bins + (same ? p.K : c1) * kSumThreads;
       const float s0 = *b0, s1 = *b1;
       *b0 = s0 + (same ? v0 + v1 : v0);
       *b1 = s1 + v1;
     }
   }
   __syncthreads();
-  for (int n = tid >> 6; n < p.K; n += kThreads / 64) {
-    const float* s = s_bins + n * kThreads + (tid & 63);
-    const float v = wave_total((s[0] + s[64]) + (s[128] + s[192]));
+  for (int n = tid >> 6; n < p.K; n += kSumThreads / 64) {
+    const float* s = s_bins + n * kSumThreads + (tid & 63);
+    const float v = wave_total((s[0] + s[64]) + s[128]);
     if ((tid & 63) == 0) p.parts[(int64_t(h) * p.K + n) * p.pieces + blockIdx.x] = v;
   }
 }
@@ -659,15 +662,15 @@ BiasParams bias_params(const mf_bucket_bias_args* a) {
 }
 
 // The chunks of 16 entries of a head, and how many of them a workgroup sums: four a thread and more, and no more workgroups
-// than are resident at two a CU (66 KB of LDS each) twice over.
+// than are resident at three a CU (50 KB of LDS each) twice over.
 void bias_pieces(const mf_bucket_bias_args* a, BiasParams& p) {
   const int V = a->bias_dtype == MF_DTYPE_F32 ? 4 : 8;
   p.plane = int64_t(a->queries) * a->keys;
   p.chunks = (p.plane + 15) / 16 + (p.plane % V != 0);
   p.total = p.chunks * a->batch;
-  const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>((p.total + 4 * kThreads - 1) / (4 * kThreads),
-                                                                std::max(1, 1024 / std::max(1, a->heads))));
-  p.piece = ((p.total + pieces - 1) / pieces + kThreads - 1) / kThreads * kThreads;
+  const int64_t pieces = std::max<int64_t>(1, std::min<int64_t>((p.total + 4 * kSumThreads - 1) / (4 * kSumThreads),
+                                                                std::max(1, 1536 / std::max(1, a->heads))));
+  p.piece = ((p.total + pieces - 1) / pieces + kSumThreads - 1) / kSumThreads * kSumThreads;
   p.pieces = int((p.total + p.piece - 1) / p.piece);
 }
 
@@ -827,17 +830,17 @@ extern "C" int mf_bucket_bias_bwd(const mf_bucket_bias_args* a, void* stream) {
   bias_pieces(a, p);
   p.parts = static_cast<float*>(a->workspace);
   const dim3 grid(unsigned(p.pieces), unsigned(a->heads));
-  const int lds = (a->buckets + 1) * kThreads * int(sizeof(float));
+  const int lds = (a->buckets + 1) * kSumThreads * int(sizeof(float));
   const void* fn = a->bias_dtype == MF_DTYPE_F32    ? reinterpret_cast<const void*>(bucket_bias_bwd_kernel<float>)
                    : a->bias_dtype == MF_DTYPE_BF16 ? reinterpret_cast<const void*>(bucket_bias_bwd_kernel<__bf16>)
                                                     : reinterpret_cast<const void*>(bucket_bias_bwd_kernel<_Float16>);
-  if (const int status = ensure_dynamic_lds(fn, (MF_MAX_BUCKETS + 1) * kThreads * int(sizeof(float)))) return status;
+  if (const int status = ensure_dynamic_lds(fn, (MF_MAX_BUCKETS + 1) * kSumThreads * int(sizeof(float)))) return status;
   if (a->bias_dtype == MF_DTYPE_F32)
-    hipLaunchKernelGGL(bucket_bias_bwd_kernel<float>, grid, dim3(kThreads), lds, s, p);
+    hipLaunchKernelGGL(bucket_bias_bwd_kernel<float>, grid, dim3(kSumThreads), lds, s, p);
   else if (a->bias_dtype == MF_DTYPE_BF16)
-    hipLaunchKernelGGL(bucket_bias_bwd_kernel<__bf16>, grid, dim3(kThreads), lds, s, p);
+    hipLaunchKernelGGL(bucket_bias_bwd_kernel<__bf16>, grid, dim3(kSumThreads), lds, s, p);
   else
-    hipLaunchKernelGGL(bucket_bias_bwd_kernel<_Float16>, grid, dim3(kThreads), lds, s, p);
+    hipLaunchKernelGGL(bucket_bias_bwd_kernel<_Float16>, grid, dim3(kSumThreads), lds, s, p);
   MF_HIP_CHECK(hipGetLastError());
   return launch_table_sum(p.parts, a->dtable, a->heads, a->buckets, p.pieces, a->table_dtype, s);
 }
