@@ -306,3 +306,52 @@ def test_a_gradient_off_16_bytes(cuda):
     (grad,) = torch.autograd.grad(bias, table, go, retain_graph=True)
     (same,) = torch.autograd.grad(bias, table, go.clone())
     assert torch.equal(grad, same)
+
+
+# edges within 1024 steps of fp32 of each other: one, neighbours, of either sign, at zero and at the ends of the range
+CLOSE_OFFSETS = [[1], [3], [64], [-64], [-3, -2], [-1, 0, 1], [5, 6, 7], [1000000, 1000001, 1000002],
+                 [-1000002, -1000001, -1000000], [2 ** 40], [-(2 ** 53)], [2 ** 53 - 1, 2 ** 53]]
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("edges", CLOSE_OFFSETS, ids=str)
+def test_offsets_of_both_signs_about_close_edges(cuda, edges, causal):
+    """Whole tiles of one bucket on either side of the diagonal, near places in no order, and places far apart."""
+    g = torch.Generator().manual_seed(abs(edges[0]) % 1000)
+    in_order = torch.arange(200)
+    near = torch.randint(-100, 100, (2, 150), generator=g)
+    far = torch.tensor([0, 2, 5, -7, 10 ** 6, 10 ** 6 + 1, -(10 ** 6), 2 ** 31, -(2 ** 31), 2 ** 40, -(2 ** 40), 2 ** 53, -(2 ** 53),
+                        2 ** 61, -(2 ** 61)])
+    for p in (in_order, near, far):
+        same(offset_buckets(p.to(cuda), p.to(cuda), edges, causal=causal), offset_buckets(p, p, edges, causal=causal))
+    one = torch.tensor([100])
+    same(offset_buckets(one.to(cuda), in_order.to(cuda), edges, causal=causal, gradients=False),
+         offset_buckets(one, in_order, edges, causal=causal, gradients=False))
+
+
+def close_values():
+    ends = [1e-45, 1e-38, 1.0, 3.5, 1e20, torch.finfo(torch.float32).max]
+    single = [[s * e] for e in ends for s in (1.0, -1.0)] + [[0.0], [-0.0]]
+    up = lambda x: torch.nextafter(torch.tensor(x), torch.tensor(math.inf)).item()
+    return single + [[x, up(x), up(up(x))] for x in (1.0, -1.0, 1000.0, -1000.0, 0.0, -1e-45)]
+
+
+@pytest.mark.parametrize("edges", close_values(), ids=str)
+def test_values_of_both_signs_about_close_edges(cuda, edges):
+    g = torch.Generator().manual_seed(3)
+    values = torch.randn(2, 70, 90, generator=g) * torch.tensor([1.0, 1e4])[:, None, None]
+    special = [0.0, -0.0, 1e-45, -1e-45, 1e-38, -1e-38, math.inf, -math.inf, math.nan, 3.4e38, -3.4e38, *edges,
+               *(-e for e in edges)]
+    values[0, 0, :len(special)] = torch.tensor(special)
+    for cutoff in (None, 2.0):
+        got = value_buckets(values.to(cuda), edges, cutoff=cutoff)
+        same(got, value_buckets(values, edges, cutoff=cutoff))
+    assert got.index[0, 0, special.index(math.inf)] == MASKED and got.index[0, 0, 8] == 0  # above the cutoff; a NaN
+
+
+def test_a_bias_about_one_edge(cuda):
+    """What the buckets are read for: keys before the query have the first entry, those behind it the second."""
+    places = torch.arange(150, device=cuda)
+    table = torch.tensor([[1.0], [2.0]], device=cuda)
+    bias = bucket_bias(table, offset_buckets(places, places, [1]))[0, 0]
+    assert torch.equal(bias, 1.0 + (places[None] > places[:, None]).float())
