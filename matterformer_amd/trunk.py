@@ -41,7 +41,8 @@ from torch import nn
 from matterformer_amd import _native
 from matterformer_amd.bucket_attention import bucket_attention, bucket_attention_torch
 from matterformer_amd.gated_mlp import ACTIVATIONS, gated_linear
-from matterformer_amd.pair_buckets import MAX_BUCKETS, PairBuckets, distance_buckets
+from matterformer_amd.geometry import NonPeriodicGeometryAdapter
+from matterformer_amd.pair_buckets import MAX_BUCKETS, PairBuckets, distance_buckets, value_buckets
 from matterformer_amd.rotary import RotaryFrequencies, check_layout, rotary_heads, rotary_heads_torch
 from matterformer_amd.simplicial_attention import SimplicialAttention
 from matterformer_amd.simplicial_types import SimplicialAttentionMask, coerce_attention_mask
@@ -409,15 +410,17 @@ class BucketAttention(nn.Module):
 
 class SimplicialTerms:
     """The simplicial blocks' shared inputs: attention mask and the optional logit / message terms (the
-    reference trunk builds them once per forward, transformer.py:1261-1296)."""
+    reference trunk builds them once per forward, transformer.py:1261-1296).  ``pair_dist`` (B, N, N): the geometry
+    adapter's distances, where the trunk's bucket blocks take them."""
 
     def __init__(self, attention_mask: SimplicialAttentionMask | None, factorized_bias=None, angle_residual=None,
-                 message_residual=None, logit_bias_fn=None) -> None:
+                 message_residual=None, logit_bias_fn=None, pair_dist: torch.Tensor | None = None) -> None:
         self.attention_mask = attention_mask
         self.factorized_bias = factorized_bias
         self.angle_residual = angle_residual
         self.message_residual = message_residual
         self.logit_bias_fn = logit_bias_fn
+        self.pair_dist = pair_dist
 
     def block_kwargs(self) -> dict:
         return dict(simplicial_attention_mask=self.attention_mask, simplicial_factorized_bias=self.factorized_bias,
@@ -444,7 +447,8 @@ class SimplicialTerms:
         msg = self.message_residual
         if msg is not None:
             msg = SimplicialLowRankMessageResidual(left=c(msg.left, 2, 3), right=c(msg.right, 2, 3))
-        return SimplicialTerms(mask, fb, ang, msg)
+        dist = None if self.pair_dist is None else c(self.pair_dist, 1, 2)
+        return SimplicialTerms(mask, fb, ang, msg, pair_dist=dist)
 
 
 def _simplicial_packed(attn: SimplicialAttention, hp: torch.Tensor, packing: TokenPacking,
@@ -602,7 +606,8 @@ class AlternatingTrunk(nn.Module):
     blocks' MLPs gated by that activation (Mlp); ``local_rotary``, ``local_rotary_layout``, ``local_hip_backward``: the
     local blocks' rotary positions and training on the HIP kernels (KnnLocalAttention).  ``bucket_edges`` (rising
     distances, one fewer than buckets), ``bucket_cutoff``, ``bucket_impl``: of the "bucket" blocks that the schedule names
-    (BucketAttention)."""
+    (BucketAttention).  Their distances are those of the coordinates in an open box, or, with a geometry adapter of another
+    kind (PeriodicGeometryAdapter), the adapter's pair_dist: minimum-image ones, in its units."""
 
     def __init__(self, d_model: int = 512, n_heads: int = 8, n_layers: int = 12, *, mlp_ratio: float = 4.0,
                  knn_k: int = 32, schedule: list[str] | None = None, simplicial_impl: str = "auto",
@@ -670,11 +675,22 @@ class AlternatingTrunk(nn.Module):
                 return False
         return True
 
-    def _pair_buckets(self, coords: torch.Tensor, pad_mask: torch.Tensor | None) -> PairBuckets | None:
+    def _adapter_distances(self) -> bool:
+        """The bucket blocks' distances are the geometry adapter's: the coordinates alone do not give them."""
+        return ("bucket" in self.schedule and self.geometry_adapter is not None
+                and getattr(self.geometry_adapter, "geometry_kind", None) != NonPeriodicGeometryAdapter.geometry_kind)
+
+    def _pair_buckets(self, coords: torch.Tensor, pad_mask: torch.Tensor | None,
+                      terms: SimplicialTerms | None) -> PairBuckets | None:
         """The bucket blocks' buckets, built once per forward."""
         if "bucket" not in self.schedule:
             return None
-        return distance_buckets(coords, self.bucket_edges, pad_mask=pad_mask, cutoff=self.bucket_cutoff)
+        if not self._adapter_distances():
+            return distance_buckets(coords, self.bucket_edges, pad_mask=pad_mask, cutoff=self.bucket_cutoff)
+        if terms is None or terms.pair_dist is None:
+            raise RuntimeError("bucket blocks need the geometry adapter's distances: simplicial terms with pair_dist")
+        return value_buckets(terms.pair_dist, self.bucket_edges, pad_mask=pad_mask, query_pad_mask=pad_mask,
+                             cutoff=self.bucket_cutoff, gradients=torch.is_grad_enabled())
 
     def simplicial_terms(self, coords: torch.Tensor, pad_mask: torch.Tensor | None = None,
                          lattice: torch.Tensor | None = None, sigma: torch.Tensor | None = None
@@ -685,15 +701,16 @@ class AlternatingTrunk(nn.Module):
             return None
         geom = self.geometry_adapter(coords=coords, pad_mask=pad_mask, lattice=lattice)
         B, N = coords.shape[:2]
+        dist = geom.pair_dist if self._adapter_distances() else None
         if self.simplicial_geometry_bias is not None:
             fb, fn, ang, msg, mask = self.simplicial_geometry_bias.build_structured_bias_inputs(
                 geom_features=geom, coords_len=N, pad_mask=pad_mask, seq_len=N, sigma=sigma)
-            return SimplicialTerms(mask, fb, ang, msg, fn)
+            return SimplicialTerms(mask, fb, ang, msg, fn, pair_dist=dist)
         from matterformer_amd.geometry_bias import build_simplicial_attention_mask
 
         mask = build_simplicial_attention_mask(coords_len=N, seq_len=N, batch_size=B, device=coords.device,
                                                pad_mask=pad_mask, geom_pair_mask=geom.pair_mask)
-        return SimplicialTerms(mask)
+        return SimplicialTerms(mask, pair_dist=dist)
 
     def forward(self, x: torch.Tensor, cond_emb: torch.Tensor | None, coords: torch.Tensor,
                 pad_mask: torch.Tensor | None = None, *, lattice: torch.Tensor | None = None,
@@ -702,6 +719,8 @@ class AlternatingTrunk(nn.Module):
         the simplicial blocks get the geometry attention mask and bias terms of (coords, lattice, sigma).
         ``packing`` (TokenPacking(pad_mask)) may be passed in, e.g. to capture the forward in a HIP graph;
         otherwise a GPU call with a pad_mask builds it."""
+        if lattice is not None and self.geometry_adapter is None and "bucket" in self.schedule:
+            raise ValueError("bucket blocks take a lattice through a geometry_adapter only (PeriodicGeometryAdapter)")
         if pad_mask is not None:
             pad_mask = pad_mask.bool()
         if packing is not None and (pad_mask is None or (packing.batch, packing.atoms) != tuple(pad_mask.shape)):
@@ -722,7 +741,7 @@ class AlternatingTrunk(nn.Module):
             mask = build_knn_mask(coords, self.knn_k, pad_mask, use_hip=self._use_hip(x),
                                   with_tables=self._trains_local(x))
         kwargs = terms.block_kwargs() if terms is not None else {}
-        kwargs["pair_buckets"] = self._pair_buckets(coords, pad_mask)
+        kwargs["pair_buckets"] = self._pair_buckets(coords, pad_mask, terms)
         # transformer.py:1298-1316: padded atoms are zeroed before every block and in the output
         for block in self.blocks:
             if pad_mask is not None:
@@ -758,7 +777,8 @@ class AlternatingTrunk(nn.Module):
         if "knn_local" in self.schedule:
             mask = build_knn_mask(packing.compact(coords.float()), self.knn_k, cpad, use_hip=True,
                                   with_tables=self._trains_local(x))
-        buckets = self._pair_buckets(packing.compact(coords.float()), cpad) if "bucket" in self.schedule else None
+        buckets = (self._pair_buckets(packing.compact(coords.float()), cpad, terms) if "bucket" in self.schedule
+                   else None)
         if terms is None:
             terms = SimplicialTerms(coerce_attention_mask(None, key_padding_mask=cpad, batch_size=B, num_tokens=W,
                                                           device=x.device))

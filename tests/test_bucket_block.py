@@ -3,9 +3,9 @@
 import pytest
 import torch
 
-from matterformer_amd.geometry import NonPeriodicGeometryAdapter
+from matterformer_amd.geometry import NonPeriodicGeometryAdapter, PeriodicGeometryAdapter
 from matterformer_amd.geometry_bias import BucketedGeometryBias, SimplicialGeometryBias
-from matterformer_amd.pair_buckets import distance_buckets
+from matterformer_amd.pair_buckets import distance_buckets, value_buckets
 from matterformer_amd.trunk import AdaLNBlock, AlternatingTrunk, BucketAttention
 
 EDGES = [0.5, 1.0, 1.5, 2.0, 3.0]
@@ -99,3 +99,40 @@ def test_bucketed_geometry_bias():
         torch.nn.init.normal_(block.ada_ln[-1].weight, std=0.1)
     trunk(torch.randn(2, 6, 32), torch.randn(2, 32), coords, pad, sigma=sigma).square().sum().backward()
     assert all(p.grad is not None and p.grad.abs().max() > 0 for p in bias.parameters())
+
+
+def periodic_batch():
+    """A trunk over fractional coordinates, padded, in two different cells."""
+    torch.manual_seed(4)
+    trunk = AlternatingTrunk(32, 4, 2, schedule=["bucket", "simplicial"], bucket_edges=EDGES, bucket_cutoff=2.5,
+                             geometry_adapter=PeriodicGeometryAdapter(), simplicial_precision="ieee_fp32").double()
+    for block in trunk.blocks:
+        torch.nn.init.normal_(block.ada_ln[-1].weight, std=0.1)
+    torch.nn.init.normal_(trunk.blocks[0].attn.bias_table)
+    x, cond = torch.randn(2, 8, 32, dtype=torch.float64), torch.randn(2, 32, dtype=torch.float64)
+    pad = torch.zeros(2, 8, dtype=torch.bool)
+    pad[0, 6:] = True
+    lattice = torch.tensor([[1.5, 1.6, 1.4, 0.1, 0.0, -0.1], [1.1, 1.2, 1.0, 0.0, 0.2, 0.1]])
+    return trunk, x, cond, torch.rand(2, 8, 3), pad, lattice
+
+
+def test_periodic_cells_have_minimum_image_distances():
+    """The bucket blocks' buckets are those of the adapter's pair_dist, in the cell's units."""
+    trunk, x, cond, frac, pad, lattice = periodic_batch()
+    seen = []
+    trunk.blocks[0].attn.register_forward_pre_hook(lambda module, args: seen.append(args[1]))
+    out = trunk(x, cond, frac, pad, lattice=lattice)
+    dist = trunk.geometry_adapter(coords=frac, pad_mask=pad, lattice=lattice).pair_dist
+    want = value_buckets(dist, EDGES, pad_mask=pad, query_pad_mask=pad, cutoff=2.5)
+    assert torch.equal(seen[0].index, want.index)
+    assert want.index[want.allowed()].max() >= 3  # (raw fractions are at most sqrt(3) apart)
+    assert not torch.allclose(trunk(x, cond, frac, pad, lattice=lattice * 0.6), out, rtol=1e-3, atol=1e-3)
+    out.square().sum().backward()
+    assert trunk.blocks[0].attn.bias_table.grad.abs().max() > 0
+
+
+def test_cells_of_open_bucket_trunks_are_refused():
+    """A lattice that no adapter takes would leave the distances those of an open box."""
+    trunk = AlternatingTrunk(32, 4, 1, schedule=["bucket"], bucket_edges=EDGES)
+    with pytest.raises(ValueError, match="geometry_adapter"):
+        trunk(torch.zeros(1, 3, 32), torch.zeros(1, 32), torch.zeros(1, 3, 3), lattice=torch.zeros(1, 6))

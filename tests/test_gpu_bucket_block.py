@@ -161,3 +161,59 @@ def test_trunk_in_a_graph(cuda):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(held, want)
+
+
+def test_periodic_trunk(cuda):
+    """Bucket blocks on periodic cells: padded and packed forwards and a step of training against the same trunk in 64 bits,
+    whose buckets are those of the same distances."""
+    adapter = PeriodicGeometryAdapter()
+    trunk = make_trunk(cuda, torch.bfloat16, geometry_adapter=adapter, bucket_cutoff=4.0)
+    x, cond, _, pad = batch(cuda, torch.bfloat16)
+    g = torch.Generator(device=cuda).manual_seed(8)
+    frac = torch.rand(*x.shape[:2], 3, generator=g, device=cuda)
+    lattice = torch.tensor([[1.5, 1.6, 1.4, 0.1, 0.0, -0.1], [1.1, 1.2, 1.0, 0.0, 0.2, 0.1]] * 2, device=cuda)
+    exact = copy.deepcopy(trunk).double()
+    for block in exact.blocks:
+        block.attn.impl = "torch"
+    seen = []
+    exact.blocks[0].attn.register_forward_pre_hook(lambda module, args: seen.append(args[1].index))
+    want = exact(x.double(), cond.double(), frac, pad, lattice=lattice)
+    dist = adapter(coords=frac, pad_mask=pad, lattice=lattice).pair_dist
+    counts = torch.stack([dist >= torch.tensor(e, device=cuda) for e in EDGES]).sum(0)
+    left_out = pad[:, None, :] | pad[:, :, None] | (dist > 4.0)
+    assert torch.equal(seen[0].long(), torch.where(left_out, 64, counts))
+    out = trunk(x, cond, frac, pad, lattice=lattice)
+    assert all(b.attn._last_impl_used == "triton" for b in trunk.blocks if b.attn_type == "bucket")
+    assert off(out, want) <= 30 * 2.0 ** -9
+    go = torch.randn_like(out)
+    out.backward(go)
+    want.backward(go.double())
+    for block, other in zip(trunk.blocks, exact.blocks):
+        if block.attn_type == "bucket":
+            assert off(block.attn.bias_table.grad, other.attn.bias_table.grad) <= 60 * 2.0 ** -9
+    with torch.no_grad():
+        packed = trunk.eval()(x, cond, frac, pad, lattice=lattice)
+        trunk.pack_tokens = False
+        padded = trunk(x, cond, frac, pad, lattice=lattice)
+    assert off(packed, want) <= 30 * 2.0 ** -9 and off(padded, want) <= 30 * 2.0 ** -9
+
+
+def test_periodic_trunk_in_a_graph(cuda):
+    trunk = make_trunk(cuda, torch.bfloat16, geometry_adapter=PeriodicGeometryAdapter()).eval()
+    x, cond, _, pad = batch(cuda, torch.bfloat16)
+    frac = torch.rand(*x.shape[:2], 3, device=cuda)
+    lattice = torch.tensor([[1.5, 1.6, 1.4, 0.1, 0.0, -0.1]] * 4, device=cuda)
+    packing = TokenPacking(pad)
+    with torch.no_grad():
+        trunk(x, cond, frac, pad, lattice=lattice, packing=packing)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = trunk(x, cond, frac, pad, lattice=lattice, packing=packing)
+        for _ in range(3):
+            x.copy_(torch.randn_like(x))
+            frac.copy_(torch.rand_like(frac))
+            want = trunk(x, cond, frac, pad, lattice=lattice, packing=packing)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(held, want)
