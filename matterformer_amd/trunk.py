@@ -470,6 +470,11 @@ def _simplicial_packed(attn: SimplicialAttention, hp: torch.Tensor, packing: Tok
     return attn.out_proj(packing.from_heads(out, hp.dtype))
 
 
+def _bucket_kwargs(block: nn.Module, buckets: PairBuckets | None) -> dict:
+    """The buckets for a bucket block; other blocks are called without, a user's own among them."""
+    return {"pair_buckets": buckets} if getattr(block, "attn_type", None) == "bucket" else {}
+
+
 class AdaLNBlock(nn.Module):
     """Pre-norm block with adaLN modulation (transformer.py:154-316) for attn_type in ATTN_TYPES."""
 
@@ -590,12 +595,12 @@ class AdaLNBlock(nn.Module):
         compact layout.  The same operations in the same dtypes as forward."""
         if not self.use_adaln_conditioning:
             h = self.norm1(xp)
-            xp = xp + self._attention_packed(h, packing, knn_mask, terms, pair_buckets)
+            xp = xp + self._attention_packed(h, packing, knn_mask, terms, **_bucket_kwargs(self, pair_buckets))
             return xp + self.mlp(self.norm2(xp))
         C = xp.shape[-1]
         mods = self._mods(cond_emb, packing.batch)
         h = adaln_rows(packing, xp, shift=mods[:, :C], scale=mods[:, C:2 * C], eps=self.norm1.eps)
-        a = self._attention_packed(h, packing, knn_mask, terms, pair_buckets)
+        a = self._attention_packed(h, packing, knn_mask, terms, **_bucket_kwargs(self, pair_buckets))
         xp, h = adaln_rows(packing, xp, a, gate=mods[:, 2 * C:3 * C], shift=mods[:, 3 * C:4 * C],
                            scale=mods[:, 4 * C:5 * C], eps=self.norm2.eps)
         return adaln_rows(packing, xp, self.mlp(h), gate=mods[:, 5 * C:])
@@ -741,12 +746,12 @@ class AlternatingTrunk(nn.Module):
             mask = build_knn_mask(coords, self.knn_k, pad_mask, use_hip=self._use_hip(x),
                                   with_tables=self._trains_local(x))
         kwargs = terms.block_kwargs() if terms is not None else {}
-        kwargs["pair_buckets"] = self._pair_buckets(coords, pad_mask, terms)
+        buckets = self._pair_buckets(coords, pad_mask, terms)
         # transformer.py:1298-1316: padded atoms are zeroed before every block and in the output
         for block in self.blocks:
             if pad_mask is not None:
                 x = x.masked_fill(pad_mask[..., None], 0.0)
-            x = block(x, cond_emb, pad_mask, knn_mask=mask, **kwargs)
+            x = block(x, cond_emb, pad_mask, knn_mask=mask, **kwargs, **_bucket_kwargs(block, buckets))
         if pad_mask is not None:
             x = x.masked_fill(pad_mask[..., None], 0.0)
         return x
@@ -785,7 +790,8 @@ class AlternatingTrunk(nn.Module):
         xp = packing.pack(x)
         if not all(blk.use_adaln_conditioning for blk in self.blocks):
             for block in self.blocks:
-                xp = block.forward_packed(xp, cond_emb, packing, knn_mask=mask, terms=terms, pair_buckets=buckets)
+                xp = block.forward_packed(xp, cond_emb, packing, knn_mask=mask, terms=terms,
+                                          **_bucket_kwargs(block, buckets))
             return packing.unpack(xp)
         C = xp.shape[-1]
         mods = self._all_mods(cond_emb, B)
@@ -793,7 +799,7 @@ class AlternatingTrunk(nn.Module):
         h = adaln_rows(packing, xp, shift=mods[0][:, :C], scale=mods[0][:, C:2 * C], eps=blocks[0].norm1.eps)
         for layer, blk in enumerate(blocks):
             m = mods[layer]
-            a = blk._attention_packed(h, packing, mask, terms, buckets)
+            a = blk._attention_packed(h, packing, mask, terms, **_bucket_kwargs(blk, buckets))
             xp, h = adaln_rows(packing, xp, a, gate=m[:, 2 * C:3 * C], shift=m[:, 3 * C:4 * C],
                                scale=m[:, 4 * C:5 * C], eps=blk.norm2.eps, inplace=layer > 0)
             y = blk.mlp(h)

@@ -136,3 +136,32 @@ def test_cells_of_open_bucket_trunks_are_refused():
     trunk = AlternatingTrunk(32, 4, 1, schedule=["bucket"], bucket_edges=EDGES)
     with pytest.raises(ValueError, match="geometry_adapter"):
         trunk(torch.zeros(1, 3, 32), torch.zeros(1, 32), torch.zeros(1, 3, 3), lattice=torch.zeros(1, 6))
+
+
+class UsersBlock(torch.nn.Module):
+    """A block of a user's own, which knows the local and simplicial inputs only."""
+
+    attn_type = "mine"
+
+    def __init__(self, block):
+        super().__init__()
+        self.block, self.attn = block, block.attn
+
+    def forward(self, x, cond_emb, pad_mask=None, *, knn_mask=None, simplicial_attention_mask=None,
+                simplicial_factorized_bias=None, simplicial_angle_residual=None, simplicial_message_residual=None,
+                simplicial_logit_bias_fn=None):
+        return self.block(x, cond_emb, pad_mask, simplicial_attention_mask=simplicial_attention_mask)
+
+
+@pytest.mark.parametrize("schedule", [["simplicial", "knn_local"], ["simplicial", "bucket"]])
+@pytest.mark.parametrize("adapter", [None, NonPeriodicGeometryAdapter()])
+def test_blocks_without_a_place_for_buckets(schedule, adapter):
+    """Only the bucket blocks are handed buckets: other blocks are called as before there were any."""
+    torch.manual_seed(6)
+    trunk = AlternatingTrunk(32, 4, 2, schedule=schedule, bucket_edges=EDGES, geometry_adapter=adapter,
+                             simplicial_precision="ieee_fp32").eval()
+    x, cond, coords = torch.randn(2, 6, 32), torch.randn(2, 32), torch.randn(2, 6, 3)
+    with torch.no_grad():
+        want = trunk(x, cond, coords)
+        trunk.blocks[0] = UsersBlock(trunk.blocks[0])
+        assert torch.equal(trunk(x, cond, coords), want)

@@ -9,7 +9,7 @@ from matterformer_amd.geometry import NonPeriodicGeometryAdapter, PeriodicGeomet
 from matterformer_amd.geometry_bias import BucketedGeometryBias
 from matterformer_amd.pair_buckets import distance_buckets
 from matterformer_amd.token_packing import TokenPacking
-from matterformer_amd.trunk import AlternatingTrunk, BucketAttention
+from matterformer_amd.trunk import AdaLNBlock, AlternatingTrunk, BucketAttention
 
 pytestmark = pytest.mark.gpu
 
@@ -217,3 +217,27 @@ def test_periodic_trunk_in_a_graph(cuda):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(held, want)
+
+
+class OlderBlock(AdaLNBlock):
+    """A block whose packed methods know the local and simplicial inputs only."""
+
+    def forward_packed(self, xp, cond_emb, packing, *, knn_mask=None, terms=None):
+        return super().forward_packed(xp, cond_emb, packing, knn_mask=knn_mask, terms=terms)
+
+    def _attention_packed(self, h, packing, knn_mask, terms):
+        return super()._attention_packed(h, packing, knn_mask, terms)
+
+
+@pytest.mark.parametrize("adaln", [True, False])
+def test_packed_blocks_without_a_place_for_buckets(cuda, adaln):
+    torch.manual_seed(5)
+    trunk = AlternatingTrunk(256, 4, 3, schedule=["bucket", "simplicial", "knn_local"], bucket_edges=EDGES, knn_k=8,
+                             use_adaln_conditioning=adaln).to(cuda, torch.bfloat16).eval()
+    x, cond, coords, pad = batch(cuda, torch.bfloat16)
+    with torch.no_grad():
+        want = trunk(x, cond, coords, pad)
+        assert all(b.attn._last_impl_used == "triton" for b in trunk.blocks)
+        for block in trunk.blocks[1:]:
+            block.__class__ = OlderBlock
+        assert torch.equal(trunk(x, cond, coords, pad), want)
