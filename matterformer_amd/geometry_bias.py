@@ -28,7 +28,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from matterformer_amd.geometry import GeometryFeatures
-from matterformer_amd.pair_buckets import bucket_bias, value_buckets
+from matterformer_amd.pair_buckets import bucket_bias, check_edges, value_buckets
 from matterformer_amd.simplicial_types import (
     SimplicialAttentionMask,
     SimplicialFactorizedBias,
@@ -396,7 +396,7 @@ class BucketedGeometryBias(_GeometryBiasBase):
 
     def __init__(self, n_heads: int, edges: Sequence[float], use_noise_gate: bool = True) -> None:
         super().__init__(n_heads, use_noise_gate)
-        self.edges = [float(e) for e in edges]
+        self.edges = check_edges(edges, distances=False)
         for name in ("u_table", "v_table", "w_table"):
             self.register_parameter(name, nn.Parameter(torch.zeros(len(self.edges) + 1, self.n_heads)))
 

@@ -98,6 +98,21 @@ def _round_edges(edges, whole: bool) -> array:
     return out
 
 
+def _distance_edges(edges) -> array:
+    out = _round_edges(edges, whole=False)
+    if out and out[0] < 0.0:
+        raise ValueError("edges of distances must not be negative")
+    return out
+
+
+def check_edges(edges, *, distances: bool, cutoff: float | None = None) -> list[float]:
+    """The edges of distance_buckets, or of value_buckets, as a list; what those refuse is refused."""
+    edges = [float(e) for e in edges]
+    _distance_edges(edges) if distances else _round_edges(edges, whole=False)
+    _check_cutoff(cutoff)
+    return edges
+
+
 def _pad_bytes(pad: torch.Tensor | None, B: int, N: int, name: str, device: torch.device) -> torch.Tensor | None:
     if pad is None:
         return None
@@ -183,9 +198,7 @@ def distance_buckets(coords: torch.Tensor, edges, *, pad_mask: torch.Tensor | No
     whose coordinates are NaN has bucket 0 with every other.)  The matrix is its own transpose."""
     if coords.ndim != 3 or coords.shape[-1] != 3:
         raise ValueError(f"coords must have shape (B, N, 3), got {tuple(coords.shape)}")
-    host = _round_edges(edges, whole=False)
-    if host and host[0] < 0.0:
-        raise ValueError("edges of distances must not be negative")
+    host = _distance_edges(edges)
     cut = _check_cutoff(cutoff)
     B, N, _ = coords.shape
     dev = coords.device

@@ -42,7 +42,7 @@ from matterformer_amd import _native
 from matterformer_amd.bucket_attention import bucket_attention, bucket_attention_torch
 from matterformer_amd.gated_mlp import ACTIVATIONS, gated_linear
 from matterformer_amd.geometry import NonPeriodicGeometryAdapter
-from matterformer_amd.pair_buckets import MAX_BUCKETS, PairBuckets, distance_buckets, value_buckets
+from matterformer_amd.pair_buckets import MAX_BUCKETS, PairBuckets, check_edges, distance_buckets, value_buckets
 from matterformer_amd.rotary import RotaryFrequencies, check_layout, rotary_heads, rotary_heads_torch
 from matterformer_amd.simplicial_attention import SimplicialAttention
 from matterformer_amd.simplicial_types import SimplicialAttentionMask, coerce_attention_mask
@@ -635,7 +635,7 @@ class AlternatingTrunk(nn.Module):
             raise ValueError("schedule must name one attention type per layer")
         if "bucket" in schedule and bucket_edges is None:
             raise ValueError("bucket blocks need bucket_edges")
-        self.bucket_edges = None if bucket_edges is None else [float(e) for e in bucket_edges]
+        self.bucket_edges = None if bucket_edges is None else check_edges(bucket_edges, distances=True, cutoff=bucket_cutoff)
         self.bucket_cutoff = bucket_cutoff
         self.knn_k = int(knn_k)
         self.schedule = list(schedule)
@@ -646,7 +646,7 @@ class AlternatingTrunk(nn.Module):
                        simplicial_content_logits=simplicial_content_logits, local_impl=local_impl,
                        use_adaln_conditioning=use_adaln_conditioning, mlp_gate=mlp_gate, local_rotary=local_rotary,
                        local_rotary_layout=local_rotary_layout, local_hip_backward=local_hip_backward,
-                       num_buckets=None if bucket_edges is None else len(bucket_edges) + 1, bucket_impl=bucket_impl)
+                       num_buckets=None if bucket_edges is None else len(self.bucket_edges) + 1, bucket_impl=bucket_impl)
             for t in self.schedule])
 
     def _use_hip(self, x: torch.Tensor) -> bool:

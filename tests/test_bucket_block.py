@@ -1,5 +1,7 @@
 """Bucket blocks of the trunk and the bucketed simplicial bias on the CPU: construction, refusals, the torch path."""
 
+import math
+
 import pytest
 import torch
 
@@ -165,3 +167,28 @@ def test_blocks_without_a_place_for_buckets(schedule, adapter):
         want = trunk(x, cond, coords)
         trunk.blocks[0] = UsersBlock(trunk.blocks[0])
         assert torch.equal(trunk(x, cond, coords), want)
+
+
+BAD_EDGES = [[1.0, 1.0], [2.0, 1.0], [1.0, 1.0 + 1e-12], [math.nan], [1.0, math.inf], [1.0, 1e39], [0.1 * i for i in range(1, 65)]]
+
+
+@pytest.mark.parametrize("edges", [*BAD_EDGES, [-1.0, 1.0]], ids=lambda e: f"{len(e)}-{e[-1]}")
+def test_edges_are_refused_when_a_module_is_made(edges):
+    for schedule in (["bucket"], ["simplicial"]):
+        with pytest.raises(ValueError, match="edges"):
+            AlternatingTrunk(32, 4, 1, schedule=schedule, bucket_edges=edges)
+    if edges in BAD_EDGES:  # (a bias may be of any rising numbers)
+        with pytest.raises(ValueError, match="edges"):
+            BucketedGeometryBias(4, edges)
+
+
+@pytest.mark.parametrize("cutoff", [-1.0, math.nan, math.inf])
+def test_cutoffs_are_refused_when_a_trunk_is_made(cutoff):
+    with pytest.raises(ValueError, match="cutoff"):
+        AlternatingTrunk(32, 4, 1, schedule=["bucket"], bucket_edges=EDGES, bucket_cutoff=cutoff)
+
+
+def test_edges_as_a_tensor_or_a_generator():
+    for edges in (torch.tensor(EDGES), tuple(EDGES), (e for e in EDGES)):
+        trunk = AlternatingTrunk(32, 4, 1, schedule=["bucket"], bucket_edges=edges)
+        assert trunk.bucket_edges == EDGES and trunk.blocks[0].attn.bias_table.shape == (6, 4)
