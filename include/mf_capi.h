@@ -827,6 +827,7 @@ int mf_gated_linear_bwd(const mf_gated_linear_bwd_args* args, void* stream);
 /*                        key_pos [B, keys, 3], fp32; d^2 in fp64 without    */
 /*                        contraction, compared with the edges' squares      */
 /*   MF_BUCKETS_OFFSET    key_pos [B, keys] - query_pos [B, queries], int64  */
+/*                        (the edges whole numbers within +-2^53)            */
 /*   MF_BUCKETS_VALUE     values [B, queries, keys], fp32                    */
 /* and MF_BUCKETS_INDEX takes the bucket itself from values (int32; below 0  */
 /* or from `buckets` on: masked).  Masked besides: pairs of a padded query   */

@@ -709,6 +709,8 @@ extern "C" int mf_pair_buckets(const mf_pair_buckets_args* a, void* stream) {
         return fail(MF_ERR_INVALID_ARGUMENT, "mf_pair_buckets: edges of distances must not be negative");
       if (std::fabs(a->edges[e]) > (a->source == MF_BUCKETS_OFFSET ? 9007199254740992.0 : 3.5e38))
         return fail(MF_ERR_INVALID_ARGUMENT, "mf_pair_buckets: edges out of range");
+      if (a->source == MF_BUCKETS_OFFSET && a->edges[e] != std::floor(a->edges[e]))  // (tiles compare them as integers)
+        return fail(MF_ERR_INVALID_ARGUMENT, "mf_pair_buckets: edges of offsets must be whole numbers");
     }
   }
   if (std::isnan(a->cutoff)) return fail(MF_ERR_INVALID_ARGUMENT, "mf_pair_buckets: cutoff must not be NaN");

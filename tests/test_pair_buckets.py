@@ -334,3 +334,20 @@ def test_counts_past_32_bits_are_refused():
     for counts in ((2 ** 32 + 5, 1, 1), (1, 2 ** 31, 1), (1, 1, 2 ** 32 + 1)):
         with pytest.raises(RuntimeError, match="2\\^31"):
             pair_buckets._launch(0, *counts, torch.device("cpu"), buckets=1, gradients=False, symmetric=False)
+
+
+def test_offset_edges_of_the_c_entry_are_whole():
+    """(between whole numbers, an edge's side would hang on the path that a tile takes)"""
+    lib = _native.lib()
+
+    def args(*edges, **kw):
+        held.append((ctypes.c_double * len(edges))(*edges))
+        return _native.MfPairBucketsArgs(query_pos=FAKE, key_pos=2 * FAKE, edges=ctypes.addressof(held[-1]), index=FAKE,
+                                         index_t=2 * FAKE, key_any=3 * FAKE, query_any=4 * FAKE, cutoff=-1.0,
+                                         source=_native.MF_BUCKETS_OFFSET, num_edges=len(edges), buckets=len(edges) + 1,
+                                         batch=kw.get("batch", 1), queries=5, keys=5)
+
+    held = []
+    for edges in ((0.5,), (0.2, 0.7), (-3.0, 2.0 ** 51 + 0.5), (-0.25, 0.0)):
+        refused(lib.mf_pair_buckets, args(*edges), INVALID, "whole")
+    assert lib.mf_pair_buckets(args(-(2.0 ** 53), -1.0, 0.0, 2.0 ** 53, batch=0), None) == _native.MF_OK
