@@ -14,7 +14,7 @@
 
 Edges e_0 < e_1 < .. rise, and a pair's bucket is how many of them are at or below its value, so there is one bucket
 more than edges.  GPU tensors run mf_pair_buckets, mf_bucket_bias and mf_bucket_bias_bwd (csrc/pair_buckets.hip); a
-missing library raises.  CPU tensors take the torch formulation.
+missing library raises.  CPU tensors, and calls with use_hip=False, take the torch formulation.
 """
 
 from __future__ import annotations
@@ -191,11 +191,12 @@ def _check_cutoff(cutoff: float | None) -> float:
 
 
 def distance_buckets(coords: torch.Tensor, edges, *, pad_mask: torch.Tensor | None = None,
-                     cutoff: float | None = None) -> PairBuckets:
+                     cutoff: float | None = None, use_hip: bool = True) -> PairBuckets:
     """Buckets of the distances of every two atoms: how many of the rising ``edges`` (fp32, not negative) are at or below
     |x_i - x_j|.  coords (B, N, 3), taken in fp32; pad_mask (B, N), True = padding, whose pairs are left out, as are those
     further apart than ``cutoff``.  Squares are compared, in fp64: a distance at an edge falls on its exact side.  (An atom
-    whose coordinates are NaN has bucket 0 with every other.)  The matrix is its own transpose."""
+    whose coordinates are NaN has bucket 0 with every other.)  The matrix is its own transpose.  ``use_hip`` = False takes
+    the torch formulation for GPU tensors too; its buckets are for bucket_attention_torch, the kernels refuse them."""
     if coords.ndim != 3 or coords.shape[-1] != 3:
         raise ValueError(f"coords must have shape (B, N, 3), got {tuple(coords.shape)}")
     host = _distance_edges(edges)
@@ -204,7 +205,7 @@ def distance_buckets(coords: torch.Tensor, edges, *, pad_mask: torch.Tensor | No
     dev = coords.device
     pad = _pad_bytes(pad_mask, B, N, "pad_mask", dev)
     c = coords.detach().float().contiguous()
-    if dev.type == "cuda":
+    if dev.type == "cuda" and use_hip:
         return _launch(_native.MF_BUCKETS_DISTANCE, B, N, N, dev, edges=host, buckets=len(host) + 1, query_pos=c,
                        key_pos=c, query_step=3 * N, key_step=3 * N, query_pad=pad, key_pad=pad, cutoff=cut,
                        gradients=True, symmetric=True)
@@ -259,9 +260,10 @@ def offset_buckets(query_positions: torch.Tensor, key_positions: torch.Tensor, e
 
 def value_buckets(values: torch.Tensor, edges, *, pad_mask: torch.Tensor | None = None,
                   query_pad_mask: torch.Tensor | None = None, cutoff: float | None = None,
-                  gradients: bool = True) -> PairBuckets:
+                  gradients: bool = True, use_hip: bool = True) -> PairBuckets:
     """Buckets of given numbers (B, Nq, Nk), taken in fp32: how many of the rising ``edges`` (fp32) are at or below each.
-    Pairs of padding (pad_mask (B, Nk), query_pad_mask (B, Nq)) and those above ``cutoff`` are left out; NaN has bucket 0."""
+    Pairs of padding (pad_mask (B, Nk), query_pad_mask (B, Nq)) and those above ``cutoff`` are left out; NaN has bucket 0.
+    ``use_hip`` as in distance_buckets."""
     if values.ndim != 3:
         raise ValueError(f"values must have shape (B, Nq, Nk), got {tuple(values.shape)}")
     host = _round_edges(edges, whole=False)
@@ -271,7 +273,7 @@ def value_buckets(values: torch.Tensor, edges, *, pad_mask: torch.Tensor | None 
     kpad = _pad_bytes(pad_mask, B, Nk, "pad_mask", dev)
     qpad = _pad_bytes(query_pad_mask, B, Nq, "query_pad_mask", dev)
     v = values.detach().float().contiguous()
-    if dev.type == "cuda":
+    if dev.type == "cuda" and use_hip:
         return _launch(_native.MF_BUCKETS_VALUE, B, Nq, Nk, dev, edges=host, buckets=len(host) + 1, values=v,
                        query_pad=qpad, key_pad=kpad, cutoff=cut, gradients=gradients, symmetric=False)
     return _from_torch(_count_edges(v, host), len(host) + 1, None if cutoff is None else ~(v > cut), qpad, kpad, gradients)

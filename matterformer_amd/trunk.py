@@ -690,12 +690,14 @@ class AlternatingTrunk(nn.Module):
         """The bucket blocks' buckets, built once per forward."""
         if "bucket" not in self.schedule:
             return None
+        use_hip = any(block.attn.impl != "torch" for block in self.blocks if getattr(block, "attn_type", None) == "bucket")
         if not self._adapter_distances():
-            return distance_buckets(coords, self.bucket_edges, pad_mask=pad_mask, cutoff=self.bucket_cutoff)
+            return distance_buckets(coords, self.bucket_edges, pad_mask=pad_mask, cutoff=self.bucket_cutoff,
+                                    use_hip=use_hip)
         if terms is None or terms.pair_dist is None:
             raise RuntimeError("bucket blocks need the geometry adapter's distances: simplicial terms with pair_dist")
         return value_buckets(terms.pair_dist, self.bucket_edges, pad_mask=pad_mask, query_pad_mask=pad_mask,
-                             cutoff=self.bucket_cutoff, gradients=torch.is_grad_enabled())
+                             cutoff=self.bucket_cutoff, gradients=torch.is_grad_enabled(), use_hip=use_hip)
 
     def simplicial_terms(self, coords: torch.Tensor, pad_mask: torch.Tensor | None = None,
                          lattice: torch.Tensor | None = None, sigma: torch.Tensor | None = None

@@ -5,9 +5,11 @@ import copy
 import pytest
 import torch
 
+from matterformer_amd import _native
+from matterformer_amd.bucket_attention import bucket_attention
 from matterformer_amd.geometry import NonPeriodicGeometryAdapter, PeriodicGeometryAdapter
 from matterformer_amd.geometry_bias import BucketedGeometryBias
-from matterformer_amd.pair_buckets import distance_buckets
+from matterformer_amd.pair_buckets import distance_buckets, value_buckets
 from matterformer_amd.token_packing import TokenPacking
 from matterformer_amd.trunk import AdaLNBlock, AlternatingTrunk, BucketAttention
 
@@ -241,3 +243,37 @@ def test_packed_blocks_without_a_place_for_buckets(cuda, adaln):
         for block in trunk.blocks[1:]:
             block.__class__ = OlderBlock
         assert torch.equal(trunk(x, cond, coords, pad), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+@pytest.mark.parametrize("periodic", [False, True])
+def test_a_torch_trunk_runs_no_bucket_kernel(cuda, periodic, dtype, monkeypatch):
+    """impl="torch" is the torch formulation throughout, the buckets too; they are those that the kernel gives."""
+    trunk = make_trunk(cuda, dtype, bucket_impl="torch", simplicial_impl="torch", bucket_cutoff=6.0,
+                       geometry_adapter=PeriodicGeometryAdapter() if periodic else NonPeriodicGeometryAdapter())
+    x, cond, coords, pad = batch(cuda, dtype)
+    lattice = torch.tensor([[1.5, 1.6, 1.4, 0.1, 0.0, -0.1]] * 4, device=cuda) if periodic else None
+    launch = _native.launch
+
+    def only_geometry(name, *args):
+        assert "bucket" not in name
+        launch(name, *args)
+
+    seen = []
+    trunk.blocks[0].attn.register_forward_pre_hook(lambda module, args: seen.append(args[1]))
+    monkeypatch.setattr(_native, "launch", only_geometry)
+    out = trunk(x, cond, coords, pad, lattice=lattice)
+    out.square().sum().backward()
+    assert all(b.attn._last_impl_used == "torch" for b in trunk.blocks)
+    assert trunk.blocks[0].attn.bias_table.grad.abs().max() > 0
+    monkeypatch.undo()
+    if periodic:
+        dist = trunk.geometry_adapter(coords=coords, pad_mask=pad, lattice=lattice).pair_dist
+        want = value_buckets(dist, EDGES, pad_mask=pad, query_pad_mask=pad, cutoff=6.0)
+    else:
+        want = distance_buckets(coords, EDGES, pad_mask=pad, cutoff=6.0)
+    assert torch.equal(seen[0].index, want.index) and torch.equal(seen[0].index_t, want.index_t)
+    # the kernels, which read another layout, refuse such buckets
+    q = torch.zeros(4, 2, 90, 32, device=cuda, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="distance_buckets"):
+        bucket_attention(q, q, q, torch.zeros(len(EDGES) + 1, 2, device=cuda), seen[0])
