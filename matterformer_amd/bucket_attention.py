@@ -131,8 +131,13 @@ class _BucketAttentionFunction(torch.autograd.Function):
 
 
 def bucket_attention_torch(q, k, v, table, buckets: PairBuckets, scale: float, *, dropout: float = 0.0):
-    """out and lse in torch, in fp32 (fp64 operands in fp64); rows without a pair are 0, whatever their operands hold.
-    ``dropout`` of the probabilities."""
+    """out and lse in torch, in fp32 under autocast too (fp64 operands in fp64); rows without a pair are 0, whatever their
+    operands hold.  ``dropout`` of the probabilities."""
+    with torch.autocast(q.device.type, enabled=False):
+        return _attention_torch(q, k, v, table, buckets, scale, dropout)
+
+
+def _attention_torch(q, k, v, table, buckets: PairBuckets, scale: float, dropout: float):
     wide = torch.float64 if q.dtype == torch.float64 else torch.float32
     allowed = buckets.allowed()
     has_key, has_query = allowed.any(2)[:, None, :, None], allowed.any(1)[:, None, :, None]

@@ -11,7 +11,7 @@ import pytest
 import torch
 
 from matterformer_amd import _native
-from matterformer_amd.bucket_attention import bucket_attention
+from matterformer_amd.bucket_attention import bucket_attention, bucket_attention_torch
 from matterformer_amd.pair_buckets import (MASKED, PairBuckets, bucket_bias, check_layout, distance_buckets, index_buckets,
                                            offset_buckets, offset_edges, value_buckets)
 from tests.bucket_reference import attention
@@ -351,3 +351,20 @@ def test_offset_edges_of_the_c_entry_are_whole():
     for edges in ((0.5,), (0.2, 0.7), (-3.0, 2.0 ** 51 + 0.5), (-0.25, 0.0)):
         refused(lib.mf_pair_buckets, args(*edges), INVALID, "whole")
     assert lib.mf_pair_buckets(args(-(2.0 ** 53), -1.0, 0.0, 2.0 ** 53, batch=0), None) == _native.MF_OK
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_torch_formulation_is_fp32_under_autocast(dtype):
+    """Autocast would take its products in 16 bits, forward and backward."""
+    torch.manual_seed(12)
+    buckets = index_buckets(torch.randint(-1, 4, (2, 9, 11)), 4)
+    q, k, v = (torch.randn(2, 4, n, 8).to(dtype) for n in (9, 11, 11))
+    table, go = torch.randn(4, 4), torch.randn(2, 4, 9, 8).to(dtype)
+    results = []
+    for on in (False, True):
+        leaves = [t.clone().requires_grad_(True) for t in (q, k, v, table)]
+        with torch.autocast("cpu", dtype=torch.bfloat16, enabled=on):
+            out, lse = bucket_attention_torch(*leaves, buckets, 0.35)
+        assert out.dtype == dtype and lse.dtype == torch.float32
+        results.append([out, lse, *torch.autograd.grad((out, lse), leaves, (go, torch.ones_like(lse)))])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
