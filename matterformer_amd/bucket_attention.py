@@ -130,9 +130,26 @@ class _BucketAttentionFunction(torch.autograd.Function):
         return dq, dk, dv, dtable, None, None
 
 
+def _check_operands(q, k, v, table, buckets: PairBuckets) -> None:
+    if q.ndim != 4 or k.ndim != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError("q must have shape (B, H, Nq, D), k and v (B, KV, Nk, D)")
+    _check_table(table, buckets)
+    B, H, Nq, D = q.shape
+    KV, Nk = k.shape[1:3]
+    if table.shape[1] != H:
+        raise ValueError(f"table must have shape ({buckets.num_buckets}, {H}), got {tuple(table.shape)}")
+    if buckets.batch not in (1, B) or (buckets.queries, buckets.keys) != (Nq, Nk):
+        raise ValueError(f"buckets must be of ({B}, {Nq}, {Nk}) pairs, got {tuple(buckets.index.shape)}")
+    if (KV == 0) != (H == 0) or (KV and H % KV):
+        raise ValueError(f"the heads of k and v must divide those of q, got {KV} and {H}")
+    if any(t.device != q.device for t in (k, v, table)):
+        raise RuntimeError("all tensors must be on the same device")
+
+
 def bucket_attention_torch(q, k, v, table, buckets: PairBuckets, scale: float, *, dropout: float = 0.0):
     """out and lse in torch, in fp32 under autocast too (fp64 operands in fp64); rows without a pair are 0, whatever their
     operands hold.  ``dropout`` of the probabilities."""
+    _check_operands(q, k, v, table, buckets)  # an index past the table would be read
     with torch.autocast(q.device.type, enabled=False):
         return _attention_torch(q, k, v, table, buckets, scale, dropout)
 
@@ -173,19 +190,9 @@ def bucket_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: t
     queries without a pair may hold anything (NaN); a key that some query attends must be finite.  Differentiable in q,
     k, v and the table through out and lse, for which the buckets need their transpose (made with gradients=True); two
     calls give identical bits."""
-    if q.ndim != 4 or k.ndim != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
-        raise ValueError("q must have shape (B, H, Nq, D), k and v (B, KV, Nk, D)")
-    _check_table(table, buckets)
+    _check_operands(q, k, v, table, buckets)
     B, H, Nq, D = q.shape
     KV, Nk = k.shape[1:3]
-    if table.shape[1] != H:
-        raise ValueError(f"table must have shape ({buckets.num_buckets}, {H}), got {tuple(table.shape)}")
-    if buckets.batch not in (1, B) or (buckets.queries, buckets.keys) != (Nq, Nk):
-        raise ValueError(f"buckets must be of ({B}, {Nq}, {Nk}) pairs, got {tuple(buckets.index.shape)}")
-    if (KV == 0) != (H == 0) or (KV and H % KV):
-        raise ValueError(f"the heads of k and v must divide those of q, got {KV} and {H}")
-    if any(t.device != q.device for t in (k, v, table)):
-        raise RuntimeError("all tensors must be on the same device")
     s = float(D ** -0.5 if scale is None else scale) if D else 1.0
     if not math.isfinite(s):
         raise ValueError("scale must be finite")

@@ -192,3 +192,18 @@ def test_edges_as_a_tensor_or_a_generator():
     for edges in (torch.tensor(EDGES), tuple(EDGES), (e for e in EDGES)):
         trunk = AlternatingTrunk(32, 4, 1, schedule=["bucket"], bucket_edges=edges)
         assert trunk.bucket_edges == EDGES and trunk.blocks[0].attn.bias_table.shape == (6, 4)
+
+
+def test_buckets_of_another_number_or_shape_are_refused():
+    """On the torch path as on the kernels': a larger table's next entry would serve pairs that are left out."""
+    h, coords = torch.randn(2, 7, 32), torch.randn(2, 7, 3)
+    for n in (5, 7, 64):
+        with pytest.raises(ValueError, match="table must have shape"):
+            BucketAttention(32, 4, n)(h, distance_buckets(coords, EDGES, cutoff=1.0))
+    attn = BucketAttention(32, 4, 6)
+    for other in (coords[:, :6], coords[:, :1], coords.repeat(2, 1, 1)):
+        with pytest.raises(ValueError, match="buckets must be of"):
+            attn(h, distance_buckets(other, EDGES))
+    with pytest.raises(TypeError, match="PairBuckets"):
+        attn(h, distance_buckets(coords, EDGES).index)
+    assert attn(h, distance_buckets(coords[:1], EDGES)).shape == h.shape  # one entry's serve a batch
