@@ -164,8 +164,8 @@ def _attention_torch(q, k, v, table, buckets: PairBuckets, scale: float, dropout
     k, v = (t.to(wide).repeat_interleave(group, dim=1) for t in (k, v))
     bias = table_with_masked(table.to(wide))[table_rows(buckets)].permute(0, 3, 1, 2)
     s = torch.matmul(q.to(wide), k.transpose(-1, -2).contiguous()) * scale + bias
-    if s.shape[-1] == 0:
-        return torch.zeros_like(q), torch.zeros(q.shape[:3], dtype=torch.float32, device=q.device)
+    if s.shape[-1] == 0:  # no maximum; zeros with gradients of zeros
+        return torch.matmul(s, v).to(q.dtype), s.sum(-1).to(torch.float32)
     top = s.detach().amax(-1, keepdim=True)
     p = torch.exp(s - torch.where(torch.isinf(top), torch.zeros_like(top), top))
     total = p.sum(-1, keepdim=True)

@@ -368,3 +368,15 @@ def test_the_torch_formulation_is_fp32_under_autocast(dtype):
         assert out.dtype == dtype and lse.dtype == torch.float32
         results.append([out, lse, *torch.autograd.grad((out, lse), leaves, (go, torch.ones_like(lse)))])
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_empty_calls_are_zeros_with_gradients():
+    for B, H, Nq, Nk in ((0, 2, 5, 5), (2, 0, 5, 5), (2, 2, 0, 5), (2, 2, 5, 0)):
+        q, k, v = (torch.randn(B, H, n, 8, requires_grad=True) for n in (Nq, Nk, Nk))
+        table = torch.randn(4, H, requires_grad=True)
+        out, lse = bucket_attention(q, k, v, table, index_buckets(torch.zeros(B, Nq, Nk, dtype=torch.int32), 4),
+                                    return_lse=True)
+        assert out.shape == q.shape and not out.any() and lse.shape == q.shape[:3] and not lse.any()
+        for t, up in ((out, torch.ones_like(out)), (lse, torch.ones_like(lse))):
+            grads = torch.autograd.grad(t, (q, k, v, table), up, retain_graph=True, allow_unused=True)
+            assert all(g is None or g.shape == x.shape and not g.any() for g, x in zip(grads, (q, k, v, table)))
