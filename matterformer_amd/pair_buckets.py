@@ -290,8 +290,8 @@ def index_buckets(index: torch.Tensor, num_buckets: int, *, pad_mask: torch.Tens
     dev = index.device
     kpad = _pad_bytes(pad_mask, B, Nk, "pad_mask", dev)
     qpad = _pad_bytes(query_pad_mask, B, Nq, "query_pad_mask", dev)
-    if index.dtype == torch.int64:
-        index = index.clamp(-1, MAX_BUCKETS)  # before it is cut to 32 bits
+    if index.dtype in (torch.int64, torch.uint64):
+        index = index.to(torch.int64).clamp(-1, MAX_BUCKETS)  # before it is cut to 32 bits (from 2^63 on: negative)
     i = index.to(torch.int32).contiguous()
     if dev.type == "cuda":
         return _launch(_native.MF_BUCKETS_INDEX, B, Nq, Nk, dev, buckets=int(num_buckets), values=i, query_pad=qpad,

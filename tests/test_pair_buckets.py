@@ -380,3 +380,17 @@ def test_empty_calls_are_zeros_with_gradients():
         for t, up in ((out, torch.ones_like(out)), (lse, torch.ones_like(lse))):
             grads = torch.autograd.grad(t, (q, k, v, table), up, retain_graph=True, allow_unused=True)
             assert all(g is None or g.shape == x.shape and not g.any() for g, x in zip(grads, (q, k, v, table)))
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.uint16, torch.int32, torch.uint32, torch.int64,
+                                   torch.uint64])
+def test_indexes_of_every_whole_type(dtype):
+    """Numbers past 32 bits leave the pair out, whatever their low bits."""
+    top = torch.iinfo(dtype).max
+    numbers = [n for n in (0, 3, 4, 63, 64, 127, 255, 256, 2 ** 31, 2 ** 32, 2 ** 32 + 1, 2 ** 63 - 1, 2 ** 63, 2 ** 64 - 1, top)
+               if n <= top]
+    index = torch.tensor(numbers, dtype=dtype).view(1, 1, -1)
+    want = [n if n < 4 else MASKED for n in numbers]
+    assert index_buckets(index, 4).index.flatten().tolist() == want
+    if dtype.is_signed:
+        assert index_buckets(torch.tensor([[[-1, torch.iinfo(dtype).min]]], dtype=dtype), 4).index.eq(MASKED).all()
