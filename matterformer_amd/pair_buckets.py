@@ -411,8 +411,8 @@ def bucket_bias(table: torch.Tensor, buckets: PairBuckets, *, batch: int | None 
     fp32 in a fixed order.  Entries of the bias at pairs that are left out take no gradient."""
     _check_table(table, buckets)
     B = buckets.batch if batch is None else int(batch)
-    if B != buckets.batch and buckets.batch != 1:
-        raise ValueError(f"batch must be {buckets.batch}, got {B}")
+    if B < 0 or (B != buckets.batch and buckets.batch != 1):
+        raise ValueError(f"batch must be {buckets.batch if buckets.batch != 1 else 'not negative'}, got {B}")
     dtype = table.dtype if dtype is None else dtype
     if table.device.type != "cuda":
         bias = table_with_masked(table)[table_rows(buckets)].permute(0, 3, 1, 2).to(dtype)

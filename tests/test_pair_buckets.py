@@ -394,3 +394,11 @@ def test_indexes_of_every_whole_type(dtype):
     assert index_buckets(index, 4).index.flatten().tolist() == want
     if dtype.is_signed:
         assert index_buckets(torch.tensor([[[-1, torch.iinfo(dtype).min]]], dtype=dtype), 4).index.eq(MASKED).all()
+
+
+def test_a_negative_batch_of_the_bias_is_refused():
+    b = index_buckets(torch.zeros(1, 3, 5, dtype=torch.int32), 4)
+    for n in (-1, -3):
+        with pytest.raises(ValueError, match="batch"):
+            bucket_bias(torch.zeros(4, 2), b, batch=n)
+    assert bucket_bias(torch.zeros(4, 2), b, batch=0).shape == (0, 2, 3, 5)
