@@ -316,7 +316,10 @@ def offset_edges(num_buckets: int, max_offset: int, *, causal: bool = False) -> 
         near = (n + 1) // 2
         out = list(range(1, near + 1))
         while len(out) < n:
-            at = near * (max_offset / near) ** ((len(out) + 1 - near) / (n - near))
+            if len(out) + 1 == n:
+                at = max_offset
+            else:
+                at = near * (max_offset / near) ** ((len(out) + 1 - near) / (n - near))
             out.append(max(out[-1] + 1, min(int(at), max_offset - (n - 1 - len(out)))))
         return out
 

@@ -402,3 +402,13 @@ def test_a_negative_batch_of_the_bias_is_refused():
         with pytest.raises(ValueError, match="batch"):
             bucket_bias(torch.zeros(4, 2), b, batch=n)
     assert bucket_bias(torch.zeros(4, 2), b, batch=0).shape == (0, 2, 3, 5)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_offset_edges_end_at_the_greatest_offset(causal):
+    """Offsets from max_offset on share the last bucket, and none before does (of sides with widening buckets)."""
+    for n in (4, 5, 14, 27, 33, 64):
+        for most in (63, 115, 122, 230, 237, 512, 1000, 4096, 99999, 2 ** 31, 2 ** 53):
+            edges = offset_edges(n, most, causal=causal)
+            assert all(a < b for a, b in zip(edges, edges[1:])) and 1 - edges[0] == most, (n, most)
+            assert causal or n < 5 or edges[-1] == most, (n, most)
