@@ -359,6 +359,8 @@ class BucketAttention(nn.Module):
             return "the HIP bucket attention has no forward-mode derivative"
         if self.bias_table.dtype not in (torch.float32, torch.float16, torch.bfloat16):
             return "the HIP bucket attention needs a float32/float16/bfloat16 table"
+        if h.dtype == torch.float64:
+            return "the HIP bucket attention needs float32/float16/bfloat16 projections"
         if torch.is_grad_enabled() and (h.requires_grad or any(p.requires_grad for p in self.parameters())):
             dtype = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else h.dtype
             if dtype not in (torch.bfloat16, torch.float16):

@@ -277,3 +277,38 @@ def test_a_torch_trunk_runs_no_bucket_kernel(cuda, periodic, dtype, monkeypatch)
     q = torch.zeros(4, 2, 90, 32, device=cuda, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="distance_buckets"):
         bucket_attention(q, q, q, torch.zeros(len(EDGES) + 1, 2, device=cuda), seen[0])
+
+
+@pytest.mark.parametrize("autocast", [False, True])
+@pytest.mark.parametrize("table", [torch.float64, torch.float32])
+def test_float64_modules_take_the_torch_path(cuda, table, autocast):
+    """In inference and in training, autocast or not (which leaves 64-bit operands alone): no core in 16 bits."""
+    attn = make_attn(cuda, 128, 2, torch.float64)
+    attn.bias_table.data = attn.bias_table.data.to(table)
+    h = torch.randn(2, 50, 128, device=cuda).double()
+    coords = torch.randn(2, 50, 3, device=cuda)
+    buckets = distance_buckets(coords, EDGES)
+    other = copy.deepcopy(attn).cpu()
+    want = other(h.cpu(), distance_buckets(coords.cpu(), EDGES))
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad), torch.autocast("cuda", dtype=torch.bfloat16, enabled=autocast):
+            out = attn(h, buckets)
+        assert attn._last_impl_used == "torch" and out.dtype == torch.float64
+        # sums of at most 128 fp64 terms, some products deep
+        assert off(out, want) <= 2.0 ** -40
+    out.sum().backward()
+    assert all(p.grad.dtype == p.dtype for p in attn.parameters())
+    attn.impl = "triton"
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="bucket attention needs"):
+            attn(h, buckets)
+
+
+def test_whole_types_of_indexes(cuda):
+    from matterformer_amd.pair_buckets import index_buckets
+
+    for dtype in (torch.uint8, torch.int8, torch.int16, torch.uint16, torch.int32, torch.uint32, torch.int64, torch.uint64):
+        top = torch.iinfo(dtype).max
+        numbers = [n for n in (0, 3, 4, 63, 64, 255, 2 ** 31, 2 ** 32, 2 ** 63, top) if n <= top]
+        index = torch.tensor(numbers, dtype=dtype).view(1, 1, -1)
+        assert index_buckets(index.to(cuda), 4).index.flatten().tolist() == [n if n < 4 else 64 for n in numbers]
