@@ -409,3 +409,117 @@ def test_forward_mode_is_refused(cuda):
         dual = forward_ad.make_dual(q, torch.ones_like(q))
         with pytest.raises(NotImplementedError):
             bucket_attention(dual, k, v, table, buckets)
+
+
+def backward_plan(B, H, KV, Nq, Nk, D, dtype, K):
+    """(pieces, row tiles a piece) of the queries' and of the keys' kernel, as csrc/bucket_attn_bwd.hip takes them; held
+    against the workspace that the library asks for."""
+    from matterformer_amd import _native
+
+    DP = 32 if D <= 32 else 64 if D <= 64 else 128
+    TQ, TK = (-(-n // 64) for n in (Nq, Nk))
+
+    def side(batch_heads, columns, tiles, keys):
+        W = 1 if columns <= 32 else 2 if columns <= 64 else 4
+        CT = -(-columns // (32 * W))
+        units, room = batch_heads * CT, 1024 * (1 if keys and DP == 128 else 2)
+        pieces = max(1, min(tiles, room // max(1, units * W)))
+        per_piece = -(-tiles // pieces)
+        pieces = -(-tiles // per_piece)
+        split = units * pieces * 32 * W * (2 * DP if keys else DP + 1) * 4 if pieces > 1 else 0
+        return CT, pieces, per_piece, split
+
+    queries, keys = side(B * H, Nq, TK, False), side(B * KV, Nk, H // KV * TQ, True)
+    up = lambda n: -(-n // 256) * 256
+    nbytes = up(B * H * TQ * 3 * 64 * 4) + up(H * K * B * keys[0] * keys[1] * 4) + up(max(queries[3], keys[3]))
+    if dtype == FP16:
+        nbytes += up((B * H * TQ + B * KV * TK) * 16)
+    args = _native.MfBucketAttnBwdArgs(dtable=16, fwd=_native.MfBucketAttnArgs(
+        batch=B, heads=H, kv_heads=KV, queries=Nq, keys=Nk, head_dim=D, buckets=K, dtype=_native.dtype_code(dtype)))
+    assert _native.lib().mf_bucket_attn_bwd_workspace_size(args) == nbytes
+    return queries[1:3], keys[1:3]
+
+
+# (shape, type, mask, pieces and row tiles a piece of the queries' and the keys' kernel): workgroups that stream many tiles,
+# through several heads, in one piece and in pieces that begin within a head
+STREAMED = [((32, 8, 8, 512, 512, 64), BF16, "none", (1, 8), (1, 8)), ((32, 8, 8, 512, 512, 64), FP16, "holes", (1, 8), (1, 8)),
+            ((64, 8, 8, 181, 181, 64), BF16, "padding", (1, 3), (1, 3)), ((64, 8, 2, 300, 181, 128), FP16, "padding", (1, 3), (1, 20)),
+            ((4, 8, 2, 1300, 1300, 64), BF16, "holes", (1, 21), (5, 17)), ((4, 8, 2, 1997, 1997, 128), FP16, "none", (1, 32), (2, 64)),
+            ((4, 8, 2, 1997, 1997, 128), BF16, "blocks", (1, 32), (2, 64)), ((40, 16, 4, 700, 60, 32), BF16, "holes", (1, 1), (6, 8)),
+            ((4, 4, 1, 500, 3000, 64), FP16, "holes", (8, 6), (5, 7)),
+            ((40, 32, 8, 20, 700, 32), FP16, "holes", (1, 11), (1, 4)), ((16, 32, 32, 130, 400, 24), BF16, "blocks", (1, 7), (1, 3))]
+
+
+@pytest.mark.parametrize("shape,dtype,mask,queries,keys", STREAMED, ids=lambda x: str(x).replace(" ", "") if isinstance(x, tuple) else None)
+def test_workgroups_that_stream_many_tiles(cuda, shape, dtype, mask, queries, keys):
+    q, k, v, table, index, go = make(cuda, *shape, dtype, K=32, mask=mask, seed=sum(shape))
+    assert backward_plan(*shape, dtype, 32) == (queries, keys)
+    got = run(q, k, v, table, index, go)
+    # batch entries have rows of their own; only the table's gradient joins them
+    total, most = 0.0, 0.0
+    per = max(1, 2 ** 27 // (shape[1] * shape[3] * shape[4]))
+    for b in range(0, shape[0], per):
+        at = slice(b, b + per)
+        r, bound = attention(q[at], k[at], v[at], table, index_buckets(index[at], 32).index, shape[5] ** -0.5, go[at])
+        check({n: got[n][at] for n in ("out", "lse", "dq", "dk", "dv")}, r, bound)
+        total, most = total + r["dtable"], most + bound["dtable"]
+    check({"dtable": got["dtable"]}, {"dtable": total}, {"dtable": most})
+
+
+@pytest.mark.parametrize("shape,dtype", [((2, 6, 3, 1500, 1500, 64), FP16), ((1, 4, 4, 2100, 2100, 128), BF16),
+                                         ((1, 12, 6, 1100, 1600, 32), BF16), ((3, 4, 2, 1700, 1200, 96), FP16)])
+def test_earlier_keys_of_few_heads(cuda, shape, dtype):
+    """Fewer than eight key heads in all and more than eight tiles: the tiles are dealt in eight sequences."""
+    B, H, KV, Nq, Nk, D = shape
+    assert B * KV < 8 and min(Nq, Nk) > 8 * 128
+    q, k, v, table, _, go = make(cuda, *shape, dtype, K=32, seed=sum(shape))
+    places = [torch.arange(n, device=cuda) for n in (Nq, Nk)]
+    buckets = offset_buckets(*places, offset_edges(32, 900, causal=True), causal=True)
+    leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v, table)]
+    out, lse = bucket_attention(*leaves, buckets, return_lse=True)
+    grads = torch.autograd.grad(out, leaves, go)
+    got = dict(zip(("out", "lse", "dq", "dk", "dv", "dtable"), (out.detach(), lse.detach(), *grads)))
+    r, bound = attention(q, k, v, table, buckets.index, D ** -0.5, go)
+    check(got, r, bound)
+
+
+@pytest.mark.parametrize("low", [-1e9, torch.finfo(BF16).min, torch.finfo(FP32).min])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("Nq", [40, 200])
+def test_gradients_of_rows_at_finite_mask_values(cuda, low, dtype, Nq):
+    """Rows all of whose biases are huge and negative: x is the bias alone (its fp32 step, 128 in log2 units at least, swallows
+    the products), so that P is 1 over the number of pairs, exactly alike."""
+    B, H, Nk, D, scale = 2, 2, 100, 64, 0.125
+    q, k, v, table, index, go = make(cuda, B, H, H, Nq, Nk, D, dtype, K=4)
+    table[1] = low
+    rows = {5: Nk, 6: 70, Nq - 1: Nk}
+    for i in rows:
+        index[0, i] = 1
+    index[0, 6, 70:] = -1
+    got = run(q, k, v, table, index, go)
+    # in 64 bits their products would count: with queries of zeros there they do not, and dk's part of them is added
+    flat = q.clone()
+    flat[0, :, list(rows)] = 0
+    codes = index_buckets(index, 4).index
+    r, bound = attention(flat, k, v, table.clamp_min(-1e9), codes, scale, go)
+    u, f = torch.finfo(dtype).eps / 2, 2.0 ** -15
+    grain = 2.0 ** -25 if dtype == FP16 else 0.0
+    g64, q64, v64 = go.double(), q.double(), v.double()
+    peak = 2.0 * g64.norm(dim=-1).max() * v64.norm(dim=-1).max()
+    for i, n in rows.items():
+        vi, g = v64[0, :, :n], g64[0, :, i]  # (H, n, D), (H, D)
+        dP = (vi @ g[..., None])[..., 0]
+        out = vi.mean(1)
+        dS = (dP - (out * g).sum(-1, keepdim=True)) / n
+        spread = vi.abs().mean(1)
+        wide = (g.abs() * (out.abs() + spread * (u + f))).sum(-1, keepdim=True)
+        off = ((vi.abs() @ g.abs()[..., None])[..., 0] + wide) * f / n
+        dS_off = dS.abs() * u + off + grain * peak * 2.0 ** -12
+        r["dk"][0, :, :n] += scale * dS[..., None] * q64[0, :, i, None]
+        bound["dk"][0, :, :n] += scale * dS_off[..., None] * q64[0, :, i, None].abs() + u * scale * (dS[..., None] * q64[0, :, i, None]).abs()
+    r.pop("lse")  # (beside the bias its 64-bit value has more bits than fp32)
+    check({n: got[n] for n in r}, r, bound)
+    # and their outputs are the plain means
+    for i, n in rows.items():
+        mean = v64[0, :, :n].mean(1)
+        assert ((got["out"][0, :, i].double() - mean).abs() <= bound["out"][0, :, i]).all()

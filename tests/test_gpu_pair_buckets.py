@@ -355,3 +355,14 @@ def test_a_bias_about_one_edge(cuda):
     table = torch.tensor([[1.0], [2.0]], device=cuda)
     bias = bucket_bias(table, offset_buckets(places, places, [1]))[0, 0]
     assert torch.equal(bias, 1.0 + (places[None] > places[:, None]).float())
+
+
+def test_more_tiles_than_one_launch(cuda):
+    """(2^23 workgroups a launch; a tile an entry here)"""
+    B = 2 ** 23 + 77
+    g = torch.Generator(device=cuda).manual_seed(4)
+    index = torch.randint(-1, 9, (B, 1, 1), generator=g, device=cuda, dtype=torch.int32)
+    got = index_buckets(index, 9)
+    want = torch.where(index < 0, MASKED, index)
+    assert torch.equal(got.index.int(), want) and torch.equal(got.index_t.int(), want)
+    assert torch.equal(got.key_any, (index >= 0).long()) and torch.equal(got.query_any, (index >= 0).long())
