@@ -74,11 +74,11 @@ __host__ __device__ __forceinline__ int ordered_bits(float x) {
 #endif
   return b ^ ((b >> 31) & 0x7fffffff);
 }
-// Clamped before base is taken off: with shift 0 (edges within 1024 steps of fp32) the distance of a value of the other sign
-// passes 32 bits.  base + kCells - 1 does not: base is at most the bits of the greatest finite number.
+// With shift 0 (edges within 1024 steps of fp32) the distance of a value of the other sign passes 32 bits: it saturates, in one
+// instruction.  (Clamping to the cells' bits first, with two scalar operands: two orders of 8192 places 1.5 us longer.)
 __host__ __device__ __forceinline__ int cell_of(float x, int base, int shift) {
-  const int c = ordered_bits(x) >> shift, last = base + (kCells - 1);
-  return (c < base ? base : c > last ? last : c) - base;
+  const int c = __builtin_elementwise_sub_sat(ordered_bits(x) >> shift, base);
+  return c < 0 ? 0 : c >= kCells ? kCells - 1 : c;
 }
 
 // The least and the greatest of a wave's values.
