@@ -904,6 +904,10 @@ int mf_bucket_bias_bwd(const mf_bucket_bias_args* args, void* stream);
 /* a pair hold reaches nothing.  Few queries over many keys are split over   */
 /* the keys and joined (workspace, no fill needed).                          */
 /* Softmax and sums in fp32; P rounded to dtype for its product with v.      */
+/* stats: P_ij = 2^(log2(e) S_ij - a_i) c_i with log2(e) S_ij - a_i < 1 for   */
+/* every pair, both 0 for a query without one.  Which such pair it is, is    */
+/* the forward's choice (a need not be the maximum, nor c 1 over the sum);   */
+/* the gradients rely on the bound and take no pair from elsewhere.          */
 typedef struct mf_bucket_attn_args {
   const void* q;
   const void* k;
@@ -915,7 +919,7 @@ typedef struct mf_bucket_attn_args {
   void* out;                   /* out_stride                                 */
   void* out_lo;                /* what out's rounding left, contiguous [B, H, queries, head_dim], or NULL */
   float* lse;                  /* [B, H, queries] or NULL                    */
-  float* stats;                /* [2, B, H, queries]: of each query the maximum of log2(e) S and 1 / sum, or NULL */
+  float* stats;                /* [2, B, H, queries] or NULL: of each query a pair (a, c) for the gradients, below */
   void* workspace;
   uint64_t workspace_bytes;
   int64_t q_stride[3];

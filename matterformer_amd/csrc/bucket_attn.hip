@@ -113,7 +113,8 @@ __device__ __forceinline__ void store_stats(const FwdParams& p, const Column& c,
   l *= __is_same(T, _Float16) ? 1.0f / 128.0f : 1.0f;  // 2^-shift_bits
   const int64_t at = (c.b * p.H + c.h) * p.Nq + c.i;
   if (p.stats) {
-    // m is raised by the whole part of log2 l, so that 2^(x - m) <= 2 for every x of the row
+    // m, which may lag behind the maximum, is raised by the whole part of log2 l, so that 2^(x - m) < 2 for every x of the
+    // row; l is what the sum from there is
     float to = m, inv = l;  // (a NaN stays one)
     if (l > 0.0f) {
       if (fabsf(m) < kExact) to = m + float(ilogbf(l));

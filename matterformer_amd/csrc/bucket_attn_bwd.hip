@@ -1,5 +1,6 @@
 // Gradients of attention with a bias by buckets (mf_bucket_attn_bwd) on gfx950.
-// With the forward's row maximum m_i and 1 / sum of it,
+// With m_i, a number near the row's maximum of x = log2(e) S (x - m_i < 1), and
+// 1 / l_i, 1 over the row's sum of 2^(x - m_i), as the forward leaves them,
 //   e_ij = 2^(log2(e) (scale q_i . k_j + bias_ij) - m_i),  P_ij = e_ij / l_i,
 //   dv_j = sum_i P_ij go_i,           dP_ij = go_i . v_j,
 //   dS_ij = P_ij (dP_ij - delta_i),   delta_i = go_i . out_i - dlse_i,
@@ -17,7 +18,8 @@
 //            dq^T += K^T dS.  A column is one query, so dS is kept without 1 / l,
 //            which the sum gets at the end.  The sum of a query's dS, which is
 //            dlse_i but for delta's error (out is a product of rounded P), corrects
-//            delta for the next kernel.
+//            delta for the next kernel.  dq itself keeps that error, at most a
+//            rounding of P in size: scale (delta's error) sum_j P_ij k_j.
 //   keys:    columns are keys (K, V in registers), rows the queries of every head
 //            of the key head (X = Q, Y = go): dk^T += Q^T dS, dv^T += go^T P, and
 //            the table's gradient, in which delta's error would not cancel (with it

@@ -523,3 +523,35 @@ def test_gradients_of_rows_at_finite_mask_values(cuda, low, dtype, Nq):
     for i, n in rows.items():
         mean = v64[0, :, :n].mean(1)
         assert ((got["out"][0, :, i].double() - mean).abs() <= bound["out"][0, :, i]).all()
+
+
+@pytest.mark.parametrize("shape", [(2, 4, 2, 70, 700, 64), (1, 8, 2, 1, 3000, 64), (16, 8, 8, 300, 300, 32)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_statistics_for_the_gradients(cuda, dtype, shape):
+    """The pairs (a, c) that the forward leaves, also where a row's maximum rises slowly from tile to tile or is huge:
+    P = 2^(log2(e) S - a) c and log2(e) S - a < 1, zeros for a row without a pair."""
+    from matterformer_amd.bucket_attention import _forward
+
+    B, H, KV, Nq, Nk, D = shape
+    q, k, v, table, index, _ = make(cuda, *shape, dtype, K=17, mask="holes")
+    index[-1, 0] = 16
+    table[16] = -1e9
+    k *= torch.linspace(0.1, 3.0, Nk, device=cuda).to(dtype)[:, None]
+    buckets = index_buckets(index, 17)
+    stats = _forward(q, k, v, table, buckets, D ** -0.5, lse=True, training=True)[3]
+    a, c = stats.double()[..., None].unbind(0)
+    allowed = (buckets.index != MASKED)[:, None]
+    wide = torch.cat([table.double(), table.new_zeros(1, H).double()])[torch.where(buckets.index == MASKED, 17, buckets.index).long()]
+    s = q.double() @ k.double().repeat_interleave(H // KV, 1).transpose(-1, -2).contiguous() * D ** -0.5 + wide.permute(0, 3, 1, 2)
+    x = torch.where(allowed, s * math.log2(math.e), -math.inf)
+    # fp32 roundings of x: of a few hundred at most by 2^-24 a term; of the huge row all of the products
+    slack = torch.where(x.amax(-1, keepdim=True) < -1e6, 300.0, 2.0 ** -12)
+    assert ((x - a < 1.0 + slack) | ~allowed).all()
+    P = torch.softmax(torch.where(allowed, s, -math.inf), -1)
+    some = allowed.any(-1, keepdim=True) & (x.amax(-1, keepdim=True) > -1e6)
+    off = (torch.exp2(x - a) * c - P).abs()
+    assert ((off <= 2.0 ** -12 * P) | ~(allowed & some)).all()
+    none = ~allowed.any(-1, keepdim=True).expand_as(a)
+    assert not a[none].any() and not c[none].any()
+    huge = (a < -1e6)
+    assert huge.any() and (c[huge] - 1.0 / allowed.expand(B, H, Nq, Nk).sum(-1, keepdim=True)[huge]).abs().max() <= 2.0 ** -20
