@@ -690,9 +690,10 @@ class AlternatingTrunk(nn.Module):
     def _pair_buckets(self, coords: torch.Tensor, pad_mask: torch.Tensor | None,
                       terms: SimplicialTerms | None) -> PairBuckets | None:
         """The bucket blocks' buckets, built once per forward."""
-        if "bucket" not in self.schedule:
+        taking = [block for block in self.blocks if getattr(block, "attn_type", None) == "bucket"]
+        if not taking:  # (a user may have replaced them)
             return None
-        use_hip = any(block.attn.impl != "torch" for block in self.blocks if getattr(block, "attn_type", None) == "bucket")
+        use_hip = any(getattr(getattr(block, "attn", None), "impl", "auto") != "torch" for block in taking)
         if not self._adapter_distances():
             return distance_buckets(coords, self.bucket_edges, pad_mask=pad_mask, cutoff=self.bucket_cutoff,
                                     use_hip=use_hip)
@@ -787,7 +788,7 @@ class AlternatingTrunk(nn.Module):
             mask = build_knn_mask(packing.compact(coords.float()), self.knn_k, cpad, use_hip=True,
                                   with_tables=self._trains_local(x))
         buckets = (self._pair_buckets(packing.compact(coords.float()), cpad, terms) if "bucket" in self.schedule
-                   else None)
+                   else None)  # (without, the coordinates need not be laid out)
         if terms is None:
             terms = SimplicialTerms(coerce_attention_mask(None, key_padding_mask=cpad, batch_size=B, num_tokens=W,
                                                           device=x.device))

@@ -207,3 +207,21 @@ def test_buckets_of_another_number_or_shape_are_refused():
     with pytest.raises(TypeError, match="PairBuckets"):
         attn(h, distance_buckets(coords, EDGES).index)
     assert attn(h, distance_buckets(coords[:1], EDGES)).shape == h.shape  # one entry's serve a batch
+
+
+def test_a_users_block_in_the_place_of_the_bucket_block():
+    """One that takes buckets says so by its attn_type; where none does, none are made."""
+    class Takes(torch.nn.Module):
+        attn_type = "bucket"
+
+        def forward(self, x, cond_emb, pad_mask=None, *, knn_mask=None, pair_buckets):
+            return x + pair_buckets.index.sum(-1, dtype=x.dtype)[..., None]
+
+    trunk = AlternatingTrunk(32, 4, 1, schedule=["bucket"], bucket_edges=EDGES)
+    x, cond, coords = torch.randn(2, 6, 32), torch.randn(2, 32), torch.randn(2, 6, 3)
+    trunk.blocks[0] = Takes()
+    index = distance_buckets(coords, EDGES).index
+    assert torch.equal(trunk(x, cond, coords), x + index.sum(-1, dtype=x.dtype)[..., None])
+    trunk.blocks[0] = UsersBlock(AdaLNBlock(32, 4, attn_type="simplicial", simplicial_precision="ieee_fp32"))
+    assert trunk._pair_buckets(coords, None, None) is None
+    assert trunk(x, cond, coords).shape == x.shape
